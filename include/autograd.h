@@ -72,6 +72,33 @@ AGNode *ag_retain(AGNode *n);
 AGNode *ag_softmax_ce(AGNode *logits, const int *labels, long rows);
 Tensor *ag_softmax_ce_probs(const AGNode *loss);
 
+/* ---- transformer nodes; the structs and the formulas are in tt_hip.h ---- */
+struct TTRope;
+struct TTAttention;
+
+/* Layer norm over the last axis; w and b (as many elements as that axis) may
+ * be NULL. */
+AGNode *ag_layernorm(AGNode *x, AGNode *w, AGNode *b, float eps);
+
+/* Rotary positions of the rows of x: its last axis holds heads * head_dim
+ * values, or its last two are heads x head_dim; the axes before count rows.
+ * positions: a host array of an int a row (not negative), or NULL: row %
+ * seq_len. */
+AGNode *ag_rope(AGNode *x, const struct TTRope *r, int heads, const int *positions, long seq_len);
+
+/* Attention; q holds batch x q_rows x q_heads x head_dim values in that order,
+ * k and v batch x k_rows x kv_heads x head_dim, whatever their axes (matmul
+ * outputs of batch * rows rows fit as they are).  The value has q's shape.
+ * Of a, the strides are 0 here, and q_start, q_len and k_len host arrays
+ * (copied) or NULL. */
+AGNode *ag_attention(AGNode *q, AGNode *k, AGNode *v, const struct TTAttention *a);
+
+/* Distillation: the mean over the rows of 2-D logits of the loss against a
+ * teacher's top logits (tt_k_distill); ids and teacher are host arrays of rows x
+ * top values. */
+AGNode *ag_distill(AGNode *logits, const int *ids, const float *teacher, int top,
+                   float temperature);
+
 /* Backward seeded from a device-resident tensor of the value's shape
  * (no host round trip); same mismatch rule as ag_backward_from. */
 void    ag_backward_from_tensor(AGNode *out, const Tensor *seed);

@@ -448,6 +448,103 @@ int tt_k_conv2d_dx_lds(const float *g, const float *w, float *dx,
                        int N, int C, int H, int W, int F, int HH, int WW,
                        int sh, int sw, int ph, int pw, int Ho, int Wo);
 
+/* ---- transformer operators (norm.hip, rotary.hip, attention.hip,
+ * distill.hip); no counterpart in the reference ----
+ * `ws` arguments are device memory of the size the matching *_ws function
+ * gives, used until the call's work is done, or NULL: taken from the caching
+ * allocator for the call.  With a workspace of its own a call allocates
+ * nothing, so it can be captured into a graph; two graphs that can run at
+ * once need a workspace each.  Outputs do not overlap inputs unless said
+ * so.  -1: bad arguments, -2: no memory, -3: the launch failed. */
+
+/* Layer norm over the last axis of a rows x cols matrix:
+ *   y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps)
+ * (var: the mean square of x - mean).  w and b may be NULL (1 and 0); mean
+ * and rstd (rows floats each) are written unless NULL. */
+int tt_k_layernorm_fwd(const float *x, const float *w, const float *b, float *y, float *mean,
+                       float *rstd, long rows, long cols, float eps);
+/* Its gradients from dy and the forward's mean and rstd: dx, dw = the sum over
+ * rows of dy * (x - mean) * rstd, db = the sum of dy; each may be NULL.  The
+ * sums over rows have a fixed order. */
+size_t tt_k_layernorm_bwd_ws(long rows, long cols);
+int tt_k_layernorm_bwd(const float *x, const float *w, const float *dy, const float *mean,
+                       const float *rstd, float *dx, float *dw, float *db, long rows, long cols,
+                       void *ws);
+
+/* Rotary positions: in each head the pair j of the first rot_dim values turns
+ * by the angle position * f_j, f_j = base^(-2j / rot_dim); the rest of the head
+ * is copied.  Pairs are (2j, 2j + 1) when interleaved, else (j, j + rot_dim/2).
+ * For positions past a trained length the frequencies are scaled:
+ *   TT_ROPE_LINEAR  f_j / factor
+ *   TT_ROPE_NTK     base * factor^(rot_dim / (rot_dim - 2)) in place of base
+ *   TT_ROPE_PARTS   with n_j = trained * f_j / (2 pi) turns over the trained
+ *                   length and r = clamp((n_j - low) / (high - low), 0, 1):
+ *                   (1 - r) f_j / factor + r f_j
+ * and every turned pair is multiplied by magnitude (0: 1). */
+#define TT_ROPE_PLAIN  0
+#define TT_ROPE_LINEAR 1
+#define TT_ROPE_NTK    2
+#define TT_ROPE_PARTS  3
+#define TT_ROPE_MAX_DIM 512  /* rot_dim is even and at most this */
+typedef struct TTRope {
+    int head_dim, rot_dim, interleaved, scaling;
+    double base, factor, trained, low, high, magnitude;
+} TTRope;
+/* the rot_dim / 2 frequencies f_j in host memory */
+int tt_rope_frequencies(const TTRope *r, double *f);
+/* rows x heads x head_dim, rows ldx / ldy floats apart (0: heads * head_dim);
+ * positions (device, rows ints, not negative) or NULL: row % seq_len.  transpose
+ * turns back (and multiplies by magnitude too): the gradient.  y may be x,
+ * with the same row distance. */
+int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *positions, long rows,
+              long seq_len, int heads, long ldx, long ldy, int transpose);
+
+/* Attention: o_i = sum_j softmax_j(scale * q_i . k_j) v_j for q, o of batch x
+ * q_rows x q_heads x head_dim and k, v of batch x k_rows x kv_heads x head_dim;
+ * q_heads / kv_heads query heads in a row share a key head.  Sequence b has
+ * k_len[b] keys and q_len[b] queries (device ints, NULL: all), its query i
+ * the position q_start[b] + i (NULL: k_rows - q_rows + i).  A query at position p
+ * sees key j when j < k_len, with causal j <= p, and with window > 0 also
+ * p - j < window (without causal |p - j| < window).  A query that sees no key,
+ * and one past q_len, has o = 0 and lse = -inf and takes no part in the
+ * gradients; what lies behind k_len and q_len is not read.  Lengths outside
+ * [0, rows] are clamped. */
+#define TT_ATTENTION_MAX_DIM 128
+typedef struct TTStrides {
+    long batch, row, head;  /* floats from one to the next; 0: packed in that order */
+} TTStrides;
+typedef struct TTAttention {
+    long batch, q_rows, k_rows;
+    int q_heads, kv_heads, head_dim, causal;
+    long window;            /* 0: none */
+    float scale;            /* 0: 1 / sqrt(head_dim) */
+    TTStrides q, k, v, o;   /* dq, dk, dv and dout lie as q, k, v and o */
+    const int32_t *q_start, *q_len, *k_len;
+} TTAttention;
+size_t tt_k_attention_fwd_ws(const TTAttention *a);
+/* lse (batch x q_heads x q_rows, for the backward pass) may be NULL */
+int tt_k_attention_fwd(const TTAttention *a, const float *q, const float *k, const float *v,
+                       float *o, float *lse, void *ws);
+/* dq, and dk with dv, or either alone (the others NULL), from the forward's o
+ * and lse; the probabilities are recomputed */
+size_t tt_k_attention_bwd_ws(const TTAttention *a);
+int tt_k_attention_bwd(const TTAttention *a, const float *q, const float *k, const float *v,
+                       const float *o, const float *dout, const float *lse, float *dq, float *dk,
+                       float *dv, void *ws);
+
+/* Distillation from a teacher's `top` logits a row (ids and teacher: rows x top,
+ * on the device): with p = softmax(teacher / T) over the row's entries and
+ * q = softmax(logits / T) over all columns,
+ *   rowloss = T^2 sum_e p_e (log p_e - log q[ids_e])
+ *   dlogits = scale * T * (q - the p_e at their columns)      (unless NULL)
+ * Entries whose id is outside [0, cols) are left out, entries of one column
+ * add up.  A row without entries, or with -inf for all of them, has loss and
+ * gradient 0.  A row of logits of -inf counts as a row of equal ones. */
+#define TT_DISTILL_MAX_TOP 1024
+int tt_k_distill(const float *logits, const int32_t *ids, const float *teacher, int top,
+                 float temperature, float *rowloss, float *dlogits, long rows, int cols,
+                 float scale);
+
 /* Dataset batch gather + normalisation (see tt_data.h):
  * out[r, j] = ((float)src[idx[r]*sample + j] / 255 - mean[c]) / stdv[c],
  * c = j / plane, channels = sample / plane <= 4.  idx values must be in

@@ -24,6 +24,30 @@ _I = ctypes.c_int
 _L = ctypes.c_long
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_D = ctypes.c_double
+
+
+class Rope(ctypes.Structure):
+    """TTRope of tt_hip.h: how the heads of a row turn with its position."""
+    _fields_ = [("head_dim", _I), ("rot_dim", _I), ("interleaved", _I), ("scaling", _I), ("base", _D),
+                ("factor", _D), ("trained", _D), ("low", _D), ("high", _D), ("magnitude", _D)]
+
+
+class Strides(ctypes.Structure):
+    """TTStrides of tt_hip.h; zeros: packed."""
+    _fields_ = [("batch", _L), ("row", _L), ("head", _L)]
+
+
+class Attention(ctypes.Structure):
+    """TTAttention of tt_hip.h: sizes, masks and layout of an attention."""
+    _fields_ = [("batch", _L), ("q_rows", _L), ("k_rows", _L), ("q_heads", _I), ("kv_heads", _I),
+                ("head_dim", _I), ("causal", _I), ("window", _L), ("scale", _F), ("q", Strides),
+                ("k", Strides), ("v", Strides), ("o", Strides), ("q_start", VP), ("q_len", VP),
+                ("k_len", VP)]
+
+
+_RP = ctypes.POINTER(Rope)
+_AP = ctypes.POINTER(Attention)
 SIGNATURES = [
     # tensor.h
     ("tt_new", VP, [I64P, _I]),
@@ -72,6 +96,10 @@ SIGNATURES = [
     ("ag_retain", VP, [VP]),
     ("ag_softmax_ce", VP, [VP, ctypes.POINTER(ctypes.c_int), _L]),
     ("ag_softmax_ce_probs", VP, [VP]),
+    ("ag_layernorm", VP, [VP, VP, VP, _F]),
+    ("ag_rope", VP, [VP, _RP, _I, VP, _L]),
+    ("ag_attention", VP, [VP, VP, VP, _AP]),
+    ("ag_distill", VP, [VP, VP, VP, _I, _F]),
     ("ag_backward_from_tensor", None, [VP, VP]),
     ("ag_sgd_step", _I, [VP, _F]),
     ("ag_sgd_step_many", _I, [ctypes.POINTER(VP), _I, _F]),
@@ -182,6 +210,16 @@ SIGNATURES = [
     ("tt_k_conv2d_chain_bwd", _I, [VP] * 10 + [_I] * 2),
     ("tt_k_conv2d_dw_lds_pooled", _I, [VP] * 5 + [_I] * 13),
     ("tt_k_conv2d_dx_lds", _I, [VP, VP, VP] + [_I] * 13),
+    ("tt_k_layernorm_fwd", _I, [VP] * 6 + [_L, _L, _F]),
+    ("tt_k_layernorm_bwd_ws", _SZ, [_L, _L]),
+    ("tt_k_layernorm_bwd", _I, [VP] * 8 + [_L, _L, VP]),
+    ("tt_rope_frequencies", _I, [_RP, ctypes.POINTER(_D)]),
+    ("tt_k_rope", _I, [_RP, VP, VP, VP, _L, _L, _I, _L, _L, _I]),
+    ("tt_k_attention_fwd_ws", _SZ, [_AP]),
+    ("tt_k_attention_fwd", _I, [_AP] + [VP] * 6),
+    ("tt_k_attention_bwd_ws", _SZ, [_AP]),
+    ("tt_k_attention_bwd", _I, [_AP] + [VP] * 10),
+    ("tt_k_distill", _I, [VP, VP, VP, _I, _F, VP, VP, _L, _I, _F]),
     ("tt_k_gather_u8_norm", _I, [VP, _L, _L, _L, _I, VP, _L, F32P, F32P, VP]),
     ("tt_k_momentum_multi", _I, [ctypes.POINTER(VP)] * 3 + [ctypes.POINTER(_L), _I, _F, _F]),
     ("tt_k_adam_multi", _I, [ctypes.POINTER(VP)] * 4 + [ctypes.POINTER(_L), _I] + [_F] * 5

@@ -1,0 +1,1126 @@
+// Attention on the fp32 matrix units: forward, the form for few query rows,
+// and the backward pass, which recomputes the probabilities.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  s_ij = scale q_i . k_j
+//   over the keys lo_i <= j < hi_i that the masks leave query i, with
+//   lse_i = log sum_j exp(s_ij); no key: o_i = 0, lse_i = -inf.
+//   delta_i = do_i . o_i,  dv_j = sum_i p_ij do_i,  dp_ij = do_i . v_j,
+//   ds_ij = p_ij (dp_ij - delta_i),  dq_i = scale sum_j ds_ij k_j,
+//   dk_j = scale sum_i ds_ij q_i  (both sums over the heads that share a key).
+//
+// Every product runs on v_mfma_f32_16x16x4_f32: A holds rows lane % 16 and B
+// columns lane % 16 of the product, both at summed index lane / 16; C holds
+// column lane % 16, rows 4 (lane / 16) + r in register r.  Two consequences
+// carry all kernels here:
+//   * a summed index may be dealt to lanes in any order that A and B share, so
+//     one 16-byte read of four consecutive values feeds four products;
+//   * a product's C registers are the B operand of the next one as they
+//     stand (register r: summed index 4 (lane / 16) + r), so probabilities go
+//     from the scores to the second product without leaving their registers.
+// Scores and probabilities are therefore formed transposed, a query (or in the
+// key gradients a key) a column: its running maximum and sum are one value a
+// lane, and rescaling is one multiplication by it.
+//
+// The query rows of the heads that share a key head are packed into one row
+// axis r = i * group + member, so shared keys are loaded once for all of them.
+//
+// All sums, statistics and products are fp32; scores are formed in units of
+// log2 (q or k is multiplied by scale * log2(e) once, a rounding of 2^-24).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include "tt_rt.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
+inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int KT = 32;  // rows of the streamed operand a tile
+
+struct Strides {
+  long b, r, h;  // elements from a sequence / row / head to the next
+};
+
+struct Args {
+  int B, Lq, Lk, Hkv, G, D;
+  int R;              // Lq * G packed rows
+  int causal;
+  long window;
+  float scale;
+  const int32_t *q_start, *q_len, *k_len;
+  Strides q, k, v, o;
+  int vec;            // every row of every operand is 16-byte aligned
+  int chunk;          // keys a workgroup takes of a row tile's (splits > 1)
+  int splits;
+};
+
+struct Range {
+  int lo, hi;
+};
+
+// keys of sequence b, queries of it that hold anything and the position of
+// its first query, whatever the lengths in device memory hold
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+  const int n = a.k_len ? a.k_len[b] : a.Lk;
+  return n < 0 ? 0 : n > a.Lk ? a.Lk : n;
+}
+__device__ __forceinline__ int queries_of(const Args &a, int b) {
+  const int n = a.q_len ? a.q_len[b] : a.Lq;
+  return n < 0 ? 0 : n > a.Lq ? a.Lq : n;
+}
+__device__ __forceinline__ long start_of(const Args &a, int b) {
+  return a.q_start ? (long)a.q_start[b] : (long)a.Lk - a.Lq;
+}
+
+// first key, and the end of the keys, that a query at position `at` sees of n:
+// both grow with `at`
+__device__ __forceinline__ int low_of(const Args &a, long at) {
+  const long lo = a.window > 0 ? at - a.window + 1 : 0;
+  return lo < 0 ? 0 : lo > a.Lk ? a.Lk : (int)lo;
+}
+__device__ __forceinline__ int high_of(const Args &a, long at, int n) {
+  const long hi = a.causal ? at + 1 : a.window > 0 ? at + a.window : n;
+  return hi < 0 ? 0 : hi > n ? n : (int)hi;
+}
+
+// the keys lo <= j < hi of [0, Lk) that query i of sequence b sees
+__device__ __forceinline__ Range range_of(const Args &a, int b, int i) {
+  const long at = start_of(a, b) + i;
+  Range g = {low_of(a, at), high_of(a, at, keys_of(a, b))};
+  if (g.hi <= g.lo || i >= queries_of(a, b)) g.lo = g.hi = 0;
+  return g;
+}
+
+// what the packed rows [r0, r1) of sequence b see: no row a key outside
+// [lo, hi), every row all keys of [ilo, ihi)
+struct Span {
+  int lo, hi, ilo, ihi;
+};
+
+__device__ __forceinline__ Span span_of(const Args &a, int b, int r0, int r1) {
+  Span s = {0, 0, 0, 0};
+  const int nq = queries_of(a, b), i0 = r0 / a.G;
+  int i1 = (r1 - 1) / a.G;
+  const bool whole = i1 < nq;
+  if (!whole) i1 = nq - 1;
+  if (i0 > i1) return s;
+  const long at = start_of(a, b);
+  const int n = keys_of(a, b);
+  s.lo = low_of(a, at + i0);
+  s.hi = high_of(a, at + i1, n);
+  if (s.hi <= s.lo) s.lo = s.hi = 0;
+  if (whole) {
+    s.ilo = low_of(a, at + i1);
+    s.ihi = high_of(a, at + i0, n);
+    if (s.ihi <= s.ilo) s.ilo = s.ihi = 0;
+  }
+  return s;
+}
+
+// four values of a row from column c on; 0 behind the row's end
+__device__ __forceinline__ f32x4 load4(const float *p, int c, int D, int vec) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (vec) {
+    if (c < D) v = *(const f32x4 *)(p + c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (c + j < D) v[j] = p[c + j];
+  }
+  return v;
+}
+
+template <int VW>
+struct Vec;
+template <>
+struct Vec<1> {
+  typedef float T;
+  static __device__ __forceinline__ float at(const T &v, int) { return v; }
+};
+template <>
+struct Vec<2> {
+  typedef f32x2 T;
+  static __device__ __forceinline__ float at(const T &v, int c) { return v[c]; }
+};
+template <>
+struct Vec<4> {
+  typedef f32x4 T;
+  static __device__ __forceinline__ float at(const T &v, int c) { return v[c]; }
+};
+
+// Output columns of a product over rows of the streamed tile: the 16-row
+// blocks of the transposed result take columns d = 16 VW t + VW m + c, so
+// that one read of VW values a lane feeds VW blocks.
+template <int DB>
+struct Cols {
+  static constexpr int VW = DB % 4 == 0 ? 4 : DB % 2 == 0 ? 2 : 1;
+  static constexpr int T = DB / VW;
+};
+
+__device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// acc (columns d of row l % 16) += sum over the tile's rows k of w[k][l % 16] x[k][d]
+template <int DB, int NB>
+__device__ __forceinline__ void product(f32x4 (&acc)[DB], const f32x4 (&w)[NB], const float *x, int ld,
+                                        int lane) {
+  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
+  typedef typename Vec<VW>::T V;
+  const int g = lane >> 4, m = lane & 15;
+#pragma unroll
+  for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const float *row = x + (kb * 16 + 4 * g + r) * ld + VW * m;
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        const V v = *(const V *)(row + 16 * VW * t);
+#pragma unroll
+        for (int c = 0; c < VW; c++) acc[t * VW + c] = mfma(Vec<VW>::at(v, c), w[kb][r], acc[t * VW + c]);
+      }
+    }
+}
+
+// the same one row at a time, leaving out what `seen(k)` does not admit to
+// this lane's column: for tiles that hold infinities or NaN where a mask hides
+// them from some of the columns (0 * inf would reach those)
+template <int DB, int NB, class SEEN>
+__device__ __forceinline__ void product_masked(f32x4 (&acc)[DB], const f32x4 (&w)[NB], const float *x, int ld,
+                                            int lane, SEEN seen) {
+  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
+  const int g = lane >> 4, m = lane & 15;
+#pragma unroll
+  for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll 1
+      for (int kg = 0; kg < 4; kg++) {
+        const int k = kb * 16 + 4 * kg + r;
+        const float p = __shfl(w[kb][r], m + 16 * kg);
+        if (!seen(k)) continue;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+#pragma unroll
+          for (int c = 0; c < VW; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              acc[t * VW + c][e] = fmaf(p, x[k * ld + 16 * VW * t + VW * (4 * g + e) + c], acc[t * VW + c][e]);
+      }
+}
+
+// row p[0 .. D) = f * the columns d that acc holds of this lane's row
+template <int DB>
+__device__ __forceinline__ void store_row(float *p, const f32x4 (&acc)[DB], float f, int D, int vec, int lane) {
+  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
+  const int g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < T; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int d = 16 * VW * t + VW * (4 * g + e);
+      if (VW == 4 && vec) {
+        if (d < D) {
+          const f32x4 v = {acc[t * VW][e] * f, acc[t * VW + (VW > 1)][e] * f, acc[t * VW + (VW > 2 ? 2 : 0)][e] * f,
+                           acc[t * VW + (VW > 2 ? 3 : 0)][e] * f};
+          *(f32x4 *)(p + d) = v;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < VW; c++)
+          if (d + c < D) p[d + c] = acc[t * VW + c][e] * f;
+      }
+    }
+}
+
+// the rows [k0, k0 + KT) of an operand on their way to LDS: NV float4 a thread
+// of NT; rows outside [0, end) are zeros
+template <int DB, int NT>
+struct Stage {
+  static constexpr int C4 = DB * 4;                         // float4 a row
+  static constexpr int NV = (KT * C4 + NT - 1) / NT;
+  static constexpr int LD = DB * 16 + 4;  // rows 4 banks apart: 16-byte reads of 8 rows meet all 32 banks
+  f32x4 v[NV];
+  __device__ __forceinline__ void load(const float *base, long stride, int k0, int end, int D, int vec,
+                                       int tid) {
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int e = tid + n * NT, row = e / C4, c = (e % C4) * 4;
+      v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (e < KT * C4 && k0 + row < end) v[n] = load4(base + (long)(k0 + row) * stride, c, D, vec);
+    }
+  }
+  // packed query rows: r = i * G + member
+  __device__ __forceinline__ void load_rows(const float *base, long rs, long hs, int G, int r0, int end, int D,
+                                            int vec, int tid) {
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int e = tid + n * NT, row = r0 + e / C4, c = (e % C4) * 4;
+      v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (e < KT * C4 && row < end) {
+        const int i = row / G;
+        v[n] = load4(base + (long)i * rs + (long)(row - i * G) * hs, c, D, vec);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float *lds, int tid) const {
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int e = tid + n * NT, row = e / C4, c = (e % C4) * 4;
+      if (e < KT * C4) *(f32x4 *)(lds + row * LD + c) = v[n];
+    }
+  }
+  __device__ __forceinline__ bool odd() const {  // holds an infinity or a NaN
+    float t = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) t = fmaf(v[n][j], 0.f, t);
+    return t != t;
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// over the four lanes that hold a column
+__device__ __forceinline__ float col_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float col_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// ---------------------------------------------------------------- forward
+
+// One workgroup: 64 QB packed rows (16 QB a wave) of one key head against the
+// keys they see, KT at a time through LDS.  With splits > 1 it takes `chunk`
+// keys of them and leaves maximum, sum and the unscaled result to the join.
+template <int DB, int QB>
+__global__ void __launch_bounds__(256, 2)
+    attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
+                    const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
+                    float *__restrict__ ws_ml, float *__restrict__ ws_o) {
+  typedef Stage<DB, 256> S;
+  __shared__ __attribute__((aligned(16))) float lk[KT * S::LD], lv[KT * S::LD];
+  constexpr int ROWS = 64 * QB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  // the last rows see the most keys under a causal mask: they start first
+  const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
+  const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
+  Span sp = span_of(a, b, r0, r1);
+  int k_first = sp.lo / KT * KT, k_end = sp.hi;
+  if (a.splits > 1) {
+    const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
+    if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
+    if (c1 < k_end) k_end = (int)c1;
+  }
+
+  f32x4 qf[QB][DB], acc[QB][DB];
+  float mx[QB], sum[QB];
+  int lo[QB], hi[QB], row[QB];
+  const float *qb_base = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
+#pragma unroll
+  for (int n = 0; n < QB; n++) {
+    row[n] = r0 + (wave * QB + n) * 16 + m;
+    const int i = row[n] / a.G;
+    const bool in = row[n] < a.R;
+    Range rg = {0, 0};
+    if (in) rg = range_of(a, b, i);
+    lo[n] = rg.lo;
+    hi[n] = rg.hi;
+    mx[n] = -INFINITY;
+    sum[n] = 0.f;
+    const float *p = qb_base + (long)i * a.q.r + (long)(row[n] - i * a.G) * a.q.h;
+    const float f = a.scale * LOG2E;
+#pragma unroll
+    for (int u = 0; u < DB; u++) {
+      qf[n][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      acc[n][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (in) qf[n][u] = load4(p, 16 * u + 4 * g, a.D, a.vec) * f;
+    }
+  }
+
+  const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
+  S sk, sv;
+  if (k_first < k_end) {
+    sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
+    sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+  }
+  for (int k0 = k_first; k0 < k_end; k0 += KT) {
+    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi;
+    sk.store(lk, tid);
+    sv.store(lv, tid);
+    bool odd = false;
+    if (mixed)
+      odd = __syncthreads_or(sv.odd());
+    else
+      __syncthreads();
+    if (k0 + KT < k_end) {
+      sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
+      sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
+    }
+    f32x4 s[QB][2];
+#pragma unroll
+    for (int n = 0; n < QB; n++)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) s[n][kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < DB; u++)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) {
+        const f32x4 ka = *(const f32x4 *)(lk + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int n = 0; n < QB; n++) s[n][kb] = mfma(ka[c], qf[n][u][c], s[n][kb]);
+      }
+#pragma unroll
+    for (int n = 0; n < QB; n++) {
+      if (mixed) {
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int key = k0 + kb * 16 + 4 * g + r;
+            if (key < lo[n] || key >= hi[n]) s[n][kb][r] = -INFINITY;
+          }
+      }
+      float t = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) t = fmaxf(t, s[n][kb][r]);
+      t = fmaxf(col_max(t), mx[n]);
+      const float base = t == -INFINITY ? 0.f : t;
+      if (__any(t > mx[n])) {
+        const float f = exp2_fast(mx[n] - base);
+        sum[n] *= f;
+#pragma unroll
+        for (int u = 0; u < DB; u++) acc[n][u] *= f;
+      }
+      mx[n] = t;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          s[n][kb][r] = exp2_fast(s[n][kb][r] - base);
+          sum[n] += s[n][kb][r];
+        }
+    }
+    if (odd) {
+#pragma unroll
+      for (int n = 0; n < QB; n++)
+        product_masked<DB, 2>(acc[n], s[n], lv, S::LD, lane,
+                              [&](int kk) { return k0 + kk >= lo[n] && k0 + kk < hi[n]; });
+    } else {
+      constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
+      typedef typename Vec<VW>::T V;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float *x = lv + (kb * 16 + 4 * g + r) * S::LD + VW * m;
+#pragma unroll
+          for (int t = 0; t < T; t++) {
+            const V va = *(const V *)(x + 16 * VW * t);
+#pragma unroll
+            for (int c = 0; c < VW; c++)
+#pragma unroll
+              for (int n = 0; n < QB; n++)
+                acc[n][t * VW + c] = mfma(Vec<VW>::at(va, c), s[n][kb][r], acc[n][t * VW + c]);
+          }
+        }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int n = 0; n < QB; n++) {
+    const float total = col_sum(sum[n]);
+    if (row[n] >= a.R) continue;
+    const int i = row[n] / a.G, hq = h * a.G + row[n] - i * a.G;
+    if (a.splits > 1) {
+      const long at = ((long)blockIdx.y * nbh + bh) * a.R + row[n];
+      if (g == 0) {
+        ws_ml[2 * at] = mx[n];
+        ws_ml[2 * at + 1] = total;
+      }
+      store_row<DB>(ws_o + at * (DB * 16), acc[n], 1.f, DB * 16, 1, lane);
+      continue;
+    }
+    if (lse && g == 0)
+      lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (mx[n] + log2f(total)) * LN2;
+    store_row<DB>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc[n],
+                  total == 0.f ? 0.f : 1.f / total, a.D, a.vec, lane);
+  }
+}
+
+// Few packed rows (one tile of 16): the keys pass once, from memory to
+// registers in the operand layouts, 16 a wave at a time, the next 16 loaded
+// while these are used.  Bandwidth-bound: the keys are split over workgroups.
+template <int DB>
+struct FewTile {
+  static constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
+  typedef typename Vec<VW>::T V;
+  f32x4 k[DB];
+  V v[4][T];
+  __device__ __forceinline__ void load(const Args &a, const float *kp, const float *vp, int k0, int lo, int hi,
+                                       int lane) {
+    const int g = lane >> 4, m = lane & 15;
+    const int key = k0 + m;
+    const bool in = key >= lo && key < hi;
+    const float *p = kp + (long)key * a.k.r;
+#pragma unroll
+    for (int u = 0; u < DB; u++) {
+      k[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (in) k[u] = load4(p, 16 * u + 4 * g, a.D, a.vec);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int kv = k0 + 4 * g + r;
+      const bool have = kv >= lo && kv < hi;
+      const float *x = vp + (long)kv * a.v.r;
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        const int d = 16 * VW * t + VW * m;
+        V w = {};
+        if (have) {
+          if (a.vec) {
+            if (d < a.D) w = *(const V *)(x + d);
+          } else {
+#pragma unroll
+            for (int c = 0; c < VW; c++)
+              if (d + c < a.D) ((float *)&w)[c] = x[d + c];
+          }
+        }
+        v[r][t] = w;
+      }
+    }
+  }
+};
+
+template <int DB>
+__global__ void __launch_bounds__(256, 2)
+    attn_few_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
+                    const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
+                    float *__restrict__ ws_ml, float *__restrict__ ws_o) {
+  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T, LD = DB * 16 + 4;
+  __shared__ __attribute__((aligned(16))) float part[4][16 * LD];
+  __shared__ float pml[4][2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int r0 = blockIdx.x / nbh * 16, r1 = r0 + 16 < a.R ? r0 + 16 : a.R;
+  const Span sp = span_of(a, b, r0, r1);
+  int k_first = sp.lo / 16 * 16, k_end = sp.hi;
+  if (a.splits > 1) {
+    const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
+    if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
+    if (c1 < k_end) k_end = (int)c1;
+  }
+  const int row = r0 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
+  const bool in = row < a.R;
+  Range rg = {0, 0};
+  if (in) rg = range_of(a, b, i);
+  f32x4 qf[DB], acc[DB];
+  float mx = -INFINITY, sum = 0.f;
+  const float *qp = q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h;
+#pragma unroll
+  for (int u = 0; u < DB; u++) {
+    qf[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (in) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
+  }
+  const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
+  FewTile<DB> cur, next;
+  int k0 = k_first + wave * 16;
+  if (k0 < k_end) cur.load(a, kp, vp, k0, sp.lo, k_end, lane);
+  for (; k0 < k_end; k0 += 64) {
+    if (k0 + 64 < k_end) next.load(a, kp, vp, k0 + 64, sp.lo, k_end, lane);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < DB; u++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) s = mfma(cur.k[u][c], qf[u][c], s);
+    float t = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int key = k0 + 4 * g + r;
+      if (key < rg.lo || key >= rg.hi) s[r] = -INFINITY;
+      t = fmaxf(t, s[r]);
+    }
+    t = fmaxf(col_max(t), mx);
+    const float base = t == -INFINITY ? 0.f : t;
+    if (__any(t > mx)) {
+      const float f = exp2_fast(mx - base);
+      sum *= f;
+#pragma unroll
+      for (int u = 0; u < DB; u++) acc[u] *= f;
+    }
+    mx = t;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      s[r] = exp2_fast(s[r] - base);
+      sum += s[r];
+    }
+    bool odd = false;
+    if (k0 < sp.ilo || k0 + 16 > sp.ihi) {
+      float z = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int t2 = 0; t2 < T; t2++)
+#pragma unroll
+          for (int c = 0; c < VW; c++) z = fmaf(Vec<VW>::at(cur.v[r][t2], c), 0.f, z);
+      odd = __any(z != z);
+    }
+    if (odd) {
+      // as product_masked, the values from memory: rows behind the keys'
+      // end are not seen and not read
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll 1
+        for (int kg = 0; kg < 4; kg++) {
+          const int key = k0 + 4 * kg + r;
+          const float p = __shfl(s[r], m + 16 * kg);
+          if (key < rg.lo || key >= rg.hi || key >= k_end) continue;
+          const float *x = vp + (long)key * a.v.r;
+#pragma unroll
+          for (int t2 = 0; t2 < T; t2++)
+#pragma unroll
+            for (int c = 0; c < VW; c++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int d = 16 * VW * t2 + VW * (4 * g + e) + c;
+                if (d < a.D) acc[t2 * VW + c][e] = fmaf(p, x[d], acc[t2 * VW + c][e]);
+              }
+        }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int t2 = 0; t2 < T; t2++)
+#pragma unroll
+          for (int c = 0; c < VW; c++)
+            acc[t2 * VW + c] = mfma(Vec<VW>::at(cur.v[r][t2], c), s[r], acc[t2 * VW + c]);
+    }
+    cur = next;
+  }
+  sum = col_sum(sum);
+  // the four waves' parts, joined in wave order
+  if (g == 0) {
+    pml[wave][0][m] = mx;
+    pml[wave][1][m] = sum;
+  }
+  store_row<DB>(&part[wave][m * LD], acc, 1.f, DB * 16, 1, lane);
+  __syncthreads();
+  for (int e = tid; e < 16 * DB * 16; e += 256) {
+    const int rr = e / (DB * 16), d = e % (DB * 16), r = r0 + rr;
+    if (r >= a.R) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) top = fmaxf(top, pml[w][0][rr]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = exp2_fast(pml[w][0][rr] - base);
+      total = fmaf(f, pml[w][1][rr], total);
+      x = fmaf(f, part[w][rr * LD + d], x);
+    }
+    if (a.splits > 1) {
+      const long at = ((long)blockIdx.y * nbh + bh) * a.R + r;
+      if (d == 0) {
+        ws_ml[2 * at] = top;
+        ws_ml[2 * at + 1] = total;
+      }
+      ws_o[at * (DB * 16) + d] = x;
+      continue;
+    }
+    const int qi = r / a.G, hh = h * a.G + r - qi * a.G;
+    if (lse && d == 0)
+      lse[((long)b * a.Hkv * a.G + hh) * a.Lq + qi] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+    if (d < a.D)
+      o[(long)b * a.o.b + (long)qi * a.o.r + (long)hh * a.o.h + d] = total == 0.f ? 0.f : x / total;
+  }
+}
+
+// The parts of a row that several workgroups took, joined in their order; one
+// wave a row.  A part without keys has sum 0 and nothing else to read.
+__global__ void __launch_bounds__(256)
+    attn_join_kernel(Args a, int width, const float *__restrict__ ws_ml, const float *__restrict__ ws_o,
+                     float *__restrict__ o, float *__restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const long rows = (long)a.B * a.Hkv * a.R;
+  for (long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6); at < rows; at += (long)gridDim.x * 4) {
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ws_ml[2 * (s * rows + at)]);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int s = 0; s < a.splits; s++) {
+    const float l = ws_ml[2 * (s * rows + at) + 1];
+    if (l == 0.f) continue;
+    const float f = exp2_fast(ws_ml[2 * (s * rows + at)] - base);
+    const float *p = ws_o + (s * rows + at) * width;
+    total = fmaf(f, l, total);
+    if (lane < a.D) x0 = fmaf(f, p[lane], x0);
+    if (lane + 64 < a.D) x1 = fmaf(f, p[lane + 64], x1);
+  }
+  const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
+  const int hq = bh % a.Hkv * a.G + r - i * a.G;
+  if (lse && lane == 0)
+    lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+  float *p = o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h;
+  const float f = total == 0.f ? 0.f : 1.f / total;
+  if (lane < a.D) p[lane] = x0 * f;
+  if (lane + 64 < a.D) p[lane + 64] = x1 * f;
+  }
+}
+
+// ---------------------------------------------------------------- backward
+
+// delta[b][h][i] = do . o, 16 lanes a row
+__global__ void __launch_bounds__(256)
+    attn_delta_kernel(Args a, const float *__restrict__ o, const float *__restrict__ dout,
+                      float *__restrict__ delta) {
+  const long rows = (long)a.B * a.Hkv * a.G * a.Lq;
+  const int m = threadIdx.x & 15;
+  // 16 lanes share `at`: whole groups leave the loop together
+  for (long at = ((long)blockIdx.x * 256 + threadIdx.x) >> 4; at < rows; at += (long)gridDim.x * 16) {
+    float s = 0.f;
+    const int i = (int)(at % a.Lq), Hq = a.Hkv * a.G;
+    const long bh = at / a.Lq;
+    const int b = (int)(bh / Hq), h = (int)(bh % Hq);
+    if (i < queries_of(a, b)) {
+      const long off = (long)b * a.o.b + (long)i * a.o.r + (long)h * a.o.h;
+      for (int c = 4 * m; c < a.D; c += 64) {
+        const f32x4 x = load4(o + off, c, a.D, a.vec), y = load4(dout + off, c, a.D, a.vec);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s = fmaf(x[j], y[j], s);
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x);
+    if (m == 0) delta[at] = s;
+  }
+}
+
+// dq of 64 packed rows (16 a wave): keys and values through LDS as in the
+// forward pass
+template <int DB>
+__global__ void __launch_bounds__(256, 2)
+    attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                   const float *__restrict__ dout, const float *__restrict__ lse,
+                   const float *__restrict__ delta, float *__restrict__ dq) {
+  typedef Stage<DB, 256> S;
+  __shared__ __attribute__((aligned(16))) float lk[KT * S::LD], lv[KT * S::LD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
+  const int r0 = tile * 64, r1 = r0 + 64 < a.R ? r0 + 64 : a.R;
+  const Span sp = span_of(a, b, r0, r1);
+  const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
+  const bool in = row < a.R;
+  Range rg = {0, 0};
+  float l2 = 0.f, dl = 0.f;
+  f32x4 qf[DB], df[DB], acc[DB];
+  const bool live = in && i < queries_of(a, b);
+  if (live) {
+    rg = range_of(a, b, i);
+    const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
+    l2 = lse[at] * LOG2E;
+    if (l2 == -INFINITY) l2 = 0.f;  // no key has weight: exp2(-inf - 0) = 0
+    dl = delta[at];
+  }
+#pragma unroll
+  for (int u = 0; u < DB; u++) {
+    qf[u] = df[u] = acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      qf[u] = load4(q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, 16 * u + 4 * g, a.D, a.vec) *
+              (a.scale * LOG2E);
+      df[u] = load4(dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, 16 * u + 4 * g, a.D, a.vec);
+    }
+  }
+  const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
+  S sk, sv;
+  const int k_first = sp.lo / KT * KT, k_end = sp.hi;
+  if (k_first < k_end) {
+    sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
+    sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+  }
+  for (int k0 = k_first; k0 < k_end; k0 += KT) {
+    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi;
+    sk.store(lk, tid);
+    sv.store(lv, tid);
+    bool odd = false;
+    if (mixed)
+      odd = __syncthreads_or(sk.odd());
+    else
+      __syncthreads();
+    if (k0 + KT < k_end) {
+      sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
+      sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
+    }
+    f32x4 s[2], dp[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++) s[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < DB; u++)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) {
+        const f32x4 ka = *(const f32x4 *)(lk + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
+        const f32x4 va = *(const f32x4 *)(lv + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          s[kb] = mfma(ka[c], qf[u][c], s[kb]);
+          dp[kb] = mfma(va[c], df[u][c], dp[kb]);
+        }
+      }
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int key = k0 + kb * 16 + 4 * g + r;
+        const float x = exp2_fast(s[kb][r] - l2) * (dp[kb][r] - dl);
+        s[kb][r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
+      }
+    if (odd)
+      product_masked<DB, 2>(acc, s, lk, S::LD, lane,
+                            [&](int kk) { return k0 + kk >= rg.lo && k0 + kk < rg.hi; });
+    else
+      product<DB, 2>(acc, s, lk, S::LD, lane);
+    __syncthreads();
+  }
+  if (in) store_row<DB>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
+}
+
+// dk and dv of 64 keys (16 a wave): the packed query rows that see any of
+// them through LDS, q and do
+template <int DB>
+__global__ void __launch_bounds__(256, 2)
+    attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                    const float *__restrict__ dout, const float *__restrict__ lse,
+                    const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv) {
+  typedef Stage<DB, 256> S;
+  __shared__ __attribute__((aligned(16))) float lq[KT * S::LD], ld[KT * S::LD], rl[KT], rd[KT];
+  __shared__ int rlo[KT], rhi[KT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int k0 = blockIdx.x / nbh * 64, key = k0 + wave * 16 + m;
+  // the queries that see a key of [k0, k0 + 64)
+  const long start = start_of(a, b);
+  const int keys = keys_of(a, b);
+  long i0 = 0, i1 = queries_of(a, b);
+  if (a.causal) {
+    if (k0 - start > i0) i0 = k0 - start;
+  } else if (a.window > 0 && k0 - a.window - start + 1 > i0) {
+    i0 = k0 - a.window - start + 1;
+  }
+  if (a.window > 0 && k0 + 64 + a.window - 1 - start < i1) i1 = k0 + 64 + a.window - 1 - start;
+  if (k0 >= keys || i0 > i1) i0 = i1 = 0;
+  if (i1 < i0) i1 = i0;
+  const int r_first = (int)i0 * a.G, r_end = (int)i1 * a.G;
+
+  const bool in = key < a.Lk, live = key < keys;
+  f32x4 kf[DB], vf[DB], ak[DB], av[DB];
+  const float *kp = k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
+  const float *vp = v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
+#pragma unroll
+  for (int u = 0; u < DB; u++) {
+    kf[u] = vf[u] = ak[u] = av[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      kf[u] = load4(kp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
+      vf[u] = load4(vp, 16 * u + 4 * g, a.D, a.vec);
+    }
+  }
+  const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
+  const float *dp_ = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
+  S sq, sd;
+  if (r_first < r_end) {
+    sq.load_rows(qp, a.q.r, a.q.h, a.G, r_first, r_end, a.D, a.vec, tid);
+    sd.load_rows(dp_, a.o.r, a.o.h, a.G, r_first, r_end, a.D, a.vec, tid);
+  }
+  for (int r0 = r_first; r0 < r_end; r0 += KT) {
+    sq.store(lq, tid);
+    sd.store(ld, tid);
+    if (tid < KT) {
+      const int row = r0 + tid, i = row / a.G;
+      Range rg = {0, 0};
+      float l2 = 0.f, dl = 0.f;
+      if (row < r_end) {
+        rg = range_of(a, b, i);
+        const long at = ((long)b * a.Hkv * a.G + h * a.G + row - i * a.G) * a.Lq + i;
+        l2 = lse[at] * LOG2E;
+        if (l2 == -INFINITY) l2 = 0.f;
+        dl = delta[at];
+      }
+      rl[tid] = l2;
+      rd[tid] = dl;
+      rlo[tid] = rg.lo;
+      rhi[tid] = rg.hi;
+    }
+    const Span sp = span_of(a, b, r0, r0 + KT < a.R ? r0 + KT : a.R);
+    const bool mixed = r0 + KT > r_end || k0 < sp.ilo || k0 + 64 > sp.ihi;
+    bool odd = false;
+    if (mixed)
+      odd = __syncthreads_or(sq.odd() || sd.odd());
+    else
+      __syncthreads();
+    if (r0 + KT < r_end) {
+      sq.load_rows(qp, a.q.r, a.q.h, a.G, r0 + KT, r_end, a.D, a.vec, tid);
+      sd.load_rows(dp_, a.o.r, a.o.h, a.G, r0 + KT, r_end, a.D, a.vec, tid);
+    }
+    f32x4 s[2], dp[2];
+#pragma unroll
+    for (int n = 0; n < 2; n++) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < DB; u++)
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        const f32x4 qa = *(const f32x4 *)(lq + (n * 16 + m) * S::LD + 16 * u + 4 * g);
+        const f32x4 da = *(const f32x4 *)(ld + (n * 16 + m) * S::LD + 16 * u + 4 * g);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          s[n] = mfma(qa[c], kf[u][c], s[n]);
+          dp[n] = mfma(da[c], vf[u][c], dp[n]);
+        }
+      }
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      const f32x4 l2 = *(const f32x4 *)(rl + n * 16 + 4 * g), dl = *(const f32x4 *)(rd + n * 16 + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        float p = exp2_fast(s[n][r] - l2[r]), x = p * (dp[n][r] - dl[r]);
+        if (mixed) {
+          const int e = n * 16 + 4 * g + r;
+          if (key < rlo[e] || key >= rhi[e]) p = x = 0.f;
+        }
+        s[n][r] = p;
+        dp[n][r] = x;
+      }
+    }
+    if (odd) {
+      auto seen = [&](int e) { return key >= rlo[e] && key < rhi[e]; };
+      product_masked<DB, 2>(av, s, ld, S::LD, lane, seen);
+      product_masked<DB, 2>(ak, dp, lq, S::LD, lane, seen);
+    } else {
+      product<DB, 2>(av, s, ld, S::LD, lane);
+      product<DB, 2>(ak, dp, lq, S::LD, lane);
+    }
+    __syncthreads();
+  }
+  if (in) {
+    store_row<DB>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
+    store_row<DB>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+Strides packed(const TTStrides &s, long rows, int heads, int dim) {
+  Strides p;
+  p.h = s.head ? s.head : dim;
+  p.r = s.row ? s.row : (long)heads * dim;
+  p.b = s.batch ? s.batch : rows * p.r;
+  return p;
+}
+
+bool aligned(const void *p, const Strides &s) {
+  return ((uintptr_t)p & 15) == 0 && s.b % 4 == 0 && s.r % 4 == 0 && s.h % 4 == 0;
+}
+
+// 16-column blocks that the kernels hold for a head dimension
+int blocks(int dim) {
+  const int n = (dim + 15) / 16;
+  return n == 7 ? 8 : n;
+}
+
+struct Plan {
+  bool few;
+  int qb;      // row blocks of 16 a wave
+  int tiles;   // row tiles
+  int splits, chunk;
+  int width;   // floats a row of the parts takes
+};
+
+// 0: the arguments describe an attention that the kernels' 32-bit row and
+// grid arithmetic covers
+int check(const TTAttention *t) {
+  if (!t || t->batch <= 0 || t->q_rows <= 0 || t->k_rows <= 0 || t->q_heads <= 0 || t->kv_heads <= 0 ||
+      t->head_dim <= 0 || t->head_dim > TT_ATTENTION_MAX_DIM || t->q_heads % t->kv_heads != 0 || t->window < 0 ||
+      !(t->scale == t->scale) || isinf(t->scale))
+    return -1;
+  const TTStrides *all[4] = {&t->q, &t->k, &t->v, &t->o};
+  for (const TTStrides *s : all)
+    if (s->batch < 0 || s->row < 0 || s->head < 0) return -1;
+  const long G = t->q_heads / t->kv_heads, lim = 1L << 30, grid = (1L << 24) - 1;
+  if (t->q_rows > lim / G || t->k_rows > lim || t->batch > grid / t->kv_heads) return -1;
+  const long nbh = t->batch * t->kv_heads;  // a grid axis has less than 2^32 threads
+  if ((t->q_rows * G + 63) / 64 > grid / nbh || (t->k_rows + 63) / 64 > grid / nbh) return -1;
+  return 0;
+}
+
+Plan plan_of(const TTAttention *t) {
+  Plan p;
+  const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
+  p.width = 16 * blocks(t->head_dim);
+  p.few = R <= 16;
+  p.qb = 1;
+  if (p.few) {
+    p.tiles = 1;
+    // parts of 64 to 1024 keys, about eight workgroups a CU
+    long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
+    c = c < 64 ? 64 : c > 1024 ? 1024 : c;
+    p.chunk = (int)c;
+    p.splits = (int)((t->k_rows + c - 1) / c);
+  } else {
+    if ((R + 127) / 128 * nbh >= 512) p.qb = 2;
+    p.tiles = (int)((R + 64 * p.qb - 1) / (64 * p.qb));
+    long s = 512 / (p.tiles * nbh), most = t->k_rows / 256;
+    s = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
+    long c = (t->k_rows + s - 1) / s;
+    c = (c + KT - 1) / KT * KT;
+    p.chunk = (int)c;
+    p.splits = (int)((t->k_rows + c - 1) / c);
+  }
+  if (p.splits > 65535) {  // the grid's second axis
+    long c = ((t->k_rows + 65534) / 65535 + 63) / 64 * 64;
+    p.chunk = (int)c;
+    p.splits = (int)((t->k_rows + c - 1) / c);
+  }
+  return p;
+}
+
+Args args_of(const TTAttention *t) {
+  Args a;
+  a.B = (int)t->batch;
+  a.Lq = (int)t->q_rows;
+  a.Lk = (int)t->k_rows;
+  a.Hkv = t->kv_heads;
+  a.G = t->q_heads / t->kv_heads;
+  a.D = t->head_dim;
+  a.R = a.Lq * a.G;
+  a.causal = t->causal != 0;
+  a.window = t->window < 1L << 40 ? t->window : 1L << 40;
+  a.scale = t->scale != 0.f ? t->scale : 1.f / sqrtf((float)t->head_dim);
+  a.q_start = t->q_start;
+  a.q_len = t->q_len;
+  a.k_len = t->k_len;
+  a.q = packed(t->q, t->q_rows, t->q_heads, t->head_dim);
+  a.k = packed(t->k, t->k_rows, t->kv_heads, t->head_dim);
+  a.v = packed(t->v, t->k_rows, t->kv_heads, t->head_dim);
+  a.o = packed(t->o, t->q_rows, t->q_heads, t->head_dim);
+  a.vec = 0;
+  a.chunk = 0;
+  a.splits = 1;
+  return a;
+}
+
+template <int DB>
+void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
+             float *ml, float *wo) {
+  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
+  if (p.few)
+    hipLaunchKernelGGL(attn_few_kernel<DB>, grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+  else if (p.qb == 1)
+    hipLaunchKernelGGL((attn_fwd_kernel<DB, 1>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+  else
+    hipLaunchKernelGGL((attn_fwd_kernel<DB, 2>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+}
+
+template <int DB>
+void run_bwd(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
+             const float *delta, float *dq, float *dk, float *dv) {
+  const long nbh = (long)a.B * a.Hkv;
+  if (dq)
+    hipLaunchKernelGGL(attn_dq_kernel<DB>, dim3((unsigned)(((long)a.R + 63) / 64 * nbh)), dim3(256), 0, stream(),
+                       a, q, k, v, dout, lse, delta, dq);
+  if (dk)
+    hipLaunchKernelGGL(attn_dkv_kernel<DB>, dim3((unsigned)(((long)a.Lk + 63) / 64 * nbh)), dim3(256), 0,
+                       stream(), a, q, k, v, dout, lse, delta, dk, dv);
+}
+
+#define BY_DIM(D, F, ...)              \
+  switch (blocks(D)) {                 \
+    case 1: F<1>(__VA_ARGS__); break;  \
+    case 2: F<2>(__VA_ARGS__); break;  \
+    case 3: F<3>(__VA_ARGS__); break;  \
+    case 4: F<4>(__VA_ARGS__); break;  \
+    case 5: F<5>(__VA_ARGS__); break;  \
+    case 6: F<6>(__VA_ARGS__); break;  \
+    default: F<8>(__VA_ARGS__); break; \
+  }
+
+size_t fwd_bytes(const TTAttention *t) {
+  const Plan p = plan_of(t);
+  if (p.splits <= 1) return 0;
+  const size_t rows = (size_t)t->batch * t->q_heads * t->q_rows;
+  return sizeof(float) * rows * p.splits * (2 + (size_t)p.width);
+}
+
+}  // namespace
+
+extern "C" size_t tt_k_attention_fwd_ws(const TTAttention *t) { return check(t) ? 0 : fwd_bytes(t); }
+
+extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const float *k, const float *v, float *o,
+                                  float *lse, void *ws) {
+  if (check(t) || !q || !k || !v || !o) return -1;
+  if (ttrt_init() != 0) return -3;
+  const Plan p = plan_of(t);
+  Args a = args_of(t);
+  a.vec = a.D % 4 == 0 && aligned(q, a.q) && aligned(k, a.k) && aligned(v, a.v) && aligned(o, a.o);
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  const size_t need = fwd_bytes(t);
+  float *own = NULL, *w = (float *)ws;
+  if (need && !w) {
+    w = own = (float *)ttrt_alloc(need);
+    if (!own) return -2;
+  }
+  float *ml = w, *wo = w ? w + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
+  Plan pl = p;
+  BY_DIM(a.D, run_fwd, pl, a, q, k, v, o, lse, ml, wo);
+  if (p.splits > 1) {
+    const long rows = (long)a.B * a.Hkv * a.R;
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((rows + 3) / 4 < 8192 ? (rows + 3) / 4 : 8192)), dim3(256), 0, stream(), a, p.width, ml,
+                       wo, o, lse);
+  }
+  ttrt_free(own);
+  return launched();
+}
+
+extern "C" size_t tt_k_attention_bwd_ws(const TTAttention *t) {
+  return check(t) ? 0 : sizeof(float) * (size_t)t->batch * t->q_heads * t->q_rows;
+}
+
+extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const float *k, const float *v,
+                                  const float *o, const float *dout, const float *lse, float *dq, float *dk,
+                                  float *dv, void *ws) {
+  if (check(t) || !q || !k || !v || !o || !dout || !lse || (dk == NULL) != (dv == NULL)) return -1;
+  if (!dq && !dk) return 0;
+  if (ttrt_init() != 0) return -3;
+  Args a = args_of(t);
+  a.vec = a.D % 4 == 0 && aligned(q, a.q) && aligned(k, a.k) && aligned(v, a.v) && aligned(o, a.o) &&
+          aligned(dout, a.o) && aligned(dq, a.q) && aligned(dk, a.k) && aligned(dv, a.v);
+  float *own = NULL, *delta = (float *)ws;
+  if (!delta) {
+    delta = own = (float *)ttrt_alloc(tt_k_attention_bwd_ws(t));
+    if (!own) return -2;
+  }
+  const long rows = (long)a.B * a.Hkv * a.R;
+  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)), dim3(256), 0, stream(), a, o, dout,
+                     delta);
+  BY_DIM(a.D, run_bwd, a, q, k, v, dout, lse, delta, dq, dk, dv);
+  ttrt_free(own);
+  return launched();
+}

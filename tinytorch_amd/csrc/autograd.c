@@ -60,6 +60,10 @@ struct AGNode {
         /* matmul: sda handed over by its softmax-CE; *stale set when the
          * weights they were formed with are about to change */
         struct { Tensor *sda[3]; int *stale; } mm;
+        struct { Tensor *stat; int w, b; } ln;  /* mean | rstd of the rows; the inputs that w and
+                                                   b are (0: none) */
+        struct { struct RopeState *s; } rope;
+        struct { struct AttnState *s; } attn;
     } at;
     unsigned long long pass;     /* backward pass that scheduled the node */
     int     walk;                /* depth-first walk: next input to enter */
@@ -96,6 +100,22 @@ static int conv_dw_deferred(const float *gd, const unsigned char *codes, const f
 static void backward_maxpool(AGNode *n);
 static void backward_avgpool(AGNode *n);
 static void backward_softmax_ce(AGNode *n);
+static void backward_layernorm(AGNode *n);
+static void backward_rope(AGNode *n);
+static void backward_attention(AGNode *n);
+
+/* what a rotation and an attention keep for their backward rules */
+struct RopeState {
+    TTRope r;
+    int heads;
+    long rows, seq_len;
+    int32_t *positions;          /* device, or NULL */
+};
+struct AttnState {
+    TTAttention a;               /* its length arrays in `lengths` */
+    int32_t *lengths;            /* device, or NULL */
+    Tensor *lse;                 /* NULL when no input needs a gradient */
+};
 
 static void drop_conv(AGNode *n) { ttrt_free(n->at.conv.col); }
 static void drop_pool(AGNode *n) { tt_release(n->at.win.codes); }
@@ -112,6 +132,20 @@ static void drop_ce(AGNode *n) {
     tt_release(n->at.ce.seed);
     spec_drop(n->at.ce.sda, &n->at.ce.stale);
 }
+static void drop_ln(AGNode *n) { tt_release(n->at.ln.stat); }
+static void rope_free(struct RopeState *s) {
+    if (!s) return;
+    ttrt_free(s->positions);
+    free(s);
+}
+static void attn_free(struct AttnState *s) {
+    if (!s) return;
+    ttrt_free(s->lengths);
+    tt_release(s->lse);
+    free(s);
+}
+static void drop_rope(AGNode *n) { rope_free(n->at.rope.s); }
+static void drop_attn(AGNode *n) { attn_free(n->at.attn.s); }
 static void drop_mm(AGNode *n) { spec_drop(n->at.mm.sda, &n->at.mm.stale); }
 
 static const AGOp OP_ADD = {"add", backward_add, NULL};
@@ -127,6 +161,10 @@ static const AGOp OP_CONV2D = {"conv2d", backward_conv2d, drop_conv};
 static const AGOp OP_MAXPOOL2D = {"maxpool2d", backward_maxpool, drop_pool};
 static const AGOp OP_AVGPOOL2D = {"avgpool2d", backward_avgpool, NULL};
 static const AGOp OP_SOFTMAX_CE = {"softmax_ce", backward_softmax_ce, drop_ce};
+static const AGOp OP_DISTILL = {"distill", backward_softmax_ce, drop_ce};
+static const AGOp OP_LAYERNORM = {"layernorm", backward_layernorm, drop_ln};
+static const AGOp OP_ROPE = {"rope", backward_rope, drop_rope};
+static const AGOp OP_ATTENTION = {"attention", backward_attention, drop_attn};
 
 /* ---------- gradient accumulation ---------- */
 
@@ -772,6 +810,148 @@ AGNode *ag_softmax_ce(AGNode *logits, const int *labels, long rows) {
 
 Tensor *ag_softmax_ce_probs(const AGNode *n) {
     return (n && n->op == &OP_SOFTMAX_CE) ? n->at.ce.probs : NULL;
+}
+
+/* ---------- transformer nodes ---------- */
+
+AGNode *ag_layernorm(AGNode *x, AGNode *w, AGNode *b, float eps) {
+    if (!x || x->val->ndim < 1 || !(eps >= 0.0f) || isinf(eps)) return NULL;
+    const Tensor *v = x->val;
+    const long cols = v->shape[v->ndim - 1], rows = v->numel / cols, two = 2 * rows;
+    if ((w && w->val->numel != cols) || (b && b->val->numel != cols)) return NULL;
+    const float *xd = tt_dev(x->val), *wd = w ? tt_dev(w->val) : NULL,
+                *bd = b ? tt_dev(b->val) : NULL;
+    if (!xd || (w && !wd) || (b && !bd)) return NULL;
+    const int grad = x->needs_grad || (w && w->needs_grad);
+    Tensor *out = tt_empty_like(v), *stat = out && grad ? tt_empty_dev(&two, 1) : NULL;
+    if (!out || (grad && !stat) ||
+        tt_k_layernorm_fwd(xd, wd, bd, out->dev, stat ? stat->dev : NULL,
+                           stat ? stat->dev + rows : NULL, rows, cols, eps) != 0) {
+        tt_release(out);
+        tt_release(stat);
+        return NULL;
+    }
+    AGNode *n = make_node(out, &OP_LAYERNORM, x, w, b);
+    if (!n) { tt_release(stat); return NULL; }
+    n->at.ln.stat = stat;
+    n->at.ln.w = w ? 1 : 0;
+    n->at.ln.b = b ? 1 + (w ? 1 : 0) : 0;
+    return n;
+}
+
+AGNode *ag_rope(AGNode *x, const TTRope *r, int heads, const int *positions, long seq_len) {
+    if (!x || !r || heads <= 0 || r->head_dim <= 0 || x->val->ndim < 1) return NULL;
+    const Tensor *v = x->val;
+    const long last = v->shape[v->ndim - 1], width = (long)heads * r->head_dim;
+    if (last != width &&
+        (v->ndim < 2 || last != r->head_dim || v->shape[v->ndim - 2] != heads))
+        return NULL;
+    const float *xd = tt_dev(x->val);
+    Tensor *out = xd ? tt_empty_like(v) : NULL;
+    struct RopeState *s = out ? (struct RopeState *)calloc(1, sizeof(*s)) : NULL;
+    if (!s) { tt_release(out); return NULL; }
+    s->r = *r;
+    s->heads = heads;
+    s->rows = v->numel / width;
+    s->seq_len = seq_len;
+    if (positions) {
+        const size_t bytes = sizeof(int32_t) * (size_t)s->rows;
+        s->positions = (int32_t *)ttrt_alloc(bytes);
+        if (!s->positions || ttrt_h2d_async(s->positions, positions, bytes) != 0) goto bad;
+    }
+    if (tt_k_rope(&s->r, xd, out->dev, s->positions, s->rows, seq_len, heads, 0, 0, 0) != 0) goto bad;
+    AGNode *n = make_node(out, &OP_ROPE, x, NULL, NULL);
+    if (!n) { rope_free(s); return NULL; }
+    n->at.rope.s = s;
+    return n;
+bad:
+    rope_free(s);
+    tt_release(out);
+    return NULL;
+}
+
+static int packed(const TTStrides *s) { return !s->batch && !s->row && !s->head; }
+
+AGNode *ag_attention(AGNode *q, AGNode *k, AGNode *v, const TTAttention *a) {
+    if (!q || !k || !v || !a || a->batch <= 0 || a->q_rows <= 0 || a->k_rows <= 0 ||
+        a->q_heads <= 0 || a->kv_heads <= 0 || a->head_dim <= 0 || !packed(&a->q) ||
+        !packed(&a->k) || !packed(&a->v) || !packed(&a->o))
+        return NULL;
+    /* element counts by division: the products could pass 64 bits */
+    const long qn = (long)a->q_heads * a->head_dim, kn = (long)a->kv_heads * a->head_dim;
+    const long qt = q->val->numel, kt = k->val->numel;
+    if (qt % qn || kt % kn || v->val->numel != kt || qt / qn % a->batch || kt / kn % a->batch ||
+        qt / qn / a->batch != a->q_rows || kt / kn / a->batch != a->k_rows)
+        return NULL;
+    const float *qd = tt_dev(q->val), *kd = tt_dev(k->val), *vd = tt_dev(v->val);
+    if (!qd || !kd || !vd) return NULL;
+    const int grad = q->needs_grad || k->needs_grad || v->needs_grad;
+    struct AttnState *s = (struct AttnState *)calloc(1, sizeof(*s));
+    Tensor *out = s ? tt_empty_like(q->val) : NULL;
+    if (!out) { free(s); return NULL; }
+    s->a = *a;
+    if (a->q_start || a->q_len || a->k_len) {
+        const int32_t *host[3] = {a->q_start, a->q_len, a->k_len};
+        const int32_t **dev[3] = {&s->a.q_start, &s->a.q_len, &s->a.k_len};
+        const size_t bytes = sizeof(int32_t) * (size_t)a->batch;
+        s->lengths = (int32_t *)ttrt_alloc(3 * bytes);
+        if (!s->lengths) goto bad;
+        for (int i = 0; i < 3; i++) {
+            if (!host[i]) continue;
+            if (ttrt_h2d_async(s->lengths + i * a->batch, host[i], bytes) != 0) goto bad;
+            *dev[i] = s->lengths + i * a->batch;
+        }
+    }
+    if (grad) {
+        const long rows = a->batch * a->q_heads * a->q_rows;
+        s->lse = tt_empty_dev(&rows, 1);
+        if (!s->lse) goto bad;
+    }
+    if (tt_k_attention_fwd(&s->a, qd, kd, vd, out->dev, s->lse ? s->lse->dev : NULL, NULL) != 0)
+        goto bad;
+    AGNode *n = make_node(out, &OP_ATTENTION, q, k, v);
+    if (!n) { attn_free(s); return NULL; }
+    n->at.attn.s = s;
+    return n;
+bad:
+    attn_free(s);
+    tt_release(out);
+    return NULL;
+}
+
+AGNode *ag_distill(AGNode *logits, const int *ids, const float *teacher, int top,
+                   float temperature) {
+    if (!logits || !ids || !teacher || top <= 0 || top > TT_DISTILL_MAX_TOP ||
+        logits->val->ndim != 2 || logits->val->shape[0] > 0x7fffffffL ||
+        logits->val->shape[1] > 0x7fffffffL)
+        return NULL;
+    const long rows = logits->val->shape[0], one = 1;
+    const int cols = (int)logits->val->shape[1];
+    const float *z = tt_dev(logits->val);
+    if (!z) return NULL;
+    const size_t n = (size_t)rows * (size_t)top;
+    int32_t *di = (int32_t *)ttrt_alloc(sizeof(int32_t) * n);
+    float *dt = (float *)ttrt_alloc(sizeof(float) * n);
+    Tensor *rl = tt_empty_dev(&rows, 1), *loss = tt_empty_dev(&one, 1);
+    Tensor *seed = logits->needs_grad ? tt_empty_like(logits->val) : NULL;
+    const int ok = di && dt && rl && loss && (seed || !logits->needs_grad) &&
+                   ttrt_h2d_async(di, ids, sizeof(int32_t) * n) == 0 &&
+                   ttrt_h2d_async(dt, teacher, sizeof(float) * n) == 0 &&
+                   tt_k_distill(z, di, dt, top, temperature, rl->dev, seed ? seed->dev : NULL, rows,
+                                cols, 1.0f / (float)rows) == 0 &&
+                   tt_k_ce_mean_rows(rl->dev, loss->dev, (int)rows) == 0;
+    ttrt_free(di);
+    ttrt_free(dt);
+    tt_release(rl);
+    if (!ok) {
+        tt_release(loss);
+        tt_release(seed);
+        return NULL;
+    }
+    AGNode *node = make_node(loss, &OP_DISTILL, logits, NULL, NULL);
+    if (!node) { tt_release(seed); return NULL; }
+    node->at.ce.seed = seed;
+    return node;
 }
 
 /* ---------- accessors ---------- */
@@ -1497,6 +1677,75 @@ static void backward_softmax_ce(AGNode *n) {
         return;
     }
     accum_move(a, t);
+}
+
+static void backward_layernorm(AGNode *n) {
+    AGNode *x = n->in[0], *w = n->at.ln.w ? n->in[n->at.ln.w] : NULL,
+           *b = n->at.ln.b ? n->in[n->at.ln.b] : NULL;
+    const Tensor *v = x->val;
+    const long cols = v->shape[v->ndim - 1], rows = v->numel / cols;
+    const float *g = tt_dev(n->grad);
+    if (!g) return;
+    if (!needs(x) && !needs(w)) {  /* no statistics were kept: db alone */
+        Tensor *db = needs(b) && cols <= 0x7fffffffL && rows <= 0x7fffffffL
+                         ? tt_empty_like(b->val) : NULL;
+        if (db && ttk_colsum(g, db->dev, (int)rows, (int)cols) == 0) accum_move(b, db);
+        else tt_release(db);
+        return;
+    }
+    const float *xd = tt_dev(x->val), *wd = w ? tt_dev(w->val) : NULL;
+    const float *st = tt_dev(n->at.ln.stat);
+    if (!xd || !st || (w && !wd)) return;
+    Tensor *dx = needs(x) ? tt_empty_like(v) : NULL;
+    Tensor *dw = needs(w) ? tt_empty_like(w->val) : NULL;
+    Tensor *db = needs(b) ? tt_empty_like(b->val) : NULL;
+    if ((needs(x) && !dx) || (needs(w) && !dw) || (needs(b) && !db) ||
+        tt_k_layernorm_bwd(xd, wd, g, st, st + rows, dx ? dx->dev : NULL, dw ? dw->dev : NULL,
+                           db ? db->dev : NULL, rows, cols, NULL) != 0) {
+        tt_release(dx);
+        tt_release(dw);
+        tt_release(db);
+        return;
+    }
+    accum_move(x, dx);
+    accum_move(w, dw);
+    accum_move(b, db);
+}
+
+static void backward_rope(AGNode *n) {
+    AGNode *x = n->in[0];
+    const struct RopeState *s = n->at.rope.s;
+    const float *g = needs(x) ? tt_dev(n->grad) : NULL;
+    Tensor *t = g ? tt_empty_like(x->val) : NULL;
+    if (!t) return;
+    if (tt_k_rope(&s->r, g, t->dev, s->positions, s->rows, s->seq_len, s->heads, 0, 0, 1) != 0) {
+        tt_release(t);
+        return;
+    }
+    accum_move(x, t);
+}
+
+static void backward_attention(AGNode *n) {
+    AGNode *q = n->in[0], *k = n->in[1], *v = n->in[2];
+    const struct AttnState *s = n->at.attn.s;
+    if (!s->lse) return;
+    const float *g = tt_dev(n->grad), *qd = tt_dev(q->val), *kd = tt_dev(k->val),
+                *vd = tt_dev(v->val), *o = tt_dev(n->val), *l = tt_dev(s->lse);
+    if (!g || !qd || !kd || !vd || !o || !l) return;
+    const int kv = needs(k) || needs(v);
+    Tensor *dq = needs(q) ? tt_empty_like(q->val) : NULL;
+    Tensor *dk = kv ? tt_empty_like(k->val) : NULL, *dv = kv ? tt_empty_like(v->val) : NULL;
+    if ((needs(q) && !dq) || (kv && (!dk || !dv)) ||
+        tt_k_attention_bwd(&s->a, qd, kd, vd, o, g, l, dq ? dq->dev : NULL, dk ? dk->dev : NULL,
+                           dv ? dv->dev : NULL, NULL) != 0) {
+        tt_release(dq);
+        tt_release(dk);
+        tt_release(dv);
+        return;
+    }
+    accum_move(q, dq);
+    accum_move(k, dk);
+    accum_move(v, dv);
 }
 
 /* ---------- scheduling and running the backward pass ---------- */

@@ -8,7 +8,8 @@
 // fresh NumPy copies of the device data, as the reference's do; with
 // copy=False they return a view of the pinned host mirror instead.
 // detach() re-enters a device-resident parameter into a new graph.  Additions of this backend:
-// softmax_ce(labels), probs(), backward_device(seed_node), sgd_step(lr), the
+// softmax_ce(labels), probs(), layernorm(w, b), rope(heads, head_dim, ...), attention(k, v, ...),
+// distill(ids, teacher), backward_device(seed_node), sgd_step(lr), the
 // Optim class (SGD-momentum, Adam), the Dataset class (device-resident
 // MNIST / CIFAR-10) and the module function available().
 #include <pybind11/numpy.h>
@@ -29,6 +30,7 @@ namespace py = pybind11;
 namespace {
 
 using Arr = py::array_t<float, py::array::c_style | py::array::forcecast>;
+using IntArr = py::array_t<int32_t, py::array::c_style | py::array::forcecast>;
 
 struct NodeRef {
   AGNode *p;
@@ -140,6 +142,55 @@ class PyNode {
   PyNode softmax_ce(py::array_t<int, py::array::c_style | py::array::forcecast> labels) {
     return PyNode(ag_softmax_ce(get(), labels.data(), (long)labels.size()));
   }
+  static AGNode *opt(const py::object &o) { return o.is_none() ? nullptr : o.cast<PyNode &>().get(); }
+  PyNode layernorm(py::object w, py::object b, float eps) {
+    return PyNode(ag_layernorm(get(), opt(w), opt(b), eps));
+  }
+  PyNode rope(int heads, int head_dim, py::object positions, long seq_len, py::object rot_dim, bool interleaved,
+              double base, int scaling, double factor, double trained, double low, double high,
+              double magnitude) {
+    const TTRope r = {head_dim, rot_dim.is_none() ? head_dim : rot_dim.cast<int>(), interleaved, scaling, base,
+                      factor, trained, low, high, magnitude};
+    if (positions.is_none()) return PyNode(ag_rope(get(), &r, heads, nullptr, seq_len));
+    auto p = positions.cast<IntArr>();
+    if (heads <= 0 || head_dim <= 0 || (long)p.size() * heads * head_dim != tt_numel(ag_value(get())))
+      throw py::value_error("tinytorch: rope needs a position for each row");
+    return PyNode(ag_rope(get(), &r, heads, p.data(), seq_len));
+  }
+  PyNode attention(const PyNode &k, const PyNode &v, long batch, int q_heads, int kv_heads, int head_dim,
+                   bool causal, long window, float scale, py::object q_start, py::object q_len,
+                   py::object k_len) {
+    if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) bad();
+    TTAttention a = {};
+    a.batch = batch;
+    a.q_rows = tt_numel(ag_value(get())) / ((long)q_heads * head_dim) / batch;
+    a.k_rows = tt_numel(ag_value(k.get())) / ((long)kv_heads * head_dim) / batch;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.causal = causal;
+    a.window = window;
+    a.scale = scale;
+    IntArr held[3];
+    const py::object *given[3] = {&q_start, &q_len, &k_len};
+    const int32_t **to[3] = {&a.q_start, &a.q_len, &a.k_len};
+    for (int i = 0; i < 3; i++) {
+      if (given[i]->is_none()) continue;
+      held[i] = given[i]->cast<IntArr>();
+      if ((long)held[i].size() != batch)
+        throw py::value_error("tinytorch: attention lengths need a value for each sequence");
+      *to[i] = held[i].data();
+    }
+    return PyNode(ag_attention(get(), k.get(), v.get(), &a));
+  }
+  PyNode distill(IntArr ids, Arr teacher, float temperature) {
+    Tensor *v = ag_value(get());
+    if (ids.ndim() != 2 || teacher.ndim() != 2 || ids.shape(0) != teacher.shape(0) ||
+        ids.shape(1) != teacher.shape(1) || ids.shape(1) > TT_DISTILL_MAX_TOP || tt_ndim(v) != 2 ||
+        v->shape[0] != (long)ids.shape(0))
+      throw py::value_error("tinytorch: distill needs ids and teacher logits of rows x top");
+    return PyNode(ag_distill(get(), ids.data(), teacher.data(), (int)ids.shape(1), temperature));
+  }
   py::object probs() const {
     Tensor *p = ag_softmax_ce_probs(get());
     if (!p) return py::none();
@@ -247,6 +298,17 @@ PYBIND11_MODULE(tinytorch_pybind, m) {
       .def("avgpool2d", &PyNode::avgpool2d, py::arg("pool_h") = 2, py::arg("pool_w") = 2,
            py::arg("stride_h") = 2, py::arg("stride_w") = 2)
       .def("softmax_ce", &PyNode::softmax_ce, py::arg("labels"))
+      .def("layernorm", &PyNode::layernorm, py::arg("w") = py::none(), py::arg("b") = py::none(),
+           py::arg("eps") = 1e-5f)
+      .def("rope", &PyNode::rope, py::arg("heads"), py::arg("head_dim"), py::arg("positions") = py::none(),
+           py::arg("seq_len") = 0, py::arg("rot_dim") = py::none(), py::arg("interleaved") = false,
+           py::arg("base") = 10000.0, py::arg("scaling") = 0, py::arg("factor") = 1.0,
+           py::arg("trained") = 0.0, py::arg("low") = 0.0, py::arg("high") = 0.0, py::arg("magnitude") = 1.0)
+      .def("attention", &PyNode::attention, py::arg("k"), py::arg("v"), py::arg("batch"), py::arg("q_heads"),
+           py::arg("kv_heads"), py::arg("head_dim"), py::arg("causal") = false, py::arg("window") = 0,
+           py::arg("scale") = 0.0f, py::arg("q_start") = py::none(), py::arg("q_len") = py::none(),
+           py::arg("k_len") = py::none())
+      .def("distill", &PyNode::distill, py::arg("ids"), py::arg("teacher"), py::arg("temperature") = 1.0f)
       .def("probs", &PyNode::probs)
       .def("sgd_step", &PyNode::sgd_step, py::arg("lr"))
       .def("__add__", &PyNode::add)

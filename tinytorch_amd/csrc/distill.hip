@@ -1,0 +1,257 @@
+// Distillation from a teacher's top logits: loss and gradient of a row of
+// student logits in one pass (HBM roofline: logits read, gradient written).
+//
+//   p = softmax over the row's `top` entries of teacher / T,
+//   q = softmax over all columns of logits / T,
+//   rowloss = T^2 sum_e p_e (log p_e - log q[ids_e]),
+//   dlogits = scale T (q - sum of the p_e at their columns).
+//
+// A workgroup holds a row in registers: its maximum, the exponentials and
+// their sum, and the gradient come from one read.  The entries (a wave's work)
+// are done while the row is on its way; their columns are written once more
+// behind the row.  Maxima, sums and exponentials are fp32.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include "tt_rt.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
+inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
+inline bool a16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct Max {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Add {
+  __device__ float operator()(float a, float b) const { return a + b; }
+};
+
+template <class OP>
+__device__ __forceinline__ float wave_all(float x, OP op) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x = op(x, __shfl_xor(x, s));
+  return x;
+}
+
+template <int NT, class OP>
+__device__ __forceinline__ float group_all(float x, float *part, OP op) {
+  x = wave_all(x, op);
+  if (NT == 64) return x;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = part[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; w++) x = op(x, part[w]);
+  return x;
+}
+
+struct Call {
+  const float *z;
+  const int32_t *ids;
+  const float *teacher;
+  float *rowloss, *dz;
+  long rows;
+  int cols, top;
+  float c;     // log2(e) / T
+  float t2;    // T^2
+  float coef;  // scale T
+};
+
+struct Entries {
+  int id[TT_DISTILL_MAX_TOP];   // -1: none
+  float p[TT_DISTILL_MAX_TOP];  // the teacher's logit, then log2 of the probability
+  float mass;                   // 1, or 0 for a row without entries
+};
+
+// wave 0: the row's entries to LDS as probabilities
+__device__ __forceinline__ void read_entries(const Call &a, long row, Entries &e, int lane) {
+  float most = -INFINITY;
+  for (int k = lane; k < a.top; k += 64) {
+    const int id = a.ids[row * a.top + k];
+    const bool ok = id >= 0 && id < a.cols;
+    const float t = ok ? a.teacher[row * a.top + k] : -INFINITY;
+    e.id[k] = ok ? id : -1;
+    e.p[k] = t;
+    most = t != t || most != most ? NAN : fmaxf(most, t);  // a NaN is the row's
+  }
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const float o = __shfl_xor(most, s);
+    most = most != most || o != o ? NAN : fmaxf(most, o);
+  }
+  const bool none = most == -INFINITY;
+  float sum = 0.f;
+  // differences before the factor and the logarithm: next to the type's lowest
+  // values either would be lost
+  for (int k = lane; k < a.top; k += 64) {
+    e.p[k] = none ? -INFINITY : (e.p[k] - most) * a.c;
+    sum += exp2_fast(e.p[k]);
+  }
+  sum = wave_all(sum, Add());
+  const float off = none ? 0.f : log2f(sum);
+  for (int k = lane; k < a.top; k += 64) e.p[k] -= off;
+  if (lane == 0) e.mass = none ? 0.f : 1.f;
+}
+
+// wave 0: the loss, and the gradient at the entries' columns
+__device__ __forceinline__ void finish(const Call &a, long row, const Entries &e, float most, bool flat,
+                                       float lse2, int lane, bool gradient) {
+  float loss = 0.f;
+  for (int k = lane; k < a.top; k += 64) {
+    const int id = e.id[k];
+    const float lp = e.p[k];
+    if (id < 0) continue;
+    const float lq = (flat ? 0.f : (a.z[row * a.cols + id] - most) * a.c) - lse2;
+    const float p = exp2_fast(lp);
+    if (p != 0.f) loss = fmaf(p, (lp - lq) * LN2, loss);
+    if (!gradient) continue;
+    // entries of one column: the first writes the sum of all
+    float sum = p;
+    bool first = true;
+    for (int o = 0; o < a.top; o++)
+      if (o != k && e.id[o] == id) {
+        if (o < k) first = false;
+        else sum += exp2_fast(e.p[o]);
+      }
+    if (first) a.dz[row * a.cols + id] = a.coef * (exp2_fast(lq) * e.mass - sum);
+  }
+  loss = wave_all(loss, Add());
+  if (lane == 0) a.rowloss[row] = e.mass == 0.f ? 0.f : loss * a.t2;
+}
+
+// a row of up to 4 NT NV columns
+template <int NT, int NV, bool VEC>
+__global__ void __launch_bounds__(NT) distill_kernel(Call a) {
+  __shared__ float part[NT / 64];
+  __shared__ Entries e;
+  const int t = threadIdx.x;
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float *z = a.z + row * a.cols;
+    f32x4 v[NV];
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      v[n] = (f32x4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (VEC) {
+        const int c = (n * NT + t) * 4;
+        if (c < a.cols) v[n] = *(const f32x4 *)(z + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int c = (n * 4 + j) * NT + t;
+          if (c < a.cols) v[n][j] = z[c];
+        }
+      }
+    }
+    if (t < 64) read_entries(a, row, e, t);
+    float most = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NV; n++) most = fmaxf(most, fmaxf(fmaxf(v[n][0], v[n][1]), fmaxf(v[n][2], v[n][3])));
+    most = group_all<NT>(most, part, Max());
+    const bool flat = most == -INFINITY;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = VEC ? (n * NT + t) * 4 + j : (n * 4 + j) * NT + t;
+        float x = flat ? 1.f : exp2_fast((v[n][j] - most) * a.c);
+        if (c >= a.cols) x = 0.f;
+        v[n][j] = x;
+        sum += x;
+      }
+    sum = group_all<NT>(sum, part, Add());
+    const float lse2 = log2f(sum);
+    if (a.dz) {
+      const float f = e.mass * a.coef / sum;
+      float *dz = a.dz + row * a.cols;
+#pragma unroll
+      for (int n = 0; n < NV; n++) {
+        v[n] *= f;
+        if (VEC) {
+          const int c = (n * NT + t) * 4;
+          if (c < a.cols) *(f32x4 *)(dz + c) = v[n];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int c = (n * 4 + j) * NT + t;
+            if (c < a.cols) dz[c] = v[n][j];
+          }
+        }
+      }
+    }
+    __syncthreads();  // the row is written: its entries' columns may be
+    if (t < 64) finish(a, row, e, most, flat, lse2, t, a.dz != NULL);
+    __syncthreads();  // the entries are read
+  }
+}
+
+// longer rows: maximum and sum in a first pass, the gradient in a second
+__global__ void __launch_bounds__(1024) distill_long_kernel(Call a) {
+  __shared__ float part[16];
+  __shared__ Entries e;
+  const int t = threadIdx.x;
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float *z = a.z + row * a.cols;
+    if (t < 64) read_entries(a, row, e, t);
+    float most = -INFINITY;
+    for (long c = t; c < a.cols; c += 1024) most = fmaxf(most, z[c]);
+    most = group_all<1024>(most, part, Max());
+    const bool flat = most == -INFINITY;
+    float sum = 0.f;
+    for (long c = t; c < a.cols; c += 1024) sum += flat ? 1.f : exp2_fast((z[c] - most) * a.c);
+    sum = group_all<1024>(sum, part, Add());
+    if (a.dz) {
+      const float f = e.mass * a.coef / sum;
+      for (long c = t; c < a.cols; c += 1024)
+        a.dz[row * a.cols + c] = (flat ? 1.f : exp2_fast((z[c] - most) * a.c)) * f;
+    }
+    __syncthreads();
+    if (t < 64) finish(a, row, e, most, flat, log2f(sum), t, a.dz != NULL);
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float *teacher, int top,
+                            float temperature, float *rowloss, float *dlogits, long rows, int cols, float scale) {
+  if (!logits || !ids || !teacher || !rowloss || rows <= 0 || cols <= 0 || top <= 0 || top > TT_DISTILL_MAX_TOP ||
+      !(temperature > 0.f) || isinf(temperature) || !(scale == scale) || isinf(scale) || rows > (1L << 40) / cols ||
+      dlogits == logits)
+    return -1;
+  if (ttrt_init() != 0) return -3;
+  const Call a = {logits, ids, teacher, rowloss, dlogits, rows, cols, top, LOG2E / temperature,
+                  temperature * temperature, scale * temperature};
+  const bool vec = cols % 4 == 0 && a16(logits) && a16(dlogits);
+  const dim3 grid((unsigned)(rows < 1 << 20 ? rows : 1 << 20));
+#define RUN(NT, NV)                                                                          \
+  if (vec)                                                                                   \
+    hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a);      \
+  else                                                                                       \
+    hipLaunchKernelGGL((distill_kernel<NT, NV, false>), grid, dim3(NT), 0, stream(), a)
+  if (cols <= 1024) {
+    RUN(256, 1);
+  } else if (cols <= 4096) {
+    RUN(256, 4);
+  } else if (cols <= 16384) {
+    RUN(1024, 4);
+  } else if (cols <= 32768) {
+    RUN(1024, 8);
+  } else if (cols <= 65536) {
+    RUN(1024, 16);
+  } else {
+    hipLaunchKernelGGL(distill_long_kernel, grid, dim3(1024), 0, stream(), a);
+  }
+#undef RUN
+  return launched();
+}

@@ -11,7 +11,7 @@ import ctypes
 
 import numpy as np
 
-from . import F32P, lib
+from . import F32P, Attention, Rope, lib
 
 LIB = lib()
 
@@ -142,6 +142,50 @@ class Node:
         lab = np.ascontiguousarray(labels, dtype=np.int32)
         return Node(_checked(LIB.ag_softmax_ce(self.ptr, lab.ctypes.data_as(
             ctypes.POINTER(ctypes.c_int)), lab.size), "ag_softmax_ce"))
+
+    def layernorm(self, w=None, b=None, eps=1e-5):
+        """Layer norm over the last axis, times w plus b."""
+        return Node(_checked(LIB.ag_layernorm(self.ptr, w.ptr if w else None, b.ptr if b else None, eps),
+                             "ag_layernorm"))
+
+    def rope(self, heads, head_dim, positions=None, seq_len=0, rot_dim=None, interleaved=False, base=10000.0,
+             scaling=0, factor=1.0, trained=0.0, low=0.0, high=0.0, magnitude=1.0):
+        """Rotary positions: `positions` an int a row, or row % seq_len."""
+        r = Rope(head_dim, head_dim if rot_dim is None else rot_dim, int(interleaved), scaling, base, factor,
+                 trained, low, high, magnitude)
+        pos = None if positions is None else np.ascontiguousarray(positions, dtype=np.int32)
+        if pos is not None and pos.size * heads * head_dim != LIB.tt_numel(LIB.ag_value(self.ptr)):
+            raise ValueError("tinytorch: rope needs a position for each row")
+        return Node(_checked(LIB.ag_rope(self.ptr, r, heads, None if pos is None else pos.ctypes.data, seq_len),
+                             "ag_rope"))
+
+    def attention(self, k, v, batch, q_heads, kv_heads, head_dim, causal=False, window=0, scale=0.0,
+                  q_start=None, q_len=None, k_len=None):
+        """Attention of these queries over k and v, rows by sequence; the
+        length arrays hold an int a sequence."""
+        rows = [int(LIB.tt_numel(LIB.ag_value(n.ptr))) // max(1, batch * h * head_dim)
+                for n, h in ((self, q_heads), (k, kv_heads))]
+        a = Attention(batch=batch, q_rows=rows[0], k_rows=rows[1], q_heads=q_heads, kv_heads=kv_heads,
+                      head_dim=head_dim, causal=int(causal), window=window, scale=scale)
+        held = []
+        for name, x in (("q_start", q_start), ("q_len", q_len), ("k_len", k_len)):
+            if x is None:
+                continue
+            held.append(np.ascontiguousarray(x, dtype=np.int32))
+            if held[-1].size != batch:
+                raise ValueError(f"tinytorch: {name} needs a value for each sequence")
+            setattr(a, name, held[-1].ctypes.data)
+        return Node(_checked(LIB.ag_attention(self.ptr, k.ptr, v.ptr, a), "ag_attention"))
+
+    def distill(self, ids, teacher, temperature=1.0):
+        """Mean distillation loss against a teacher's top logits (rows x top)."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        teacher = np.ascontiguousarray(teacher, dtype=np.float32)
+        rows = Tensor(LIB.ag_value(self.ptr), owned=False).shape()[0]
+        if ids.ndim != 2 or ids.shape != teacher.shape or ids.shape[0] != rows:
+            raise ValueError("tinytorch: distill needs ids and teacher logits of rows x top")
+        return Node(_checked(LIB.ag_distill(self.ptr, ids.ctypes.data, teacher.ctypes.data, ids.shape[1],
+                                            temperature), "ag_distill"))
 
     def probs(self):
         p = LIB.ag_softmax_ce_probs(self.ptr)
