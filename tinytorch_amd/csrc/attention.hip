@@ -42,6 +42,9 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 constexpr int KT = 32;  // rows of the streamed operand a tile
+// waves a SIMD that the registers are held to: as many as do without spilling
+#define FWD_WAVES(DB) ((DB) <= 5 ? 4 : 3)
+#define DQ_WAVES(DB) ((DB) <= 4 ? 4 : (DB) <= 6 ? 3 : 2)
 
 struct Strides {
   long b, r, h;  // elements from a sequence / row / head to the next
@@ -167,52 +170,90 @@ __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Operands go from LDS to registers one step ahead of the products that use
+// them, and no further: left alone, the compiler moves every read of an
+// unrolled loop to its front and runs out of registers.
+__device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
+
+// s[n] += the tile's rows 16 n + lane % 16 times b, over DB blocks of 16 columns
+template <int DB>
+__device__ __forceinline__ void dots(f32x4 (&s)[2], const f32x4 (&b)[DB], const float *x, int ld, int lane) {
+  const float *p = x + (lane & 15) * ld + 4 * (lane >> 4);
+  f32x4 cur[2], nxt[2];
+  cur[0] = *(const f32x4 *)p;
+  cur[1] = *(const f32x4 *)(p + 16 * ld);
+#pragma unroll
+  for (int u = 0; u < DB; u++) {
+    if (u + 1 < DB) {
+      nxt[0] = *(const f32x4 *)(p + 16 * (u + 1));
+      nxt[1] = *(const f32x4 *)(p + 16 * ld + 16 * (u + 1));
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      s[0] = mfma(cur[0][c], b[u][c], s[0]);
+      s[1] = mfma(cur[1][c], b[u][c], s[1]);
+    }
+    step_end();
+    cur[0] = nxt[0];
+    cur[1] = nxt[1];
+  }
+}
+
 // acc (columns d of row l % 16) += sum over the tile's rows k of w[k][l % 16] x[k][d]
 template <int DB, int NB>
 __device__ __forceinline__ void product(f32x4 (&acc)[DB], const f32x4 (&w)[NB], const float *x, int ld,
                                         int lane) {
   constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
   typedef typename Vec<VW>::T V;
-  const int g = lane >> 4, m = lane & 15;
+  const float *p = x + 4 * (lane >> 4) * ld + VW * (lane & 15);
+  V cur[T], nxt[T];
 #pragma unroll
-  for (int kb = 0; kb < NB; kb++)
+  for (int t = 0; t < T; t++) cur[t] = *(const V *)(p + 16 * VW * t);
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const float *row = x + (kb * 16 + 4 * g + r) * ld + VW * m;
+  for (int k = 0; k < 4 * NB; k++) {
+    if (k + 1 < 4 * NB) {
 #pragma unroll
-      for (int t = 0; t < T; t++) {
-        const V v = *(const V *)(row + 16 * VW * t);
-#pragma unroll
-        for (int c = 0; c < VW; c++) acc[t * VW + c] = mfma(Vec<VW>::at(v, c), w[kb][r], acc[t * VW + c]);
-      }
+      for (int t = 0; t < T; t++)
+        nxt[t] = *(const V *)(p + ((k + 1) / 4 * 16 + (k + 1) % 4) * ld + 16 * VW * t);
     }
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+      for (int c = 0; c < VW; c++)
+        acc[t * VW + c] = mfma(Vec<VW>::at(cur[t], c), w[k / 4][k % 4], acc[t * VW + c]);
+    step_end();
+#pragma unroll
+    for (int t = 0; t < T; t++) cur[t] = nxt[t];
+  }
 }
 
-// the same one row at a time, leaving out what `seen(k)` does not admit to
-// this lane's column: for tiles that hold infinities or NaN where a mask hides
-// them from some of the columns (0 * inf would reach those)
-template <int DB, int NB, class SEEN>
-__device__ __forceinline__ void product_masked(f32x4 (&acc)[DB], const f32x4 (&w)[NB], const float *x, int ld,
-                                            int lane, SEEN seen) {
-  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
-  const int g = lane >> 4, m = lane & 15;
+// One query (or key) at a time, its values over the lanes (two each): what a
+// workgroup falls back to when a tile holds an infinity or NaN that a mask
+// hides from some of its columns (in the matrix units 0 * inf would reach
+// them).  Nothing hidden is read here.  Rare, so small rather than fast: kept
+// apart from the loops that run, whose registers it must not take.
+struct Pair {
+  float x, y;
+};
+__device__ __forceinline__ Pair load2(const float *p, int D, int lane) {
+  Pair r = {0.f, 0.f};
+  if (lane < D) r.x = p[lane];
+  if (lane + 64 < D) r.y = p[lane + 64];
+  return r;
+}
+__device__ __forceinline__ void store2(float *p, Pair v, float f, int D, int lane) {
+  if (lane < D) p[lane] = v.x * f;
+  if (lane + 64 < D) p[lane + 64] = v.y * f;
+}
+__device__ __forceinline__ float dot2(Pair a, Pair b) {
+  float s = fmaf(a.x, b.x, a.y * b.y);
 #pragma unroll
-  for (int kb = 0; kb < NB; kb++)
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll 1
-      for (int kg = 0; kg < 4; kg++) {
-        const int k = kb * 16 + 4 * kg + r;
-        const float p = __shfl(w[kb][r], m + 16 * kg);
-        if (!seen(k)) continue;
-#pragma unroll
-        for (int t = 0; t < T; t++)
-#pragma unroll
-          for (int c = 0; c < VW; c++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              acc[t * VW + c][e] = fmaf(p, x[k * ld + 16 * VW * t + VW * (4 * g + e) + c], acc[t * VW + c][e]);
-      }
+  for (int n = 1; n < 64; n <<= 1) s += __shfl_xor(s, n);
+  return s;
+}
+__device__ __forceinline__ void add2(Pair &a, float f, Pair b) {
+  a.x = fmaf(f, b.x, a.x);
+  a.y = fmaf(f, b.y, a.y);
 }
 
 // row p[0 .. D) = f * the columns d that acc holds of this lane's row
@@ -300,168 +341,160 @@ __device__ __forceinline__ float col_sum(float x) {
 
 // ---------------------------------------------------------------- forward
 
-// One workgroup: 64 QB packed rows (16 QB a wave) of one key head against the
-// keys they see, KT at a time through LDS.  With splits > 1 it takes `chunk`
-// keys of them and leaves maximum, sum and the unscaled result to the join.
-template <int DB, int QB>
-__global__ void __launch_bounds__(256, 2)
+// 16 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
+__device__ __forceinline__ void fwd_one_by_one(const Args &a, int b, int h, int first, int r1, int k0, int k1,
+                                               const float *q, const float *k, const float *v, float *o, float *lse,
+                                               float *ws_ml, float *ws_o, int width, int lane) {
+#pragma unroll 1
+  for (int row = first; row < first + 16 && row < r1; row++) {
+    const int i = row / a.G, hm = row - i * a.G;
+    Range rg = range_of(a, b, i);
+    if (rg.lo < k0) rg.lo = k0;
+    if (rg.hi > k1) rg.hi = k1;
+    Pair qv = load2(q + (long)i * a.q.r + (long)hm * a.q.h, a.D, lane), acc = {0.f, 0.f};
+    qv.x *= a.scale * LOG2E;
+    qv.y *= a.scale * LOG2E;
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int j = rg.lo; j < rg.hi; j++) {
+      const float s = dot2(qv, load2(k + (long)j * a.k.r, a.D, lane)), t = fmaxf(s, mx);
+      const float base = t == -INFINITY ? 0.f : t, f = exp2_fast(mx - base), p = exp2_fast(s - base);
+      mx = t;
+      sum = fmaf(sum, f, p);
+      acc.x *= f;
+      acc.y *= f;
+      add2(acc, p, load2(v + (long)j * a.v.r, a.D, lane));
+    }
+    const int hq = h * a.G + hm;
+    if (a.splits > 1) {
+      const long at = ((long)blockIdx.y * a.B * a.Hkv + (long)b * a.Hkv + h) * a.R + row;
+      if (lane == 0) {
+        ws_ml[2 * at] = mx;
+        ws_ml[2 * at + 1] = sum;
+      }
+      store2(ws_o + at * width, acc, 1.f, a.D, lane);
+      continue;
+    }
+    if (lse && lane == 0)
+      lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * LN2;
+    store2(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc, sum == 0.f ? 0.f : 1.f / sum, a.D, lane);
+  }
+}
+
+// One workgroup of NW waves: 16 NW packed rows (16 a wave) of one key head
+// against the keys they see, KT at a time through LDS: a tile is loaded to
+// registers while the one before it is used, and goes to the other half of the
+// LDS behind that (one barrier a tile).  With splits > 1 it takes `chunk` keys
+// of them and leaves maximum, sum and the unscaled result to the join.
+template <int DB, int NW>
+__global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
-  typedef Stage<DB, 256> S;
-  __shared__ __attribute__((aligned(16))) float lk[KT * S::LD], lv[KT * S::LD];
-  constexpr int ROWS = 64 * QB;
+  typedef Stage<DB, 64 * NW> S;
+  __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
+  constexpr int ROWS = 16 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   // the last rows see the most keys under a causal mask: they start first
   const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
   const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
-  Span sp = span_of(a, b, r0, r1);
+  const Span sp = span_of(a, b, r0, r1);
   int k_first = sp.lo / KT * KT, k_end = sp.hi;
   if (a.splits > 1) {
     const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
     if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
     if (c1 < k_end) k_end = (int)c1;
   }
-
-  f32x4 qf[QB][DB], acc[QB][DB];
-  float mx[QB], sum[QB];
-  int lo[QB], hi[QB], row[QB];
-  const float *qb_base = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
+  const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
+  const bool in = row < a.R;
+  Range rg = {0, 0};
+  if (in) rg = range_of(a, b, i);
+  f32x4 qf[DB], acc[DB];
+  float mx = -INFINITY, sum = 0.f;
+  const float *qp0 = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
+  const float *qp = qp0 + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h;
 #pragma unroll
-  for (int n = 0; n < QB; n++) {
-    row[n] = r0 + (wave * QB + n) * 16 + m;
-    const int i = row[n] / a.G;
-    const bool in = row[n] < a.R;
-    Range rg = {0, 0};
-    if (in) rg = range_of(a, b, i);
-    lo[n] = rg.lo;
-    hi[n] = rg.hi;
-    mx[n] = -INFINITY;
-    sum[n] = 0.f;
-    const float *p = qb_base + (long)i * a.q.r + (long)(row[n] - i * a.G) * a.q.h;
-    const float f = a.scale * LOG2E;
-#pragma unroll
-    for (int u = 0; u < DB; u++) {
-      qf[n][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      acc[n][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (in) qf[n][u] = load4(p, 16 * u + 4 * g, a.D, a.vec) * f;
-    }
+  for (int u = 0; u < DB; u++) {
+    qf[u] = acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (in) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
   }
-
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
   S sk, sv;
+  bool odd = false;
   if (k_first < k_end) {
     sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
     sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+    sk.store(lk[0], tid);
+    sv.store(lv[0], tid);
+    odd = __syncthreads_or(sv.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
   }
-  for (int k0 = k_first; k0 < k_end; k0 += KT) {
-    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi;
-    sk.store(lk, tid);
-    sv.store(lv, tid);
-    bool odd = false;
-    if (mixed)
-      odd = __syncthreads_or(sv.odd());
-    else
-      __syncthreads();
-    if (k0 + KT < k_end) {
+  int buf = 0;
+  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
+    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
+    if (odd) break;
+    if (more) {
       sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
       sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
     }
-    f32x4 s[QB][2];
-#pragma unroll
-    for (int n = 0; n < QB; n++)
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++) s[n][kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < DB; u++)
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++) {
-        const f32x4 ka = *(const f32x4 *)(lk + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int n = 0; n < QB; n++) s[n][kb] = mfma(ka[c], qf[n][u][c], s[n][kb]);
-      }
-#pragma unroll
-    for (int n = 0; n < QB; n++) {
-      if (mixed) {
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int key = k0 + kb * 16 + 4 * g + r;
-            if (key < lo[n] || key >= hi[n]) s[n][kb][r] = -INFINITY;
-          }
-      }
-      float t = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) t = fmaxf(t, s[n][kb][r]);
-      t = fmaxf(col_max(t), mx[n]);
-      const float base = t == -INFINITY ? 0.f : t;
-      if (__any(t > mx[n])) {
-        const float f = exp2_fast(mx[n] - base);
-        sum[n] *= f;
-#pragma unroll
-        for (int u = 0; u < DB; u++) acc[n][u] *= f;
-      }
-      mx[n] = t;
+    f32x4 s[2];
+    s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    dots<DB>(s, qf, lk[buf], S::LD, lane);
+    if (mixed) {
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          s[n][kb][r] = exp2_fast(s[n][kb][r] - base);
-          sum[n] += s[n][kb][r];
+          const int key = k0 + kb * 16 + 4 * g + r;
+          if (key < rg.lo || key >= rg.hi) s[kb][r] = -INFINITY;
         }
     }
-    if (odd) {
+    float t = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    t = fmaxf(col_max(t), mx);
+    const float base = t == -INFINITY ? 0.f : t;
+    if (__any(t > mx)) {
+      const float f = exp2_fast(mx - base);
+      sum *= f;
 #pragma unroll
-      for (int n = 0; n < QB; n++)
-        product_masked<DB, 2>(acc[n], s[n], lv, S::LD, lane,
-                              [&](int kk) { return k0 + kk >= lo[n] && k0 + kk < hi[n]; });
-    } else {
-      constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
-      typedef typename Vec<VW>::T V;
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float *x = lv + (kb * 16 + 4 * g + r) * S::LD + VW * m;
-#pragma unroll
-          for (int t = 0; t < T; t++) {
-            const V va = *(const V *)(x + 16 * VW * t);
-#pragma unroll
-            for (int c = 0; c < VW; c++)
-#pragma unroll
-              for (int n = 0; n < QB; n++)
-                acc[n][t * VW + c] = mfma(Vec<VW>::at(va, c), s[n][kb][r], acc[n][t * VW + c]);
-          }
-        }
+      for (int u = 0; u < DB; u++) acc[u] *= f;
+      mx = t;
     }
-    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[kb][r] = exp2_fast(s[kb][r] - base);
+    sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+    product<DB, 2>(acc, s, lv[buf], S::LD, lane);
+    if (more) {
+      sk.store(lk[buf ^ 1], tid);
+      sv.store(lv[buf ^ 1], tid);
+      if (k0 + KT < sp.ilo || k0 + 2 * KT > sp.ihi)
+        odd = __syncthreads_or(sv.odd());
+      else
+        __syncthreads();
+    }
+  }
+  if (odd) {
+    fwd_one_by_one(a, b, h, r0 + wave * 16, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, DB * 16, lane);
+    return;
   }
 
-#pragma unroll
-  for (int n = 0; n < QB; n++) {
-    const float total = col_sum(sum[n]);
-    if (row[n] >= a.R) continue;
-    const int i = row[n] / a.G, hq = h * a.G + row[n] - i * a.G;
-    if (a.splits > 1) {
-      const long at = ((long)blockIdx.y * nbh + bh) * a.R + row[n];
-      if (g == 0) {
-        ws_ml[2 * at] = mx[n];
-        ws_ml[2 * at + 1] = total;
-      }
-      store_row<DB>(ws_o + at * (DB * 16), acc[n], 1.f, DB * 16, 1, lane);
-      continue;
+  const float total = col_sum(sum);
+  if (!in) return;
+  if (a.splits > 1) {
+    const long at = ((long)blockIdx.y * nbh + bh) * a.R + row;
+    if (g == 0) {
+      ws_ml[2 * at] = mx;
+      ws_ml[2 * at + 1] = total;
     }
-    if (lse && g == 0)
-      lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (mx[n] + log2f(total)) * LN2;
-    store_row<DB>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc[n],
-                  total == 0.f ? 0.f : 1.f / total, a.D, a.vec, lane);
+    store_row<DB>(ws_o + at * (DB * 16), acc, 1.f, DB * 16, 1, lane);
+    return;
   }
+  if (lse && g == 0)
+    lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (mx + log2f(total)) * LN2;
+  store_row<DB>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc, total == 0.f ? 0.f : 1.f / total,
+                a.D, a.vec, lane);
 }
 
 // Few packed rows (one tile of 16): the keys pass once, from memory to
@@ -585,24 +618,29 @@ __global__ void __launch_bounds__(256, 2)
     if (odd) {
       // as product_masked, the values from memory: rows behind the keys'
       // end are not seen and not read
+      float *mine = part[wave];
 #pragma unroll
-      for (int r = 0; r < 4; r++)
+      for (int r = 0; r < 4; r++) mine[(4 * g + r) * 16 + m] = s[r];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll 1
-        for (int kg = 0; kg < 4; kg++) {
-          const int key = k0 + 4 * kg + r;
-          const float p = __shfl(s[r], m + 16 * kg);
-          if (key < rg.lo || key >= rg.hi || key >= k_end) continue;
-          const float *x = vp + (long)key * a.v.r;
+      for (int kk = 0; kk < 16; kk++) {
+        const int key = k0 + kk;
+        if (key < rg.lo || key >= rg.hi || key >= k_end) continue;
+        const float p = mine[kk * 16 + m];
+        const float *x = vp + (long)key * a.v.r;
 #pragma unroll
-          for (int t2 = 0; t2 < T; t2++)
+        for (int t2 = 0; t2 < T; t2++)
 #pragma unroll
-            for (int c = 0; c < VW; c++)
+          for (int c = 0; c < VW; c++)
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const int d = 16 * VW * t2 + VW * (4 * g + e) + c;
-                if (d < a.D) acc[t2 * VW + c][e] = fmaf(p, x[d], acc[t2 * VW + c][e]);
-              }
-        }
+            for (int e = 0; e < 4; e++) {
+              const int d = 16 * VW * t2 + VW * (4 * g + e) + c;
+              if (d < a.D) acc[t2 * VW + c][e] = fmaf(p, x[d], acc[t2 * VW + c][e]);
+            }
+      }
+      __builtin_amdgcn_wave_barrier();
     } else {
 #pragma unroll
       for (int r = 0; r < 4; r++)
@@ -715,19 +753,49 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dq of 64 packed rows (16 a wave): keys and values through LDS as in the
+// dq of 16 packed rows from `first` on
+__device__ __forceinline__ void dq_one_by_one(const Args &a, int b, int h, int first, int r1, const float *q,
+                                              const float *k, const float *v, const float *dout, const float *lse,
+                                              const float *delta, float *dq, int lane) {
+#pragma unroll 1
+  for (int row = first; row < first + 16 && row < r1; row++) {
+    const int i = row / a.G, hq = h * a.G + row - i * a.G;
+    const Range rg = range_of(a, b, i);
+    Pair acc = {0.f, 0.f};
+    const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i, qo = (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h;
+    if (rg.lo < rg.hi) {
+      Pair qv = load2(q + qo, a.D, lane);
+      const Pair dv = load2(dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, a.D, lane);
+      qv.x *= a.scale * LOG2E;
+      qv.y *= a.scale * LOG2E;
+      float l2 = lse[at] * LOG2E;
+      if (l2 == -INFINITY) l2 = 0.f;
+      const float dl = delta[at];
+#pragma unroll 1
+      for (int j = rg.lo; j < rg.hi; j++) {
+        const Pair kv = load2(k + (long)j * a.k.r, a.D, lane);
+        const float p = exp2_fast(dot2(qv, kv) - l2);
+        add2(acc, p * (dot2(dv, load2(v + (long)j * a.v.r, a.D, lane)) - dl), kv);
+      }
+    }
+    store2(dq + qo, acc, a.scale, a.D, lane);
+  }
+}
+
+// dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
 // forward pass
-template <int DB>
-__global__ void __launch_bounds__(256, 2)
+template <int DB, int NW>
+__global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
     attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ dout, const float *__restrict__ lse,
                    const float *__restrict__ delta, float *__restrict__ dq) {
-  typedef Stage<DB, 256> S;
-  __shared__ __attribute__((aligned(16))) float lk[KT * S::LD], lv[KT * S::LD];
+  typedef Stage<DB, 64 * NW> S;
+  __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
+  constexpr int ROWS = 16 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
-  const int r0 = tile * 64, r1 = r0 + 64 < a.R ? r0 + 64 : a.R;
+  const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
   const Span sp = span_of(a, b, r0, r1);
   const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
@@ -754,38 +822,27 @@ __global__ void __launch_bounds__(256, 2)
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
   S sk, sv;
   const int k_first = sp.lo / KT * KT, k_end = sp.hi;
+  bool odd = false;
   if (k_first < k_end) {
     sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
     sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+    sk.store(lk[0], tid);
+    sv.store(lv[0], tid);
+    odd = __syncthreads_or(sk.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
   }
-  for (int k0 = k_first; k0 < k_end; k0 += KT) {
-    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi;
-    sk.store(lk, tid);
-    sv.store(lv, tid);
-    bool odd = false;
-    if (mixed)
-      odd = __syncthreads_or(sk.odd());
-    else
-      __syncthreads();
-    if (k0 + KT < k_end) {
+  int buf = 0;
+  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
+    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
+    if (odd) break;
+    if (more) {
       sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
       sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
     }
     f32x4 s[2], dp[2];
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) s[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < DB; u++)
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++) {
-        const f32x4 ka = *(const f32x4 *)(lk + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
-        const f32x4 va = *(const f32x4 *)(lv + (kb * 16 + m) * S::LD + 16 * u + 4 * g);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          s[kb] = mfma(ka[c], qf[u][c], s[kb]);
-          dp[kb] = mfma(va[c], df[u][c], dp[kb]);
-        }
-      }
+    dots<DB>(s, qf, lk[buf], S::LD, lane);
+    dots<DB>(dp, df, lv[buf], S::LD, lane);
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -794,44 +851,110 @@ __global__ void __launch_bounds__(256, 2)
         const float x = exp2_fast(s[kb][r] - l2) * (dp[kb][r] - dl);
         s[kb][r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
       }
-    if (odd)
-      product_masked<DB, 2>(acc, s, lk, S::LD, lane,
-                            [&](int kk) { return k0 + kk >= rg.lo && k0 + kk < rg.hi; });
-    else
-      product<DB, 2>(acc, s, lk, S::LD, lane);
-    __syncthreads();
+    product<DB, 2>(acc, s, lk[buf], S::LD, lane);
+    if (more) {
+      sk.store(lk[buf ^ 1], tid);
+      sv.store(lv[buf ^ 1], tid);
+      if (k0 + KT < sp.ilo || k0 + 2 * KT > sp.ihi)
+        odd = __syncthreads_or(sk.odd());
+      else
+        __syncthreads();
+    }
+  }
+  if (odd) {
+    dq_one_by_one(a, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
+    return;
   }
   if (in) store_row<DB>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
 }
 
-// dk and dv of 64 keys (16 a wave): the packed query rows that see any of
-// them through LDS, q and do
-template <int DB>
-__global__ void __launch_bounds__(256, 2)
-    attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
-                    const float *__restrict__ dout, const float *__restrict__ lse,
-                    const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv) {
-  typedef Stage<DB, 256> S;
-  __shared__ __attribute__((aligned(16))) float lq[KT * S::LD], ld[KT * S::LD], rl[KT], rd[KT];
-  __shared__ int rlo[KT], rhi[KT];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int k0 = blockIdx.x / nbh * 64, key = k0 + wave * 16 + m;
-  // the queries that see a key of [k0, k0 + 64)
+// the packed rows that see a key of [k0, k1)
+struct Rows {
+  int first, end;
+};
+__device__ __forceinline__ Rows rows_of(const Args &a, int b, int k0, int k1) {
   const long start = start_of(a, b);
-  const int keys = keys_of(a, b);
   long i0 = 0, i1 = queries_of(a, b);
   if (a.causal) {
     if (k0 - start > i0) i0 = k0 - start;
   } else if (a.window > 0 && k0 - a.window - start + 1 > i0) {
     i0 = k0 - a.window - start + 1;
   }
-  if (a.window > 0 && k0 + 64 + a.window - 1 - start < i1) i1 = k0 + 64 + a.window - 1 - start;
-  if (k0 >= keys || i0 > i1) i0 = i1 = 0;
-  if (i1 < i0) i1 = i0;
-  const int r_first = (int)i0 * a.G, r_end = (int)i1 * a.G;
+  if (a.window > 0 && k1 - 1 + a.window - start < i1) i1 = k1 - 1 + a.window - start;
+  Rows r = {0, 0};
+  if (k0 >= keys_of(a, b) || i0 >= i1) return r;
+  r.first = (int)i0 * a.G;
+  r.end = (int)i1 * a.G;
+  return r;
+}
 
-  const bool in = key < a.Lk, live = key < keys;
+// dk and dv of 16 keys from `first` on, from the packed rows [r0, r1)
+__device__ __forceinline__ void dkv_one_by_one(const Args &a, int b, int h, int first, int r0, int r1,
+                                               const float *q, const float *k, const float *v, const float *dout,
+                                               const float *lse, const float *delta, float *dk, float *dv, float *ws,
+                                               int width, int lane) {
+  const int keys = keys_of(a, b);
+#pragma unroll 1
+  for (int key = first; key < first + 16 && key < a.Lk; key++) {
+    Pair ak = {0.f, 0.f}, av = {0.f, 0.f};
+    const long ko = (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
+    const long vo = (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
+    if (key < keys) {
+      Pair kv = load2(k + ko, a.D, lane);
+      const Pair vv = load2(v + vo, a.D, lane);
+      kv.x *= a.scale * LOG2E;
+      kv.y *= a.scale * LOG2E;
+#pragma unroll 1
+      for (int row = r0; row < r1; row++) {
+        const int i = row / a.G, hq = h * a.G + row - i * a.G;
+        const Range rg = range_of(a, b, i);
+        if (key < rg.lo || key >= rg.hi) continue;
+        const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
+        float l2 = lse[at] * LOG2E;
+        if (l2 == -INFINITY) l2 = 0.f;
+        const Pair qv = load2(q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, a.D, lane);
+        const Pair dw = load2(dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, a.D, lane);
+        const float p = exp2_fast(dot2(qv, kv) - l2);
+        add2(av, p, dw);
+        add2(ak, p * (dot2(dw, vv) - delta[at]), qv);
+      }
+    }
+    if (a.splits > 1) {
+      const long nbh = (long)a.B * a.Hkv, at = ((long)blockIdx.y * nbh + (long)b * a.Hkv + h) * a.Lk + key;
+      store2(ws + at * width, ak, a.scale, a.D, lane);
+      store2(ws + ((long)a.splits * nbh * a.Lk + at) * width, av, 1.f, a.D, lane);
+    } else {
+      store2(dk + ko, ak, a.scale, a.D, lane);
+      store2(dv + vo, av, 1.f, a.D, lane);
+    }
+  }
+}
+
+// dk and dv of 16 NW keys (16 a wave): the packed query rows that see any of
+// them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of
+// the rows and leaves its sums to the join: where many rows meet few keys, and
+// so that no fp32 sum runs over more rows than that.
+template <int DB, int NW>
+__global__ void __launch_bounds__(64 * NW, 2)
+    attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                    const float *__restrict__ dout, const float *__restrict__ lse,
+                    const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
+                    float *__restrict__ ws) {
+  typedef Stage<DB, 64 * NW> S;
+  __shared__ __attribute__((aligned(16))) float lq[2][KT * S::LD], ld[2][KT * S::LD], rl[2][KT], rd[2][KT];
+  __shared__ int rlo[2][KT], rhi[2][KT];
+  constexpr int KEYS = 16 * NW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int k0 = blockIdx.x / nbh * KEYS, key = k0 + wave * 16 + m;
+  Rows rows = rows_of(a, b, k0, k0 + KEYS);
+  if (a.splits > 1) {
+    const long c0 = rows.first + (long)blockIdx.y * a.chunk;
+    if (c0 >= rows.end && blockIdx.y > 0) return;  // the join leaves it out
+    if (c0 + a.chunk < rows.end) rows.end = (int)c0 + a.chunk;
+    rows.first = (int)c0;
+  }
+  const bool in = key < a.Lk, live = key < keys_of(a, b);
   f32x4 kf[DB], vf[DB], ak[DB], av[DB];
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
   const float *vp = v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
@@ -846,82 +969,125 @@ __global__ void __launch_bounds__(256, 2)
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *dp_ = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
   S sq, sd;
-  if (r_first < r_end) {
-    sq.load_rows(qp, a.q.r, a.q.h, a.G, r_first, r_end, a.D, a.vec, tid);
-    sd.load_rows(dp_, a.o.r, a.o.h, a.G, r_first, r_end, a.D, a.vec, tid);
-  }
-  for (int r0 = r_first; r0 < r_end; r0 += KT) {
-    sq.store(lq, tid);
-    sd.store(ld, tid);
+  // row statistics of a tile, by the first KT threads
+  float l2_ = 0.f, dl_ = 0.f;
+  Range rg_ = {0, 0};
+  auto load = [&](int r0) {
+    sq.load_rows(qp, a.q.r, a.q.h, a.G, r0, rows.end, a.D, a.vec, tid);
+    sd.load_rows(dp_, a.o.r, a.o.h, a.G, r0, rows.end, a.D, a.vec, tid);
     if (tid < KT) {
       const int row = r0 + tid, i = row / a.G;
-      Range rg = {0, 0};
-      float l2 = 0.f, dl = 0.f;
-      if (row < r_end) {
-        rg = range_of(a, b, i);
+      l2_ = dl_ = 0.f;
+      rg_.lo = rg_.hi = 0;
+      if (row < rows.end) {
+        rg_ = range_of(a, b, i);
         const long at = ((long)b * a.Hkv * a.G + h * a.G + row - i * a.G) * a.Lq + i;
-        l2 = lse[at] * LOG2E;
-        if (l2 == -INFINITY) l2 = 0.f;
-        dl = delta[at];
+        l2_ = lse[at] * LOG2E;
+        if (l2_ == -INFINITY) l2_ = 0.f;
+        dl_ = delta[at];
       }
-      rl[tid] = l2;
-      rd[tid] = dl;
-      rlo[tid] = rg.lo;
-      rhi[tid] = rg.hi;
     }
+  };
+  auto store = [&](int to) {
+    sq.store(lq[to], tid);
+    sd.store(ld[to], tid);
+    if (tid < KT) {
+      rl[to][tid] = l2_;
+      rd[to][tid] = dl_;
+      rlo[to][tid] = rg_.lo;
+      rhi[to][tid] = rg_.hi;
+    }
+  };
+  // whether a mask hides some of the tile's rows from some of the keys
+  auto is_mixed = [&](int r0) {
     const Span sp = span_of(a, b, r0, r0 + KT < a.R ? r0 + KT : a.R);
-    const bool mixed = r0 + KT > r_end || k0 < sp.ilo || k0 + 64 > sp.ihi;
-    bool odd = false;
-    if (mixed)
-      odd = __syncthreads_or(sq.odd() || sd.odd());
-    else
-      __syncthreads();
-    if (r0 + KT < r_end) {
-      sq.load_rows(qp, a.q.r, a.q.h, a.G, r0 + KT, r_end, a.D, a.vec, tid);
-      sd.load_rows(dp_, a.o.r, a.o.h, a.G, r0 + KT, r_end, a.D, a.vec, tid);
-    }
+    return r0 + KT > rows.end || k0 < sp.ilo || k0 + KEYS > sp.ihi;
+  };
+  bool odd = false, mixed = true;
+  if (rows.first < rows.end) {
+    load(rows.first);
+    store(0);
+    mixed = is_mixed(rows.first);
+    odd = __syncthreads_or(sq.odd() || sd.odd()) && mixed;
+  }
+  int buf = 0;
+  for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
+    const bool more = r0 + KT < rows.end;
+    if (odd) break;
+    if (more) load(r0 + KT);
     f32x4 s[2], dp[2];
 #pragma unroll
     for (int n = 0; n < 2; n++) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < DB; u++)
-#pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const f32x4 qa = *(const f32x4 *)(lq + (n * 16 + m) * S::LD + 16 * u + 4 * g);
-        const f32x4 da = *(const f32x4 *)(ld + (n * 16 + m) * S::LD + 16 * u + 4 * g);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          s[n] = mfma(qa[c], kf[u][c], s[n]);
-          dp[n] = mfma(da[c], vf[u][c], dp[n]);
-        }
-      }
+    dots<DB>(s, kf, lq[buf], S::LD, lane);
+    dots<DB>(dp, vf, ld[buf], S::LD, lane);
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-      const f32x4 l2 = *(const f32x4 *)(rl + n * 16 + 4 * g), dl = *(const f32x4 *)(rd + n * 16 + 4 * g);
+      const f32x4 l2 = *(const f32x4 *)(rl[buf] + n * 16 + 4 * g), dl = *(const f32x4 *)(rd[buf] + n * 16 + 4 * g);
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         float p = exp2_fast(s[n][r] - l2[r]), x = p * (dp[n][r] - dl[r]);
         if (mixed) {
           const int e = n * 16 + 4 * g + r;
-          if (key < rlo[e] || key >= rhi[e]) p = x = 0.f;
+          if (key < rlo[buf][e] || key >= rhi[buf][e]) p = x = 0.f;
         }
         s[n][r] = p;
         dp[n][r] = x;
       }
     }
-    if (odd) {
-      auto seen = [&](int e) { return key >= rlo[e] && key < rhi[e]; };
-      product_masked<DB, 2>(av, s, ld, S::LD, lane, seen);
-      product_masked<DB, 2>(ak, dp, lq, S::LD, lane, seen);
-    } else {
-      product<DB, 2>(av, s, ld, S::LD, lane);
-      product<DB, 2>(ak, dp, lq, S::LD, lane);
+    product<DB, 2>(av, s, ld[buf], S::LD, lane);
+    product<DB, 2>(ak, dp, lq[buf], S::LD, lane);
+    if (more) {
+      store(buf ^ 1);
+      mixed = is_mixed(r0 + KT);
+      if (mixed)
+        odd = __syncthreads_or(sq.odd() || sd.odd());
+      else
+        __syncthreads();
     }
-    __syncthreads();
   }
-  if (in) {
-    store_row<DB>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
-    store_row<DB>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
+  if (odd) {
+    dkv_one_by_one(a, b, h, k0 + wave * 16, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, DB * 16,
+                   lane);
+    return;
+  }
+  if (!in) return;
+  if (a.splits > 1) {
+    const long at = ((long)blockIdx.y * nbh + bh) * a.Lk + key, half = (long)a.splits * nbh * a.Lk;
+    store_row<DB>(ws + at * (DB * 16), ak, a.scale, DB * 16, 1, lane);
+    store_row<DB>(ws + (half + at) * (DB * 16), av, 1.f, DB * 16, 1, lane);
+    return;
+  }
+  store_row<DB>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
+  store_row<DB>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
+}
+
+// the workgroups' sums of a key, added in their order; 32 lanes a key
+__global__ void __launch_bounds__(256)
+    attn_dkv_join_kernel(Args a, int width, int keys_a_group, const float *__restrict__ ws, float *__restrict__ dk,
+                         float *__restrict__ dv) {
+  const long nbh = (long)a.B * a.Hkv, all = nbh * a.Lk;
+  const int lane = threadIdx.x & 31;
+  for (long e = (long)blockIdx.x * 8 + (threadIdx.x >> 5); e < all; e += (long)gridDim.x * 8) {
+    const int bh = (int)(e / a.Lk), key = (int)(e % a.Lk), b = bh / a.Hkv, h = bh % a.Hkv;
+    const int k0 = key / keys_a_group * keys_a_group;
+    const Rows rows = rows_of(a, b, k0, k0 + keys_a_group);
+    int parts = (rows.end - rows.first + a.chunk - 1) / a.chunk;
+    if (parts < 1) parts = 1;
+    if (4 * lane >= width) continue;
+    f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
+    for (int p = 0; p < parts; p++) {
+      const float *x = ws + ((p * nbh + bh) * a.Lk + key) * width + 4 * lane;
+      sk += *(const f32x4 *)x;
+      sv += *(const f32x4 *)(x + (long)a.splits * all * width);
+    }
+    float *ok = dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
+    float *ov = dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (4 * lane + j < a.D) {
+        ok[4 * lane + j] = sk[j];
+        ov[4 * lane + j] = sv[j];
+      }
   }
 }
 
@@ -947,8 +1113,8 @@ int blocks(int dim) {
 
 struct Plan {
   bool few;
-  int qb;      // row blocks of 16 a wave
-  int tiles;   // row tiles
+  int waves;   // of a workgroup, each with 16 rows
+  int tiles;   // row (key gradients: key) tiles
   int splits, chunk;
   int width;   // floats a row of the parts takes
 };
@@ -970,34 +1136,48 @@ int check(const TTAttention *t) {
   return 0;
 }
 
+// n in parts of `least` or more, about `want` of them and a multiple of `step`
+void split(Plan &p, long n, long want, long least, long step) {
+  long parts = want < 1 ? 1 : want;
+  if (parts > n / least) parts = n / least;
+  if (parts < 1) parts = 1;
+  if (parts > 65535) parts = 65535;  // the grid's second axis
+  const long c = ((n + parts - 1) / parts + step - 1) / step * step;
+  p.chunk = (int)c;
+  p.splits = (int)((n + c - 1) / c);
+}
+
+// Workgroups of 8 waves where two of them a CU are there, else of 4: tiles of
+// half the rows, which read the streamed operand twice as often.
 Plan plan_of(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = R <= 16;
-  p.qb = 1;
+  p.waves = !p.few && (R + 127) / 128 * nbh >= 512 ? 8 : 4;
   if (p.few) {
     p.tiles = 1;
     // parts of 64 to 1024 keys, about eight workgroups a CU
     long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
-    p.chunk = (int)c;
-    p.splits = (int)((t->k_rows + c - 1) / c);
+    split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    if ((R + 127) / 128 * nbh >= 512) p.qb = 2;
-    p.tiles = (int)((R + 64 * p.qb - 1) / (64 * p.qb));
-    long s = 512 / (p.tiles * nbh), most = t->k_rows / 256;
-    s = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
-    long c = (t->k_rows + s - 1) / s;
-    c = (c + KT - 1) / KT * KT;
-    p.chunk = (int)c;
-    p.splits = (int)((t->k_rows + c - 1) / c);
+    p.tiles = (int)((R + 16 * p.waves - 1) / (16 * p.waves));
+    split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
   }
-  if (p.splits > 65535) {  // the grid's second axis
-    long c = ((t->k_rows + 65534) / 65535 + 63) / 64 * 64;
-    p.chunk = (int)c;
-    p.splits = (int)((t->k_rows + c - 1) / c);
-  }
+  return p;
+}
+
+Plan dkv_plan(const TTAttention *t) {
+  Plan p;
+  const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
+  p.width = 16 * blocks(t->head_dim);
+  p.few = false;
+  p.waves = (t->k_rows + 127) / 128 * nbh >= 512 ? 8 : 4;
+  p.tiles = (int)((t->k_rows + 16 * p.waves - 1) / (16 * p.waves));
+  // fp32 sums over at most 2048 rows (16384 in one: 3.1e-6 off, in parts 1e-6)
+  const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
+  split(p, R, fill > sums ? fill : sums, 256, KT);
   return p;
 }
 
@@ -1032,22 +1212,34 @@ void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const
   const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
   if (p.few)
     hipLaunchKernelGGL(attn_few_kernel<DB>, grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
-  else if (p.qb == 1)
-    hipLaunchKernelGGL((attn_fwd_kernel<DB, 1>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+  else if (p.waves == 4)
+    hipLaunchKernelGGL((attn_fwd_kernel<DB, 4>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
   else
-    hipLaunchKernelGGL((attn_fwd_kernel<DB, 2>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+    hipLaunchKernelGGL((attn_fwd_kernel<DB, 8>), grid, dim3(512), 0, stream(), a, q, k, v, o, lse, ml, wo);
 }
 
 template <int DB>
-void run_bwd(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
-             const float *delta, float *dq, float *dk, float *dv) {
+void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
+            const float *delta, float *dq) {
   const long nbh = (long)a.B * a.Hkv;
-  if (dq)
-    hipLaunchKernelGGL(attn_dq_kernel<DB>, dim3((unsigned)(((long)a.R + 63) / 64 * nbh)), dim3(256), 0, stream(),
-                       a, q, k, v, dout, lse, delta, dq);
-  if (dk)
-    hipLaunchKernelGGL(attn_dkv_kernel<DB>, dim3((unsigned)(((long)a.Lk + 63) / 64 * nbh)), dim3(256), 0,
-                       stream(), a, q, k, v, dout, lse, delta, dk, dv);
+  if (((long)a.R + 127) / 128 * nbh >= 512)
+    hipLaunchKernelGGL((attn_dq_kernel<DB, 8>), dim3((unsigned)(((long)a.R + 127) / 128 * nbh)), dim3(512), 0,
+                       stream(), a, q, k, v, dout, lse, delta, dq);
+  else
+    hipLaunchKernelGGL((attn_dq_kernel<DB, 4>), dim3((unsigned)(((long)a.R + 63) / 64 * nbh)), dim3(256), 0,
+                       stream(), a, q, k, v, dout, lse, delta, dq);
+}
+
+template <int DB>
+void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
+             const float *lse, const float *delta, float *dk, float *dv, float *ws) {
+  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
+  if (p.waves == 4)
+    hipLaunchKernelGGL((attn_dkv_kernel<DB, 4>), grid, dim3(256), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv,
+                       ws);
+  else
+    hipLaunchKernelGGL((attn_dkv_kernel<DB, 8>), grid, dim3(512), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv,
+                       ws);
 }
 
 #define BY_DIM(D, F, ...)              \
@@ -1088,8 +1280,7 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
     if (!own) return -2;
   }
   float *ml = w, *wo = w ? w + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
-  Plan pl = p;
-  BY_DIM(a.D, run_fwd, pl, a, q, k, v, o, lse, ml, wo);
+  BY_DIM(a.D, run_fwd, p, a, q, k, v, o, lse, ml, wo);
   if (p.splits > 1) {
     const long rows = (long)a.B * a.Hkv * a.R;
     hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((rows + 3) / 4 < 8192 ? (rows + 3) / 4 : 8192)), dim3(256), 0, stream(), a, p.width, ml,
@@ -1099,8 +1290,14 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   return launched();
 }
 
+// delta of every query row, and the parts of dk and dv
+static size_t delta_floats(const TTAttention *t) { return ((size_t)t->batch * t->q_heads * t->q_rows + 3) / 4 * 4; }
+
 extern "C" size_t tt_k_attention_bwd_ws(const TTAttention *t) {
-  return check(t) ? 0 : sizeof(float) * (size_t)t->batch * t->q_heads * t->q_rows;
+  if (check(t)) return 0;
+  const Plan p = dkv_plan(t);
+  const size_t parts = p.splits > 1 ? 2 * (size_t)p.splits * t->batch * t->kv_heads * t->k_rows * p.width : 0;
+  return sizeof(float) * (delta_floats(t) + parts);
 }
 
 extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const float *k, const float *v,
@@ -1118,9 +1315,23 @@ extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const fl
     if (!own) return -2;
   }
   const long rows = (long)a.B * a.Hkv * a.R;
-  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)), dim3(256), 0, stream(), a, o, dout,
-                     delta);
-  BY_DIM(a.D, run_bwd, a, q, k, v, dout, lse, delta, dq, dk, dv);
+  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)),
+                     dim3(256), 0, stream(), a, o, dout, delta);
+  if (dq) {
+    BY_DIM(a.D, run_dq, a, q, k, v, dout, lse, delta, dq);
+  }
+  if (dk) {
+    const Plan p = dkv_plan(t);
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    float *parts = delta + delta_floats(t);
+    BY_DIM(a.D, run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts);
+    if (p.splits > 1) {
+      const long keys = (long)a.B * a.Hkv * a.Lk;
+      hipLaunchKernelGGL(attn_dkv_join_kernel, dim3((unsigned)((keys + 7) / 8 < 8192 ? (keys + 7) / 8 : 8192)),
+                         dim3(256), 0, stream(), a, p.width, 16 * p.waves, parts, dk, dv);
+    }
+  }
   ttrt_free(own);
   return launched();
 }
