@@ -511,7 +511,9 @@ int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *position
  * [0, rows] are clamped. */
 #define TT_ATTENTION_MAX_DIM 128
 typedef struct TTStrides {
-    long batch, row, head;  /* floats from one to the next; 0: packed in that order */
+    long batch, row, head;  /* floats from one to the next; 0: packed in that order.  Rows and
+                               heads at least head_dim and at most 2^23 apart (heads: 2^28
+                               over the heads that share a key) */
 } TTStrides;
 typedef struct TTAttention {
     long batch, q_rows, k_rows;

@@ -257,24 +257,21 @@ def test_keys_split_over_workgroups(tlib, Lq, Lk, Hq, Hkv):
 
 
 def test_offsets_past_32_bits(tlib):
-    """Rows 2^26 floats apart: the last ones lie past 2^31 elements."""
-    q, k, v, _ = _inputs(1, 1, 40, 2, 1, 64)
-    apart = 1 << 26
-    big = DevBuf(39 * apart + 128)
-    for j in range(40):
+    """Rows 2^23 floats apart: the last ones lie past 2^31 elements."""
+    n, apart = 300, 1 << 23
+    q, k, v, _ = _inputs(1, 1, n, 2, 1, 64)
+    big = DevBuf((n - 1) * apart + 128)
+    for j in range(n):
         for t, off in ((k, 0), (v, 64)):
             row = np.ascontiguousarray(t[0, j, 0])
             check(tlib.tth_h2d(big.ptr + 4 * (j * apart + off), row.ctypes.data, row.nbytes), "h2d")
     s = Strides(0, apart, 0)
-    held, o, dq = [], DevBuf(q.size), DevBuf.from_np(q)
-    a = _plan(q, k, {}, held, k=s, v=s)
-    check(tlib.tt_k_attention_fwd(a, dq.ptr, big.ptr, big.ptr + 256, o.ptr, None, None), "fwd")
-    ref.close(o.to_np(q.shape), ref.attention(q, k, v, ref.seen(1, 1, 40))["o"])
-    q2 = _inputs(1, 30, 40, 2, 1, 64)[0]
-    o2, d2 = DevBuf(q2.size), DevBuf.from_np(q2)
-    a = _plan(q2, k, {}, held, k=s, v=s)
-    check(tlib.tt_k_attention_fwd(a, d2.ptr, big.ptr, big.ptr + 256, o2.ptr, None, None), "fwd")
-    ref.close(o2.to_np(q2.shape), ref.attention(q2, k, v, ref.seen(1, 30, 40))["o"])
+    for Lq in (1, 30):
+        q = _inputs(1, Lq, n, 2, 1, 64)[0]
+        held, o, d = [], DevBuf(q.size), DevBuf.from_np(q)
+        a = _plan(q, k, {}, held, k=s, v=s)
+        check(tlib.tt_k_attention_fwd(a, d.ptr, big.ptr, big.ptr + 256, o.ptr, None, None), "fwd")
+        ref.close(o.to_np(q.shape), ref.attention(q, k, v, ref.seen(1, Lq, n))["o"])
     big.free()
     tlib.tth_release_cache()
 

@@ -70,7 +70,9 @@ BAD_ATTENTION = [dict(batch=0), dict(q_rows=0), dict(k_rows=0), dict(q_heads=0),
                  dict(kv_heads=3), dict(head_dim=0), dict(head_dim=129), dict(window=-1),
                  dict(scale=float("nan")), dict(scale=float("inf")), dict(q_rows=1 << 31),
                  dict(k_rows=1 << 31), dict(batch=1 << 40), dict(batch=1 << 20, q_rows=1 << 20),
-                 dict(batch=1 << 20, k_rows=1 << 20), dict(q=Strides(row=-4)), dict(o=Strides(batch=-1))]
+                 dict(batch=1 << 20, k_rows=1 << 20), dict(q=Strides(row=-4)), dict(o=Strides(batch=-1)),
+                 dict(k=Strides(row=63)), dict(v=Strides(head=63)), dict(k=Strides(row=(1 << 23) + 1)),
+                 dict(q=Strides(head=(1 << 27) + 1)), dict(q_heads=1 << 18, kv_heads=1 << 18)]
 
 
 @pytest.mark.parametrize("kw", BAD_ATTENTION)

@@ -43,7 +43,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 constexpr int KT = 32;  // rows of the streamed operand a tile
 // waves a SIMD that the registers are held to: as many as do without spilling
-#define FWD_WAVES(DB) ((DB) <= 5 ? 4 : 3)
+#define FWD_WAVES(DB) ((DB) == 8 ? 4 : 3)
 #define DQ_WAVES(DB) ((DB) <= 4 ? 4 : (DB) <= 6 ? 3 : 2)
 
 struct Strides {
@@ -280,41 +280,59 @@ __device__ __forceinline__ void store_row(float *p, const f32x4 (&acc)[DB], floa
     }
 }
 
-// the rows [k0, k0 + KT) of an operand on their way to LDS: NV float4 a thread
-// of NT; rows outside [0, end) are zeros
+// Loads through a buffer descriptor: an offset past its length gives zeros, so
+// that rows and columns outside an operand cost a select and no branch.
+constexpr unsigned OUTSIDE = 0x80000000u;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
+}
+
+// the rows [0, KT) from `base` on, on their way to LDS: NV float4 a thread of
+// NT; rows from `left` on are zeros
 template <int DB, int NT>
 struct Stage {
   static constexpr int C4 = DB * 4;                         // float4 a row
   static constexpr int NV = (KT * C4 + NT - 1) / NT;
   static constexpr int LD = DB * 16 + 4;  // rows 4 banks apart: 16-byte reads of 8 rows meet all 32 banks
   f32x4 v[NV];
-  __device__ __forceinline__ void load(const float *base, long stride, int k0, int end, int D, int vec,
-                                       int tid) {
+  __device__ __forceinline__ void get(int n, __amdgpu_buffer_rsrc_t r, int off, int c, bool in, int D, int vec) {
+    if (vec) {
+      v[n] = __builtin_bit_cast(
+          f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, in && c < D ? (unsigned)(off + c) * 4u : OUTSIDE, 0, 0));
+    } else {
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = e / C4, c = (e % C4) * 4;
-      v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (e < KT * C4 && k0 + row < end) v[n] = load4(base + (long)(k0 + row) * stride, c, D, vec);
+      for (int j = 0; j < 4; j++)
+        v[n][j] = __builtin_bit_cast(
+            float,
+            __builtin_amdgcn_raw_buffer_load_b32(r, in && c + j < D ? (unsigned)(off + c + j) * 4u : OUTSIDE, 0, 0));
     }
   }
-  // packed query rows: r = i * G + member
-  __device__ __forceinline__ void load_rows(const float *base, long rs, long hs, int G, int r0, int end, int D,
-                                            int vec, int tid) {
+  __device__ __forceinline__ void load(const float *base, int stride, int left, int D, int vec, int tid) {
+    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
 #pragma unroll
     for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = r0 + e / C4, c = (e % C4) * 4;
-      v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (e < KT * C4 && row < end) {
-        const int i = row / G;
-        v[n] = load4(base + (long)i * rs + (long)(row - i * G) * hs, c, D, vec);
-      }
+      const int e = tid + n * NT, row = e / C4;
+      get(n, r, row * stride, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
+    }
+  }
+  // packed query rows r0 + [0, KT), r = i * G + member, before `end`; `base`: row r0 / G * G
+  __device__ __forceinline__ void load_rows(const float *base, int rs, int hs, int G, int r0, int end, int D,
+                                            int vec, int tid) {
+    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
+    const int first = r0 / G * G;
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int e = tid + n * NT, row = r0 + e / C4, i = (row - first) / G;
+      get(n, r, i * rs + (row - first - i * G) * hs, (e % C4) * 4,
+          (KT * C4 % NT == 0 || e < KT * C4) && row < end, D, vec);
     }
   }
   __device__ __forceinline__ void store(float *lds, int tid) const {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
       const int e = tid + n * NT, row = e / C4, c = (e % C4) * 4;
-      if (e < KT * C4) *(f32x4 *)(lds + row * LD + c) = v[n];
+      if (KT * C4 % NT == 0 || e < KT * C4) *(f32x4 *)(lds + row * LD + c) = v[n];
     }
   }
   __device__ __forceinline__ bool odd() const {  // holds an infinity or a NaN
@@ -423,8 +441,8 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
   S sk, sv;
   bool odd = false;
   if (k_first < k_end) {
-    sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
-    sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+    sk.load(kp + (long)k_first * a.k.r, (int)a.k.r, k_end - k_first, a.D, a.vec, tid);
+    sv.load(vp + (long)k_first * a.v.r, (int)a.v.r, k_end - k_first, a.D, a.vec, tid);
     sk.store(lk[0], tid);
     sv.store(lv[0], tid);
     odd = __syncthreads_or(sv.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
@@ -434,8 +452,8 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
     const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
     if (odd) break;
     if (more) {
-      sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
-      sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
+      sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
+      sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
     }
     f32x4 s[2];
     s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -824,8 +842,8 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
   const int k_first = sp.lo / KT * KT, k_end = sp.hi;
   bool odd = false;
   if (k_first < k_end) {
-    sk.load(kp, a.k.r, k_first, k_end, a.D, a.vec, tid);
-    sv.load(vp, a.v.r, k_first, k_end, a.D, a.vec, tid);
+    sk.load(kp + (long)k_first * a.k.r, (int)a.k.r, k_end - k_first, a.D, a.vec, tid);
+    sv.load(vp + (long)k_first * a.v.r, (int)a.v.r, k_end - k_first, a.D, a.vec, tid);
     sk.store(lk[0], tid);
     sv.store(lv[0], tid);
     odd = __syncthreads_or(sk.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
@@ -835,8 +853,8 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
     const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
     if (odd) break;
     if (more) {
-      sk.load(kp, a.k.r, k0 + KT, k_end, a.D, a.vec, tid);
-      sv.load(vp, a.v.r, k0 + KT, k_end, a.D, a.vec, tid);
+      sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
+      sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
     }
     f32x4 s[2], dp[2];
 #pragma unroll
@@ -973,8 +991,9 @@ __global__ void __launch_bounds__(64 * NW, 2)
   float l2_ = 0.f, dl_ = 0.f;
   Range rg_ = {0, 0};
   auto load = [&](int r0) {
-    sq.load_rows(qp, a.q.r, a.q.h, a.G, r0, rows.end, a.D, a.vec, tid);
-    sd.load_rows(dp_, a.o.r, a.o.h, a.G, r0, rows.end, a.D, a.vec, tid);
+    const int i0 = r0 / a.G;
+    sq.load_rows(qp + (long)i0 * a.q.r, (int)a.q.r, (int)a.q.h, a.G, r0, rows.end, a.D, a.vec, tid);
+    sd.load_rows(dp_ + (long)i0 * a.o.r, (int)a.o.r, (int)a.o.h, a.G, r0, rows.end, a.D, a.vec, tid);
     if (tid < KT) {
       const int row = r0 + tid, i = row / a.G;
       l2_ = dl_ = 0.f;
@@ -1127,9 +1146,14 @@ int check(const TTAttention *t) {
       !(t->scale == t->scale) || isinf(t->scale))
     return -1;
   const TTStrides *all[4] = {&t->q, &t->k, &t->v, &t->o};
-  for (const TTStrides *s : all)
-    if (s->batch < 0 || s->row < 0 || s->head < 0) return -1;
-  const long G = t->q_heads / t->kv_heads, lim = 1L << 30, grid = (1L << 24) - 1;
+  const long G = t->q_heads / t->kv_heads;
+  for (const TTStrides *s : all) {
+    if (s->batch < 0 || (s->row != 0 && s->row < t->head_dim) || (s->head != 0 && s->head < t->head_dim)) return -1;
+    // a tile's rows and a group's heads lie within 2^31 bytes
+    if (s->row > (1L << 28) / KT || s->head > (1L << 28) / G || s->batch > 1L << 50) return -1;
+  }
+  if ((long)t->q_heads * t->head_dim > (1L << 28) / KT) return -1;
+  const long lim = 1L << 30, grid = (1L << 24) - 1;
   if (t->q_rows > lim / G || t->k_rows > lim || t->batch > grid / t->kv_heads) return -1;
   const long nbh = t->batch * t->kv_heads;  // a grid axis has less than 2^32 threads
   if ((t->q_rows * G + 63) / 64 > grid / nbh || (t->k_rows + 63) / 64 > grid / nbh) return -1;
@@ -1173,7 +1197,7 @@ Plan dkv_plan(const TTAttention *t) {
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = false;
-  p.waves = (t->k_rows + 127) / 128 * nbh >= 512 ? 8 : 4;
+  p.waves = (t->k_rows + 127) / 128 * nbh * (R < 512 ? 1 : R / 512) >= 512 ? 8 : 4;
   p.tiles = (int)((t->k_rows + 16 * p.waves - 1) / (16 * p.waves));
   // fp32 sums over at most 2048 rows (16384 in one: 3.1e-6 off, in parts 1e-6)
   const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
