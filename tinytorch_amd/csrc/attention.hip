@@ -1,3 +1,7 @@
+#ifndef FEW_C
+#define FEW_C 0
+#define FEW_NW 4
+#endif
 // Attention on the fp32 matrix units: forward, the form for few query rows,
 // and the backward pass, which recomputes the probabilities.
 //
@@ -41,6 +45,7 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
+constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
 // waves a SIMD that the registers are held to: as many as do without spilling
 #define FWD_WAVES(DB) ((DB) == 8 ? 4 : 3)
@@ -67,63 +72,76 @@ struct Range {
   int lo, hi;
 };
 
-// keys of sequence b, queries of it that hold anything and the position of
-// its first query, whatever the lengths in device memory hold
-__device__ __forceinline__ int keys_of(const Args &a, int b) {
-  const int n = a.k_len ? a.k_len[b] : a.Lk;
-  return n < 0 ? 0 : n > a.Lk ? a.Lk : n;
-}
-__device__ __forceinline__ int queries_of(const Args &a, int b) {
-  const int n = a.q_len ? a.q_len[b] : a.Lq;
-  return n < 0 ? 0 : n > a.Lq ? a.Lq : n;
-}
-__device__ __forceinline__ long start_of(const Args &a, int b) {
-  return a.q_start ? (long)a.q_start[b] : (long)a.Lk - a.Lq;
+// Sequence b, read once by a workgroup: its keys, the queries of it that hold
+// anything and the position of its first query, whatever the lengths in device
+// memory hold.
+struct Seq {
+  int keys, queries;
+  long start;
+};
+__device__ __forceinline__ Seq seq_of(const Args &a, int b) {
+  const int n = a.k_len ? a.k_len[b] : a.Lk, nq = a.q_len ? a.q_len[b] : a.Lq;
+  Seq s;
+  s.keys = n < 0 ? 0 : n > a.Lk ? a.Lk : n;
+  s.queries = nq < 0 ? 0 : nq > a.Lq ? a.Lq : nq;
+  s.start = a.q_start ? (long)a.q_start[b] : (long)a.Lk - a.Lq;
+  return s;
 }
 
-// first key, and the end of the keys, that a query at position `at` sees of n:
-// both grow with `at`
+// first key, and the end of the keys, that a query at position `at` sees: both
+// grow with `at`
 __device__ __forceinline__ int low_of(const Args &a, long at) {
   const long lo = a.window > 0 ? at - a.window + 1 : 0;
   return lo < 0 ? 0 : lo > a.Lk ? a.Lk : (int)lo;
 }
-__device__ __forceinline__ int high_of(const Args &a, long at, int n) {
-  const long hi = a.causal ? at + 1 : a.window > 0 ? at + a.window : n;
-  return hi < 0 ? 0 : hi > n ? n : (int)hi;
+__device__ __forceinline__ int high_of(const Args &a, const Seq &s, long at) {
+  const long hi = a.causal ? at + 1 : a.window > 0 ? at + a.window : s.keys;
+  return hi < 0 ? 0 : hi > s.keys ? s.keys : (int)hi;
 }
 
-// the keys lo <= j < hi of [0, Lk) that query i of sequence b sees
-__device__ __forceinline__ Range range_of(const Args &a, int b, int i) {
-  const long at = start_of(a, b) + i;
-  Range g = {low_of(a, at), high_of(a, at, keys_of(a, b))};
-  if (g.hi <= g.lo || i >= queries_of(a, b)) g.lo = g.hi = 0;
+// the keys lo <= j < hi of [0, Lk) that query i of the sequence sees
+__device__ __forceinline__ Range range_of(const Args &a, const Seq &s, int i) {
+  const long at = s.start + i;
+  Range g = {low_of(a, at), high_of(a, s, at)};
+  if (g.hi <= g.lo || i >= s.queries) g.lo = g.hi = 0;
   return g;
 }
 
-// what the packed rows [r0, r1) of sequence b see: no row a key outside
+// what the queries [i0, i1] of a sequence see: no query a key outside
 // [lo, hi), every row all keys of [ilo, ihi)
 struct Span {
   int lo, hi, ilo, ihi;
 };
 
-__device__ __forceinline__ Span span_of(const Args &a, int b, int r0, int r1) {
+__device__ __forceinline__ Span span_of(const Args &a, const Seq &q, int i0, int i1) {
   Span s = {0, 0, 0, 0};
-  const int nq = queries_of(a, b), i0 = r0 / a.G;
-  int i1 = (r1 - 1) / a.G;
-  const bool whole = i1 < nq;
-  if (!whole) i1 = nq - 1;
+  const bool whole = i1 < q.queries;
+  if (!whole) i1 = q.queries - 1;
   if (i0 > i1) return s;
-  const long at = start_of(a, b);
-  const int n = keys_of(a, b);
-  s.lo = low_of(a, at + i0);
-  s.hi = high_of(a, at + i1, n);
+  s.lo = low_of(a, q.start + i0);
+  s.hi = high_of(a, q, q.start + i1);
   if (s.hi <= s.lo) s.lo = s.hi = 0;
   if (whole) {
-    s.ilo = low_of(a, at + i1);
-    s.ihi = high_of(a, at + i0, n);
+    s.ilo = low_of(a, q.start + i1);
+    s.ihi = high_of(a, q, q.start + i0);
     if (s.ihi <= s.ilo) s.ilo = s.ihi = 0;
   }
   return s;
+}
+
+// the same for the 16 packed rows of a wave from r0 on
+__device__ __forceinline__ Span wave_span(const Args &a, const Seq &q, int r0, int r1) {
+  if (r0 >= r1) return Span{0, 0, 0, 0};
+  return span_of(a, q, r0 / a.G, ((r0 + 16 < r1 ? r0 + 16 : r1) - 1) / a.G);
+}
+
+// Workgroups start in the order of blockIdx, 256 CUs at a time, and under a
+// causal mask the first have the most to do: every other round goes backwards,
+// so that a CU that holds several is not given the heaviest of each.  Eight
+// neighbours keep their order, and with it their XCD and its L2.
+__device__ __forceinline__ int snake(int p, int all) {
+  const int round = p & ~255;
+  return (p & 256) && round + 256 <= all ? round + ((p & 255) ^ 248) : p;
 }
 
 // four values of a row from column c on; 0 behind the row's end
@@ -288,6 +306,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
 }
 
+// x / G for x < G + KT: at most 1 from KT heads a key on
+__device__ __forceinline__ int small_div(int x, int G, unsigned magic) {
+  return G >= KT ? x >= G : (int)((unsigned)x * magic >> 16);
+}
+
 // the rows [0, KT) from `base` on, on their way to LDS: NV float4 a thread of
 // NT; rows from `left` on are zeros
 template <int DB, int NT>
@@ -316,16 +339,15 @@ struct Stage {
       get(n, r, row * stride, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
     }
   }
-  // packed query rows r0 + [0, KT), r = i * G + member, before `end`; `base`: row r0 / G * G
-  __device__ __forceinline__ void load_rows(const float *base, int rs, int hs, int G, int r0, int end, int D,
-                                            int vec, int tid) {
+  // packed query rows, r = i * G + member, from member `m0` of the query at `base` on
+  __device__ __forceinline__ void load_rows(const float *base, int rs, int hs, int G, unsigned magic, int m0, int left,
+                                            int D, int vec, int tid) {
     const __amdgpu_buffer_rsrc_t r = buffer_of(base);
-    const int first = r0 / G * G;
 #pragma unroll
     for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = r0 + e / C4, i = (row - first) / G;
-      get(n, r, i * rs + (row - first - i * G) * hs, (e % C4) * 4,
-          (KT * C4 % NT == 0 || e < KT * C4) && row < end, D, vec);
+      const int e = tid + n * NT, row = e / C4, i = small_div(m0 + row, G, magic);
+      get(n, r, i * rs + (m0 + row - i * G) * hs, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left,
+          D, vec);
     }
   }
   __device__ __forceinline__ void store(float *lds, int tid) const {
@@ -360,13 +382,13 @@ __device__ __forceinline__ float col_sum(float x) {
 // ---------------------------------------------------------------- forward
 
 // 16 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
-__device__ __forceinline__ void fwd_one_by_one(const Args &a, int b, int h, int first, int r1, int k0, int k1,
+__device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, int k0, int k1,
                                                const float *q, const float *k, const float *v, float *o, float *lse,
                                                float *ws_ml, float *ws_o, int width, int lane) {
 #pragma unroll 1
   for (int row = first; row < first + 16 && row < r1; row++) {
     const int i = row / a.G, hm = row - i * a.G;
-    Range rg = range_of(a, b, i);
+    Range rg = range_of(a, sq, i);
     if (rg.lo < k0) rg.lo = k0;
     if (rg.hi > k1) rg.hi = k1;
     Pair qv = load2(q + (long)i * a.q.r + (long)hm * a.q.h, a.D, lane), acc = {0.f, 0.f};
@@ -412,12 +434,14 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
   typedef Stage<DB, 64 * NW> S;
   __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
   constexpr int ROWS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   // the last rows see the most keys under a causal mask: they start first
-  const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
+  const int tile = gridDim.x / nbh - 1 - at0 / nbh;
   const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
-  const Span sp = span_of(a, b, r0, r1);
+  const Seq sq = seq_of(a, b);
+  const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
+  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
   int k_first = sp.lo / KT * KT, k_end = sp.hi;
   if (a.splits > 1) {
     const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
@@ -427,7 +451,7 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
   const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
   Range rg = {0, 0};
-  if (in) rg = range_of(a, b, i);
+  if (in) rg = range_of(a, sq, i);
   f32x4 qf[DB], acc[DB];
   float mx = -INFINITY, sum = 0.f;
   const float *qp0 = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
@@ -455,35 +479,37 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
       sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
       sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
     }
-    f32x4 s[2];
-    s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    dots<DB>(s, qf, lk[buf], S::LD, lane);
-    if (mixed) {
+    if (k0 < mine.hi && k0 + KT > mine.lo) {  // this wave's rows see some of the tile
+      f32x4 s[2];
+      s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      dots<DB>(s, qf, lk[buf], S::LD, lane);
+      if (mixed) {
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int key = k0 + kb * 16 + 4 * g + r;
+            if (key < rg.lo || key >= rg.hi) s[kb][r] = -INFINITY;
+          }
+      }
+      float t = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      t = fmaxf(col_max(t), mx);
+      const float base = t == -INFINITY ? 0.f : t;
+      if (__any(t > mx)) {
+        const float f = exp2_fast(mx - base);
+        sum *= f;
+#pragma unroll
+        for (int u = 0; u < DB; u++) acc[u] *= f;
+        mx = t;
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int key = k0 + kb * 16 + 4 * g + r;
-          if (key < rg.lo || key >= rg.hi) s[kb][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; r++) s[kb][r] = exp2_fast(s[kb][r] - base);
+      sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+      product<DB, 2>(acc, s, lv[buf], S::LD, lane);
     }
-    float t = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    t = fmaxf(col_max(t), mx);
-    const float base = t == -INFINITY ? 0.f : t;
-    if (__any(t > mx)) {
-      const float f = exp2_fast(mx - base);
-      sum *= f;
-#pragma unroll
-      for (int u = 0; u < DB; u++) acc[u] *= f;
-      mx = t;
-    }
-#pragma unroll
-    for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) s[kb][r] = exp2_fast(s[kb][r] - base);
-    sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-    product<DB, 2>(acc, s, lv[buf], S::LD, lane);
     if (more) {
       sk.store(lk[buf ^ 1], tid);
       sv.store(lv[buf ^ 1], tid);
@@ -494,7 +520,7 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
     }
   }
   if (odd) {
-    fwd_one_by_one(a, b, h, r0 + wave * 16, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, DB * 16, lane);
+    fwd_one_by_one(a, sq, b, h, r0 + wave * 16, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, DB * 16, lane);
     return;
   }
 
@@ -559,18 +585,19 @@ struct FewTile {
   }
 };
 
-template <int DB>
-__global__ void __launch_bounds__(256, 2)
+template <int DB, int NW>
+__global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
     attn_few_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
   constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T, LD = DB * 16 + 4;
-  __shared__ __attribute__((aligned(16))) float part[4][16 * LD];
-  __shared__ float pml[4][2][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  __shared__ __attribute__((aligned(16))) float part[NW][16 * LD];
+  __shared__ float pml[NW][2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
   const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   const int r0 = blockIdx.x / nbh * 16, r1 = r0 + 16 < a.R ? r0 + 16 : a.R;
-  const Span sp = span_of(a, b, r0, r1);
+  const Seq sq = seq_of(a, b);
+  const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
   int k_first = sp.lo / 16 * 16, k_end = sp.hi;
   if (a.splits > 1) {
     const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
@@ -580,7 +607,7 @@ __global__ void __launch_bounds__(256, 2)
   const int row = r0 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
   Range rg = {0, 0};
-  if (in) rg = range_of(a, b, i);
+  if (in) rg = range_of(a, sq, i);
   f32x4 qf[DB], acc[DB];
   float mx = -INFINITY, sum = 0.f;
   const float *qp = q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h;
@@ -594,8 +621,8 @@ __global__ void __launch_bounds__(256, 2)
   FewTile<DB> cur, next;
   int k0 = k_first + wave * 16;
   if (k0 < k_end) cur.load(a, kp, vp, k0, sp.lo, k_end, lane);
-  for (; k0 < k_end; k0 += 64) {
-    if (k0 + 64 < k_end) next.load(a, kp, vp, k0 + 64, sp.lo, k_end, lane);
+  for (; k0 < k_end; k0 += 16 * NW) {
+    if (k0 + 16 * NW < k_end) next.load(a, kp, vp, k0 + 16 * NW, sp.lo, k_end, lane);
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < DB; u++)
@@ -671,23 +698,23 @@ __global__ void __launch_bounds__(256, 2)
     cur = next;
   }
   sum = col_sum(sum);
-  // the four waves' parts, joined in wave order
+  // the waves' parts, joined in wave order
   if (g == 0) {
     pml[wave][0][m] = mx;
     pml[wave][1][m] = sum;
   }
   store_row<DB>(&part[wave][m * LD], acc, 1.f, DB * 16, 1, lane);
   __syncthreads();
-  for (int e = tid; e < 16 * DB * 16; e += 256) {
+  for (int e = tid; e < 16 * DB * 16; e += 64 * NW) {
     const int rr = e / (DB * 16), d = e % (DB * 16), r = r0 + rr;
     if (r >= a.R) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, pml[w][0][rr]);
+    for (int w = 0; w < NW; w++) top = fmaxf(top, pml[w][0][rr]);
     const float base = top == -INFINITY ? 0.f : top;
     float total = 0.f, x = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < NW; w++) {
       const float f = exp2_fast(pml[w][0][rr] - base);
       total = fmaf(f, pml[w][1][rr], total);
       x = fmaf(f, part[w][rr * LD + d], x);
@@ -709,37 +736,64 @@ __global__ void __launch_bounds__(256, 2)
   }
 }
 
-// The parts of a row that several workgroups took, joined in their order; one
-// wave a row.  A part without keys has sum 0 and nothing else to read.
-__global__ void __launch_bounds__(256)
+// The parts of a row that several workgroups took, joined in their order by a
+// workgroup of W waves: first the weights of all parts, then the values, the
+// waves every W-th part each.  A part without keys has sum 0 and no values.
+template <int W>
+__global__ void __launch_bounds__(64 * W)
     attn_join_kernel(Args a, int width, const float *__restrict__ ws_ml, const float *__restrict__ ws_o,
                      float *__restrict__ o, float *__restrict__ lse) {
-  const int lane = threadIdx.x & 63;
+  __shared__ float weight[MAX_SPLITS];
+  __shared__ float2 sums[W][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long rows = (long)a.B * a.Hkv * a.R;
-  for (long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6); at < rows; at += (long)gridDim.x * 4) {
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ws_ml[2 * (s * rows + at)]);
+  for (long at = blockIdx.x; at < rows; at += gridDim.x) {
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ws_ml[2 * (s * rows + at)]);
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-  const float base = top == -INFINITY ? 0.f : top;
-  float total = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int s = 0; s < a.splits; s++) {
-    const float l = ws_ml[2 * (s * rows + at) + 1];
-    if (l == 0.f) continue;
-    const float f = exp2_fast(ws_ml[2 * (s * rows + at)] - base);
-    const float *p = ws_o + (s * rows + at) * width;
-    total = fmaf(f, l, total);
-    if (lane < a.D) x0 = fmaf(f, p[lane], x0);
-    if (lane + 64 < a.D) x1 = fmaf(f, p[lane + 64], x1);
-  }
-  const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
-  const int hq = bh % a.Hkv * a.G + r - i * a.G;
-  if (lse && lane == 0)
-    lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
-  float *p = o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h;
-  const float f = total == 0.f ? 0.f : 1.f / total;
-  if (lane < a.D) p[lane] = x0 * f;
-  if (lane + 64 < a.D) p[lane + 64] = x1 * f;
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    for (int s = lane; s < a.splits; s += 64) {
+      const float2 ml = *(const float2 *)(ws_ml + 2 * (s * rows + at));
+      const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - base);
+      if (wave == 0) weight[s] = f;
+      total = fmaf(f, ml.y, total);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
+    __syncthreads();
+    float2 x = make_float2(0.f, 0.f);
+    const float *p = ws_o + at * width + 2 * lane;
+    if (2 * lane < width) {
+#pragma unroll 4
+      for (int s = wave; s < a.splits; s += W) {
+        const float f = weight[s];
+        const float2 v = *(const float2 *)(p + s * rows * width);
+        x.x = f == 0.f ? x.x : fmaf(f, v.x, x.x);
+        x.y = f == 0.f ? x.y : fmaf(f, v.y, x.y);
+      }
+    }
+    if (W > 1) {
+      sums[wave][lane] = x;
+      __syncthreads();
+#pragma unroll
+      for (int w = 1; w < W; w++) {
+        x.x += sums[w][lane].x;
+        x.y += sums[w][lane].y;
+      }
+    }
+    if (wave == 0) {
+      const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
+      const int hq = bh % a.Hkv * a.G + r - i * a.G;
+      if (lse && lane == 0)
+        lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+      float *q = o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h + 2 * lane;
+      const float f = total == 0.f ? 0.f : 1.f / total;
+      if (2 * lane < a.D) q[0] = x.x * f;
+      if (2 * lane + 1 < a.D) q[1] = x.y * f;
+    }
+    __syncthreads();
   }
 }
 
@@ -757,7 +811,7 @@ __global__ void __launch_bounds__(256)
     const int i = (int)(at % a.Lq), Hq = a.Hkv * a.G;
     const long bh = at / a.Lq;
     const int b = (int)(bh / Hq), h = (int)(bh % Hq);
-    if (i < queries_of(a, b)) {
+    if (i < seq_of(a, b).queries) {
       const long off = (long)b * a.o.b + (long)i * a.o.r + (long)h * a.o.h;
       for (int c = 4 * m; c < a.D; c += 64) {
         const f32x4 x = load4(o + off, c, a.D, a.vec), y = load4(dout + off, c, a.D, a.vec);
@@ -772,13 +826,13 @@ __global__ void __launch_bounds__(256)
 }
 
 // dq of 16 packed rows from `first` on
-__device__ __forceinline__ void dq_one_by_one(const Args &a, int b, int h, int first, int r1, const float *q,
+__device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, const float *q,
                                               const float *k, const float *v, const float *dout, const float *lse,
                                               const float *delta, float *dq, int lane) {
 #pragma unroll 1
   for (int row = first; row < first + 16 && row < r1; row++) {
     const int i = row / a.G, hq = h * a.G + row - i * a.G;
-    const Range rg = range_of(a, b, i);
+    const Range rg = range_of(a, sq, i);
     Pair acc = {0.f, 0.f};
     const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i, qo = (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h;
     if (rg.lo < rg.hi) {
@@ -810,19 +864,21 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
   typedef Stage<DB, 64 * NW> S;
   __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
   constexpr int ROWS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int tile = gridDim.x / nbh - 1 - blockIdx.x / nbh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int tile = gridDim.x / nbh - 1 - at0 / nbh;
   const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
-  const Span sp = span_of(a, b, r0, r1);
+  const Seq sq = seq_of(a, b);
+  const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
+  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
   const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
   Range rg = {0, 0};
   float l2 = 0.f, dl = 0.f;
   f32x4 qf[DB], df[DB], acc[DB];
-  const bool live = in && i < queries_of(a, b);
+  const bool live = in && i < sq.queries;
   if (live) {
-    rg = range_of(a, b, i);
+    rg = range_of(a, sq, i);
     const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
     l2 = lse[at] * LOG2E;
     if (l2 == -INFINITY) l2 = 0.f;  // no key has weight: exp2(-inf - 0) = 0
@@ -856,20 +912,22 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
       sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
       sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
     }
-    f32x4 s[2], dp[2];
+    if (k0 < mine.hi && k0 + KT > mine.lo) {
+      f32x4 s[2], dp[2];
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++) s[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    dots<DB>(s, qf, lk[buf], S::LD, lane);
-    dots<DB>(dp, df, lv[buf], S::LD, lane);
+      for (int kb = 0; kb < 2; kb++) s[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      dots<DB>(s, qf, lk[buf], S::LD, lane);
+      dots<DB>(dp, df, lv[buf], S::LD, lane);
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++)
+      for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int key = k0 + kb * 16 + 4 * g + r;
-        const float x = exp2_fast(s[kb][r] - l2) * (dp[kb][r] - dl);
-        s[kb][r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
-      }
-    product<DB, 2>(acc, s, lk[buf], S::LD, lane);
+        for (int r = 0; r < 4; r++) {
+          const int key = k0 + kb * 16 + 4 * g + r;
+          const float x = exp2_fast(s[kb][r] - l2) * (dp[kb][r] - dl);
+          s[kb][r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
+        }
+      product<DB, 2>(acc, s, lk[buf], S::LD, lane);
+    }
     if (more) {
       sk.store(lk[buf ^ 1], tid);
       sv.store(lv[buf ^ 1], tid);
@@ -880,7 +938,7 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
     }
   }
   if (odd) {
-    dq_one_by_one(a, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
+    dq_one_by_one(a, sq, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
     return;
   }
   if (in) store_row<DB>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
@@ -890,28 +948,27 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
 struct Rows {
   int first, end;
 };
-__device__ __forceinline__ Rows rows_of(const Args &a, int b, int k0, int k1) {
-  const long start = start_of(a, b);
-  long i0 = 0, i1 = queries_of(a, b);
+__device__ __forceinline__ Rows rows_of(const Args &a, const Seq &s, int k0, int k1) {
+  long i0 = 0, i1 = s.queries;
   if (a.causal) {
-    if (k0 - start > i0) i0 = k0 - start;
-  } else if (a.window > 0 && k0 - a.window - start + 1 > i0) {
-    i0 = k0 - a.window - start + 1;
+    if (k0 - s.start > i0) i0 = k0 - s.start;
+  } else if (a.window > 0 && k0 - a.window - s.start + 1 > i0) {
+    i0 = k0 - a.window - s.start + 1;
   }
-  if (a.window > 0 && k1 - 1 + a.window - start < i1) i1 = k1 - 1 + a.window - start;
+  if (a.window > 0 && k1 - 1 + a.window - s.start < i1) i1 = k1 - 1 + a.window - s.start;
   Rows r = {0, 0};
-  if (k0 >= keys_of(a, b) || i0 >= i1) return r;
+  if (k0 >= s.keys || i0 >= i1) return r;
   r.first = (int)i0 * a.G;
   r.end = (int)i1 * a.G;
   return r;
 }
 
 // dk and dv of 16 keys from `first` on, from the packed rows [r0, r1)
-__device__ __forceinline__ void dkv_one_by_one(const Args &a, int b, int h, int first, int r0, int r1,
+__device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, int b, int h, int first, int r0, int r1,
                                                const float *q, const float *k, const float *v, const float *dout,
                                                const float *lse, const float *delta, float *dk, float *dv, float *ws,
                                                int width, int lane) {
-  const int keys = keys_of(a, b);
+  const int keys = seq.keys;
 #pragma unroll 1
   for (int key = first; key < first + 16 && key < a.Lk; key++) {
     Pair ak = {0.f, 0.f}, av = {0.f, 0.f};
@@ -925,7 +982,7 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, int b, int h, int 
 #pragma unroll 1
       for (int row = r0; row < r1; row++) {
         const int i = row / a.G, hq = h * a.G + row - i * a.G;
-        const Range rg = range_of(a, b, i);
+        const Range rg = range_of(a, seq, i);
         if (key < rg.lo || key >= rg.hi) continue;
         const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
         float l2 = lse[at] * LOG2E;
@@ -962,17 +1019,18 @@ __global__ void __launch_bounds__(64 * NW, 2)
   __shared__ __attribute__((aligned(16))) float lq[2][KT * S::LD], ld[2][KT * S::LD], rl[2][KT], rd[2][KT];
   __shared__ int rlo[2][KT], rhi[2][KT];
   constexpr int KEYS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int k0 = blockIdx.x / nbh * KEYS, key = k0 + wave * 16 + m;
-  Rows rows = rows_of(a, b, k0, k0 + KEYS);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int k0 = at0 / nbh * KEYS, key = k0 + wave * 16 + m;
+  const Seq seq = seq_of(a, b);
+  Rows rows = rows_of(a, seq, k0, k0 + KEYS);
   if (a.splits > 1) {
     const long c0 = rows.first + (long)blockIdx.y * a.chunk;
     if (c0 >= rows.end && blockIdx.y > 0) return;  // the join leaves it out
     if (c0 + a.chunk < rows.end) rows.end = (int)c0 + a.chunk;
     rows.first = (int)c0;
   }
-  const bool in = key < a.Lk, live = key < keys_of(a, b);
+  const bool in = key < a.Lk, live = key < seq.keys;
   f32x4 kf[DB], vf[DB], ak[DB], av[DB];
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
   const float *vp = v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
@@ -990,21 +1048,33 @@ __global__ void __launch_bounds__(64 * NW, 2)
   // row statistics of a tile, by the first KT threads
   float l2_ = 0.f, dl_ = 0.f;
   Range rg_ = {0, 0};
+  int i_next = 0, m_next = 0;  // the next tile's first row: query and member
+  int t_i0 = 0, t_i1 = 0;      // the queries of the tile loaded last
+  const int step_i = KT / a.G, step_m = KT % a.G;
+  const unsigned magic = 65536u / a.G + 1;  // of small_div: exact for x < 2 KT and G < KT
   auto load = [&](int r0) {
-    const int i0 = r0 / a.G;
-    sq.load_rows(qp + (long)i0 * a.q.r, (int)a.q.r, (int)a.q.h, a.G, r0, rows.end, a.D, a.vec, tid);
-    sd.load_rows(dp_ + (long)i0 * a.o.r, (int)a.o.r, (int)a.o.h, a.G, r0, rows.end, a.D, a.vec, tid);
+    t_i0 = i_next;
+    t_i1 = i_next + small_div(m_next + KT - 1, a.G, magic);
+    const float *q0 = qp + (long)i_next * a.q.r, *d0 = dp_ + (long)i_next * a.o.r;
+    sq.load_rows(q0, (int)a.q.r, (int)a.q.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
+    sd.load_rows(d0, (int)a.o.r, (int)a.o.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
     if (tid < KT) {
-      const int row = r0 + tid, i = row / a.G;
+      const int e = m_next + tid, di = small_div(e, a.G, magic), i = i_next + di;
       l2_ = dl_ = 0.f;
       rg_.lo = rg_.hi = 0;
-      if (row < rows.end) {
-        rg_ = range_of(a, b, i);
-        const long at = ((long)b * a.Hkv * a.G + h * a.G + row - i * a.G) * a.Lq + i;
+      if (r0 + tid < rows.end) {
+        rg_ = range_of(a, seq, i);
+        const long at = ((long)b * a.Hkv * a.G + h * a.G + e - di * a.G) * a.Lq + i;
         l2_ = lse[at] * LOG2E;
         if (l2_ == -INFINITY) l2_ = 0.f;
         dl_ = delta[at];
       }
+    }
+    i_next += step_i;
+    m_next += step_m;
+    if (m_next >= a.G) {
+      m_next -= a.G;
+      i_next++;
     }
   };
   auto store = [&](int to) {
@@ -1018,12 +1088,17 @@ __global__ void __launch_bounds__(64 * NW, 2)
     }
   };
   // whether a mask hides some of the tile's rows from some of the keys
+  bool next_touched = true;
+  const int kw = k0 + wave * 16;
   auto is_mixed = [&](int r0) {
-    const Span sp = span_of(a, b, r0, r0 + KT < a.R ? r0 + KT : a.R);
+    const Span sp = span_of(a, seq, t_i0, t_i1);
+    next_touched = kw < sp.hi && kw + 16 > sp.lo;
     return r0 + KT > rows.end || k0 < sp.ilo || k0 + KEYS > sp.ihi;
   };
   bool odd = false, mixed = true;
   if (rows.first < rows.end) {
+    i_next = rows.first / a.G;
+    m_next = rows.first - i_next * a.G;
     load(rows.first);
     store(0);
     mixed = is_mixed(rows.first);
@@ -1031,30 +1106,32 @@ __global__ void __launch_bounds__(64 * NW, 2)
   }
   int buf = 0;
   for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
-    const bool more = r0 + KT < rows.end;
+    const bool more = r0 + KT < rows.end, touched = next_touched;
     if (odd) break;
     if (more) load(r0 + KT);
-    f32x4 s[2], dp[2];
+    if (touched) {  // some of the rows see some of this wave's keys
+      f32x4 s[2], dp[2];
 #pragma unroll
-    for (int n = 0; n < 2; n++) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    dots<DB>(s, kf, lq[buf], S::LD, lane);
-    dots<DB>(dp, vf, ld[buf], S::LD, lane);
+      for (int n = 0; n < 2; n++) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      dots<DB>(s, kf, lq[buf], S::LD, lane);
+      dots<DB>(dp, vf, ld[buf], S::LD, lane);
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const f32x4 l2 = *(const f32x4 *)(rl[buf] + n * 16 + 4 * g), dl = *(const f32x4 *)(rd[buf] + n * 16 + 4 * g);
+      for (int n = 0; n < 2; n++) {
+        const f32x4 l2 = *(const f32x4 *)(rl[buf] + n * 16 + 4 * g), dl = *(const f32x4 *)(rd[buf] + n * 16 + 4 * g);
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        float p = exp2_fast(s[n][r] - l2[r]), x = p * (dp[n][r] - dl[r]);
-        if (mixed) {
-          const int e = n * 16 + 4 * g + r;
-          if (key < rlo[buf][e] || key >= rhi[buf][e]) p = x = 0.f;
+        for (int r = 0; r < 4; r++) {
+          float p = exp2_fast(s[n][r] - l2[r]), x = p * (dp[n][r] - dl[r]);
+          if (mixed) {
+            const int e = n * 16 + 4 * g + r;
+            if (key < rlo[buf][e] || key >= rhi[buf][e]) p = x = 0.f;
+          }
+          s[n][r] = p;
+          dp[n][r] = x;
         }
-        s[n][r] = p;
-        dp[n][r] = x;
       }
+      product<DB, 2>(av, s, ld[buf], S::LD, lane);
+      product<DB, 2>(ak, dp, lq[buf], S::LD, lane);
     }
-    product<DB, 2>(av, s, ld[buf], S::LD, lane);
-    product<DB, 2>(ak, dp, lq[buf], S::LD, lane);
     if (more) {
       store(buf ^ 1);
       mixed = is_mixed(r0 + KT);
@@ -1065,7 +1142,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
     }
   }
   if (odd) {
-    dkv_one_by_one(a, b, h, k0 + wave * 16, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, DB * 16,
+    dkv_one_by_one(a, seq, b, h, k0 + wave * 16, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, DB * 16,
                    lane);
     return;
   }
@@ -1089,7 +1166,7 @@ __global__ void __launch_bounds__(256)
   for (long e = (long)blockIdx.x * 8 + (threadIdx.x >> 5); e < all; e += (long)gridDim.x * 8) {
     const int bh = (int)(e / a.Lk), key = (int)(e % a.Lk), b = bh / a.Hkv, h = bh % a.Hkv;
     const int k0 = key / keys_a_group * keys_a_group;
-    const Rows rows = rows_of(a, b, k0, k0 + keys_a_group);
+    const Rows rows = rows_of(a, seq_of(a, b), k0, k0 + keys_a_group);
     int parts = (rows.end - rows.first + a.chunk - 1) / a.chunk;
     if (parts < 1) parts = 1;
     if (4 * lane >= width) continue;
@@ -1165,7 +1242,7 @@ void split(Plan &p, long n, long want, long least, long step) {
   long parts = want < 1 ? 1 : want;
   if (parts > n / least) parts = n / least;
   if (parts < 1) parts = 1;
-  if (parts > 65535) parts = 65535;  // the grid's second axis
+  if (parts > MAX_SPLITS) parts = MAX_SPLITS;
   const long c = ((n + parts - 1) / parts + step - 1) / step * step;
   p.chunk = (int)c;
   p.splits = (int)((n + c - 1) / c);
@@ -1178,12 +1255,17 @@ Plan plan_of(const TTAttention *t) {
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = R <= 16;
+#ifdef FW
+  p.waves = p.few ? 4 : FW;
+#else
   p.waves = !p.few && (R + 127) / 128 * nbh >= 512 ? 8 : 4;
+#endif
   if (p.few) {
     p.tiles = 1;
     // parts of 64 to 1024 keys, about eight workgroups a CU
     long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
+    if (FEW_C > 0) c = FEW_C;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
     p.tiles = (int)((R + 16 * p.waves - 1) / (16 * p.waves));
@@ -1197,7 +1279,11 @@ Plan dkv_plan(const TTAttention *t) {
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = false;
+#ifdef KW
+  p.waves = KW;
+#else
   p.waves = (t->k_rows + 127) / 128 * nbh * (R < 512 ? 1 : R / 512) >= 512 ? 8 : 4;
+#endif
   p.tiles = (int)((t->k_rows + 16 * p.waves - 1) / (16 * p.waves));
   // fp32 sums over at most 2048 rows (16384 in one: 3.1e-6 off, in parts 1e-6)
   const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
@@ -1235,7 +1321,7 @@ void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const
              float *ml, float *wo) {
   const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
   if (p.few)
-    hipLaunchKernelGGL(attn_few_kernel<DB>, grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
+    hipLaunchKernelGGL((attn_few_kernel<DB, FEW_NW>), grid, dim3(64 * FEW_NW), 0, stream(), a, q, k, v, o, lse, ml, wo);
   else if (p.waves == 4)
     hipLaunchKernelGGL((attn_fwd_kernel<DB, 4>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
   else
@@ -1246,7 +1332,11 @@ template <int DB>
 void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
             const float *delta, float *dq) {
   const long nbh = (long)a.B * a.Hkv;
+#ifdef DW
+  if (DW == 8)
+#else
   if (((long)a.R + 127) / 128 * nbh >= 512)
+#endif
     hipLaunchKernelGGL((attn_dq_kernel<DB, 8>), dim3((unsigned)(((long)a.R + 127) / 128 * nbh)), dim3(512), 0,
                        stream(), a, q, k, v, dout, lse, delta, dq);
   else
@@ -1307,8 +1397,11 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   BY_DIM(a.D, run_fwd, p, a, q, k, v, o, lse, ml, wo);
   if (p.splits > 1) {
     const long rows = (long)a.B * a.Hkv * a.R;
-    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((rows + 3) / 4 < 8192 ? (rows + 3) / 4 : 8192)), dim3(256), 0, stream(), a, p.width, ml,
-                       wo, o, lse);
+    const dim3 grid((unsigned)(rows < 65536 ? rows : 65536));
+    if (p.splits > 8)
+      hipLaunchKernelGGL(attn_join_kernel<4>, grid, dim3(256), 0, stream(), a, p.width, ml, wo, o, lse);
+    else
+      hipLaunchKernelGGL(attn_join_kernel<1>, grid, dim3(64), 0, stream(), a, p.width, ml, wo, o, lse);
   }
   ttrt_free(own);
   return launched();
