@@ -306,6 +306,22 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
 }
 
+__device__ __forceinline__ float get1(__amdgpu_buffer_rsrc_t r, int off, int c, bool in, int D) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_raw_buffer_load_b32(r, in && c < D ? (unsigned)(off + c) * 4u : OUTSIDE, 0, 0));
+}
+__device__ __forceinline__ f32x4 get4(__amdgpu_buffer_rsrc_t r, int off, int c, bool in, int D, int vec) {
+  f32x4 v;
+  if (vec) {
+    v = __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, in && c < D ? (unsigned)(off + c) * 4u : OUTSIDE, 0, 0));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = get1(r, off, c + j, in, D);
+  }
+  return v;
+}
+
 // x / G for x < G + KT: at most 1 from KT heads a key on
 __device__ __forceinline__ int small_div(int x, int G, unsigned magic) {
   return G >= KT ? x >= G : (int)((unsigned)x * magic >> 16);
@@ -319,24 +335,12 @@ struct Stage {
   static constexpr int NV = (KT * C4 + NT - 1) / NT;
   static constexpr int LD = DB * 16 + 4;  // rows 4 banks apart: 16-byte reads of 8 rows meet all 32 banks
   f32x4 v[NV];
-  __device__ __forceinline__ void get(int n, __amdgpu_buffer_rsrc_t r, int off, int c, bool in, int D, int vec) {
-    if (vec) {
-      v[n] = __builtin_bit_cast(
-          f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, in && c < D ? (unsigned)(off + c) * 4u : OUTSIDE, 0, 0));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        v[n][j] = __builtin_bit_cast(
-            float,
-            __builtin_amdgcn_raw_buffer_load_b32(r, in && c + j < D ? (unsigned)(off + c + j) * 4u : OUTSIDE, 0, 0));
-    }
-  }
   __device__ __forceinline__ void load(const float *base, int stride, int left, int D, int vec, int tid) {
     const __amdgpu_buffer_rsrc_t r = buffer_of(base);
 #pragma unroll
     for (int n = 0; n < NV; n++) {
       const int e = tid + n * NT, row = e / C4;
-      get(n, r, row * stride, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
+      v[n] = get4(r, row * stride, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
     }
   }
   // packed query rows, r = i * G + member, from member `m0` of the query at `base` on
@@ -346,8 +350,8 @@ struct Stage {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
       const int e = tid + n * NT, row = e / C4, i = small_div(m0 + row, G, magic);
-      get(n, r, i * rs + (m0 + row - i * G) * hs, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left,
-          D, vec);
+      v[n] = get4(r, i * rs + (m0 + row - i * G) * hs, (e % C4) * 4,
+                  (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
     }
   }
   __device__ __forceinline__ void store(float *lds, int tid) const {
@@ -542,44 +546,45 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
 }
 
 // Few packed rows (one tile of 16): the keys pass once, from memory to
-// registers in the operand layouts, 16 a wave at a time, the next 16 loaded
-// while these are used.  Bandwidth-bound: the keys are split over workgroups.
+// registers in the operand layouts, 16 a wave at a time.  Bandwidth-bound, so
+// the keys are split over workgroups; a wave's next keys are on their way as
+// soon as its scores are done, its next values as soon as these are used.
 template <int DB>
 struct FewTile {
   static constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
   typedef typename Vec<VW>::T V;
   f32x4 k[DB];
   V v[4][T];
-  __device__ __forceinline__ void load(const Args &a, const float *kp, const float *vp, int k0, int lo, int hi,
-                                       int lane) {
+  // keys [0, 16) from `base` on, those of [from, left)
+  __device__ __forceinline__ void load_k(const float *base, int stride, int from, int left, int D, int vec, int lane) {
+    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
     const int g = lane >> 4, m = lane & 15;
-    const int key = k0 + m;
-    const bool in = key >= lo && key < hi;
-    const float *p = kp + (long)key * a.k.r;
+    const bool in = m >= from && m < left;
 #pragma unroll
-    for (int u = 0; u < DB; u++) {
-      k[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (in) k[u] = load4(p, 16 * u + 4 * g, a.D, a.vec);
-    }
+    for (int u = 0; u < DB; u++) k[u] = get4(r, m * stride, 16 * u + 4 * g, in, D, vec);
+  }
+  __device__ __forceinline__ void load_v(const float *base, int stride, int from, int left, int D, int vec, int lane) {
+    const __amdgpu_buffer_rsrc_t rs = buffer_of(base);
+    const int g = lane >> 4, m = lane & 15;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const int kv = k0 + 4 * g + r;
-      const bool have = kv >= lo && kv < hi;
-      const float *x = vp + (long)kv * a.v.r;
+      const int key = 4 * g + r;
+      const bool in = key >= from && key < left;
 #pragma unroll
       for (int t = 0; t < T; t++) {
         const int d = 16 * VW * t + VW * m;
-        V w = {};
-        if (have) {
-          if (a.vec) {
-            if (d < a.D) w = *(const V *)(x + d);
-          } else {
-#pragma unroll
-            for (int c = 0; c < VW; c++)
-              if (d + c < a.D) ((float *)&w)[c] = x[d + c];
-          }
+        if constexpr (VW == 4) {
+          v[r][t] = get4(rs, key * stride, d, in, D, vec);
+        } else if constexpr (VW == 2) {
+          if (vec)
+            v[r][t] = __builtin_bit_cast(
+                V, __builtin_amdgcn_raw_buffer_load_b64(rs, in && d < D ? (unsigned)(key * stride + d) * 4u : OUTSIDE,
+                                                        0, 0));
+          else
+            v[r][t] = (V){get1(rs, key * stride, d, in, D), get1(rs, key * stride, d + 1, in, D)};
+        } else {
+          v[r][t] = get1(rs, key * stride, d, in, D);
         }
-        v[r][t] = w;
       }
     }
   }
@@ -618,16 +623,29 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
     if (in) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
   }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
-  FewTile<DB> cur, next;
+  FewTile<DB> cur;
+  auto load_k = [&](int k0) {
+    cur.load_k(kp + (long)k0 * a.k.r, (int)a.k.r, sp.lo - k0, k_end - k0, a.D, a.vec, lane);
+  };
+  auto load_v = [&](int k0) {
+    cur.load_v(vp + (long)k0 * a.v.r, (int)a.v.r, sp.lo - k0, k_end - k0, a.D, a.vec, lane);
+  };
   int k0 = k_first + wave * 16;
-  if (k0 < k_end) cur.load(a, kp, vp, k0, sp.lo, k_end, lane);
+  if (k0 < k_end) {
+    load_k(k0);
+    load_v(k0);
+  }
   for (; k0 < k_end; k0 += 16 * NW) {
-    if (k0 + 16 * NW < k_end) next.load(a, kp, vp, k0 + 16 * NW, sp.lo, k_end, lane);
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = s;  // two chains: one waits for each product's result
 #pragma unroll
     for (int u = 0; u < DB; u++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) s = mfma(cur.k[u][c], qf[u][c], s);
+      for (int c = 0; c < 4; c += 2) {
+        s = mfma(cur.k[u][c], qf[u][c], s);
+        s2 = mfma(cur.k[u][c + 1], qf[u][c + 1], s2);
+      }
+    s += s2;
+    if (k0 + 16 * NW < k_end) load_k(k0 + 16 * NW);
     float t = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
@@ -695,7 +713,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
           for (int c = 0; c < VW; c++)
             acc[t2 * VW + c] = mfma(Vec<VW>::at(cur.v[r][t2], c), s[r], acc[t2 * VW + c]);
     }
-    cur = next;
+    if (k0 + 16 * NW < k_end) load_v(k0 + 16 * NW);
   }
   sum = col_sum(sum);
   // the waves' parts, joined in wave order

@@ -68,7 +68,8 @@ struct Call {
 };
 
 struct Entries {
-  int id[TT_DISTILL_MAX_TOP];   // -1: none
+  int4 id[TT_DISTILL_MAX_TOP / 4];  // -1: none
+  float z[TT_DISTILL_MAX_TOP];  // the student's logits at them
   float p[TT_DISTILL_MAX_TOP];  // the teacher's logit, then log2 of the probability
   float mass;                   // 1, or 0 for a row without entries
 };
@@ -76,11 +77,14 @@ struct Entries {
 // wave 0: the row's entries to LDS as probabilities
 __device__ __forceinline__ void read_entries(const Call &a, long row, Entries &e, int lane) {
   float most = -INFINITY;
+  int *ids = (int *)e.id;
+  for (int k = a.top + lane; k < (a.top + 3 & ~3); k += 64) ids[k] = -1;
   for (int k = lane; k < a.top; k += 64) {
     const int id = a.ids[row * a.top + k];
     const bool ok = id >= 0 && id < a.cols;
     const float t = ok ? a.teacher[row * a.top + k] : -INFINITY;
-    e.id[k] = ok ? id : -1;
+    ids[k] = ok ? id : -1;
+    if (ok) e.z[k] = a.z[row * a.cols + id];
     e.p[k] = t;
     most = t != t || most != most ? NAN : fmaxf(most, t);  // a NaN is the row's
   }
@@ -107,23 +111,33 @@ __device__ __forceinline__ void read_entries(const Call &a, long row, Entries &e
 __device__ __forceinline__ void finish(const Call &a, long row, const Entries &e, float most, bool flat,
                                        float lse2, int lane, bool gradient) {
   float loss = 0.f;
+  const int *ids = (const int *)e.id;
   for (int k = lane; k < a.top; k += 64) {
-    const int id = e.id[k];
+    const int id = ids[k];
     const float lp = e.p[k];
     if (id < 0) continue;
-    const float lq = (flat ? 0.f : (a.z[row * a.cols + id] - most) * a.c) - lse2;
+    const float lq = (flat ? 0.f : (e.z[k] - most) * a.c) - lse2;
     const float p = exp2_fast(lp);
     if (p != 0.f) loss = fmaf(p, (lp - lq) * LN2, loss);
     if (!gradient) continue;
     // entries of one column: the first writes the sum of all
+    int same = 0, first = k;
+    for (int o = (a.top + 3) / 4 - 1; o >= 0; o--) {
+      const int4 t = e.id[o];
+      same += (t.x == id) + (t.y == id) + (t.z == id) + (t.w == id);
+      if (t.w == id) first = 4 * o + 3;
+      if (t.z == id) first = 4 * o + 2;
+      if (t.y == id) first = 4 * o + 1;
+      if (t.x == id) first = 4 * o;
+    }
+    if (first != k) continue;
     float sum = p;
-    bool first = true;
-    for (int o = 0; o < a.top; o++)
-      if (o != k && e.id[o] == id) {
-        if (o < k) first = false;
-        else sum += exp2_fast(e.p[o]);
+    for (int o = k + 1; same > 1; o++)
+      if (ids[o] == id) {
+        sum += exp2_fast(e.p[o]);
+        same--;
       }
-    if (first) a.dz[row * a.cols + id] = a.coef * (exp2_fast(lq) * e.mass - sum);
+    a.dz[row * a.cols + id] = a.coef * (exp2_fast(lq) * e.mass - sum);
   }
   loss = wave_all(loss, Add());
   if (lane == 0) a.rowloss[row] = e.mass == 0.f ? 0.f : loss * a.t2;
@@ -239,14 +253,18 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
     hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a);      \
   else                                                                                       \
     hipLaunchKernelGGL((distill_kernel<NT, NV, false>), grid, dim3(NT), 0, stream(), a)
+  // rows of up to 32768 columns leave room for two workgroups a CU, so that one
+  // reads while the other reduces or writes
   if (cols <= 1024) {
     RUN(256, 1);
   } else if (cols <= 4096) {
     RUN(256, 4);
+  } else if (cols <= 8192) {
+    RUN(512, 4);
   } else if (cols <= 16384) {
-    RUN(1024, 4);
+    RUN(512, 8);
   } else if (cols <= 32768) {
-    RUN(1024, 8);
+    RUN(512, 16);
   } else if (cols <= 65536) {
     RUN(1024, 16);
   } else {

@@ -205,24 +205,30 @@ __global__ void __launch_bounds__(threads_of(NT))
   }
 }
 
-// dw / db from the workgroups' sums: 64 columns a workgroup, 16 threads a
-// column, each a run of them
+// dw / db from the workgroups' sums: 16 columns a workgroup, 64 threads a
+// column, each every 64th of them, then in a fixed tree.  Latency-bound (4 MB
+// at 1024 columns): a thread's reads do not wait for each other.
 __global__ void __launch_bounds__(1024)
     ln_join_kernel(const float *__restrict__ part, float *__restrict__ dw, float *__restrict__ db, int blocks,
                    long cols) {
-  __shared__ float sum[16][65];
-  const int lane = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const long c = (long)blockIdx.x * 64 + lane;
+  __shared__ float sum[16][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long c = (long)blockIdx.x * 16 + (lane & 15);
   float *out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0.f;
-  if (c < cols)
-    for (int k = y; k < blocks; k += 16) s += part[((long)k * 2 + blockIdx.y) * cols + c];
-  sum[y][lane] = s;
+  if (c < cols) {
+#pragma unroll 8
+    for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += part[((long)k * 2 + blockIdx.y) * cols + c];
+  }
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (lane < 16) sum[wave][lane] = s;
   __syncthreads();
-  if (y == 0 && c < cols) {
+  if (threadIdx.x < 16 && c < cols) {
+    s = 0.f;
 #pragma unroll
-    for (int k = 1; k < 16; k++) s += sum[k][lane];
+    for (int k = 0; k < 16; k++) s += sum[k][lane];
     out[c] = s;
   }
 }
@@ -392,7 +398,7 @@ extern "C" int tt_k_layernorm_bwd(const float *x, const float *w, const float *d
 #undef RUN
   }
   if (part)
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((cols + 63) / 64), 2), dim3(1024), 0, stream(), part, dw, db,
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((cols + 15) / 16), 2), dim3(1024), 0, stream(), part, dw, db,
                        blocks, cols);
   ttrt_free(own);
   return launched();
