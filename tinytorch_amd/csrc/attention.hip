@@ -39,6 +39,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;  // in memory, at any float
 
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
@@ -63,7 +64,7 @@ struct Args {
   float scale;
   const int32_t *q_start, *q_len, *k_len;
   Strides q, k, v, o;
-  int vec;            // every row of every operand is 16-byte aligned
+  int vec;            // D is a multiple of 4: rows are read four values at a time
   int chunk;          // keys a workgroup takes of a row tile's (splits > 1)
   int splits;
 };
@@ -148,7 +149,7 @@ __device__ __forceinline__ int snake(int p, int all) {
 __device__ __forceinline__ f32x4 load4(const float *p, int c, int D, int vec) {
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (vec) {
-    if (c < D) v = *(const f32x4 *)(p + c);
+    if (c < D) v = *(const f32x4_any *)(p + c);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -288,7 +289,7 @@ __device__ __forceinline__ void store_row(float *p, const f32x4 (&acc)[DB], floa
         if (d < D) {
           const f32x4 v = {acc[t * VW][e] * f, acc[t * VW + (VW > 1)][e] * f, acc[t * VW + (VW > 2 ? 2 : 0)][e] * f,
                            acc[t * VW + (VW > 2 ? 3 : 0)][e] * f};
-          *(f32x4 *)(p + d) = v;
+          *(f32x4_any *)(p + d) = v;
         }
       } else {
 #pragma unroll
@@ -1215,10 +1216,6 @@ Strides packed(const TTStrides &s, long rows, int heads, int dim) {
   return p;
 }
 
-bool aligned(const void *p, const Strides &s) {
-  return ((uintptr_t)p & 15) == 0 && s.b % 4 == 0 && s.r % 4 == 0 && s.h % 4 == 0;
-}
-
 // 16-column blocks that the kernels hold for a head dimension
 int blocks(int dim) {
   const int n = (dim + 15) / 16;
@@ -1328,7 +1325,7 @@ Args args_of(const TTAttention *t) {
   a.k = packed(t->k, t->k_rows, t->kv_heads, t->head_dim);
   a.v = packed(t->v, t->k_rows, t->kv_heads, t->head_dim);
   a.o = packed(t->o, t->q_rows, t->q_heads, t->head_dim);
-  a.vec = 0;
+  a.vec = a.D % 4 == 0;
   a.chunk = 0;
   a.splits = 1;
   return a;
@@ -1402,7 +1399,6 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   if (ttrt_init() != 0) return -3;
   const Plan p = plan_of(t);
   Args a = args_of(t);
-  a.vec = a.D % 4 == 0 && aligned(q, a.q) && aligned(k, a.k) && aligned(v, a.v) && aligned(o, a.o);
   a.splits = p.splits;
   a.chunk = p.chunk;
   const size_t need = fwd_bytes(t);
@@ -1442,8 +1438,6 @@ extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const fl
   if (!dq && !dk) return 0;
   if (ttrt_init() != 0) return -3;
   Args a = args_of(t);
-  a.vec = a.D % 4 == 0 && aligned(q, a.q) && aligned(k, a.k) && aligned(v, a.v) && aligned(o, a.o) &&
-          aligned(dout, a.o) && aligned(dq, a.q) && aligned(dk, a.k) && aligned(dv, a.v);
   float *own = NULL, *delta = (float *)ws;
   if (!delta) {
     delta = own = (float *)ttrt_alloc(tt_k_attention_bwd_ws(t));

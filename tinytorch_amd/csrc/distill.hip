@@ -18,10 +18,10 @@
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;  // in memory, at any float
 
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
-inline bool a16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
@@ -143,8 +143,9 @@ __device__ __forceinline__ void finish(const Call &a, long row, const Entries &e
   if (lane == 0) a.rowloss[row] = e.mass == 0.f ? 0.f : loss * a.t2;
 }
 
-// a row of up to 4 NT NV columns
-template <int NT, int NV, bool VEC>
+// a row of up to 4 NT NV columns; TAIL: their number is no multiple of 4, and
+// the last group of 4 is taken value by value
+template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
   __shared__ float part[NT / 64];
   __shared__ Entries e;
@@ -155,15 +156,13 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
       v[n] = (f32x4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (VEC) {
-        const int c = (n * NT + t) * 4;
-        if (c < a.cols) v[n] = *(const f32x4 *)(z + c);
-      } else {
+      const int c = (n * NT + t) * 4;
+      if (c + (TAIL ? 3 : 0) < a.cols) {
+        v[n] = *(const f32x4_any *)(z + c);
+      } else if (TAIL) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int c = (n * 4 + j) * NT + t;
-          if (c < a.cols) v[n][j] = z[c];
-        }
+        for (int j = 0; j < 3; j++)
+          if (c + j < a.cols) v[n][j] = z[c + j];
       }
     }
     if (t < 64) read_entries(a, row, e, t);
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
     for (int n = 0; n < NV; n++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int c = VEC ? (n * NT + t) * 4 + j : (n * 4 + j) * NT + t;
+        const int c = (n * NT + t) * 4 + j;
         float x = flat ? 1.f : exp2_fast((v[n][j] - most) * a.c);
         if (c >= a.cols) x = 0.f;
         v[n][j] = x;
@@ -191,15 +190,13 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
 #pragma unroll
       for (int n = 0; n < NV; n++) {
         v[n] *= f;
-        if (VEC) {
-          const int c = (n * NT + t) * 4;
-          if (c < a.cols) *(f32x4 *)(dz + c) = v[n];
-        } else {
+        const int c = (n * NT + t) * 4;
+        if (c + (TAIL ? 3 : 0) < a.cols) {
+          *(f32x4_any *)(dz + c) = v[n];
+        } else if (TAIL) {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const int c = (n * 4 + j) * NT + t;
-            if (c < a.cols) dz[c] = v[n][j];
-          }
+          for (int j = 0; j < 3; j++)
+            if (c + j < a.cols) dz[c + j] = v[n][j];
         }
       }
     }
@@ -246,13 +243,12 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
   if (ttrt_init() != 0) return -3;
   const Call a = {logits, ids, teacher, rowloss, dlogits, rows, cols, top, LOG2E / temperature,
                   temperature * temperature, scale * temperature};
-  const bool vec = cols % 4 == 0 && a16(logits) && a16(dlogits);
   const dim3 grid((unsigned)(rows < 1 << 20 ? rows : 1 << 20));
 #define RUN(NT, NV)                                                                          \
-  if (vec)                                                                                   \
-    hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a);      \
+  if (cols % 4 == 0)                                                                                  \
+    hipLaunchKernelGGL((distill_kernel<NT, NV, false>), grid, dim3(NT), 0, stream(), a);      \
   else                                                                                       \
-    hipLaunchKernelGGL((distill_kernel<NT, NV, false>), grid, dim3(NT), 0, stream(), a)
+    hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a)
   // rows of up to 32768 columns leave room for two workgroups a CU, so that one
   // reads while the other reduces or writes
   if (cols <= 1024) {

@@ -17,10 +17,12 @@
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+// in memory: 16-byte accesses need no more than a float's alignment here, so
+// rows of any length and place take them
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
-inline bool a16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
@@ -49,51 +51,47 @@ __device__ __forceinline__ void row_sum2(float &x, float &y, float (*part)[2]) {
   }
 }
 
-// column of value j of group n: 4 consecutive ones of a thread where rows are
-// 16-byte aligned, else consecutive ones of consecutive threads
-template <int NT, bool VEC>
-__device__ __forceinline__ int col_of(int n, int j, int t) {
-  return VEC ? (n * NT + t) * 4 + j : (n * 4 + j) * NT + t;
+// Group n of a thread's values: the columns from this one on.  With TAIL (cols
+// not a multiple of 4) the row's last group is taken value by value.
+template <int NT>
+__device__ __forceinline__ int col_of(int n, int t) {
+  return (n * NT + t) * 4;
 }
 
-template <int NT, int NV, bool VEC>
+template <int NT, int NV, bool TAIL>
 __device__ __forceinline__ void load_row(f32x4 (&v)[NV], const float *p, int cols, int t) {
 #pragma unroll
   for (int n = 0; n < NV; n++) {
+    const int c = col_of<NT>(n, t);
     v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (VEC) {
-      const int c = col_of<NT, VEC>(n, 0, t);
-      if (c < cols) v[n] = *(const f32x4 *)(p + c);
-    } else {
+    if (c + (TAIL ? 3 : 0) < cols) {
+      v[n] = *(const f32x4_any *)(p + c);
+    } else if (TAIL) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int c = col_of<NT, VEC>(n, j, t);
-        if (c < cols) v[n][j] = p[c];
-      }
+      for (int j = 0; j < 3; j++)
+        if (c + j < cols) v[n][j] = p[c + j];
     }
   }
 }
 
-template <int NT, int NV, bool VEC>
+template <int NT, int NV, bool TAIL>
 __device__ __forceinline__ void store_row(const f32x4 (&v)[NV], float *p, int cols, int t) {
 #pragma unroll
   for (int n = 0; n < NV; n++) {
-    if (VEC) {
-      const int c = col_of<NT, VEC>(n, 0, t);
-      if (c < cols) *(f32x4 *)(p + c) = v[n];
-    } else {
+    const int c = col_of<NT>(n, t);
+    if (c + (TAIL ? 3 : 0) < cols) {
+      *(f32x4_any *)(p + c) = v[n];
+    } else if (TAIL) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int c = col_of<NT, VEC>(n, j, t);
-        if (c < cols) p[c] = v[n][j];
-      }
+      for (int j = 0; j < 3; j++)
+        if (c + j < cols) p[c + j] = v[n][j];
     }
   }
 }
 
 constexpr int threads_of(int nt) { return nt < 256 ? 256 : nt; }
 
-template <int NT, int NV, bool VEC>
+template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(threads_of(NT))
     ln_fwd_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                   float *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, long rows, int cols,
@@ -103,7 +101,7 @@ __global__ void __launch_bounds__(threads_of(NT))
   const int t = threadIdx.x % NT;
   for (long row = (long)blockIdx.x * RB + threadIdx.x / NT; row < rows; row += (long)gridDim.x * RB) {
     f32x4 v[NV];
-    load_row<NT, NV, VEC>(v, x + row * cols, cols, t);
+    load_row<NT, NV, TAIL>(v, x + row * cols, cols, t);
     float s = 0.f, z = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; n++) s += (v[n][0] + v[n][1]) + (v[n][2] + v[n][3]);
@@ -115,14 +113,14 @@ __global__ void __launch_bounds__(threads_of(NT))
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         v[n][j] -= mu;
-        if (col_of<NT, VEC>(n, j, t) < cols) q = fmaf(v[n][j], v[n][j], q);
+        if (col_of<NT>(n, t) + j < cols) q = fmaf(v[n][j], v[n][j], q);
       }
     z = 0.f;
     row_sum2<NT>(q, z, part);
     const float r = 1.f / sqrtf(q / (float)cols + eps);
     f32x4 g[NV], o[NV];
-    if (w) load_row<NT, NV, VEC>(g, w, cols, t);
-    if (b) load_row<NT, NV, VEC>(o, b, cols, t);
+    if (w) load_row<NT, NV, TAIL>(g, w, cols, t);
+    if (b) load_row<NT, NV, TAIL>(o, b, cols, t);
 #pragma unroll
     for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -130,7 +128,7 @@ __global__ void __launch_bounds__(threads_of(NT))
         const float h = v[n][j] * r;
         v[n][j] = fmaf(h, w ? g[n][j] : 1.f, b ? o[n][j] : 0.f);
       }
-    store_row<NT, NV, VEC>(v, y + row * cols, cols, t);
+    store_row<NT, NV, TAIL>(v, y + row * cols, cols, t);
     if (t == 0) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
@@ -139,7 +137,7 @@ __global__ void __launch_bounds__(threads_of(NT))
 }
 
 // dx, and (part) this workgroup's sums over its rows for dw and db: part[block][2][cols]
-template <int NT, int NV, bool VEC>
+template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(threads_of(NT))
     ln_bwd_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ dy,
                   const float *__restrict__ mean, const float *__restrict__ rstd, float *__restrict__ dx,
@@ -153,11 +151,11 @@ __global__ void __launch_bounds__(threads_of(NT))
   for (int n = 0; n < NV; n++) aw[n] = ab[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   for (long row = (long)blockIdx.x * RB + threadIdx.x / NT; row < rows; row += (long)gridDim.x * RB) {
     f32x4 v[NV], d[NV];
-    load_row<NT, NV, VEC>(v, x + row * cols, cols, t);
-    load_row<NT, NV, VEC>(d, dy + row * cols, cols, t);
+    load_row<NT, NV, TAIL>(v, x + row * cols, cols, t);
+    load_row<NT, NV, TAIL>(d, dy + row * cols, cols, t);
     const float mu = mean[row], r = rstd[row];
     f32x4 g[NV];
-    if (w) load_row<NT, NV, VEC>(g, w, cols, t);
+    if (w) load_row<NT, NV, TAIL>(g, w, cols, t);
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; n++)
@@ -178,7 +176,7 @@ __global__ void __launch_bounds__(threads_of(NT))
       for (int n = 0; n < NV; n++)
 #pragma unroll
         for (int j = 0; j < 4; j++) v[n][j] = r * (d[n][j] - s - v[n][j] * q);
-      store_row<NT, NV, VEC>(v, dx + row * cols, cols, t);
+      store_row<NT, NV, TAIL>(v, dx + row * cols, cols, t);
     }
   }
   if (!part) return;
@@ -198,7 +196,7 @@ __global__ void __launch_bounds__(threads_of(NT))
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int c = col_of<NT, VEC>(n, j, t);
+        const int c = col_of<NT>(n, t) + j;
         if (c < cols) out[(long)p * cols + c] = a[j];
       }
     }
@@ -343,15 +341,14 @@ extern "C" int tt_k_layernorm_fwd(const float *x, const float *w, const float *b
                        x, w, b, y, mean, rstd, rows, cols, eps);
     return launched();
   }
-  const bool vec = cols % 4 == 0 && a16(x) && a16(y) && a16(w) && a16(b);
   const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols);
   const unsigned grid = (unsigned)(groups < 1 << 20 ? groups : 1 << 20);
 #define RUN(NT, NV)                                                                                            \
-  if (vec)                                                                                                     \
-    hipLaunchKernelGGL((ln_fwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, b, y, \
+  if (cols % 4 == 0)                                                                                                    \
+    hipLaunchKernelGGL((ln_fwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, b, y, \
                        mean, rstd, rows, (int)cols, eps);                                                      \
   else                                                                                                         \
-    hipLaunchKernelGGL((ln_fwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, b, y, \
+    hipLaunchKernelGGL((ln_fwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, b, y, \
                        mean, rstd, rows, (int)cols, eps)
   BY_COLS(RUN)
 #undef RUN
@@ -383,16 +380,15 @@ extern "C" int tt_k_layernorm_bwd(const float *x, const float *w, const float *d
       hipLaunchKernelGGL(ln_cols_long_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)blocks), dim3(256), 0,
                          stream(), x, dy, mean, rstd, part, rows, cols);
   } else {
-    const bool vec = cols % 4 == 0 && a16(x) && a16(dy) && a16(w) && a16(dx);
     // without sums every row group has a workgroup of its own
     const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols);
     const unsigned grid = part ? (unsigned)blocks : (unsigned)(groups < 1 << 20 ? groups : 1 << 20);
 #define RUN(NT, NV)                                                                                           \
-  if (vec)                                                                                                    \
-    hipLaunchKernelGGL((ln_bwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, dy, \
+  if (cols % 4 == 0)                                                                                                   \
+    hipLaunchKernelGGL((ln_bwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, dy, \
                        mean, rstd, dx, part, rows, (int)cols);                                                \
   else                                                                                                        \
-    hipLaunchKernelGGL((ln_bwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, dy, \
+    hipLaunchKernelGGL((ln_bwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, dy, \
                        mean, rstd, dx, part, rows, (int)cols)
     BY_COLS(RUN)
 #undef RUN

@@ -18,10 +18,10 @@
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;  // in memory, at any float
 
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
-inline bool a16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr int MAX_PAIRS = TT_ROPE_MAX_DIM / 2;
 
@@ -38,7 +38,7 @@ template <int V>
 __device__ __forceinline__ Vals<V> get(const float *p) {
   Vals<V> x;
   if (V == 4) {
-    const f32x4 t = *(const f32x4 *)p;
+    const f32x4 t = *(const f32x4_any *)p;
 #pragma unroll
     for (int j = 0; j < V; j++) x.v[j] = t[j];
   } else {
@@ -52,7 +52,7 @@ template <int V>
 __device__ __forceinline__ void put(float *p, const Vals<V> &x) {
   if (V == 4) {
     const f32x4 t = {x.v[0], x.v[V > 1], x.v[V > 2 ? 2 : 0], x.v[V > 3 ? 3 : 0]};
-    *(f32x4 *)p = t;
+    *(f32x4_any *)p = t;
   } else {
 #pragma unroll
     for (int j = 0; j < V; j++) p[j] = x.v[j];
@@ -193,8 +193,7 @@ extern "C" int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_
   const float sign = transpose ? -1.f : 1.f, mag = r->magnitude != 0 ? (float)r->magnitude : 1.f;
   const dim3 grid((unsigned)((rows + n - 1) / n));
   const size_t lds = sizeof(float2) * n * pairs;
-  const bool vec = pairs % 4 == 0 && r->head_dim % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && a16(x) && a16(y);
-  if (vec)
+  if (pairs % 4 == 0 && r->head_dim % 4 == 0)
     hipLaunchKernelGGL(rope_kernel<4>, grid, dim3(256), lds, stream(), t, x, y, positions, rows, seq_len, heads,
                        r->head_dim, pairs, r->interleaved != 0, ldx, ldy, sign, mag, (int)n);
   else
