@@ -1,7 +1,3 @@
-#ifndef FEW_C
-#define FEW_C 0
-#define FEW_NW 4
-#endif
 // Attention on the fp32 matrix units: forward, the form for few query rows,
 // and the backward pass, which recomputes the probabilities.
 //
@@ -48,9 +44,6 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
-// waves a SIMD that the registers are held to: as many as do without spilling
-#define FWD_WAVES(DB) ((DB) == 8 ? 4 : 3)
-#define DQ_WAVES(DB) ((DB) <= 4 ? 4 : (DB) <= 6 ? 3 : 2)
 
 struct Strides {
   long b, r, h;  // elements from a sequence / row / head to the next
@@ -130,10 +123,10 @@ __device__ __forceinline__ Span span_of(const Args &a, const Seq &q, int i0, int
   return s;
 }
 
-// the same for the 16 packed rows of a wave from r0 on
+// the same for the 32 packed rows of a wave from r0 on
 __device__ __forceinline__ Span wave_span(const Args &a, const Seq &q, int r0, int r1) {
   if (r0 >= r1) return Span{0, 0, 0, 0};
-  return span_of(a, q, r0 / a.G, ((r0 + 16 < r1 ? r0 + 16 : r1) - 1) / a.G);
+  return span_of(a, q, r0 / a.G, ((r0 + 32 < r1 ? r0 + 32 : r1) - 1) / a.G);
 }
 
 // Workgroups start in the order of blockIdx, 256 CUs at a time, and under a
@@ -187,63 +180,6 @@ struct Cols {
 
 __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-// Operands go from LDS to registers one step ahead of the products that use
-// them, and no further: left alone, the compiler moves every read of an
-// unrolled loop to its front and runs out of registers.
-__device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
-
-// s[n] += the tile's rows 16 n + lane % 16 times b, over DB blocks of 16 columns
-template <int DB>
-__device__ __forceinline__ void dots(f32x4 (&s)[2], const f32x4 (&b)[DB], const float *x, int ld, int lane) {
-  const float *p = x + (lane & 15) * ld + 4 * (lane >> 4);
-  f32x4 cur[2], nxt[2];
-  cur[0] = *(const f32x4 *)p;
-  cur[1] = *(const f32x4 *)(p + 16 * ld);
-#pragma unroll
-  for (int u = 0; u < DB; u++) {
-    if (u + 1 < DB) {
-      nxt[0] = *(const f32x4 *)(p + 16 * (u + 1));
-      nxt[1] = *(const f32x4 *)(p + 16 * ld + 16 * (u + 1));
-    }
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      s[0] = mfma(cur[0][c], b[u][c], s[0]);
-      s[1] = mfma(cur[1][c], b[u][c], s[1]);
-    }
-    step_end();
-    cur[0] = nxt[0];
-    cur[1] = nxt[1];
-  }
-}
-
-// acc (columns d of row l % 16) += sum over the tile's rows k of w[k][l % 16] x[k][d]
-template <int DB, int NB>
-__device__ __forceinline__ void product(f32x4 (&acc)[DB], const f32x4 (&w)[NB], const float *x, int ld,
-                                        int lane) {
-  constexpr int VW = Cols<DB>::VW, T = Cols<DB>::T;
-  typedef typename Vec<VW>::T V;
-  const float *p = x + 4 * (lane >> 4) * ld + VW * (lane & 15);
-  V cur[T], nxt[T];
-#pragma unroll
-  for (int t = 0; t < T; t++) cur[t] = *(const V *)(p + 16 * VW * t);
-#pragma unroll
-  for (int k = 0; k < 4 * NB; k++) {
-    if (k + 1 < 4 * NB) {
-#pragma unroll
-      for (int t = 0; t < T; t++)
-        nxt[t] = *(const V *)(p + ((k + 1) / 4 * 16 + (k + 1) % 4) * ld + 16 * VW * t);
-    }
-#pragma unroll
-    for (int t = 0; t < T; t++)
-#pragma unroll
-      for (int c = 0; c < VW; c++)
-        acc[t * VW + c] = mfma(Vec<VW>::at(cur[t], c), w[k / 4][k % 4], acc[t * VW + c]);
-    step_end();
-#pragma unroll
-    for (int t = 0; t < T; t++) cur[t] = nxt[t];
-  }
 }
 
 // One query (or key) at a time, its values over the lanes (two each): what a
@@ -328,53 +264,238 @@ __device__ __forceinline__ int small_div(int x, int G, unsigned magic) {
   return G >= KT ? x >= G : (int)((unsigned)x * magic >> 16);
 }
 
-// the rows [0, KT) from `base` on, on their way to LDS: NV float4 a thread of
-// NT; rows from `left` on are zeros
-template <int DB, int NT>
-struct Stage {
-  static constexpr int C4 = DB * 4;                         // float4 a row
-  static constexpr int NV = (KT * C4 + NT - 1) / NT;
-  static constexpr int LD = DB * 16 + 4;  // rows 4 banks apart: 16-byte reads of 8 rows meet all 32 banks
-  f32x4 v[NV];
-  __device__ __forceinline__ void load(const float *base, int stride, int left, int D, int vec, int tid) {
-    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
+// ---------------------------------------------------------------- fp32 products in bf16 parts
+//
+// The fp32 matrix instructions run at 1/16 of the bf16 ones.  An fp32 value is
+// the sum of three bf16 values, x = x1 + x2 + x3, cut from its 24 significant
+// bits eight at a time (each difference is exact), and of the nine products of
+// two such values the six
+//   x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1
+// leave out at most 2^-21 of |x y|, 2^-24 on average and in proportion to x y
+// itself: less than the roundings of an fp32 sum of a few terms.  Each bf16
+// product is exact and added in fp32.  So the matrix units do an fp32 product in
+// 6/16 of their time.  An infinity has no such parts: it comes out as NaN.
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
+// the leading parts of two values, the first in the low half
+__device__ __forceinline__ unsigned lead(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+// what the leading part leaves
+__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
+struct Parts {
+  u32x4 p[3];  // eight values: part 1, 2 and 3
+};
+__device__ __forceinline__ Parts parts_of(float (&x)[8]) {
+  Parts r;
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = e / C4;
-      v[n] = get4(r, row * stride, (e % C4) * 4, (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
+  for (int n = 0; n < 3; n++) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) r.p[n][j] = lead(x[2 * j], x[2 * j + 1]);
+    if (n < 2) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = rest(x[j]);
     }
+  }
+  return r;
+}
+
+// The 32x32x16 product: A holds row lane % 32 and B column lane % 32, both at
+// eight summed indices of their lane / 32; C holds column lane % 32, rows
+// 8 (r / 4) + 4 (lane / 32) + r % 4 in register r.  DU: steps of 16 columns of a
+// head; its rows are held as DU of them, its transposed results as DO blocks of
+// 32 of DP columns.
+template <int DU>
+struct Dim {
+  static constexpr int DO = (DU + 1) / 2, DP = 32 * DO, C4 = DP / 4;
+  // a row's parts in LDS: 2 DU units of eight values and one left free, an odd
+  // number, so that neighbouring rows start on other banks
+  static constexpr int RU = 2 * DU + 1;
+  static constexpr int ROWS = KT * RU * 16;       // bytes a part, rows as they are
+  static constexpr int COLS = 4 * DP * 16;        // bytes a part, transposed
+};
+
+// 4 x 4 blocks of a tile of KT rows on their way from memory to LDS: rows 4 j ..
+// 4 j + 3, columns 4 c .. 4 c + 3 of a thread
+template <int DU>
+struct Block {
+  f32x4 v[4];
+  __device__ __forceinline__ void load(const float *base, int stride, int left, int D, int vec, int task) {
+    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
+    const int j = task / Dim<DU>::C4, c = task % Dim<DU>::C4;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = get4(r, (4 * j + e) * stride, 4 * c, 4 * j + e < left, D, vec);
   }
   // packed query rows, r = i * G + member, from member `m0` of the query at `base` on
   __device__ __forceinline__ void load_rows(const float *base, int rs, int hs, int G, unsigned magic, int m0, int left,
-                                            int D, int vec, int tid) {
+                                            int D, int vec, int task) {
     const __amdgpu_buffer_rsrc_t r = buffer_of(base);
+    const int j = task / Dim<DU>::C4, c = task % Dim<DU>::C4;
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = e / C4, i = small_div(m0 + row, G, magic);
-      v[n] = get4(r, i * rs + (m0 + row - i * G) * hs, (e % C4) * 4,
-                  (KT * C4 % NT == 0 || e < KT * C4) && row < left, D, vec);
-    }
-  }
-  __device__ __forceinline__ void store(float *lds, int tid) const {
-#pragma unroll
-    for (int n = 0; n < NV; n++) {
-      const int e = tid + n * NT, row = e / C4, c = (e % C4) * 4;
-      if (KT * C4 % NT == 0 || e < KT * C4) *(f32x4 *)(lds + row * LD + c) = v[n];
+    for (int e = 0; e < 4; e++) {
+      const int i = small_div(m0 + 4 * j + e, G, magic);
+      v[e] = get4(r, i * rs + (m0 + 4 * j + e - i * G) * hs, 4 * c, 4 * j + e < left, D, vec);
     }
   }
   __device__ __forceinline__ bool odd() const {  // holds an infinity or a NaN
     float t = 0.f;
 #pragma unroll
-    for (int n = 0; n < NV; n++)
+    for (int e = 0; e < 4; e++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) t = fmaf(v[n][j], 0.f, t);
+      for (int j = 0; j < 4; j++) t = fmaf(v[e][j], 0.f, t);
     return t != t;
+  }
+  // The parts to LDS, as rows (`rows`) and transposed (`cols`), either NULL.
+  // Transposed, a unit of eight summed indices (rows 16 t + 4 h + {0 .. 3, 8 ..
+  // 11}: what a lane of half h holds of a product's registers 8 t .. 8 t + 7)
+  // of column d = 4 c + e lies at place C4 e + c, so that neighbouring threads
+  // write and neighbouring lanes read neighbouring units.
+  template <bool AS_ROWS, bool AS_COLS>
+  __device__ __forceinline__ void store(char *rows, char *cols, int task) {
+    typedef Dim<DU> M;
+    const int j = task / M::C4, c = task % M::C4;
+    char *pr = rows + 4 * j * M::RU * 16 + c * 8;
+    char *pc = cols + ((j / 4 * 2 + j % 2) * M::DP + c) * 16 + j % 4 / 2 * 8;
+    const bool in = M::DP == 16 * DU || c < 4 * DU;
+#pragma unroll
+    for (int n = 0; n < 3; n++) {
+      if (AS_ROWS && in) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          *(u32x2 *)(pr + n * M::ROWS + e * M::RU * 16) = (u32x2){lead(v[e][0], v[e][1]), lead(v[e][2], v[e][3])};
+      }
+      if (AS_COLS) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          *(u32x2 *)(pc + n * M::COLS + e * M::C4 * 16) = (u32x2){lead(v[0][e], v[1][e]), lead(v[2][e], v[3][e])};
+      }
+      if (n < 2) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) v[e][k] = rest(v[e][k]);
+      }
+    }
   }
 };
 
+// Operands go from LDS to registers one step ahead of the products that use
+// them, and no further: left alone, the compiler moves every read of an
+// unrolled loop to its front and runs out of registers.
+__device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
+
+__device__ __forceinline__ Parts read_parts(const char *p, int part) {
+  Parts r;
+#pragma unroll
+  for (int n = 0; n < 3; n++) r.p[n] = *(const u32x4 *)(p + n * part);
+  return r;
+}
+
+// the tile's rows times this lane's row, columns 16 u + 8 h + ..: the six
+// products in two chains, so that none waits for the one before it
+template <int DU>
+__device__ __forceinline__ f32x16 dots(const char *rows, const Parts (&b)[DU], int lane) {
+  typedef Dim<DU> M;
+  const char *p = rows + (lane & 31) * M::RU * 16 + (lane >> 5) * 16;
+  f32x16 s = {}, t = {};
+  Parts a = read_parts(p, M::ROWS), next = a;
+#pragma unroll
+  for (int u = 0; u < DU; u++) {
+    if (u + 1 < DU) next = read_parts(p + (u + 1) * 32, M::ROWS);
+    s = mma(a.p[0], b[u].p[0], s);
+    t = mma(a.p[0], b[u].p[1], t);
+    s = mma(a.p[1], b[u].p[0], s);
+    t = mma(a.p[1], b[u].p[1], t);
+    s = mma(a.p[0], b[u].p[2], s);
+    t = mma(a.p[2], b[u].p[0], t);
+    step_end();
+    a = next;
+  }
+  return s + t;
+}
+
+// acc (the columns of block b at rows l % 32) += sum over the tile's rows k of
+// x[k][column] w[k][l % 32], w the registers of a product with these rows
+template <int DU>
+__device__ __forceinline__ void product(f32x16 (&acc)[Dim<DU>::DO], const f32x16 &w, const char *cols, int lane) {
+  typedef Dim<DU> M;
+  constexpr int DO = M::DO;
+  const char *p = cols + ((lane >> 5) * M::DP + (lane & 31)) * 16;
+  Parts a = read_parts(p, M::COLS), next = a, b;
+#pragma unroll
+  for (int n = 0; n < 2 * DO; n++) {
+    const int t = n / DO, o = n % DO;
+    if (o == 0) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = w[8 * t + e];
+      b = parts_of(x);
+    }
+    if (n + 1 < 2 * DO) next = read_parts(p + ((n + 1) / DO * 2 * M::DP + (n + 1) % DO * 32) * 16, M::COLS);
+    acc[o] = mma(a.p[0], b.p[0], acc[o]);
+    acc[o] = mma(a.p[0], b.p[1], acc[o]);
+    acc[o] = mma(a.p[1], b.p[0], acc[o]);
+    acc[o] = mma(a.p[1], b.p[1], acc[o]);
+    acc[o] = mma(a.p[0], b.p[2], acc[o]);
+    acc[o] = mma(a.p[2], b.p[0], acc[o]);
+    step_end();
+    a = next;
+  }
+}
+
+// this lane's row p[0 .. D) times f as parts, columns 16 u + 8 h + ..
+template <int DU>
+__device__ __forceinline__ void load_parts(Parts (&b)[DU], const float *p, bool in, float f, int D, int vec, int lane) {
+#pragma unroll
+  for (int u = 0; u < DU; u++) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (in) v = load4(p, 16 * u + 8 * (lane >> 5) + 4 * k, D, vec);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[4 * k + j] = v[j] * f;
+    }
+    b[u] = parts_of(x);
+  }
+}
+
+// row p[0 .. D) = f * the columns that acc holds of this lane's row: register
+// 4 q + i of the place 32 o + 8 q + 4 h + i, column 4 c + e at place C4 e + c
+template <int DU>
+__device__ __forceinline__ void store_columns(float *p, const f32x16 (&acc)[Dim<DU>::DO], float f, int D, int vec,
+                                              int lane) {
+  constexpr int C4 = Dim<DU>::C4;
+#pragma unroll
+  for (int q = 0; q < Dim<DU>::DO; q++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int d = 4 * (8 * q + 4 * (lane >> 5) + i);
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = acc[(C4 * e + 8 * q) / 32][(C4 * e + 8 * q) % 32 / 2 + i] * f;
+      if (vec) {
+        if (d < D) *(f32x4_any *)(p + d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (d + e < D) p[d + e] = v[e];
+      }
+    }
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// over the four lanes that hold a column
+// over the four lanes that hold a column of a 16-column product
 __device__ __forceinline__ float col_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -386,12 +507,12 @@ __device__ __forceinline__ float col_sum(float x) {
 
 // ---------------------------------------------------------------- forward
 
-// 16 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
+// 32 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
 __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, int k0, int k1,
                                                const float *q, const float *k, const float *v, float *o, float *lse,
                                                float *ws_ml, float *ws_o, int width, int lane) {
 #pragma unroll 1
-  for (int row = first; row < first + 16 && row < r1; row++) {
+  for (int row = first; row < first + 32 && row < r1; row++) {
     const int i = row / a.G, hm = row - i * a.G;
     Range rg = range_of(a, sq, i);
     if (rg.lo < k0) rg.lo = k0;
@@ -426,110 +547,122 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
   }
 }
 
-// One workgroup of NW waves: 16 NW packed rows (16 a wave) of one key head
-// against the keys they see, KT at a time through LDS: a tile is loaded to
-// registers while the one before it is used, and goes to the other half of the
-// LDS behind that (one barrier a tile).  With splits > 1 it takes `chunk` keys
-// of them and leaves maximum, sum and the unscaled result to the join.
-template <int DB, int NW>
-__global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
+// One workgroup: 128 packed rows (32 a wave) of one key head against the keys
+// they see, KT at a time through LDS.  A tile is on its way to registers while
+// the one before it is used, and goes to LDS as parts between two barriers; two
+// workgroups a CU cover each other's.  With splits > 1 it takes `chunk` keys of
+// them and leaves maximum, sum and the unscaled result to the join.
+template <int DU>
+__global__ void __launch_bounds__(256, 2)
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
-  typedef Stage<DB, 64 * NW> S;
-  __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
-  constexpr int ROWS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  typedef Dim<DU> M;
+  __shared__ __attribute__((aligned(16))) char lk[3 * M::ROWS], lv[3 * M::COLS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   // the last rows see the most keys under a causal mask: they start first
   const int tile = gridDim.x / nbh - 1 - at0 / nbh;
-  const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
+  const int r0 = tile * 128, r1 = r0 + 128 < a.R ? r0 + 128 : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
-  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
+  const Span mine = wave_span(a, sq, r0 + wave * 32, r1);
   int k_first = sp.lo / KT * KT, k_end = sp.hi;
   if (a.splits > 1) {
     const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
     if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
     if (c1 < k_end) k_end = (int)c1;
   }
-  const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
+  const int row = r0 + wave * 32 + (lane & 31), i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
   Range rg = {0, 0};
   if (in) rg = range_of(a, sq, i);
-  f32x4 qf[DB], acc[DB];
-  float mx = -INFINITY, sum = 0.f;
   const float *qp0 = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
-  const float *qp = qp0 + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h;
-#pragma unroll
-  for (int u = 0; u < DB; u++) {
-    qf[u] = acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (in) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
-  }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
-  S sk, sv;
+  // the tile's blocks: keys, then values
+  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
+  Block<DU> block[NB];
   bool odd = false;
-  if (k_first < k_end) {
-    sk.load(kp + (long)k_first * a.k.r, (int)a.k.r, k_end - k_first, a.D, a.vec, tid);
-    sv.load(vp + (long)k_first * a.v.r, (int)a.v.r, k_end - k_first, a.D, a.vec, tid);
-    sk.store(lk[0], tid);
-    sv.store(lv[0], tid);
-    odd = __syncthreads_or(sv.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
-  }
-  int buf = 0;
-  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
-    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
-    if (odd) break;
-    if (more) {
-      sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
-      sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (t < TASKS)
+        block[n].load(kp + (long)k0 * a.k.r, (int)a.k.r, k_end - k0, a.D, a.vec, t);
+      else if (t < 2 * TASKS)
+        block[n].load(vp + (long)k0 * a.v.r, (int)a.v.r, k_end - k0, a.D, a.vec, t - TASKS);
     }
+  };
+  auto store = [&](bool look) {
+    bool found = false;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (t < TASKS) {
+        block[n].template store<true, false>(lk, lv, t);
+      } else if (t < 2 * TASKS) {
+        if (look) found |= block[n].odd();
+        block[n].template store<false, true>(lk, lv, t - TASKS);
+      }
+    }
+    if (look)
+      odd = __syncthreads_or(found);
+    else
+      __syncthreads();
+  };
+  auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
+  if (k_first < k_end) load(k_first);
+  Parts qf[DU];
+  f32x16 acc[M::DO];
+  float mx = -INFINITY, sum = 0.f;
+  load_parts<DU>(qf, qp0 + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, in, a.scale * LOG2E, a.D, a.vec, lane);
+#pragma unroll
+  for (int n = 0; n < M::DO; n++) acc[n] = (f32x16){};
+  if (k_first < k_end) store(is_mixed(k_first));
+  for (int k0 = k_first; k0 < k_end; k0 += KT) {
+    const bool mixed = is_mixed(k0), more = k0 + KT < k_end;
+    if (odd) break;
+    if (more) load(k0 + KT);
     if (k0 < mine.hi && k0 + KT > mine.lo) {  // this wave's rows see some of the tile
-      f32x4 s[2];
-      s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      dots<DB>(s, qf, lk[buf], S::LD, lane);
+      f32x16 s = dots<DU>(lk, qf, lane);
       if (mixed) {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int key = k0 + kb * 16 + 4 * g + r;
-            if (key < rg.lo || key >= rg.hi) s[kb][r] = -INFINITY;
-          }
+        for (int r = 0; r < 16; r++) {
+          const int key = k0 + 8 * (r / 4) + 4 * g + r % 4;
+          if (key < rg.lo || key >= rg.hi) s[r] = -INFINITY;
+        }
       }
-      float t = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      t = fmaxf(col_max(t), mx);
+      float t = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; r++) t = fmaxf(t, s[r]);
+      t = fmaxf(fmaxf(t, __shfl_xor(t, 32)), mx);
       const float base = t == -INFINITY ? 0.f : t;
       if (__any(t > mx)) {
         const float f = exp2_fast(mx - base);
         sum *= f;
 #pragma unroll
-        for (int u = 0; u < DB; u++) acc[u] *= f;
+        for (int n = 0; n < M::DO; n++) acc[n] *= f;
         mx = t;
       }
 #pragma unroll
-      for (int kb = 0; kb < 2; kb++)
+      for (int r = 0; r < 16; r++) s[r] = exp2_fast(s[r] - base);
+      float u[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) s[kb][r] = exp2_fast(s[kb][r] - base);
-      sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-      product<DB, 2>(acc, s, lv[buf], S::LD, lane);
+      for (int r = 0; r < 4; r++) u[r] = (s[r] + s[r + 4]) + (s[r + 8] + s[r + 12]);
+      sum += (u[0] + u[1]) + (u[2] + u[3]);
+      product<DU>(acc, s, lv, lane);
     }
     if (more) {
-      sk.store(lk[buf ^ 1], tid);
-      sv.store(lv[buf ^ 1], tid);
-      if (k0 + KT < sp.ilo || k0 + 2 * KT > sp.ihi)
-        odd = __syncthreads_or(sv.odd());
-      else
-        __syncthreads();
+      __syncthreads();
+      store(is_mixed(k0 + KT));
     }
   }
   if (odd) {
-    fwd_one_by_one(a, sq, b, h, r0 + wave * 16, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, DB * 16, lane);
+    fwd_one_by_one(a, sq, b, h, r0 + wave * 32, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, M::DP, lane);
     return;
   }
 
-  const float total = col_sum(sum);
+  const float total = sum + __shfl_xor(sum, 32);
   if (!in) return;
   if (a.splits > 1) {
     const long at = ((long)blockIdx.y * nbh + bh) * a.R + row;
@@ -537,13 +670,13 @@ __global__ void __launch_bounds__(64 * NW, FWD_WAVES(DB))
       ws_ml[2 * at] = mx;
       ws_ml[2 * at + 1] = total;
     }
-    store_row<DB>(ws_o + at * (DB * 16), acc, 1.f, DB * 16, 1, lane);
+    store_columns<DU>(ws_o + at * M::DP, acc, 1.f, M::DP, 1, lane);
     return;
   }
   if (lse && g == 0)
     lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (mx + log2f(total)) * LN2;
-  store_row<DB>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc, total == 0.f ? 0.f : 1.f / total,
-                a.D, a.vec, lane);
+  store_columns<DU>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc, total == 0.f ? 0.f : 1.f / total,
+                    a.D, a.vec, lane);
 }
 
 // Few packed rows (one tile of 16): the keys pass once, from memory to
@@ -844,12 +977,12 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dq of 16 packed rows from `first` on
+// dq of 32 packed rows from `first` on
 __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, const float *q,
                                               const float *k, const float *v, const float *dout, const float *lse,
                                               const float *delta, float *dq, int lane) {
 #pragma unroll 1
-  for (int row = first; row < first + 16 && row < r1; row++) {
+  for (int row = first; row < first + 32 && row < r1; row++) {
     const int i = row / a.G, hq = h * a.G + row - i * a.G;
     const Range rg = range_of(a, sq, i);
     Pair acc = {0.f, 0.f};
@@ -873,29 +1006,26 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
   }
 }
 
-// dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
-// forward pass
-template <int DB, int NW>
-__global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
+// dq of 128 packed rows (32 a wave): the keys through LDS as rows and transposed,
+// the values as rows
+template <int DU>
+__global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
     attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ dout, const float *__restrict__ lse,
                    const float *__restrict__ delta, float *__restrict__ dq) {
-  typedef Stage<DB, 64 * NW> S;
-  __shared__ __attribute__((aligned(16))) float lk[2][KT * S::LD], lv[2][KT * S::LD];
-  constexpr int ROWS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  typedef Dim<DU> M;
+  __shared__ __attribute__((aligned(16))) char lk[3 * M::ROWS], lkt[3 * M::COLS], lv[3 * M::ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   const int tile = gridDim.x / nbh - 1 - at0 / nbh;
-  const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
+  const int r0 = tile * 128, r1 = r0 + 128 < a.R ? r0 + 128 : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
-  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
-  const int row = r0 + wave * 16 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
-  const bool in = row < a.R;
+  const Span mine = wave_span(a, sq, r0 + wave * 32, r1);
+  const int row = r0 + wave * 32 + (lane & 31), i = row / a.G, hq = h * a.G + row - i * a.G;
+  const bool in = row < a.R, live = in && i < sq.queries;
   Range rg = {0, 0};
   float l2 = 0.f, dl = 0.f;
-  f32x4 qf[DB], df[DB], acc[DB];
-  const bool live = in && i < sq.queries;
   if (live) {
     rg = range_of(a, sq, i);
     const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
@@ -903,64 +1033,72 @@ __global__ void __launch_bounds__(64 * NW, DQ_WAVES(DB))
     if (l2 == -INFINITY) l2 = 0.f;  // no key has weight: exp2(-inf - 0) = 0
     dl = delta[at];
   }
-#pragma unroll
-  for (int u = 0; u < DB; u++) {
-    qf[u] = df[u] = acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      qf[u] = load4(q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, 16 * u + 4 * g, a.D, a.vec) *
-              (a.scale * LOG2E);
-      df[u] = load4(dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, 16 * u + 4 * g, a.D, a.vec);
-    }
-  }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
-  S sk, sv;
   const int k_first = sp.lo / KT * KT, k_end = sp.hi;
+  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
+  Block<DU> block[NB];
   bool odd = false;
-  if (k_first < k_end) {
-    sk.load(kp + (long)k_first * a.k.r, (int)a.k.r, k_end - k_first, a.D, a.vec, tid);
-    sv.load(vp + (long)k_first * a.v.r, (int)a.v.r, k_end - k_first, a.D, a.vec, tid);
-    sk.store(lk[0], tid);
-    sv.store(lv[0], tid);
-    odd = __syncthreads_or(sk.odd()) && (k_first < sp.ilo || k_first + KT > sp.ihi);
-  }
-  int buf = 0;
-  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
-    const bool mixed = k0 < sp.ilo || k0 + KT > sp.ihi, more = k0 + KT < k_end;
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (t < TASKS)
+        block[n].load(kp + (long)k0 * a.k.r, (int)a.k.r, k_end - k0, a.D, a.vec, t);
+      else if (t < 2 * TASKS)
+        block[n].load(vp + (long)k0 * a.v.r, (int)a.v.r, k_end - k0, a.D, a.vec, t - TASKS);
+    }
+  };
+  auto store = [&](bool look) {
+    bool found = false;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (t < TASKS) {
+        if (look) found |= block[n].odd();
+        block[n].template store<true, true>(lk, lkt, t);
+      } else if (t < 2 * TASKS) {
+        block[n].template store<true, false>(lv, lkt, t - TASKS);
+      }
+    }
+    if (look)
+      odd = __syncthreads_or(found);
+    else
+      __syncthreads();
+  };
+  auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
+  if (k_first < k_end) load(k_first);
+  Parts qf[DU], df[DU];
+  f32x16 acc[M::DO];
+  load_parts<DU>(qf, q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, live, a.scale * LOG2E, a.D, a.vec, lane);
+  load_parts<DU>(df, dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, live, 1.f, a.D, a.vec, lane);
+#pragma unroll
+  for (int n = 0; n < M::DO; n++) acc[n] = (f32x16){};
+  if (k_first < k_end) store(is_mixed(k_first));
+  for (int k0 = k_first; k0 < k_end; k0 += KT) {
+    const bool mixed = is_mixed(k0), more = k0 + KT < k_end;
     if (odd) break;
-    if (more) {
-      sk.load(kp + (long)(k0 + KT) * a.k.r, (int)a.k.r, k_end - k0 - KT, a.D, a.vec, tid);
-      sv.load(vp + (long)(k0 + KT) * a.v.r, (int)a.v.r, k_end - k0 - KT, a.D, a.vec, tid);
-    }
+    if (more) load(k0 + KT);
     if (k0 < mine.hi && k0 + KT > mine.lo) {
-      f32x4 s[2], dp[2];
+      f32x16 s = dots<DU>(lk, qf, lane), dp = dots<DU>(lv, df, lane);
 #pragma unroll
-      for (int kb = 0; kb < 2; kb++) s[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      dots<DB>(s, qf, lk[buf], S::LD, lane);
-      dots<DB>(dp, df, lv[buf], S::LD, lane);
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int key = k0 + kb * 16 + 4 * g + r;
-          const float x = exp2_fast(s[kb][r] - l2) * (dp[kb][r] - dl);
-          s[kb][r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
-        }
-      product<DB, 2>(acc, s, lk[buf], S::LD, lane);
+      for (int r = 0; r < 16; r++) {
+        const int key = k0 + 8 * (r / 4) + 4 * g + r % 4;
+        const float x = exp2_fast(s[r] - l2) * (dp[r] - dl);
+        s[r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
+      }
+      product<DU>(acc, s, lkt, lane);
     }
     if (more) {
-      sk.store(lk[buf ^ 1], tid);
-      sv.store(lv[buf ^ 1], tid);
-      if (k0 + KT < sp.ilo || k0 + 2 * KT > sp.ihi)
-        odd = __syncthreads_or(sk.odd());
-      else
-        __syncthreads();
+      __syncthreads();
+      store(is_mixed(k0 + KT));
     }
   }
   if (odd) {
-    dq_one_by_one(a, sq, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
+    dq_one_by_one(a, sq, b, h, r0 + wave * 32, r1, q, kp, vp, dout, lse, delta, dq, lane);
     return;
   }
-  if (in) store_row<DB>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
+  if (in)
+    store_columns<DU>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
 }
 
 // the packed rows that see a key of [k0, k1)
@@ -982,14 +1120,14 @@ __device__ __forceinline__ Rows rows_of(const Args &a, const Seq &s, int k0, int
   return r;
 }
 
-// dk and dv of 16 keys from `first` on, from the packed rows [r0, r1)
+// dk and dv of 32 keys from `first` on, from the packed rows [r0, r1)
 __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, int b, int h, int first, int r0, int r1,
                                                const float *q, const float *k, const float *v, const float *dout,
                                                const float *lse, const float *delta, float *dk, float *dv, float *ws,
                                                int width, int lane) {
   const int keys = seq.keys;
 #pragma unroll 1
-  for (int key = first; key < first + 16 && key < a.Lk; key++) {
+  for (int key = first; key < first + 32 && key < a.Lk; key++) {
     Pair ak = {0.f, 0.f}, av = {0.f, 0.f};
     const long ko = (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
     const long vo = (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
@@ -1024,25 +1162,26 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
   }
 }
 
-// dk and dv of 16 NW keys (16 a wave): the packed query rows that see any of
-// them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of
-// the rows and leaves its sums to the join: where many rows meet few keys, and
-// so that no fp32 sum runs over more rows than that.
-template <int DB, int NW>
-__global__ void __launch_bounds__(64 * NW, 2)
+// dk and dv of 128 keys (32 a wave): the packed query rows that see any of
+// them through LDS, q and do as rows and transposed.  With splits > 1 a
+// workgroup takes `chunk` of the rows and leaves its sums to the join: where
+// many rows meet few keys, and so that no fp32 sum runs over more rows than
+// that.
+template <int DU>
+__global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
     attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                     const float *__restrict__ dout, const float *__restrict__ lse,
                     const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
                     float *__restrict__ ws) {
-  typedef Stage<DB, 64 * NW> S;
-  __shared__ __attribute__((aligned(16))) float lq[2][KT * S::LD], ld[2][KT * S::LD], rl[2][KT], rd[2][KT];
-  __shared__ int rlo[2][KT], rhi[2][KT];
-  constexpr int KEYS = 16 * NW;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  typedef Dim<DU> M;
+  __shared__ __attribute__((aligned(16))) char lq[3 * M::ROWS], lqt[3 * M::COLS], ld[3 * M::ROWS], ldt[3 * M::COLS];
+  __shared__ __attribute__((aligned(16))) float rl[KT], rd[KT];
+  __shared__ int rlo[KT], rhi[KT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int k0 = at0 / nbh * KEYS, key = k0 + wave * 16 + m;
+  const int k0 = at0 / nbh * 128, kw = k0 + wave * 32, key = kw + (lane & 31);
   const Seq seq = seq_of(a, b);
-  Rows rows = rows_of(a, seq, k0, k0 + KEYS);
+  Rows rows = rows_of(a, seq, k0, k0 + 128);
   if (a.splits > 1) {
     const long c0 = rows.first + (long)blockIdx.y * a.chunk;
     if (c0 >= rows.end && blockIdx.y > 0) return;  // the join leaves it out
@@ -1050,20 +1189,10 @@ __global__ void __launch_bounds__(64 * NW, 2)
     rows.first = (int)c0;
   }
   const bool in = key < a.Lk, live = key < seq.keys;
-  f32x4 kf[DB], vf[DB], ak[DB], av[DB];
-  const float *kp = k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
-  const float *vp = v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
-#pragma unroll
-  for (int u = 0; u < DB; u++) {
-    kf[u] = vf[u] = ak[u] = av[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      kf[u] = load4(kp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
-      vf[u] = load4(vp, 16 * u + 4 * g, a.D, a.vec);
-    }
-  }
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
-  const float *dp_ = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
-  S sq, sd;
+  const float *op = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
+  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
+  Block<DU> block[NB];
   // row statistics of a tile, by the first KT threads
   float l2_ = 0.f, dl_ = 0.f;
   Range rg_ = {0, 0};
@@ -1074,9 +1203,15 @@ __global__ void __launch_bounds__(64 * NW, 2)
   auto load = [&](int r0) {
     t_i0 = i_next;
     t_i1 = i_next + small_div(m_next + KT - 1, a.G, magic);
-    const float *q0 = qp + (long)i_next * a.q.r, *d0 = dp_ + (long)i_next * a.o.r;
-    sq.load_rows(q0, (int)a.q.r, (int)a.q.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
-    sd.load_rows(d0, (int)a.o.r, (int)a.o.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
+    const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (t < TASKS)
+        block[n].load_rows(q0, (int)a.q.r, (int)a.q.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, t);
+      else if (t < 2 * TASKS)
+        block[n].load_rows(d0, (int)a.o.r, (int)a.o.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, t - TASKS);
+    }
     if (tid < KT) {
       const int e = m_next + tid, di = small_div(e, a.G, magic), i = i_next + di;
       l2_ = dl_ = 0.f;
@@ -1096,96 +1231,99 @@ __global__ void __launch_bounds__(64 * NW, 2)
       i_next++;
     }
   };
-  auto store = [&](int to) {
-    sq.store(lq[to], tid);
-    sd.store(ld[to], tid);
-    if (tid < KT) {
-      rl[to][tid] = l2_;
-      rd[to][tid] = dl_;
-      rlo[to][tid] = rg_.lo;
-      rhi[to][tid] = rg_.hi;
-    }
-  };
-  // whether a mask hides some of the tile's rows from some of the keys
-  bool next_touched = true;
-  const int kw = k0 + wave * 16;
-  auto is_mixed = [&](int r0) {
+  // mixed: a mask hides some of the tile's rows from some of the keys; touched:
+  // some of the rows see some of this wave's keys
+  bool odd = false, mixed = true, touched = true;
+  auto store = [&](int r0) {
     const Span sp = span_of(a, seq, t_i0, t_i1);
-    next_touched = kw < sp.hi && kw + 16 > sp.lo;
-    return r0 + KT > rows.end || k0 < sp.ilo || k0 + KEYS > sp.ihi;
+    touched = kw < sp.hi && kw + 32 > sp.lo;
+    mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + 128 > sp.ihi;
+    bool found = false;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int t = tid + n * 256;
+      if (mixed) found |= t < 2 * TASKS && block[n].odd();
+      if (t < TASKS)
+        block[n].template store<true, true>(lq, lqt, t);
+      else if (t < 2 * TASKS)
+        block[n].template store<true, true>(ld, ldt, t - TASKS);
+    }
+    if (tid < KT) {
+      rl[tid] = l2_;
+      rd[tid] = dl_;
+      rlo[tid] = rg_.lo;
+      rhi[tid] = rg_.hi;
+    }
+    if (mixed)
+      odd = __syncthreads_or(found);
+    else
+      __syncthreads();
   };
-  bool odd = false, mixed = true;
   if (rows.first < rows.end) {
     i_next = rows.first / a.G;
     m_next = rows.first - i_next * a.G;
     load(rows.first);
-    store(0);
-    mixed = is_mixed(rows.first);
-    odd = __syncthreads_or(sq.odd() || sd.odd()) && mixed;
   }
-  int buf = 0;
-  for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
-    const bool more = r0 + KT < rows.end, touched = next_touched;
+  Parts kf[DU], vf[DU];
+  f32x16 ak[M::DO], av[M::DO];
+  load_parts<DU>(kf, k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, live, a.scale * LOG2E, a.D, a.vec, lane);
+  load_parts<DU>(vf, v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, live, 1.f, a.D, a.vec, lane);
+#pragma unroll
+  for (int n = 0; n < M::DO; n++) ak[n] = av[n] = (f32x16){};
+  if (rows.first < rows.end) store(rows.first);
+  for (int r0 = rows.first; r0 < rows.end; r0 += KT) {
+    const bool more = r0 + KT < rows.end;
     if (odd) break;
     if (more) load(r0 + KT);
-    if (touched) {  // some of the rows see some of this wave's keys
-      f32x4 s[2], dp[2];
+    if (touched) {
+      f32x16 s = dots<DU>(lq, kf, lane), dp = dots<DU>(ld, vf, lane);
 #pragma unroll
-      for (int n = 0; n < 2; n++) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      dots<DB>(s, kf, lq[buf], S::LD, lane);
-      dots<DB>(dp, vf, ld[buf], S::LD, lane);
+      for (int n = 0; n < 4; n++) {
+        const f32x4 l2 = *(const f32x4 *)(rl + 8 * n + 4 * g), dl = *(const f32x4 *)(rd + 8 * n + 4 * g);
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const f32x4 l2 = *(const f32x4 *)(rl[buf] + n * 16 + 4 * g), dl = *(const f32x4 *)(rd[buf] + n * 16 + 4 * g);
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          float p = exp2_fast(s[n][r] - l2[r]), x = p * (dp[n][r] - dl[r]);
+        for (int j = 0; j < 4; j++) {
+          float p = exp2_fast(s[4 * n + j] - l2[j]), x = p * (dp[4 * n + j] - dl[j]);
           if (mixed) {
-            const int e = n * 16 + 4 * g + r;
-            if (key < rlo[buf][e] || key >= rhi[buf][e]) p = x = 0.f;
+            const int e = 8 * n + 4 * g + j;
+            if (key < rlo[e] || key >= rhi[e]) p = x = 0.f;
           }
-          s[n][r] = p;
-          dp[n][r] = x;
+          s[4 * n + j] = p;
+          dp[4 * n + j] = x;
         }
       }
-      product<DB, 2>(av, s, ld[buf], S::LD, lane);
-      product<DB, 2>(ak, dp, lq[buf], S::LD, lane);
+      product<DU>(av, s, ldt, lane);
+      product<DU>(ak, dp, lqt, lane);
     }
     if (more) {
-      store(buf ^ 1);
-      mixed = is_mixed(r0 + KT);
-      if (mixed)
-        odd = __syncthreads_or(sq.odd() || sd.odd());
-      else
-        __syncthreads();
+      __syncthreads();
+      store(r0 + KT);
     }
   }
   if (odd) {
-    dkv_one_by_one(a, seq, b, h, k0 + wave * 16, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, DB * 16,
-                   lane);
+    dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, M::DP, lane);
     return;
   }
   if (!in) return;
   if (a.splits > 1) {
     const long at = ((long)blockIdx.y * nbh + bh) * a.Lk + key, half = (long)a.splits * nbh * a.Lk;
-    store_row<DB>(ws + at * (DB * 16), ak, a.scale, DB * 16, 1, lane);
-    store_row<DB>(ws + (half + at) * (DB * 16), av, 1.f, DB * 16, 1, lane);
+    store_columns<DU>(ws + at * M::DP, ak, a.scale, M::DP, 1, lane);
+    store_columns<DU>(ws + (half + at) * M::DP, av, 1.f, M::DP, 1, lane);
     return;
   }
-  store_row<DB>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
-  store_row<DB>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
+  store_columns<DU>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
+  store_columns<DU>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
 }
 
 // the workgroups' sums of a key, added in their order; 32 lanes a key
 __global__ void __launch_bounds__(256)
-    attn_dkv_join_kernel(Args a, int width, int keys_a_group, const float *__restrict__ ws, float *__restrict__ dk,
+    attn_dkv_join_kernel(Args a, int width, const float *__restrict__ ws, float *__restrict__ dk,
                          float *__restrict__ dv) {
   const long nbh = (long)a.B * a.Hkv, all = nbh * a.Lk;
   const int lane = threadIdx.x & 31;
   for (long e = (long)blockIdx.x * 8 + (threadIdx.x >> 5); e < all; e += (long)gridDim.x * 8) {
     const int bh = (int)(e / a.Lk), key = (int)(e % a.Lk), b = bh / a.Hkv, h = bh % a.Hkv;
-    const int k0 = key / keys_a_group * keys_a_group;
-    const Rows rows = rows_of(a, seq_of(a, b), k0, k0 + keys_a_group);
+    const int k0 = key / 128 * 128;
+    const Rows rows = rows_of(a, seq_of(a, b), k0, k0 + 128);
     int parts = (rows.end - rows.first + a.chunk - 1) / a.chunk;
     if (parts < 1) parts = 1;
     if (4 * lane >= width) continue;
@@ -1216,7 +1354,7 @@ Strides packed(const TTStrides &s, long rows, int heads, int dim) {
   return p;
 }
 
-// 16-column blocks that the kernels hold for a head dimension
+// 16-column blocks that the kernel of few rows holds for a head dimension
 int blocks(int dim) {
   const int n = (dim + 15) / 16;
   return n == 7 ? 8 : n;
@@ -1224,7 +1362,6 @@ int blocks(int dim) {
 
 struct Plan {
   bool few;
-  int waves;   // of a workgroup, each with 16 rows
   int tiles;   // row (key gradients: key) tiles
   int splits, chunk;
   int width;   // floats a row of the parts takes
@@ -1263,27 +1400,20 @@ void split(Plan &p, long n, long want, long least, long step) {
   p.splits = (int)((n + c - 1) / c);
 }
 
-// Workgroups of 8 waves where two of them a CU are there, else of 4: tiles of
-// half the rows, which read the streamed operand twice as often.
 Plan plan_of(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
-  p.width = 16 * blocks(t->head_dim);
   p.few = R <= 16;
-#ifdef FW
-  p.waves = p.few ? 4 : FW;
-#else
-  p.waves = !p.few && (R + 127) / 128 * nbh >= 512 ? 8 : 4;
-#endif
   if (p.few) {
+    p.width = 16 * blocks(t->head_dim);
     p.tiles = 1;
     // parts of 64 to 1024 keys, about eight workgroups a CU
     long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
-    if (FEW_C > 0) c = FEW_C;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    p.tiles = (int)((R + 16 * p.waves - 1) / (16 * p.waves));
+    p.width = (t->head_dim + 31) / 32 * 32;
+    p.tiles = (int)((R + 127) / 128);
     split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
   }
   return p;
@@ -1292,15 +1422,10 @@ Plan plan_of(const TTAttention *t) {
 Plan dkv_plan(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
-  p.width = 16 * blocks(t->head_dim);
+  p.width = (t->head_dim + 31) / 32 * 32;
   p.few = false;
-#ifdef KW
-  p.waves = KW;
-#else
-  p.waves = (t->k_rows + 127) / 128 * nbh * (R < 512 ? 1 : R / 512) >= 512 ? 8 : 4;
-#endif
-  p.tiles = (int)((t->k_rows + 16 * p.waves - 1) / (16 * p.waves));
-  // fp32 sums over at most 2048 rows (16384 in one: 3.1e-6 off, in parts 1e-6)
+  p.tiles = (int)((t->k_rows + 127) / 128);
+  // fp32 sums over at most 2048 rows
   const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
   split(p, R, fill > sums ? fill : sums, 256, KT);
   return p;
@@ -1332,47 +1457,36 @@ Args args_of(const TTAttention *t) {
 }
 
 template <int DB>
+void run_few(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
+             float *ml, float *wo) {
+  hipLaunchKernelGGL((attn_few_kernel<DB, 4>), dim3((unsigned)(a.B * a.Hkv), (unsigned)p.splits), dim3(256), 0,
+                     stream(), a, q, k, v, o, lse, ml, wo);
+}
+
+template <int DU>
 void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
              float *ml, float *wo) {
-  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
-  if (p.few)
-    hipLaunchKernelGGL((attn_few_kernel<DB, FEW_NW>), grid, dim3(64 * FEW_NW), 0, stream(), a, q, k, v, o, lse, ml, wo);
-  else if (p.waves == 4)
-    hipLaunchKernelGGL((attn_fwd_kernel<DB, 4>), grid, dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
-  else
-    hipLaunchKernelGGL((attn_fwd_kernel<DB, 8>), grid, dim3(512), 0, stream(), a, q, k, v, o, lse, ml, wo);
+  hipLaunchKernelGGL(attn_fwd_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(256),
+                     0, stream(), a, q, k, v, o, lse, ml, wo);
 }
 
-template <int DB>
+template <int DU>
 void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
             const float *delta, float *dq) {
-  const long nbh = (long)a.B * a.Hkv;
-#ifdef DW
-  if (DW == 8)
-#else
-  if (((long)a.R + 127) / 128 * nbh >= 512)
-#endif
-    hipLaunchKernelGGL((attn_dq_kernel<DB, 8>), dim3((unsigned)(((long)a.R + 127) / 128 * nbh)), dim3(512), 0,
-                       stream(), a, q, k, v, dout, lse, delta, dq);
-  else
-    hipLaunchKernelGGL((attn_dq_kernel<DB, 4>), dim3((unsigned)(((long)a.R + 63) / 64 * nbh)), dim3(256), 0,
-                       stream(), a, q, k, v, dout, lse, delta, dq);
+  const long tiles = ((long)a.R + 127) / 128 * a.B * a.Hkv;
+  hipLaunchKernelGGL(attn_dq_kernel<DU>, dim3((unsigned)tiles), dim3(256), 0, stream(), a, q, k, v, dout, lse, delta,
+                     dq);
 }
 
-template <int DB>
+template <int DU>
 void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
              const float *lse, const float *delta, float *dk, float *dv, float *ws) {
-  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
-  if (p.waves == 4)
-    hipLaunchKernelGGL((attn_dkv_kernel<DB, 4>), grid, dim3(256), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv,
-                       ws);
-  else
-    hipLaunchKernelGGL((attn_dkv_kernel<DB, 8>), grid, dim3(512), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv,
-                       ws);
+  hipLaunchKernelGGL(attn_dkv_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(256),
+                     0, stream(), a, q, k, v, dout, lse, delta, dk, dv, ws);
 }
 
-#define BY_DIM(D, F, ...)              \
-  switch (blocks(D)) {                 \
+#define BY_STEPS(N, F, ...)            \
+  switch (N) {                         \
     case 1: F<1>(__VA_ARGS__); break;  \
     case 2: F<2>(__VA_ARGS__); break;  \
     case 3: F<3>(__VA_ARGS__); break;  \
@@ -1408,7 +1522,11 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
     if (!own) return -2;
   }
   float *ml = w, *wo = w ? w + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
-  BY_DIM(a.D, run_fwd, p, a, q, k, v, o, lse, ml, wo);
+  if (p.few) {
+    BY_STEPS(blocks(a.D), run_few, p, a, q, k, v, o, lse, ml, wo);
+  } else {
+    BY_STEPS(blocks(a.D), run_fwd, p, a, q, k, v, o, lse, ml, wo);
+  }
   if (p.splits > 1) {
     const long rows = (long)a.B * a.Hkv * a.R;
     const dim3 grid((unsigned)(rows < 65536 ? rows : 65536));
@@ -1447,18 +1565,18 @@ extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const fl
   hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)),
                      dim3(256), 0, stream(), a, o, dout, delta);
   if (dq) {
-    BY_DIM(a.D, run_dq, a, q, k, v, dout, lse, delta, dq);
+    BY_STEPS(blocks(a.D), run_dq, a, q, k, v, dout, lse, delta, dq);
   }
   if (dk) {
     const Plan p = dkv_plan(t);
     a.splits = p.splits;
     a.chunk = p.chunk;
     float *parts = delta + delta_floats(t);
-    BY_DIM(a.D, run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts);
+    BY_STEPS(blocks(a.D), run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts);
     if (p.splits > 1) {
       const long keys = (long)a.B * a.Hkv * a.Lk;
       hipLaunchKernelGGL(attn_dkv_join_kernel, dim3((unsigned)((keys + 7) / 8 < 8192 ? (keys + 7) / 8 : 8192)),
-                         dim3(256), 0, stream(), a, p.width, 16 * p.waves, parts, dk, dv);
+                         dim3(256), 0, stream(), a, p.width, parts, dk, dv);
     }
   }
   ttrt_free(own);
