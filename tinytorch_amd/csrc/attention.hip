@@ -123,10 +123,10 @@ __device__ __forceinline__ Span span_of(const Args &a, const Seq &q, int i0, int
   return s;
 }
 
-// the same for the 32 packed rows of a wave from r0 on
+// the same for the 16 packed rows of a wave from r0 on
 __device__ __forceinline__ Span wave_span(const Args &a, const Seq &q, int r0, int r1) {
   if (r0 >= r1) return Span{0, 0, 0, 0};
-  return span_of(a, q, r0 / a.G, ((r0 + 32 < r1 ? r0 + 32 : r1) - 1) / a.G);
+  return span_of(a, q, r0 / a.G, ((r0 + 16 < r1 ? r0 + 16 : r1) - 1) / a.G);
 }
 
 // Workgroups start in the order of blockIdx, 256 CUs at a time, and under a
@@ -235,12 +235,30 @@ __device__ __forceinline__ void store_row(float *p, const f32x4 (&acc)[DB], floa
     }
 }
 
+// row p[0 .. D) = f * the columns that acc holds of this lane's row, block by block
+template <int DB>
+__device__ __forceinline__ void store_columns(float *p, const f32x4 (&acc)[DB], float f, int D, int vec, int lane) {
+#pragma unroll
+  for (int o = 0; o < DB; o++) {
+    const int d = 16 * o + 4 * (lane >> 4);
+    const f32x4 v = acc[o] * f;
+    if (vec) {
+      if (d < D) *(f32x4_any *)(p + d) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (d + e < D) p[d + e] = v[e];
+    }
+  }
+}
+
 // Loads through a buffer descriptor: an offset past its length gives zeros, so
 // that rows and columns outside an operand cost a select and no branch.
 constexpr unsigned OUTSIDE = 0x80000000u;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p) {
-  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p, int bytes = 0x7fffffff) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, bytes, 0x00020000);
 }
 
 __device__ __forceinline__ float get1(__amdgpu_buffer_rsrc_t r, int off, int c, bool in, int D) {
@@ -278,10 +296,9 @@ __device__ __forceinline__ int small_div(int x, int G, unsigned magic) {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                  0);
 }
 
@@ -309,159 +326,170 @@ __device__ __forceinline__ Parts parts_of(float (&x)[8]) {
   return r;
 }
 
-// The 32x32x16 product: A holds row lane % 32 and B column lane % 32, both at
-// eight summed indices of their lane / 32; C holds column lane % 32, rows
-// 8 (r / 4) + 4 (lane / 32) + r % 4 in register r.  DU: steps of 16 columns of a
-// head; its rows are held as DU of them, its transposed results as DO blocks of
-// 32 of DP columns.
-template <int DU>
+// The 16x16x32 product: A holds row m = lane % 16 and B column m, both at the
+// eight summed indices of their group g = lane / 16; C holds column m, rows 4 g +
+// r in register r.  A wave has 16 query rows (or keys), so that two to four of
+// them fit a SIMD's registers and cover each other's waits; 32 a wave would
+// halve the reads of LDS, which is busy 17 % of the time, and leave one wave a
+// SIMD at 128 columns.  DB: blocks of 16 columns of a head, DK: steps of 32.
+//
+// A tile of KT rows lies in LDS as its parts, a row RC chunks of eight values
+// (a power of two), chunk c of row r at place c ^ f(r): sixteen lanes that read
+// one chunk of sixteen rows, and the 32 that read two chunks of eight rows (the
+// transposing reads), meet every bank once.
+template <int DB>
 struct Dim {
-  static constexpr int DO = (DU + 1) / 2, DP = 32 * DO, C4 = DP / 4;
-  // a row's parts in LDS: 2 DU units of eight values and one left free, an odd
-  // number, so that neighbouring rows start on other banks
-  static constexpr int RU = 2 * DU + 1;
-  static constexpr int ROWS = KT * RU * 16;       // bytes a part, rows as they are
-  static constexpr int COLS = 4 * DP * 16;        // bytes a part, transposed
+  static constexpr int DK = (DB + 1) / 2;
+  static constexpr int RC = DK == 1 ? 4 : DK == 2 ? 8 : 16, CHUNKS = 4 * DK;
+  static constexpr int PART = KT * RC * 16, SIZE = 3 * PART;  // bytes of a part, of a tile
+  static __device__ __forceinline__ int f(int r) {
+    return RC == 16  ? (r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1)
+           : RC == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1)
+                     : (r >> 2 & 1) << 1 | (r >> 3 & 1);
+  }
+  static constexpr int TASKS = KT * CHUNKS;  // chunks of a tile
 };
 
-// 4 x 4 blocks of a tile of KT rows on their way from memory to LDS: rows 4 j ..
-// 4 j + 3, columns 4 c .. 4 c + 3 of a thread
+// a chunk of a tile on its way from memory to LDS
 template <int DU>
-struct Block {
-  f32x4 v[4];
-  __device__ __forceinline__ void load(const float *base, int stride, int left, int D, int vec, int task) {
-    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
-    const int j = task / Dim<DU>::C4, c = task % Dim<DU>::C4;
+struct Chunk {
+  f32x4 v[2];
+  // the eight values at byte `off` of the buffer, of which D - c are the row's:
+  // VEC, all of a group of four or none, and where none `off` is OUTSIDE
+  template <bool VEC>
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned off, int c, int D) {
+    if (VEC) {
+      v[0] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+      v[1] = __builtin_bit_cast(f32x4,
+                                __builtin_amdgcn_raw_buffer_load_b128(r, c + 4 < D ? off + 16 : OUTSIDE, 0, 0));
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = get4(r, (4 * j + e) * stride, 4 * c, 4 * j + e < left, D, vec);
-  }
-  // packed query rows, r = i * G + member, from member `m0` of the query at `base` on
-  __device__ __forceinline__ void load_rows(const float *base, int rs, int hs, int G, unsigned magic, int m0, int left,
-                                            int D, int vec, int task) {
-    const __amdgpu_buffer_rsrc_t r = buffer_of(base);
-    const int j = task / Dim<DU>::C4, c = task % Dim<DU>::C4;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int i = small_div(m0 + 4 * j + e, G, magic);
-      v[e] = get4(r, i * rs + (m0 + 4 * j + e - i * G) * hs, 4 * c, 4 * j + e < left, D, vec);
+      for (int j = 0; j < 8; j++)
+        v[j / 4][j % 4] = __builtin_bit_cast(
+            float, __builtin_amdgcn_raw_buffer_load_b32(r, c + j < D ? off + 4 * j : OUTSIDE, 0, 0));
     }
   }
-  __device__ __forceinline__ bool odd() const {  // holds an infinity or a NaN
-    float t = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) t = fmaf(v[e][j], 0.f, t);
-    return t != t;
-  }
-  // The parts to LDS, as rows (`rows`) and transposed (`cols`), either NULL.
-  // Transposed, a unit of eight summed indices (rows 16 t + 4 h + {0 .. 3, 8 ..
-  // 11}: what a lane of half h holds of a product's registers 8 t .. 8 t + 7)
-  // of column d = 4 c + e lies at place C4 e + c, so that neighbouring threads
-  // write and neighbouring lanes read neighbouring units.
-  template <bool AS_ROWS, bool AS_COLS>
-  __device__ __forceinline__ void store(char *rows, char *cols, int task) {
+  // to LDS as parts; NaN for an infinity or NaN among them, else 0
+  __device__ __forceinline__ float store(char *tile, int task) const {
     typedef Dim<DU> M;
-    const int j = task / M::C4, c = task % M::C4;
-    char *pr = rows + 4 * j * M::RU * 16 + c * 8;
-    char *pc = cols + ((j / 4 * 2 + j % 2) * M::DP + c) * 16 + j % 4 / 2 * 8;
-    const bool in = M::DP == 16 * DU || c < 4 * DU;
+    const int row = task / M::CHUNKS, c = task % M::CHUNKS;
+    float x[8], t = 0.f;
 #pragma unroll
-    for (int n = 0; n < 3; n++) {
-      if (AS_ROWS && in) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          *(u32x2 *)(pr + n * M::ROWS + e * M::RU * 16) = (u32x2){lead(v[e][0], v[e][1]), lead(v[e][2], v[e][3])};
-      }
-      if (AS_COLS) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          *(u32x2 *)(pc + n * M::COLS + e * M::C4 * 16) = (u32x2){lead(v[0][e], v[1][e]), lead(v[2][e], v[3][e])};
-      }
-      if (n < 2) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) v[e][k] = rest(v[e][k]);
-      }
+    for (int j = 0; j < 8; j++) {
+      x[j] = v[j / 4][j % 4];
+      t = fmaf(x[j], 0.f, t);
     }
+    const Parts p = parts_of(x);
+    char *to = tile + row * M::RC * 16 + ((c ^ M::f(row)) << 4);
+#pragma unroll
+    for (int n = 0; n < 3; n++) *(u32x4 *)(to + n * M::PART) = p.p[n];
+    return t;
   }
 };
 
-// Operands go from LDS to registers one step ahead of the products that use
-// them, and no further: left alone, the compiler moves every read of an
-// unrolled loop to its front and runs out of registers.
-__device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
+// A step: the reads of the next one's operands, six products, and some of the
+// work of `side`, whose instructions go between the products.  Nothing moves from step to step:
+// left alone, the compiler moves every read of an unrolled loop to its front
+// and runs out of registers.
+__device__ __forceinline__ void step_end() {
+#pragma unroll
+  for (int n = 0; n < 6; n++) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+    __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);  // vector instructions
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
 
-__device__ __forceinline__ Parts read_parts(const char *p, int part) {
+__device__ __forceinline__ Parts read_rows(const char *p, int part) {
   Parts r;
 #pragma unroll
   for (int n = 0; n < 3; n++) r.p[n] = *(const u32x4 *)(p + n * part);
   return r;
 }
 
-// the tile's rows times this lane's row, columns 16 u + 8 h + ..: the six
-// products in two chains, so that none waits for the one before it
+__device__ __forceinline__ void six(const Parts &a, const Parts &b, f32x4 &c) {
+  c = mma(a.p[0], b.p[0], c);
+  c = mma(a.p[0], b.p[1], c);
+  c = mma(a.p[1], b.p[0], c);
+  c = mma(a.p[1], b.p[1], c);
+  c = mma(a.p[0], b.p[2], c);
+  c = mma(a.p[2], b.p[0], c);
+}
+
+// s[n] = the tile's rows 16 n + .. times this lane's row, columns 32 u + 8 g + ..
 template <int DU>
-__device__ __forceinline__ f32x16 dots(const char *rows, const Parts (&b)[DU], int lane) {
+__device__ __forceinline__ void dots(f32x4 (&s)[2], const char *tile, const Parts (&b)[Dim<DU>::DK], int lane) {
   typedef Dim<DU> M;
-  const char *p = rows + (lane & 31) * M::RU * 16 + (lane >> 5) * 16;
-  f32x16 s = {}, t = {};
-  Parts a = read_parts(p, M::ROWS), next = a;
+  const int r = lane & 15, at = r * M::RC * 16 + ((M::f(r) ^ (lane >> 4)) << 4);
+  s[0] = s[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  Parts a = read_rows(tile + at, M::PART), next = a;
 #pragma unroll
-  for (int u = 0; u < DU; u++) {
-    if (u + 1 < DU) next = read_parts(p + (u + 1) * 32, M::ROWS);
-    s = mma(a.p[0], b[u].p[0], s);
-    t = mma(a.p[0], b[u].p[1], t);
-    s = mma(a.p[1], b[u].p[0], s);
-    t = mma(a.p[1], b[u].p[1], t);
-    s = mma(a.p[0], b[u].p[2], s);
-    t = mma(a.p[2], b[u].p[0], t);
+  for (int n = 0; n < 2 * M::DK; n++) {
+    if (n + 1 < 2 * M::DK)
+      next = read_rows(tile + (at ^ (n + 1) / 2 << 6) + (n + 1) % 2 * 16 * M::RC * 16, M::PART);
+    six(a, b[n / 2], s[n % 2]);
     step_end();
     a = next;
   }
-  return s + t;
 }
 
-// acc (the columns of block b at rows l % 32) += sum over the tile's rows k of
-// x[k][column] w[k][l % 32], w the registers of a product with these rows
+// The transposing read: sixteen lanes read four values each of four rows and
+// sixteen columns (lane l: row l / 4, columns 4 (l % 4) ..) and get the four
+// rows of column l.  Two of them are the eight summed indices of a lane's group
+// g, rows 4 g + {0 .. 3, 16 .. 19}: what it holds of a product's two blocks.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_transposed(const char *p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p)));
+}
 template <int DU>
-__device__ __forceinline__ void product(f32x16 (&acc)[Dim<DU>::DO], const f32x16 &w, const char *cols, int lane) {
+__device__ __forceinline__ Parts read_columns(const char *tile, int at, int o) {
   typedef Dim<DU> M;
-  constexpr int DO = M::DO;
-  const char *p = cols + ((lane >> 5) * M::DP + (lane & 31)) * 16;
-  Parts a = read_parts(p, M::COLS), next = a, b;
+  Parts r;
 #pragma unroll
-  for (int n = 0; n < 2 * DO; n++) {
-    const int t = n / DO, o = n % DO;
-    if (o == 0) {
-      float x[8];
+  for (int n = 0; n < 3; n++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = w[8 * t + e];
-      b = parts_of(x);
+    for (int x = 0; x < 2; x++) {
+      const u32x2 w = read_transposed(tile + n * M::PART + (at ^ 2 * o << 4) + 16 * x * M::RC * 16);
+      r.p[n][2 * x] = w[0];
+      r.p[n][2 * x + 1] = w[1];
     }
-    if (n + 1 < 2 * DO) next = read_parts(p + ((n + 1) / DO * 2 * M::DP + (n + 1) % DO * 32) * 16, M::COLS);
-    acc[o] = mma(a.p[0], b.p[0], acc[o]);
-    acc[o] = mma(a.p[0], b.p[1], acc[o]);
-    acc[o] = mma(a.p[1], b.p[0], acc[o]);
-    acc[o] = mma(a.p[1], b.p[1], acc[o]);
-    acc[o] = mma(a.p[0], b.p[2], acc[o]);
-    acc[o] = mma(a.p[2], b.p[0], acc[o]);
+  return r;
+}
+
+// acc (columns 16 o + .. of block o) += sum over the tile's rows k of
+// x[k][column] w[k][l % 16], w the registers of a product with these rows
+template <int DU, class SIDE>
+__device__ __forceinline__ void product(f32x4 (&acc)[DU], const f32x4 (&w)[2], const char *tile, int lane, SIDE side) {
+  typedef Dim<DU> M;
+  const int l = lane & 15, r = 4 * (lane >> 4) + l / 4;
+  const int at = r * M::RC * 16 + ((l % 4 / 2 ^ M::f(r)) << 4) + l % 2 * 8;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) x[e] = w[e / 4][e % 4];
+  const Parts b = parts_of(x);
+  Parts a = read_columns<DU>(tile, at, 0), next = a;
+#pragma unroll
+  for (int n = 0; n < DU; n++) {
+    if (n + 1 < DU) next = read_columns<DU>(tile, at, n + 1);
+    six(a, b, acc[n]);
+    side(n);
     step_end();
     a = next;
   }
 }
 
-// this lane's row p[0 .. D) times f as parts, columns 16 u + 8 h + ..
+// this lane's row p[0 .. D) times f as parts, columns 32 u + 8 g + ..
 template <int DU>
-__device__ __forceinline__ void load_parts(Parts (&b)[DU], const float *p, bool in, float f, int D, int vec, int lane) {
+__device__ __forceinline__ void load_parts(Parts (&b)[Dim<DU>::DK], const float *p, bool in, float f, int D, int vec,
+                                           int lane) {
 #pragma unroll
-  for (int u = 0; u < DU; u++) {
+  for (int u = 0; u < Dim<DU>::DK; u++) {
     float x[8];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (in) v = load4(p, 16 * u + 8 * (lane >> 5) + 4 * k, D, vec);
+      if (in) v = load4(p, 32 * u + 8 * (lane >> 4) + 4 * k, D, vec);
 #pragma unroll
       for (int j = 0; j < 4; j++) x[4 * k + j] = v[j] * f;
     }
@@ -469,29 +497,86 @@ __device__ __forceinline__ void load_parts(Parts (&b)[DU], const float *p, bool 
   }
 }
 
-// row p[0 .. D) = f * the columns that acc holds of this lane's row: register
-// 4 q + i of the place 32 o + 8 q + 4 h + i, column 4 c + e at place C4 e + c
-template <int DU>
-__device__ __forceinline__ void store_columns(float *p, const f32x16 (&acc)[Dim<DU>::DO], float f, int D, int vec,
-                                              int lane) {
-  constexpr int C4 = Dim<DU>::C4;
+// Two tiles (keys and values, or the packed rows of q and do) in turn through
+// two buffers: a thread's chunks of the next one are loaded, and go to LDS as
+// side work of the products with the present one.
+template <int DU, int NT>
+struct Stream {
+  typedef Dim<DU> M;
+  static constexpr int N = (2 * M::TASKS + NT - 1) / NT;
+  Chunk<DU> c[N];
+  unsigned at[N];  // keys: byte offsets within a tile
+  float odd;
+  static __device__ __forceinline__ bool has(int t) { return 2 * M::TASKS % NT == 0 || t < 2 * M::TASKS; }
+  // a wave's chunks are of one tile of the two
+  static __device__ __forceinline__ bool second(int t) { return __builtin_amdgcn_readfirstlane(t) >= M::TASKS; }
+  static __device__ __forceinline__ int row_of(int t) { return t % M::TASKS / M::CHUNKS; }
+  static __device__ __forceinline__ int col_of(int t) { return t % M::TASKS % M::CHUNKS * 8; }
+
+  __device__ __forceinline__ void init(int s0, int s1, int D, int tid) {
 #pragma unroll
-  for (int q = 0; q < Dim<DU>::DO; q++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int d = 4 * (8 * q + 4 * (lane >> 5) + i);
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = acc[(C4 * e + 8 * q) / 32][(C4 * e + 8 * q) % 32 / 2 + i] * f;
-      if (vec) {
-        if (d < D) *(f32x4_any *)(p + d) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (d + e < D) p[d + e] = v[e];
-      }
+    for (int n = 0; n < N; n++) {
+      const int t = tid + n * NT;
+      at[n] = col_of(t) < D ? (unsigned)(row_of(t) * (second(t) ? s1 : s0) + col_of(t)) * 4u : OUTSIDE;
     }
-}
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void load_some(__amdgpu_buffer_rsrc_t r0, __amdgpu_buffer_rsrc_t r1, int D, int tid) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int t = tid + n * NT;
+      if (has(t)) c[n].template load<VEC>(second(t) ? r1 : r0, at[n], col_of(t), D);
+    }
+  }
+  // the rows from p0 (p1) on, s0 (s1) floats apart, zeros from `left` on: past
+  // the buffer's length
+  __device__ __forceinline__ void load(const float *p0, const float *p1, int s0, int s1, int left, int D, int vec,
+                                       int tid) {
+    left = left < 0 ? 0 : left < KT ? left : KT;
+    const __amdgpu_buffer_rsrc_t r0 = buffer_of(p0, 4 * left * s0), r1 = buffer_of(p1, 4 * left * s1);
+    if (vec)
+      load_some<true>(r0, r1, D, tid);
+    else
+      load_some<false>(r0, r1, D, tid);
+    odd = 0.f;
+  }
+  // the same for packed query rows, r = i * G + member, from member m0 of the
+  // query at p0 (p1) on
+  __device__ __forceinline__ void load_rows(const float *p0, const float *p1, const Strides &s0, const Strides &s1, int G,
+                                            unsigned magic, int m0, int left, int D, int vec, int tid) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int t = tid + n * NT, row = row_of(t), i = small_div(m0 + row, G, magic), m = m0 + row - i * G;
+      const int rs = second(t) ? (int)s1.r : (int)s0.r, hs = second(t) ? (int)s1.h : (int)s0.h;
+      at[n] = (row < left && col_of(t) < D) ? (unsigned)(i * rs + m * hs + col_of(t)) * 4u : OUTSIDE;
+    }
+    const __amdgpu_buffer_rsrc_t r0 = buffer_of(p0), r1 = buffer_of(p1);
+    if (vec)
+      load_some<true>(r0, r1, D, tid);
+    else
+      load_some<false>(r0, r1, D, tid);
+    odd = 0.f;
+  }
+  // chunk n to the pair of tiles at `to`; the tiles of `look` (bits) are looked
+  // through for infinities and NaN
+  __device__ __forceinline__ void store(int n, char *to, int look, int tid) {
+    const int t = tid + n * NT;
+    if (has(t)) {
+      const float z = c[n].store(to + (second(t) ? M::SIZE : 0), t % M::TASKS);
+      if (look == 3 || (look == 1) != second(t)) odd += z;
+    }
+  }
+  // at step n of `steps`: the chunks whose turn it is
+  __device__ __forceinline__ void side(int n, int steps, char *to, int look, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; k++)
+      if (n == (2 * k + 1) * steps / (2 * N)) store(k, to, look, tid);
+  }
+  __device__ __forceinline__ void all(char *to, int look, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; k++) store(k, to, look, tid);
+  }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -507,12 +592,12 @@ __device__ __forceinline__ float col_sum(float x) {
 
 // ---------------------------------------------------------------- forward
 
-// 32 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
+// 16 packed rows from `first` on, for attn_fwd_kernel's keys [k0, k1)
 __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, int k0, int k1,
                                                const float *q, const float *k, const float *v, float *o, float *lse,
                                                float *ws_ml, float *ws_o, int width, int lane) {
 #pragma unroll 1
-  for (int row = first; row < first + 32 && row < r1; row++) {
+  for (int row = first; row < first + 16 && row < r1; row++) {
     const int i = row / a.G, hm = row - i * a.G;
     Range rg = range_of(a, sq, i);
     if (rg.lo < k0) rg.lo = k0;
@@ -547,122 +632,99 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
   }
 }
 
-// One workgroup: 128 packed rows (32 a wave) of one key head against the keys
-// they see, KT at a time through LDS.  A tile is on its way to registers while
-// the one before it is used, and goes to LDS as parts between two barriers; two
-// workgroups a CU cover each other's.  With splits > 1 it takes `chunk` keys of
-// them and leaves maximum, sum and the unscaled result to the join.
-template <int DU>
-__global__ void __launch_bounds__(256, 2)
+// One workgroup of NW waves: 16 packed rows a wave of one key head against the
+// keys they see, KT at a time through LDS.  With splits > 1 it takes `chunk` keys of them
+// and leaves maximum, sum and the unscaled result to the join.
+template <int DU, int NW>
+__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 4 : 2)
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
   typedef Dim<DU> M;
-  __shared__ __attribute__((aligned(16))) char lk[3 * M::ROWS], lv[3 * M::COLS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   // the last rows see the most keys under a causal mask: they start first
   const int tile = gridDim.x / nbh - 1 - at0 / nbh;
-  const int r0 = tile * 128, r1 = r0 + 128 < a.R ? r0 + 128 : a.R;
+  const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
-  const Span mine = wave_span(a, sq, r0 + wave * 32, r1);
+  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
   int k_first = sp.lo / KT * KT, k_end = sp.hi;
   if (a.splits > 1) {
     const long c0 = (long)blockIdx.y * a.chunk, c1 = c0 + a.chunk;
     if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
     if (c1 < k_end) k_end = (int)c1;
   }
-  const int row = r0 + wave * 32 + (lane & 31), i = row / a.G, hq = h * a.G + row - i * a.G;
+  const int row = r0 + wave * 16 + (lane & 15), i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R;
   Range rg = {0, 0};
   if (in) rg = range_of(a, sq, i);
-  const float *qp0 = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
+  const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
-  // the tile's blocks: keys, then values
-  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
-  Block<DU> block[NB];
-  bool odd = false;
+  Stream<DU, 64 * NW> next;
+  next.init((int)a.k.r, (int)a.v.r, a.D, tid);
   auto load = [&](int k0) {
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (t < TASKS)
-        block[n].load(kp + (long)k0 * a.k.r, (int)a.k.r, k_end - k0, a.D, a.vec, t);
-      else if (t < 2 * TASKS)
-        block[n].load(vp + (long)k0 * a.v.r, (int)a.v.r, k_end - k0, a.D, a.vec, t - TASKS);
-    }
-  };
-  auto store = [&](bool look) {
-    bool found = false;
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (t < TASKS) {
-        block[n].template store<true, false>(lk, lv, t);
-      } else if (t < 2 * TASKS) {
-        if (look) found |= block[n].odd();
-        block[n].template store<false, true>(lk, lv, t - TASKS);
-      }
-    }
-    if (look)
-      odd = __syncthreads_or(found);
-    else
-      __syncthreads();
+    next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
   };
   auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
+  bool odd = false;
   if (k_first < k_end) load(k_first);
-  Parts qf[DU];
-  f32x16 acc[M::DO];
+  Parts qf[M::DK];
+  f32x4 acc[DU];
   float mx = -INFINITY, sum = 0.f;
-  load_parts<DU>(qf, qp0 + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, in, a.scale * LOG2E, a.D, a.vec, lane);
+  load_parts<DU>(qf, qp + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, in, a.scale * LOG2E, a.D, a.vec, lane);
 #pragma unroll
-  for (int n = 0; n < M::DO; n++) acc[n] = (f32x16){};
-  if (k_first < k_end) store(is_mixed(k_first));
-  for (int k0 = k_first; k0 < k_end; k0 += KT) {
-    const bool mixed = is_mixed(k0), more = k0 + KT < k_end;
+  for (int n = 0; n < DU; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (k_first < k_end) {
+    next.all(lds[0], 2, tid);
+    odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+  }
+  int buf = 0;
+  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
     if (odd) break;
-    if (more) load(k0 + KT);
+    const char *lk = lds[buf], *lv = lk + M::SIZE;
+    char *to = lds[buf ^ 1];
+    load(k0 + KT);  // zeros behind the last
     if (k0 < mine.hi && k0 + KT > mine.lo) {  // this wave's rows see some of the tile
-      f32x16 s = dots<DU>(lk, qf, lane);
-      if (mixed) {
+      f32x4 s[2];
+      dots<DU>(s, lk, qf, lane);
+      if (is_mixed(k0)) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int key = k0 + 8 * (r / 4) + 4 * g + r % 4;
-          if (key < rg.lo || key >= rg.hi) s[r] = -INFINITY;
+        for (int r = 0; r < 8; r++) {
+          const int key = k0 + 16 * (r / 4) + 4 * g + r % 4;
+          s[r / 4][r % 4] = ((key < rg.lo) | (key >= rg.hi)) ? -INFINITY : s[r / 4][r % 4];
         }
       }
-      float t = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; r++) t = fmaxf(t, s[r]);
-      t = fmaxf(fmaxf(t, __shfl_xor(t, 32)), mx);
+      float t = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      t = fmaxf(col_max(t), mx);
       const float base = t == -INFINITY ? 0.f : t;
       if (__any(t > mx)) {
         const float f = exp2_fast(mx - base);
         sum *= f;
 #pragma unroll
-        for (int n = 0; n < M::DO; n++) acc[n] *= f;
+        for (int n = 0; n < DU; n++) acc[n] *= f;
         mx = t;
       }
 #pragma unroll
-      for (int r = 0; r < 16; r++) s[r] = exp2_fast(s[r] - base);
-      float u[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) u[r] = (s[r] + s[r + 4]) + (s[r + 8] + s[r + 12]);
-      sum += (u[0] + u[1]) + (u[2] + u[3]);
-      product<DU>(acc, s, lv, lane);
+      for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - base);
+      sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+      product<DU>(acc, s, lv, lane, [&](int n) { next.side(n, DU, to, 2, tid); });
+    } else {
+      next.all(to, 2, tid);
     }
-    if (more) {
+    if (is_mixed(k0 + KT))
+      odd = __syncthreads_or(next.odd != next.odd);
+    else
       __syncthreads();
-      store(is_mixed(k0 + KT));
-    }
   }
   if (odd) {
-    fwd_one_by_one(a, sq, b, h, r0 + wave * 32, r1, k_first, k_end, qp0, kp, vp, o, lse, ws_ml, ws_o, M::DP, lane);
+    fwd_one_by_one(a, sq, b, h, r0 + wave * 16, r1, k_first, k_end, qp, kp, vp, o, lse, ws_ml, ws_o, 16 * DU, lane);
     return;
   }
 
-  const float total = sum + __shfl_xor(sum, 32);
+  const float total = col_sum(sum);
   if (!in) return;
   if (a.splits > 1) {
     const long at = ((long)blockIdx.y * nbh + bh) * a.R + row;
@@ -670,7 +732,7 @@ __global__ void __launch_bounds__(256, 2)
       ws_ml[2 * at] = mx;
       ws_ml[2 * at + 1] = total;
     }
-    store_columns<DU>(ws_o + at * M::DP, acc, 1.f, M::DP, 1, lane);
+    store_columns<DU>(ws_o + at * 16 * DU, acc, 1.f, 16 * DU, 1, lane);
     return;
   }
   if (lse && g == 0)
@@ -977,12 +1039,12 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dq of 32 packed rows from `first` on
+// dq of 16 packed rows from `first` on
 __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int b, int h, int first, int r1, const float *q,
                                               const float *k, const float *v, const float *dout, const float *lse,
                                               const float *delta, float *dq, int lane) {
 #pragma unroll 1
-  for (int row = first; row < first + 32 && row < r1; row++) {
+  for (int row = first; row < first + 16 && row < r1; row++) {
     const int i = row / a.G, hq = h * a.G + row - i * a.G;
     const Range rg = range_of(a, sq, i);
     Pair acc = {0.f, 0.f};
@@ -1006,23 +1068,23 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
   }
 }
 
-// dq of 128 packed rows (32 a wave): the keys through LDS as rows and transposed,
-// the values as rows
-template <int DU>
-__global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
+// dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
+// forward pass
+template <int DU, int NW>
+__global__ void __launch_bounds__(64 * NW, DU <= 2 ? 4 : 2)
     attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ dout, const float *__restrict__ lse,
                    const float *__restrict__ delta, float *__restrict__ dq) {
   typedef Dim<DU> M;
-  __shared__ __attribute__((aligned(16))) char lk[3 * M::ROWS], lkt[3 * M::COLS], lv[3 * M::ROWS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
   const int tile = gridDim.x / nbh - 1 - at0 / nbh;
-  const int r0 = tile * 128, r1 = r0 + 128 < a.R ? r0 + 128 : a.R;
+  const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
-  const Span mine = wave_span(a, sq, r0 + wave * 32, r1);
-  const int row = r0 + wave * 32 + (lane & 31), i = row / a.G, hq = h * a.G + row - i * a.G;
+  const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
+  const int row = r0 + wave * 16 + (lane & 15), i = row / a.G, hq = h * a.G + row - i * a.G;
   const bool in = row < a.R, live = in && i < sq.queries;
   Range rg = {0, 0};
   float l2 = 0.f, dl = 0.f;
@@ -1035,66 +1097,54 @@ __global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
   }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
   const int k_first = sp.lo / KT * KT, k_end = sp.hi;
-  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
-  Block<DU> block[NB];
-  bool odd = false;
+  Stream<DU, 64 * NW> next;
+  next.init((int)a.k.r, (int)a.v.r, a.D, tid);
   auto load = [&](int k0) {
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (t < TASKS)
-        block[n].load(kp + (long)k0 * a.k.r, (int)a.k.r, k_end - k0, a.D, a.vec, t);
-      else if (t < 2 * TASKS)
-        block[n].load(vp + (long)k0 * a.v.r, (int)a.v.r, k_end - k0, a.D, a.vec, t - TASKS);
-    }
-  };
-  auto store = [&](bool look) {
-    bool found = false;
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (t < TASKS) {
-        if (look) found |= block[n].odd();
-        block[n].template store<true, true>(lk, lkt, t);
-      } else if (t < 2 * TASKS) {
-        block[n].template store<true, false>(lv, lkt, t - TASKS);
-      }
-    }
-    if (look)
-      odd = __syncthreads_or(found);
-    else
-      __syncthreads();
+    next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
   };
   auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
+  bool odd = false;
   if (k_first < k_end) load(k_first);
-  Parts qf[DU], df[DU];
-  f32x16 acc[M::DO];
+  Parts qf[M::DK], df[M::DK];
+  f32x4 acc[DU];
   load_parts<DU>(qf, q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, live, a.scale * LOG2E, a.D, a.vec, lane);
   load_parts<DU>(df, dout + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, live, 1.f, a.D, a.vec, lane);
 #pragma unroll
-  for (int n = 0; n < M::DO; n++) acc[n] = (f32x16){};
-  if (k_first < k_end) store(is_mixed(k_first));
-  for (int k0 = k_first; k0 < k_end; k0 += KT) {
-    const bool mixed = is_mixed(k0), more = k0 + KT < k_end;
+  for (int n = 0; n < DU; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (k_first < k_end) {
+    next.all(lds[0], 1, tid);
+    odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+  }
+  int buf = 0;
+  for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
     if (odd) break;
-    if (more) load(k0 + KT);
+    const char *lk = lds[buf], *lv = lk + M::SIZE;
+    char *to = lds[buf ^ 1];
+    load(k0 + KT);
     if (k0 < mine.hi && k0 + KT > mine.lo) {
-      f32x16 s = dots<DU>(lk, qf, lane), dp = dots<DU>(lv, df, lane);
+      f32x4 s[2], dp[2];
+      dots<DU>(s, lk, qf, lane);
+      dots<DU>(dp, lv, df, lane);
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int key = k0 + 8 * (r / 4) + 4 * g + r % 4;
-        const float x = exp2_fast(s[r] - l2) * (dp[r] - dl);
-        s[r] = mixed && (key < rg.lo || key >= rg.hi) ? 0.f : x;
+      for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - l2) * (dp[r / 4][r % 4] - dl);
+      if (is_mixed(k0)) {
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+          const int key = k0 + 16 * (r / 4) + 4 * g + r % 4;
+          s[r / 4][r % 4] = ((key < rg.lo) | (key >= rg.hi)) ? 0.f : s[r / 4][r % 4];
+        }
       }
-      product<DU>(acc, s, lkt, lane);
+      product<DU>(acc, s, lk, lane, [&](int n) { next.side(n, DU, to, 1, tid); });
+    } else {
+      next.all(to, 1, tid);
     }
-    if (more) {
+    if (is_mixed(k0 + KT))
+      odd = __syncthreads_or(next.odd != next.odd);
+    else
       __syncthreads();
-      store(is_mixed(k0 + KT));
-    }
   }
   if (odd) {
-    dq_one_by_one(a, sq, b, h, r0 + wave * 32, r1, q, kp, vp, dout, lse, delta, dq, lane);
+    dq_one_by_one(a, sq, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
     return;
   }
   if (in)
@@ -1120,14 +1170,14 @@ __device__ __forceinline__ Rows rows_of(const Args &a, const Seq &s, int k0, int
   return r;
 }
 
-// dk and dv of 32 keys from `first` on, from the packed rows [r0, r1)
+// dk and dv of 16 keys from `first` on, from the packed rows [r0, r1)
 __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, int b, int h, int first, int r0, int r1,
                                                const float *q, const float *k, const float *v, const float *dout,
                                                const float *lse, const float *delta, float *dk, float *dv, float *ws,
                                                int width, int lane) {
   const int keys = seq.keys;
 #pragma unroll 1
-  for (int key = first; key < first + 32 && key < a.Lk; key++) {
+  for (int key = first; key < first + 16 && key < a.Lk; key++) {
     Pair ak = {0.f, 0.f}, av = {0.f, 0.f};
     const long ko = (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r;
     const long vo = (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r;
@@ -1162,24 +1212,23 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
   }
 }
 
-// dk and dv of 128 keys (32 a wave): the packed query rows that see any of
-// them through LDS, q and do as rows and transposed.  With splits > 1 a
-// workgroup takes `chunk` of the rows and leaves its sums to the join: where
-// many rows meet few keys, and so that no fp32 sum runs over more rows than
-// that.
+// dk and dv of 128 keys (16 a wave): the packed query rows that see any of
+// them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of the
+// rows and leaves its sums to the join: where many rows meet few keys, and so
+// that no fp32 sum runs over more rows than that.
 template <int DU>
-__global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
+__global__ void __launch_bounds__(512, 2)
     attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                     const float *__restrict__ dout, const float *__restrict__ lse,
                     const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
                     float *__restrict__ ws) {
   typedef Dim<DU> M;
-  __shared__ __attribute__((aligned(16))) char lq[3 * M::ROWS], lqt[3 * M::COLS], ld[3 * M::ROWS], ldt[3 * M::COLS];
-  __shared__ __attribute__((aligned(16))) float rl[KT], rd[KT];
-  __shared__ int rlo[KT], rhi[KT];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
+  __shared__ __attribute__((aligned(16))) float rl[2][KT], rd[2][KT];
+  __shared__ __attribute__((aligned(16))) int rlo[2][KT], rhi[2][KT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int k0 = at0 / nbh * 128, kw = k0 + wave * 32, key = kw + (lane & 31);
+  const int k0 = at0 / nbh * 128, kw = k0 + wave * 16, key = kw + (lane & 15);
   const Seq seq = seq_of(a, b);
   Rows rows = rows_of(a, seq, k0, k0 + 128);
   if (a.splits > 1) {
@@ -1191,27 +1240,22 @@ __global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
   const bool in = key < a.Lk, live = key < seq.keys;
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *op = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
-  constexpr int TASKS = 8 * M::C4, NB = (2 * TASKS + 255) / 256;
-  Block<DU> block[NB];
+  Stream<DU, 512> next;
   // row statistics of a tile, by the first KT threads
   float l2_ = 0.f, dl_ = 0.f;
   Range rg_ = {0, 0};
   int i_next = 0, m_next = 0;  // the next tile's first row: query and member
-  int t_i0 = 0, t_i1 = 0;      // the queries of the tile loaded last
   const int step_i = KT / a.G, step_m = KT % a.G;
   const unsigned magic = 65536u / a.G + 1;  // of small_div: exact for x < 2 KT and G < KT
+  // mixed: a mask hides some of the tile's rows from some of the keys; touched:
+  // some of the rows see some of this wave's keys
+  bool next_mixed = true, next_touched = false;
   auto load = [&](int r0) {
-    t_i0 = i_next;
-    t_i1 = i_next + small_div(m_next + KT - 1, a.G, magic);
+    const Span sp = span_of(a, seq, i_next, i_next + small_div(m_next + KT - 1, a.G, magic));
+    next_touched = kw < sp.hi && kw + 16 > sp.lo;
+    next_mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + 128 > sp.ihi;
     const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (t < TASKS)
-        block[n].load_rows(q0, (int)a.q.r, (int)a.q.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, t);
-      else if (t < 2 * TASKS)
-        block[n].load_rows(d0, (int)a.o.r, (int)a.o.h, a.G, magic, m_next, rows.end - r0, a.D, a.vec, t - TASKS);
-    }
+    next.load_rows(q0, d0, a.q, a.o, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
     if (tid < KT) {
       const int e = m_next + tid, di = small_div(e, a.G, magic), i = i_next + di;
       l2_ = dl_ = 0.f;
@@ -1231,83 +1275,83 @@ __global__ void __launch_bounds__(256, DU > 4 ? 1 : 2)
       i_next++;
     }
   };
-  // mixed: a mask hides some of the tile's rows from some of the keys; touched:
-  // some of the rows see some of this wave's keys
-  bool odd = false, mixed = true, touched = true;
-  auto store = [&](int r0) {
-    const Span sp = span_of(a, seq, t_i0, t_i1);
-    touched = kw < sp.hi && kw + 32 > sp.lo;
-    mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + 128 > sp.ihi;
-    bool found = false;
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-      const int t = tid + n * 256;
-      if (mixed) found |= t < 2 * TASKS && block[n].odd();
-      if (t < TASKS)
-        block[n].template store<true, true>(lq, lqt, t);
-      else if (t < 2 * TASKS)
-        block[n].template store<true, true>(ld, ldt, t - TASKS);
-    }
+  auto store_statistics = [&](int to) {
     if (tid < KT) {
-      rl[tid] = l2_;
-      rd[tid] = dl_;
-      rlo[tid] = rg_.lo;
-      rhi[tid] = rg_.hi;
+      rl[to][tid] = l2_;
+      rd[to][tid] = dl_;
+      rlo[to][tid] = rg_.lo;
+      rhi[to][tid] = rg_.hi;
     }
-    if (mixed)
-      odd = __syncthreads_or(found);
-    else
-      __syncthreads();
   };
   if (rows.first < rows.end) {
     i_next = rows.first / a.G;
     m_next = rows.first - i_next * a.G;
     load(rows.first);
   }
-  Parts kf[DU], vf[DU];
-  f32x16 ak[M::DO], av[M::DO];
+  Parts kf[M::DK], vf[M::DK];
+  f32x4 ak[DU], av[DU];
   load_parts<DU>(kf, k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, live, a.scale * LOG2E, a.D, a.vec, lane);
   load_parts<DU>(vf, v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, live, 1.f, a.D, a.vec, lane);
 #pragma unroll
-  for (int n = 0; n < M::DO; n++) ak[n] = av[n] = (f32x16){};
-  if (rows.first < rows.end) store(rows.first);
-  for (int r0 = rows.first; r0 < rows.end; r0 += KT) {
-    const bool more = r0 + KT < rows.end;
+  for (int n = 0; n < DU; n++) ak[n] = av[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  bool odd = false;
+  if (rows.first < rows.end) {
+    next.all(lds[0], 3, tid);
+    store_statistics(0);
+    odd = __syncthreads_or(next.odd != next.odd) && next_mixed;
+  }
+  int buf = 0;
+  for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
     if (odd) break;
-    if (more) load(r0 + KT);
+    const bool mixed = next_mixed, touched = next_touched;
+    const char *lq = lds[buf], *ld = lq + M::SIZE;
+    char *to = lds[buf ^ 1];
+    load(r0 + KT);
     if (touched) {
-      f32x16 s = dots<DU>(lq, kf, lane), dp = dots<DU>(ld, vf, lane);
+      f32x4 s[2], dp[2];
+      dots<DU>(s, lq, kf, lane);
+      dots<DU>(dp, ld, vf, lane);
 #pragma unroll
-      for (int n = 0; n < 4; n++) {
-        const f32x4 l2 = *(const f32x4 *)(rl + 8 * n + 4 * g), dl = *(const f32x4 *)(rd + 8 * n + 4 * g);
+      for (int n = 0; n < 2; n++) {
+        const f32x4 l2 = *(const f32x4 *)(rl[buf] + 16 * n + 4 * g), dl = *(const f32x4 *)(rd[buf] + 16 * n + 4 * g);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          float p = exp2_fast(s[4 * n + j] - l2[j]), x = p * (dp[4 * n + j] - dl[j]);
-          if (mixed) {
-            const int e = 8 * n + 4 * g + j;
-            if (key < rlo[e] || key >= rhi[e]) p = x = 0.f;
-          }
-          s[4 * n + j] = p;
-          dp[4 * n + j] = x;
+          s[n][j] = exp2_fast(s[n][j] - l2[j]);
+          dp[n][j] = s[n][j] * (dp[n][j] - dl[j]);
         }
       }
-      product<DU>(av, s, ldt, lane);
-      product<DU>(ak, dp, lqt, lane);
+      if (mixed) {
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const i32x4 lo = *(const i32x4 *)(rlo[buf] + 16 * n + 4 * g), hi = *(const i32x4 *)(rhi[buf] + 16 * n + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const bool hidden = (key < lo[j]) | (key >= hi[j]);
+            s[n][j] = hidden ? 0.f : s[n][j];
+            dp[n][j] = hidden ? 0.f : dp[n][j];
+          }
+        }
+      }
+      product<DU>(av, s, ld, lane, [&](int n) { next.side(n, 2 * DU, to, 3, tid); });
+      product<DU>(ak, dp, lq, lane, [&](int n) { next.side(DU + n, 2 * DU, to, 3, tid); });
+    } else {
+      next.all(to, 3, tid);
     }
-    if (more) {
+    store_statistics(buf ^ 1);
+    if (next_mixed)
+      odd = __syncthreads_or(next.odd != next.odd);
+    else
       __syncthreads();
-      store(r0 + KT);
-    }
   }
   if (odd) {
-    dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, M::DP, lane);
+    dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, 16 * DU, lane);
     return;
   }
   if (!in) return;
   if (a.splits > 1) {
     const long at = ((long)blockIdx.y * nbh + bh) * a.Lk + key, half = (long)a.splits * nbh * a.Lk;
-    store_columns<DU>(ws + at * M::DP, ak, a.scale, M::DP, 1, lane);
-    store_columns<DU>(ws + (half + at) * M::DP, av, 1.f, M::DP, 1, lane);
+    store_columns<DU>(ws + at * 16 * DU, ak, a.scale, 16 * DU, 1, lane);
+    store_columns<DU>(ws + (half + at) * 16 * DU, av, 1.f, 16 * DU, 1, lane);
     return;
   }
   store_columns<DU>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
@@ -1362,6 +1406,7 @@ int blocks(int dim) {
 
 struct Plan {
   bool few;
+  int rows;    // of a workgroup
   int tiles;   // row (key gradients: key) tiles
   int splits, chunk;
   int width;   // floats a row of the parts takes
@@ -1404,16 +1449,16 @@ Plan plan_of(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.few = R <= 16;
+  p.width = 16 * blocks(t->head_dim);
   if (p.few) {
-    p.width = 16 * blocks(t->head_dim);
     p.tiles = 1;
     // parts of 64 to 1024 keys, about eight workgroups a CU
     long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    p.width = (t->head_dim + 31) / 32 * 32;
-    p.tiles = (int)((R + 127) / 128);
+    p.rows = 128;
+    p.tiles = (int)((R + p.rows - 1) / p.rows);
     split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
   }
   return p;
@@ -1422,7 +1467,7 @@ Plan plan_of(const TTAttention *t) {
 Plan dkv_plan(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
-  p.width = (t->head_dim + 31) / 32 * 32;
+  p.width = 16 * blocks(t->head_dim);
   p.few = false;
   p.tiles = (int)((t->k_rows + 127) / 128);
   // fp32 sums over at most 2048 rows
@@ -1466,22 +1511,23 @@ void run_few(const Plan &p, const Args &a, const float *q, const float *k, const
 template <int DU>
 void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
              float *ml, float *wo) {
-  hipLaunchKernelGGL(attn_fwd_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(256),
-                     0, stream(), a, q, k, v, o, lse, ml, wo);
+  constexpr int NW = 8;
+  hipLaunchKernelGGL((attn_fwd_kernel<DU, NW>), dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits),
+                     dim3(64 * NW), 0, stream(), a, q, k, v, o, lse, ml, wo);
 }
 
 template <int DU>
 void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
             const float *delta, float *dq) {
   const long tiles = ((long)a.R + 127) / 128 * a.B * a.Hkv;
-  hipLaunchKernelGGL(attn_dq_kernel<DU>, dim3((unsigned)tiles), dim3(256), 0, stream(), a, q, k, v, dout, lse, delta,
+  hipLaunchKernelGGL((attn_dq_kernel<DU, 8>), dim3((unsigned)tiles), dim3(512), 0, stream(), a, q, k, v, dout, lse, delta,
                      dq);
 }
 
 template <int DU>
 void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
              const float *lse, const float *delta, float *dk, float *dv, float *ws) {
-  hipLaunchKernelGGL(attn_dkv_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(256),
+  hipLaunchKernelGGL(attn_dkv_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(512),
                      0, stream(), a, q, k, v, dout, lse, delta, dk, dv, ws);
 }
 
