@@ -138,6 +138,58 @@ __device__ __forceinline__ int snake(int p, int all) {
   return (p & 256) && round + 256 <= all ? round + ((p & 255) ^ 248) : p;
 }
 
+// What workgroup p of T tiles of `per` a (sequence, key head) takes.  Plain: tile
+// by tile, the last (which see the most keys under a causal mask) first.  Where
+// the sequences' lengths are given and few enough for a wave, tile by tile of
+// those that reach so far, so that the heaviest come first and tiles behind a
+// sequence's end last: 64 heads in a batch of 1024 to 600 rows otherwise leave
+// the CUs idle for 40 % of the time.  from_end: tile T - 1 is a sequence's first
+// (key tiles, the first of which meet the most queries).
+struct Item {
+  int b, h, tile;
+};
+__device__ __forceinline__ Item item_of(const Args &a, const int32_t *len, int rows, int G, int per, int T, bool from_end) {
+  int p = snake(blockIdx.x, gridDim.x);
+  Item it;
+  if (!len || a.B > 64 || a.B == 1 || T > 256) {
+    const int nbh = a.B * a.Hkv, bh = p % nbh;
+    it.b = bh / a.Hkv;
+    it.h = bh % a.Hkv;
+    it.tile = from_end ? p / nbh : T - 1 - p / nbh;
+    return it;
+  }
+  const int lane = threadIdx.x & 63;
+  int n = -1;
+  if (lane < a.B) {
+    const int v = len[lane];
+    n = (int)(((long)(v < 0 ? 0 : v > rows ? rows : v) * G + per - 1) / per);
+  }
+  unsigned long long m = 0;
+  int t = T - 1;
+  bool empty = false;
+  for (; t >= 0; t--) {
+    m = __ballot(n > t);
+    const int c = __popcll(m) * a.Hkv;
+    if (p < c) break;
+    p -= c;
+  }
+  if (t < 0) {
+    empty = true;
+    for (t = 0; t < T - 1; t++) {
+      m = __ballot(n >= 0 && n <= t);
+      const int c = __popcll(m) * a.Hkv;
+      if (p < c) break;
+      p -= c;
+    }
+    if (t == T - 1) m = __ballot(n >= 0 && n <= t);
+  }
+  for (int k = p / a.Hkv; k > 0; k--) m &= m - 1;
+  it.b = __ffsll(m) - 1;
+  it.h = p % a.Hkv;
+  it.tile = from_end && !empty ? __builtin_amdgcn_readlane(n, it.b) - 1 - t : t;
+  return it;
+}
+
 // four values of a row from column c on; 0 behind the row's end
 __device__ __forceinline__ f32x4 load4(const float *p, int c, int D, int vec) {
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -334,18 +386,18 @@ __device__ __forceinline__ Parts parts_of(float (&x)[8]) {
 // SIMD at 128 columns.  DB: blocks of 16 columns of a head, DK: steps of 32.
 //
 // A tile of KT rows lies in LDS as its parts, a row RC chunks of eight values
-// (a power of two), chunk c of row r at place c ^ f(r): sixteen lanes that read
-// one chunk of sixteen rows, and the 32 that read two chunks of eight rows (the
-// transposing reads), meet every bank once.
+// (a power of two), chunk c of row r at place c ^ f(r): the lanes that LDS
+// serves at once (of a read of 16 bytes: 0-3, 12-15, 20-23, 24-27 and so on: rows
+// of two groups; of a transposing read, two chunks of eight rows) meet every bank
+// once.
 template <int DB>
 struct Dim {
   static constexpr int DK = (DB + 1) / 2;
   static constexpr int RC = DK == 1 ? 4 : DK == 2 ? 8 : 16, CHUNKS = 4 * DK;
   static constexpr int PART = KT * RC * 16, SIZE = 3 * PART;  // bytes of a part, of a tile
   static __device__ __forceinline__ int f(int r) {
-    return RC == 16  ? (r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1)
-           : RC == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1)
-                     : (r >> 2 & 1) << 1 | (r >> 3 & 1);
+    const int quad = ((r >> 2 ^ r >> 3) & 1) << 1 | (r >> 3 & 1);
+    return RC == 16 ? (r & 3) << 2 | quad : RC == 8 ? (r >> 1 & 1) << 2 | quad : quad;
   }
   static constexpr int TASKS = KT * CHUNKS;  // chunks of a tile
 };
@@ -636,16 +688,16 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
 // keys they see, KT at a time through LDS.  With splits > 1 it takes `chunk` keys of them
 // and leaves maximum, sum and the unscaled result to the join.
 template <int DU, int NW>
-__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 4 : 2)
+__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
   typedef Dim<DU> M;
   __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  // the last rows see the most keys under a causal mask: they start first
-  const int tile = gridDim.x / nbh - 1 - at0 / nbh;
+  const int nbh = a.B * a.Hkv;
+  const Item it = item_of(a, a.q_len, a.Lq, a.G, 16 * NW, gridDim.x / nbh, false);
+  const int b = it.b, h = it.h, tile = it.tile, bh = b * a.Hkv + h;
   const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
@@ -1071,15 +1123,15 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
 // dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
 // forward pass
 template <int DU, int NW>
-__global__ void __launch_bounds__(64 * NW, DU <= 2 ? 4 : 2)
+__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ dout, const float *__restrict__ lse,
                    const float *__restrict__ delta, float *__restrict__ dq) {
   typedef Dim<DU> M;
   __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int tile = gridDim.x / nbh - 1 - at0 / nbh;
+  const Item it = item_of(a, a.q_len, a.Lq, a.G, 16 * NW, gridDim.x / (a.B * a.Hkv), false);
+  const int b = it.b, h = it.h, tile = it.tile;
   const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
@@ -1212,25 +1264,27 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
   }
 }
 
-// dk and dv of 128 keys (16 a wave): the packed query rows that see any of
+// dk and dv of 16 NW keys (16 a wave): the packed query rows that see any of
 // them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of the
 // rows and leaves its sums to the join: where many rows meet few keys, and so
 // that no fp32 sum runs over more rows than that.
-template <int DU>
-__global__ void __launch_bounds__(512, 2)
+template <int DU, int NW>
+__global__ void __launch_bounds__(64 * NW, 2)
     attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                     const float *__restrict__ dout, const float *__restrict__ lse,
                     const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
                     float *__restrict__ ws) {
   typedef Dim<DU> M;
+  constexpr int KEYS = 16 * NW;
   __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
   __shared__ __attribute__((aligned(16))) float rl[2][KT], rd[2][KT];
   __shared__ __attribute__((aligned(16))) int rlo[2][KT], rhi[2][KT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int nbh = a.B * a.Hkv, at0 = snake(blockIdx.x, gridDim.x), bh = at0 % nbh, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int k0 = at0 / nbh * 128, kw = k0 + wave * 16, key = kw + (lane & 15);
+  const int nbh = a.B * a.Hkv;
+  const Item it = item_of(a, a.k_len, a.Lk, 1, KEYS, gridDim.x / nbh, true);
+  const int b = it.b, h = it.h, bh = b * a.Hkv + h, k0 = it.tile * KEYS, kw = k0 + wave * 16, key = kw + (lane & 15);
   const Seq seq = seq_of(a, b);
-  Rows rows = rows_of(a, seq, k0, k0 + 128);
+  Rows rows = rows_of(a, seq, k0, k0 + KEYS);
   if (a.splits > 1) {
     const long c0 = rows.first + (long)blockIdx.y * a.chunk;
     if (c0 >= rows.end && blockIdx.y > 0) return;  // the join leaves it out
@@ -1240,7 +1294,7 @@ __global__ void __launch_bounds__(512, 2)
   const bool in = key < a.Lk, live = key < seq.keys;
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *op = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
-  Stream<DU, 512> next;
+  Stream<DU, 64 * NW> next;
   // row statistics of a tile, by the first KT threads
   float l2_ = 0.f, dl_ = 0.f;
   Range rg_ = {0, 0};
@@ -1253,7 +1307,7 @@ __global__ void __launch_bounds__(512, 2)
   auto load = [&](int r0) {
     const Span sp = span_of(a, seq, i_next, i_next + small_div(m_next + KT - 1, a.G, magic));
     next_touched = kw < sp.hi && kw + 16 > sp.lo;
-    next_mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + 128 > sp.ihi;
+    next_mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + KEYS > sp.ihi;
     const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
     next.load_rows(q0, d0, a.q, a.o, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
     if (tid < KT) {
@@ -1360,14 +1414,14 @@ __global__ void __launch_bounds__(512, 2)
 
 // the workgroups' sums of a key, added in their order; 32 lanes a key
 __global__ void __launch_bounds__(256)
-    attn_dkv_join_kernel(Args a, int width, const float *__restrict__ ws, float *__restrict__ dk,
+    attn_dkv_join_kernel(Args a, int width, int keys_a_group, const float *__restrict__ ws, float *__restrict__ dk,
                          float *__restrict__ dv) {
   const long nbh = (long)a.B * a.Hkv, all = nbh * a.Lk;
   const int lane = threadIdx.x & 31;
   for (long e = (long)blockIdx.x * 8 + (threadIdx.x >> 5); e < all; e += (long)gridDim.x * 8) {
     const int bh = (int)(e / a.Lk), key = (int)(e % a.Lk), b = bh / a.Hkv, h = bh % a.Hkv;
-    const int k0 = key / 128 * 128;
-    const Rows rows = rows_of(a, seq_of(a, b), k0, k0 + 128);
+    const int k0 = key / keys_a_group * keys_a_group;
+    const Rows rows = rows_of(a, seq_of(a, b), k0, k0 + keys_a_group);
     int parts = (rows.end - rows.first + a.chunk - 1) / a.chunk;
     if (parts < 1) parts = 1;
     if (4 * lane >= width) continue;
@@ -1445,6 +1499,14 @@ void split(Plan &p, long n, long want, long least, long step) {
   p.splits = (int)((n + c - 1) / c);
 }
 
+// Rows (keys) of a workgroup.  Up to 64 columns three workgroups of four waves fit
+// a CU; above, two waves a SIMD fit in all, and one workgroup of them reads and
+// splits each tile once.
+#ifndef SMALL
+#define SMALL 64
+#endif
+int rows_of_group(const TTAttention *t) { return t->head_dim <= SMALL ? 64 : 128; }
+
 Plan plan_of(const TTAttention *t) {
   Plan p;
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
@@ -1457,7 +1519,7 @@ Plan plan_of(const TTAttention *t) {
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    p.rows = 128;
+    p.rows = rows_of_group(t);
     p.tiles = (int)((R + p.rows - 1) / p.rows);
     split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
   }
@@ -1469,7 +1531,8 @@ Plan dkv_plan(const TTAttention *t) {
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = false;
-  p.tiles = (int)((t->k_rows + 127) / 128);
+  p.rows = rows_of_group(t);
+  p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
   // fp32 sums over at most 2048 rows
   const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
   split(p, R, fill > sums ? fill : sums, 256, KT);
@@ -1511,7 +1574,7 @@ void run_few(const Plan &p, const Args &a, const float *q, const float *k, const
 template <int DU>
 void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
              float *ml, float *wo) {
-  constexpr int NW = 8;
+  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
   hipLaunchKernelGGL((attn_fwd_kernel<DU, NW>), dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits),
                      dim3(64 * NW), 0, stream(), a, q, k, v, o, lse, ml, wo);
 }
@@ -1519,16 +1582,18 @@ void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const
 template <int DU>
 void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
             const float *delta, float *dq) {
-  const long tiles = ((long)a.R + 127) / 128 * a.B * a.Hkv;
-  hipLaunchKernelGGL((attn_dq_kernel<DU, 8>), dim3((unsigned)tiles), dim3(512), 0, stream(), a, q, k, v, dout, lse, delta,
-                     dq);
+  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
+  const long tiles = ((long)a.R + 16 * NW - 1) / (16 * NW) * a.B * a.Hkv;
+  hipLaunchKernelGGL((attn_dq_kernel<DU, NW>), dim3((unsigned)tiles), dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
+                     delta, dq);
 }
 
 template <int DU>
 void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
              const float *lse, const float *delta, float *dk, float *dv, float *ws) {
-  hipLaunchKernelGGL(attn_dkv_kernel<DU>, dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits), dim3(512),
-                     0, stream(), a, q, k, v, dout, lse, delta, dk, dv, ws);
+  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
+  hipLaunchKernelGGL((attn_dkv_kernel<DU, NW>), dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits),
+                     dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv, ws);
 }
 
 #define BY_STEPS(N, F, ...)            \
@@ -1622,7 +1687,7 @@ extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const fl
     if (p.splits > 1) {
       const long keys = (long)a.B * a.Hkv * a.Lk;
       hipLaunchKernelGGL(attn_dkv_join_kernel, dim3((unsigned)((keys + 7) / 8 < 8192 ? (keys + 7) / 8 : 8192)),
-                         dim3(256), 0, stream(), a, p.width, parts, dk, dv);
+                         dim3(256), 0, stream(), a, p.width, p.rows, parts, dk, dv);
     }
   }
   ttrt_free(own);
