@@ -42,6 +42,9 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
+#ifndef PRIO
+#define PRIO
+#endif
 constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
 
@@ -511,16 +514,22 @@ __device__ __forceinline__ Parts read_columns(const char *tile, int at, int o) {
 
 // acc (columns 16 o + .. of block o) += sum over the tile's rows k of
 // x[k][column] w[k][l % 16], w the registers of a product with these rows
-template <int DU, class SIDE>
-__device__ __forceinline__ void product(f32x4 (&acc)[DU], const f32x4 (&w)[2], const char *tile, int lane, SIDE side) {
+template <int DU>
+__device__ __forceinline__ int columns_at(int lane) {
   typedef Dim<DU> M;
   const int l = lane & 15, r = 4 * (lane >> 4) + l / 4;
-  const int at = r * M::RC * 16 + ((l % 4 / 2 ^ M::f(r)) << 4) + l % 2 * 8;
+  return r * M::RC * 16 + ((l % 4 / 2 ^ M::f(r)) << 4) + l % 2 * 8;
+}
+// `a`: read_columns of block 0, which the caller has on its way by now
+template <int DU, class SIDE>
+__device__ __forceinline__ void product(f32x4 (&acc)[DU], const f32x4 (&w)[2], Parts a, const char *tile, int lane,
+                                        SIDE side) {
+  const int at = columns_at<DU>(lane);
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) x[e] = w[e / 4][e % 4];
   const Parts b = parts_of(x);
-  Parts a = read_columns<DU>(tile, at, 0), next = a;
+  Parts next = a;
 #pragma unroll
   for (int n = 0; n < DU; n++) {
     if (n + 1 < DU) next = read_columns<DU>(tile, at, n + 1);
@@ -632,14 +641,19 @@ struct Stream {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// over the four lanes that hold a column of a 16-column product
+// over the four lanes that hold a column: exchanges of 16 and 32 lanes between
+// registers, without a trip through LDS
 __device__ __forceinline__ float col_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float col_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
 // ---------------------------------------------------------------- forward
@@ -732,6 +746,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     next.all(lds[0], 2, tid);
     odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
   }
+  PRIO
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
     if (odd) break;
@@ -741,6 +756,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     if (k0 < mine.hi && k0 + KT > mine.lo) {  // this wave's rows see some of the tile
       f32x4 s[2];
       dots<DU>(s, lk, qf, lane);
+      const Parts first = read_columns<DU>(lv, columns_at<DU>(lane), 0);
       if (is_mixed(k0)) {
 #pragma unroll
         for (int r = 0; r < 8; r++) {
@@ -762,7 +778,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
 #pragma unroll
       for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - base);
       sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-      product<DU>(acc, s, lv, lane, [&](int n) { next.side(n, DU, to, 2, tid); });
+      product<DU>(acc, s, first, lv, lane, [&](int n) { next.side(n, DU, to, 2, tid); });
     } else {
       next.all(to, 2, tid);
     }
@@ -1167,6 +1183,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     next.all(lds[0], 1, tid);
     odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
   }
+  PRIO
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
     if (odd) break;
@@ -1177,6 +1194,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
       f32x4 s[2], dp[2];
       dots<DU>(s, lk, qf, lane);
       dots<DU>(dp, lv, df, lane);
+      const Parts first = read_columns<DU>(lk, columns_at<DU>(lane), 0);
 #pragma unroll
       for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - l2) * (dp[r / 4][r % 4] - dl);
       if (is_mixed(k0)) {
@@ -1186,7 +1204,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
           s[r / 4][r % 4] = ((key < rg.lo) | (key >= rg.hi)) ? 0.f : s[r / 4][r % 4];
         }
       }
-      product<DU>(acc, s, lk, lane, [&](int n) { next.side(n, DU, to, 1, tid); });
+      product<DU>(acc, s, first, lk, lane, [&](int n) { next.side(n, DU, to, 1, tid); });
     } else {
       next.all(to, 1, tid);
     }
@@ -1354,6 +1372,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
     store_statistics(0);
     odd = __syncthreads_or(next.odd != next.odd) && next_mixed;
   }
+  PRIO
   int buf = 0;
   for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
     if (odd) break;
@@ -1365,6 +1384,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
       f32x4 s[2], dp[2];
       dots<DU>(s, lq, kf, lane);
       dots<DU>(dp, ld, vf, lane);
+      const Parts first = read_columns<DU>(ld, columns_at<DU>(lane), 0);
 #pragma unroll
       for (int n = 0; n < 2; n++) {
         const f32x4 l2 = *(const f32x4 *)(rl[buf] + 16 * n + 4 * g), dl = *(const f32x4 *)(rd[buf] + 16 * n + 4 * g);
@@ -1386,8 +1406,8 @@ __global__ void __launch_bounds__(64 * NW, 2)
           }
         }
       }
-      product<DU>(av, s, ld, lane, [&](int n) { next.side(n, 2 * DU, to, 3, tid); });
-      product<DU>(ak, dp, lq, lane, [&](int n) { next.side(DU + n, 2 * DU, to, 3, tid); });
+      product<DU>(av, s, first, ld, lane, [&](int n) { next.side(n, 2 * DU, to, 3, tid); });
+      product<DU>(ak, dp, read_columns<DU>(lq, columns_at<DU>(lane), 0), lq, lane, [&](int n) { next.side(DU + n, 2 * DU, to, 3, tid); });
     } else {
       next.all(to, 3, tid);
     }
