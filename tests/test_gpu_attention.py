@@ -68,6 +68,18 @@ def test_head_sizes(tlib, D):
     _check(tlib, *_inputs(2, 37, 70, 4, 2, D), dict(causal=True))
 
 
+@pytest.mark.parametrize("D", [8, 31, 40, 64, 80, 95, 100, 128])
+@pytest.mark.parametrize("masks", [
+    dict(causal=True), dict(), dict(window=50),
+    dict(causal=True, window=77, k_len=[330, 0, 100], q_len=[300, 7, 33], q_start=[30, 0, 67])])
+def test_many_rows(tlib, D, masks):
+    """From 1024 packed rows on the tiles are split into parts beforehand."""
+    _check(tlib, *_inputs(3, 300, 330, 4, 1, D), masks)
+    if D == 64:
+        _check(tlib, *_inputs(1, 1025, 257, 2, 2, D), {n: m for n, m in masks.items() if not isinstance(m, list)})
+        _check(tlib, *_inputs(2, 1024, 256, 1, 1, D), {n: m for n, m in masks.items() if not isinstance(m, list)})
+
+
 @pytest.mark.parametrize("Lq,Lk", [(1, 1), (1, 2), (2, 1), (1, 15), (1, 17), (1, 64), (1, 65), (1, 1000), (3, 3),
                                    (15, 16), (16, 16), (17, 31), (32, 32), (33, 33), (63, 64), (64, 65), (65, 64),
                                    (100, 300), (129, 127), (257, 257), (40, 3000)])
@@ -113,7 +125,7 @@ def test_masks(tlib, masks, Hq, Hkv):
         _check(tlib, *t, masks)
 
 
-@pytest.mark.parametrize("Lq,Lk,Hq", [(1, 300, 4), (3, 300, 4), (70, 100, 2), (130, 130, 2)])
+@pytest.mark.parametrize("Lq,Lk,Hq", [(1, 300, 4), (3, 300, 4), (70, 100, 2), (130, 130, 2), (300, 330, 8)])
 def test_padding_is_not_read(tlib, Lq, Lk, Hq):
     """NaN behind k_len and q_len reaches nothing."""
     q, k, v, do = _inputs(3, Lq, Lk, Hq, 2, 64)
@@ -130,7 +142,7 @@ def test_padding_is_not_read(tlib, Lq, Lk, Hq):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(70, 70, 2, 2), (4, 90, 4, 2), (200, 300, 3, 1)])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(70, 70, 2, 2), (4, 90, 4, 2), (200, 300, 3, 1), (300, 300, 4, 1)])
 def test_what_a_mask_hides_stays_hidden(tlib, bad, Lq, Lk, Hq, Hkv):
     """A causal mask over infinities and NaN in one key's and one query's rows:
     what does not see them stays within its bounds, results and gradients."""
@@ -194,7 +206,7 @@ def _unlayout(buf, kind, first, shape):
 
 
 @pytest.mark.parametrize("kind", ["heads", "wide", "odd"])
-@pytest.mark.parametrize("Lq,Hq", [(1, 4), (50, 4), (300, 2)])
+@pytest.mark.parametrize("Lq,Hq", [(1, 4), (50, 4), (300, 2), (300, 8)])
 def test_layouts(tlib, kind, Lq, Hq):
     """Head-major, and rows of a wider buffer (16-byte aligned or not): the same
     results; what lies between rows stays."""
@@ -231,7 +243,7 @@ def test_layouts(tlib, kind, Lq, Hq):
 
 
 @pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(1, 5000, 4, 2), (2, 1300, 4, 1), (1, 130, 16, 16), (20, 5000, 4, 2),
-                                          (130, 2000, 1, 1)])
+                                          (130, 2000, 1, 1), (600, 2000, 2, 1)])
 def test_keys_split_over_workgroups(tlib, Lq, Lk, Hq, Hkv):
     """Long caches with ragged lengths, some within the first part; the parts
     join to the same bits with a workspace of the caller's, and nothing is
@@ -256,6 +268,31 @@ def test_keys_split_over_workgroups(tlib, Lq, Lk, Hq, Hkv):
     assert np.array_equal(o.to_np(q.shape), got["o"])
 
 
+@pytest.mark.parametrize("Lq,Lk", [(40, 60), (700, 300)])
+def test_backward_in_a_workspace_of_the_caller(tlib, Lq, Lk):
+    """Whatever it holds before: the same bits, with nothing allocated."""
+    q, k, v, do = _inputs(2, Lq, Lk, 4, 2, 96)
+    masks = dict(causal=True, k_len=[Lk, Lk // 3], q_start=[0, Lk // 3 - Lq])
+    want = _run(tlib, q, k, v, do, masks)
+    held = []
+    a = _plan(q, k, masks, held)
+    need = tlib.tt_k_attention_bwd_ws(a)
+    ws, d = DevBuf(need // 4 + 8), [DevBuf.from_np(t) for t in (q, k, v, want["o"], do, want["lse"])]
+    out = [DevBuf(t.size) for t in (q, k, v)]
+    for fill in (np.nan, 1e30):
+        ws.fill(fill)
+        assert tlib.tth_fail_alloc_after(0) == 0
+        try:
+            rc = tlib.tt_k_attention_bwd(a, *[x.ptr for x in d], *[x.ptr for x in out], ws.ptr)
+            none = tlib.tt_k_attention_bwd(a, *[x.ptr for x in d], *[x.ptr for x in out], None)
+        finally:
+            tlib.tth_fail_alloc_after(-1)
+        assert rc == 0 and none == -2
+        for n, x, t in zip(("dq", "dk", "dv"), out, (q, k, v)):
+            assert np.array_equal(x.to_np(t.shape), want[n]), n
+        assert (ws.to_np()[need // 4:] == np.float32(fill)).all() or np.isnan(fill)
+
+
 def test_offsets_past_32_bits(tlib):
     """Rows 2^23 floats apart: the last ones lie past 2^31 elements."""
     n, apart = 300, 1 << 23
@@ -266,7 +303,7 @@ def test_offsets_past_32_bits(tlib):
             row = np.ascontiguousarray(t[0, j, 0])
             check(tlib.tth_h2d(big.ptr + 4 * (j * apart + off), row.ctypes.data, row.nbytes), "h2d")
     s = Strides(0, apart, 0)
-    for Lq in (1, 30):
+    for Lq in (1, 30, 1100):
         q = _inputs(1, Lq, n, 2, 1, 64)[0]
         held, o, d = [], DevBuf(q.size), DevBuf.from_np(q)
         a = _plan(q, k, {}, held, k=s, v=s)

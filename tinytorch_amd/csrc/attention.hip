@@ -8,15 +8,18 @@
 //   ds_ij = p_ij (dp_ij - delta_i),  dq_i = scale sum_j ds_ij k_j,
 //   dk_j = scale sum_i ds_ij q_i  (both sums over the heads that share a key).
 //
-// Every product runs on v_mfma_f32_16x16x4_f32: A holds rows lane % 16 and B
-// columns lane % 16 of the product, both at summed index lane / 16; C holds
-// column lane % 16, rows 4 (lane / 16) + r in register r.  Two consequences
-// carry all kernels here:
-//   * a summed index may be dealt to lanes in any order that A and B share, so
-//     one 16-byte read of four consecutive values feeds four products;
+// The matrix units multiply fp32 at 1/16 the rate of bf16.  A float is the sum of
+// three bf16 values, exactly (three times 8 bits of its 24), and a product of two
+// such sums is their nine products; the six greatest (all above 2^-23 of it)
+// come out of v_mfma_f32_16x16x32_bf16, which adds in fp32.  The fp32 products,
+// v_mfma_f32_16x16x4_f32, are left to the form for few rows, which waits for
+// memory.  In both A holds rows lane % 16 and B columns lane % 16, each the summed
+// indexes of its group lane / 16, and C holds column lane % 16, rows
+// 4 (lane / 16) + r in register r.  Two consequences carry all kernels here:
+//   * a summed index may be dealt to lanes in any order that A and B share;
 //   * a product's C registers are the B operand of the next one as they
-//     stand (register r: summed index 4 (lane / 16) + r), so probabilities go
-//     from the scores to the second product without leaving their registers.
+//     stand, so probabilities go from the scores to the second product without
+//     leaving their registers.
 // Scores and probabilities are therefore formed transposed, a query (or in the
 // key gradients a key) a column: its running maximum and sum are one value a
 // lane, and rescaling is one multiplication by it.
@@ -24,8 +27,9 @@
 // The query rows of the heads that share a key head are packed into one row
 // axis r = i * group + member, so shared keys are loaded once for all of them.
 //
-// All sums, statistics and products are fp32; scores are formed in units of
-// log2 (q or k is multiplied by scale * log2(e) once, a rounding of 2^-24).
+// All sums and statistics are fp32; scores are formed in units of log2 (q or k is
+// multiplied by scale * log2(e) once, a rounding of 2^-24).  An infinity in an
+// operand's place that a mask leaves makes NaN: its parts are it and NaN.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -42,9 +46,6 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
-#ifndef PRIO
-#define PRIO
-#endif
 constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
 
@@ -512,15 +513,15 @@ __device__ __forceinline__ Parts read_columns(const char *tile, int at, int o) {
   return r;
 }
 
-// acc (columns 16 o + .. of block o) += sum over the tile's rows k of
-// x[k][column] w[k][l % 16], w the registers of a product with these rows
 template <int DU>
 __device__ __forceinline__ int columns_at(int lane) {
   typedef Dim<DU> M;
   const int l = lane & 15, r = 4 * (lane >> 4) + l / 4;
   return r * M::RC * 16 + ((l % 4 / 2 ^ M::f(r)) << 4) + l % 2 * 8;
 }
-// `a`: read_columns of block 0, which the caller has on its way by now
+// acc (columns 16 o + .. of block o) += sum over the tile's rows k of
+// x[k][column] w[k][l % 16], w the registers of a product with these rows; `a`:
+// read_columns of block 0, which the caller has on its way by now
 template <int DU, class SIDE>
 __device__ __forceinline__ void product(f32x4 (&acc)[DU], const f32x4 (&w)[2], Parts a, const char *tile, int lane,
                                         SIDE side) {
@@ -639,6 +640,39 @@ struct Stream {
   }
 };
 
+// ---- tiles split beforehand
+//
+// Where a tile is used by many workgroups, a kernel before them writes its parts
+// to memory once, as the image of a pair of tiles in LDS, and direct loads bring
+// it there: no registers hold it on the way, and the main loops' vector work
+// falls by half.  Rows outside an operand are zeros in the image.
+
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
+}
+// lane l's 16 bytes at base + off to LDS at lds + 16 l
+__device__ __forceinline__ void dma16(const char *base, int off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory");
+}
+template <int DU, int NW>
+__device__ __forceinline__ void feed(const char *image, const char *lds, int wave, int lane) {
+  constexpr int N = 2 * Dim<DU>::SIZE / 1024;  // what a wave's load moves
+  static_assert(N % NW == 0, "a pair of tiles is a whole number of loads a wave");
+  const unsigned to = lds_address(lds);
+#pragma unroll
+  for (int n = 0; n < N; n += NW) dma16(image, (n + wave) * 1024 + lane * 16, to + (n + wave) * 1024);
+}
+// what is on its way to LDS has arrived, for every wave
+__device__ __forceinline__ void arrived() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+constexpr int STATS = 4 * KT * 4;  // bytes of a row tile's statistics: lse / ln 2, delta, first key, end of keys
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // over the four lanes that hold a column: exchanges of 16 and 32 lanes between
@@ -654,6 +688,106 @@ __device__ __forceinline__ float col_sum(float x) {
   x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// ---------------------------------------------------------------- images
+
+// eight values from column c of a row on; 0 behind its end and where not `in`
+__device__ __forceinline__ void load8(float (&x)[8], const float *p, int c, bool in, int D, int vec) {
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (in) v = load4(p, c + 4 * k, D, vec);
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[4 * k + j] = v[j];
+  }
+}
+template <int DU>
+__device__ __forceinline__ bool put8(char *tile, float (&x)[8], int row, int c) {
+  typedef Dim<DU> M;
+  float t = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) t = fmaf(x[j], 0.f, t);
+  const Parts p = parts_of(x);
+  char *to = tile + row * M::RC * 16 + ((c ^ M::f(row)) << 4);
+#pragma unroll
+  for (int n = 0; n < 3; n++) *(u32x4 *)(to + n * M::PART) = p.p[n];
+  return t != t;
+}
+
+// The image of a pair of key tiles; flags: 1 where the keys hold an infinity or
+// NaN, 2 where the values do.
+template <int DU>
+__global__ void __launch_bounds__(256)
+    attn_kv_images_kernel(Args a, const float *__restrict__ k, const float *__restrict__ v, char *__restrict__ images,
+                          int *__restrict__ flags) {
+  typedef Dim<DU> M;
+  const int tiles = (a.Lk + KT - 1) / KT, bh = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = bh / a.Hkv,
+            h = bh % a.Hkv;
+  const int keys = seq_of(a, b).keys;
+  char *image = images + (long)blockIdx.x * 2 * M::SIZE;
+  if (tile * KT >= keys) return;  // behind the sequence: never read
+  bool ok = false, ov = false;
+  for (int t = threadIdx.x; t < KT * M::RC; t += 256) {
+    const int row = t / M::RC, c = t % M::RC, key = tile * KT + row;
+    const bool in = key < keys;
+    float x[8];
+    load8(x, k + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, 8 * c, in, a.D, a.vec);
+    ok |= put8<DU>(image, x, row, c);
+    load8(x, v + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, 8 * c, in, a.D, a.vec);
+    ov |= put8<DU>(image + M::SIZE, x, row, c);
+  }
+  const int f = (__syncthreads_or(ok) ? 1 : 0) | (__syncthreads_or(ov) ? 2 : 0);
+  if (threadIdx.x == 0) flags[blockIdx.x] = f;
+}
+
+// The image of a pair of tiles of packed rows, q and do, with the rows'
+// statistics behind them; delta = do . o on the way.  flags: not 0 where they
+// hold an infinity or NaN.
+template <int DU>
+__global__ void __launch_bounds__(256)
+    attn_row_images_kernel(Args a, const float *__restrict__ q, const float *__restrict__ dout,
+                           const float *__restrict__ o, const float *__restrict__ lse, float *__restrict__ delta,
+                           char *__restrict__ images, int *__restrict__ flags) {
+  typedef Dim<DU> M;
+  const int tiles = (a.R + KT - 1) / KT, bh = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = bh / a.Hkv,
+            h = bh % a.Hkv;
+  const Seq sq = seq_of(a, b);
+  char *image = images + (long)blockIdx.x * (2 * M::SIZE + STATS);
+  float *st = (float *)(image + 2 * M::SIZE);
+  bool odd = false;
+  for (int t = threadIdx.x; t < KT * M::RC; t += 256) {
+    const int row = t / M::RC, c = t % M::RC, r = tile * KT + row, i = r / a.G, hq = h * a.G + r - i * a.G;
+    const bool in = r < a.R && i < sq.queries;
+    const long oo = (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h;
+    float x[8], y[8], dl = 0.f;
+    load8(x, dout + oo, 8 * c, in, a.D, a.vec);
+    load8(y, o + oo, 8 * c, in, a.D, a.vec);
+#pragma unroll
+    for (int j = 0; j < 8; j++) dl = fmaf(x[j], y[j], dl);
+#pragma unroll
+    for (int n = 1; n < M::RC; n <<= 1) dl += __shfl_xor(dl, n);
+    odd |= put8<DU>(image + M::SIZE, x, row, c);
+    load8(x, q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, 8 * c, in, a.D, a.vec);
+    odd |= put8<DU>(image, x, row, c);
+    if (c == 0) {
+      Range rg = {0, 0};
+      float l2 = 0.f;
+      if (in) {
+        rg = range_of(a, sq, i);
+        const long at = ((long)b * a.Hkv * a.G + hq) * a.Lq + i;
+        l2 = lse[at] * LOG2E;
+        if (l2 == -INFINITY) l2 = 0.f;
+        delta[at] = dl;
+      }
+      st[row] = l2;
+      st[KT + row] = dl;
+      ((int *)st)[2 * KT + row] = rg.lo;
+      ((int *)st)[3 * KT + row] = rg.hi;
+    }
+  }
+  odd = __syncthreads_or(odd);
+  if (threadIdx.x == 0) flags[blockIdx.x] = odd;
 }
 
 // ---------------------------------------------------------------- forward
@@ -698,21 +832,24 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
   }
 }
 
-// One workgroup of NW waves: 16 packed rows a wave of one key head against the
-// keys they see, KT at a time through LDS.  With splits > 1 it takes `chunk` keys of them
-// and leaves maximum, sum and the unscaled result to the join.
-template <int DU, int NW>
+// One workgroup of NW waves: 16 packed rows a wave of one key head against
+// the keys they see, KT at a time through LDS, from memory or (PRE) from images.
+// With splits > 1 it takes `chunk` keys of them and leaves maximum, sum and the
+// unscaled result to the join.
+template <int DU, int NW, bool PRE>
 __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
-                    float *__restrict__ ws_ml, float *__restrict__ ws_o) {
+                    float *__restrict__ ws_ml, float *__restrict__ ws_o, const char *__restrict__ images,
+                    const int *__restrict__ flags) {
   typedef Dim<DU> M;
   __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
+  constexpr int ROWS = 16 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv;
-  const Item it = item_of(a, a.q_len, a.Lq, a.G, 16 * NW, gridDim.x / nbh, false);
+  const Item it = item_of(a, a.q_len, a.Lq, a.G, ROWS, gridDim.x / nbh, false);
   const int b = it.b, h = it.h, tile = it.tile, bh = b * a.Hkv + h;
-  const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
+  const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
   const Seq sq = seq_of(a, b);
   const Span sp = span_of(a, sq, r0 / a.G, (r1 - 1) / a.G);
   const Span mine = wave_span(a, sq, r0 + wave * 16, r1);
@@ -722,37 +859,45 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     if (c0 > k_first) k_first = c0 < sp.hi ? (int)c0 : sp.hi;
     if (c1 < k_end) k_end = (int)c1;
   }
-  const int row = r0 + wave * 16 + (lane & 15), i = row / a.G, hq = h * a.G + row - i * a.G;
-  const bool in = row < a.R;
-  Range rg = {0, 0};
-  if (in) rg = range_of(a, sq, i);
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
+  const long tile0 = (long)bh * ((a.Lk + KT - 1) / KT);  // of the images
   Stream<DU, 64 * NW> next;
-  next.init((int)a.k.r, (int)a.v.r, a.D, tid);
-  auto load = [&](int k0) {
-    next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
+  if constexpr (!PRE) next.init((int)a.k.r, (int)a.v.r, a.D, tid);
+  auto load = [&](int k0, int buf) {
+    if constexpr (PRE)
+      feed<DU, NW>(images + (tile0 + k0 / KT) * 2 * M::SIZE, lds[buf], wave, lane);
+    else
+      next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
   };
   auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
   bool odd = false;
-  if (k_first < k_end) load(k_first);
+  if (k_first < k_end) load(k_first, 0);
   Parts qf[M::DK];
   f32x4 acc[DU];
   float mx = -INFINITY, sum = 0.f;
+  const int row = r0 + wave * 16 + (lane & 15), i = row / a.G;
+  const bool in = row < a.R;
+  Range rg = {0, 0};
+  if (in) rg = range_of(a, sq, i);
   load_parts<DU>(qf, qp + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, in, a.scale * LOG2E, a.D, a.vec, lane);
 #pragma unroll
   for (int n = 0; n < DU; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (k_first < k_end) {
-    next.all(lds[0], 2, tid);
-    odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      next.all(lds[0], 2, tid);
+      odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+    }
   }
-  PRIO
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
+    if (PRE && is_mixed(k0)) odd = flags[tile0 + k0 / KT] & 2;
     if (odd) break;
     const char *lk = lds[buf], *lv = lk + M::SIZE;
     char *to = lds[buf ^ 1];
-    load(k0 + KT);  // zeros behind the last
+    if (!PRE || k0 + KT < k_end) load(k0 + KT, buf ^ 1);  // from memory: zeros behind the last
     if (k0 < mine.hi && k0 + KT > mine.lo) {  // this wave's rows see some of the tile
       f32x4 s[2];
       dots<DU>(s, lk, qf, lane);
@@ -778,14 +923,20 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
 #pragma unroll
       for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - base);
       sum += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-      product<DU>(acc, s, first, lv, lane, [&](int n) { next.side(n, DU, to, 2, tid); });
-    } else {
+      product<DU>(acc, s, first, lv, lane, [&](int n) {
+        if constexpr (!PRE) next.side(n, DU, to, 2, tid);
+      });
+    } else if constexpr (!PRE) {
       next.all(to, 2, tid);
     }
-    if (is_mixed(k0 + KT))
-      odd = __syncthreads_or(next.odd != next.odd);
-    else
-      __syncthreads();
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      if (is_mixed(k0 + KT))
+        odd = __syncthreads_or(next.odd != next.odd);
+      else
+        __syncthreads();
+    }
   }
   if (odd) {
     fwd_one_by_one(a, sq, b, h, r0 + wave * 16, r1, k_first, k_end, qp, kp, vp, o, lse, ws_ml, ws_o, 16 * DU, lane);
@@ -803,6 +954,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     store_columns<DU>(ws_o + at * 16 * DU, acc, 1.f, 16 * DU, 1, lane);
     return;
   }
+  const int hq = h * a.G + row - i * a.G;
   if (lse && g == 0)
     lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (mx + log2f(total)) * LN2;
   store_columns<DU>(o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h, acc, total == 0.f ? 0.f : 1.f / total,
@@ -1138,11 +1290,12 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
 
 // dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
 // forward pass
-template <int DU, int NW>
+template <int DU, int NW, bool PRE>
 __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ dout, const float *__restrict__ lse,
-                   const float *__restrict__ delta, float *__restrict__ dq) {
+                   const float *__restrict__ delta, float *__restrict__ dq, const char *__restrict__ images,
+                   const int *__restrict__ flags) {
   typedef Dim<DU> M;
   __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
@@ -1165,14 +1318,18 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
   }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
   const int k_first = sp.lo / KT * KT, k_end = sp.hi;
+  const long tile0 = (long)(b * a.Hkv + h) * ((a.Lk + KT - 1) / KT);
   Stream<DU, 64 * NW> next;
-  next.init((int)a.k.r, (int)a.v.r, a.D, tid);
-  auto load = [&](int k0) {
-    next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
+  if constexpr (!PRE) next.init((int)a.k.r, (int)a.v.r, a.D, tid);
+  auto load = [&](int k0, int buf) {
+    if constexpr (PRE)
+      feed<DU, NW>(images + (tile0 + k0 / KT) * 2 * M::SIZE, lds[buf], wave, lane);
+    else
+      next.load(kp + (long)k0 * a.k.r, vp + (long)k0 * a.v.r, (int)a.k.r, (int)a.v.r, k_end - k0, a.D, a.vec, tid);
   };
   auto is_mixed = [&](int k0) { return k0 < sp.ilo || k0 + KT > sp.ihi; };
   bool odd = false;
-  if (k_first < k_end) load(k_first);
+  if (k_first < k_end) load(k_first, 0);
   Parts qf[M::DK], df[M::DK];
   f32x4 acc[DU];
   load_parts<DU>(qf, q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, live, a.scale * LOG2E, a.D, a.vec, lane);
@@ -1180,23 +1337,28 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
 #pragma unroll
   for (int n = 0; n < DU; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (k_first < k_end) {
-    next.all(lds[0], 1, tid);
-    odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      next.all(lds[0], 1, tid);
+      odd = __syncthreads_or(next.odd != next.odd) && is_mixed(k_first);
+    }
   }
-  PRIO
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += KT, buf ^= 1) {
+    if (PRE && is_mixed(k0)) odd = flags[tile0 + k0 / KT] & 1;
     if (odd) break;
     const char *lk = lds[buf], *lv = lk + M::SIZE;
     char *to = lds[buf ^ 1];
-    load(k0 + KT);
+    if (!PRE || k0 + KT < k_end) load(k0 + KT, buf ^ 1);
     if (k0 < mine.hi && k0 + KT > mine.lo) {
       f32x4 s[2], dp[2];
       dots<DU>(s, lk, qf, lane);
       dots<DU>(dp, lv, df, lane);
       const Parts first = read_columns<DU>(lk, columns_at<DU>(lane), 0);
 #pragma unroll
-      for (int r = 0; r < 8; r++) s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - l2) * (dp[r / 4][r % 4] - dl);
+      for (int r = 0; r < 8; r++)
+        s[r / 4][r % 4] = exp2_fast(s[r / 4][r % 4] - l2) * (dp[r / 4][r % 4] - dl);
       if (is_mixed(k0)) {
 #pragma unroll
         for (int r = 0; r < 8; r++) {
@@ -1204,14 +1366,20 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
           s[r / 4][r % 4] = ((key < rg.lo) | (key >= rg.hi)) ? 0.f : s[r / 4][r % 4];
         }
       }
-      product<DU>(acc, s, first, lk, lane, [&](int n) { next.side(n, DU, to, 1, tid); });
-    } else {
+      product<DU>(acc, s, first, lk, lane, [&](int n) {
+        if constexpr (!PRE) next.side(n, DU, to, 1, tid);
+      });
+    } else if constexpr (!PRE) {
       next.all(to, 1, tid);
     }
-    if (is_mixed(k0 + KT))
-      odd = __syncthreads_or(next.odd != next.odd);
-    else
-      __syncthreads();
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      if (is_mixed(k0 + KT))
+        odd = __syncthreads_or(next.odd != next.odd);
+      else
+        __syncthreads();
+    }
   }
   if (odd) {
     dq_one_by_one(a, sq, b, h, r0 + wave * 16, r1, q, kp, vp, dout, lse, delta, dq, lane);
@@ -1221,7 +1389,7 @@ __global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
     store_columns<DU>(dq + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, acc, a.scale, a.D, a.vec, lane);
 }
 
-// the packed rows that see a key of [k0, k1)
+// the packed rows that see a key of [k0, k1), from the start of their tile on
 struct Rows {
   int first, end;
 };
@@ -1235,7 +1403,7 @@ __device__ __forceinline__ Rows rows_of(const Args &a, const Seq &s, int k0, int
   if (a.window > 0 && k1 - 1 + a.window - s.start < i1) i1 = k1 - 1 + a.window - s.start;
   Rows r = {0, 0};
   if (k0 >= s.keys || i0 >= i1) return r;
-  r.first = (int)i0 * a.G;
+  r.first = (int)i0 * a.G / KT * KT;
   r.end = (int)i1 * a.G;
   return r;
 }
@@ -1286,17 +1454,15 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
 // them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of the
 // rows and leaves its sums to the join: where many rows meet few keys, and so
 // that no fp32 sum runs over more rows than that.
-template <int DU, int NW>
+template <int DU, int NW, bool PRE>
 __global__ void __launch_bounds__(64 * NW, 2)
     attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                     const float *__restrict__ dout, const float *__restrict__ lse,
                     const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
-                    float *__restrict__ ws) {
+                    float *__restrict__ ws, const char *__restrict__ images, const int *__restrict__ flags) {
   typedef Dim<DU> M;
   constexpr int KEYS = 16 * NW;
-  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
-  __shared__ __attribute__((aligned(16))) float rl[2][KT], rd[2][KT];
-  __shared__ __attribute__((aligned(16))) int rlo[2][KT], rhi[2][KT];
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE + STATS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv;
   const Item it = item_of(a, a.k_len, a.Lk, 1, KEYS, gridDim.x / nbh, true);
@@ -1312,6 +1478,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
   const bool in = key < a.Lk, live = key < seq.keys;
   const float *qp = q + (long)b * a.q.b + (long)h * a.G * a.q.h;
   const float *op = dout + (long)b * a.o.b + (long)h * a.G * a.o.h;
+  const long tile0 = (long)bh * ((a.R + KT - 1) / KT);
   Stream<DU, 64 * NW> next;
   // row statistics of a tile, by the first KT threads
   float l2_ = 0.f, dl_ = 0.f;
@@ -1322,22 +1489,30 @@ __global__ void __launch_bounds__(64 * NW, 2)
   // mixed: a mask hides some of the tile's rows from some of the keys; touched:
   // some of the rows see some of this wave's keys
   bool next_mixed = true, next_touched = false;
-  auto load = [&](int r0) {
+  auto load = [&](int r0, int buf) {
     const Span sp = span_of(a, seq, i_next, i_next + small_div(m_next + KT - 1, a.G, magic));
     next_touched = kw < sp.hi && kw + 16 > sp.lo;
     next_mixed = r0 + KT > rows.end || k0 < sp.ilo || k0 + KEYS > sp.ihi;
-    const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
-    next.load_rows(q0, d0, a.q, a.o, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
-    if (tid < KT) {
-      const int e = m_next + tid, di = small_div(e, a.G, magic), i = i_next + di;
-      l2_ = dl_ = 0.f;
-      rg_.lo = rg_.hi = 0;
-      if (r0 + tid < rows.end) {
-        rg_ = range_of(a, seq, i);
-        const long at = ((long)b * a.Hkv * a.G + h * a.G + e - di * a.G) * a.Lq + i;
-        l2_ = lse[at] * LOG2E;
-        if (l2_ == -INFINITY) l2_ = 0.f;
-        dl_ = delta[at];
+    if constexpr (PRE) {
+      const char *from = images + (tile0 + r0 / KT) * (2 * M::SIZE + STATS);
+      if (r0 < rows.end) {
+        feed<DU, NW>(from, lds[buf], wave, lane);
+        if (wave == 0 && lane < STATS / 16) dma16(from, 2 * M::SIZE + lane * 16, lds_address(lds[buf]) + 2 * M::SIZE);
+      }
+    } else {
+      const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
+      next.load_rows(q0, d0, a.q, a.o, a.G, magic, m_next, rows.end - r0, a.D, a.vec, tid);
+      if (tid < KT) {
+        const int e = m_next + tid, di = small_div(e, a.G, magic), i = i_next + di;
+        l2_ = dl_ = 0.f;
+        rg_.lo = rg_.hi = 0;
+        if (r0 + tid < rows.end) {
+          rg_ = range_of(a, seq, i);
+          const long at = ((long)b * a.Hkv * a.G + h * a.G + e - di * a.G) * a.Lq + i;
+          l2_ = lse[at] * LOG2E;
+          if (l2_ == -INFINITY) l2_ = 0.f;
+          dl_ = delta[at];
+        }
       }
     }
     i_next += step_i;
@@ -1349,16 +1524,17 @@ __global__ void __launch_bounds__(64 * NW, 2)
   };
   auto store_statistics = [&](int to) {
     if (tid < KT) {
-      rl[to][tid] = l2_;
-      rd[to][tid] = dl_;
-      rlo[to][tid] = rg_.lo;
-      rhi[to][tid] = rg_.hi;
+      float *st = (float *)(lds[to] + 2 * M::SIZE);
+      st[tid] = l2_;
+      st[KT + tid] = dl_;
+      ((int *)st)[2 * KT + tid] = rg_.lo;
+      ((int *)st)[3 * KT + tid] = rg_.hi;
     }
   };
   if (rows.first < rows.end) {
     i_next = rows.first / a.G;
     m_next = rows.first - i_next * a.G;
-    load(rows.first);
+    load(rows.first, 0);
   }
   Parts kf[M::DK], vf[M::DK];
   f32x4 ak[DU], av[DU];
@@ -1368,18 +1544,23 @@ __global__ void __launch_bounds__(64 * NW, 2)
   for (int n = 0; n < DU; n++) ak[n] = av[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   bool odd = false;
   if (rows.first < rows.end) {
-    next.all(lds[0], 3, tid);
-    store_statistics(0);
-    odd = __syncthreads_or(next.odd != next.odd) && next_mixed;
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      next.all(lds[0], 3, tid);
+      store_statistics(0);
+      odd = __syncthreads_or(next.odd != next.odd) && next_mixed;
+    }
   }
-  PRIO
   int buf = 0;
   for (int r0 = rows.first; r0 < rows.end; r0 += KT, buf ^= 1) {
-    if (odd) break;
     const bool mixed = next_mixed, touched = next_touched;
+    if (PRE && mixed) odd = flags[tile0 + r0 / KT];
+    if (odd) break;
     const char *lq = lds[buf], *ld = lq + M::SIZE;
+    const float *st = (const float *)(lq + 2 * M::SIZE);
     char *to = lds[buf ^ 1];
-    load(r0 + KT);
+    load(r0 + KT, buf ^ 1);
     if (touched) {
       f32x4 s[2], dp[2];
       dots<DU>(s, lq, kf, lane);
@@ -1387,7 +1568,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
       const Parts first = read_columns<DU>(ld, columns_at<DU>(lane), 0);
 #pragma unroll
       for (int n = 0; n < 2; n++) {
-        const f32x4 l2 = *(const f32x4 *)(rl[buf] + 16 * n + 4 * g), dl = *(const f32x4 *)(rd[buf] + 16 * n + 4 * g);
+        const f32x4 l2 = *(const f32x4 *)(st + 16 * n + 4 * g), dl = *(const f32x4 *)(st + KT + 16 * n + 4 * g);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           s[n][j] = exp2_fast(s[n][j] - l2[j]);
@@ -1397,7 +1578,8 @@ __global__ void __launch_bounds__(64 * NW, 2)
       if (mixed) {
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-          const i32x4 lo = *(const i32x4 *)(rlo[buf] + 16 * n + 4 * g), hi = *(const i32x4 *)(rhi[buf] + 16 * n + 4 * g);
+          const i32x4 lo = *(const i32x4 *)(st + 2 * KT + 16 * n + 4 * g);
+          const i32x4 hi = *(const i32x4 *)(st + 3 * KT + 16 * n + 4 * g);
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const bool hidden = (key < lo[j]) | (key >= hi[j]);
@@ -1406,16 +1588,24 @@ __global__ void __launch_bounds__(64 * NW, 2)
           }
         }
       }
-      product<DU>(av, s, first, ld, lane, [&](int n) { next.side(n, 2 * DU, to, 3, tid); });
-      product<DU>(ak, dp, read_columns<DU>(lq, columns_at<DU>(lane), 0), lq, lane, [&](int n) { next.side(DU + n, 2 * DU, to, 3, tid); });
-    } else {
+      product<DU>(av, s, first, ld, lane, [&](int n) {
+        if constexpr (!PRE) next.side(n, 2 * DU, to, 3, tid);
+      });
+      product<DU>(ak, dp, read_columns<DU>(lq, columns_at<DU>(lane), 0), lq, lane, [&](int n) {
+        if constexpr (!PRE) next.side(DU + n, 2 * DU, to, 3, tid);
+      });
+    } else if constexpr (!PRE) {
       next.all(to, 3, tid);
     }
-    store_statistics(buf ^ 1);
-    if (next_mixed)
-      odd = __syncthreads_or(next.odd != next.odd);
-    else
-      __syncthreads();
+    if constexpr (PRE) {
+      arrived();
+    } else {
+      store_statistics(buf ^ 1);
+      if (next_mixed)
+        odd = __syncthreads_or(next.odd != next.odd);
+      else
+        __syncthreads();
+    }
   }
   if (odd) {
     dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, 16 * DU, lane);
@@ -1519,13 +1709,35 @@ void split(Plan &p, long n, long want, long least, long step) {
   p.splits = (int)((n + c - 1) / c);
 }
 
-// Rows (keys) of a workgroup.  Up to 64 columns three workgroups of four waves fit
-// a CU; above, two waves a SIMD fit in all, and one workgroup of them reads and
-// splits each tile once.
-#ifndef SMALL
-#define SMALL 64
-#endif
-int rows_of_group(const TTAttention *t) { return t->head_dim <= SMALL ? 64 : 128; }
+// bytes of a pair of tiles' image
+size_t pair_bytes(int head_dim) {
+  const int dk = (blocks(head_dim) + 1) / 2;
+  return (size_t)2 * 3 * KT * 16 * (dk == 1 ? 4 : dk == 2 ? 8 : 16);
+}
+// Tiles are split beforehand from 1024 packed rows on, where eight workgroups or
+// more use each.  us with and without, causal, 8 heads, 8192 rows in all, batches
+// of 512 / 1024 / 2048 rows:
+//   forward   64 columns  47 - 42,   68 - 71,   110 - 118
+//            128 columns  95 - 87,   132 - 136, 221 - 250
+//   backward  64 columns  128 - 129, 194 - 216, 321 - 374
+//            128 columns  277 - 337, 407 - 546, 697 - 950
+// The backward pass writes the rows' images too and has to have keys to use them
+// for (4 heads a key head, 1024 packed rows and 256 keys: 194 - 218).  At most
+// 4 GiB each: past that the tiles are split where they are used.
+constexpr long IMAGE_ROWS = 1024, IMAGE_KEYS = 256;
+bool fits_images(const TTAttention *t, long rows) {
+  return (double)t->batch * t->kv_heads * ((rows + KT - 1) / KT) * (pair_bytes(t->head_dim) + STATS) < 4294967296.;
+}
+bool images_for_rows(const TTAttention *t) {
+  return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS && fits_images(t, t->k_rows);
+}
+bool images_for_keys(const TTAttention *t) {
+  return images_for_rows(t) && t->k_rows >= IMAGE_KEYS && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
+}
+
+// Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU;
+// above, two waves a SIMD in all, and one workgroup of them reads each tile once.
+constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
 
 Plan plan_of(const TTAttention *t) {
   Plan p;
@@ -1539,7 +1751,7 @@ Plan plan_of(const TTAttention *t) {
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    p.rows = rows_of_group(t);
+    p.rows = 16 * waves(blocks(t->head_dim));
     p.tiles = (int)((R + p.rows - 1) / p.rows);
     split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
   }
@@ -1551,7 +1763,7 @@ Plan dkv_plan(const TTAttention *t) {
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = false;
-  p.rows = rows_of_group(t);
+  p.rows = 16 * waves(blocks(t->head_dim));
   p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
   // fp32 sums over at most 2048 rows
   const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
@@ -1591,29 +1803,80 @@ void run_few(const Plan &p, const Args &a, const float *q, const float *k, const
                      stream(), a, q, k, v, o, lse, ml, wo);
 }
 
+// where the images and flags lie in a workspace
+struct Images {
+  char *kv, *rows;
+  int *kv_flags, *row_flags;
+  size_t bytes;
+};
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+Images images_of(const TTAttention *t, bool kv, bool rows, void *base) {
+  const long nbh = t->batch * t->kv_heads, kt = (t->k_rows + KT - 1) / KT,
+             rt = (t->q_rows * (t->q_heads / t->kv_heads) + KT - 1) / KT;
+  const size_t pair = pair_bytes(t->head_dim);
+  const size_t n[4] = {kv ? up(nbh * kt * pair) : 0, rows ? up(nbh * rt * (pair + STATS)) : 0,
+                       kv ? up(nbh * kt * sizeof(int)) : 0, rows ? up(nbh * rt * sizeof(int)) : 0};
+  char *p = (char *)base;
+  Images m;
+  m.kv = p;
+  m.rows = p + n[0];
+  m.kv_flags = (int *)(p + n[0] + n[1]);
+  m.row_flags = (int *)(p + n[0] + n[1] + n[2]);
+  m.bytes = n[0] + n[1] + n[2] + n[3];
+  return m;
+}
+
+template <int DU>
+void run_kv_images(const Args &a, const float *k, const float *v, const Images &m) {
+  const long tiles = (long)a.B * a.Hkv * ((a.Lk + KT - 1) / KT);
+  hipLaunchKernelGGL(attn_kv_images_kernel<DU>, dim3((unsigned)tiles), dim3(256), 0, stream(), a, k, v, m.kv,
+                     m.kv_flags);
+}
+template <int DU>
+void run_row_images(const Args &a, const float *q, const float *dout, const float *o, const float *lse, float *delta,
+                    const Images &m) {
+  const long tiles = (long)a.B * a.Hkv * ((a.R + KT - 1) / KT);
+  hipLaunchKernelGGL(attn_row_images_kernel<DU>, dim3((unsigned)tiles), dim3(256), 0, stream(), a, q, dout, o, lse,
+                     delta, m.rows, m.row_flags);
+}
+
 template <int DU>
 void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
-             float *ml, float *wo) {
-  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
-  hipLaunchKernelGGL((attn_fwd_kernel<DU, NW>), dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits),
-                     dim3(64 * NW), 0, stream(), a, q, k, v, o, lse, ml, wo);
+             float *ml, float *wo, const Images *m) {
+  constexpr int NW = waves(DU);
+  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
+  if (m)
+    hipLaunchKernelGGL((attn_fwd_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, o, lse,
+                       ml, wo, m->kv, m->kv_flags);
+  else
+    hipLaunchKernelGGL((attn_fwd_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, o, lse, ml,
+                       wo, NULL, NULL);
 }
 
 template <int DU>
 void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
-            const float *delta, float *dq) {
-  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
-  const long tiles = ((long)a.R + 16 * NW - 1) / (16 * NW) * a.B * a.Hkv;
-  hipLaunchKernelGGL((attn_dq_kernel<DU, NW>), dim3((unsigned)tiles), dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
-                     delta, dq);
+            const float *delta, float *dq, const Images *m) {
+  constexpr int NW = waves(DU);
+  const dim3 grid((unsigned)(((long)a.R + 16 * NW - 1) / (16 * NW) * a.B * a.Hkv));
+  if (m)
+    hipLaunchKernelGGL((attn_dq_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta,
+                       dq, m->kv, m->kv_flags);
+  else
+    hipLaunchKernelGGL((attn_dq_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
+                       delta, dq, NULL, NULL);
 }
 
 template <int DU>
 void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
-             const float *lse, const float *delta, float *dk, float *dv, float *ws) {
-  constexpr int NW = DU * 16 <= SMALL ? 4 : 8;
-  hipLaunchKernelGGL((attn_dkv_kernel<DU, NW>), dim3((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits),
-                     dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta, dk, dv, ws);
+             const float *lse, const float *delta, float *dk, float *dv, float *ws, const Images *m) {
+  constexpr int NW = waves(DU);
+  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
+  if (m)
+    hipLaunchKernelGGL((attn_dkv_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta,
+                       dk, dv, ws, m->rows, m->row_flags);
+  else
+    hipLaunchKernelGGL((attn_dkv_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
+                       delta, dk, dv, ws, NULL, NULL);
 }
 
 #define BY_STEPS(N, F, ...)            \
@@ -1627,36 +1890,49 @@ void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const
     default: F<8>(__VA_ARGS__); break; \
   }
 
-size_t fwd_bytes(const TTAttention *t) {
-  const Plan p = plan_of(t);
-  if (p.splits <= 1) return 0;
+size_t fwd_parts(const TTAttention *t, const Plan &p) {
   const size_t rows = (size_t)t->batch * t->q_heads * t->q_rows;
-  return sizeof(float) * rows * p.splits * (2 + (size_t)p.width);
+  return p.splits > 1 ? up(sizeof(float) * rows * p.splits * (2 + (size_t)p.width)) : 0;
+}
+
+// delta of every query row, and the parts of dk and dv
+size_t delta_bytes(const TTAttention *t) { return up(sizeof(float) * t->batch * t->q_heads * t->q_rows); }
+size_t dkv_parts(const TTAttention *t, const Plan &p) {
+  return p.splits > 1 ? up(sizeof(float) * 2 * p.splits * t->batch * t->kv_heads * t->k_rows * p.width) : 0;
 }
 
 }  // namespace
 
-extern "C" size_t tt_k_attention_fwd_ws(const TTAttention *t) { return check(t) ? 0 : fwd_bytes(t); }
+extern "C" size_t tt_k_attention_fwd_ws(const TTAttention *t) {
+  if (check(t)) return 0;
+  const Plan p = plan_of(t);
+  return fwd_parts(t, p) + images_of(t, images_for_rows(t), false, NULL).bytes;
+}
 
 extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const float *k, const float *v, float *o,
                                   float *lse, void *ws) {
-  if (check(t) || !q || !k || !v || !o) return -1;
+  if (check(t) || !q || !k || !v || !o || ((uintptr_t)ws & 15)) return -1;
   if (ttrt_init() != 0) return -3;
   const Plan p = plan_of(t);
   Args a = args_of(t);
   a.splits = p.splits;
   a.chunk = p.chunk;
-  const size_t need = fwd_bytes(t);
-  float *own = NULL, *w = (float *)ws;
-  if (need && !w) {
-    w = own = (float *)ttrt_alloc(need);
+  const size_t need = tt_k_attention_fwd_ws(t);
+  void *own = NULL;
+  if (need && !ws) {
+    ws = own = ttrt_alloc(need);
     if (!own) return -2;
   }
-  float *ml = w, *wo = w ? w + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
+  float *ml = (float *)ws, *wo = ml ? ml + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
   if (p.few) {
     BY_STEPS(blocks(a.D), run_few, p, a, q, k, v, o, lse, ml, wo);
   } else {
-    BY_STEPS(blocks(a.D), run_fwd, p, a, q, k, v, o, lse, ml, wo);
+    const bool pre = images_for_rows(t);
+    const Images m = images_of(t, pre, false, (char *)ws + fwd_parts(t, p));
+    if (pre) {
+      BY_STEPS(blocks(a.D), run_kv_images, a, k, v, m);
+    }
+    BY_STEPS(blocks(a.D), run_fwd, p, a, q, k, v, o, lse, ml, wo, pre ? &m : NULL);
   }
   if (p.splits > 1) {
     const long rows = (long)a.B * a.Hkv * a.R;
@@ -1670,40 +1946,46 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   return launched();
 }
 
-// delta of every query row, and the parts of dk and dv
-static size_t delta_floats(const TTAttention *t) { return ((size_t)t->batch * t->q_heads * t->q_rows + 3) / 4 * 4; }
-
 extern "C" size_t tt_k_attention_bwd_ws(const TTAttention *t) {
   if (check(t)) return 0;
-  const Plan p = dkv_plan(t);
-  const size_t parts = p.splits > 1 ? 2 * (size_t)p.splits * t->batch * t->kv_heads * t->k_rows * p.width : 0;
-  return sizeof(float) * (delta_floats(t) + parts);
+  const bool pre = images_for_keys(t);
+  return delta_bytes(t) + dkv_parts(t, dkv_plan(t)) + images_of(t, pre, pre, NULL).bytes;
 }
 
 extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const float *k, const float *v,
                                   const float *o, const float *dout, const float *lse, float *dq, float *dk,
                                   float *dv, void *ws) {
-  if (check(t) || !q || !k || !v || !o || !dout || !lse || (dk == NULL) != (dv == NULL)) return -1;
+  if (check(t) || !q || !k || !v || !o || !dout || !lse || (dk == NULL) != (dv == NULL) || ((uintptr_t)ws & 15))
+    return -1;
   if (!dq && !dk) return 0;
   if (ttrt_init() != 0) return -3;
   Args a = args_of(t);
-  float *own = NULL, *delta = (float *)ws;
-  if (!delta) {
-    delta = own = (float *)ttrt_alloc(tt_k_attention_bwd_ws(t));
+  void *own = NULL;
+  if (!ws) {
+    ws = own = ttrt_alloc(tt_k_attention_bwd_ws(t));
     if (!own) return -2;
   }
-  const long rows = (long)a.B * a.Hkv * a.R;
-  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)),
-                     dim3(256), 0, stream(), a, o, dout, delta);
+  const Plan p = dkv_plan(t);
+  const bool pre = images_for_keys(t);
+  float *delta = (float *)ws, *parts = (float *)((char *)ws + delta_bytes(t));
+  const Images m = images_of(t, pre, pre, (char *)ws + delta_bytes(t) + dkv_parts(t, p));
+  if (pre) {
+    BY_STEPS(blocks(a.D), run_row_images, a, q, dout, o, lse, delta, m);
+  } else {
+    const long rows = (long)a.B * a.Hkv * a.R;
+    hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)),
+                       dim3(256), 0, stream(), a, o, dout, delta);
+  }
   if (dq) {
-    BY_STEPS(blocks(a.D), run_dq, a, q, k, v, dout, lse, delta, dq);
+    if (pre) {
+      BY_STEPS(blocks(a.D), run_kv_images, a, k, v, m);
+    }
+    BY_STEPS(blocks(a.D), run_dq, a, q, k, v, dout, lse, delta, dq, pre ? &m : NULL);
   }
   if (dk) {
-    const Plan p = dkv_plan(t);
     a.splits = p.splits;
     a.chunk = p.chunk;
-    float *parts = delta + delta_floats(t);
-    BY_STEPS(blocks(a.D), run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts);
+    BY_STEPS(blocks(a.D), run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts, pre ? &m : NULL);
     if (p.splits > 1) {
       const long keys = (long)a.B * a.Hkv * a.Lk;
       hipLaunchKernelGGL(attn_dkv_join_kernel, dim3((unsigned)((keys + 7) / 8 < 8192 ? (keys + 7) / 8 : 8192)),
