@@ -389,21 +389,25 @@ __device__ __forceinline__ Parts parts_of(float (&x)[8]) {
 // halve the reads of LDS, which is busy 17 % of the time, and leave one wave a
 // SIMD at 128 columns.  DB: blocks of 16 columns of a head, DK: steps of 32.
 //
-// A tile of KT rows lies in LDS as its parts, a row RC chunks of eight values
-// (a power of two), chunk c of row r at place c ^ f(r): the lanes that LDS
-// serves at once (of a read of 16 bytes: 0-3, 12-15, 20-23, 24-27 and so on: rows
-// of two groups; of a transposing read, two chunks of eight rows) meet every bank
-// once.
+// A tile of KT rows lies in LDS as its parts, a row RC chunks of eight values,
+// chunk c of row r at place c ^ f(r): the lanes that LDS serves at once (of a read
+// of 16 bytes: 0-3, 12-15, 20-23, 24-27 and so on: rows of two groups; of a
+// transposing read, two chunks of eight rows) meet every bank once.  With an odd
+// number of fours of chunks the rows' starts already differ in these.
 template <int DB>
 struct Dim {
   static constexpr int DK = (DB + 1) / 2;
-  static constexpr int RC = DK == 1 ? 4 : DK == 2 ? 8 : 16, CHUNKS = 4 * DK;
+  static constexpr int RC = 4 * DK;
   static constexpr int PART = KT * RC * 16, SIZE = 3 * PART;  // bytes of a part, of a tile
   static __device__ __forceinline__ int f(int r) {
     const int quad = ((r >> 2 ^ r >> 3) & 1) << 1 | (r >> 3 & 1);
     return RC == 16 ? (r & 3) << 2 | quad : RC == 8 ? (r >> 1 & 1) << 2 | quad : quad;
   }
-  static constexpr int TASKS = KT * CHUNKS;  // chunks of a tile
+  // the place of fours of chunks u (and, x: 0 or 2, of chunk x in it) for a lane whose place in the first is `at`
+  static __device__ __forceinline__ int four(int at, int u, int x = 0) {
+    return RC % 8 == 4 ? (at ^ x << 4) + u * 64 : at ^ (4 * u + x) << 4;
+  }
+  static constexpr int TASKS = KT * RC;  // chunks of a tile
 };
 
 // a chunk of a tile on its way from memory to LDS
@@ -428,7 +432,7 @@ struct Chunk {
   // to LDS as parts; NaN for an infinity or NaN among them, else 0
   __device__ __forceinline__ float store(char *tile, int task) const {
     typedef Dim<DU> M;
-    const int row = task / M::CHUNKS, c = task % M::CHUNKS;
+    const int row = task / M::RC, c = task % M::RC;
     float x[8], t = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -482,7 +486,7 @@ __device__ __forceinline__ void dots(f32x4 (&s)[2], const char *tile, const Part
 #pragma unroll
   for (int n = 0; n < 2 * M::DK; n++) {
     if (n + 1 < 2 * M::DK)
-      next = read_rows(tile + (at ^ (n + 1) / 2 << 6) + (n + 1) % 2 * 16 * M::RC * 16, M::PART);
+      next = read_rows(tile + M::four(at, (n + 1) / 2) + (n + 1) % 2 * 16 * M::RC * 16, M::PART);
     six(a, b[n / 2], s[n % 2]);
     step_end();
     a = next;
@@ -506,7 +510,7 @@ __device__ __forceinline__ Parts read_columns(const char *tile, int at, int o) {
   for (int n = 0; n < 3; n++)
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      const u32x2 w = read_transposed(tile + n * M::PART + (at ^ 2 * o << 4) + 16 * x * M::RC * 16);
+      const u32x2 w = read_transposed(tile + n * M::PART + M::four(at, o / 2, o % 2 * 2) + 16 * x * M::RC * 16);
       r.p[n][2 * x] = w[0];
       r.p[n][2 * x + 1] = w[1];
     }
@@ -572,8 +576,8 @@ struct Stream {
   static __device__ __forceinline__ bool has(int t) { return 2 * M::TASKS % NT == 0 || t < 2 * M::TASKS; }
   // a wave's chunks are of one tile of the two
   static __device__ __forceinline__ bool second(int t) { return __builtin_amdgcn_readfirstlane(t) >= M::TASKS; }
-  static __device__ __forceinline__ int row_of(int t) { return t % M::TASKS / M::CHUNKS; }
-  static __device__ __forceinline__ int col_of(int t) { return t % M::TASKS % M::CHUNKS * 8; }
+  static __device__ __forceinline__ int row_of(int t) { return t % M::TASKS / M::RC; }
+  static __device__ __forceinline__ int col_of(int t) { return t % M::TASKS % M::RC * 8; }
 
   __device__ __forceinline__ void init(int s0, int s1, int D, int tid) {
 #pragma unroll
@@ -660,10 +664,10 @@ __device__ __forceinline__ void dma16(const char *base, int off, unsigned lds) {
 template <int DU, int NW>
 __device__ __forceinline__ void feed(const char *image, const char *lds, int wave, int lane) {
   constexpr int N = 2 * Dim<DU>::SIZE / 1024;  // what a wave's load moves
-  static_assert(N % NW == 0, "a pair of tiles is a whole number of loads a wave");
   const unsigned to = lds_address(lds);
 #pragma unroll
-  for (int n = 0; n < N; n += NW) dma16(image, (n + wave) * 1024 + lane * 16, to + (n + wave) * 1024);
+  for (int n = 0; n < N; n += NW)
+    if (N % NW == 0 || n + wave < N) dma16(image, (n + wave) * 1024 + lane * 16, to + (n + wave) * 1024);
 }
 // what is on its way to LDS has arrived, for every wave
 __device__ __forceinline__ void arrived() {
@@ -689,6 +693,12 @@ __device__ __forceinline__ float col_sum(float x) {
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
+
+// Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU;
+// above, two waves a SIMD in all, and one workgroup of them reads each tile once.
+constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
+// waves a SIMD that the registers have to allow
+constexpr int fwd_lives(int DU, bool pre) { return DU <= 4 ? 3 : DU <= 6 && pre ? 4 : 2; }
 
 // ---------------------------------------------------------------- images
 
@@ -756,8 +766,9 @@ __global__ void __launch_bounds__(256)
   char *image = images + (long)blockIdx.x * (2 * M::SIZE + STATS);
   float *st = (float *)(image + 2 * M::SIZE);
   bool odd = false;
-  for (int t = threadIdx.x; t < KT * M::RC; t += 256) {
-    const int row = t / M::RC, c = t % M::RC, r = tile * KT + row, i = r / a.G, hq = h * a.G + r - i * a.G;
+  constexpr int W = M::RC <= 4 ? 4 : M::RC <= 8 ? 8 : 16;  // lanes of a row
+  for (int t = threadIdx.x; t < KT * W; t += 256) {
+    const int row = t / W, c = t % W, r = tile * KT + row, i = r / a.G, hq = h * a.G + r - i * a.G;
     const bool in = r < a.R && i < sq.queries;
     const long oo = (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h;
     float x[8], y[8], dl = 0.f;
@@ -766,10 +777,10 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int j = 0; j < 8; j++) dl = fmaf(x[j], y[j], dl);
 #pragma unroll
-    for (int n = 1; n < M::RC; n <<= 1) dl += __shfl_xor(dl, n);
-    odd |= put8<DU>(image + M::SIZE, x, row, c);
+    for (int n = 1; n < W; n <<= 1) dl += __shfl_xor(dl, n);
+    if (c < M::RC) odd |= put8<DU>(image + M::SIZE, x, row, c);
     load8(x, q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h, 8 * c, in, a.D, a.vec);
-    odd |= put8<DU>(image, x, row, c);
+    if (c < M::RC) odd |= put8<DU>(image, x, row, c);
     if (c == 0) {
       Range rg = {0, 0};
       float l2 = 0.f;
@@ -837,7 +848,7 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
 // With splits > 1 it takes `chunk` keys of them and leaves maximum, sum and the
 // unscaled result to the join.
 template <int DU, int NW, bool PRE>
-__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
+__global__ void __launch_bounds__(64 * NW, fwd_lives(DU, PRE))
     attn_fwd_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o, const char *__restrict__ images,
@@ -1173,10 +1184,57 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
 // The parts of a row that several workgroups took, joined in their order by a
 // workgroup of W waves: first the weights of all parts, then the values, the
 // waves every W-th part each.  A part without keys has sum 0 and no values.
-template <int W>
-__global__ void __launch_bounds__(64 * W)
+__device__ __forceinline__ void join_store(const Args &a, long at, float top, float total, float2 x, int lane,
+                                           float *o, float *lse) {
+  const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
+  const int hq = bh % a.Hkv * a.G + r - i * a.G;
+  if (lse && lane == 0)
+    lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+  float *q = o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h + 2 * lane;
+  const float f = total == 0.f ? 0.f : 1.f / total;
+  if (2 * lane < a.D) q[0] = x.x * f;
+  if (2 * lane + 1 < a.D) q[1] = x.y * f;
+}
+
+// Up to FEW_PARTS parts: a wave a row, the parts' weights in its lanes.
+constexpr int FEW_PARTS = 8;
+__global__ void __launch_bounds__(256)
+    attn_join_few_kernel(Args a, int width, const float *__restrict__ ws_ml, const float *__restrict__ ws_o,
+                         float *__restrict__ o, float *__restrict__ lse) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long rows = (long)a.B * a.Hkv * a.R;
+  for (long at = blockIdx.x * 4L + wave; at < rows; at += gridDim.x * 4L) {
+    float2 v[FEW_PARTS], ml = make_float2(-INFINITY, 0.f);
+    const float *p = ws_o + at * width + 2 * lane;
+    if (lane < a.splits) ml = *(const float2 *)(ws_ml + 2 * (lane * rows + at));
+#pragma unroll
+    for (int s = 0; s < FEW_PARTS; s++) {
+      v[s] = make_float2(0.f, 0.f);
+      if (s < a.splits && 2 * lane < width) v[s] = *(const float2 *)(p + s * rows * width);
+    }
+    float top = ml.x;
+#pragma unroll
+    for (int x = 1; x < FEW_PARTS; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -INFINITY ? 0.f : top, f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - base);
+    float total = f * ml.y;
+#pragma unroll
+    for (int x = 1; x < FEW_PARTS; x <<= 1) total += __shfl_xor(total, x);
+    total = __shfl(total, 0);
+    float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < FEW_PARTS; s++) {
+      const float w = __shfl(f, s);
+      x.x = w == 0.f ? x.x : fmaf(w, v[s].x, x.x);
+      x.y = w == 0.f ? x.y : fmaf(w, v[s].y, x.y);
+    }
+    join_store(a, at, __shfl(top, 0), total, x, lane, o, lse);
+  }
+}
+
+__global__ void __launch_bounds__(256)
     attn_join_kernel(Args a, int width, const float *__restrict__ ws_ml, const float *__restrict__ ws_o,
                      float *__restrict__ o, float *__restrict__ lse) {
+  constexpr int W = 4;
   __shared__ float weight[MAX_SPLITS];
   __shared__ float2 sums[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1208,25 +1266,14 @@ __global__ void __launch_bounds__(64 * W)
         x.y = f == 0.f ? x.y : fmaf(f, v.y, x.y);
       }
     }
-    if (W > 1) {
-      sums[wave][lane] = x;
-      __syncthreads();
+    sums[wave][lane] = x;
+    __syncthreads();
 #pragma unroll
-      for (int w = 1; w < W; w++) {
-        x.x += sums[w][lane].x;
-        x.y += sums[w][lane].y;
-      }
+    for (int w = 1; w < W; w++) {
+      x.x += sums[w][lane].x;
+      x.y += sums[w][lane].y;
     }
-    if (wave == 0) {
-      const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
-      const int hq = bh % a.Hkv * a.G + r - i * a.G;
-      if (lse && lane == 0)
-        lse[((long)b * a.Hkv * a.G + hq) * a.Lq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
-      float *q = o + (long)b * a.o.b + (long)i * a.o.r + (long)hq * a.o.h + 2 * lane;
-      const float f = total == 0.f ? 0.f : 1.f / total;
-      if (2 * lane < a.D) q[0] = x.x * f;
-      if (2 * lane + 1 < a.D) q[1] = x.y * f;
-    }
+    if (wave == 0) join_store(a, at, top, total, x, lane, o, lse);
     __syncthreads();
   }
 }
@@ -1711,8 +1758,7 @@ void split(Plan &p, long n, long want, long least, long step) {
 
 // bytes of a pair of tiles' image
 size_t pair_bytes(int head_dim) {
-  const int dk = (blocks(head_dim) + 1) / 2;
-  return (size_t)2 * 3 * KT * 16 * (dk == 1 ? 4 : dk == 2 ? 8 : 16);
+  return (size_t)2 * 3 * KT * 16 * 4 * ((blocks(head_dim) + 1) / 2);
 }
 // Tiles are split beforehand from 1024 packed rows on, where eight workgroups or
 // more use each.  us with and without, causal, 8 heads, 8192 rows in all, batches
@@ -1734,10 +1780,6 @@ bool images_for_rows(const TTAttention *t) {
 bool images_for_keys(const TTAttention *t) {
   return images_for_rows(t) && t->k_rows >= IMAGE_KEYS && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
 }
-
-// Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU;
-// above, two waves a SIMD in all, and one workgroup of them reads each tile once.
-constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
 
 Plan plan_of(const TTAttention *t) {
   Plan p;
@@ -1936,11 +1978,12 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   }
   if (p.splits > 1) {
     const long rows = (long)a.B * a.Hkv * a.R;
-    const dim3 grid((unsigned)(rows < 65536 ? rows : 65536));
-    if (p.splits > 8)
-      hipLaunchKernelGGL(attn_join_kernel<4>, grid, dim3(256), 0, stream(), a, p.width, ml, wo, o, lse);
+    if (p.splits <= FEW_PARTS)
+      hipLaunchKernelGGL(attn_join_few_kernel, dim3((unsigned)((rows + 3) / 4 < 65536 ? (rows + 3) / 4 : 65536)),
+                         dim3(256), 0, stream(), a, p.width, ml, wo, o, lse);
     else
-      hipLaunchKernelGGL(attn_join_kernel<1>, grid, dim3(64), 0, stream(), a, p.width, ml, wo, o, lse);
+      hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256), 0, stream(), a,
+                         p.width, ml, wo, o, lse);
   }
   ttrt_free(own);
   return launched();
