@@ -71,7 +71,8 @@ def test_head_sizes(tlib, D):
 @pytest.mark.parametrize("D", [8, 31, 40, 64, 80, 95, 100, 128])
 @pytest.mark.parametrize("masks", [
     dict(causal=True), dict(), dict(window=50),
-    dict(causal=True, window=77, k_len=[330, 0, 100], q_len=[300, 7, 33], q_start=[30, 0, 67])])
+    dict(causal=True, window=77, k_len=[330, 0, 100], q_len=[300, 7, 33], q_start=[30, 0, 67]),
+    dict(causal=True, q_start=[2147483647, -2147483648, -7]), dict(window=3, q_start=[2147483647, -200, 300])])
 def test_many_rows(tlib, D, masks):
     """From 1024 packed rows on the tiles are split into parts beforehand."""
     _check(tlib, *_inputs(3, 300, 330, 4, 1, D), masks)
@@ -142,7 +143,8 @@ def test_padding_is_not_read(tlib, Lq, Lk, Hq):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(70, 70, 2, 2), (4, 90, 4, 2), (200, 300, 3, 1), (300, 300, 4, 1)])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(70, 70, 2, 2), (4, 90, 4, 2), (200, 300, 3, 1), (300, 300, 4, 1),
+                                           (40, 2000, 2, 1), (1100, 600, 1, 1)])
 def test_what_a_mask_hides_stays_hidden(tlib, bad, Lq, Lk, Hq, Hkv):
     """A causal mask over infinities and NaN in one key's and one query's rows:
     what does not see them stays within its bounds, results and gradients."""
@@ -266,6 +268,19 @@ def test_keys_split_over_workgroups(tlib, Lq, Lk, Hq, Hkv):
         tlib.tth_fail_alloc_after(-1)
     assert rc == 0 and none == -2
     assert np.array_equal(o.to_np(q.shape), got["o"])
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H", [(100, 40, 50, 1), (64, 70, 33, 3), (2, 33, 17000, 1), (2, 17000, 40, 1),
+                                       (3, 1100, 1500, 2)])
+def test_ragged_batches_over_many_workgroups(tlib, B, Lq, Lk, H):
+    """Batches of up to 64 sequences, and up to 256 tiles of a sequence, are taken
+    tile by tile from the fullest on; others in their own order.  Every row and
+    key is written once, whatever the lengths."""
+    t = _inputs(B, Lq, Lk, H, H, 16)
+    rng = np.random.default_rng(B)
+    q_len, k_len = rng.integers(0, Lq + 1, B), rng.integers(0, Lk + 1, B)
+    k_len[-1], q_len[0] = Lk, Lq
+    _check(tlib, *t, dict(k_len=k_len, q_len=q_len, q_start=np.zeros(B, np.int64), causal=Lq > Lk))
 
 
 @pytest.mark.parametrize("Lq,Lk", [(40, 60), (700, 300)])

@@ -1,6 +1,8 @@
 """The transformer operators together: a block trained by distillation, its
 gradients against differences of the same block in 64 bits; and tokens
 answered one at a time from a cache, against the whole text at once."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -170,3 +172,93 @@ def test_tokens_from_a_cache(tlib, interleaved):
     want = ref.attention(x[:, :, :HQ], x[:, :, HQ:HQ + HKV], x[:, :, HQ + HKV:], ref.seen(1, T, T, causal=True))["o"]
     ref.close(whole, want)
     ref.close(got, want)
+
+
+def test_calls_captured_into_a_graph(tlib):
+    """With workspaces of the caller's the operators are captured, forward and
+    backward, and replayed over new inputs with eager work in between: the
+    eager bits each time."""
+    hip = {n: getattr(tlib, n) for n in ("hipStreamBeginCapture", "hipStreamEndCapture", "hipGraphInstantiate",
+                                         "hipGraphLaunch", "hipGraphExecDestroy", "hipGraphDestroy")}
+    hip["hipStreamBeginCapture"].argtypes = [ctypes.c_void_p, ctypes.c_int]
+    hip["hipStreamEndCapture"].argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    hip["hipGraphInstantiate"].argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_size_t]
+    for n in ("hipGraphExecDestroy", "hipGraphDestroy"):
+        hip[n].argtypes = [ctypes.c_void_p]
+    hip["hipGraphLaunch"].argtypes = [ctypes.c_void_p] * 2
+    stream = ctypes.c_void_p(tlib.tth_stream())
+    rng = np.random.default_rng(4)
+    nb, rows, hq, hkv, dim, cols, top = 2, 300, 8, 2, 32, 500, 6
+    rope = Rope(head_dim=dim, rot_dim=dim, base=10000.0)
+    shapes = dict(x=(nb * rows, hq * dim), w=(hq * dim,), k=(nb * rows, hkv * dim), v=(nb * rows, hkv * dim),
+                  do=(nb * rows, hq * dim), z=(nb * rows, cols), teacher=(nb * rows, top))
+    given = {n: DevBuf(int(np.prod(s))) for n, s in shapes.items()}
+    ids = DevBuf.from_np(rng.integers(0, cols, (nb * rows, top)).astype(np.int32))
+    wide, narrow, per_row = nb * rows * hq * dim, nb * rows * hkv * dim, nb * rows
+
+    def outputs():
+        return dict(y=DevBuf(wide), mean=DevBuf(per_row), rstd=DevBuf(per_row), q=DevBuf(wide), o=DevBuf(wide),
+                    one=DevBuf(nb * hq * dim), lse=DevBuf(nb * hq * rows), dq=DevBuf(wide), dk=DevBuf(narrow),
+                    dv=DevBuf(narrow), dy=DevBuf(wide), dx=DevBuf(wide), dw=DevBuf(hq * dim), db=DevBuf(hq * dim),
+                    loss=DevBuf(per_row), dz=DevBuf(per_row * cols))
+
+    a = Attention(batch=nb, q_rows=rows, k_rows=rows, q_heads=hq, kv_heads=hkv, head_dim=dim, causal=1)
+    few = Attention(batch=nb, q_rows=1, k_rows=rows, q_heads=hq, kv_heads=hkv, head_dim=dim)
+    need = (tlib.tt_k_attention_fwd_ws(a), tlib.tt_k_attention_fwd_ws(few), tlib.tt_k_attention_bwd_ws(a),
+            tlib.tt_k_layernorm_bwd_ws(per_row, hq * dim))
+    assert need[0] and need[1] and need[2] and need[3]
+    ws = [DevBuf(n // 4 + 1) for n in need]
+
+    def run(out):
+        o = {n: d.ptr for n, d in out.items()}
+        i = {n: d.ptr for n, d in given.items()}
+        L = tlib
+        check(L.tt_k_layernorm_fwd(i["x"], i["w"], None, o["y"], o["mean"], o["rstd"], per_row, hq * dim, 1e-5), "ln")
+        check(L.tt_k_rope(rope, o["y"], o["q"], None, per_row, rows, hq, 0, 0, 0), "rope")
+        check(L.tt_k_attention_fwd(a, o["q"], i["k"], i["v"], o["o"], o["lse"], ws[0].ptr), "attention")
+        check(L.tt_k_attention_fwd(few, o["q"], i["k"], i["v"], o["one"], None, ws[1].ptr), "attention")
+        check(L.tt_k_attention_bwd(a, o["q"], i["k"], i["v"], o["o"], i["do"], o["lse"], o["dq"], o["dk"], o["dv"],
+                                   ws[2].ptr), "attention")
+        check(L.tt_k_rope(rope, o["dq"], o["dy"], None, per_row, rows, hq, 0, 0, 1), "rope")
+        check(L.tt_k_layernorm_bwd(i["x"], i["w"], o["dy"], o["mean"], o["rstd"], o["dx"], o["dw"], o["db"], per_row,
+                                   hq * dim, ws[3].ptr), "ln")
+        check(L.tt_k_distill(i["z"], ids.ptr, i["teacher"], top, 2.0, o["loss"], o["dz"], per_row, cols, 1.0), "distill")
+
+    def renew():
+        for n, d in given.items():
+            x = rng.standard_normal(shapes[n]).astype(np.float32)
+            check(tlib.tth_h2d(d.ptr, x.ctypes.data, x.nbytes), "h2d")
+
+    renew()
+    got, want = outputs(), outputs()
+    run(want)
+    check(tlib.tth_sync(), "sync")
+    graph, ready = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip["hipStreamBeginCapture"](stream, 1) == 0
+    try:
+        run(got)
+    finally:
+        rc = hip["hipStreamEndCapture"](stream, ctypes.byref(graph))
+    assert rc == 0
+    assert hip["hipGraphInstantiate"](ctypes.byref(ready), graph, None, None, 0) == 0
+    try:
+        for replay in range(4):
+            renew()
+            for d in got.values():
+                d.fill(np.nan)
+            for d in ws:
+                d.fill(np.nan)
+            if replay % 2:
+                run(want)
+                check(tlib.tth_sync(), "sync")
+            assert hip["hipGraphLaunch"](ready, stream) == 0
+            check(tlib.tth_sync(), "sync")
+            if replay % 2 == 0:
+                run(want)
+            for n in got:
+                assert np.array_equal(got[n].to_np().view(np.uint32), want[n].to_np().view(np.uint32)), (replay, n)
+                assert np.isfinite(got[n].to_np()).all(), n
+    finally:
+        check(tlib.tth_sync(), "sync")
+        assert hip["hipGraphExecDestroy"](ready) == 0
+        assert hip["hipGraphDestroy"](graph) == 0

@@ -145,7 +145,7 @@ class Node:
 
     def layernorm(self, w=None, b=None, eps=1e-5):
         """Layer norm over the last axis, times w plus b."""
-        return Node(_checked(LIB.ag_layernorm(self.ptr, w.ptr if w else None, b.ptr if b else None, eps),
+        return Node(_checked(LIB.ag_layernorm(self.ptr, None if w is None else w.ptr, None if b is None else b.ptr, eps),
                              "ag_layernorm"))
 
     def rope(self, heads, head_dim, positions=None, seq_len=0, rot_dim=None, interleaved=False, base=10000.0,
