@@ -1181,9 +1181,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
   }
 }
 
-// The parts of a row that several workgroups took, joined in their order by a
-// workgroup of W waves: first the weights of all parts, then the values, the
-// waves every W-th part each.  A part without keys has sum 0 and no values.
+// The parts of a row that several workgroups took, joined in a fixed order.  A
+// part without keys has sum 0 and no values.
 __device__ __forceinline__ void join_store(const Args &a, long at, float top, float total, float2 x, int lane,
                                            float *o, float *lse) {
   const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
@@ -1231,49 +1230,73 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-__global__ void __launch_bounds__(256)
+// More parts: a workgroup a row.  The weights of all parts first; then the
+// values, four columns a thread and as many parts at once as threads allow, so
+// that few loads wait for each other (256 parts of 64 columns: 28 us with a wave
+// for every fourth part, 5.4 so).
+constexpr int JOIN = 512;
+__global__ void __launch_bounds__(JOIN)
     attn_join_kernel(Args a, int width, const float *__restrict__ ws_ml, const float *__restrict__ ws_o,
                      float *__restrict__ o, float *__restrict__ lse) {
-  constexpr int W = 4;
   __shared__ float weight[MAX_SPLITS];
-  __shared__ float2 sums[W][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float red[2][JOIN / 64];
+  __shared__ __attribute__((aligned(16))) float sums[JOIN * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lanes = width / 4, groups = JOIN / lanes, group = tid / lanes, c = tid % lanes * 4;
   const long rows = (long)a.B * a.Hkv * a.R;
   for (long at = blockIdx.x; at < rows; at += gridDim.x) {
-    float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ws_ml[2 * (s * rows + at)]);
+    float2 ml[MAX_SPLITS / JOIN];
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int n = 0; n < MAX_SPLITS / JOIN; n++) {
+      const int s = n * JOIN + tid;
+      ml[n] = make_float2(-INFINITY, 0.f);
+      if (s < a.splits) ml[n] = *(const float2 *)(ws_ml + 2 * (s * rows + at));
+      top = fmaxf(top, ml[n].x);
+    }
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < JOIN / 64; w++) top = fmaxf(top, red[0][w]);
     const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    for (int s = lane; s < a.splits; s += 64) {
-      const float2 ml = *(const float2 *)(ws_ml + 2 * (s * rows + at));
-      const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - base);
-      if (wave == 0) weight[s] = f;
-      total = fmaf(f, ml.y, total);
+#pragma unroll
+    for (int n = 0; n < MAX_SPLITS / JOIN; n++) {
+      const float f = ml[n].y == 0.f ? 0.f : exp2_fast(ml[n].x - base);
+      weight[n * JOIN + tid] = f;
+      total = fmaf(f, ml[n].y, total);
     }
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
+    if (lane == 0) red[1][wave] = total;
     __syncthreads();
-    float2 x = make_float2(0.f, 0.f);
-    const float *p = ws_o + at * width + 2 * lane;
-    if (2 * lane < width) {
-#pragma unroll 4
-      for (int s = wave; s < a.splits; s += W) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (group < groups) {
+      const float *p = ws_o + at * width + c;
+#pragma unroll 8
+      for (int s = group; s < a.splits; s += groups) {
         const float f = weight[s];
-        const float2 v = *(const float2 *)(p + s * rows * width);
-        x.x = f == 0.f ? x.x : fmaf(f, v.x, x.x);
-        x.y = f == 0.f ? x.y : fmaf(f, v.y, x.y);
-      }
-    }
-    sums[wave][lane] = x;
-    __syncthreads();
+        const f32x4 v = *(const f32x4 *)(p + s * rows * width);
 #pragma unroll
-    for (int w = 1; w < W; w++) {
-      x.x += sums[w][lane].x;
-      x.y += sums[w][lane].y;
+        for (int j = 0; j < 4; j++) x[j] = f == 0.f ? x[j] : fmaf(f, v[j], x[j]);
+      }
+      *(f32x4 *)(sums + group * width + c) = x;
     }
-    if (wave == 0) join_store(a, at, top, total, x, lane, o, lse);
+    total = 0.f;
+#pragma unroll
+    for (int w = 0; w < JOIN / 64; w++) total += red[1][w];
+    __syncthreads();
+    if (wave == 0) {
+      float2 y = make_float2(0.f, 0.f);
+      if (2 * lane < width)
+        for (int g = 0; g < groups && g < a.splits; g++) {
+          const float2 v = *(const float2 *)(sums + g * width + 2 * lane);
+          y.x += v.x;
+          y.y += v.y;
+        }
+      join_store(a, at, top, total, y, lane, o, lse);
+    }
     __syncthreads();
   }
 }
@@ -1788,8 +1811,10 @@ Plan plan_of(const TTAttention *t) {
   p.width = 16 * blocks(t->head_dim);
   if (p.few) {
     p.tiles = 1;
-    // parts of 64 to 1024 keys, about eight workgroups a CU
-    long c = (nbh * t->k_rows / 2048 + 63) / 64 * 64;
+    // parts of 64 to 1024 keys, about two workgroups a CU (eight: 8 heads of 32768
+    // keys of 128 columns 71 us, so 51; 64 of 2048 keys 44 and 30; half as many: 52
+    // and 29)
+    long c = (nbh * t->k_rows / 512 + 63) / 64 * 64;
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
@@ -1982,7 +2007,7 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
       hipLaunchKernelGGL(attn_join_few_kernel, dim3((unsigned)((rows + 3) / 4 < 65536 ? (rows + 3) / 4 : 65536)),
                          dim3(256), 0, stream(), a, p.width, ml, wo, o, lse);
     else
-      hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256), 0, stream(), a,
+      hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(JOIN), 0, stream(), a,
                          p.width, ml, wo, o, lse);
   }
   ttrt_free(own);
