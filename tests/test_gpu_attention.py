@@ -144,7 +144,7 @@ def test_padding_is_not_read(tlib, Lq, Lk, Hq):
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(70, 70, 2, 2), (4, 90, 4, 2), (200, 300, 3, 1), (300, 300, 4, 1),
-                                           (40, 2000, 2, 1), (1100, 600, 1, 1)])
+                                           (40, 2000, 2, 1), (1100, 600, 1, 1), (24, 90, 1, 1)])
 def test_what_a_mask_hides_stays_hidden(tlib, bad, Lq, Lk, Hq, Hkv):
     """A causal mask over infinities and NaN in one key's and one query's rows:
     what does not see them stays within its bounds, results and gradients."""
@@ -244,7 +244,7 @@ def test_layouts(tlib, kind, Lq, Hq):
                 ref.close(_unlayout(d.to_np(), kind, p[1], x.shape), want[n], n)
 
 
-@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(1, 5000, 4, 2), (2, 1300, 4, 1), (1, 130, 16, 16), (20, 5000, 4, 2),
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(1, 5000, 4, 2), (2, 1300, 4, 1), (1, 130, 16, 16), (24, 3000, 1, 1), (20, 5000, 4, 2),
                                           (130, 2000, 1, 1), (600, 2000, 2, 1)])
 def test_keys_split_over_workgroups(tlib, Lq, Lk, Hq, Hkv):
     """Long caches with ragged lengths, some within the first part; the parts
