@@ -143,8 +143,40 @@ __device__ __forceinline__ void finish(const Call &a, long row, const Entries &e
   if (lane == 0) a.rowloss[row] = e.mass == 0.f ? 0.f : loss * a.t2;
 }
 
-// a row of up to 4 NT NV columns; TAIL: their number is no multiple of 4, and
-// the last group of 4 is taken value by value
+// A thread's groups of four columns, from column c on.  With TAIL (cols not a
+// multiple of 4, and more than 4) the groups at and behind the row's end are its
+// last four columns, of which a thread's own are those that no other has: every
+// load is one instruction with no branch around it, and none waits for the one
+// before.
+template <bool TAIL>
+struct Group {
+  int at, by;  // where it is loaded from; its first value that is the thread's own (TAIL: 4 and more: none)
+  __device__ __forceinline__ Group(int c, int cols) {
+    at = TAIL && c > cols - 4 ? cols - 4 : c;
+    by = TAIL ? c - at : c < cols ? 0 : 4;
+  }
+  __device__ __forceinline__ f32x4 load(const float *p) const {
+    f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (TAIL || by == 0) v = *(const f32x4_any *)(p + at);
+    return v;
+  }
+  __device__ __forceinline__ void mask(f32x4 &v) const {
+    if (!TAIL) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = j >= by ? v[j] : -INFINITY;
+  }
+  __device__ __forceinline__ void store(float *p, f32x4 v) const {
+    if (by == 0) {
+      *(f32x4_any *)(p + at) = v;
+    } else if (TAIL) {
+#pragma unroll
+      for (int j = 1; j < 4; j++)
+        if (j >= by) p[at + j] = v[j];
+    }
+  }
+};
+
+// a row of up to 4 NT NV columns; TAIL: their number is no multiple of 4
 template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
   __shared__ float part[NT / 64];
@@ -154,18 +186,10 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
     const float *z = a.z + row * a.cols;
     f32x4 v[NV];
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-      v[n] = (f32x4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      const int c = (n * NT + t) * 4;
-      if (c + (TAIL ? 3 : 0) < a.cols) {
-        v[n] = *(const f32x4_any *)(z + c);
-      } else if (TAIL) {
-#pragma unroll
-        for (int j = 0; j < 3; j++)
-          if (c + j < a.cols) v[n][j] = z[c + j];
-      }
-    }
+    for (int n = 0; n < NV; n++) v[n] = Group<TAIL>((n * NT + t) * 4, a.cols).load(z);
     if (t < 64) read_entries(a, row, e, t);
+#pragma unroll
+    for (int n = 0; n < NV; n++) Group<TAIL>((n * NT + t) * 4, a.cols).mask(v[n]);
     float most = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NV; n++) most = fmaxf(most, fmaxf(fmaxf(v[n][0], v[n][1]), fmaxf(v[n][2], v[n][3])));
@@ -176,9 +200,8 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
     for (int n = 0; n < NV; n++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int c = (n * NT + t) * 4 + j;
         float x = flat ? 1.f : exp2_fast((v[n][j] - most) * a.c);
-        if (c >= a.cols) x = 0.f;
+        if (j < Group<TAIL>((n * NT + t) * 4, a.cols).by) x = 0.f;
         v[n][j] = x;
         sum += x;
       }
@@ -190,14 +213,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
 #pragma unroll
       for (int n = 0; n < NV; n++) {
         v[n] *= f;
-        const int c = (n * NT + t) * 4;
-        if (c + (TAIL ? 3 : 0) < a.cols) {
-          *(f32x4_any *)(dz + c) = v[n];
-        } else if (TAIL) {
-#pragma unroll
-          for (int j = 0; j < 3; j++)
-            if (c + j < a.cols) dz[c + j] = v[n][j];
-        }
+        Group<TAIL>((n * NT + t) * 4, a.cols).store(dz, v[n]);
       }
     }
     __syncthreads();  // the row is written: its entries' columns may be
@@ -206,25 +222,70 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
   }
 }
 
-// longer rows: maximum and sum in a first pass, the gradient in a second
+// Longer rows: running maximum and sum in a first pass, the gradient in a second
+// that finds most of the row in a cache.  TINY: rows of up to 3 columns.
+template <bool TINY>
 __global__ void __launch_bounds__(1024) distill_long_kernel(Call a) {
+  constexpr int U = 4, STEP = U * 4096;  // groups of four on their way at once
   __shared__ float part[16];
   __shared__ Entries e;
   const int t = threadIdx.x;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float *z = a.z + row * a.cols;
+    // groups past the end take its last columns, and none of them as their own
+    auto group = [&](long c) { return Group<true>((int)(c < a.cols ? c : a.cols), a.cols); };
+    auto load = [&](f32x4(&v)[U], long c0) {
+      if (TINY) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[u][j] = u == 0 && c0 + j < a.cols ? z[c0 + j] : -INFINITY;
+        return;
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) v[u] = group(c0 + u * 4096).load(z);
+#pragma unroll
+      for (int u = 0; u < U; u++) group(c0 + u * 4096).mask(v[u]);
+    };
     if (t < 64) read_entries(a, row, e, t);
-    float most = -INFINITY;
-    for (long c = t; c < a.cols; c += 1024) most = fmaxf(most, z[c]);
+    float most = -INFINITY, sum = 0.f;
+    for (long c0 = 4 * t; c0 < a.cols; c0 += STEP) {
+      f32x4 v[U];
+      load(v, c0);
+      float top = most;
+#pragma unroll
+      for (int u = 0; u < U; u++) top = fmaxf(top, fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])));
+      const float base = top == -INFINITY ? 0.f : top;
+      sum *= exp2_fast((most - base) * a.c);
+      most = top;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum += exp2_fast((v[u][j] - base) * a.c);
+    }
+    const float mine = most;
     most = group_all<1024>(most, part, Max());
     const bool flat = most == -INFINITY;
-    float sum = 0.f;
-    for (long c = t; c < a.cols; c += 1024) sum += flat ? 1.f : exp2_fast((z[c] - most) * a.c);
+    sum *= flat ? 0.f : exp2_fast((mine - most) * a.c);
     sum = group_all<1024>(sum, part, Add());
+    if (flat) sum += (float)a.cols;  // equal logits; a NaN stays
     if (a.dz) {
       const float f = e.mass * a.coef / sum;
-      for (long c = t; c < a.cols; c += 1024)
-        a.dz[row * a.cols + c] = (flat ? 1.f : exp2_fast((z[c] - most) * a.c)) * f;
+      float *dz = a.dz + row * a.cols;
+      for (long c0 = 4 * t; c0 < a.cols; c0 += STEP) {
+        f32x4 v[U];
+        load(v, c0);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            v[u][j] = (flat ? 1.f : exp2_fast((v[u][j] - most) * a.c)) * f;
+            if (TINY && u == 0 && c0 + j < a.cols) dz[c0 + j] = v[u][j];
+          }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (!TINY) group(c0 + u * 4096).store(dz, v[u]);
+      }
     }
     __syncthreads();
     if (t < 64) finish(a, row, e, most, flat, log2f(sum), t, a.dz != NULL);
@@ -251,7 +312,9 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
     hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a)
   // rows of up to 32768 columns leave room for two workgroups a CU, so that one
   // reads while the other reduces or writes
-  if (cols <= 1024) {
+  if (cols < 4) {
+    hipLaunchKernelGGL(distill_long_kernel<true>, grid, dim3(1024), 0, stream(), a);
+  } else if (cols <= 1024) {
     RUN(256, 1);
   } else if (cols <= 4096) {
     RUN(256, 4);
@@ -261,10 +324,14 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
     RUN(512, 8);
   } else if (cols <= 32768) {
     RUN(512, 16);
-  } else if (cols <= 65536) {
-    RUN(1024, 16);
+  } else if (cols <= 65536 && cols % 4 == 0) {
+    hipLaunchKernelGGL((distill_kernel<1024, 16, false>), grid, dim3(1024), 0, stream(), a);
   } else {
-    hipLaunchKernelGGL(distill_long_kernel, grid, dim3(1024), 0, stream(), a);
+    // the second pass reads from the last cache (256 MB) while the rows at work
+    // take no more than half of it; a workgroup a CU at least
+    long most = (128L << 20) / (4L * cols);
+    if (most < 256) most = 256;
+    hipLaunchKernelGGL(distill_long_kernel<false>, dim3((unsigned)(rows < most ? rows : most)), dim3(1024), 0, stream(), a);
   }
 #undef RUN
   return launched();

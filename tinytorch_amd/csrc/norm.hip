@@ -51,43 +51,57 @@ __device__ __forceinline__ void row_sum2(float &x, float &y, float (*part)[2]) {
   }
 }
 
-// Group n of a thread's values: the columns from this one on.  With TAIL (cols
-// not a multiple of 4) the row's last group is taken value by value.
+// Group n of a thread's values: the four columns from this one on.
 template <int NT>
 __device__ __forceinline__ int col_of(int n, int t) {
   return (n * NT + t) * 4;
 }
 
+// With TAIL (cols not a multiple of 4, and more than 4) the groups at and behind
+// the row's end are its last four columns, of which a thread's own are those that
+// no other has: every load is one instruction with no branch around it, so none
+// waits for the one before (4725 rows of 2555 columns, backward with the sums:
+// 75 us with the last columns loaded one by one, 38 so, 35 for 2556 columns).
 template <int NT, int NV, bool TAIL>
-__device__ __forceinline__ void load_row(f32x4 (&v)[NV], const float *p, int cols, int t) {
+struct Groups {
+  int at[NV], cols, t;
+  __device__ __forceinline__ Groups(int cols_, int t_) : cols(cols_), t(t_) {
 #pragma unroll
-  for (int n = 0; n < NV; n++) {
-    const int c = col_of<NT>(n, t);
-    v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (c + (TAIL ? 3 : 0) < cols) {
-      v[n] = *(const f32x4_any *)(p + c);
-    } else if (TAIL) {
-#pragma unroll
-      for (int j = 0; j < 3; j++)
-        if (c + j < cols) v[n][j] = p[c + j];
+    for (int n = 0; n < NV; n++) {
+      const int c = col_of<NT>(n, t);
+      at[n] = TAIL && c > cols - 4 ? cols - 4 : c;
     }
   }
-}
-
-template <int NT, int NV, bool TAIL>
-__device__ __forceinline__ void store_row(const f32x4 (&v)[NV], float *p, int cols, int t) {
+  __device__ __forceinline__ bool own(int n, int j) const {
+    return TAIL ? j >= col_of<NT>(n, t) - at[n] : col_of<NT>(n, t) < cols;
+  }
+  __device__ __forceinline__ void load(f32x4 (&v)[NV], const float *p) const {
 #pragma unroll
-  for (int n = 0; n < NV; n++) {
-    const int c = col_of<NT>(n, t);
-    if (c + (TAIL ? 3 : 0) < cols) {
-      *(f32x4_any *)(p + c) = v[n];
-    } else if (TAIL) {
-#pragma unroll
-      for (int j = 0; j < 3; j++)
-        if (c + j < cols) p[c + j] = v[n][j];
+    for (int n = 0; n < NV; n++) {
+      v[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (TAIL || col_of<NT>(n, t) < cols) v[n] = *(const f32x4_any *)(p + at[n]);
     }
   }
-}
+  __device__ __forceinline__ void mask(f32x4 (&v)[NV]) const {
+    if (!TAIL) return;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[n][j] = own(n, j) ? v[n][j] : 0.f;
+  }
+  __device__ __forceinline__ void store(const f32x4 (&v)[NV], float *p) const {
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      if (own(n, 0)) {
+        *(f32x4_any *)(p + at[n]) = v[n];
+      } else if (TAIL) {
+#pragma unroll
+        for (int j = 1; j < 4; j++)
+          if (own(n, j)) p[at[n] + j] = v[n][j];
+      }
+    }
+  }
+};
 
 constexpr int threads_of(int nt) { return nt < 256 ? 256 : nt; }
 
@@ -98,10 +112,12 @@ __global__ void __launch_bounds__(threads_of(NT))
                   float eps) {
   constexpr int RB = threads_of(NT) / NT;  // rows a workgroup
   __shared__ float part[NT / 64][2];
-  const int t = threadIdx.x % NT;
-  for (long row = (long)blockIdx.x * RB + threadIdx.x / NT; row < rows; row += (long)gridDim.x * RB) {
+  const int t = threadIdx.x % NT, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const Groups<NT, NV, TAIL> gr(cols, t);
+  for (long row = (long)blockIdx.x * RB + sub; row < rows; row += (long)gridDim.x * RB) {
     f32x4 v[NV];
-    load_row<NT, NV, TAIL>(v, x + row * cols, cols, t);
+    gr.load(v, x + row * cols);
+    gr.mask(v);
     float s = 0.f, z = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; n++) s += (v[n][0] + v[n][1]) + (v[n][2] + v[n][3]);
@@ -113,14 +129,14 @@ __global__ void __launch_bounds__(threads_of(NT))
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         v[n][j] -= mu;
-        if (col_of<NT>(n, t) + j < cols) q = fmaf(v[n][j], v[n][j], q);
+        if (gr.own(n, j)) q = fmaf(v[n][j], v[n][j], q);
       }
     z = 0.f;
     row_sum2<NT>(q, z, part);
     const float r = 1.f / sqrtf(q / (float)cols + eps);
     f32x4 g[NV], o[NV];
-    if (w) load_row<NT, NV, TAIL>(g, w, cols, t);
-    if (b) load_row<NT, NV, TAIL>(o, b, cols, t);
+    if (w) gr.load(g, w);
+    if (b) gr.load(o, b);
 #pragma unroll
     for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -128,7 +144,7 @@ __global__ void __launch_bounds__(threads_of(NT))
         const float h = v[n][j] * r;
         v[n][j] = fmaf(h, w ? g[n][j] : 1.f, b ? o[n][j] : 0.f);
       }
-    store_row<NT, NV, TAIL>(v, y + row * cols, cols, t);
+    gr.store(v, y + row * cols);
     if (t == 0) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
@@ -145,23 +161,27 @@ __global__ void __launch_bounds__(threads_of(NT))
   constexpr int RB = threads_of(NT) / NT;
   __shared__ float red[NT / 64][2];
   __shared__ __attribute__((aligned(16))) float join[RB > 1 ? RB * NT * 4 : 4];
-  const int t = threadIdx.x % NT;
+  const int t = threadIdx.x % NT, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const Groups<NT, NV, TAIL> gr(cols, t);
   f32x4 aw[NV], ab[NV];
 #pragma unroll
   for (int n = 0; n < NV; n++) aw[n] = ab[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (long row = (long)blockIdx.x * RB + threadIdx.x / NT; row < rows; row += (long)gridDim.x * RB) {
+  for (long row = (long)blockIdx.x * RB + sub; row < rows; row += (long)gridDim.x * RB) {
     f32x4 v[NV], d[NV];
-    load_row<NT, NV, TAIL>(v, x + row * cols, cols, t);
-    load_row<NT, NV, TAIL>(d, dy + row * cols, cols, t);
+    gr.load(v, x + row * cols);
+    gr.load(d, dy + row * cols);
     const float mu = mean[row], r = rstd[row];
     f32x4 g[NV];
-    if (w) load_row<NT, NV, TAIL>(g, w, cols, t);
+    if (w) gr.load(g, w);
+    gr.mask(v);
+    gr.mask(d);
+    if (w) gr.mask(g);  // an infinite weight times 0 would count
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; n++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        v[n][j] = (v[n][j] - mu) * r;  // behind the row's end: dy is 0, so nothing counts
+        v[n][j] = (v[n][j] - mu) * r;  // where not its own: dy is 0, so nothing counts
         aw[n][j] = fmaf(d[n][j], v[n][j], aw[n][j]);
         ab[n][j] += d[n][j];
         if (w) d[n][j] *= g[n][j];
@@ -176,7 +196,7 @@ __global__ void __launch_bounds__(threads_of(NT))
       for (int n = 0; n < NV; n++)
 #pragma unroll
         for (int j = 0; j < 4; j++) v[n][j] = r * (d[n][j] - s - v[n][j] * q);
-      store_row<NT, NV, TAIL>(v, dx + row * cols, cols, t);
+      gr.store(v, dx + row * cols);
     }
   }
   if (!part) return;
@@ -195,10 +215,8 @@ __global__ void __launch_bounds__(threads_of(NT))
         for (int k = 1; k < RB; k++) a += *(const f32x4 *)(join + (k * NT + t) * 4);
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int c = col_of<NT>(n, t) + j;
-        if (c < cols) out[(long)p * cols + c] = a[j];
-      }
+      for (int j = 0; j < 4; j++)
+        if (gr.own(n, j)) out[(long)p * cols + gr.at[n] + j] = a[j];
     }
   }
 }
@@ -231,7 +249,7 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// rows too long for registers: read again for each sum
+// rows too long for registers (or shorter than a group): read again for each sum
 __global__ void __launch_bounds__(1024)
     ln_fwd_long_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                        float *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, long rows,
@@ -297,7 +315,8 @@ __global__ void __launch_bounds__(256)
   part[((long)blockIdx.y * 2 + 1) * cols + c] = sb;
 }
 
-constexpr long LONG = 16384;  // columns that 1024 threads hold 16 each of
+// columns that 1024 threads hold 16 each of; and rows without a whole group
+bool long_rows(long cols) { return cols > 16384 || cols < 4; }
 
 // threads of a row and float4 a thread
 #define BY_COLS(RUN)              \
@@ -323,7 +342,7 @@ int rows_a_group(long cols) { return cols <= 1024 ? 4 : 1; }
 // threads, one of 1024, and two row groups at least for each; a few more of them
 // where that saves a pass (4099 rows of 1003 columns: 20.1 -> 19.0 us).
 int bwd_blocks(long rows, long cols) {
-  if (cols > LONG) return rows < 64 ? (int)rows : 64;
+  if (long_rows(cols)) return rows < 64 ? (int)rows : 64;
   const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols), most = cols <= 4096 ? 512 : 256;
   const long each = groups < 2 * most ? 2 : groups / most;
   return (int)((groups + each - 1) / each);
@@ -337,7 +356,7 @@ extern "C" int tt_k_layernorm_fwd(const float *x, const float *w, const float *b
                                   float *rstd, long rows, long cols, float eps) {
   if (!x || !y || !good(rows, cols) || !(eps >= 0.f) || isinf(eps)) return -1;
   if (ttrt_init() != 0) return -3;
-  if (cols > LONG) {
+  if (long_rows(cols)) {
     hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(1024), 0, stream(),
                        x, w, b, y, mean, rstd, rows, cols, eps);
     return launched();
@@ -373,7 +392,7 @@ extern "C" int tt_k_layernorm_bwd(const float *x, const float *w, const float *d
     if (!part) part = own = (float *)ttrt_alloc(tt_k_layernorm_bwd_ws(rows, cols));
     if (!part) return -2;
   }
-  if (cols > LONG) {
+  if (long_rows(cols)) {
     if (dx)
       hipLaunchKernelGGL(ln_dx_long_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(1024), 0, stream(),
                          x, w, dy, mean, rstd, dx, rows, cols);
