@@ -46,6 +46,15 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
+#ifndef LF
+#define LF 256
+#endif
+#ifndef LK
+#define LK 256
+#endif
+#ifndef LT
+#define LT 512
+#endif
 constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
 
@@ -142,7 +151,7 @@ __device__ __forceinline__ int snake(int p, int all) {
   return (p & 256) && round + 256 <= all ? round + ((p & 255) ^ 248) : p;
 }
 
-// What workgroup p of T tiles of `per` a (sequence, key head) takes.  Plain: tile
+// What workgroup `block` of T tiles of `per` a (sequence, key head) takes.  Plain: tile
 // by tile, the last (which see the most keys under a causal mask) first.  Where
 // the sequences' lengths are given and few enough for a wave, tile by tile of
 // those that reach so far, so that the heaviest come first and tiles behind a
@@ -152,8 +161,10 @@ __device__ __forceinline__ int snake(int p, int all) {
 struct Item {
   int b, h, tile;
 };
-__device__ __forceinline__ Item item_of(const Args &a, const int32_t *len, int rows, int G, int per, int T, bool from_end) {
-  int p = snake(blockIdx.x, gridDim.x);
+__device__ __forceinline__ Item item_of(const Args &a, int block, int blocks, const int32_t *len, int rows, int G, int per,
+                                        bool from_end) {
+  int p = snake(block, blocks);
+  const int T = blocks / (a.B * a.Hkv);
   Item it;
   if (!len || a.B > 64 || a.B == 1 || T > 256) {
     const int nbh = a.B * a.Hkv, bh = p % nbh;
@@ -661,10 +672,17 @@ __device__ __forceinline__ void dma16(const char *base, int off, unsigned lds) {
                : "s"(lds), "v"(off), "s"(base)
                : "memory");
 }
+// a pointer that is the same for all lanes, in scalar registers
+__device__ __forceinline__ const char *scalar(const char *p) {
+  const uint64_t x = (uint64_t)p;
+  return (const char *)((uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
 template <int DU, int NW>
-__device__ __forceinline__ void feed(const char *image, const char *lds, int wave, int lane) {
+__device__ __forceinline__ void feed(const char *image_, const char *lds, int wave, int lane) {
   constexpr int N = 2 * Dim<DU>::SIZE / 1024;  // what a wave's load moves
   const unsigned to = lds_address(lds);
+  const char *image = scalar(image_);
 #pragma unroll
   for (int n = 0; n < N; n += NW)
     if (N % NW == 0 || n + wave < N) dma16(image, (n + wave) * 1024 + lane * 16, to + (n + wave) * 1024);
@@ -698,9 +716,17 @@ __device__ __forceinline__ float col_sum(float x) {
 // above, two waves a SIMD in all, and one workgroup of them reads each tile once.
 constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
 // waves a SIMD that the registers have to allow
+constexpr int bwd_lives(int DU, bool pre) { return DU <= 4 && pre ? 3 : 2; }
 constexpr int fwd_lives(int DU, bool pre) { return DU <= 4 ? 3 : DU <= 6 && pre ? 4 : 2; }
 
 // ---------------------------------------------------------------- images
+
+// where the images and flags lie in a workspace
+struct Images {
+  char *kv, *rows;
+  int *kv_flags, *row_flags;
+  size_t bytes;
+};
 
 // eight values from column c of a row on; 0 behind its end and where not `in`
 __device__ __forceinline__ void load8(float (&x)[8], const float *p, int c, bool in, int D, int vec) {
@@ -858,7 +884,7 @@ __global__ void __launch_bounds__(64 * NW, fwd_lives(DU, PRE))
   constexpr int ROWS = 16 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv;
-  const Item it = item_of(a, a.q_len, a.Lq, a.G, ROWS, gridDim.x / nbh, false);
+  const Item it = item_of(a, blockIdx.x, gridDim.x, a.q_len, a.Lq, a.G, ROWS, false);
   const int b = it.b, h = it.h, tile = it.tile, bh = b * a.Hkv + h;
   const int r0 = tile * ROWS, r1 = r0 + ROWS < a.R ? r0 + ROWS : a.R;
   const Seq sq = seq_of(a, b);
@@ -1361,15 +1387,15 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
 // dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
 // forward pass
 template <int DU, int NW, bool PRE>
-__global__ void __launch_bounds__(64 * NW, DU <= 4 ? 3 : 2)
-    attn_dq_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
-                   const float *__restrict__ dout, const float *__restrict__ lse,
-                   const float *__restrict__ delta, float *__restrict__ dq, const char *__restrict__ images,
-                   const int *__restrict__ flags) {
+__device__ __forceinline__ void dq_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
+                                        const float *__restrict__ q, const float *__restrict__ k,
+                                        const float *__restrict__ v, const float *__restrict__ dout,
+                                        const float *__restrict__ lse, const float *__restrict__ delta,
+                                        float *__restrict__ dq, const char *__restrict__ images,
+                                        const int *__restrict__ flags) {
   typedef Dim<DU> M;
-  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const Item it = item_of(a, a.q_len, a.Lq, a.G, 16 * NW, gridDim.x / (a.B * a.Hkv), false);
+  const Item it = item_of(a, block, blocks, a.q_len, a.Lq, a.G, 16 * NW, false);
   const int b = it.b, h = it.h, tile = it.tile;
   const int r0 = tile * 16 * NW, r1 = r0 + 16 * NW < a.R ? r0 + 16 * NW : a.R;
   const Seq sq = seq_of(a, b);
@@ -1482,7 +1508,7 @@ __device__ __forceinline__ Rows rows_of(const Args &a, const Seq &s, int k0, int
 __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, int b, int h, int first, int r0, int r1,
                                                const float *q, const float *k, const float *v, const float *dout,
                                                const float *lse, const float *delta, float *dk, float *dv, float *ws,
-                                               int width, int lane) {
+                                               int split, int width, int lane) {
   const int keys = seq.keys;
 #pragma unroll 1
   for (int key = first; key < first + 16 && key < a.Lk; key++) {
@@ -1510,7 +1536,7 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
       }
     }
     if (a.splits > 1) {
-      const long nbh = (long)a.B * a.Hkv, at = ((long)blockIdx.y * nbh + (long)b * a.Hkv + h) * a.Lk + key;
+      const long nbh = (long)a.B * a.Hkv, at = ((long)split * nbh + (long)b * a.Hkv + h) * a.Lk + key;
       store2(ws + at * width, ak, a.scale, a.D, lane);
       store2(ws + ((long)a.splits * nbh * a.Lk + at) * width, av, 1.f, a.D, lane);
     } else {
@@ -1525,23 +1551,23 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
 // rows and leaves its sums to the join: where many rows meet few keys, and so
 // that no fp32 sum runs over more rows than that.
 template <int DU, int NW, bool PRE>
-__global__ void __launch_bounds__(64 * NW, 2)
-    attn_dkv_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
-                    const float *__restrict__ dout, const float *__restrict__ lse,
-                    const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
-                    float *__restrict__ ws, const char *__restrict__ images, const int *__restrict__ flags) {
+__device__ __forceinline__ void dkv_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
+                                         int split, const float *__restrict__ q, const float *__restrict__ k,
+                                         const float *__restrict__ v, const float *__restrict__ dout,
+                                         const float *__restrict__ lse, const float *__restrict__ delta,
+                                         float *__restrict__ dk, float *__restrict__ dv, float *__restrict__ ws,
+                                         const char *__restrict__ images, const int *__restrict__ flags) {
   typedef Dim<DU> M;
   constexpr int KEYS = 16 * NW;
-  __shared__ __attribute__((aligned(16))) char lds[2][2 * M::SIZE + STATS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int nbh = a.B * a.Hkv;
-  const Item it = item_of(a, a.k_len, a.Lk, 1, KEYS, gridDim.x / nbh, true);
+  const Item it = item_of(a, block, blocks, a.k_len, a.Lk, 1, KEYS, true);
   const int b = it.b, h = it.h, bh = b * a.Hkv + h, k0 = it.tile * KEYS, kw = k0 + wave * 16, key = kw + (lane & 15);
   const Seq seq = seq_of(a, b);
   Rows rows = rows_of(a, seq, k0, k0 + KEYS);
   if (a.splits > 1) {
-    const long c0 = rows.first + (long)blockIdx.y * a.chunk;
-    if (c0 >= rows.end && blockIdx.y > 0) return;  // the join leaves it out
+    const long c0 = rows.first + (long)split * a.chunk;
+    if (c0 >= rows.end && split > 0) return;  // the join leaves it out
     if (c0 + a.chunk < rows.end) rows.end = (int)c0 + a.chunk;
     rows.first = (int)c0;
   }
@@ -1567,7 +1593,7 @@ __global__ void __launch_bounds__(64 * NW, 2)
       const char *from = images + (tile0 + r0 / KT) * (2 * M::SIZE + STATS);
       if (r0 < rows.end) {
         feed<DU, NW>(from, lds[buf], wave, lane);
-        if (wave == 0 && lane < STATS / 16) dma16(from, 2 * M::SIZE + lane * 16, lds_address(lds[buf]) + 2 * M::SIZE);
+        if (wave == 0 && lane < STATS / 16) dma16(scalar(from), 2 * M::SIZE + lane * 16, lds_address(lds[buf]) + 2 * M::SIZE);
       }
     } else {
       const float *q0 = qp + (long)i_next * a.q.r, *d0 = op + (long)i_next * a.o.r;
@@ -1678,18 +1704,39 @@ __global__ void __launch_bounds__(64 * NW, 2)
     }
   }
   if (odd) {
-    dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, 16 * DU, lane);
+    dkv_one_by_one(a, seq, b, h, kw, rows.first, rows.end, q, k, v, dout, lse, delta, dk, dv, ws, split,
+                   16 * DU, lane);
     return;
   }
   if (!in) return;
   if (a.splits > 1) {
-    const long at = ((long)blockIdx.y * nbh + bh) * a.Lk + key, half = (long)a.splits * nbh * a.Lk;
+    const long at = ((long)split * nbh + bh) * a.Lk + key, half = (long)a.splits * nbh * a.Lk;
     store_columns<DU>(ws + at * 16 * DU, ak, a.scale, 16 * DU, 1, lane);
     store_columns<DU>(ws + (half + at) * 16 * DU, av, 1.f, 16 * DU, 1, lane);
     return;
   }
   store_columns<DU>(dk + (long)b * a.k.b + (long)h * a.k.h + (long)key * a.k.r, ak, a.scale, a.D, a.vec, lane);
   store_columns<DU>(dv + (long)b * a.v.b + (long)h * a.v.h + (long)key * a.v.r, av, 1.f, a.D, a.vec, lane);
+}
+
+// Both gradients in one launch, the keys' tiles first (they take the longest): where
+// either leaves CUs idle, or at its end, the other fills them.  dkv_blocks: the
+// tiles of dk and dv times their splits.
+template <int DU, int NW, bool PRE>
+__global__ void __launch_bounds__(64 * NW, bwd_lives(DU, PRE))
+    attn_bwd_kernel(Args a, int dkv_blocks, const float *__restrict__ q, const float *__restrict__ k,
+                    const float *__restrict__ v, const float *__restrict__ dout, const float *__restrict__ lse,
+                    const float *__restrict__ delta, float *__restrict__ dq, float *__restrict__ dk,
+                    float *__restrict__ dv, float *__restrict__ ws, Images m) {
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * Dim<DU>::SIZE + STATS];
+  const int p = blockIdx.x;
+  if (p < dkv_blocks) {
+    const int n = __builtin_amdgcn_readfirstlane(dkv_blocks / a.splits), split = __builtin_amdgcn_readfirstlane(p / n);
+    dkv_tile<DU, NW, PRE>(a, lds, p - split * n, n, split, q, k, v, dout, lse, delta, dk, dv, ws, m.rows, m.row_flags);
+  } else {
+    dq_tile<DU, NW, PRE>(a, lds, p - dkv_blocks, gridDim.x - dkv_blocks, q, k, v, dout, lse, delta, dq, m.kv,
+                         m.kv_flags);
+  }
 }
 
 // the workgroups' sums of a key, added in their order; 32 lanes a key
@@ -1824,7 +1871,7 @@ Plan plan_of(const TTAttention *t) {
   } else {
     p.rows = 16 * waves(blocks(t->head_dim));
     p.tiles = (int)((R + p.rows - 1) / p.rows);
-    split(p, t->k_rows, 512 / (p.tiles * nbh), 256, KT);
+    split(p, t->k_rows, 512 / (p.tiles * nbh), LF, KT);
   }
   return p;
 }
@@ -1837,8 +1884,8 @@ Plan dkv_plan(const TTAttention *t) {
   p.rows = 16 * waves(blocks(t->head_dim));
   p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
   // fp32 sums over at most 2048 rows
-  const long fill = 512 / (p.tiles * nbh), sums = (R + 2047) / 2048;
-  split(p, R, fill > sums ? fill : sums, 256, KT);
+  const long fill = LT / (p.tiles * nbh), sums = (R + 2047) / 2048;
+  split(p, R, fill > sums ? fill : sums, LK, KT);
   return p;
 }
 
@@ -1874,12 +1921,6 @@ void run_few(const Plan &p, const Args &a, const float *q, const float *k, const
                      dim3(256), 0, stream(), a, q, k, v, o, lse, ml, wo);
 }
 
-// where the images and flags lie in a workspace
-struct Images {
-  char *kv, *rows;
-  int *kv_flags, *row_flags;
-  size_t bytes;
-};
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 Images images_of(const TTAttention *t, bool kv, bool rows, void *base) {
   const long nbh = t->batch * t->kv_heads, kt = (t->k_rows + KT - 1) / KT,
@@ -1925,29 +1966,18 @@ void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const
 }
 
 template <int DU>
-void run_dq(const Args &a, const float *q, const float *k, const float *v, const float *dout, const float *lse,
-            const float *delta, float *dq, const Images *m) {
+void run_bwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
+             const float *lse, const float *delta, float *dq, float *dk, float *dv, float *ws, bool pre,
+             const Images &m) {
   constexpr int NW = waves(DU);
-  const dim3 grid((unsigned)(((long)a.R + 16 * NW - 1) / (16 * NW) * a.B * a.Hkv));
-  if (m)
-    hipLaunchKernelGGL((attn_dq_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta,
-                       dq, m->kv, m->kv_flags);
+  const long nbh = (long)a.B * a.Hkv, nk = dk ? p.tiles * nbh * p.splits : 0,
+             nq = dq ? ((long)a.R + 16 * NW - 1) / (16 * NW) * nbh : 0;
+  if (pre)
+    hipLaunchKernelGGL((attn_bwd_kernel<DU, NW, true>), dim3((unsigned)(nk + nq)), dim3(64 * NW), 0, stream(), a,
+                       (int)nk, q, k, v, dout, lse, delta, dq, dk, dv, ws, m);
   else
-    hipLaunchKernelGGL((attn_dq_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
-                       delta, dq, NULL, NULL);
-}
-
-template <int DU>
-void run_dkv(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
-             const float *lse, const float *delta, float *dk, float *dv, float *ws, const Images *m) {
-  constexpr int NW = waves(DU);
-  const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
-  if (m)
-    hipLaunchKernelGGL((attn_dkv_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse, delta,
-                       dk, dv, ws, m->rows, m->row_flags);
-  else
-    hipLaunchKernelGGL((attn_dkv_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, dout, lse,
-                       delta, dk, dv, ws, NULL, NULL);
+    hipLaunchKernelGGL((attn_bwd_kernel<DU, NW, false>), dim3((unsigned)(nk + nq)), dim3(64 * NW), 0, stream(), a,
+                       (int)nk, q, k, v, dout, lse, delta, dq, dk, dv, ws, m);
 }
 
 #define BY_STEPS(N, F, ...)            \
@@ -2048,16 +2078,13 @@ extern "C" int tt_k_attention_bwd(const TTAttention *t, const float *q, const fl
     hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16 < 8192 ? (rows + 15) / 16 : 8192)),
                        dim3(256), 0, stream(), a, o, dout, delta);
   }
-  if (dq) {
-    if (pre) {
-      BY_STEPS(blocks(a.D), run_kv_images, a, k, v, m);
-    }
-    BY_STEPS(blocks(a.D), run_dq, a, q, k, v, dout, lse, delta, dq, pre ? &m : NULL);
+  if (dq && pre) {
+    BY_STEPS(blocks(a.D), run_kv_images, a, k, v, m);
   }
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  BY_STEPS(blocks(a.D), run_bwd, p, a, q, k, v, dout, lse, delta, dq, dk, dv, parts, pre, m);
   if (dk) {
-    a.splits = p.splits;
-    a.chunk = p.chunk;
-    BY_STEPS(blocks(a.D), run_dkv, p, a, q, k, v, dout, lse, delta, dk, dv, parts, pre ? &m : NULL);
     if (p.splits > 1) {
       const long keys = (long)a.B * a.Hkv * a.Lk;
       hipLaunchKernelGGL(attn_dkv_join_kernel, dim3((unsigned)((keys + 7) / 8 < 8192 ? (keys + 7) / 8 : 8192)),
