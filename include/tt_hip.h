@@ -508,7 +508,11 @@ int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *position
  * p - j < window (without causal |p - j| < window).  A query that sees no key,
  * and one past q_len, has o = 0 and lse = -inf and takes no part in the
  * gradients; what lies behind k_len and q_len is not read.  Lengths outside
- * [0, rows] are clamped. */
+ * [0, rows] are clamped.  An infinity that a query sees in q, k, v or dout
+ * comes out as NaN; one that the masks hide from it does not reach it.
+ * Workspaces are 16-byte aligned; with many rows they hold q, k, v and dout
+ * once more at 1.5 times their size (at most 4 GiB each for k with v and for q
+ * with dout). */
 #define TT_ATTENTION_MAX_DIM 128
 typedef struct TTStrides {
     long batch, row, head;  /* floats from one to the next; 0: packed in that order.  Rows and
@@ -541,7 +545,7 @@ int tt_k_attention_bwd(const TTAttention *a, const float *q, const float *k, con
  *   dlogits = scale * T * (q - the p_e at their columns)      (unless NULL)
  * Entries whose id is outside [0, cols) are left out, entries of one column
  * add up.  A row without entries, or with -inf for all of them, has loss and
- * gradient 0.  A row of logits of -inf counts as a row of equal ones. */
+ * gradient 0; dlogits may not be logits.  A row of logits of -inf counts as a row of equal ones. */
 #define TT_DISTILL_MAX_TOP 1024
 int tt_k_distill(const float *logits, const int32_t *ids, const float *teacher, int top,
                  float temperature, float *rowloss, float *dlogits, long rows, int cols,

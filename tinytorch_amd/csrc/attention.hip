@@ -46,15 +46,6 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
-#ifndef LF
-#define LF 256
-#endif
-#ifndef LK
-#define LK 256
-#endif
-#ifndef LT
-#define LT 512
-#endif
 constexpr int MAX_SPLITS = 1024;  // parts that a join takes
 constexpr int KT = 32;  // rows of the streamed operand a tile
 
@@ -396,9 +387,9 @@ __device__ __forceinline__ Parts parts_of(float (&x)[8]) {
 // The 16x16x32 product: A holds row m = lane % 16 and B column m, both at the
 // eight summed indices of their group g = lane / 16; C holds column m, rows 4 g +
 // r in register r.  A wave has 16 query rows (or keys), so that two to four of
-// them fit a SIMD's registers and cover each other's waits; 32 a wave would
-// halve the reads of LDS, which is busy 17 % of the time, and leave one wave a
-// SIMD at 128 columns.  DB: blocks of 16 columns of a head, DK: steps of 32.
+// them fit a SIMD's registers and cover each other's waits (32 a wave, with half
+// the reads of LDS: 671 against 658 us for the forward pass of 4096 rows and 128
+// columns, 76 against 59 for 1024 rows and 64 columns).  DB: blocks of 16 columns of a head, DK: steps of 32.
 //
 // A tile of KT rows lies in LDS as its parts, a row RC chunks of eight values,
 // chunk c of row r at place c ^ f(r): the lanes that LDS serves at once (of a read
@@ -659,8 +650,10 @@ struct Stream {
 //
 // Where a tile is used by many workgroups, a kernel before them writes its parts
 // to memory once, as the image of a pair of tiles in LDS, and direct loads bring
-// it there: no registers hold it on the way, and the main loops' vector work
-// falls by half.  Rows outside an operand are zeros in the image.
+// it there: no registers hold it on the way and no vector work cuts it up (2 x
+// 4096 causal rows, 16 heads on 4, 128 columns: forward 768 -> 640 us, dq 1021 ->
+// 953, dk and dv, which spilled, 2247 -> 1410).  Rows outside an operand are zeros
+// in the image.
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
@@ -712,8 +705,10 @@ __device__ __forceinline__ float col_sum(float x) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
-// Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU;
-// above, two waves a SIMD in all, and one workgroup of them reads each tile once.
+// Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU (two of
+// eight: 8 x 600 to 1024 rows, 8 heads of 64 columns, forward 65 against 60 us, dq
+// 87 - 83, dk and dv 108 - 94); above, one of eight or, forward up to 96 columns
+// (1000 rows of 3500 keys, 16 heads on 4, 80 columns: 120 -> 103 us), two.
 constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
 // waves a SIMD that the registers have to allow
 constexpr int bwd_lives(int DU, bool pre) { return DU <= 4 && pre ? 3 : 2; }
@@ -871,6 +866,9 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
 
 // One workgroup of NW waves: 16 packed rows a wave of one key head against
 // the keys they see, KT at a time through LDS, from memory or (PRE) from images.
+// Bound by the matrix units and by what lies between their products (2 x 4096
+// causal rows, 16 heads on 4, 128 columns: 640 us, 215 TFLOP/s of fp32, matrix
+// units 62 % busy at 1.8 GHz, LDS without conflicts).
 // With splits > 1 it takes `chunk` keys of them and leaves maximum, sum and the
 // unscaled result to the join.
 template <int DU, int NW, bool PRE>
@@ -1385,7 +1383,7 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
 }
 
 // dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
-// forward pass
+// forward pass (the same case: 216 TFLOP/s, matrix units 68 % busy)
 template <int DU, int NW, bool PRE>
 __device__ __forceinline__ void dq_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
                                         const float *__restrict__ q, const float *__restrict__ k,
@@ -1549,7 +1547,8 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
 // dk and dv of 16 NW keys (16 a wave): the packed query rows that see any of
 // them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of the
 // rows and leaves its sums to the join: where many rows meet few keys, and so
-// that no fp32 sum runs over more rows than that.
+// that no fp32 sum runs over more rows than that.  The same case: 195 TFLOP/s,
+// matrix units 64 % busy.
 template <int DU, int NW, bool PRE>
 __device__ __forceinline__ void dkv_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
                                          int split, const float *__restrict__ q, const float *__restrict__ k,
@@ -1720,7 +1719,8 @@ __device__ __forceinline__ void dkv_tile(const Args &a, char (*lds)[2 * Dim<DU>:
 }
 
 // Both gradients in one launch, the keys' tiles first (they take the longest): where
-// either leaves CUs idle, or at its end, the other fills them.  dkv_blocks: the
+// either leaves CUs idle, or at its end, the other fills them (10 x 203 rows, 8
+// heads of 64 columns, with the forward pass: 66 -> 49 us).  dkv_blocks: the
 // tiles of dk and dv times their splits.
 template <int DU, int NW, bool PRE>
 __global__ void __launch_bounds__(64 * NW, bwd_lives(DU, PRE))
@@ -1830,17 +1830,19 @@ void split(Plan &p, long n, long want, long least, long step) {
 size_t pair_bytes(int head_dim) {
   return (size_t)2 * 3 * KT * 16 * 4 * ((blocks(head_dim) + 1) / 2);
 }
-// Tiles are split beforehand from 1024 packed rows on, where eight workgroups or
-// more use each.  us with and without, causal, 8 heads, 8192 rows in all, batches
-// of 512 / 1024 / 2048 rows:
-//   forward   64 columns  47 - 42,   68 - 71,   110 - 118
-//            128 columns  95 - 87,   132 - 136, 221 - 250
-//   backward  64 columns  128 - 129, 194 - 216, 321 - 374
-//            128 columns  277 - 337, 407 - 546, 697 - 950
-// The backward pass writes the rows' images too and has to have keys to use them
-// for (4 heads a key head, 1024 packed rows and 256 keys: 194 - 218).  At most
-// 4 GiB each: past that the tiles are split where they are used.
+// Tiles are split beforehand where enough workgroups use each: forward from 1024
+// packed rows on, backward (whose products spill registers otherwise, and whose
+// rows' images hold delta too) from 384, with 65 to 96 columns from 1024.  us with
+// and without, causal, 8 heads, batches of 384 / 512 / 1024 rows, 8192 in all:
+//   forward   64 columns   43 - 36,   49 - 43,    70 - 73
+//            128 columns   88 - 77,   96 - 87,   135 - 137
+//   backward  64 columns  107 - 113, 125 - 132,  190 - 219
+//             80 columns  180 - 160, 205 - 190,  294 - 297
+//            128 columns  239 - 278, 270 - 326,  398 - 547
+// and, backward, there have to be 256 keys to use the rows' for.  At most 4 GiB
+// each: past that the tiles are split where they are used.
 constexpr long IMAGE_ROWS = 1024, IMAGE_KEYS = 256;
+long image_rows_bwd(int head_dim) { return head_dim > 64 && head_dim <= 96 ? 1024 : 384; }
 bool fits_images(const TTAttention *t, long rows) {
   return (double)t->batch * t->kv_heads * ((rows + KT - 1) / KT) * (pair_bytes(t->head_dim) + STATS) < 4294967296.;
 }
@@ -1848,7 +1850,7 @@ bool images_for_rows(const TTAttention *t) {
   return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS && fits_images(t, t->k_rows);
 }
 bool images_for_keys(const TTAttention *t) {
-  return images_for_rows(t) && t->k_rows >= IMAGE_KEYS && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
+  return t->q_rows * (t->q_heads / t->kv_heads) >= image_rows_bwd(t->head_dim) && t->k_rows >= IMAGE_KEYS && fits_images(t, t->k_rows) && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
 }
 
 Plan plan_of(const TTAttention *t) {
@@ -1871,7 +1873,10 @@ Plan plan_of(const TTAttention *t) {
   } else {
     p.rows = 16 * waves(blocks(t->head_dim));
     p.tiles = (int)((R + p.rows - 1) / p.rows);
-    split(p, t->k_rows, 512 / (p.tiles * nbh), LF, KT);
+    // two workgroups a CU, of 128 keys or more (256: 2 x 141 rows of 698 keys, 2
+    // heads, 24.5 against 15.9 us; 64: 3 x 78 rows of 974 keys, 13 heads of 128
+    // columns, 50 against 37)
+    split(p, t->k_rows, 512 / (p.tiles * nbh), 128, KT);
   }
   return p;
 }
@@ -1883,9 +1888,11 @@ Plan dkv_plan(const TTAttention *t) {
   p.few = false;
   p.rows = 16 * waves(blocks(t->head_dim));
   p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
-  // fp32 sums over at most 2048 rows
-  const long fill = LT / (p.tiles * nbh), sums = (R + 2047) / 2048;
-  split(p, R, fill > sums ? fill : sums, LK, KT);
+  // As many workgroups as the CUs hold (512 for three of them: 7 x 152 rows, 40
+  // heads on 5, 65 against 54 us; 768 for two: 8 x 524 rows, 8 on 2 of 128
+  // columns, 183 against 177); fp32 sums over at most 2048 rows
+  const long fill = (p.width <= 64 ? 768 : 512) / (p.tiles * nbh), sums = (R + 2047) / 2048;
+  split(p, R, fill > sums ? fill : sums, 128, KT);
   return p;
 }
 
