@@ -1890,8 +1890,8 @@ Plan dkv_plan(const TTAttention *t) {
   p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
   // As many workgroups as the CUs hold (512 for three of them: 7 x 152 rows, 40
   // heads on 5, 65 against 54 us; 768 for two: 8 x 524 rows, 8 on 2 of 128
-  // columns, 183 against 177); fp32 sums over at most 2048 rows
-  const long fill = (p.width <= 64 ? 768 : 512) / (p.tiles * nbh), sums = (R + 2047) / 2048;
+  // columns, 183 against 177); fp32 sums over at most 4096 rows
+  const long fill = (p.width <= 64 ? 768 : 512) / (p.tiles * nbh), sums = (R + 4095) / 4096;
   split(p, R, fill > sums ? fill : sums, 128, KT);
   return p;
 }
