@@ -12,7 +12,6 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
-#include <string.h>
 #include "tt_rt.h"
 
 namespace {
@@ -138,20 +137,6 @@ bool good(const TTRope *r) {
   }
 }
 
-// the frequencies of the call before, which most calls ask for again: the
-// powers take the host longer than a launch
-TTRope g_last;
-Turns g_turns;
-
-const Turns &turns_of(const TTRope *r) {
-  if (memcmp(r, &g_last, sizeof(TTRope)) != 0) {
-    tt_rope_frequencies(r, g_turns.f);
-    for (int j = 0; j < r->rot_dim / 2; j++) g_turns.f[j] /= 2 * M_PI;
-    g_last = *r;
-  }
-  return g_turns;
-}
-
 }  // namespace
 
 extern "C" int tt_rope_frequencies(const TTRope *r, double *f) {
@@ -159,13 +144,19 @@ extern "C" int tt_rope_frequencies(const TTRope *r, double *f) {
   const int R = r->rot_dim;
   double base = r->base;
   if (r->scaling == TT_ROPE_NTK && R > 2) base *= pow(r->factor, (double)R / (R - 2));
+  // one power in 64, and products between them (off by at most 126 roundings of
+  // 2^-53), so that a token's 64 frequencies do not take the host as long as the launch
+  const double ratio = pow(base, -2.0 / R), per = 1 / r->factor, turns = r->trained / (2 * M_PI),
+               range = 1 / (r->high - r->low);
+  double g = 1;
   for (int j = 0; j < R / 2; j++) {
-    f[j] = pow(base, -2.0 * j / R);
-    if (r->scaling == TT_ROPE_LINEAR) f[j] /= r->factor;
+    g = j % 64 ? g * ratio : pow(base, -2.0 * j / R);
+    f[j] = g;
+    if (r->scaling == TT_ROPE_LINEAR) f[j] *= per;
     if (r->scaling == TT_ROPE_PARTS) {
-      double keep = (r->trained * f[j] / (2 * M_PI) - r->low) / (r->high - r->low);
+      double keep = (turns * f[j] - r->low) * range;
       keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
-      f[j] = (1 - keep) * f[j] / r->factor + keep * f[j];
+      f[j] = (1 - keep) * f[j] * per + keep * f[j];
     }
   }
   return 0;
@@ -189,7 +180,9 @@ extern "C" int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_
   if ((rows + n - 1) / n > (1L << 24) - 1) n = (rows + (1L << 24) - 2) / ((1L << 24) - 1);
   if (n > 4096 / pairs || n * width > 0x7fffffffL) return -1;
   if (ttrt_init() != 0) return -3;
-  const Turns &t = turns_of(r);
+  Turns t;
+  tt_rope_frequencies(r, t.f);
+  for (int j = 0; j < r->rot_dim / 2; j++) t.f[j] *= 1 / (2 * M_PI);
   const float sign = transpose ? -1.f : 1.f, mag = r->magnitude != 0 ? (float)r->magnitude : 1.f;
   const dim3 grid((unsigned)((rows + n - 1) / n));
   const size_t lds = sizeof(float2) * n * pairs;
