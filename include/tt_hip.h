@@ -512,7 +512,7 @@ int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *position
  * comes out as NaN; one that the masks hide from it does not reach it.
  * Workspaces are 16-byte aligned; with many rows they hold q, k, v and dout
  * once more at 1.5 times their size (at most 4 GiB each for k with v and for q
- * with dout). */
+ * with dout), and parts of dk and dv (at most 4 GiB). */
 #define TT_ATTENTION_MAX_DIM 128
 typedef struct TTStrides {
     long batch, row, head;  /* floats from one to the next; 0: packed in that order.  Rows and

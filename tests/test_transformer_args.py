@@ -83,6 +83,19 @@ def test_attention_refuses(L, kw):
     assert L.tt_k_attention_fwd_ws(a) == 0 and L.tt_k_attention_bwd_ws(a) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(batch=1, q_rows=1 << 17, k_rows=1 << 17, q_heads=64, kv_heads=8),
+                                dict(batch=1, q_rows=1 << 22, k_rows=1 << 20, q_heads=1, kv_heads=1),
+                                dict(batch=64, q_rows=4096, k_rows=1 << 17, q_heads=64, kv_heads=8),
+                                dict(batch=1, q_rows=1 << 28, k_rows=1 << 28, q_heads=1, kv_heads=1)])
+def test_attention_workspaces_stay_small(L, kw):
+    """Next to operands of gigabytes: 4 GiB at most for each of two kinds of
+    images and for the parts of the gradients, and two floats a row."""
+    a = attention(head_dim=128, **kw)
+    rows = kw["batch"] * kw["q_heads"] * kw["q_rows"]
+    assert L.tt_k_attention_fwd_ws(a) <= 4.01 * 2**30
+    assert 4 * rows <= L.tt_k_attention_bwd_ws(a) <= 12.01 * 2**30 + 4 * rows
+
+
 def test_attention_refuses_missing_operands(L):
     a = attention()
     for i in range(4):

@@ -1808,9 +1808,9 @@ int check(const TTAttention *t) {
     if (s->row > (1L << 28) / KT || s->head > (1L << 28) / G || s->batch > 1L << 50) return -1;
   }
   if ((long)t->q_heads * t->head_dim > (1L << 28) / KT) return -1;
-  const long lim = 1L << 30, grid = (1L << 24) - 1;
+  const long lim = 1L << 30, grid = (1L << 23) - 1;
   if (t->q_rows > lim / G || t->k_rows > lim || t->batch > grid / t->kv_heads) return -1;
-  const long nbh = t->batch * t->kv_heads;  // a grid axis has less than 2^32 threads
+  const long nbh = t->batch * t->kv_heads;  // the two parts of a grid axis have less than 2^32 threads
   if ((t->q_rows * G + 63) / 64 > grid / nbh || (t->k_rows + 63) / 64 > grid / nbh) return -1;
   return 0;
 }
@@ -1892,7 +1892,12 @@ Plan dkv_plan(const TTAttention *t) {
   // heads on 5, 65 against 54 us; 768 for two: 8 x 524 rows, 8 on 2 of 128
   // columns, 183 against 177); fp32 sums over at most 4096 rows
   const long fill = (p.width <= 64 ? 768 : 512) / (p.tiles * nbh), sums = (R + 4095) / 4096;
-  split(p, R, fill > sums ? fill : sums, 128, KT);
+  // within 4 GiB of parts (4096 rows a part up to 65536 x 65536 rows and keys of 4
+  // heads of 128 columns; sums of more rows past that) and the grid's axis
+  const long part = 8L * nbh * t->k_rows * p.width, room = (1L << 32) / part, axis = (1L << 22) / (p.tiles * nbh);
+  long want = fill > sums ? fill : sums;
+  if (want > room) want = room;
+  split(p, R, want < axis ? want : axis, 128, KT);
   return p;
 }
 
