@@ -68,6 +68,23 @@ def test_head_sizes(tlib, D):
     _check(tlib, *_inputs(2, 37, 70, 4, 2, D), dict(causal=True))
 
 
+@pytest.mark.parametrize("D", [16, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("Lq", [16, 17, 24, 32, 33, 48, 64, 65])
+def test_rows_about_a_tile(tlib, D, Lq):
+    """Where one kernel takes over from another, in a workspace of the size asked for."""
+    q, k, v, do = _inputs(1, Lq, 700, 2, 2, D)
+    masks = dict(causal=True)
+    _check(tlib, q, k, v, do, masks)
+    held = []
+    a = _plan(q, k, masks, held)
+    need = tlib.tt_k_attention_fwd_ws(a) // 4
+    ws, o, d = DevBuf(need + 64), DevBuf(q.size), [DevBuf.from_np(t) for t in (q, k, v)]
+    ws.fill(7.0)
+    check(tlib.tt_k_attention_fwd(a, *[x.ptr for x in d], o.ptr, None, ws.ptr), "fwd")
+    ref.close(o.to_np(q.shape), ref.attention(q, k, v, ref.seen(1, Lq, 700, **masks))["o"])
+    assert (ws.to_np()[need:] == 7.0).all()
+
+
 @pytest.mark.parametrize("D", [8, 31, 40, 64, 80, 95, 100, 128])
 @pytest.mark.parametrize("masks", [
     dict(causal=True), dict(), dict(window=50),

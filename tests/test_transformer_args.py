@@ -96,6 +96,17 @@ def test_attention_workspaces_stay_small(L, kw):
     assert 4 * rows <= L.tt_k_attention_bwd_ws(a) <= 12.01 * 2**30 + 4 * rows
 
 
+def test_attention_workspace_sizes_stand(L):
+    """The size asked for is that of the call, whatever was asked before."""
+    kinds = [attention(batch=2, q_rows=r, k_rows=900, q_heads=2, kv_heads=2, head_dim=d)
+             for d in (16, 64, 80, 96, 112, 128) for r in (1, 16, 17, 32, 33, 100, 1100)]
+    sizes = [(L.tt_k_attention_fwd_ws(a), L.tt_k_attention_bwd_ws(a)) for a in kinds]
+    assert min(min(s) for s in sizes) > 0
+    for i in np.random.default_rng(0).permutation(len(kinds) * 4) % len(kinds):
+        a = kinds[i]
+        assert (L.tt_k_attention_fwd_ws(a), L.tt_k_attention_bwd_ws(a)) == sizes[i]
+
+
 def test_attention_refuses_missing_operands(L):
     a = attention()
     for i in range(4):

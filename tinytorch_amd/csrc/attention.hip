@@ -707,9 +707,15 @@ __device__ __forceinline__ float col_sum(float x) {
 
 // Waves of a workgroup.  Up to 64 columns three workgroups of four fit a CU (two of
 // eight: 8 x 600 to 1024 rows, 8 heads of 64 columns, forward 65 against 60 us, dq
-// 87 - 83, dk and dv 108 - 94); above, one of eight or, forward up to 96 columns
-// (1000 rows of 3500 keys, 16 heads on 4, 80 columns: 120 -> 103 us), two.
+// 87 - 83, dk and dv 108 - 94).  Past 96 columns LDS holds one, of eight.  Between,
+// two: of four where they split the tiles themselves forward (8 x 900 rows, 8 heads
+// of 80 columns: 104 -> 81 us, 8 x 48 rows of 2048 keys 48 -> 33) and in the backward
+// pass over images (8 x 1024 rows, 8 heads on 2: 271 -> 243), of eight in the forward
+// pass over images, whose registers are fewer; the backward pass that splits tiles
+// itself loses by four (8 x 900 rows: 263 -> 277).
 constexpr int waves(int DU) { return DU <= 4 ? 4 : 8; }
+constexpr int fwd_waves(int DU, bool pre) { return !pre && DU <= 6 ? 4 : waves(DU); }
+constexpr int bwd_waves(int DU, bool pre) { return pre && DU <= 6 ? 4 : waves(DU); }
 // waves a SIMD that the registers have to allow
 constexpr int bwd_lives(int DU, bool pre) { return DU <= 4 && pre ? 3 : 2; }
 constexpr int fwd_lives(int DU, bool pre) { return DU <= 4 ? 3 : DU <= 6 && pre ? 4 : 2; }
@@ -1832,17 +1838,16 @@ size_t pair_bytes(int head_dim) {
 }
 // Tiles are split beforehand where enough workgroups use each: forward from 1024
 // packed rows on, backward (whose products spill registers otherwise, and whose
-// rows' images hold delta too) from 384, with 65 to 96 columns from 1024.  us with
-// and without, causal, 8 heads, batches of 384 / 512 / 1024 rows, 8192 in all:
+// rows' images hold delta too) from 384.  us with and without, causal, 8 heads,
+// batches of 384 / 512 / 1024 rows, 8192 in all:
 //   forward   64 columns   43 - 36,   49 - 43,    70 - 73
 //            128 columns   88 - 77,   96 - 87,   135 - 137
 //   backward  64 columns  107 - 113, 125 - 132,  190 - 219
-//             80 columns  180 - 160, 205 - 190,  294 - 297
+//             80 columns  161 - 160, 184 - 189,  260 - 297
 //            128 columns  239 - 278, 270 - 326,  398 - 547
 // and, backward, there have to be 256 keys to use the rows' for.  At most 4 GiB
 // each: past that the tiles are split where they are used.
-constexpr long IMAGE_ROWS = 1024, IMAGE_KEYS = 256;
-long image_rows_bwd(int head_dim) { return head_dim > 64 && head_dim <= 96 ? 1024 : 384; }
+constexpr long IMAGE_ROWS = 1024, IMAGE_ROWS_BWD = 384, IMAGE_KEYS = 256;
 bool fits_images(const TTAttention *t, long rows) {
   return (double)t->batch * t->kv_heads * ((rows + KT - 1) / KT) * (pair_bytes(t->head_dim) + STATS) < 4294967296.;
 }
@@ -1850,18 +1855,19 @@ bool images_for_rows(const TTAttention *t) {
   return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS && fits_images(t, t->k_rows);
 }
 bool images_for_keys(const TTAttention *t) {
-  return t->q_rows * (t->q_heads / t->kv_heads) >= image_rows_bwd(t->head_dim) && t->k_rows >= IMAGE_KEYS && fits_images(t, t->k_rows) && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
+  return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS_BWD && t->k_rows >= IMAGE_KEYS && fits_images(t, t->k_rows) && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
 }
 
 Plan plan_of(const TTAttention *t) {
-  Plan p;
+  Plan p = {};
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
+  p.width = 16 * blocks(t->head_dim);
   // Two tiles of few rows, each reading the keys, the second from a cache: 20 rows
   // of 32 x 8 heads of 4096 keys 64 / 80 / 128 columns 161 / 194 / 280 us against
   // 151 / 297 / 311 through LDS, of 8 heads of 32768 keys 38 / 46 / 68 against 41 /
-  // 77 / 89; three lose (48 rows: 204 / 317 / 471 against 156 / 304 / 320)
-  p.few = R <= 32;
-  p.width = 16 * blocks(t->head_dim);
+  // 77 / 89; three lose (48 rows: 204 / 317 / 471 against 156 / 304 / 320), and two
+  // of 96 columns, which come 8 bytes at a time (235 against 195, 56 against 52)
+  p.few = R <= (p.width == 96 ? 16 : 32);
   if (p.few) {
     p.tiles = (int)((R + 15) / 16);
     // parts of 64 to 1024 keys, about two workgroups a CU (eight: 8 heads of 32768
@@ -1871,7 +1877,7 @@ Plan plan_of(const TTAttention *t) {
     c = c < 64 ? 64 : c > 1024 ? 1024 : c;
     split(p, t->k_rows, (t->k_rows + c - 1) / c, 1, 64);
   } else {
-    p.rows = 16 * waves(blocks(t->head_dim));
+    p.rows = 16 * fwd_waves(blocks(t->head_dim), images_for_rows(t));
     p.tiles = (int)((R + p.rows - 1) / p.rows);
     // two workgroups a CU, of 128 keys or more (256: 2 x 141 rows of 698 keys, 2
     // heads, 24.5 against 15.9 us; 64: 3 x 78 rows of 974 keys, 13 heads of 128
@@ -1882,11 +1888,11 @@ Plan plan_of(const TTAttention *t) {
 }
 
 Plan dkv_plan(const TTAttention *t) {
-  Plan p;
+  Plan p = {};
   const long G = t->q_heads / t->kv_heads, R = t->q_rows * G, nbh = t->batch * t->kv_heads;
   p.width = 16 * blocks(t->head_dim);
   p.few = false;
-  p.rows = 16 * waves(blocks(t->head_dim));
+  p.rows = 16 * bwd_waves(blocks(t->head_dim), images_for_keys(t));
   p.tiles = (int)((t->k_rows + p.rows - 1) / p.rows);
   // As many workgroups as the CUs hold (512 for three of them: 7 x 152 rows, 40
   // heads on 5, 65 against 54 us; 768 for two: 8 x 524 rows, 8 on 2 of 128
@@ -1967,10 +1973,10 @@ void run_row_images(const Args &a, const float *q, const float *dout, const floa
 template <int DU>
 void run_fwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, float *o, float *lse,
              float *ml, float *wo, const Images *m) {
-  constexpr int NW = waves(DU);
+  constexpr int NW = fwd_waves(DU, false), NP = fwd_waves(DU, true);
   const dim3 grid((unsigned)(p.tiles * (long)a.B * a.Hkv), (unsigned)p.splits);
   if (m)
-    hipLaunchKernelGGL((attn_fwd_kernel<DU, NW, true>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, o, lse,
+    hipLaunchKernelGGL((attn_fwd_kernel<DU, NP, true>), grid, dim3(64 * NP), 0, stream(), a, q, k, v, o, lse,
                        ml, wo, m->kv, m->kv_flags);
   else
     hipLaunchKernelGGL((attn_fwd_kernel<DU, NW, false>), grid, dim3(64 * NW), 0, stream(), a, q, k, v, o, lse, ml,
@@ -1981,11 +1987,12 @@ template <int DU>
 void run_bwd(const Plan &p, const Args &a, const float *q, const float *k, const float *v, const float *dout,
              const float *lse, const float *delta, float *dq, float *dk, float *dv, float *ws, bool pre,
              const Images &m) {
-  constexpr int NW = waves(DU);
+  constexpr int NW = bwd_waves(DU, false), NP = bwd_waves(DU, true);
+  const int rows = 16 * (pre ? NP : NW);
   const long nbh = (long)a.B * a.Hkv, nk = dk ? p.tiles * nbh * p.splits : 0,
-             nq = dq ? ((long)a.R + 16 * NW - 1) / (16 * NW) * nbh : 0;
+             nq = dq ? ((long)a.R + rows - 1) / rows * nbh : 0;
   if (pre)
-    hipLaunchKernelGGL((attn_bwd_kernel<DU, NW, true>), dim3((unsigned)(nk + nq)), dim3(64 * NW), 0, stream(), a,
+    hipLaunchKernelGGL((attn_bwd_kernel<DU, NP, true>), dim3((unsigned)(nk + nq)), dim3(64 * NP), 0, stream(), a,
                        (int)nk, q, k, v, dout, lse, delta, dq, dk, dv, ws, m);
   else
     hipLaunchKernelGGL((attn_bwd_kernel<DU, NW, false>), dim3((unsigned)(nk + nq)), dim3(64 * NW), 0, stream(), a,
@@ -2003,9 +2010,16 @@ void run_bwd(const Plan &p, const Args &a, const float *q, const float *k, const
     default: F<8>(__VA_ARGS__); break; \
   }
 
+// maxima and sums of the parts of a row, and the results behind them
+size_t ml_bytes(const TTAttention *t, const Plan &p) {
+  return up(sizeof(float) * 2 * p.splits * t->batch * t->q_heads * t->q_rows);
+}
 size_t fwd_parts(const TTAttention *t, const Plan &p) {
   const size_t rows = (size_t)t->batch * t->q_heads * t->q_rows;
-  return p.splits > 1 ? up(sizeof(float) * rows * p.splits * (2 + (size_t)p.width)) : 0;
+  return p.splits > 1 ? ml_bytes(t, p) + up(sizeof(float) * rows * p.splits * p.width) : 0;
+}
+size_t fwd_bytes(const TTAttention *t, const Plan &p) {
+  return fwd_parts(t, p) + images_of(t, !p.few && images_for_rows(t), false, NULL).bytes;
 }
 
 // delta of every query row, and the parts of dk and dv
@@ -2018,8 +2032,7 @@ size_t dkv_parts(const TTAttention *t, const Plan &p) {
 
 extern "C" size_t tt_k_attention_fwd_ws(const TTAttention *t) {
   if (check(t)) return 0;
-  const Plan p = plan_of(t);
-  return fwd_parts(t, p) + images_of(t, images_for_rows(t), false, NULL).bytes;
+  return fwd_bytes(t, plan_of(t));
 }
 
 extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const float *k, const float *v, float *o,
@@ -2030,13 +2043,13 @@ extern "C" int tt_k_attention_fwd(const TTAttention *t, const float *q, const fl
   Args a = args_of(t);
   a.splits = p.splits;
   a.chunk = p.chunk;
-  const size_t need = tt_k_attention_fwd_ws(t);
+  const size_t need = fwd_bytes(t, p);
   void *own = NULL;
   if (need && !ws) {
     ws = own = ttrt_alloc(need);
     if (!own) return -2;
   }
-  float *ml = (float *)ws, *wo = ml ? ml + 2 * (size_t)p.splits * t->batch * t->q_heads * t->q_rows : NULL;
+  float *ml = (float *)ws, *wo = (float *)((char *)ws + ml_bytes(t, p));
   if (p.few) {
     BY_STEPS(blocks(a.D), run_few, p, a, q, k, v, o, lse, ml, wo);
   } else {
