@@ -29,7 +29,8 @@ def _run(L, z, ids, t, T, scale, grad=True):
     return loss.to_np(), dz.to_np(z.shape) if grad else None
 
 
-@pytest.mark.parametrize("rows,cols,top", [(1, 1, 1), (3, 2, 2), (5, 10, 3), (130, 63, 8), (4, 64, 64), (3, 100, 65),
+@pytest.mark.parametrize("rows,cols,top", [(1, 1, 1), (3, 2, 2), (700, 3, 3), (9, 5, 2), (9, 6, 6), (9, 7, 1),
+                                           (3, 131071, 40), (600, 66001, 5), (5, 10, 3), (130, 63, 8), (4, 64, 64), (3, 100, 65),
                                            (7, 1003, 8), (2, 1024, 1), (2, 1025, 17), (5, 4096, 128), (3, 4097, 5),
                                            (2, 16384, 64), (3, 16387, 3), (2, 32000, 64), (2, 32769, 33),
                                            (2, 65536, 16), (3, 65537, 9), (2, 131072, 50), (2, 2000, 1024),

@@ -10,7 +10,8 @@ from tinytorch_amd.hip import DevBuf, check
 
 pytestmark = pytest.mark.gpu
 
-SIZES = [(1, 1), (3, 1), (1, 7), (5, 4), (257, 64), (33, 255), (7, 256), (9, 257), (600, 512), (5, 516), (3, 1000),
+SIZES = [(5000, 3), (4097, 2), (3000, 1), (4099, 5), (3, 6), (3, 7), (600, 2555), (2, 16383), (2, 16385),
+         (1, 1), (3, 1), (1, 7), (5, 4), (257, 64), (33, 255), (7, 256), (9, 257), (600, 512), (5, 516), (3, 1000),
          (1025, 1024), (4099, 1003), (4, 1028), (17, 2047), (3, 2048), (70, 3000), (5, 4096), (3, 4100),
          (9, 8191), (2, 8192), (300, 8200), (3, 16384), (5, 16385), (70, 20000)]
 

@@ -342,7 +342,10 @@ int rows_a_group(long cols) { return cols <= 1024 ? 4 : 1; }
 // threads, one of 1024, and two row groups at least for each; a few more of them
 // where that saves a pass (4099 rows of 1003 columns: 20.1 -> 19.0 us).
 int bwd_blocks(long rows, long cols) {
-  if (long_rows(cols)) return rows < 64 ? (int)rows : 64;
+  if (long_rows(cols)) {  // few columns leave few threads, so more runs of rows
+    const long runs = cols < 4 ? 2048 : 64;
+    return (int)(rows < runs ? rows : runs);
+  }
   const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols), most = cols <= 4096 ? 512 : 256;
   const long each = groups < 2 * most ? 2 : groups / most;
   return (int)((groups + each - 1) / each);
