@@ -1751,6 +1751,8 @@ __global__ void __launch_bounds__(64 * NW, bwd_lives(DU, PRE))
   __shared__ __attribute__((aligned(16))) char lds[2][2 * Dim<DU>::SIZE + STATS];
   const int p = blockIdx.x;
   if (p < dkv_blocks) {
+    // splits outermost: the tiles at work at once share rows in the caches (side by
+    // side: 2 x 4096 rows, 16 heads on 4, 128 columns 2757 against 2200 us)
     const int n = __builtin_amdgcn_readfirstlane(dkv_blocks / a.splits), split = __builtin_amdgcn_readfirstlane(p / n);
     dkv_tile<DU, NW, PRE>(a, lds, p - split * n, n, split, q, k, v, dout, lse, delta, dk, dv, ws, m.rows, m.row_flags);
   } else {
