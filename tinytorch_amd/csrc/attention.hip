@@ -152,8 +152,8 @@ __device__ __forceinline__ int snake(int p, int all) {
 struct Item {
   int b, h, tile;
 };
-__device__ __forceinline__ Item item_of(const Args &a, int block, int blocks, const int32_t *len, int rows, int G, int per,
-                                        bool from_end) {
+__device__ __forceinline__ Item item_of(const Args &a, int block, int blocks, const int32_t *len, int rows, int G,
+                                        int per, bool from_end) {
   int p = snake(block, blocks);
   const int T = blocks / (a.B * a.Hkv);
   Item it;
@@ -405,7 +405,7 @@ struct Dim {
     const int quad = ((r >> 2 ^ r >> 3) & 1) << 1 | (r >> 3 & 1);
     return RC == 16 ? (r & 3) << 2 | quad : RC == 8 ? (r >> 1 & 1) << 2 | quad : quad;
   }
-  // the place of fours of chunks u (and, x: 0 or 2, of chunk x in it) for a lane whose place in the first is `at`
+  // the place of chunk x (0 or 2) of the u-th four, where a lane's place in the first is `at`
   static __device__ __forceinline__ int four(int at, int u, int x = 0) {
     return RC % 8 == 4 ? (at ^ x << 4) + u * 64 : at ^ (4 * u + x) << 4;
   }
@@ -450,8 +450,8 @@ struct Chunk {
 };
 
 // A step: the reads of the next one's operands, six products, and some of the
-// work of `side`, whose instructions go between the products.  Nothing moves from step to step:
-// left alone, the compiler moves every read of an unrolled loop to its front
+// work of `side`, whose instructions go between the products.  Nothing moves from
+// step to step: left alone, the compiler moves every read of an unrolled loop to its front
 // and runs out of registers.
 __device__ __forceinline__ void step_end() {
 #pragma unroll
@@ -1871,7 +1871,8 @@ bool images_for_rows(const TTAttention *t) {
   return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS && fits_images(t, t->k_rows);
 }
 bool images_for_keys(const TTAttention *t) {
-  return t->q_rows * (t->q_heads / t->kv_heads) >= IMAGE_ROWS_BWD && t->k_rows >= IMAGE_KEYS && fits_images(t, t->k_rows) && fits_images(t, t->q_rows * (t->q_heads / t->kv_heads));
+  const long rows = t->q_rows * (t->q_heads / t->kv_heads);
+  return rows >= IMAGE_ROWS_BWD && t->k_rows >= IMAGE_KEYS && fits_images(t, t->k_rows) && fits_images(t, rows);
 }
 
 Plan plan_of(const TTAttention *t) {
