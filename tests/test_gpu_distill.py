@@ -119,3 +119,26 @@ def test_distill_gradient_by_differences(tlib):
     d = np.random.default_rng(2).standard_normal(z.shape)
     f = [ref.distill(z.astype(np.float64) + h * d, ids, t, 2.0, 1.0)[0][0].sum() for h in (1e-5, -1e-5)]
     assert abs((f[0] - f[1]) / 2e-5 - (dz * d).sum()) <= 1e-5 * np.abs(dz * d).sum()
+
+
+WIDTHS = [2, 50, 1003, 4096, 5000, 16384, 32001, 65536, 70001]  # each kernel, with and without a tail
+
+
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_distill_rows_of_nan(tlib, cols):
+    """Rows of NaN, and of NaN and -inf, have no finite loss and no finite
+    gradient, whatever their width; a row of -inf and the others do."""
+    z, ids, t = _inputs(6, cols, 2)
+    z[1] = np.nan
+    z[2] = -np.inf
+    z[2, cols - 1] = np.nan
+    z[3] = np.nan
+    z[3, 0] = -np.inf
+    z[4] = -np.inf
+    want = ref.distill(z[[0, 4, 5]], ids[[0, 4, 5]], t[[0, 4, 5]], 2.0, 0.5)
+    loss, dz = _run(tlib, z, ids, t, 2.0, 0.5)
+    assert np.isnan(loss[1:4]).all() and np.isnan(dz[1:4]).all()
+    ref.close(loss[[0, 4, 5]], want[0], "loss")
+    ref.close(dz[[0, 4, 5]], want[1], "dlogits")
+    only, _ = _run(tlib, z, ids, t, 2.0, 0.5, grad=False)
+    assert np.array_equal(only, loss, equal_nan=True)

@@ -194,13 +194,16 @@ __global__ void __launch_bounds__(NT) distill_kernel(Call a) {
 #pragma unroll
     for (int n = 0; n < NV; n++) most = fmaxf(most, fmaxf(fmaxf(v[n][0], v[n][1]), fmaxf(v[n][2], v[n][3])));
     most = group_all<NT>(most, part, Max());
+    // a flat row holds -inf, which count as equal, or NaN, which the maximum
+    // passed over and the sum takes to the loss and the gradient
     const bool flat = most == -INFINITY;
+    const float base = flat ? 0.f : most, equal = flat ? 1.f : 0.f;
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; n++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        float x = flat ? 1.f : exp2_fast((v[n][j] - most) * a.c);
+        float x = exp2_fast((v[n][j] - base) * a.c) + equal;
         if (j < Group<TAIL>((n * NT + t) * 4, a.cols).by) x = 0.f;
         v[n][j] = x;
         sum += x;
