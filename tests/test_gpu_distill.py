@@ -142,3 +142,26 @@ def test_distill_rows_of_nan(tlib, cols):
     ref.close(dz[[0, 4, 5]], want[1], "dlogits")
     only, _ = _run(tlib, z, ids, t, 2.0, 0.5, grad=False)
     assert np.array_equal(only, loss, equal_nan=True)
+
+
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_distill_rows_left_out(tlib, cols):
+    """Rows without entries, or with -inf for all of them, have loss and gradient
+    0 whatever their logits hold."""
+    z, ids, t = _inputs(7, cols, 2)
+    z[0] = np.nan
+    z[1, 0] = np.nan
+    z[2, cols - 1] = np.inf
+    z[3] = np.inf
+    z[4, cols // 2] = np.nan
+    z[5] = -np.inf
+    ids[:3], ids[3] = -1, cols
+    t[4:6] = -np.inf
+    ids[4] = cols // 2
+    loss, dz = _run(tlib, z, ids, t, 2.0, 0.5)
+    assert not loss[:6].any() and not dz[:6].any()
+    want = ref.distill(z[6:], ids[6:], t[6:], 2.0, 0.5)
+    ref.close(loss[6:], want[0], "loss")
+    ref.close(dz[6:], want[1], "dlogits")
+    only, _ = _run(tlib, z, ids, t, 2.0, 0.5, grad=False)
+    assert np.array_equal(only, loss)
