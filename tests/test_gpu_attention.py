@@ -403,3 +403,25 @@ def test_gradients_by_differences(tlib):
             p[i] = p[i] + h * d
             f.append((ref.attention(*p, m)["o"][0] * do).sum())
         assert abs((f[0] - f[1]) / 2e-5 - (got[name] * d).sum()) <= 1e-5 * np.abs(got[name] * d).sum()
+
+
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv", [(1, 300, 4, 2), (1, 5000, 4, 2), (20, 3000, 1, 1), (70, 70, 2, 2),
+                                          (130, 2000, 1, 1), (300, 330, 4, 1), (1100, 900, 1, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_nan_that_has_no_weight_is_seen(tlib, Lq, Lk, Hq, Hkv, causal):
+    """0 * NaN is NaN, also where a key's weight is 0 next to the others' and it
+    lies in a part of keys that have none."""
+    q, k, v, do = _inputs(1, Lq, Lk, Hq, Hkv, 64)
+    q, k = np.abs(q) + 1, np.abs(k) + 1
+    see = ref.seen(1, Lq, Lk, causal=causal)
+    for none, j in ((slice(0, Lk // 2), 0), (slice(Lk // 2, Lk), Lk // 2 + 1)):
+        k2, v2 = k.copy(), v.copy()
+        k2[0, none] = -60   # hundreds below the others: exp is 0 in 32 bits
+        want = ref.attention(q, k2, v, see, None, do)["o"]
+        v2[0, j, :, 3] = np.nan
+        got = _run(tlib, q, k2, v2, do, dict(causal=causal))["o"]
+        meet = see[0, :, j]
+        assert np.isnan(got[0, meet, :, 3]).all()
+        rest = np.ones(got.shape, bool)
+        rest[0, meet, :, 3] = False
+        ref.close(got[rest], tuple(x[rest] for x in want), "o")

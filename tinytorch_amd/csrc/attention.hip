@@ -1212,7 +1212,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
 }
 
 // The parts of a row that several workgroups took, joined in a fixed order.  A
-// part without keys has sum 0 and no values.
+// part without keys has sum 0 and values 0; one without weight next to the others
+// counts times 0, so that a NaN that the row sees in it stays.
 __device__ __forceinline__ void join_store(const Args &a, long at, float top, float total, float2 x, int lane,
                                            float *o, float *lse) {
   const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
@@ -1256,7 +1257,7 @@ __global__ void __launch_bounds__(256)
       const float f = ml[s].y == 0.f ? 0.f : exp2_fast(ml[s].x - base);
       total = fmaf(f, ml[s].y, total);
 #pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = f == 0.f ? x[j] : fmaf(f, v[s][j], x[j]);
+      for (int j = 0; j < 4; j++) x[j] = fmaf(f, v[s][j], x[j]);
     }
     const int bh = (int)(at / a.R), r = (int)(at % a.R), b = bh / a.Hkv, i = r / a.G;
     const int hq = bh % a.Hkv * a.G + r - i * a.G;
@@ -1323,7 +1324,7 @@ __global__ void __launch_bounds__(JOIN)
         const float f = weight[s];
         const f32x4 v = *(const f32x4 *)(p + s * rows * width);
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = f == 0.f ? x[j] : fmaf(f, v[j], x[j]);
+        for (int j = 0; j < 4; j++) x[j] = fmaf(f, v[j], x[j]);
       }
       *(f32x4 *)(sums + group * width + c) = x;
     }
