@@ -425,3 +425,37 @@ def test_nan_that_has_no_weight_is_seen(tlib, Lq, Lk, Hq, Hkv, causal):
         rest = np.ones(got.shape, bool)
         rest[0, meet, :, 3] = False
         ref.close(got[rest], tuple(x[rest] for x in want), "o")
+
+
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv,causal", [(1, 300, 4, 2, False), (20, 700, 1, 1, True), (70, 100, 2, 2, True),
+                                                 (130, 2000, 1, 1, False), (300, 330, 8, 2, True),
+                                                 (1100, 900, 1, 1, True)])
+@pytest.mark.parametrize("bad", [0.0, np.nan])
+def test_operands_that_end_with_the_last_sequence(tlib, Lq, Lk, Hq, Hkv, causal, bad):
+    """q, k, v and dout lie at the end of an allocation, their last sequence cut
+    off behind its q_len and k_len; a NaN in the last key brings the slow paths."""
+    q, k, v, do = _inputs(2, Lq, Lk, Hq, Hkv, 48)
+    masks = dict(q_len=[Lq, Lq // 2], k_len=[Lk, Lk // 3], q_start=[Lk - Lq, Lk // 3 - Lq // 2], causal=causal)
+    see = ref.seen(2, Lq, Lk, **masks)
+    want = ref.attention(q, k, v, see, None, do)
+    j = masks["k_len"][1] - 1
+    k[1, j, :, 5] += bad
+    v[1, j, :, 3] += bad
+    held, at = [], []
+    size = 66 << 20
+    for t, n in ((q, masks["q_len"][1]), (k, j + 1), (v, j + 1), (do, masks["q_len"][1])):
+        x = np.ascontiguousarray(t.reshape(-1)[:t[0].size + t[1, :n].size])
+        held.append(DevBuf(size // 4))
+        at.append(held[-1].ptr + size - x.nbytes)
+        check(tlib.tth_h2d(at[-1], x.ctypes.data, x.nbytes), "h2d")
+    a = _plan(q, k, masks, held)
+    o, lse, out = DevBuf(q.size), DevBuf(2 * Hq * Lq), [DevBuf(t.size) for t in (q, k, v)]
+    check(tlib.tt_k_attention_fwd(a, *at[:3], o.ptr, lse.ptr, None), "fwd")
+    check(tlib.tt_k_attention_bwd(a, *at[:3], o.ptr, at[3], lse.ptr, *[x.ptr for x in out], None), "bwd")
+    rest = ~see[:, :, j] if bad else np.ones((2, Lq), bool)
+    rest[0] = True
+    for n, x in (("o", o), ("dq", out[0])):
+        ref.close(x.to_np(q.shape)[rest], tuple(w[rest] for w in want[n]), n)
+    if not bad:
+        ref.close(out[1].to_np(k.shape), want["dk"], "dk")
+        ref.close(out[2].to_np(v.shape), want["dv"], "dv")

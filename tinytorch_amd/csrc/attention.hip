@@ -840,7 +840,8 @@ __device__ __forceinline__ void fwd_one_by_one(const Args &a, const Seq &sq, int
     Range rg = range_of(a, sq, i);
     if (rg.lo < k0) rg.lo = k0;
     if (rg.hi > k1) rg.hi = k1;
-    Pair qv = load2(q + (long)i * a.q.r + (long)hm * a.q.h, a.D, lane), acc = {0.f, 0.f};
+    Pair qv = {0.f, 0.f}, acc = qv;
+    if (rg.lo < rg.hi) qv = load2(q + (long)i * a.q.r + (long)hm * a.q.h, a.D, lane);
     qv.x *= a.scale * LOG2E;
     qv.y *= a.scale * LOG2E;
     float mx = -INFINITY, sum = 0.f;
@@ -918,10 +919,10 @@ __global__ void __launch_bounds__(64 * NW, fwd_lives(DU, PRE))
   f32x4 acc[DU];
   float mx = -INFINITY, sum = 0.f;
   const int row = r0 + wave * 16 + (lane & 15), i = row / a.G;
-  const bool in = row < a.R;
+  const bool in = row < a.R, live = in && i < sq.queries;  // q holds nothing behind the sequence's queries
   Range rg = {0, 0};
-  if (in) rg = range_of(a, sq, i);
-  load_parts<DU>(qf, qp + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, in, a.scale * LOG2E, a.D, a.vec, lane);
+  if (live) rg = range_of(a, sq, i);
+  load_parts<DU>(qf, qp + (long)i * a.q.r + (long)(row - i * a.G) * a.q.h, live, a.scale * LOG2E, a.D, a.vec, lane);
 #pragma unroll
   for (int n = 0; n < DU; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (k_first < k_end) {
@@ -1068,9 +1069,9 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
     if (c1 < k_end) k_end = (int)c1;
   }
   const int row = r0 + m, i = row / a.G, hq = h * a.G + row - i * a.G;
-  const bool in = row < a.R;
+  const bool live = row < a.R && i < sq.queries;  // q holds nothing behind the sequence's queries
   Range rg = {0, 0};
-  if (in) rg = range_of(a, sq, i);
+  if (live) rg = range_of(a, sq, i);
   f32x4 qf[DB], acc[DB];
   float mx = -INFINITY, sum = 0.f;
   const float *qp = q + (long)b * a.q.b + (long)i * a.q.r + (long)hq * a.q.h;
@@ -1078,7 +1079,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
   for (int u = 0; u < DB; u++) {
     qf[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
     acc[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (in) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
+    if (live) qf[u] = load4(qp, 16 * u + 4 * g, a.D, a.vec) * (a.scale * LOG2E);
   }
   const float *kp = k + (long)b * a.k.b + (long)h * a.k.h, *vp = v + (long)b * a.v.b + (long)h * a.v.h;
   FewTile<DB> cur;
