@@ -509,7 +509,8 @@ int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *position
  * and one past q_len, has o = 0 and lse = -inf and takes no part in the
  * gradients; what lies behind k_len and q_len is not read.  Lengths outside
  * [0, rows] are clamped.  An infinity that a query sees in q, k, v or dout
- * comes out as NaN; one that the masks hide from it does not reach it.
+ * comes out as NaN; one that the masks hide from it does not reach it.  A score
+ * below the type's range has no weight or is NaN, one above it is NaN.
  * Workspaces are 16-byte aligned; with many rows they hold q, k, v and dout
  * once more at 1.5 times their size (at most 4 GiB each for k with v and for q
  * with dout), and parts of dk and dv (at most 4 GiB). */

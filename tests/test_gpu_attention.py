@@ -459,3 +459,98 @@ def test_operands_that_end_with_the_last_sequence(tlib, Lq, Lk, Hq, Hkv, causal,
     if not bad:
         ref.close(out[1].to_np(k.shape), want["dk"], "dk")
         ref.close(out[2].to_np(v.shape), want["dv"], "dv")
+
+
+INFINITE = [(1, 300, 4, 2), (1, 5000, 4, 2), (16, 90, 1, 1), (32, 700, 1, 1), (33, 700, 1, 1), (70, 70, 2, 2),
+            (300, 330, 4, 1), (1100, 600, 1, 1)]
+
+
+def _infinite(tlib, shape, masks, which, bad):
+    """Results with an infinity at column 5 (at 3 in v and dout) of one key's or
+    query's first head, what to expect without it, and who sees it."""
+    Lq, Lk, Hq, Hkv = shape
+    q, k, v, do = _inputs(1, Lq, Lk, Hq, Hkv, 40)
+    see = ref.seen(1, Lq, Lk, **masks)
+    want = ref.attention(q, k, v, see, None, do)
+    # the last key that some but not all queries see, or the last
+    n = see[0].sum(0)
+    j = int(np.flatnonzero((n > 0) & (n < Lq) if ((n > 0) & (n < Lq)).any() else n > 0)[-1])
+    i = Lq // 2
+    dict(q=q, k=k, v=v, do=do)[which][0, j if which in "kv" else i, 0, 5 if which in "qk" else 3] = bad
+    return _run(tlib, q, k, v, do, masks), want, see[0], i, j
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+@pytest.mark.parametrize("masks", [dict(), dict(causal=True)])
+@pytest.mark.parametrize("shape", INFINITE)
+def test_infinite_keys(tlib, shape, masks, bad):
+    """One infinity in k, of either sign of the product: NaN for the queries that
+    see it and what comes of them, whichever kernel takes them."""
+    got, want, see, _, j = _infinite(tlib, shape, masks, "k", bad)
+    G, meet = shape[2] // shape[3], see[:, j]
+    assert meet.any()
+    heads = np.arange(shape[2]) < G
+    for n in ("o", "dq"):
+        assert np.isnan(got[n][0][meet][:, heads]).all(), n
+        for rows, hs in ((~meet, slice(None)), (slice(None), ~heads)):
+            ref.close(got[n][0][rows][:, hs], tuple(x[0][rows][:, hs] for x in want[n]), n)
+    assert np.isnan(got["lse"][0][heads][:, meet]).all()
+    ref.close(got["lse"][0][heads][:, ~meet], tuple(x[0][heads][:, ~meet] for x in want["lse"]), "lse")
+    touched = see[meet].any(0)
+    for n in ("dk", "dv"):
+        assert np.isnan(got[n][0, touched, 0]).all(), n
+        ref.close(got[n][0, ~touched, 0], tuple(x[0, ~touched, 0] for x in want[n]), n)
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+@pytest.mark.parametrize("masks", [dict(), dict(causal=True)])
+@pytest.mark.parametrize("shape", INFINITE)
+def test_infinite_values(tlib, shape, masks, bad):
+    """One infinity in v: NaN in its column of the results that see it, and in
+    what their rows' gradients reach; dv and lse do not depend on it."""
+    got, want, see, _, j = _infinite(tlib, shape, masks, "v", bad)
+    G, meet = shape[2] // shape[3], see[:, j]
+    heads = np.arange(shape[2]) < G
+    o = got["o"][0]
+    assert np.isnan(o[meet][:, heads, 3]).all()
+    rest = np.ones(o.shape, bool)
+    rest[np.ix_(meet, heads, [3])] = False
+    ref.close(o[rest], tuple(x[0][rest] for x in want["o"]), "o")
+    ref.close(got["lse"], want["lse"], "lse")
+    ref.close(got["dv"], want["dv"], "dv")
+    assert np.isnan(got["dq"][0][meet][:, heads]).all()
+    ref.close(got["dq"][0][~meet], tuple(x[0][~meet] for x in want["dq"]), "dq")
+    assert np.isnan(got["dk"][0, see[meet].any(0), 0]).all()
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+@pytest.mark.parametrize("masks", [dict(), dict(causal=True)])
+@pytest.mark.parametrize("shape", INFINITE)
+def test_infinite_queries_and_gradients(tlib, shape, masks, bad):
+    """One infinity in q: NaN for its row and the keys that it sees; in dout: NaN
+    in dq of its row, in dk of these keys and in its column of their dv."""
+    for which in ("q", "do"):
+        got, want, see, i, _ = _infinite(tlib, shape, masks, which, bad)
+        rest, keys = np.arange(shape[0]) != i, see[i]
+        for n in ("o", "dq"):
+            if which == "q" or n == "dq":
+                assert np.isnan(got[n][0, i, 0]).all(), (which, n)
+            else:
+                ref.close(got[n], want[n], n)
+            ref.close(got[n][0, rest], tuple(x[0, rest] for x in want[n]), n)
+        assert np.isnan(got["lse"][0, 0, i]) == (which == "q")
+        assert np.isnan(got["dk"][0, keys, 0]).all(), which
+        at = slice(None) if which == "q" else 3
+        assert np.isnan(got["dv"][0, keys, 0][:, at]).all(), which
+        for n in ("dk", "dv"):
+            ref.close(got[n][0, ~keys], tuple(x[0, ~keys] for x in want[n]), n)
+
+
+def test_infinite_queries_that_see_no_key(tlib):
+    """No key: 0 and -inf, whatever the query holds."""
+    for Lq in (1, 20, 70, 1100):
+        q, k, v, do = _inputs(1, Lq, 90, 1, 1, 40)
+        q[0, Lq // 2] = np.inf
+        got = _run(tlib, q, k, v, do, dict(k_len=[0]))
+        assert np.isneginf(got["lse"]).all()
+        assert not any(got[n].any() for n in ("o", "dq", "dk", "dv")), Lq
