@@ -480,6 +480,7 @@ int tt_k_layernorm_bwd(const float *x, const float *w, const float *dy, const fl
  *   TT_ROPE_PARTS   with n_j = trained * f_j / (2 pi) turns over the trained
  *                   length and r = clamp((n_j - low) / (high - low), 0, 1):
  *                   (1 - r) f_j / factor + r f_j
+ * Parameters that leave a frequency without a finite value are refused.
  * and every turned pair is multiplied by magnitude (0: 1). */
 #define TT_ROPE_PLAIN  0
 #define TT_ROPE_LINEAR 1

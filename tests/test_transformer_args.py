@@ -171,3 +171,28 @@ def test_node_methods_exist():
         sys.path.pop(0)
     for meth in ("layernorm", "rope", "attention", "distill"):
         assert hasattr(m.Node, meth) and hasattr(Node, meth)
+
+
+@pytest.mark.parametrize("kw", [dict(low=float("-inf"), high=1.0), dict(low=float("-inf"), high=float("inf"))])
+def test_rope_refuses_a_ramp_without_a_start(L, kw):
+    """r = clamp((n - low) / (high - low)) has no value there: NaN frequencies."""
+    f = (ctypes.c_double * 32)()
+    r = rope(scaling=3, factor=8.0, trained=8192.0, **kw)
+    assert L.tt_rope_frequencies(r, f) == -1
+    assert L.tt_k_rope(r, P, P, None, 4, 4, 2, 0, 0, 0) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(scaling=2, factor=1e-200, rot_dim=4), dict(base=5e-324),
+                                dict(scaling=1, factor=1e-310), dict(scaling=3, factor=1e-310, trained=1.0, high=9.0)])
+def test_rope_refuses_frequencies_past_the_range(L, kw):
+    """Finite parameters whose frequencies are not: position 0 times them is NaN."""
+    f = (ctypes.c_double * 32)()
+    assert L.tt_rope_frequencies(rope(**kw), f) == -1
+    assert L.tt_k_rope(rope(**kw), P, P, None, 4, 4, 2, 0, 0, 0) == -1
+
+
+def test_rope_takes_a_ramp_without_an_end(L):
+    """high = infinity keeps no frequency."""
+    f = (ctypes.c_double * 32)()
+    assert L.tt_rope_frequencies(rope(scaling=3, factor=8.0, trained=8192.0, low=1.0, high=float("inf")), f) == 0
+    np.testing.assert_allclose(np.array(f), frequencies(64, 10000.0) / 8, rtol=1e-13)

@@ -158,6 +158,7 @@ extern "C" int tt_rope_frequencies(const TTRope *r, double *f) {
       keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
       f[j] = (1 - keep) * f[j] * per + keep * f[j];
     }
+    if (!(fabs(f[j]) < INFINITY)) return -1;  // low = -infinity, or past the range: NaN at every position
   }
   return 0;
 }
@@ -179,9 +180,9 @@ extern "C" int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_
   if (n < 1) n = 1;
   if ((rows + n - 1) / n > (1L << 24) - 1) n = (rows + (1L << 24) - 2) / ((1L << 24) - 1);
   if (n > 4096 / pairs || n * width > 0x7fffffffL) return -1;
-  if (ttrt_init() != 0) return -3;
   Turns t;
-  tt_rope_frequencies(r, t.f);
+  if (tt_rope_frequencies(r, t.f) != 0) return -1;
+  if (ttrt_init() != 0) return -3;
   for (int j = 0; j < r->rot_dim / 2; j++) t.f[j] *= 1 / (2 * M_PI);
   const float sign = transpose ? -1.f : 1.f, mag = r->magnitude != 0 ? (float)r->magnitude : 1.f;
   const dim3 grid((unsigned)((rows + n - 1) / n));
