@@ -547,7 +547,10 @@ int tt_k_attention_bwd(const TTAttention *a, const float *q, const float *k, con
  *   dlogits = scale * T * (q - the p_e at their columns)      (unless NULL)
  * Entries whose id is outside [0, cols) are left out, entries of one column
  * add up.  A row without entries, or with -inf for all of them, has loss and
- * gradient 0; dlogits may not be logits.  A row of logits of -inf counts as a row of equal ones. */
+ * gradient 0 whatever its logits; of the others one with a NaN or +inf among its
+ * logits has NaN for both, and one of -inf alone counts as a row of equal ones.
+ * dlogits may not be logits.  T is refused outside about [2^-63, 2^64), where T^2
+ * leaves the type's normal range. */
 #define TT_DISTILL_MAX_TOP 1024
 int tt_k_distill(const float *logits, const int32_t *ids, const float *teacher, int top,
                  float temperature, float *rowloss, float *dlogits, long rows, int cols,

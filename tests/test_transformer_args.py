@@ -196,3 +196,11 @@ def test_rope_takes_a_ramp_without_an_end(L):
     f = (ctypes.c_double * 32)()
     assert L.tt_rope_frequencies(rope(scaling=3, factor=8.0, trained=8192.0, low=1.0, high=float("inf")), f) == 0
     np.testing.assert_allclose(np.array(f), frequencies(64, 10000.0) / 8, rtol=1e-13)
+
+
+@pytest.mark.parametrize("T,scale", [(1e-39, 1.0), (1e-30, 1.0), (1e-19, 1.0), (1.9e19, 1.0), (1e38, 0.0),
+                                     (1e18, 1e30)])
+def test_distill_refuses_temperatures_past_the_range(L, T, scale):
+    """1 / T, T^2 and scale T are factors in 32 bits: infinite or without their
+    bits they leave NaN or a wrong loss."""
+    assert L.tt_k_distill(P, P, P, 3, T, P, 2 * P, 4, 10, scale) == -1

@@ -314,6 +314,9 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
       !(temperature > 0.f) || isinf(temperature) || !(scale == scale) || isinf(scale) || rows > (1L << 40) / cols ||
       dlogits == logits)
     return -1;
+  // factors in 32 bits: T^2 and scale T, and 1 / T with them, within its normal numbers
+  if (!(temperature * temperature >= 0x1p-126f) || isinf(temperature * temperature) || isinf(scale * temperature))
+    return -1;
   if (ttrt_init() != 0) return -3;
   const Call a = {logits, ids, teacher, rowloss, dlogits, rows, cols, top, LOG2E / temperature,
                   temperature * temperature, scale * temperature};
