@@ -153,3 +153,18 @@ def test_layernorm_gradient_by_differences(tlib):
         slope = (f[0] - f[1]) / 2e-5
         # the differences are good to about 1e-9, the gradient to its bound
         assert abs(slope - (g * d).sum()) <= 1e-5 * np.abs(g * d).sum()
+
+
+def test_layernorm_gradients_of_the_longest_rows(tlib):
+    """Past 2^26 columns: the sums for dw and db pass a grid axis's threads.  With
+    one row, mean 0 and rstd 1 they are dy x and dy, to the bit."""
+    cols = (1 << 26) + 5
+    rng = np.random.default_rng(3)
+    x, dy = rng.standard_normal(cols, np.float32), rng.standard_normal(cols, np.float32)
+    d = [DevBuf.from_np(t) for t in (x, dy, np.zeros(1, np.float32), np.ones(1, np.float32))]
+    dw, db = DevBuf(cols), DevBuf(cols)
+    check(tlib.tt_k_layernorm_bwd(d[0].ptr, None, *[t.ptr for t in d[1:]], None, dw.ptr, db.ptr, 1, cols, None), "bwd")
+    assert np.array_equal(dw.to_np(), dy * x) and np.array_equal(db.to_np(), dy)
+    for t in d + [dw, db]:
+        t.free()
+    tlib.tth_release_cache()

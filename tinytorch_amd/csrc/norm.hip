@@ -229,23 +229,26 @@ __global__ void __launch_bounds__(1024)
                    long cols) {
   __shared__ float sum[16][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long c = (long)blockIdx.x * 16 + (lane & 15);
   float *out = blockIdx.y ? db : dw;
   if (!out) return;
-  float s = 0.f;
-  if (c < cols) {
+  for (long c0 = (long)blockIdx.x * 16; c0 < cols; c0 += (long)gridDim.x * 16) {
+    const long c = c0 + (lane & 15);
+    float s = 0.f;
+    if (c < cols) {
 #pragma unroll 8
-    for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += part[((long)k * 2 + blockIdx.y) * cols + c];
-  }
-  s += __shfl_xor(s, 16);
-  s += __shfl_xor(s, 32);
-  if (lane < 16) sum[wave][lane] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && c < cols) {
-    s = 0.f;
+      for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += part[((long)k * 2 + blockIdx.y) * cols + c];
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (lane < 16) sum[wave][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < cols) {
+      s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; k++) s += sum[k][lane];
-    out[c] = s;
+      for (int k = 0; k < 16; k++) s += sum[k][lane];
+      out[c] = s;
+    }
+    __syncthreads();
   }
 }
 
@@ -416,9 +419,12 @@ extern "C" int tt_k_layernorm_bwd(const float *x, const float *w, const float *d
     BY_COLS(RUN)
 #undef RUN
   }
-  if (part)
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((cols + 15) / 16), 2), dim3(1024), 0, stream(), part, dw, db,
-                       blocks, cols);
+  if (part) {
+    // a grid axis has less than 2^32 threads (with more, columns stay unwritten)
+    const long groups = (cols + 15) / 16;
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20), 2), dim3(1024), 0,
+                       stream(), part, dw, db, blocks, cols);
+  }
   ttrt_free(own);
   return launched();
 }
