@@ -511,10 +511,13 @@ int tt_k_rope(const TTRope *r, const float *x, float *y, const int32_t *position
  * gradients; what lies behind k_len and q_len is not read.  Lengths outside
  * [0, rows] are clamped.  An infinity that a query sees in q, k, v or dout
  * comes out as NaN; one that the masks hide from it does not reach it.  A score
- * below the type's range has no weight or is NaN, one above it is NaN.
+ * below the type's range has no weight or is NaN, one above it is NaN.  Infinities
+ * and NaN within a tile (32 keys or rows) of the masks' edges are taken a row at a
+ * time: a batch full of them takes about a hundred times as long.
  * Workspaces are 16-byte aligned; with many rows they hold q, k, v and dout
- * once more at 1.5 times their size (at most 4 GiB each for k with v and for q
- * with dout), and parts of dk and dv (at most 4 GiB). */
+ * once more, 6 bytes a value with head_dim rounded up to a multiple of 32 (at
+ * most 4 GiB each for k with v and for q with dout), and parts of dk and dv (at
+ * most 4 GiB). */
 #define TT_ATTENTION_MAX_DIM 128
 typedef struct TTStrides {
     long batch, row, head;  /* floats from one to the next; 0: packed in that order.  Rows and

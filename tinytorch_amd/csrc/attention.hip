@@ -1,5 +1,5 @@
-// Attention on the fp32 matrix units: forward, the form for few query rows,
-// and the backward pass, which recomputes the probabilities.
+// Attention on the matrix units: forward, the form for few query rows, and the
+// backward pass, which recomputes the probabilities.
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  s_ij = scale q_i . k_j
 //   over the keys lo_i <= j < hi_i that the masks leave query i, with
@@ -10,8 +10,8 @@
 //
 // The matrix units multiply fp32 at 1/16 the rate of bf16.  A float is the sum of
 // three bf16 values, exactly (three times 8 bits of its 24), and a product of two
-// such sums is their nine products; the six greatest (all above 2^-23 of it)
-// come out of v_mfma_f32_16x16x32_bf16, which adds in fp32.  The fp32 products,
+// such sums is their nine products; six of them, all but 2^-21 of it (below), come
+// out of v_mfma_f32_16x16x32_bf16, which adds in fp32.  The fp32 products,
 // v_mfma_f32_16x16x4_f32, are left to the form for few rows, which waits for
 // memory.  In both A holds rows lane % 16 and B columns lane % 16, each the summed
 // indexes of its group lane / 16, and C holds column lane % 16, rows
@@ -28,8 +28,9 @@
 // axis r = i * group + member, so shared keys are loaded once for all of them.
 //
 // All sums and statistics are fp32; scores are formed in units of log2 (q or k is
-// multiplied by scale * log2(e) once, a rounding of 2^-24).  An infinity in an
-// operand's place that a mask leaves makes NaN: its parts are it and NaN.
+// multiplied by scale * log2(e) once, a rounding of 2^-24).  An infinity that the
+// masks leave makes NaN: its parts are it and NaN, and the forms without parts do
+// the same.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -244,7 +245,9 @@ __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
 // workgroup falls back to when a tile holds an infinity or NaN that a mask
 // hides from some of its columns (in the matrix units 0 * inf would reach
 // them).  Nothing hidden is read here.  Rare, so small rather than fast: kept
-// apart from the loops that run, whose registers it must not take.
+// apart from the loops that run, whose registers it must not take.  A pass whose
+// tiles on the masks' edges all hold NaN takes about a hundred times as long (8 x
+// 600 to 1024 rows, 8 heads of 64, forward and backward: 0.2 -> 23 ms).
 struct Pair {
   float x, y;
 };
@@ -1052,7 +1055,7 @@ struct FewTile {
 };
 
 template <int DB, int NW>
-__global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : 2)
+__global__ void __launch_bounds__(64 * NW, 2)
     attn_few_kernel(Args a, const float *__restrict__ q, const float *__restrict__ k,
                     const float *__restrict__ v, float *__restrict__ o, float *__restrict__ lse,
                     float *__restrict__ ws_ml, float *__restrict__ ws_o) {
@@ -1416,7 +1419,7 @@ __device__ __forceinline__ void dq_one_by_one(const Args &a, const Seq &sq, int 
 }
 
 // dq of 16 NW packed rows (16 a wave): keys and values through LDS as in the
-// forward pass (the same case: 216 TFLOP/s, matrix units 68 % busy)
+// forward pass
 template <int DU, int NW, bool PRE>
 __device__ __forceinline__ void dq_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
                                         const float *__restrict__ q, const float *__restrict__ k,
@@ -1580,8 +1583,7 @@ __device__ __forceinline__ void dkv_one_by_one(const Args &a, const Seq &seq, in
 // dk and dv of 16 NW keys (16 a wave): the packed query rows that see any of
 // them through LDS, q and do.  With splits > 1 a workgroup takes `chunk` of the
 // rows and leaves its sums to the join: where many rows meet few keys, and so
-// that no fp32 sum runs over more rows than that.  The same case: 195 TFLOP/s,
-// matrix units 64 % busy.
+// that no fp32 sum runs over more rows than that.
 template <int DU, int NW, bool PRE>
 __device__ __forceinline__ void dkv_tile(const Args &a, char (*lds)[2 * Dim<DU>::SIZE + STATS], int block, int blocks,
                                          int split, const float *__restrict__ q, const float *__restrict__ k,
@@ -1753,8 +1755,11 @@ __device__ __forceinline__ void dkv_tile(const Args &a, char (*lds)[2 * Dim<DU>:
 
 // Both gradients in one launch, the keys' tiles first (they take the longest): where
 // either leaves CUs idle, or at its end, the other fills them (10 x 203 rows, 8
-// heads of 64 columns, with the forward pass: 66 -> 49 us).  dkv_blocks: the
-// tiles of dk and dv times their splits.
+// heads of 64 columns, with the forward pass: 66 -> 49 us).  Bound like the forward
+// pass; both gradients form scores and do . v for themselves, seven products a pair
+// for the five that a pass needs (2 x 4096 causal rows, 16 heads on 4, 128 columns:
+// 2.25 ms with the images and the join, 153 TFLOP/s of the five, matrix units 66 %
+// busy at 1.8 GHz).  dkv_blocks: the tiles of dk and dv times their splits.
 template <int DU, int NW, bool PRE>
 __global__ void __launch_bounds__(64 * NW, bwd_lives(DU, PRE))
     attn_bwd_kernel(Args a, int dkv_blocks, const float *__restrict__ q, const float *__restrict__ k,

@@ -327,7 +327,11 @@ extern "C" int tt_k_distill(const float *logits, const int32_t *ids, const float
   else                                                                                       \
     hipLaunchKernelGGL((distill_kernel<NT, NV, true>), grid, dim3(NT), 0, stream(), a)
   // rows of up to 32768 columns leave room for two workgroups a CU, so that one
-  // reads while the other reduces or writes
+  // reads while the other reduces or writes (with a tail past 16384 columns for
+  // one, of 136 registers: 2048 x 20001 108 us, x 20000 67).  Past that a row's 1024
+  // threads have 128 registers each, which a tail overruns: in two passes 2048 x
+  // 32769 / 50257 / 65535 take 141 / 211 / 254 us, in registers that spill 185 / 229
+  // / 262; without a tail 50256 columns take 172 in registers.
   if (cols < 4) {
     hipLaunchKernelGGL(distill_long_kernel<true>, grid, dim3(1024), 0, stream(), a);
   } else if (cols <= 1024) {
