@@ -204,3 +204,19 @@ def test_distill_refuses_temperatures_past_the_range(L, T, scale):
     """1 / T, T^2 and scale T are factors in 32 bits: infinite or without their
     bits they leave NaN or a wrong loss."""
     assert L.tt_k_distill(P, P, P, 3, T, P, 2 * P, 4, 10, scale) == -1
+
+
+def test_inline_assembly_names_the_registers_it_writes():
+    """m0 holds the address of a direct load to LDS: the compiler has to know
+    that it changes."""
+    import glob
+    import os
+    import re
+    found = 0
+    for path in glob.glob(os.path.join(tinytorch_amd.ROOT, "tinytorch_amd", "csrc", "*")):
+        with open(path) as f:
+            for block in re.findall(r"asm volatile\((.*?)\);", f.read(), re.S):
+                if re.search(r"_mov_b32 m0\b", block):
+                    found += 1
+                    assert '"m0"' in block, (path, block)
+    assert found

@@ -668,7 +668,7 @@ __device__ __forceinline__ void dma16(const char *base, int off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds), "v"(off), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 // a pointer that is the same for all lanes, in scalar registers
 __device__ __forceinline__ const char *scalar(const char *p) {

@@ -94,7 +94,7 @@ __device__ __forceinline__ void dma4(const float *base, int voff, unsigned lds) 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                :
                : "s"(lds), "v"(voff), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 
 __device__ __forceinline__ void dma4_if(const float *base, int voff, unsigned lds) {
@@ -106,7 +106,7 @@ __device__ __forceinline__ void dma4_if(const float *base, int voff, unsigned ld
                "s_mov_b64 exec, %0"
                : "=&s"(keep)
                : "s"(lds), "v"(voff), "s"(base)
-               : "memory", "vcc");
+               : "memory", "m0", "vcc");
 }
 
 __device__ __forceinline__ void dma16_if(const float *base, int voff, unsigned lds) {
@@ -118,7 +118,7 @@ __device__ __forceinline__ void dma16_if(const float *base, int voff, unsigned l
                "s_mov_b64 exec, %0"
                : "=&s"(keep)
                : "s"(lds), "v"(voff), "s"(base)
-               : "memory", "vcc");
+               : "memory", "m0", "vcc");
 }
 
 __device__ __forceinline__ const float *uniform(const float *p) {
