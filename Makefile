@@ -23,7 +23,7 @@ CFLAGS_HOST := -O2 -fPIC -std=c11 -Wall -Wextra -D__HIP_PLATFORM_AMD__ -I$(ROCM)
 HOST_SRCS := $(CSRC)/runtime.c $(CSRC)/tensor.c $(CSRC)/ops.c $(CSRC)/autograd.c $(CSRC)/dataset.c
 HIP_SRCS  := $(CSRC)/gemm.hip $(CSRC)/conv.hip $(CSRC)/elementwise.hip $(CSRC)/spatial.hip \
              $(CSRC)/head.hip $(CSRC)/conv_gen.hip $(CSRC)/attention.hip \
-             $(CSRC)/norm.hip $(CSRC)/rotary.hip $(CSRC)/distill.hip
+             $(CSRC)/norm.hip $(CSRC)/rotary.hip $(CSRC)/distill.hip $(CSRC)/embedding.hip $(CSRC)/muon.hip
 HDRS      := $(wildcard include/*.h) $(wildcard $(CSRC)/*.h)
 HOST_OBJS := $(patsubst $(CSRC)/%.c,$(BUILD)/obj/%.o,$(HOST_SRCS))
 HIP_OBJS  := $(patsubst $(CSRC)/%.hip,$(BUILD)/obj/%.o,$(HIP_SRCS))
@@ -42,9 +42,9 @@ $(BUILD)/obj/%.o: $(CSRC)/%.c $(HDRS) | $(BUILD)/obj
 $(BUILD)/obj/gemm.o: $(CSRC)/gemm.hip $(HDRS) | $(BUILD)/obj
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
-# direct convolution and attention: MFMA accumulators in VGPRs (the AGPR form made the
-# compiler copy accumulators between register files every loop iteration)
-$(BUILD)/obj/conv.o $(BUILD)/obj/conv_gen.o $(BUILD)/obj/attention.o: $(BUILD)/obj/%.o: $(CSRC)/%.hip $(HDRS) | $(BUILD)/obj
+# direct convolution, attention and Newton-Schulz steps: MFMA accumulators in VGPRs (the AGPR
+# form made the compiler copy accumulators between register files every loop iteration)
+$(BUILD)/obj/conv.o $(BUILD)/obj/conv_gen.o $(BUILD)/obj/attention.o $(BUILD)/obj/muon.o: $(BUILD)/obj/%.o: $(CSRC)/%.hip $(HDRS) | $(BUILD)/obj
 	$(HIPCC) $(HIPFLAGS) -ffp-contract=off -mllvm -amdgpu-mfma-vgpr-form=1 -c $< -o $@
 
 $(BUILD)/obj/%.o: $(CSRC)/%.hip $(HDRS) | $(BUILD)/obj

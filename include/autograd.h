@@ -93,6 +93,15 @@ AGNode *ag_rope(AGNode *x, const struct TTRope *r, int heads, const int *positio
  * (copied) or NULL. */
 AGNode *ag_attention(AGNode *q, AGNode *k, AGNode *v, const struct TTAttention *a);
 
+/* RMS norm over the last axis of x + residual (residual NULL: of x; w, as many
+ * elements as that axis, may be NULL).  With a residual of x's shape *sum gets the
+ * node of x + residual, owned by the caller (sum NULL: not handed out). */
+AGNode *ag_rmsnorm(AGNode *x, AGNode *residual, AGNode *w, float eps, AGNode **sum);
+
+/* Token embeddings: rows x cols, scale times the rows of the 2-D table w at ids, a
+ * host array of `rows` ints (copied).  Ids outside the table: rows of zeros. */
+AGNode *ag_embedding(AGNode *w, const int *ids, long rows, float scale);
+
 /* Distillation: the mean over the rows of 2-D logits of the loss against a
  * teacher's top logits (tt_k_distill); ids and teacher are host arrays of rows x
  * top values. */
@@ -121,11 +130,15 @@ int     ag_sgd_step_many(AGNode *const *leaves, int count, float lr);
  *                 m = b1*m + (1-b1)*g; v = b2*v + (1-b2)*g*g;
  *                 w -= lr_t*m/(sqrt(v)+eps)
  *                 (reference tests/gate_cifar_cnn.py:81-98)
- * Arithmetic matches NumPy's on float32 arrays with Python-float
+ *   muon:         tt_k_muon_multi (tt_hip.h) on shape[0] x the other axes of
+ *                 each parameter; a list with a parameter of one axis or of a
+ *                 single tensor twice is refused, nothing is updated
+ * Arithmetic of the first two matches NumPy's on float32 arrays with Python-float
  * hyperparameters.  Returns NULL / -1 on bad arguments or OOM. */
 typedef struct AGOptim AGOptim;
 AGOptim *ag_optim_sgd_momentum(double lr, double momentum);
 AGOptim *ag_optim_adam(double lr, double beta1, double beta2, double eps);
+AGOptim *ag_optim_muon(double lr, double momentum, int nesterov, double weight_decay);
 int      ag_optim_step(AGOptim *opt, AGNode *const *params, int count);
 long     ag_optim_steps(const AGOptim *opt);     /* Adam's t; -1 for NULL */
 /* learning-rate schedule: the CIFAR harness decays Adam's lr between epochs

@@ -449,7 +449,7 @@ int tt_k_conv2d_dx_lds(const float *g, const float *w, float *dx,
                        int sh, int sw, int ph, int pw, int Ho, int Wo);
 
 /* ---- transformer operators (norm.hip, rotary.hip, attention.hip,
- * distill.hip); no counterpart in the reference ----
+ * distill.hip, embedding.hip, muon.hip); no counterpart in the reference ----
  * `ws` arguments are device memory of the size the matching *_ws function
  * gives, used until the call's work is done, or NULL: taken from the caching
  * allocator for the call.  With a workspace of its own a call allocates
@@ -470,6 +470,63 @@ size_t tt_k_layernorm_bwd_ws(long rows, long cols);
 int tt_k_layernorm_bwd(const float *x, const float *w, const float *dy, const float *mean,
                        const float *rstd, float *dx, float *dw, float *db, long rows, long cols,
                        void *ws);
+
+/* RMS norm of s = x + residual over the last axis of rows x cols matrices:
+ *   y = s * rstd * w,  rstd = 1 / sqrt(mean(s^2) + eps)
+ * residual and w may be NULL (0 and 1); s goes to sum (what the next layer adds
+ * to) and rstd (rows floats) is written, unless NULL.  sum may be x or residual.
+ * A row whose sum of squares passes the type's range has rstd 0. */
+int tt_k_rmsnorm_fwd(const float *x, const float *residual, const float *w, float *y, float *sum,
+                     float *rstd, long rows, long cols, float eps);
+/* Its gradients from dy, from dsum (what reaches s past the norm; NULL: nothing),
+ * the forward's s (x where there was no residual) and rstd: dx, of x and of the
+ * residual alike, and dw = the sum over rows of dy * s * rstd; either may be
+ * NULL.  dx may be dsum.  The sums over rows have a fixed order. */
+size_t tt_k_rmsnorm_bwd_ws(long rows, long cols);
+int tt_k_rmsnorm_bwd(const float *s, const float *w, const float *dy, const float *dsum,
+                     const float *rstd, float *dx, float *dw, long rows, long cols, void *ws);
+
+/* Token embeddings: y[r] = scale * w[ids[r]] for a table w of vocab x cols, ids
+ * on the device.  A token outside [0, vocab) (padding) has a row of zeros and
+ * no gradient.  rows at most 2^28, vocab 2^30, cols 2^22. */
+int tt_k_embedding_fwd(const float *w, const int32_t *ids, float *y, long rows, long vocab,
+                       long cols, float scale);
+/* The table's gradient: dw[v] = scale * the sum of dy's rows whose token is v, in
+ * the order of the rows; accumulate != 0: added to dw, whose other rows are then
+ * not touched (0: they are cleared).  ws: 16-byte aligned. */
+size_t tt_k_embedding_bwd_ws(long rows, long vocab, long cols);
+int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows, long vocab,
+                       long cols, float scale, int accumulate, void *ws);
+
+/* Newton-Schulz steps towards the orthogonal factor of each of `count` matrices
+ * x (rows x cols, one behind the other): X = x / |x|_F (zeros: zeros), then
+ * `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X, which takes singular
+ * values s to a s + b s^3 + c s^5.  y may be x.  A matrix with an infinity or a
+ * NaN has NaN throughout.  Sides at most 2^20, rows * cols 2^32.  ws: 256-byte
+ * aligned; about 14 bytes a value of up to TT_SGD_MAX matrices, 20 of square
+ * ones. */
+#define TT_NS_A 3.4445f
+#define TT_NS_B (-4.7750f)
+#define TT_NS_C 2.0315f
+#define TT_NS_MAX_STEPS 64
+#define TT_MUON_MAX_SIDE (1L << 20)
+size_t tt_k_newton_schulz_ws(long count, long rows, long cols);
+int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps,
+                       void *ws);
+/* Muon, per matrix i (rows[i] x cols[i], count <= TT_SGD_MAX, one run of
+ * launches): the momentum's direction made orthogonal,
+ *   v = mu * v + g;  u = nesterov ? mu * v + g : v
+ *   w = (1 - lr * decay) * w - lr * TT_MUON_RMS * sqrt(max(rows, cols)) * X
+ * with X what TT_MUON_STEPS Newton-Schulz steps make of u.  A matrix of full rank
+ * then changes by about lr * TT_MUON_RMS a value whatever its shape and its
+ * gradient's size, as under Adam.  The matrices do not overlap (one that is there
+ * twice is refused). */
+#define TT_MUON_STEPS 5
+#define TT_MUON_RMS 0.2
+size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int count);
+int tt_k_muon_multi(float *const *w, const float *const *g, float *const *v, const long *rows,
+                    const long *cols, int count, float lr, float mu, int nesterov, float decay,
+                    void *ws);
 
 /* Rotary positions: in each head the pair j of the first rot_dim values turns
  * by the angle position * f_j, f_j = base^(-2j / rot_dim); the rest of the head

@@ -97,6 +97,8 @@ SIGNATURES = [
     ("ag_softmax_ce", VP, [VP, ctypes.POINTER(ctypes.c_int), _L]),
     ("ag_softmax_ce_probs", VP, [VP]),
     ("ag_layernorm", VP, [VP, VP, VP, _F]),
+    ("ag_rmsnorm", VP, [VP, VP, VP, _F, ctypes.POINTER(VP)]),
+    ("ag_embedding", VP, [VP, VP, _L, _F]),
     ("ag_rope", VP, [VP, _RP, _I, VP, _L]),
     ("ag_attention", VP, [VP, VP, VP, _AP]),
     ("ag_distill", VP, [VP, VP, VP, _I, _F]),
@@ -105,6 +107,7 @@ SIGNATURES = [
     ("ag_sgd_step_many", _I, [ctypes.POINTER(VP), _I, _F]),
     ("ag_optim_sgd_momentum", VP, [ctypes.c_double, ctypes.c_double]),
     ("ag_optim_adam", VP, [ctypes.c_double] * 4),
+    ("ag_optim_muon", VP, [_D, _D, _I, _D]),
     ("ag_optim_step", _I, [VP, ctypes.POINTER(VP), _I]),
     ("ag_optim_steps", _L, [VP]),
     ("ag_optim_release", None, [VP]),
@@ -213,6 +216,16 @@ SIGNATURES = [
     ("tt_k_layernorm_fwd", _I, [VP] * 6 + [_L, _L, _F]),
     ("tt_k_layernorm_bwd_ws", _SZ, [_L, _L]),
     ("tt_k_layernorm_bwd", _I, [VP] * 8 + [_L, _L, VP]),
+    ("tt_k_rmsnorm_fwd", _I, [VP] * 6 + [_L, _L, _F]),
+    ("tt_k_rmsnorm_bwd_ws", _SZ, [_L, _L]),
+    ("tt_k_rmsnorm_bwd", _I, [VP] * 7 + [_L, _L, VP]),
+    ("tt_k_embedding_fwd", _I, [VP] * 3 + [_L] * 3 + [_F]),
+    ("tt_k_embedding_bwd_ws", _SZ, [_L] * 3),
+    ("tt_k_embedding_bwd", _I, [VP] * 3 + [_L] * 3 + [_F, _I, VP]),
+    ("tt_k_newton_schulz_ws", _SZ, [_L] * 3),
+    ("tt_k_newton_schulz", _I, [VP, VP] + [_L] * 3 + [_I, VP]),
+    ("tt_k_muon_multi_ws", _SZ, [ctypes.POINTER(_L)] * 2 + [_I]),
+    ("tt_k_muon_multi", _I, [ctypes.POINTER(VP)] * 3 + [ctypes.POINTER(_L)] * 2 + [_I, _F, _F, _I, _F, VP]),
     ("tt_rope_frequencies", _I, [_RP, ctypes.POINTER(_D)]),
     ("tt_k_rope", _I, [_RP, VP, VP, VP, _L, _L, _I, _L, _L, _I]),
     ("tt_k_attention_fwd_ws", _SZ, [_AP]),

@@ -62,6 +62,8 @@ struct AGNode {
         struct { Tensor *sda[3]; int *stale; } mm;
         struct { Tensor *stat; int w, b; } ln;  /* mean | rstd of the rows; the inputs that w and
                                                    b are (0: none) */
+        struct { Tensor *rstd; } rms;           /* of the rows; NULL: no gradient needed */
+        struct { int32_t *ids; float scale; } embed;  /* device */
         struct { struct RopeState *s; } rope;
         struct { struct AttnState *s; } attn;
     } at;
@@ -103,6 +105,8 @@ static void backward_softmax_ce(AGNode *n);
 static void backward_layernorm(AGNode *n);
 static void backward_rope(AGNode *n);
 static void backward_attention(AGNode *n);
+static void backward_rmsnorm(AGNode *n);
+static void backward_embedding(AGNode *n);
 
 /* what a rotation and an attention keep for their backward rules */
 struct RopeState {
@@ -144,6 +148,8 @@ static void attn_free(struct AttnState *s) {
     tt_release(s->lse);
     free(s);
 }
+static void drop_rms(AGNode *n) { tt_release(n->at.rms.rstd); }
+static void drop_embed(AGNode *n) { ttrt_free(n->at.embed.ids); }
 static void drop_rope(AGNode *n) { rope_free(n->at.rope.s); }
 static void drop_attn(AGNode *n) { attn_free(n->at.attn.s); }
 static void drop_mm(AGNode *n) { spec_drop(n->at.mm.sda, &n->at.mm.stale); }
@@ -163,6 +169,8 @@ static const AGOp OP_AVGPOOL2D = {"avgpool2d", backward_avgpool, NULL};
 static const AGOp OP_SOFTMAX_CE = {"softmax_ce", backward_softmax_ce, drop_ce};
 static const AGOp OP_DISTILL = {"distill", backward_softmax_ce, drop_ce};
 static const AGOp OP_LAYERNORM = {"layernorm", backward_layernorm, drop_ln};
+static const AGOp OP_RMSNORM = {"rmsnorm", backward_rmsnorm, drop_rms};
+static const AGOp OP_EMBEDDING = {"embedding", backward_embedding, drop_embed};
 static const AGOp OP_ROPE = {"rope", backward_rope, drop_rope};
 static const AGOp OP_ATTENTION = {"attention", backward_attention, drop_attn};
 
@@ -836,6 +844,70 @@ AGNode *ag_layernorm(AGNode *x, AGNode *w, AGNode *b, float eps) {
     n->at.ln.stat = stat;
     n->at.ln.w = w ? 1 : 0;
     n->at.ln.b = b ? 1 + (w ? 1 : 0) : 0;
+    return n;
+}
+
+static int same_shape(const Tensor *a, const Tensor *b) {
+    if (a->ndim != b->ndim) return 0;
+    for (int i = 0; i < a->ndim; i++)
+        if (a->shape[i] != b->shape[i]) return 0;
+    return 1;
+}
+
+/* With a residual the sum is a node of its own, an addition; the norm's rule adds
+ * what it has for it to what has reached it past the norm in one pass. */
+AGNode *ag_rmsnorm(AGNode *x, AGNode *residual, AGNode *w, float eps, AGNode **sum) {
+    if (sum) *sum = NULL;
+    if (!x || x->val->ndim < 1 || !(eps >= 0.0f) || isinf(eps)) return NULL;
+    const Tensor *v = x->val;
+    const long cols = v->shape[v->ndim - 1], rows = v->numel / cols;
+    if ((w && w->val->numel != cols) || (residual && !same_shape(v, residual->val))) return NULL;
+    const float *xd = tt_dev(x->val), *rd = residual ? tt_dev(residual->val) : NULL,
+                *wd = w ? tt_dev(w->val) : NULL;
+    if (!xd || (residual && !rd) || (w && !wd)) return NULL;
+    const int grad = x->needs_grad || (residual && residual->needs_grad) || (w && w->needs_grad);
+    Tensor *out = tt_empty_like(v), *s = residual ? tt_empty_like(v) : NULL,
+           *rstd = grad ? tt_empty_dev(&rows, 1) : NULL;
+    if (!out || (residual && !s) || (grad && !rstd) ||
+        tt_k_rmsnorm_fwd(xd, rd, wd, out->dev, s ? s->dev : NULL, rstd ? rstd->dev : NULL, rows,
+                         cols, eps) != 0) {
+        tt_release(out);
+        tt_release(s);
+        tt_release(rstd);
+        return NULL;
+    }
+    AGNode *in = residual ? make_node(s, &OP_ADD, x, residual, NULL) : ag_retain(x);
+    if (!in) {
+        tt_release(out);
+        tt_release(rstd);
+        return NULL;
+    }
+    AGNode *n = make_node(out, &OP_RMSNORM, in, w, NULL);
+    if (n) n->at.rms.rstd = rstd;
+    else tt_release(rstd);
+    if (n && residual && sum) *sum = in;
+    else ag_release(in);
+    return n;
+}
+
+AGNode *ag_embedding(AGNode *w, const int *ids, long rows, float scale) {
+    if (!w || !ids || rows <= 0 || w->val->ndim != 2) return NULL;
+    const long vocab = w->val->shape[0], shape[2] = {rows, w->val->shape[1]};
+    const float *wd = tt_dev(w->val);
+    if (!wd || rows > (long)(PTRDIFF_MAX / 4) / shape[1]) return NULL;
+    const size_t bytes = sizeof(int32_t) * (size_t)rows;
+    Tensor *out = tt_empty_dev(shape, 2);
+    int32_t *di = out ? (int32_t *)ttrt_alloc(bytes) : NULL;
+    if (!di || ttrt_h2d_async(di, ids, bytes) != 0 ||
+        tt_k_embedding_fwd(wd, di, out->dev, rows, vocab, shape[1], scale) != 0) {
+        ttrt_free(di);
+        tt_release(out);
+        return NULL;
+    }
+    AGNode *n = make_node(out, &OP_EMBEDDING, w, NULL, NULL);
+    if (!n) { ttrt_free(di); return NULL; }
+    n->at.embed.ids = di;
+    n->at.embed.scale = scale;
     return n;
 }
 
@@ -1712,6 +1784,56 @@ static void backward_layernorm(AGNode *n) {
     accum_move(b, db);
 }
 
+static void backward_rmsnorm(AGNode *n) {
+    AGNode *x = n->in[0], *w = n->n_in > 1 ? n->in[1] : NULL;
+    if (!n->at.rms.rstd) return;
+    const Tensor *v = x->val;
+    const long cols = v->shape[v->ndim - 1], rows = v->numel / cols;
+    const float *g = tt_dev(n->grad), *xd = tt_dev(x->val), *wd = w ? tt_dev(w->val) : NULL,
+                *st = tt_dev(n->at.rms.rstd);
+    if (!g || !xd || !st || (w && !wd)) return;
+    /* what has reached x already is added in the same pass, in place */
+    float *have = NULL;
+    if (needs(x) && x->grad) {
+        tt_lazy_before_write(x->grad);
+        if (!(have = tt_dev(x->grad))) return;
+    }
+    Tensor *dx = needs(x) && !have ? tt_empty_like(v) : NULL;
+    Tensor *dw = needs(w) ? tt_empty_like(w->val) : NULL;
+    if ((needs(x) && !have && !dx) || (needs(w) && !dw) ||
+        tt_k_rmsnorm_bwd(xd, wd, g, have, st, have ? have : dx ? dx->dev : NULL,
+                         dw ? dw->dev : NULL, rows, cols, NULL) != 0) {
+        tt_release(dx);
+        tt_release(dw);
+        return;
+    }
+    if (have) tt_mark_dev_written(x->grad);
+    accum_move(x, dx);
+    accum_move(w, dw);
+}
+
+/* only the rows of the batch's tokens are added to a gradient that is there */
+static void backward_embedding(AGNode *n) {
+    AGNode *w = n->in[0];
+    const float *g = needs(w) ? tt_dev(n->grad) : NULL;
+    if (!g) return;
+    const long rows = n->val->shape[0], vocab = w->val->shape[0], cols = w->val->shape[1];
+    if (w->grad) {
+        tt_lazy_before_write(w->grad);
+        float *have = tt_dev(w->grad);
+        if (have && tt_k_embedding_bwd(n->at.embed.ids, g, have, rows, vocab, cols,
+                                       n->at.embed.scale, 1, NULL) == 0)
+            tt_mark_dev_written(w->grad);
+        return;
+    }
+    Tensor *dw = tt_empty_like(w->val);
+    if (dw && tt_k_embedding_bwd(n->at.embed.ids, g, dw->dev, rows, vocab, cols, n->at.embed.scale,
+                                 0, NULL) == 0)
+        accum_move(w, dw);
+    else
+        tt_release(dw);
+}
+
 static void backward_rope(AGNode *n) {
     AGNode *x = n->in[0];
     const struct RopeState *s = n->at.rope.s;
@@ -1906,11 +2028,12 @@ int ag_sgd_step(AGNode *leaf, float lr) {
  * because the reference harness keeps them as Python floats: the fp32
  * factors are the doubles rounded once, as NumPy rounds a Python scalar
  * against a float32 array, and Adam's bias-corrected rate stays a double. */
-enum { OPT_MOMENTUM = 1, OPT_ADAM = 2 };
+enum { OPT_MOMENTUM = 1, OPT_ADAM = 2, OPT_MUON = 3 };
 
 struct AGOptim {
     int kind;
-    double lr, mu, b1, b2, eps;
+    double lr, mu, b1, b2, eps, decay;
+    int nesterov;
     long t;            /* Adam steps taken */
     int nslots;        /* fixed by the first step */
     long *numel;       /* per slot */
@@ -1941,6 +2064,36 @@ AGOptim *ag_optim_adam(double lr, double beta1, double beta2, double eps) {
     o->b2 = beta2;
     o->eps = eps;
     return o;
+}
+
+AGOptim *ag_optim_muon(double lr, double momentum, int nesterov, double weight_decay) {
+    if (!isfinite(lr) || !isfinite(momentum) || !isfinite(weight_decay)) return NULL;
+    AGOptim *o = optim_new(OPT_MUON);
+    if (!o) return NULL;
+    o->lr = lr;
+    o->mu = momentum;
+    o->nesterov = nesterov ? 1 : 0;
+    o->decay = weight_decay;
+    return o;
+}
+
+/* a parameter as a matrix: its first axis by the others */
+static void sides(const Tensor *t, long *rows, long *cols) {
+    *rows = t->shape[0];
+    *cols = t->numel / t->shape[0];
+}
+
+/* whether Muon can step these: matrices, of which none is there twice */
+static int muon_takes(AGNode *const *params, int count) {
+    for (int i = 0; i < count; i++) {
+        long rows, cols;
+        if (!params[i] || params[i]->val->ndim < 2) return 0;
+        sides(params[i]->val, &rows, &cols);
+        if (!tt_k_muon_multi_ws(&rows, &cols, 1)) return 0;
+        for (int j = 0; j < i; j++)
+            if (params[j]->val == params[i]->val) return 0;
+    }
+    return 1;
 }
 
 void ag_optim_release(AGOptim *o) {
@@ -1989,6 +2142,7 @@ static int optim_bind(AGOptim *o, AGNode *const *params, int count) {
 
 int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
     if (!o || count < 0 || (count > 0 && !params)) return -1;
+    if (o->kind == OPT_MUON && !muon_takes(params, count)) return -1;
     if (o->nslots == 0 && count > 0) {
         if (optim_bind(o, params, count)) {
             for (int i = 0; i < o->nslots; i++) {
@@ -2013,7 +2167,7 @@ int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
     for (int base = 0; base < count; base += TT_SGD_MAX) {
         float *w[TT_SGD_MAX], *m[TT_SGD_MAX], *v[TT_SGD_MAX];
         const float *g[TT_SGD_MAX];
-        long n[TT_SGD_MAX];
+        long n[TT_SGD_MAX], rows[TT_SGD_MAX], cols[TT_SGD_MAX];
         int k = 0;
         for (int i = base; i < count && i < base + TT_SGD_MAX; i++)
             if (params[i]->grad) tt_lazy_before_write(params[i]->val);
@@ -2026,12 +2180,16 @@ int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
             m[k] = o->m[i];
             v[k] = o->v[i];
             n[k] = o->numel[i];
+            sides(l->val, &rows[k], &cols[k]);
             tt_mark_dev_written(l->val);
             k++;
         }
         int rc;
         if (o->kind == OPT_MOMENTUM)
             rc = tt_k_momentum_multi(w, g, m, n, k, (float)o->lr, (float)o->mu);
+        else if (o->kind == OPT_MUON)
+            rc = tt_k_muon_multi(w, g, m, rows, cols, k, (float)o->lr, (float)o->mu, o->nesterov,
+                                 (float)o->decay, NULL);
         else
             rc = tt_k_adam_multi(w, g, m, v, n, k, (float)o->b1, (float)(1.0 - o->b1),
                                  (float)o->b2, (float)(1.0 - o->b2), (float)o->eps, lr_t);

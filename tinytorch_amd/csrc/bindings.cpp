@@ -8,9 +8,9 @@
 // fresh NumPy copies of the device data, as the reference's do; with
 // copy=False they return a view of the pinned host mirror instead.
 // detach() re-enters a device-resident parameter into a new graph.  Additions of this backend:
-// softmax_ce(labels), probs(), layernorm(w, b), rope(heads, head_dim, ...), attention(k, v, ...),
-// distill(ids, teacher), backward_device(seed_node), sgd_step(lr), the
-// Optim class (SGD-momentum, Adam), the Dataset class (device-resident
+// softmax_ce(labels), probs(), layernorm(w, b), rmsnorm(w, residual), embedding(ids, scale),
+// rope(heads, head_dim, ...), attention(k, v, ...), distill(ids, teacher), sgd_step(lr), the
+// Optim class (SGD-momentum, Adam, Muon), the Dataset class (device-resident
 // MNIST / CIFAR-10) and the module function available().
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
@@ -146,6 +146,15 @@ class PyNode {
   PyNode layernorm(py::object w, py::object b, float eps) {
     return PyNode(ag_layernorm(get(), opt(w), opt(b), eps));
   }
+  py::object rmsnorm(py::object w, py::object residual, float eps) {
+    AGNode *sum = nullptr;
+    PyNode y(ag_rmsnorm(get(), opt(residual), opt(w), eps, &sum));
+    if (residual.is_none()) return py::cast(y);
+    return py::make_tuple(y, PyNode(sum));
+  }
+  PyNode embedding(IntArr ids, float scale) {
+    return PyNode(ag_embedding(get(), ids.data(), (long)ids.size(), scale));
+  }
   PyNode rope(int heads, int head_dim, py::object positions, long seq_len, py::object rot_dim, bool interleaved,
               double base, int scaling, double factor, double trained, double low, double high,
               double magnitude) {
@@ -215,6 +224,9 @@ class PyOptim {
   }
   static PyOptim adam(double lr, double b1, double b2, double eps) {
     return PyOptim(ag_optim_adam(lr, b1, b2, eps));
+  }
+  static PyOptim muon(double lr, double momentum, bool nesterov, double weight_decay) {
+    return PyOptim(ag_optim_muon(lr, momentum, nesterov, weight_decay));
   }
   void step(const std::vector<PyNode> &params) {
     std::vector<AGNode *> ps;
@@ -300,6 +312,9 @@ PYBIND11_MODULE(tinytorch_pybind, m) {
       .def("softmax_ce", &PyNode::softmax_ce, py::arg("labels"))
       .def("layernorm", &PyNode::layernorm, py::arg("w") = py::none(), py::arg("b") = py::none(),
            py::arg("eps") = 1e-5f)
+      .def("rmsnorm", &PyNode::rmsnorm, py::arg("w") = py::none(), py::arg("residual") = py::none(),
+           py::arg("eps") = 1e-5f)
+      .def("embedding", &PyNode::embedding, py::arg("ids"), py::arg("scale") = 1.0f)
       .def("rope", &PyNode::rope, py::arg("heads"), py::arg("head_dim"), py::arg("positions") = py::none(),
            py::arg("seq_len") = 0, py::arg("rot_dim") = py::none(), py::arg("interleaved") = false,
            py::arg("base") = 10000.0, py::arg("scaling") = 0, py::arg("factor") = 1.0,
@@ -329,6 +344,8 @@ PYBIND11_MODULE(tinytorch_pybind, m) {
       .def_static("sgd_momentum", &PyOptim::sgd_momentum, py::arg("lr"), py::arg("momentum"))
       .def_static("adam", &PyOptim::adam, py::arg("lr") = 0.003, py::arg("beta1") = 0.9,
                   py::arg("beta2") = 0.999, py::arg("eps") = 1e-8)
+      .def_static("muon", &PyOptim::muon, py::arg("lr") = 0.02, py::arg("momentum") = 0.95,
+                  py::arg("nesterov") = true, py::arg("weight_decay") = 0.0)
       .def("step", &PyOptim::step, py::arg("params"))
       .def_property_readonly("t", &PyOptim::steps)
       .def_property("lr", &PyOptim::lr, &PyOptim::set_lr);

@@ -1,0 +1,430 @@
+// Newton-Schulz steps towards the orthogonal factor of matrices, and the step of
+// the optimizer that goes along it (Muon).
+//
+//   X = U / |U|_F, along the shorter side m (U^T where there are more rows), then
+//   P = X X^T,  Q = b P + c P P,  X <- a X + Q X      (a, b, c: TT_NS_*)
+//
+// which keeps the singular vectors and moves every singular value s to
+// a s + b s^3 + c s^5: after five steps those from about 0.003 on lie within
+// [0.68, 1.21].  P and P P are symmetric: half of their tiles are computed.
+//
+// The products take fp32 results from the fp16 matrix units, which are 16 times as
+// fast as the fp32 ones: a value times 2^14 is h + l, two fp16 numbers (l what h
+// leaves), 22 bits, and h h' + h l' + l h' has all of the product but l l', 2^-22
+// of it.  That is what fp32 sums of these lengths leave too: against 64 bits both
+// are off by 1e-6 to 9e-6 (what the steps make of the first rounding).  2^14
+// keeps both in the type's range: s stays under 1.21, so the values of X, P and Q
+// are within 1.21, 1.46 and 2.81 (46100 of 65504 times 2^14), and l is exact to
+// 2^-38.
+//
+// X, X^T, P and Q are kept as images: rows of blocks of 32 values, a block the 32
+// h and then the 32 l, 128 bytes, with zeros behind the last value.  Both operands
+// of a product are read along rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include "tt_rt.h"
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+
+inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
+inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
+
+constexpr float UP = 16384.f, DOWN2 = 1.f / (16384.f * 16384.f);
+constexpr int MOST = TT_SGD_MAX;   // matrices in one run of launches
+constexpr int NORM_PARTS = 1024;   // sums of squares of a matrix
+
+struct Matrix {
+  const float *g;   // what is orthogonalised, or the gradient (rows x cols)
+  float *v, *w;     // momenta and weights; v NULL: the result goes to w
+  char *x, *t[2];   // images of X (m rows), X^T (n rows; the steps write one from the other)
+  char *p, *q;      // of P and Q
+  double *norm;     // NORM_PARTS partial sums of squares
+  float keep, rate; // w = keep w + rate X
+  int m, n;         // shorter and longer side
+  int turned;       // more rows than columns: X is U^T
+  int parts;        // of the norm
+};
+struct Matrices {
+  Matrix at[MOST];
+  unsigned first[MOST + 1];  // matrix i has the workgroups [first[i], first[i + 1])
+  int count;
+};
+
+__host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
+
+// which matrix a workgroup belongs to; b becomes its number among that one's
+__device__ __forceinline__ int matrix_of(const Matrices &a, unsigned &b) {
+  int i = 0;
+  while (i + 1 < a.count && b >= a.first[i + 1]) i++;
+  b -= a.first[i];
+  return i;
+}
+
+// x 2^14 in two parts
+__device__ __forceinline__ void split(float y, _Float16 &h, _Float16 &l) {
+  h = (_Float16)y;
+  l = (_Float16)(y - (float)h);
+}
+__device__ __forceinline__ _Float16 *place(char *image, long blocks, long r, long c) {
+  return (_Float16 *)(image + (r * blocks + (c >> 5)) * 128) + (c & 31);
+}
+
+// ---------------------------------------------------------------- before the steps
+
+// v = mu v + g, and the sum of squares of u = g + mu v (nesterov) or v; without
+// momenta of g.  In 64 bits: the squares of any fp32 values are within its range.
+__global__ void __launch_bounds__(256) momentum_kernel(Matrices a, float mu, int nesterov) {
+  __shared__ double sums[4];
+  unsigned b = blockIdx.x;
+  const Matrix &M = a.at[matrix_of(a, b)];
+  const long count = (long)M.m * M.n;
+  double s = 0.0;
+  for (long i = ((long)b * 256 + threadIdx.x) * 4; i < count; i += (long)M.parts * 1024) {
+    if (i + 4 <= count) {
+      f32x4 u = *(const f32x4_any *)(M.g + i);
+      if (M.v) {
+        const f32x4 v = *(const f32x4_any *)(M.v + i) * mu + u;
+        *(f32x4_any *)(M.v + i) = v;
+        u = nesterov ? v * mu + u : v;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) s = fma((double)u[j], (double)u[j], s);
+    } else {
+      for (long j = i; j < count; j++) {
+        float u = M.g[j];
+        if (M.v) {
+          const float v = M.v[j] * mu + u;
+          M.v[j] = v;
+          u = nesterov ? v * mu + u : v;
+        }
+        s = fma((double)u, (double)u, s);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) M.norm[b] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+// The images of U / |U|_F and its transpose, a tile of 64 x 64 at a time through
+// LDS; both are written along their rows.
+__global__ void __launch_bounds__(256) image_kernel(Matrices a, float mu, int nesterov) {
+  __shared__ double sums[4];
+  __shared__ float tile[64][65];
+  unsigned b = blockIdx.x;
+  const Matrix &M = a.at[matrix_of(a, b)];
+  const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < M.parts; i += 256) s += M.norm[i];
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  const double scale = s == 0.0 ? 0.0 : (double)UP / sqrt(s);  // zeros stay zeros
+  const unsigned across = (unsigned)((cols + 63) / 64);
+  const long r0 = (long)(b / across) * 64, c0 = (long)(b % across) * 64;
+#pragma unroll 4
+  for (int k = 0; k < 16; k++) {
+    const long r = r0 + k * 4 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63);
+    float u = 0.f;
+    if (r < rows && c < cols) {
+      u = M.g[r * cols + c];
+      if (M.v) {
+        const float v = M.v[r * cols + c];
+        u = nesterov ? v * mu + u : v;
+      }
+    }
+    tile[k * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)u * scale);
+  }
+  __syncthreads();
+  char *along = M.turned ? M.t[0] : M.x, *down = M.turned ? M.x : M.t[0];
+  const long row_blocks = blocks_of(cols), col_blocks = blocks_of(rows);
+#pragma unroll 4
+  for (int k = 0; k < 16; k++) {
+    const int i = k * 4 + (threadIdx.x >> 6), j = threadIdx.x & 63;
+    _Float16 h, l;
+    if (r0 + i < rows && c0 + j < row_blocks * 32) {
+      split(tile[i][j], h, l);
+      _Float16 *p = place(along, row_blocks, r0 + i, c0 + j);
+      p[0] = h;
+      p[32] = l;
+    }
+    if (c0 + i < cols && r0 + j < col_blocks * 32) {
+      split(tile[j][i], h, l);
+      _Float16 *p = place(down, col_blocks, c0 + i, r0 + j);
+      p[0] = h;
+      p[32] = l;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- products
+
+enum { GRAM, SQUARE, STEP, LAST };  // P = X X^T; Q = b P + c P P; X <- a X + Q X; the same, to w
+
+// Tile `b` of a symmetric matrix: those of the lower triangle row by row.
+__device__ __forceinline__ void triangle(unsigned b, int &i, int &j) {
+  int r = (int)((sqrt(8.0 * b + 1.0) - 1.0) * 0.5);
+  while ((unsigned)r * (r + 1u) / 2 > b) r--;
+  while ((unsigned)(r + 1) * (r + 2u) / 2 <= b) r++;
+  i = r;
+  j = (int)(b - (unsigned)r * (r + 1u) / 2);
+}
+
+template <int KIND>
+struct Operands {
+  const char *a, *b;    // images whose rows are multiplied
+  const char *add;      // image of the matrix added, times `times` (GRAM: none)
+  char *out, *down;     // images of the result and its transpose
+  int rows, cols, k;    // of the result; the products' length
+  float by, times;
+  __device__ __forceinline__ Operands(const Matrix &M, int step) {
+    if (KIND == GRAM) {
+      a = b = M.x, add = nullptr, out = down = M.p;
+      rows = cols = M.m, k = M.n, by = 1.f, times = 0.f;
+    } else if (KIND == SQUARE) {
+      a = b = add = M.p, out = down = M.q;
+      rows = cols = k = M.m, by = TT_NS_C, times = TT_NS_B;
+    } else {
+      a = M.q, b = M.t[step & 1], add = M.x, out = M.x, down = M.t[~step & 1];
+      rows = k = M.m, cols = M.n, by = 1.f, times = TT_NS_A;
+    }
+  }
+};
+
+// Tiles of 32 x 32, one a workgroup, the operands read from memory as the matrix
+// instructions take them and each wave with a share of the products' length:
+// eight sums, joined in LDS.
+template <int KIND>
+__global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
+  constexpr int WAVES = 8;
+  __shared__ float sums[WAVES][32][33];
+  unsigned t = blockIdx.x;
+  const Matrix &M = a.at[matrix_of(a, t)];
+  const Operands<KIND> o(M, step);
+  int ti, tj;
+  if (KIND <= SQUARE) {
+    triangle(t, ti, tj);
+  } else {
+    const unsigned across = (unsigned)blocks_of(o.cols);
+    ti = (int)(t / across), tj = (int)(t % across);
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long blocks = blocks_of(o.k);
+  // a row behind the last is the last once more: its results are not written
+  const int ra = ti * 32 + (lane & 31), rb = tj * 32 + (lane & 31);
+  const char *pa = o.a + (ra < o.rows ? ra : o.rows - 1) * blocks * 128 + (lane >> 5) * 16;
+  const char *pb = o.b + (rb < o.cols ? rb : o.cols - 1) * blocks * 128 + (lane >> 5) * 16;
+  f32x16 acc = {};
+#pragma unroll 2
+  for (long k = wave; k < blocks; k += WAVES) {
+    half8 ha[2], la[2], hb[2], lb[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      ha[s] = *(const half8 *)(pa + k * 128 + s * 32);
+      la[s] = *(const half8 *)(pa + k * 128 + s * 32 + 64);
+      hb[s] = *(const half8 *)(pb + k * 128 + s * 32);
+      lb[s] = *(const half8 *)(pb + k * 128 + s * 32 + 64);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(la[s], hb[s], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[s], lb[s], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[s], hb[s], acc, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++) sums[wave][8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
+  __syncthreads();
+  const int r = threadIdx.x >> 5, c = threadIdx.x & 31;  // and row r + 16
+  float v[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int i = r + e * 16, row = ti * 32 + i, col = tj * 32 + c;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) s += sums[w][i][c];
+    s *= o.by * DOWN2;
+    if (KIND != GRAM && row < o.rows && col < o.cols) {
+      const _Float16 *p = place((char *)o.add, blocks_of(o.cols), row, col);
+      s += o.times * (1.f / UP) * ((float)p[0] + (float)p[32]);
+    }
+    v[e] = s;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int i = r + e * 16, row = ti * 32 + i, col = tj * 32 + c;
+    const bool in = row < o.rows && col < o.cols;
+    if (KIND == LAST) {
+      if (in && !M.turned) {
+        float *w = M.w + (long)row * o.cols + col;
+        *w = M.v ? M.keep * *w + M.rate * v[e] : v[e];
+      }
+    } else if (row < o.rows) {
+      _Float16 h, l;
+      split(in ? v[e] * UP : 0.f, h, l);
+      _Float16 *p = place(o.out, blocks_of(o.cols), row, col);
+      p[0] = h;
+      p[32] = l;
+    }
+    sums[0][i][c] = in ? v[e] : 0.f;
+  }
+  if ((KIND <= SQUARE && ti == tj) || (KIND == LAST && !M.turned)) return;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; e++) {  // the transpose
+    const int i = r + e * 16, row = ti * 32 + c, col = tj * 32 + i;
+    if (col >= o.cols) continue;
+    if (KIND == LAST) {
+      if (row < o.rows) {
+        float *w = M.w + (long)col * o.rows + row;
+        *w = M.v ? M.keep * *w + M.rate * sums[0][c][i] : sums[0][c][i];
+      }
+    } else {
+      _Float16 h, l;
+      split(sums[0][c][i] * UP, h, l);
+      _Float16 *p = place(o.down, blocks_of(o.rows), col, row);
+      p[0] = h;
+      p[32] = l;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+bool good_sides(long rows, long cols) {
+  return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= 1L << 32;
+}
+
+size_t ws_of(long rows, long cols) {
+  const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return up((size_t)m * blocks_of((int)n) * 128) + 2 * up((size_t)n * blocks_of((int)m) * 128) +
+         2 * up((size_t)m * blocks_of((int)m) * 128) + up(sizeof(double) * NORM_PARTS);
+}
+
+void lay(Matrix &M, long rows, long cols, char *&ws) {
+  M.turned = rows > cols;
+  M.m = (int)(M.turned ? cols : rows);
+  M.n = (int)(M.turned ? rows : cols);
+  const long parts = ((long)M.m * M.n + 8191) / 8192;
+  M.parts = (int)(parts < NORM_PARTS ? parts : NORM_PARTS);
+  auto take = [&](size_t bytes) {
+    char *p = ws;
+    ws += up(bytes);
+    return p;
+  };
+  M.x = take((size_t)M.m * blocks_of(M.n) * 128);
+  for (int i = 0; i < 2; i++) M.t[i] = take((size_t)M.n * blocks_of(M.m) * 128);
+  M.p = take((size_t)M.m * blocks_of(M.m) * 128);
+  M.q = take((size_t)M.m * blocks_of(M.m) * 128);
+  M.norm = (double *)take(sizeof(double) * NORM_PARTS);
+}
+
+template <class F>
+unsigned number(Matrices &a, F workgroups) {
+  unsigned long at = 0;
+  for (int i = 0; i < a.count; i++) {
+    a.first[i] = (unsigned)at;
+    at += (unsigned long)workgroups(a.at[i]);
+  }
+  a.first[a.count] = (unsigned)at;
+  return (unsigned)at;
+}
+
+void run(Matrices &a, int steps, float mu, int nesterov) {
+  unsigned grid = number(a, [](const Matrix &M) { return (long)M.parts; });
+  hipLaunchKernelGGL(momentum_kernel, dim3(grid), dim3(256), 0, stream(), a, mu, nesterov);
+  grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
+  hipLaunchKernelGGL(image_kernel, dim3(grid), dim3(256), 0, stream(), a, mu, nesterov);
+  Matrices half = a;
+  const unsigned lower = number(half, [](const Matrix &M) { return blocks_of(M.m) * (blocks_of(M.m) + 1) / 2; });
+  const unsigned all = number(a, [](const Matrix &M) { return blocks_of(M.m) * blocks_of(M.n); });
+  for (int s = 0; s < steps; s++) {
+    hipLaunchKernelGGL(small_kernel<GRAM>, dim3(lower), dim3(512), 0, stream(), half, s);
+    hipLaunchKernelGGL(small_kernel<SQUARE>, dim3(lower), dim3(512), 0, stream(), half, s);
+    if (s + 1 < steps) hipLaunchKernelGGL(small_kernel<STEP>, dim3(all), dim3(512), 0, stream(), a, s);
+    else hipLaunchKernelGGL(small_kernel<LAST>, dim3(all), dim3(512), 0, stream(), a, s);
+  }
+}
+
+}  // namespace
+
+extern "C" size_t tt_k_newton_schulz_ws(long count, long rows, long cols) {
+  if (count <= 0 || !good_sides(rows, cols)) return 0;
+  return (size_t)(count < MOST ? count : MOST) * ws_of(rows, cols);
+}
+
+extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps, void *ws) {
+  if (!x || !y || count <= 0 || !good_sides(rows, cols) || count > (1L << 40) / (rows * cols) || steps < 1 ||
+      steps > TT_NS_MAX_STEPS)
+    return -1;
+  if (ttrt_init() != 0) return -3;
+  void *own = NULL;
+  if (!ws) ws = own = ttrt_alloc(tt_k_newton_schulz_ws(count, rows, cols));
+  if (!ws) return -2;
+  for (long base = 0; base < count; base += MOST) {
+    Matrices a = {};
+    a.count = (int)(count - base < MOST ? count - base : MOST);
+    char *at = (char *)ws;
+    for (int i = 0; i < a.count; i++) {
+      a.at[i].g = x + (base + i) * rows * cols;
+      a.at[i].w = y + (base + i) * rows * cols;
+      lay(a.at[i], rows, cols, at);
+    }
+    run(a, steps, 0.f, 0);
+  }
+  ttrt_free(own);
+  return launched();
+}
+
+extern "C" size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int count) {
+  if (!rows || !cols || count < 1 || count > TT_SGD_MAX) return 0;
+  size_t bytes = 0;
+  for (int i = 0; i < count; i++) {
+    if (!good_sides(rows[i], cols[i])) return 0;
+    bytes += ws_of(rows[i], cols[i]);
+  }
+  return bytes;
+}
+
+extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *const *v, const long *rows,
+                               const long *cols, int count, float lr, float mu, int nesterov, float decay, void *ws) {
+  if (!w || !g || !v || !rows || !cols || count < 0 || count > TT_SGD_MAX || !isfinite(lr) || !isfinite(mu) ||
+      !isfinite(decay))
+    return -1;
+  for (int i = 0; i < count; i++) {
+    if (!w[i] || !g[i] || !v[i] || !good_sides(rows[i], cols[i])) return -1;
+    for (int j = 0; j < i; j++)
+      if (w[j] == w[i] || v[j] == v[i]) return -1;
+  }
+  if (count == 0) return 0;
+  if (ttrt_init() != 0) return -3;
+  void *own = NULL;
+  if (!ws) ws = own = ttrt_alloc(tt_k_muon_multi_ws(rows, cols, count));
+  if (!ws) return -2;
+  Matrices a = {};
+  a.count = count;
+  char *at = (char *)ws;
+  for (int i = 0; i < count; i++) {
+    Matrix &M = a.at[i];
+    M.g = g[i], M.v = v[i], M.w = w[i];
+    M.keep = (float)(1.0 - (double)lr * decay);
+    M.rate = (float)(-(double)lr * TT_MUON_RMS * sqrt((double)(rows[i] > cols[i] ? rows[i] : cols[i])));
+    lay(M, rows[i], cols[i], at);
+  }
+  run(a, TT_MUON_STEPS, mu, nesterov);
+  ttrt_free(own);
+  return launched();
+}

@@ -1,9 +1,15 @@
-// Layer norm over the last axis, forward and backward (HBM roofline: the
-// forward pass reads x and writes y, the backward pass reads x and dy and
-// writes dx).
+// Layer norm and RMS norm over the last axis, forward and backward (HBM
+// roofline: each value of the inputs is read once, each of the outputs written
+// once).  Layer norm:
 //
 //   y = h w + b, h = (x - mean) rstd;  with g = dy w over a row of C values
 //   dx = rstd (g - mean(g) - h mean(g h));  dw = sum_rows dy h, db = sum_rows dy
+//
+// RMS norm of s = x + residual (both written: s is the next residual):
+//
+//   y = n w, n = s rstd, rstd = 1 / sqrt(mean(s^2) + eps);  with g = dy w
+//   dx = ds + rstd (g - n mean(g n)), ds the gradient that s has from elsewhere,
+//   and the residual's gradient is the same;  dw = sum_rows dy n
 //
 // A row is held in registers by the NT threads that share it, so memory sees
 // each value once and the variance is that of the deviations (two sums over
@@ -221,12 +227,13 @@ __global__ void __launch_bounds__(threads_of(NT))
   }
 }
 
-// dw / db from the workgroups' sums: 16 columns a workgroup, 64 threads a
-// column, each every 64th of them, then in a fixed tree.  Latency-bound (4 MB
-// at 1024 columns): a thread's reads do not wait for each other.
+// dw / db from the workgroups' SUMS sums a column: 16 columns a workgroup, 64
+// threads a column, each every 64th of them, then in a fixed tree.  Latency-bound
+// (4 MB at 1024 columns and two sums): a thread's reads do not wait for each other.
+template <int SUMS>
 __global__ void __launch_bounds__(1024)
-    ln_join_kernel(const float *__restrict__ part, float *__restrict__ dw, float *__restrict__ db, int blocks,
-                   long cols) {
+    join_kernel(const float *__restrict__ part, float *__restrict__ dw, float *__restrict__ db, int blocks,
+                long cols) {
   __shared__ float sum[16][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float *out = blockIdx.y ? db : dw;
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(1024)
     float s = 0.f;
     if (c < cols) {
 #pragma unroll 8
-      for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += part[((long)k * 2 + blockIdx.y) * cols + c];
+      for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += part[((long)k * SUMS + blockIdx.y) * cols + c];
     }
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
@@ -316,6 +323,168 @@ __global__ void __launch_bounds__(256)
   }
   part[((long)blockIdx.y * 2) * cols + c] = sw;
   part[((long)blockIdx.y * 2 + 1) * cols + c] = sb;
+}
+
+// s = x + res (res may be NULL), written to sum unless NULL, and its RMS norm.
+// sum may be res or x: a thread reads its own columns before it writes them, and
+// of another's it keeps nothing.
+template <int NT, int NV, bool TAIL>
+__global__ void __launch_bounds__(threads_of(NT))
+    rms_fwd_kernel(const float *x, const float *res, const float *__restrict__ w, float *__restrict__ y, float *sum,
+                   float *__restrict__ rstd, long rows, int cols, float eps) {
+  constexpr int RB = threads_of(NT) / NT;
+  __shared__ float part[NT / 64][2];
+  const int t = threadIdx.x % NT, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const Groups<NT, NV, TAIL> gr(cols, t);
+  f32x4 g[NV];
+  if (w) gr.load(g, w);
+  for (long row = (long)blockIdx.x * RB + sub; row < rows; row += (long)gridDim.x * RB) {
+    f32x4 v[NV];
+    gr.load(v, x + row * cols);
+    if (res) {
+      f32x4 u[NV];
+      gr.load(u, res + row * cols);
+#pragma unroll
+      for (int n = 0; n < NV; n++) v[n] += u[n];
+    }
+    gr.mask(v);
+    float q = 0.f, z = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) q = fmaf(v[n][j], v[n][j], q);
+    row_sum2<NT>(q, z, part);
+    const float r = 1.f / sqrtf(q / (float)cols + eps);
+    if (sum) gr.store(v, sum + row * cols);
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[n][j] *= r;
+        if (w) v[n][j] *= g[n][j];
+      }
+    gr.store(v, y + row * cols);
+    if (t == 0 && rstd) rstd[row] = r;
+  }
+}
+
+// dx (which may be ds), and (part) this workgroup's sums over its rows for dw:
+// part[block][cols]
+template <int NT, int NV, bool TAIL>
+__global__ void __launch_bounds__(threads_of(NT))
+    rms_bwd_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ dy,
+                   const float *ds, const float *__restrict__ rstd, float *dx, float *__restrict__ part, long rows,
+                   int cols) {
+  constexpr int RB = threads_of(NT) / NT;
+  __shared__ float red[NT / 64][2];
+  __shared__ __attribute__((aligned(16))) float join[RB > 1 ? RB * NT * 4 : 4];
+  const int t = threadIdx.x % NT, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const Groups<NT, NV, TAIL> gr(cols, t);
+  f32x4 aw[NV], g[NV];
+#pragma unroll
+  for (int n = 0; n < NV; n++) aw[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (w) gr.load(g, w);
+  for (long row = (long)blockIdx.x * RB + sub; row < rows; row += (long)gridDim.x * RB) {
+    f32x4 v[NV], d[NV], u[NV];
+    gr.load(v, x + row * cols);
+    gr.load(d, dy + row * cols);
+    if (ds && dx) gr.load(u, ds + row * cols);
+    const float r = rstd[row];
+    gr.mask(v);
+    gr.mask(d);
+    float q = 0.f, z = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[n][j] *= r;
+        aw[n][j] = fmaf(d[n][j], v[n][j], aw[n][j]);
+        if (w) d[n][j] = gr.own(n, j) ? d[n][j] * g[n][j] : 0.f;  // an infinite weight times 0 would count
+        q = fmaf(d[n][j], v[n][j], q);
+      }
+    if (!dx) continue;
+    row_sum2<NT>(q, z, red);
+    q /= (float)cols;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[n][j] = r * (d[n][j] - v[n][j] * q);
+        if (ds) v[n][j] += u[n][j];
+      }
+    gr.store(v, dx + row * cols);
+  }
+  if (!part) return;
+  float *out = part + (long)blockIdx.x * cols;
+#pragma unroll
+  for (int n = 0; n < NV; n++) {
+    f32x4 a = aw[n];
+    if (RB > 1) {  // the workgroup's rows, in order
+      __syncthreads();
+      *(f32x4 *)(join + threadIdx.x * 4) = a;
+      __syncthreads();
+      if (threadIdx.x >= NT) continue;
+#pragma unroll
+      for (int k = 1; k < RB; k++) a += *(const f32x4 *)(join + (k * NT + t) * 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (gr.own(n, j)) out[gr.at[n] + j] = a[j];
+  }
+}
+
+// the same of rows too long for registers (or shorter than a group)
+__global__ void __launch_bounds__(1024)
+    rms_fwd_long_kernel(const float *x, const float *res, const float *__restrict__ w, float *__restrict__ y,
+                        float *sum, float *__restrict__ rstd, long rows, long cols, float eps) {
+  __shared__ float part[16][2];
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float *p = x + row * cols, *u = res ? res + row * cols : nullptr;
+    float *s = sum ? sum + row * cols : nullptr;
+    float q = 0.f, z = 0.f;
+    for (long c = threadIdx.x; c < cols; c += 1024) {
+      const float v = u ? p[c] + u[c] : p[c];
+      if (s) s[c] = v;
+      q = fmaf(v, v, q);
+    }
+    row_sum2<1024>(q, z, part);
+    const float r = 1.f / sqrtf(q / (float)cols + eps);
+    for (long c = threadIdx.x; c < cols; c += 1024) {
+      const float v = s ? s[c] : u ? p[c] + u[c] : p[c];  // a thread's own columns
+      y[row * cols + c] = w ? v * r * w[c] : v * r;
+    }
+    if (threadIdx.x == 0 && rstd) rstd[row] = r;
+  }
+}
+
+__global__ void __launch_bounds__(1024)
+    rms_dx_long_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ dy,
+                       const float *ds, const float *__restrict__ rstd, float *dx, long rows, long cols) {
+  __shared__ float part[16][2];
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float *p = x + row * cols, *d = dy + row * cols;
+    const float r = rstd[row];
+    float q = 0.f, z = 0.f;
+    for (long c = threadIdx.x; c < cols; c += 1024) q = fmaf(w ? d[c] * w[c] : d[c], p[c] * r, q);
+    row_sum2<1024>(q, z, part);
+    q /= (float)cols;
+    for (long c = threadIdx.x; c < cols; c += 1024) {
+      const float v = r * ((w ? d[c] * w[c] : d[c]) - p[c] * r * q);
+      dx[row * cols + c] = ds ? v + ds[row * cols + c] : v;
+    }
+  }
+}
+
+// part[blockIdx.y][cols]: the sums for dw over a run of rows
+__global__ void __launch_bounds__(256)
+    rms_cols_long_kernel(const float *__restrict__ x, const float *__restrict__ dy, const float *__restrict__ rstd,
+                         float *__restrict__ part, long rows, long cols) {
+  const long c = (long)blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (long row = blockIdx.y; row < rows; row += gridDim.y)
+    s = fmaf(dy[row * cols + c], x[row * cols + c] * rstd[row], s);
+  part[(long)blockIdx.y * cols + c] = s;
 }
 
 // columns that 1024 threads hold 16 each of; and rows without a whole group
@@ -422,8 +591,77 @@ extern "C" int tt_k_layernorm_bwd(const float *x, const float *w, const float *d
   if (part) {
     // a grid axis has less than 2^32 threads (with more, columns stay unwritten)
     const long groups = (cols + 15) / 16;
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20), 2), dim3(1024), 0,
+    hipLaunchKernelGGL(join_kernel<2>, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20), 2), dim3(1024), 0,
                        stream(), part, dw, db, blocks, cols);
+  }
+  ttrt_free(own);
+  return launched();
+}
+
+extern "C" int tt_k_rmsnorm_fwd(const float *x, const float *residual, const float *w, float *y, float *sum,
+                                float *rstd, long rows, long cols, float eps) {
+  if (!x || !y || !good(rows, cols) || !(eps >= 0.f) || isinf(eps)) return -1;
+  if (ttrt_init() != 0) return -3;
+  if (long_rows(cols)) {
+    hipLaunchKernelGGL(rms_fwd_long_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(1024), 0, stream(),
+                       x, residual, w, y, sum, rstd, rows, cols, eps);
+    return launched();
+  }
+  const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols);
+  const unsigned grid = (unsigned)(groups < 1 << 20 ? groups : 1 << 20);
+#define RUN(NT, NV)                                                                                             \
+  if (cols % 4 == 0)                                                                                            \
+    hipLaunchKernelGGL((rms_fwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x,       \
+                       residual, w, y, sum, rstd, rows, (int)cols, eps);                                        \
+  else                                                                                                          \
+    hipLaunchKernelGGL((rms_fwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x,        \
+                       residual, w, y, sum, rstd, rows, (int)cols, eps)
+  BY_COLS(RUN)
+#undef RUN
+  return launched();
+}
+
+extern "C" size_t tt_k_rmsnorm_bwd_ws(long rows, long cols) {
+  return good(rows, cols) ? sizeof(float) * (size_t)cols * bwd_blocks(rows, cols) : 0;
+}
+
+extern "C" int tt_k_rmsnorm_bwd(const float *x, const float *w, const float *dy, const float *dsum,
+                                const float *rstd, float *dx, float *dw, long rows, long cols, void *ws) {
+  if (!x || !dy || !rstd || !good(rows, cols)) return -1;
+  if (!dx && !dw) return 0;
+  if (ttrt_init() != 0) return -3;
+  const int blocks = bwd_blocks(rows, cols);
+  float *own = NULL, *part = NULL;
+  if (dw) {
+    part = (float *)ws;
+    if (!part) part = own = (float *)ttrt_alloc(tt_k_rmsnorm_bwd_ws(rows, cols));
+    if (!part) return -2;
+  }
+  if (long_rows(cols)) {
+    if (dx)
+      hipLaunchKernelGGL(rms_dx_long_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(1024), 0, stream(),
+                         x, w, dy, dsum, rstd, dx, rows, cols);
+    if (part)
+      hipLaunchKernelGGL(rms_cols_long_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)blocks), dim3(256), 0,
+                         stream(), x, dy, rstd, part, rows, cols);
+  } else {
+    // without sums every row group has a workgroup of its own
+    const long groups = (rows + rows_a_group(cols) - 1) / rows_a_group(cols);
+    const unsigned grid = part ? (unsigned)blocks : (unsigned)(groups < 1 << 20 ? groups : 1 << 20);
+#define RUN(NT, NV)                                                                                            \
+  if (cols % 4 == 0)                                                                                           \
+    hipLaunchKernelGGL((rms_bwd_kernel<NT, NV, false>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w,   \
+                       dy, dsum, rstd, dx, part, rows, (int)cols);                                             \
+  else                                                                                                         \
+    hipLaunchKernelGGL((rms_bwd_kernel<NT, NV, true>), dim3(grid), dim3(threads_of(NT)), 0, stream(), x, w, dy, \
+                       dsum, rstd, dx, part, rows, (int)cols)
+    BY_COLS(RUN)
+#undef RUN
+  }
+  if (part) {
+    const long groups = (cols + 15) / 16;
+    hipLaunchKernelGGL(join_kernel<1>, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20)), dim3(1024), 0,
+                       stream(), part, dw, (float *)NULL, blocks, cols);
   }
   ttrt_free(own);
   return launched();

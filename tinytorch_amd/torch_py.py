@@ -148,6 +148,20 @@ class Node:
         return Node(_checked(LIB.ag_layernorm(self.ptr, None if w is None else w.ptr, None if b is None else b.ptr, eps),
                              "ag_layernorm"))
 
+    def rmsnorm(self, w=None, residual=None, eps=1e-5):
+        """RMS norm over the last axis, times w; with a residual of self + residual,
+        and the pair of the norm and that sum."""
+        s = ctypes.c_void_p()
+        y = Node(_checked(LIB.ag_rmsnorm(self.ptr, None if residual is None else residual.ptr,
+                                         None if w is None else w.ptr, eps, ctypes.byref(s)), "ag_rmsnorm"))
+        return y if residual is None else (y, Node(s.value))
+
+    def embedding(self, ids, scale=1.0):
+        """scale times this table's rows at ids (any shape, flattened); an id outside
+        the table: a row of zeros."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        return Node(_checked(LIB.ag_embedding(self.ptr, ids.ctypes.data, ids.size, scale), "ag_embedding"))
+
     def rope(self, heads, head_dim, positions=None, seq_len=0, rot_dim=None, interleaved=False, base=10000.0,
              scaling=0, factor=1.0, trained=0.0, low=0.0, high=0.0, magnitude=1.0):
         """Rotary positions: `positions` an int a row, or row % seq_len."""
@@ -202,9 +216,10 @@ class Node:
 
 
 class Optim:
-    """Optimizer with device-resident state (SGD-momentum or Adam).
+    """Optimizer with device-resident state (SGD-momentum, Adam, or Muon for
+    parameters of two axes or more).
 
-    The update rules are the reference harness's NumPy optimizers
+    The update rules of the first two are the reference harness's NumPy optimizers
     (reference tests/gate_mnist_mlp.py:121-124, tests/gate_cifar_cnn.py:81-98)
     run on the GPU; step(params) takes the parameter nodes in the same order
     on every call."""
@@ -221,6 +236,10 @@ class Optim:
     @classmethod
     def adam(cls, lr=0.003, beta1=0.9, beta2=0.999, eps=1e-8):
         return cls(LIB.ag_optim_adam(lr, beta1, beta2, eps))
+
+    @classmethod
+    def muon(cls, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0):
+        return cls(LIB.ag_optim_muon(lr, momentum, int(nesterov), weight_decay))
 
     def step(self, params):
         arr = (ctypes.c_void_p * len(params))(*[p.ptr for p in params])
