@@ -52,17 +52,18 @@ struct Matrix {
 };
 struct Matrices {
   Matrix at[MOST];
-  unsigned first[MOST + 1];  // matrix i has the workgroups [first[i], first[i + 1])
+  unsigned long first[MOST + 1];  // matrix i has the workgroups, or the units of work, [first[i], first[i + 1])
   int count;
 };
 
 __host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
 
-// which matrix a workgroup belongs to; b becomes its number among that one's
-__device__ __forceinline__ int matrix_of(const Matrices &a, unsigned &b) {
+// which matrix a workgroup or unit belongs to; b becomes its number among that one's
+template <class N>
+__device__ __forceinline__ int matrix_of(const Matrices &a, N &b) {
   int i = 0;
   while (i + 1 < a.count && b >= a.first[i + 1]) i++;
-  b -= a.first[i];
+  b -= (N)a.first[i];
   return i;
 }
 
@@ -300,6 +301,323 @@ __global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
   }
 }
 
+// ---------------------------------------------------------------- large products
+//
+// Tiles of 128 x 128, four waves with a quarter each, the operands through LDS in
+// two buffers of a block (32 of the products' length): while one is multiplied the
+// next is on its way by direct loads.  Per block and wave 24 matrix instructions
+// stand against 16 KB read from LDS, and two workgroups a CU fill each other's
+// waits.  The tiles' blocks are dealt evenly to the workgroups, whatever the
+// matrices' shapes: a workgroup has whole tiles and at most two pieces of tiles
+// that others have the rest of.  Pieces go to memory, and join_kernel adds them.
+
+#ifndef TT_LARGE
+#define TT_LARGE 8e8
+#endif
+#ifndef TT_HUGE
+#define TT_HUGE 1.7e10
+#endif
+// Tiles of T x T: four waves of 64 x 64 or eight of 128 x 64 values, each FI x 2
+// blocks of 32 x 32.
+template <int T>
+struct Shape {
+  static constexpr int WAVES = T == 256 ? 8 : 4, ACROSS = WAVES / 2, FI = T / 64, BLOCKS = 2 * FI;
+  static constexpr int GROUPS = T == 256 ? 256 : 512;  // workgroups at most: one or two a CU
+  static constexpr int PIECE = T * T;                  // floats
+  static constexpr int BUFFER = 2 * T * 128;           // bytes of both operands' block
+};
+
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
+}
+// lane l's 16 bytes at base + off to LDS at lds + 16 l
+__device__ __forceinline__ void dma16(const char *base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ const char *scalar(const char *p) {
+  const uint64_t x = (uint64_t)p;
+  return (const char *)((uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+
+// Tiles in bands of eight rows, column by column, so that the workgroups of an XCD
+// (consecutive ones) share rows and columns.
+constexpr int BAND = 8;
+template <int KIND, int T>
+__device__ __forceinline__ void tile_of(unsigned long tile, int rows, int cols, int &ti, int &tj) {
+  const int nr = (rows + T - 1) / T, nc = (cols + T - 1) / T;
+  if (KIND <= SQUARE) {
+    // below band b: 32 b^2 + 4 b tiles of the lower triangle
+    int b = (int)((sqrt(128.0 * (double)tile + 16.0) - 4.0) / 64.0);
+    while (b > 0 && 32ul * b * b + 4ul * b > tile) b--;
+    while (32ul * (b + 1) * (b + 1) + 4ul * (b + 1) <= tile) b++;
+    const unsigned in = (unsigned)(tile - (32ul * b * b + 4ul * b));
+    const unsigned h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
+    if (in < (unsigned)b * BAND * h) {
+      ti = b * BAND + (int)(in % h), tj = (int)(in / h);
+    } else {
+      triangle(in - (unsigned)b * BAND * h, ti, tj);
+      ti += b * BAND, tj += b * BAND;
+    }
+  } else {
+    const unsigned long band = (unsigned long)BAND * nc;
+    const int b = (int)(tile / band);
+    const unsigned in = (unsigned)(tile % band), h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
+    ti = b * BAND + (int)(in % h), tj = (int)(in / h);
+  }
+}
+
+// A wave's 32 x 32 values, `acc` as the matrix instructions leave them, to where
+// they go: through LDS, so that a lane has 16 of a row (and, for the transpose, of a
+// column) and lines are written whole.
+template <int KIND>
+__device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, long r0, long c0,
+                                        float (*buf)[33], int lane, bool transpose) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) buf[8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
+  __builtin_amdgcn_wave_barrier();
+  const int line = lane >> 1, from = (lane & 1) * 16;
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; j++) v[j] = buf[line][from + j] * (o.by * DOWN2);
+  const long row = r0 + line, col = c0 + from, blocks = blocks_of(o.cols);
+  if (KIND != GRAM && row < o.rows && c0 < o.cols) {
+    const half8 *p = (const half8 *)place((char *)o.add, blocks, row, col);
+    const half8 h[2] = {p[0], p[1]}, l[2] = {p[4], p[5]};
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] += o.times * (1.f / UP) * ((float)h[j / 8][j % 8] + (float)l[j / 8][j % 8]);
+  }
+#pragma unroll
+  for (int j = 0; j < 16; j++)
+    if (row >= o.rows || col + j >= o.cols) v[j] = 0.f;
+  if (transpose) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) buf[line][from + j] = v[j];
+  }
+  if (KIND == LAST) {
+    if (!transpose && row < o.rows) {
+      float *w = M.w + row * o.cols + col;
+      if (col + 16 <= o.cols) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          f32x4 u = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+          if (M.v) u = *(const f32x4_any *)(w + j) * M.keep + u * M.rate;
+          *(f32x4_any *)(w + j) = u;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+          if (col + j < o.cols) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
+      }
+    }
+  } else if (row < o.rows && c0 < o.cols) {
+    half8 h[2], l[2];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      _Float16 a, b;
+      split(v[j] * UP, a, b);
+      h[j / 8][j % 8] = a;
+      l[j / 8][j % 8] = b;
+    }
+    half8 *p = (half8 *)place(o.out, blocks, row, col);
+    p[0] = h[0], p[1] = h[1], p[4] = l[0], p[5] = l[1];
+  }
+  if (!transpose) return;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < 16; j++) v[j] = buf[from + j][line];
+  const long trow = c0 + line, tcol = r0 + from;
+  if (trow >= o.cols) return;
+  if (KIND == LAST) {
+    float *w = M.w + trow * o.rows + tcol;
+    if (tcol + 16 <= o.rows) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        f32x4 u = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+        if (M.v) u = *(const f32x4_any *)(w + j) * M.keep + u * M.rate;
+        *(f32x4_any *)(w + j) = u;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (tcol + j < o.rows) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
+    }
+  } else if (r0 < o.rows) {
+    half8 h[2], l[2];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      _Float16 a, b;
+      split(v[j] * UP, a, b);
+      h[j / 8][j % 8] = a;
+      l[j / 8][j % 8] = b;
+    }
+    half8 *p = (half8 *)place(o.down, blocks_of(o.rows), trow, tcol);
+    p[0] = h[0], p[1] = h[1], p[4] = l[0], p[5] = l[1];
+  }
+}
+
+// where the 32 x 32 block f of a wave's lies
+template <int T>
+__device__ __forceinline__ long row_of(int ti, int wave, int f) {
+  return (long)ti * T + (wave / Shape<T>::ACROSS) * (T / 2) + f / 2 * 32;
+}
+template <int T>
+__device__ __forceinline__ long col_of(int tj, int wave, int f) {
+  return (long)tj * T + (wave % Shape<T>::ACROSS) * 64 + f % 2 * 32;
+}
+template <int KIND>
+__device__ __forceinline__ bool transposed(const Matrix &M, int ti, int tj) {
+  return KIND <= SQUARE ? ti != tj : KIND == STEP || M.turned;
+}
+
+// the first unit of workgroup w's
+__device__ __forceinline__ unsigned long begins(unsigned long units, unsigned w, unsigned groups) {
+  return units * w / groups;
+}
+
+template <int KIND, int T>
+__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices a, int step, float *pieces) {
+  typedef Shape<T> S;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * S::BUFFER];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // consecutive workgroups go to the eight XCDs in turn: give each XCD a run of them
+  const unsigned groups = gridDim.x, each = groups / 8, b = blockIdx.x;
+  const unsigned w = b < each * 8 ? (b % 8) * each + b / 8 : b;
+  const unsigned long units = a.first[a.count], end = begins(units, w + 1, groups);
+  const unsigned to = lds_address(lds);
+  for (unsigned long u = begins(units, w, groups); u < end;) {
+    unsigned long in = u;
+    const Matrix &M = a.at[matrix_of(a, in)];
+    const Operands<KIND> o(M, step);
+    const long blocks = blocks_of(o.k);
+    int ti, tj;
+    tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
+    const int k0 = (int)(in % blocks), k1 = (int)(end - u < (unsigned long)(blocks - k0) ? k0 + (end - u) : blocks);
+    // lane l brings 16 bytes of row 8 i + l / 8; where it puts them, l % 8 of the row's
+    // eight places, is where its (l % 8) ^ (l / 8) belong: rows then differ in their
+    // places, and the reads below meet no bank twice.  A row behind the last is the
+    // last once more: its results are not written.
+    constexpr int EACH = T / 8 / S::WAVES;
+    unsigned off[2][EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const int r = (wave * EACH + i) * 8 + (lane >> 3), chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+      const int ra = ti * T + r < o.rows ? r : o.rows - 1 - ti * T, rb = tj * T + r < o.cols ? r : o.cols - 1 - tj * T;
+      off[0][i] = (unsigned)(ra * blocks * 128) + chunk;
+      off[1][i] = (unsigned)(rb * blocks * 128) + chunk;
+    }
+    const char *pa = scalar(o.a + ((long)ti * T * blocks + k0) * 128);
+    const char *pb = scalar(o.b + ((long)tj * T * blocks + k0) * 128);
+    auto bring = [&](int k, unsigned at) {
+#pragma unroll
+      for (int i = 0; i < EACH; i++) dma16(pa + (long)k * 128, off[0][i], at + (wave * EACH + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < EACH; i++) dma16(pb + (long)k * 128, off[1][i], at + T * 128 + (wave * EACH + i) * 1024);
+    };
+    f32x16 acc[S::FI][2] = {};
+    __syncthreads();  // the last tile's LDS is read
+    bring(0, to);
+    const int n = k1 - k0, row = lane & 31, half = lane >> 5;
+    // the wave's rows of either operand in a buffer
+    const char *mine[2] = {lds + ((wave / S::ACROSS) * (T / 2) + row) * 128,
+                           lds + (T + (wave % S::ACROSS) * 64 + row) * 128};
+    for (int k = 0; k < n; k++) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const int now = (k & 1) * S::BUFFER;
+      if (k + 1 < n) bring(k + 1, to + (S::BUFFER - now));
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const int ph = now + (((s * 2 + half) ^ (row & 7)) * 16), pl = now + (((s * 2 + half + 4) ^ (row & 7)) * 16);
+        half8 ha[S::FI], la[S::FI], hb[2], lb[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          hb[j] = *(const half8 *)(mine[1] + ph + j * 4096);
+          lb[j] = *(const half8 *)(mine[1] + pl + j * 4096);
+        }
+#pragma unroll
+        for (int i = 0; i < S::FI; i++) {
+          ha[i] = *(const half8 *)(mine[0] + ph + i * 4096);
+          la[i] = *(const half8 *)(mine[0] + pl + i * 4096);
+        }
+#pragma unroll
+        for (int i = 0; i < S::FI; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(la[i], hb[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < S::FI; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[i], lb[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < S::FI; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[i], hb[j], acc[i][j], 0, 0, 0);
+      }
+    }
+    if (n == blocks) {
+      __syncthreads();  // the operands are read
+      const bool transpose = transposed<KIND>(M, ti, tj);
+#pragma unroll
+      for (int f = 0; f < S::BLOCKS; f++) {
+        write32<KIND>(M, o, acc[f / 2][f % 2], row_of<T>(ti, wave, f), col_of<T>(tj, wave, f),
+                      (float(*)[33])(lds + wave * 8192), lane, transpose);
+        __builtin_amdgcn_wave_barrier();
+      }
+    } else {
+      f32x4 *p = (f32x4 *)(pieces + (2l * w + (k0 == 0)) * S::PIECE) + wave * S::BLOCKS * 256 + lane;
+#pragma unroll
+      for (int i = 0; i < S::BLOCKS * 4; i++) {
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = acc[i / 8][i / 4 % 2][i % 4 * 4 + j];
+        p[i * 64] = v;
+      }
+    }
+    u += n;
+  }
+}
+
+// Workgroups (w - 1, .) add the pieces of the tile in which the units of
+// tile_kernel's workgroup w begin, where that is the first to begin inside it; a
+// wave has 32 x 32 of its values.
+template <int KIND, int T>
+__global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, const float *pieces, unsigned groups) {
+  typedef Shape<T> S;
+  __shared__ float buf[4][32][33];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned w = blockIdx.x + 1;
+  const unsigned long units = a.first[a.count], u = begins(units, w, groups);
+  unsigned long in = u;
+  const Matrix &M = a.at[matrix_of(a, in)];
+  const Operands<KIND> o(M, step);
+  const unsigned long blocks = blocks_of(o.k), k0 = in % blocks, first = u - k0, last = first + blocks;
+  if (k0 == 0 || begins(units, w - 1, groups) > first) return;
+  int ti, tj;
+  tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
+  const int block = blockIdx.y * 4 + wave;
+  unsigned stop = w;  // the first workgroup behind the tile
+  while (stop < groups && begins(units, stop, groups) < last) stop++;
+  f32x16 acc = {};
+  const f32x4 *p = (const f32x4 *)pieces + block * 256 + lane;
+#pragma unroll 4
+  for (unsigned g = w - 1; g < stop; g++) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const f32x4 v = p[(2l * g + (g < w)) * (S::PIECE / 4) + i * 64];
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
+    }
+  }
+  write32<KIND>(M, o, acc, row_of<T>(ti, block / S::BLOCKS, block % S::BLOCKS),
+                col_of<T>(tj, block / S::BLOCKS, block % S::BLOCKS), buf[wave], lane, transposed<KIND>(M, ti, tj));
+}
+
 // ---------------------------------------------------------------- host
 
 size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
@@ -308,7 +626,7 @@ bool good_sides(long rows, long cols) {
   return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= 1L << 32;
 }
 
-size_t ws_of(long rows, long cols) {
+size_t images_of(long rows, long cols) {
   const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
   return up((size_t)m * blocks_of((int)n) * 128) + 2 * up((size_t)n * blocks_of((int)m) * 128) +
          2 * up((size_t)m * blocks_of((int)m) * 128) + up(sizeof(double) * NORM_PARTS);
@@ -333,37 +651,85 @@ void lay(Matrix &M, long rows, long cols, char *&ws) {
 }
 
 template <class F>
-unsigned number(Matrices &a, F workgroups) {
+unsigned long number(Matrices &a, F workgroups) {
   unsigned long at = 0;
   for (int i = 0; i < a.count; i++) {
-    a.first[i] = (unsigned)at;
+    a.first[i] = at;
     at += (unsigned long)workgroups(a.at[i]);
   }
-  a.first[a.count] = (unsigned)at;
-  return (unsigned)at;
+  a.first[a.count] = at;
+  return at;
 }
 
-void run(Matrices &a, int steps, float mu, int nesterov) {
-  unsigned grid = number(a, [](const Matrix &M) { return (long)M.parts; });
-  hipLaunchKernelGGL(momentum_kernel, dim3(grid), dim3(256), 0, stream(), a, mu, nesterov);
+// How the products of such matrices go: by tiles of 32 (0), 128 or 256.
+int tile_size(const Matrices &a) {
+  double work = 0;
+  for (int i = 0; i < a.count; i++) work += (double)a.at[i].m * a.at[i].m * a.at[i].n;
+  return work < TT_LARGE ? 0 : work < TT_HUGE ? 128 : 256;
+}
+
+template <int KIND>
+void small_product(Matrices &a, int step) {
+  const unsigned long grid = number(a, [](const Matrix &M) {
+    return KIND <= SQUARE ? blocks_of(M.m) * (blocks_of(M.m) + 1) / 2 : blocks_of(M.m) * blocks_of(M.n);
+  });
+  hipLaunchKernelGGL(small_kernel<KIND>, dim3((unsigned)grid), dim3(512), 0, stream(), a, step);
+}
+
+template <int KIND, int T>
+void tile_product(Matrices &a, int step, float *pieces) {
+  typedef Shape<T> S;
+  bool whole = true;
+  long blocks = 0;
+  const unsigned long units = number(a, [&](const Matrix &M) {
+    const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T, k = blocks_of(KIND == GRAM ? M.n : M.m);
+    whole = whole && (!blocks || blocks == k);
+    blocks = k;
+    return (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * k;
+  });
+  const unsigned groups = (unsigned)(units < 8 * S::GROUPS ? (units + 7) / 8 : S::GROUPS);
+  hipLaunchKernelGGL((tile_kernel<KIND, T>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, pieces);
+  if (groups > 1 && (!whole || units % (groups * blocks)))  // else nobody has a piece
+    hipLaunchKernelGGL((join_kernel<KIND, T>), dim3(groups - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step,
+                       (const float *)pieces, groups);
+}
+
+template <int KIND>
+void product(Matrices &a, int step, int tile, float *pieces) {
+  if (tile == 0) small_product<KIND>(a, step);
+  else if (tile == 128) tile_product<KIND, 128>(a, step, pieces);
+  else tile_product<KIND, 256>(a, step, pieces);
+}
+
+void run(Matrices &a, int steps, float mu, int nesterov, char *rest) {
+  unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
+  hipLaunchKernelGGL(momentum_kernel, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
-  hipLaunchKernelGGL(image_kernel, dim3(grid), dim3(256), 0, stream(), a, mu, nesterov);
-  Matrices half = a;
-  const unsigned lower = number(half, [](const Matrix &M) { return blocks_of(M.m) * (blocks_of(M.m) + 1) / 2; });
-  const unsigned all = number(a, [](const Matrix &M) { return blocks_of(M.m) * blocks_of(M.n); });
+  hipLaunchKernelGGL(image_kernel, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
+  const int tile = tile_size(a);
   for (int s = 0; s < steps; s++) {
-    hipLaunchKernelGGL(small_kernel<GRAM>, dim3(lower), dim3(512), 0, stream(), half, s);
-    hipLaunchKernelGGL(small_kernel<SQUARE>, dim3(lower), dim3(512), 0, stream(), half, s);
-    if (s + 1 < steps) hipLaunchKernelGGL(small_kernel<STEP>, dim3(all), dim3(512), 0, stream(), a, s);
-    else hipLaunchKernelGGL(small_kernel<LAST>, dim3(all), dim3(512), 0, stream(), a, s);
+    product<GRAM>(a, s, tile, (float *)rest);
+    product<SQUARE>(a, s, tile, (float *)rest);
+    if (s + 1 < steps) product<STEP>(a, s, tile, (float *)rest);
+    else product<LAST>(a, s, tile, (float *)rest);
   }
+}
+
+// the images of up to MOST matrices, and two pieces a workgroup
+size_t ws_of(const Matrices &a, size_t images) {
+  const int t = tile_size(a);
+  return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * (t == 128 ? Shape<128>::GROUPS : Shape<256>::GROUPS));
 }
 
 }  // namespace
 
 extern "C" size_t tt_k_newton_schulz_ws(long count, long rows, long cols) {
   if (count <= 0 || !good_sides(rows, cols)) return 0;
-  return (size_t)(count < MOST ? count : MOST) * ws_of(rows, cols);
+  Matrices a = {};
+  a.count = (int)(count < MOST ? count : MOST);
+  char *at = NULL;
+  for (int i = 0; i < a.count; i++) lay(a.at[i], rows, cols, at);
+  return ws_of(a, a.count * images_of(rows, cols));
 }
 
 extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps, void *ws) {
@@ -383,7 +749,7 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
       a.at[i].w = y + (base + i) * rows * cols;
       lay(a.at[i], rows, cols, at);
     }
-    run(a, steps, 0.f, 0);
+    run(a, steps, 0.f, 0, at);
   }
   ttrt_free(own);
   return launched();
@@ -391,12 +757,16 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
 
 extern "C" size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int count) {
   if (!rows || !cols || count < 1 || count > TT_SGD_MAX) return 0;
+  Matrices a = {};
+  a.count = count;
   size_t bytes = 0;
+  char *at = NULL;
   for (int i = 0; i < count; i++) {
     if (!good_sides(rows[i], cols[i])) return 0;
-    bytes += ws_of(rows[i], cols[i]);
+    lay(a.at[i], rows[i], cols[i], at);
+    bytes += images_of(rows[i], cols[i]);
   }
-  return bytes;
+  return ws_of(a, bytes);
 }
 
 extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *const *v, const long *rows,
@@ -424,7 +794,7 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
     M.rate = (float)(-(double)lr * TT_MUON_RMS * sqrt((double)(rows[i] > cols[i] ? rows[i] : cols[i])));
     lay(M, rows[i], cols[i], at);
   }
-  run(a, TT_MUON_STEPS, mu, nesterov);
+  run(a, TT_MUON_STEPS, mu, nesterov, at);
   ttrt_free(own);
   return launched();
 }
