@@ -503,13 +503,14 @@ int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows
  * `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X, which takes singular
  * values s to a s + b s^3 + c s^5.  y may be x.  A matrix with an infinity or a
  * NaN has NaN throughout.  Sides at most 2^20, rows * cols 2^32.  ws: 256-byte
- * aligned; about 14 bytes a value of up to TT_SGD_MAX matrices, 20 of square
- * ones. */
+ * aligned; about 14 bytes a value of up to 64 matrices, 20 of square ones, and up
+ * to 128 MiB; none (size 0) where a matrix fits a CU's LDS. */
 #define TT_NS_A 3.4445f
 #define TT_NS_B (-4.7750f)
 #define TT_NS_C 2.0315f
 #define TT_NS_MAX_STEPS 64
 #define TT_MUON_MAX_SIDE (1L << 20)
+#define TT_MUON_MAX_VALUES (1L << 32)
 size_t tt_k_newton_schulz_ws(long count, long rows, long cols);
 int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps,
                        void *ws);

@@ -16,7 +16,8 @@ pytestmark = pytest.mark.gpu
 NEAR = ref.A**4 * ref.PART
 
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (4, 31), (32, 32), (33, 32), (31, 65), (10, 785), (129, 10), (64, 64),
-          (65, 127), (100, 333), (257, 128), (128, 129), (150, 2100), (1030, 70)]
+          (65, 127), (100, 333), (257, 128), (128, 129), (150, 2100), (1030, 70), (31, 1100), (60, 500), (90, 260),
+          (120, 160), (160, 128), (129, 129), (300, 300)]
 
 
 def _matrix(rows, cols, kind="full", seed=0):
@@ -105,17 +106,18 @@ def test_steps_of_zeros_and_bad_values(tlib):
     assert np.abs(_steps(tlib, x, 5) - want).max() <= 1e-5
 
 
-@pytest.mark.parametrize("count", [1, 2, 16, 17, 40])
-def test_steps_of_many(tlib, count):
+@pytest.mark.parametrize("rows,cols", [(37, 50), (150, 140)])
+@pytest.mark.parametrize("count", [1, 2, 17, 64, 65, 140])
+def test_steps_of_many(tlib, count, rows, cols):
     """Each as alone, whatever the others hold."""
-    x = np.stack([_matrix(37, 50, seed=i) for i in range(count)])
+    x = np.stack([_matrix(rows, cols, seed=i) for i in range(count)])
     if count > 2:
         x[1] = np.nan
     got = _steps(tlib, x, 5)
     for i in {0, min(1, count - 1), count // 2, count - 1}:
         one = _steps(tlib, x[i], 5)
         assert np.array_equal(got[i], one, equal_nan=True)
-    ws = DevBuf(tlib.tt_k_newton_schulz_ws(count, 37, 50) // 4 + 16)
+    ws = DevBuf(tlib.tt_k_newton_schulz_ws(count, rows, cols) // 4 + 16)
     ws.fill(-7.0)
     assert np.array_equal(_steps(tlib, x, 5, ws.ptr), got, equal_nan=True)
     assert (ws.to_np()[-16:] == -7).all()
@@ -168,22 +170,26 @@ def test_muon_step(tlib, shapes, nesterov):
             assert np.array_equal(G[i].to_np(s), g[i])
 
 
-def test_muon_workspace_allocates_nothing(tlib):
-    x = _matrix(70, 90)
+@pytest.mark.parametrize("rows,cols", [(70, 90), (270, 390)])
+def test_muon_workspace_allocates_nothing(tlib, rows, cols):
+    """The smaller needs none."""
+    x = _matrix(rows, cols)
     want = _steps(tlib, x, 5)
-    X, y, ws = DevBuf.from_np(x), DevBuf(x.size), DevBuf(tlib.tt_k_newton_schulz_ws(1, 70, 90) // 4)
-    w, g, v = (DevBuf.from_np(_matrix(70, 90, seed=s)) for s in (1, 2, 3))
-    wss = DevBuf(tlib.tt_k_muon_multi_ws(_long([70]), _long([90]), 1) // 4)
+    need = tlib.tt_k_newton_schulz_ws(1, rows, cols)
+    X, y, ws = DevBuf.from_np(x), DevBuf(x.size), DevBuf(need // 4 + 1)
+    w, g, v = (DevBuf.from_np(_matrix(rows, cols, seed=s)) for s in (1, 2, 3))
+    wss = DevBuf(tlib.tt_k_muon_multi_ws(_long([rows]), _long([cols]), 1) // 4 + 1)
+    assert (need == 0) == (rows == 70)
     assert tlib.tth_fail_alloc_after(0) == 0
     try:
-        rc = [tlib.tt_k_newton_schulz(X.ptr, y.ptr, 1, 70, 90, 5, ws.ptr),
-              tlib.tt_k_newton_schulz(X.ptr, y.ptr, 1, 70, 90, 5, None)]
+        rc = [tlib.tt_k_newton_schulz(X.ptr, y.ptr, 1, rows, cols, 5, ws.ptr),
+              tlib.tt_k_newton_schulz(X.ptr, y.ptr, 1, rows, cols, 5, None)]
         for p in (wss.ptr, None):
-            rc.append(tlib.tt_k_muon_multi(_ptrs([w]), _ptrs([g]), _ptrs([v]), _long([70]), _long([90]), 1, 0.1, 0.9,
-                                           1, 0.0, p))
+            rc.append(tlib.tt_k_muon_multi(_ptrs([w]), _ptrs([g]), _ptrs([v]), _long([rows]), _long([cols]), 1, 0.1,
+                                           0.9, 1, 0.0, p))
     finally:
         tlib.tth_fail_alloc_after(-1)
-    assert rc == [0, -2, 0, -2]
+    assert rc == ([0, -2, 0, -2] if need else [0] * 4)
     assert np.array_equal(y.to_np(x.shape), want)
 
 

@@ -91,13 +91,19 @@ def test_muon_without_matrices(L):
 
 
 def test_workspace_sizes(L):
-    """About 14 bytes a value and 20 of a square matrix's, for 16 matrices at most."""
-    one = L.tt_k_newton_schulz_ws(1, 1024, 4096)
-    assert 12 * 1024 * 4096 <= one <= 14.1 * 1024 * 4096
-    assert L.tt_k_newton_schulz_ws(16, 1024, 4096) == 16 * one == L.tt_k_newton_schulz_ws(1000, 1024, 4096)
-    assert 20 * 512 * 512 <= L.tt_k_newton_schulz_ws(1, 512, 512) <= 20.2 * 512 * 512
+    """About 14 bytes a value, 20 of a square matrix's, for 64 matrices of a shape at
+    most, and up to 128 MiB; nothing for small matrices."""
+    more = 128 << 20
+    for m, n, least, most in ((1024, 4096, 12, 14.1), (512, 512, 20, 20.2), (300, 400, 16, 20)):
+        one = L.tt_k_newton_schulz_ws(1, m, n)
+        assert least * m * n <= one <= most * m * n + more
+        many = L.tt_k_newton_schulz_ws(64, m, n)
+        assert 64 * least * m * n <= many <= 64 * most * m * n + more
+        assert many == L.tt_k_newton_schulz_ws(1000, m, n) == L.tt_k_newton_schulz_ws(64, n, m)
+    assert L.tt_k_newton_schulz_ws(1000, 128, 128) == 0 == L.tt_k_newton_schulz_ws(1, 10, 785)
     r, c = (ctypes.c_long * 2)(1024, 512), (ctypes.c_long * 2)(4096, 512)
-    assert L.tt_k_muon_multi_ws(r, c, 2) == one + L.tt_k_newton_schulz_ws(1, 512, 512)
+    both = L.tt_k_muon_multi_ws(r, c, 2)
+    assert 12 * 1024 * 4096 + 20 * 512 * 512 <= both <= 14.1 * 1024 * 4096 + 20.2 * 512 * 512 + more
     assert L.tt_k_embedding_bwd_ws(8192, 32000, 1024) <= 17 * 8192 + 8 * 256 * 1024 + 64
 
 

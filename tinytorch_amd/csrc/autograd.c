@@ -2089,7 +2089,8 @@ static int muon_takes(AGNode *const *params, int count) {
         long rows, cols;
         if (!params[i] || params[i]->val->ndim < 2) return 0;
         sides(params[i]->val, &rows, &cols);
-        if (!tt_k_muon_multi_ws(&rows, &cols, 1)) return 0;
+        if (rows > TT_MUON_MAX_SIDE || cols > TT_MUON_MAX_SIDE || rows > TT_MUON_MAX_VALUES / cols)
+            return 0;
         for (int j = 0; j < i; j++)
             if (params[j]->val == params[i]->val) return 0;
     }

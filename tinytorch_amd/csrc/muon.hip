@@ -35,14 +35,18 @@ typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
+#ifndef TT_NOBLOCK
+#define TT_NOBLOCK 0
+#endif
 constexpr float UP = 16384.f, DOWN2 = 1.f / (16384.f * 16384.f);
-constexpr int MOST = TT_SGD_MAX;   // matrices in one run of launches
+constexpr int MOST = TT_SGD_MAX;   // matrices of different shapes in one run of launches
+constexpr int ALIKE = 64;          // of one shape
 constexpr int NORM_PARTS = 1024;   // sums of squares of a matrix
 
 struct Matrix {
   const float *g;   // what is orthogonalised, or the gradient (rows x cols)
   float *v, *w;     // momenta and weights; v NULL: the result goes to w
-  char *x, *t[2];   // images of X (m rows), X^T (n rows; the steps write one from the other)
+  char *x, *t0, *t1;  // images of X (m rows), X^T (n rows; the steps write one from the other)
   char *p, *q;      // of P and Q
   double *norm;     // NORM_PARTS partial sums of squares
   float keep, rate; // w = keep w + rate X
@@ -54,17 +58,33 @@ struct Matrices {
   Matrix at[MOST];
   unsigned long first[MOST + 1];  // matrix i has the workgroups, or the units of work, [first[i], first[i + 1])
   int count;
+  int alike;       // all are at[0]'s shape: matrix i lies behind it by i times
+  long images;     // bytes of the workspace
 };
 
 __host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
 
 // which matrix a workgroup or unit belongs to; b becomes its number among that one's
+__device__ __forceinline__ Matrix matrix(const Matrices &a, int i) {
+  if (!a.alike) return a.at[i];
+  Matrix M = a.at[0];
+  M.g += (long)i * M.m * M.n, M.w += (long)i * M.m * M.n;
+  const long off = i * a.images;
+  M.x += off, M.t0 += off, M.t1 += off, M.p += off, M.q += off;
+  M.norm += off / (long)sizeof(double);
+  return M;
+}
 template <class N>
-__device__ __forceinline__ int matrix_of(const Matrices &a, N &b) {
+__device__ __forceinline__ Matrix matrix_of(const Matrices &a, N &b) {
   int i = 0;
-  while (i + 1 < a.count && b >= a.first[i + 1]) i++;
-  b -= (N)a.first[i];
-  return i;
+  if (a.alike) {
+    i = (int)(b / (N)a.first[1]);
+    b -= (N)i * (N)a.first[1];
+  } else {
+    while (i + 1 < a.count && b >= a.first[i + 1]) i++;
+    b -= (N)a.first[i];
+  }
+  return matrix(a, i);
 }
 
 // x 2^14 in two parts
@@ -76,6 +96,254 @@ __device__ __forceinline__ _Float16 *place(char *image, long blocks, long r, lon
   return (_Float16 *)(image + (r * blocks + (c >> 5)) * 128) + (c & 31);
 }
 
+// ---------------------------------------------------------------- small matrices
+//
+// A matrix whose image of X and of P or Q (which follow each other in one place) fit
+// LDS has a workgroup, which takes it from the gradient to the weights in one
+// launch.  A wave has blocks of 32 x 32 of each result, kept in registers until all
+// have read what they replace.  X^T is X read by transposing loads.  The products
+// are formed transposed: a lane then holds four neighbours of a row, and P and Q
+// are symmetric.
+
+constexpr int BLOCK_WAVES = 16, BLOCK_LDS = 160 * 1024 - 256;
+constexpr int BLOCK_KEEP = 3;  // blocks of X a wave
+// X, P and the partial sums of P (one or four blocks of it: eight or two waves each)
+__host__ __device__ inline long block_bytes(int m, int n) {
+  const long mb = blocks_of(m), nb = blocks_of(n);
+  return 4096 * (mb * nb + mb * mb + (mb == 1 ? 7 : mb == 2 ? 4 : 0));
+}
+inline bool fits_block(int m, int n) {
+  return block_bytes(m, n) <= BLOCK_LDS && blocks_of(m) * blocks_of(n) <= BLOCK_WAVES * BLOCK_KEEP;
+}
+
+// Chunk (16 bytes) c of a block's eight in row r lies at c ^ (r / 2 % 8), and odd
+// rows begin in the other half of the banks: where a row has an even number of
+// blocks, neighbouring ones change places there.  No two of the lanes that LDS
+// serves at once meet a bank (128 x 128: 71 us with half of them in one).
+__device__ __forceinline__ const char *chunk_of(const char *image, int blocks, int r, int block, int c) {
+  block ^= r & ~blocks & 1;
+  return image + (r * blocks + block) * 128 + ((c ^ (r >> 1 & 7)) << 4);
+}
+__device__ __forceinline__ half8 along(const char *image, int blocks, int r0, int block, int half, int part, int lane) {
+  return *(const half8 *)chunk_of(image, blocks, r0 + (lane & 31), block, part * 4 + half * 2 + (lane >> 5));
+}
+// The transposing read: sixteen lanes read four values each of four rows and sixteen
+// columns (lane l: row l / 4, columns 4 (l % 4) ..) and get the four rows of column l.
+// Eight rows r0 + 8 (lane / 32) .. of column lane % 32 of a block.
+__device__ __forceinline__ half8 across(const char *image, int blocks, int r0, int block, int part, int lane) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  s16x8 v;
+  const int l = lane & 15, c = (lane >> 4 & 1) * 16 + 4 * (l & 3);
+#pragma unroll
+  for (int x = 0; x < 2; x++) {
+    const char *p = chunk_of(image, blocks, r0 + (lane >> 5) * 8 + x * 4 + l / 4, block, part * 4 + c / 8) + (c & 4) * 2;
+    const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p));
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[x * 4 + j] = w[j];
+  }
+  return __builtin_bit_cast(half8, v);
+}
+__device__ __forceinline__ void three(f32x16 &acc, half8 ha, half8 la, half8 hb, half8 lb) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(la, hb, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha, lb, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha, hb, acc, 0, 0, 0);
+}
+// four values of row r from column c on, and back
+__device__ __forceinline__ f32x4 get4(const char *image, int blocks, int r, int c) {
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  const half4 h = *(const half4 *)(chunk_of(image, blocks, r, c >> 5, c >> 3 & 3) + (c & 4) * 2);
+  const half4 l = *(const half4 *)(chunk_of(image, blocks, r, c >> 5, 4 + (c >> 3 & 3)) + (c & 4) * 2);
+  f32x4 v;
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = ((float)h[j] + (float)l[j]) * (1.f / UP);
+  return v;
+}
+__device__ __forceinline__ void put4(char *image, int blocks, int r, int c, f32x4 v) {
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  half4 h, l;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    _Float16 a, b;
+    split(v[j] * UP, a, b);
+    h[j] = a, l[j] = b;
+  }
+  *(half4 *)(chunk_of(image, blocks, r, c >> 5, c >> 3 & 3) + (c & 4) * 2) = h;
+  *(half4 *)(chunk_of(image, blocks, r, c >> 5, 4 + (c >> 3 & 3)) + (c & 4) * 2) = l;
+}
+
+// v = mu v + g where there are momenta, and u = g + mu v (nesterov) or v; without g
+template <class V>
+__device__ __forceinline__ V momentum(const float *g, float *v, float mu, int nesterov, bool store) {
+  V u = *(const V *)g;
+  if (!v) return u;
+  V w = *(const V *)v;
+  if (store) {
+    w = w * mu + u;
+    *(V *)v = w;
+  }
+  return nesterov ? w * mu + u : w;
+}
+
+__global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices a, int steps, float mu, int nesterov) {
+  __shared__ __attribute__((aligned(1024))) char lds[BLOCK_LDS];
+  __shared__ double sums[BLOCK_WAVES];
+  const Matrix M = matrix(a, blockIdx.x);
+  int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int mb = (int)blocks_of(M.m), nb = (int)blocks_of(M.n), count = M.m * M.n, cols = M.turned ? M.m : M.n;
+  char *const X = lds, *const P = lds + mb * nb * 4096, *const rest = P + mb * mb * 4096;
+  constexpr int THREADS = BLOCK_WAVES * 64;
+  for (int i = threadIdx.x * 16; i < mb * nb * 4096; i += THREADS * 16) *(f32x4 *)(X + i) = (f32x4){0.f, 0.f, 0.f, 0.f};
+  double s = 0.0;
+  for (int i = threadIdx.x * 4; i + 4 <= count; i += THREADS * 4) {
+    const f32x4 u = momentum<f32x4_any>(M.g + i, M.v ? M.v + i : nullptr, mu, nesterov, true);
+#pragma unroll
+    for (int j = 0; j < 4; j++) s = fma((double)u[j], (double)u[j], s);
+  }
+  const int tail = count / 4 * 4 + threadIdx.x;  // up to three more
+  if (tail < count) {
+    const float u = momentum<float>(M.g + tail, M.v ? M.v + tail : nullptr, mu, nesterov, true);
+    s = fma((double)u, (double)u, s);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  if (lane == 0) sums[wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int k = 0; k < BLOCK_WAVES; k++) s += sums[k];
+  const double scale = s == 0.0 ? 0.0 : (double)UP / sqrt(s);  // zeros stay zeros
+  auto place1 = [&](int i, float u) {
+    const int r = i / cols, c = i % cols, row = M.turned ? c : r, col = M.turned ? r : c;
+    _Float16 h, l;
+    split((float)((double)u * scale), h, l);
+    *(_Float16 *)(chunk_of(X, nb, row, col >> 5, col >> 3 & 3) + (col & 7) * 2) = h;
+    *(_Float16 *)(chunk_of(X, nb, row, col >> 5, 4 + (col >> 3 & 3)) + (col & 7) * 2) = l;
+  };
+  for (int i = threadIdx.x * 4; i + 4 <= count; i += THREADS * 4) {  // what this thread wrote itself
+    const f32x4 u = momentum<f32x4_any>(M.g + i, M.v ? M.v + i : nullptr, mu, nesterov, false);
+#pragma unroll
+    for (int j = 0; j < 4; j++) place1(i + j, u[j]);
+  }
+  if (tail < count) place1(tail, momentum<float>(M.g + tail, M.v ? M.v + tail : nullptr, mu, nesterov, false));
+
+  for (int step = 0;; step++) {
+    __syncthreads();
+    // the lane as the compiler does not know it from step to step: it would keep every
+    // address of the loop in registers, and spill them
+    asm volatile("" : "+v"(lane));
+    const int low = lane & 31, high = (lane >> 5) * 4;  // result i: values high + 8 (i / 4) + i % 4 of row low
+    // P = X X^T: with one block of it (four) eight waves (two) share the sum
+    const int pb = mb * mb, ways = mb == 1 ? 8 : mb == 2 ? 2 : 1;
+    {
+      const int f = wave % pb, way = wave / pb;
+      f32x16 acc = {};
+      if (way < ways) {
+#pragma unroll 1
+        for (int k = way; k < nb; k += ways)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            three(acc, along(X, nb, f / mb * 32, k, h, 0, lane), along(X, nb, f / mb * 32, k, h, 1, lane),
+                  along(X, nb, f % mb * 32, k, h, 0, lane), along(X, nb, f % mb * 32, k, h, 1, lane));
+        if (way > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            *(f32x4 *)(rest + (((way - 1) * pb + f) * 4 + i) * 1024 + lane * 16) =
+                (f32x4){acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
+        }
+      }
+      if (ways > 1) __syncthreads();
+      if (way == 0) {
+#pragma unroll 1
+        for (int w = 1; w < ways; w++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const f32x4 v = *(const f32x4 *)(rest + (((w - 1) * pb + f) * 4 + i) * 1024 + lane * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
+          }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x4 v = {acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
+          put4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i, v * DOWN2);
+        }
+      }
+    }
+    __syncthreads();
+    {  // Q = b P + c P P, in P's place
+      const bool on = wave < pb;
+      const int f = on ? wave : 0;
+      f32x16 acc = {};
+      f32x4 q[4];
+      if (on) {
+#pragma unroll 1
+        for (int k = 0; k < mb; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            three(acc, along(P, mb, f / mb * 32, k, h, 0, lane), along(P, mb, f / mb * 32, k, h, 1, lane),
+                  along(P, mb, f % mb * 32, k, h, 0, lane), along(P, mb, f % mb * 32, k, h, 1, lane));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x4 v = {acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
+          q[i] = get4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i) * TT_NS_B + v * (TT_NS_C * DOWN2);
+        }
+      }
+      __syncthreads();
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) put4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i, q[i]);
+      }
+    }
+    __syncthreads();
+    asm volatile("" : "+v"(lane));
+    // X^T <- a X^T + X^T Q: block f has the columns f % nb of X and its rows f / nb
+    f32x16 acc[BLOCK_KEEP] = {};
+#pragma unroll
+    for (int b = 0; b < BLOCK_KEEP; b++) {
+      const int f = wave + b * BLOCK_WAVES, r0 = f / nb * 32, cb = f % nb;
+      if (f >= mb * nb) continue;
+#pragma unroll 1
+      for (int k = 0; k < mb; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          three(acc[b], across(X, nb, k * 32 + h * 16, cb, 0, lane), across(X, nb, k * 32 + h * 16, cb, 1, lane),
+                along(P, mb, r0, k, h, 0, lane), along(P, mb, r0, k, h, 1, lane));
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 v = get4(X, nb, r0 + low, cb * 32 + high + 8 * i) * TT_NS_A;
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[b][i * 4 + j] = v[j] + acc[b][i * 4 + j] * DOWN2;
+      }
+    }
+    if (step + 1 == steps) {
+#pragma unroll
+      for (int b = 0; b < BLOCK_KEEP; b++) {
+        const int f = wave + b * BLOCK_WAVES, row = f / nb * 32 + low;
+        if (f >= mb * nb || row >= M.m) continue;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int col = f % nb * 32 + high + 8 * (i / 4) + i % 4;
+          if (col >= M.n) continue;
+          float *w = M.w + (M.turned ? col * M.m + row : row * M.n + col);
+          *w = M.v ? M.keep * *w + M.rate * acc[b][i] : acc[b][i];
+        }
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < BLOCK_KEEP; b++) {
+      const int f = wave + b * BLOCK_WAVES;
+      if (f >= mb * nb) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        put4(X, nb, f / nb * 32 + low, f % nb * 32 + high + 8 * i,
+             (f32x4){acc[b][i * 4], acc[b][i * 4 + 1], acc[b][i * 4 + 2], acc[b][i * 4 + 3]});
+    }
+  }
+}
+
 // ---------------------------------------------------------------- before the steps
 
 // v = mu v + g, and the sum of squares of u = g + mu v (nesterov) or v; without
@@ -83,7 +351,7 @@ __device__ __forceinline__ _Float16 *place(char *image, long blocks, long r, lon
 __global__ void __launch_bounds__(256) momentum_kernel(Matrices a, float mu, int nesterov) {
   __shared__ double sums[4];
   unsigned b = blockIdx.x;
-  const Matrix &M = a.at[matrix_of(a, b)];
+  const Matrix M = matrix_of(a, b);
   const long count = (long)M.m * M.n;
   double s = 0.0;
   for (long i = ((long)b * 256 + threadIdx.x) * 4; i < count; i += (long)M.parts * 1024) {
@@ -121,7 +389,7 @@ __global__ void __launch_bounds__(256) image_kernel(Matrices a, float mu, int ne
   __shared__ double sums[4];
   __shared__ float tile[64][65];
   unsigned b = blockIdx.x;
-  const Matrix &M = a.at[matrix_of(a, b)];
+  const Matrix M = matrix_of(a, b);
   const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n;
   double s = 0.0;
   for (int i = threadIdx.x; i < M.parts; i += 256) s += M.norm[i];
@@ -147,7 +415,7 @@ __global__ void __launch_bounds__(256) image_kernel(Matrices a, float mu, int ne
     tile[k * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)u * scale);
   }
   __syncthreads();
-  char *along = M.turned ? M.t[0] : M.x, *down = M.turned ? M.x : M.t[0];
+  char *along = M.turned ? M.t0 : M.x, *down = M.turned ? M.x : M.t0;
   const long row_blocks = blocks_of(cols), col_blocks = blocks_of(rows);
 #pragma unroll 4
   for (int k = 0; k < 16; k++) {
@@ -196,7 +464,7 @@ struct Operands {
       a = b = add = M.p, out = down = M.q;
       rows = cols = k = M.m, by = TT_NS_C, times = TT_NS_B;
     } else {
-      a = M.q, b = M.t[step & 1], add = M.x, out = M.x, down = M.t[~step & 1];
+      a = M.q, b = step & 1 ? M.t1 : M.t0, add = M.x, out = M.x, down = step & 1 ? M.t0 : M.t1;
       rows = k = M.m, cols = M.n, by = 1.f, times = TT_NS_A;
     }
   }
@@ -210,7 +478,7 @@ __global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
   constexpr int WAVES = 8;
   __shared__ float sums[WAVES][32][33];
   unsigned t = blockIdx.x;
-  const Matrix &M = a.at[matrix_of(a, t)];
+  const Matrix M = matrix_of(a, t);
   const Operands<KIND> o(M, step);
   int ti, tj;
   if (KIND <= SQUARE) {
@@ -473,38 +741,57 @@ __device__ __forceinline__ bool transposed(const Matrix &M, int ti, int tj) {
   return KIND <= SQUARE ? ti != tj : KIND == STEP || M.turned;
 }
 
-// the first unit of workgroup w's
-__device__ __forceinline__ unsigned long begins(unsigned long units, unsigned w, unsigned groups) {
-  return units * w / groups;
-}
+// How the units (tiles' blocks, tile by tile) are dealt: `rounds` whole tiles to every
+// workgroup, then the units from `base` on evenly to the first `sharers`.
+struct Deal {
+  unsigned rounds, sharers;
+  unsigned long base, units;
+  // the first of workgroup w's share
+  __device__ __forceinline__ unsigned long begins(unsigned w) const {
+    return base + (w < sharers ? units * w / sharers : units);
+  }
+};
 
 template <int KIND, int T>
-__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices a, int step, float *pieces) {
+__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices a, int step, Deal deal, float *pieces) {
   typedef Shape<T> S;
   __shared__ __attribute__((aligned(1024))) char lds[2 * S::BUFFER];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // consecutive workgroups go to the eight XCDs in turn: give each XCD a run of them
   const unsigned groups = gridDim.x, each = groups / 8, b = blockIdx.x;
   const unsigned w = b < each * 8 ? (b % 8) * each + b / 8 : b;
-  const unsigned long units = a.first[a.count], end = begins(units, w + 1, groups);
   const unsigned to = lds_address(lds);
-  for (unsigned long u = begins(units, w, groups); u < end;) {
+  unsigned round = 0;
+  for (unsigned long u = 0, end = 0;;) {
+    if (u == end) {
+      if (round < deal.rounds) {  // then all tiles have the same number of blocks
+        const Operands<KIND> o(a.at[0], step);
+        u = ((unsigned long)round * groups + w) * blocks_of(o.k);
+        end = u + blocks_of(o.k);
+      } else if (round == deal.rounds) {
+        u = deal.begins(w), end = deal.begins(w + 1);
+        if (u == end) return;
+      } else {
+        return;
+      }
+      round++;
+    }
     unsigned long in = u;
-    const Matrix &M = a.at[matrix_of(a, in)];
+    const Matrix M = matrix_of(a, in);
     const Operands<KIND> o(M, step);
     const long blocks = blocks_of(o.k);
     int ti, tj;
     tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
     const int k0 = (int)(in % blocks), k1 = (int)(end - u < (unsigned long)(blocks - k0) ? k0 + (end - u) : blocks);
-    // lane l brings 16 bytes of row 8 i + l / 8; where it puts them, l % 8 of the row's
-    // eight places, is where its (l % 8) ^ (l / 8) belong: rows then differ in their
-    // places, and the reads below meet no bank twice.  A row behind the last is the
-    // last once more: its results are not written.
+    // lane l brings 16 bytes of row r = 8 i + l / 8; where it puts them, l % 8 of the
+    // row's eight places, is where its (l % 8) ^ (r / 2 % 8) belong: the 16 lanes that
+    // the reads below serve at once then have a bank each.  A row behind the last is
+    // the last once more: its results are not written.
     constexpr int EACH = T / 8 / S::WAVES;
     unsigned off[2][EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-      const int r = (wave * EACH + i) * 8 + (lane >> 3), chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+      const int r = (wave * EACH + i) * 8 + (lane >> 3), chunk = ((lane & 7) ^ (r >> 1 & 7)) * 16;
       const int ra = ti * T + r < o.rows ? r : o.rows - 1 - ti * T, rb = tj * T + r < o.cols ? r : o.cols - 1 - tj * T;
       off[0][i] = (unsigned)(ra * blocks * 128) + chunk;
       off[1][i] = (unsigned)(rb * blocks * 128) + chunk;
@@ -531,7 +818,8 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices 
       if (k + 1 < n) bring(k + 1, to + (S::BUFFER - now));
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        const int ph = now + (((s * 2 + half) ^ (row & 7)) * 16), pl = now + (((s * 2 + half + 4) ^ (row & 7)) * 16);
+        const int ph = now + (((s * 2 + half) ^ (row >> 1 & 7)) * 16),
+                  pl = now + (((s * 2 + half + 4) ^ (row >> 1 & 7)) * 16);
         half8 ha[S::FI], la[S::FI], hb[2], lb[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -583,26 +871,26 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices 
   }
 }
 
-// Workgroups (w - 1, .) add the pieces of the tile in which the units of
-// tile_kernel's workgroup w begin, where that is the first to begin inside it; a
+// Workgroups (w - 1, .) add the pieces of the tile in which the share of
+// tile_kernel's workgroup w begins, where that is the first to begin inside it; a
 // wave has 32 x 32 of its values.
 template <int KIND, int T>
-__global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, const float *pieces, unsigned groups) {
+__global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, Deal deal, const float *pieces) {
   typedef Shape<T> S;
   __shared__ float buf[4][32][33];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned w = blockIdx.x + 1;
-  const unsigned long units = a.first[a.count], u = begins(units, w, groups);
+  const unsigned long u = deal.begins(w);
   unsigned long in = u;
-  const Matrix &M = a.at[matrix_of(a, in)];
+  const Matrix M = matrix_of(a, in);
   const Operands<KIND> o(M, step);
   const unsigned long blocks = blocks_of(o.k), k0 = in % blocks, first = u - k0, last = first + blocks;
-  if (k0 == 0 || begins(units, w - 1, groups) > first) return;
+  if (k0 == 0 || deal.begins(w - 1) > first) return;
   int ti, tj;
   tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
   const int block = blockIdx.y * 4 + wave;
   unsigned stop = w;  // the first workgroup behind the tile
-  while (stop < groups && begins(units, stop, groups) < last) stop++;
+  while (stop < deal.sharers && deal.begins(stop) < last) stop++;
   f32x16 acc = {};
   const f32x4 *p = (const f32x4 *)pieces + block * 256 + lane;
 #pragma unroll 4
@@ -623,7 +911,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, const f
 size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 bool good_sides(long rows, long cols) {
-  return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= 1L << 32;
+  return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= TT_MUON_MAX_VALUES;
 }
 
 size_t images_of(long rows, long cols) {
@@ -644,7 +932,8 @@ void lay(Matrix &M, long rows, long cols, char *&ws) {
     return p;
   };
   M.x = take((size_t)M.m * blocks_of(M.n) * 128);
-  for (int i = 0; i < 2; i++) M.t[i] = take((size_t)M.n * blocks_of(M.m) * 128);
+  M.t0 = take((size_t)M.n * blocks_of(M.m) * 128);
+  M.t1 = take((size_t)M.n * blocks_of(M.m) * 128);
   M.p = take((size_t)M.m * blocks_of(M.m) * 128);
   M.q = take((size_t)M.m * blocks_of(M.m) * 128);
   M.norm = (double *)take(sizeof(double) * NORM_PARTS);
@@ -653,18 +942,29 @@ void lay(Matrix &M, long rows, long cols, char *&ws) {
 template <class F>
 unsigned long number(Matrices &a, F workgroups) {
   unsigned long at = 0;
-  for (int i = 0; i < a.count; i++) {
+  const int kinds = a.alike ? 1 : a.count;
+  for (int i = 0; i < kinds; i++) {
     a.first[i] = at;
     at += (unsigned long)workgroups(a.at[i]);
   }
-  a.first[a.count] = at;
-  return at;
+  a.first[kinds] = at;
+  return a.alike ? at * a.count : at;
+}
+
+// Whether every matrix has a workgroup of its own.
+bool by_block(const Matrices &a) {
+  for (int i = 0; i < (a.alike ? 1 : a.count); i++)
+    if (!fits_block(a.at[i].m, a.at[i].n)) return false;
+  return !TT_NOBLOCK;
 }
 
 // How the products of such matrices go: by tiles of 32 (0), 128 or 256.
 int tile_size(const Matrices &a) {
   double work = 0;
-  for (int i = 0; i < a.count; i++) work += (double)a.at[i].m * a.at[i].m * a.at[i].n;
+  for (int i = 0; i < a.count; i++) {
+    const Matrix &M = a.at[a.alike ? 0 : i];
+    work += (double)M.m * M.m * M.n;
+  }
   return work < TT_LARGE ? 0 : work < TT_HUGE ? 128 : 256;
 }
 
@@ -679,19 +979,28 @@ void small_product(Matrices &a, int step) {
 template <int KIND, int T>
 void tile_product(Matrices &a, int step, float *pieces) {
   typedef Shape<T> S;
-  bool whole = true;
+  bool alike = true;  // in their blocks
   long blocks = 0;
-  const unsigned long units = number(a, [&](const Matrix &M) {
+  unsigned long tiles = 0;
+  Deal d = {};
+  d.units = number(a, [&](const Matrix &M) {
     const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T, k = blocks_of(KIND == GRAM ? M.n : M.m);
-    whole = whole && (!blocks || blocks == k);
+    alike = alike && (!blocks || blocks == k);
     blocks = k;
+    tiles += (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * (a.alike ? a.count : 1);
     return (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * k;
   });
-  const unsigned groups = (unsigned)(units < 8 * S::GROUPS ? (units + 7) / 8 : S::GROUPS);
-  hipLaunchKernelGGL((tile_kernel<KIND, T>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, pieces);
-  if (groups > 1 && (!whole || units % (groups * blocks)))  // else nobody has a piece
-    hipLaunchKernelGGL((join_kernel<KIND, T>), dim3(groups - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step,
-                       (const float *)pieces, groups);
+  const unsigned groups = (unsigned)(d.units < 8 * S::GROUPS ? (d.units + 7) / 8 : S::GROUPS);
+  if (alike) {  // whole tiles side by side read the same blocks at about the same time
+    d.rounds = (unsigned)(tiles / groups);
+    d.base = (unsigned long)d.rounds * groups * blocks;
+    d.units -= d.base;
+  }
+  d.sharers = (unsigned)(d.units < 8ul * groups ? (d.units + 7) / 8 : groups);
+  hipLaunchKernelGGL((tile_kernel<KIND, T>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
+  if (d.sharers > 1)
+    hipLaunchKernelGGL((join_kernel<KIND, T>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, d,
+                       (const float *)pieces);
 }
 
 template <int KIND>
@@ -702,6 +1011,10 @@ void product(Matrices &a, int step, int tile, float *pieces) {
 }
 
 void run(Matrices &a, int steps, float mu, int nesterov, char *rest) {
+  if (by_block(a)) {
+    hipLaunchKernelGGL(block_kernel, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov);
+    return;
+  }
   unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
   hipLaunchKernelGGL(momentum_kernel, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
@@ -715,21 +1028,29 @@ void run(Matrices &a, int steps, float mu, int nesterov, char *rest) {
   }
 }
 
-// the images of up to MOST matrices, and two pieces a workgroup
+// the images (of a group of matrices), and two pieces a workgroup
 size_t ws_of(const Matrices &a, size_t images) {
+  if (by_block(a)) return 0;
   const int t = tile_size(a);
   return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * (t == 128 ? Shape<128>::GROUPS : Shape<256>::GROUPS));
+}
+
+// `count` matrices of one shape
+void alike(Matrices &a, long count, long rows, long cols, char *ws) {
+  a = {};
+  a.count = (int)(count < ALIKE ? count : ALIKE);
+  a.alike = 1;
+  a.images = (long)images_of(rows, cols);
+  lay(a.at[0], rows, cols, ws);
 }
 
 }  // namespace
 
 extern "C" size_t tt_k_newton_schulz_ws(long count, long rows, long cols) {
   if (count <= 0 || !good_sides(rows, cols)) return 0;
-  Matrices a = {};
-  a.count = (int)(count < MOST ? count : MOST);
-  char *at = NULL;
-  for (int i = 0; i < a.count; i++) lay(a.at[i], rows, cols, at);
-  return ws_of(a, a.count * images_of(rows, cols));
+  Matrices a;
+  alike(a, count, rows, cols, NULL);
+  return ws_of(a, a.count * (size_t)a.images);
 }
 
 extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps, void *ws) {
@@ -737,19 +1058,20 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
       steps > TT_NS_MAX_STEPS)
     return -1;
   if (ttrt_init() != 0) return -3;
+  const size_t need = tt_k_newton_schulz_ws(count, rows, cols);
   void *own = NULL;
-  if (!ws) ws = own = ttrt_alloc(tt_k_newton_schulz_ws(count, rows, cols));
-  if (!ws) return -2;
-  for (long base = 0; base < count; base += MOST) {
-    Matrices a = {};
-    a.count = (int)(count - base < MOST ? count - base : MOST);
-    char *at = (char *)ws;
-    for (int i = 0; i < a.count; i++) {
-      a.at[i].g = x + (base + i) * rows * cols;
-      a.at[i].w = y + (base + i) * rows * cols;
-      lay(a.at[i], rows, cols, at);
-    }
-    run(a, steps, 0.f, 0, at);
+  if (need && !ws) {
+    ws = own = ttrt_alloc(need);
+    if (!ws) return -2;
+  }
+  Matrices a;
+  alike(a, count, rows, cols, (char *)ws);
+  const int most = by_block(a) ? 1 << 20 : a.count;  // without images any number at once
+  for (long base = 0; base < count; base += most) {
+    a.count = (int)(count - base < most ? count - base : most);
+    a.at[0].g = x + base * rows * cols;
+    a.at[0].w = y + base * rows * cols;
+    run(a, steps, 0.f, 0, (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images);
   }
   ttrt_free(own);
   return launched();
@@ -781,9 +1103,12 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
   }
   if (count == 0) return 0;
   if (ttrt_init() != 0) return -3;
+  const size_t need = tt_k_muon_multi_ws(rows, cols, count);
   void *own = NULL;
-  if (!ws) ws = own = ttrt_alloc(tt_k_muon_multi_ws(rows, cols, count));
-  if (!ws) return -2;
+  if (need && !ws) {
+    ws = own = ttrt_alloc(need);
+    if (!ws) return -2;
+  }
   Matrices a = {};
   a.count = count;
   char *at = (char *)ws;
