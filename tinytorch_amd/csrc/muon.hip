@@ -17,9 +17,13 @@
 // are within 1.21, 1.46 and 2.81 (46100 of 65504 times 2^14), and l is exact to
 // 2^-38.
 //
-// X, X^T, P and Q are kept as images: rows of blocks of 32 values, a block the 32
-// h and then the 32 l, 128 bytes, with zeros behind the last value.  Both operands
-// of a product are read along rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
+// X, X^T, P and Q are kept as images: blocks of 32 x 32 values as the matrix
+// instructions take them, four times 1 KB: h of the columns 0 to 15, where lane l
+// has eight of row l % 32 from column 8 (l / 32) on, of the columns 16 to 31, and l
+// of both; zeros behind the last row and column.  A wave's load is then 1 KB in one
+// piece (rows of 128 bytes, 32 of them a load, take the address unit 40 cycles: 16 x
+// 4000 20 us a product instead of 6).  Both operands of a product are read along
+// rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -54,19 +58,22 @@ struct Matrix {
   int turned;       // more rows than columns: X is U^T
   int parts;        // of the norm
 };
+// N matrices, or with N = 1 `count` of at[0]'s shape one behind the other.  (A kernel's
+// arguments come from afar: of the longer form each line that it needs costs it 0.5 us.)
+template <int N>
 struct Matrices {
-  Matrix at[MOST];
-  unsigned long first[MOST + 1];  // matrix i has the workgroups, or the units of work, [first[i], first[i + 1])
+  Matrix at[N];
+  unsigned long first[N + 1];  // matrix i has the workgroups, or the units of work, [first[i], first[i + 1])
   int count;
-  int alike;       // all are at[0]'s shape: matrix i lies behind it by i times
-  long images;     // bytes of the workspace
+  long images;  // N = 1: bytes of a matrix's workspace
 };
 
 __host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
 
 // which matrix a workgroup or unit belongs to; b becomes its number among that one's
-__device__ __forceinline__ Matrix matrix(const Matrices &a, int i) {
-  if (!a.alike) return a.at[i];
+template <int N>
+__device__ __forceinline__ Matrix matrix(const Matrices<N> &a, int i) {
+  if (N > 1) return a.at[i];
   Matrix M = a.at[0];
   M.g += (long)i * M.m * M.n, M.w += (long)i * M.m * M.n;
   const long off = i * a.images;
@@ -74,15 +81,15 @@ __device__ __forceinline__ Matrix matrix(const Matrices &a, int i) {
   M.norm += off / (long)sizeof(double);
   return M;
 }
-template <class N>
-__device__ __forceinline__ Matrix matrix_of(const Matrices &a, N &b) {
+template <int N, class U>
+__device__ __forceinline__ Matrix matrix_of(const Matrices<N> &a, U &b) {
   int i = 0;
-  if (a.alike) {
-    i = (int)(b / (N)a.first[1]);
-    b -= (N)i * (N)a.first[1];
-  } else {
+  if (N > 1) {
     while (i + 1 < a.count && b >= a.first[i + 1]) i++;
-    b -= (N)a.first[i];
+    b -= (U)a.first[i];
+  } else if (a.count > 1) {
+    i = (int)(b / (U)a.first[1]);
+    b -= (U)i * (U)a.first[1];
   }
   return matrix(a, i);
 }
@@ -92,8 +99,37 @@ __device__ __forceinline__ void split(float y, _Float16 &h, _Float16 &l) {
   h = (_Float16)y;
   l = (_Float16)(y - (float)h);
 }
-__device__ __forceinline__ _Float16 *place(char *image, long blocks, long r, long c) {
-  return (_Float16 *)(image + (r * blocks + (c >> 5)) * 128) + (c & 31);
+// where h of row r and column c of an image lies (l 1024 values further)
+__device__ __forceinline__ _Float16 *place(char *image, long blocks, int r, int c) {
+  return (_Float16 *)(image + ((r >> 5) * blocks + (c >> 5)) * 4096 + (c >> 4 & 1) * 1024 +
+                      ((r & 31) + (c >> 3 & 1) * 32) * 16) +
+         (c & 7);
+}
+// two values of row r from the even column c on
+__device__ __forceinline__ void put2(char *image, long blocks, int r, int c, float x, float y) {
+  typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+  half2 h, l;
+  _Float16 a, b;
+  split(x * UP, a, b);
+  h[0] = a, l[0] = b;
+  split(y * UP, a, b);
+  h[1] = a, l[1] = b;
+  _Float16 *p = place(image, blocks, r, c);
+  *(half2 *)p = h;
+  *(half2 *)(p + 1024) = l;
+}
+// 16 values (times 2^14 already) of row r from column c on, a multiple of 16
+__device__ __forceinline__ void put16(char *image, long blocks, int r, int c, const float (&v)[16]) {
+  half8 h[2], l[2];
+#pragma unroll
+  for (int j = 0; j < 16; j++) {
+    _Float16 a, b;
+    split(v[j], a, b);
+    h[j / 8][j % 8] = a;
+    l[j / 8][j % 8] = b;
+  }
+  half8 *p = (half8 *)place(image, blocks, r, c);
+  p[0] = h[0], p[32] = h[1], p[128] = l[0], p[160] = l[1];
 }
 
 // ---------------------------------------------------------------- small matrices
@@ -185,7 +221,8 @@ __device__ __forceinline__ V momentum(const float *g, float *v, float mu, int ne
   return nesterov ? w * mu + u : w;
 }
 
-__global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices a, int steps, float mu, int nesterov) {
+template <int N>
+__global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices<N> a, int steps, float mu, int nesterov) {
   __shared__ __attribute__((aligned(1024))) char lds[BLOCK_LDS];
   __shared__ double sums[BLOCK_WAVES];
   const Matrix M = matrix(a, blockIdx.x);
@@ -348,33 +385,30 @@ __global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices a, int
 
 // v = mu v + g, and the sum of squares of u = g + mu v (nesterov) or v; without
 // momenta of g.  In 64 bits: the squares of any fp32 values are within its range.
-__global__ void __launch_bounds__(256) momentum_kernel(Matrices a, float mu, int nesterov) {
+template <int N>
+__global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, int nesterov) {
   __shared__ double sums[4];
   unsigned b = blockIdx.x;
   const Matrix M = matrix_of(a, b);
-  const long count = (long)M.m * M.n;
+  const long count = (long)M.m * M.n, groups = count / 4;
   double s = 0.0;
-  for (long i = ((long)b * 256 + threadIdx.x) * 4; i < count; i += (long)M.parts * 1024) {
-    if (i + 4 <= count) {
-      f32x4 u = *(const f32x4_any *)(M.g + i);
-      if (M.v) {
-        const f32x4 v = *(const f32x4_any *)(M.v + i) * mu + u;
-        *(f32x4_any *)(M.v + i) = v;
-        u = nesterov ? v * mu + u : v;
-      }
+  for (long i = (long)b * 512 + threadIdx.x; i < groups; i += (long)M.parts * 512) {
+    f32x4 u[2];
 #pragma unroll
-      for (int j = 0; j < 4; j++) s = fma((double)u[j], (double)u[j], s);
-    } else {
-      for (long j = i; j < count; j++) {
-        float u = M.g[j];
-        if (M.v) {
-          const float v = M.v[j] * mu + u;
-          M.v[j] = v;
-          u = nesterov ? v * mu + u : v;
-        }
-        s = fma((double)u, (double)u, s);
-      }
+    for (int k = 0; k < 2; k++) {
+      u[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      const long at = (i + k * 256) * 4;
+      if (i + k * 256 < groups) u[k] = momentum<f32x4_any>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, true);
     }
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) s = fma((double)u[k][j], (double)u[k][j], s);
+  }
+  const long tail = groups * 4 + threadIdx.x;  // up to three more
+  if (b == 0 && tail < count) {
+    const float u = momentum<float>(M.g + tail, M.v ? M.v + tail : nullptr, mu, nesterov, true);
+    s = fma((double)u, (double)u, s);
   }
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
@@ -385,54 +419,49 @@ __global__ void __launch_bounds__(256) momentum_kernel(Matrices a, float mu, int
 
 // The images of U / |U|_F and its transpose, a tile of 64 x 64 at a time through
 // LDS; both are written along their rows.
-__global__ void __launch_bounds__(256) image_kernel(Matrices a, float mu, int nesterov) {
+template <int N>
+__global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int nesterov) {
   __shared__ double sums[4];
   __shared__ float tile[64][65];
   unsigned b = blockIdx.x;
   const Matrix M = matrix_of(a, b);
-  const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n;
+  const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned across = (unsigned)((cols + 63) / 64);
+  const int r0 = (int)(b / across) * 64, c0 = (int)(b % across) * 64;
+  float u[16];  // on their way while the norm is added up
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    const int r = r0 + k * 4 + wave, c = c0 + lane;
+    u[k] = 0.f;
+    if (r < rows && c < cols) {
+      const long at = (long)r * cols + c;
+      u[k] = momentum<float>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, false);
+    }
+  }
   double s = 0.0;
   for (int i = threadIdx.x; i < M.parts; i += 256) s += M.norm[i];
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  if (lane == 0) sums[wave] = s;
   __syncthreads();
   s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   const double scale = s == 0.0 ? 0.0 : (double)UP / sqrt(s);  // zeros stay zeros
-  const unsigned across = (unsigned)((cols + 63) / 64);
-  const long r0 = (long)(b / across) * 64, c0 = (long)(b % across) * 64;
-#pragma unroll 4
-  for (int k = 0; k < 16; k++) {
-    const long r = r0 + k * 4 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63);
-    float u = 0.f;
-    if (r < rows && c < cols) {
-      u = M.g[r * cols + c];
-      if (M.v) {
-        const float v = M.v[r * cols + c];
-        u = nesterov ? v * mu + u : v;
-      }
-    }
-    tile[k * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)u * scale);
-  }
+#pragma unroll
+  for (int k = 0; k < 16; k++) tile[k * 4 + wave][lane] = (float)((double)u[k] * scale);
   __syncthreads();
   char *along = M.turned ? M.t0 : M.x, *down = M.turned ? M.x : M.t0;
   const long row_blocks = blocks_of(cols), col_blocks = blocks_of(rows);
-#pragma unroll 4
-  for (int k = 0; k < 16; k++) {
-    const int i = k * 4 + (threadIdx.x >> 6), j = threadIdx.x & 63;
-    _Float16 h, l;
-    if (r0 + i < rows && c0 + j < row_blocks * 32) {
-      split(tile[i][j], h, l);
-      _Float16 *p = place(along, row_blocks, r0 + i, c0 + j);
-      p[0] = h;
-      p[32] = l;
-    }
-    if (c0 + i < cols && r0 + j < col_blocks * 32) {
-      split(tile[j][i], h, l);
-      _Float16 *p = place(down, col_blocks, c0 + i, r0 + j);
-      p[0] = h;
-      p[32] = l;
-    }
+  const int line = threadIdx.x >> 2, from = (threadIdx.x & 3) * 16;  // 16 values of a row, then of a column
+  float v[16];
+  if ((r0 + line) / 32 < col_blocks && (c0 + from) / 32 < row_blocks) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = tile[line][from + j];
+    put16(along, row_blocks, r0 + line, c0 + from, v);
+  }
+  if ((c0 + line) / 32 < row_blocks && (r0 + from) / 32 < col_blocks) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = tile[from + j][line];
+    put16(down, col_blocks, c0 + line, r0 + from, v);
   }
 }
 
@@ -472,9 +501,12 @@ struct Operands {
 
 // Tiles of 32 x 32, one a workgroup, the operands read from memory as the matrix
 // instructions take them and each wave with a share of the products' length:
-// eight sums, joined in LDS.
-template <int KIND>
-__global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
+// eight sums, joined in LDS.  What bounds these is the way from memory (the L2 of
+// another XCD has what the last launch wrote), so the added matrix is on its way
+// first, and a tile on the diagonal reads its rows once.
+template <int KIND, int N>
+__global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) {
+  typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   constexpr int WAVES = 8;
   __shared__ float sums[WAVES][32][33];
   unsigned t = blockIdx.x;
@@ -488,84 +520,70 @@ __global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
     ti = (int)(t / across), tj = (int)(t % across);
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long blocks = blocks_of(o.k);
-  // a row behind the last is the last once more: its results are not written
-  const int ra = ti * 32 + (lane & 31), rb = tj * 32 + (lane & 31);
-  const char *pa = o.a + (ra < o.rows ? ra : o.rows - 1) * blocks * 128 + (lane >> 5) * 16;
-  const char *pb = o.b + (rb < o.cols ? rb : o.cols - 1) * blocks * 128 + (lane >> 5) * 16;
+  const int r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 2;  // this thread's two results
+  const int row = ti * 32 + r, col = tj * 32 + c;
+  float v[2] = {0.f, 0.f};
+  if (KIND != GRAM) {
+    const _Float16 *p = place((char *)o.add, blocks_of(o.cols), row, col);
+    const half2 h = *(const half2 *)p, l = *(const half2 *)(p + 1024);
+#pragma unroll
+    for (int e = 0; e < 2; e++) v[e] = o.times * (1.f / UP) * ((float)h[e] + (float)l[e]);
+  }
+  const int blocks = (int)blocks_of(o.k);
+  const char *pa = o.a + (long)ti * blocks * 4096 + lane * 16, *pb = o.b + (long)tj * blocks * 4096 + lane * 16;
   f32x16 acc = {};
-#pragma unroll 2
-  for (long k = wave; k < blocks; k += WAVES) {
-    half8 ha[2], la[2], hb[2], lb[2];
+  const bool same = KIND <= SQUARE && ti == tj;
+  for (int k = wave; k < blocks; k += WAVES) {
+    half8 x[4], y[4];
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      ha[s] = *(const half8 *)(pa + k * 128 + s * 32);
-      la[s] = *(const half8 *)(pa + k * 128 + s * 32 + 64);
-      hb[s] = *(const half8 *)(pb + k * 128 + s * 32);
-      lb[s] = *(const half8 *)(pb + k * 128 + s * 32 + 64);
+    for (int s = 0; s < 4; s++) {
+      x[s] = *(const half8 *)(pa + k * 4096l + s * 1024);
+      y[s] = x[s];
+    }
+    if (!same) {
+#pragma unroll
+      for (int s = 0; s < 4; s++) y[s] = *(const half8 *)(pb + k * 4096l + s * 1024);
     }
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(la[s], hb[s], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[s], lb[s], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[s], hb[s], acc, 0, 0, 0);
-    }
+    for (int s = 0; s < 2; s++) three(acc, x[s], x[2 + s], y[s], y[2 + s]);
   }
 #pragma unroll
   for (int i = 0; i < 16; i++) sums[wave][8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
   __syncthreads();
-  const int r = threadIdx.x >> 5, c = threadIdx.x & 31;  // and row r + 16
-  float v[2];
+  bool in[2];
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    const int i = r + e * 16, row = ti * 32 + i, col = tj * 32 + c;
+    in[e] = row < o.rows && col + e < o.cols;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) s += sums[w][i][c];
-    s *= o.by * DOWN2;
-    if (KIND != GRAM && row < o.rows && col < o.cols) {
-      const _Float16 *p = place((char *)o.add, blocks_of(o.cols), row, col);
-      s += o.times * (1.f / UP) * ((float)p[0] + (float)p[32]);
-    }
-    v[e] = s;
+    for (int w = 0; w < WAVES; w++) s += sums[w][r][c + e];
+    v[e] = in[e] ? v[e] + s * (o.by * DOWN2) : 0.f;
   }
-  __syncthreads();
+  if (KIND == LAST) {
 #pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const int i = r + e * 16, row = ti * 32 + i, col = tj * 32 + c;
-    const bool in = row < o.rows && col < o.cols;
-    if (KIND == LAST) {
-      if (in && !M.turned) {
-        float *w = M.w + (long)row * o.cols + col;
+    for (int e = 0; e < 2; e++)
+      if (in[e] && !M.turned) {
+        float *w = M.w + (long)row * o.cols + col + e;
         *w = M.v ? M.keep * *w + M.rate * v[e] : v[e];
       }
-    } else if (row < o.rows) {
-      _Float16 h, l;
-      split(in ? v[e] * UP : 0.f, h, l);
-      _Float16 *p = place(o.out, blocks_of(o.cols), row, col);
-      p[0] = h;
-      p[32] = l;
-    }
-    sums[0][i][c] = in ? v[e] : 0.f;
+  } else {
+    put2(o.out, blocks_of(o.cols), row, col, v[0], v[1]);
   }
   if ((KIND <= SQUARE && ti == tj) || (KIND == LAST && !M.turned)) return;
   __syncthreads();
+  sums[0][r][c] = v[0];
+  sums[0][r][c + 1] = v[1];
+  __syncthreads();
+  const int trow = tj * 32 + r, tcol = ti * 32 + c;  // the transpose
+  if (KIND == LAST) {
 #pragma unroll
-  for (int e = 0; e < 2; e++) {  // the transpose
-    const int i = r + e * 16, row = ti * 32 + c, col = tj * 32 + i;
-    if (col >= o.cols) continue;
-    if (KIND == LAST) {
-      if (row < o.rows) {
-        float *w = M.w + (long)col * o.rows + row;
-        *w = M.v ? M.keep * *w + M.rate * sums[0][c][i] : sums[0][c][i];
+    for (int e = 0; e < 2; e++)
+      if (trow < o.cols && tcol + e < o.rows) {
+        float *w = M.w + (long)trow * o.rows + tcol + e;
+        *w = M.v ? M.keep * *w + M.rate * sums[0][c + e][r] : sums[0][c + e][r];
       }
-    } else {
-      _Float16 h, l;
-      split(sums[0][c][i] * UP, h, l);
-      _Float16 *p = place(o.down, blocks_of(o.rows), col, row);
-      p[0] = h;
-      p[32] = l;
-    }
+  } else {
+    put2(o.down, blocks_of(o.rows), trow, tcol, sums[0][c][r], sums[0][c + 1][r]);
   }
 }
 
@@ -580,7 +598,7 @@ __global__ void __launch_bounds__(512) small_kernel(Matrices a, int step) {
 // that others have the rest of.  Pieces go to memory, and join_kernel adds them.
 
 #ifndef TT_LARGE
-#define TT_LARGE 8e8
+#define TT_LARGE 3.5e9
 #endif
 #ifndef TT_HUGE
 #define TT_HUGE 1.7e10
@@ -642,7 +660,7 @@ __device__ __forceinline__ void tile_of(unsigned long tile, int rows, int cols, 
 // they go: through LDS, so that a lane has 16 of a row (and, for the transpose, of a
 // column) and lines are written whole.
 template <int KIND>
-__device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, long r0, long c0,
+__device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, int r0, int c0,
                                         float (*buf)[33], int lane, bool transpose) {
 #pragma unroll
   for (int i = 0; i < 16; i++) buf[8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
@@ -651,10 +669,12 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
   float v[16];
 #pragma unroll
   for (int j = 0; j < 16; j++) v[j] = buf[line][from + j] * (o.by * DOWN2);
-  const long row = r0 + line, col = c0 + from, blocks = blocks_of(o.cols);
-  if (KIND != GRAM && row < o.rows && c0 < o.cols) {
+  const int row = r0 + line, col = c0 + from;
+  const long blocks = blocks_of(o.cols);
+  if (r0 >= o.rows || c0 >= o.cols) return;
+  if (KIND != GRAM) {
     const half8 *p = (const half8 *)place((char *)o.add, blocks, row, col);
-    const half8 h[2] = {p[0], p[1]}, l[2] = {p[4], p[5]};
+    const half8 h[2] = {p[0], p[32]}, l[2] = {p[128], p[160]};
 #pragma unroll
     for (int j = 0; j < 16; j++) v[j] += o.times * (1.f / UP) * ((float)h[j / 8][j % 8] + (float)l[j / 8][j % 8]);
   }
@@ -667,7 +687,7 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
   }
   if (KIND == LAST) {
     if (!transpose && row < o.rows) {
-      float *w = M.w + row * o.cols + col;
+      float *w = M.w + (long)row * o.cols + col;
       if (col + 16 <= o.cols) {
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -681,26 +701,20 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
           if (col + j < o.cols) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
       }
     }
-  } else if (row < o.rows && c0 < o.cols) {
-    half8 h[2], l[2];
+  } else {
+    float up[16];
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-      _Float16 a, b;
-      split(v[j] * UP, a, b);
-      h[j / 8][j % 8] = a;
-      l[j / 8][j % 8] = b;
-    }
-    half8 *p = (half8 *)place(o.out, blocks, row, col);
-    p[0] = h[0], p[1] = h[1], p[4] = l[0], p[5] = l[1];
+    for (int j = 0; j < 16; j++) up[j] = v[j] * UP;
+    put16(o.out, blocks, row, col, up);
   }
   if (!transpose) return;
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int j = 0; j < 16; j++) v[j] = buf[from + j][line];
-  const long trow = c0 + line, tcol = r0 + from;
-  if (trow >= o.cols) return;
+  const int trow = c0 + line, tcol = r0 + from;
   if (KIND == LAST) {
-    float *w = M.w + trow * o.rows + tcol;
+    if (trow >= o.cols) return;
+    float *w = M.w + (long)trow * o.rows + tcol;
     if (tcol + 16 <= o.rows) {
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
@@ -713,28 +727,21 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
       for (int j = 0; j < 16; j++)
         if (tcol + j < o.rows) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
     }
-  } else if (r0 < o.rows) {
-    half8 h[2], l[2];
+  } else {
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-      _Float16 a, b;
-      split(v[j] * UP, a, b);
-      h[j / 8][j % 8] = a;
-      l[j / 8][j % 8] = b;
-    }
-    half8 *p = (half8 *)place(o.down, blocks_of(o.rows), trow, tcol);
-    p[0] = h[0], p[1] = h[1], p[4] = l[0], p[5] = l[1];
+    for (int j = 0; j < 16; j++) v[j] *= UP;
+    put16(o.down, blocks_of(o.rows), trow, tcol, v);
   }
 }
 
 // where the 32 x 32 block f of a wave's lies
 template <int T>
-__device__ __forceinline__ long row_of(int ti, int wave, int f) {
-  return (long)ti * T + (wave / Shape<T>::ACROSS) * (T / 2) + f / 2 * 32;
+__device__ __forceinline__ int row_of(int ti, int wave, int f) {
+  return ti * T + (wave / Shape<T>::ACROSS) * (T / 2) + f / 2 * 32;
 }
 template <int T>
-__device__ __forceinline__ long col_of(int tj, int wave, int f) {
-  return (long)tj * T + (wave % Shape<T>::ACROSS) * 64 + f % 2 * 32;
+__device__ __forceinline__ int col_of(int tj, int wave, int f) {
+  return tj * T + (wave % Shape<T>::ACROSS) * 64 + f % 2 * 32;
 }
 template <int KIND>
 __device__ __forceinline__ bool transposed(const Matrix &M, int ti, int tj) {
@@ -752,8 +759,8 @@ struct Deal {
   }
 };
 
-template <int KIND, int T>
-__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices a, int step, Deal deal, float *pieces) {
+template <int KIND, int T, int N>
+__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<N> a, int step, Deal deal, float *pieces) {
   typedef Shape<T> S;
   __shared__ __attribute__((aligned(1024))) char lds[2 * S::BUFFER];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -783,34 +790,31 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices 
     int ti, tj;
     tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
     const int k0 = (int)(in % blocks), k1 = (int)(end - u < (unsigned long)(blocks - k0) ? k0 + (end - u) : blocks);
-    // lane l brings 16 bytes of row r = 8 i + l / 8; where it puts them, l % 8 of the
-    // row's eight places, is where its (l % 8) ^ (r / 2 % 8) belong: the 16 lanes that
-    // the reads below serve at once then have a bank each.  A row behind the last is
-    // the last once more: its results are not written.
+    // a wave brings every WAVES-th KB of the tiles' T / 32 blocks; a block behind the
+    // last is the last once more: its results are not written
     constexpr int EACH = T / 8 / S::WAVES;
     unsigned off[2][EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-      const int r = (wave * EACH + i) * 8 + (lane >> 3), chunk = ((lane & 7) ^ (r >> 1 & 7)) * 16;
-      const int ra = ti * T + r < o.rows ? r : o.rows - 1 - ti * T, rb = tj * T + r < o.cols ? r : o.cols - 1 - tj * T;
-      off[0][i] = (unsigned)(ra * blocks * 128) + chunk;
-      off[1][i] = (unsigned)(rb * blocks * 128) + chunk;
+      const int kb = wave * EACH + i, ra = (o.rows - 1) / 32 - ti * (T / 32), rb = (o.cols - 1) / 32 - tj * (T / 32);
+      off[0][i] = (unsigned)((kb / 4 < ra ? kb / 4 : ra) * blocks * 4096) + kb % 4 * 1024 + lane * 16;
+      off[1][i] = (unsigned)((kb / 4 < rb ? kb / 4 : rb) * blocks * 4096) + kb % 4 * 1024 + lane * 16;
     }
-    const char *pa = scalar(o.a + ((long)ti * T * blocks + k0) * 128);
-    const char *pb = scalar(o.b + ((long)tj * T * blocks + k0) * 128);
+    const char *pa = scalar(o.a + ((long)ti * (T / 32) * blocks + k0) * 4096);
+    const char *pb = scalar(o.b + ((long)tj * (T / 32) * blocks + k0) * 4096);
     auto bring = [&](int k, unsigned at) {
 #pragma unroll
-      for (int i = 0; i < EACH; i++) dma16(pa + (long)k * 128, off[0][i], at + (wave * EACH + i) * 1024);
+      for (int i = 0; i < EACH; i++) dma16(pa + (long)k * 4096, off[0][i], at + (wave * EACH + i) * 1024);
 #pragma unroll
-      for (int i = 0; i < EACH; i++) dma16(pb + (long)k * 128, off[1][i], at + T * 128 + (wave * EACH + i) * 1024);
+      for (int i = 0; i < EACH; i++) dma16(pb + (long)k * 4096, off[1][i], at + T * 128 + (wave * EACH + i) * 1024);
     };
     f32x16 acc[S::FI][2] = {};
     __syncthreads();  // the last tile's LDS is read
     bring(0, to);
-    const int n = k1 - k0, row = lane & 31, half = lane >> 5;
-    // the wave's rows of either operand in a buffer
-    const char *mine[2] = {lds + ((wave / S::ACROSS) * (T / 2) + row) * 128,
-                           lds + (T + (wave % S::ACROSS) * 64 + row) * 128};
+    const int n = k1 - k0;
+    // the wave's blocks of either operand in a buffer
+    const char *mine[2] = {lds + (wave / S::ACROSS) * (T / 2) * 128 + lane * 16,
+                           lds + (T + (wave % S::ACROSS) * 64) * 128 + lane * 16};
     for (int k = 0; k < n; k++) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
@@ -818,8 +822,7 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices 
       if (k + 1 < n) bring(k + 1, to + (S::BUFFER - now));
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        const int ph = now + (((s * 2 + half) ^ (row >> 1 & 7)) * 16),
-                  pl = now + (((s * 2 + half + 4) ^ (row >> 1 & 7)) * 16);
+        const int ph = now + s * 1024, pl = ph + 2048;
         half8 ha[S::FI], la[S::FI], hb[2], lb[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -874,8 +877,8 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices 
 // Workgroups (w - 1, .) add the pieces of the tile in which the share of
 // tile_kernel's workgroup w begins, where that is the first to begin inside it; a
 // wave has 32 x 32 of its values.
-template <int KIND, int T>
-__global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, Deal deal, const float *pieces) {
+template <int KIND, int T, int N>
+__global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal deal, const float *pieces) {
   typedef Shape<T> S;
   __shared__ float buf[4][32][33];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -908,76 +911,77 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices a, int step, Deal de
 
 // ---------------------------------------------------------------- host
 
-size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
-
 bool good_sides(long rows, long cols) {
   return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= TT_MUON_MAX_VALUES;
 }
 
 size_t images_of(long rows, long cols) {
   const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-  return up((size_t)m * blocks_of((int)n) * 128) + 2 * up((size_t)n * blocks_of((int)m) * 128) +
-         2 * up((size_t)m * blocks_of((int)m) * 128) + up(sizeof(double) * NORM_PARTS);
+  const size_t mb = blocks_of((int)m), nb = blocks_of((int)n);
+  return 4096 * (3 * mb * nb + 2 * mb * mb) + sizeof(double) * NORM_PARTS;
 }
 
 void lay(Matrix &M, long rows, long cols, char *&ws) {
   M.turned = rows > cols;
   M.m = (int)(M.turned ? cols : rows);
   M.n = (int)(M.turned ? rows : cols);
-  const long parts = ((long)M.m * M.n + 8191) / 8192;
+  const long parts = ((long)M.m * M.n + 2047) / 2048;
   M.parts = (int)(parts < NORM_PARTS ? parts : NORM_PARTS);
+  const size_t mb = blocks_of(M.m), nb = blocks_of(M.n);
   auto take = [&](size_t bytes) {
     char *p = ws;
-    ws += up(bytes);
+    ws += bytes;
     return p;
   };
-  M.x = take((size_t)M.m * blocks_of(M.n) * 128);
-  M.t0 = take((size_t)M.n * blocks_of(M.m) * 128);
-  M.t1 = take((size_t)M.n * blocks_of(M.m) * 128);
-  M.p = take((size_t)M.m * blocks_of(M.m) * 128);
-  M.q = take((size_t)M.m * blocks_of(M.m) * 128);
+  M.x = take(4096 * mb * nb);
+  M.t0 = take(4096 * mb * nb);
+  M.t1 = take(4096 * mb * nb);
+  M.p = take(4096 * mb * mb);
+  M.q = take(4096 * mb * mb);
   M.norm = (double *)take(sizeof(double) * NORM_PARTS);
 }
 
-template <class F>
-unsigned long number(Matrices &a, F workgroups) {
+template <int N, class F>
+unsigned long number(Matrices<N> &a, F workgroups) {
   unsigned long at = 0;
-  const int kinds = a.alike ? 1 : a.count;
+  const int kinds = N > 1 ? a.count : 1;
   for (int i = 0; i < kinds; i++) {
     a.first[i] = at;
     at += (unsigned long)workgroups(a.at[i]);
   }
   a.first[kinds] = at;
-  return a.alike ? at * a.count : at;
+  return N > 1 ? at : at * a.count;
 }
 
 // Whether every matrix has a workgroup of its own.
-bool by_block(const Matrices &a) {
-  for (int i = 0; i < (a.alike ? 1 : a.count); i++)
+template <int N>
+bool by_block(const Matrices<N> &a) {
+  for (int i = 0; i < (N > 1 ? a.count : 1); i++)
     if (!fits_block(a.at[i].m, a.at[i].n)) return false;
   return !TT_NOBLOCK;
 }
 
 // How the products of such matrices go: by tiles of 32 (0), 128 or 256.
-int tile_size(const Matrices &a) {
+template <int N>
+int tile_size(const Matrices<N> &a) {
   double work = 0;
   for (int i = 0; i < a.count; i++) {
-    const Matrix &M = a.at[a.alike ? 0 : i];
+    const Matrix &M = a.at[N > 1 ? i : 0];
     work += (double)M.m * M.m * M.n;
   }
   return work < TT_LARGE ? 0 : work < TT_HUGE ? 128 : 256;
 }
 
-template <int KIND>
-void small_product(Matrices &a, int step) {
+template <int KIND, int N>
+void small_product(Matrices<N> &a, int step) {
   const unsigned long grid = number(a, [](const Matrix &M) {
     return KIND <= SQUARE ? blocks_of(M.m) * (blocks_of(M.m) + 1) / 2 : blocks_of(M.m) * blocks_of(M.n);
   });
-  hipLaunchKernelGGL(small_kernel<KIND>, dim3((unsigned)grid), dim3(512), 0, stream(), a, step);
+  hipLaunchKernelGGL((small_kernel<KIND, N>), dim3((unsigned)grid), dim3(512), 0, stream(), a, step);
 }
 
-template <int KIND, int T>
-void tile_product(Matrices &a, int step, float *pieces) {
+template <int KIND, int T, int N>
+void tile_product(Matrices<N> &a, int step, float *pieces) {
   typedef Shape<T> S;
   bool alike = true;  // in their blocks
   long blocks = 0;
@@ -987,7 +991,7 @@ void tile_product(Matrices &a, int step, float *pieces) {
     const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T, k = blocks_of(KIND == GRAM ? M.n : M.m);
     alike = alike && (!blocks || blocks == k);
     blocks = k;
-    tiles += (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * (a.alike ? a.count : 1);
+    tiles += (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * (N > 1 ? 1 : a.count);
     return (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * k;
   });
   const unsigned groups = (unsigned)(d.units < 8 * S::GROUPS ? (d.units + 7) / 8 : S::GROUPS);
@@ -997,59 +1001,60 @@ void tile_product(Matrices &a, int step, float *pieces) {
     d.units -= d.base;
   }
   d.sharers = (unsigned)(d.units < 8ul * groups ? (d.units + 7) / 8 : groups);
-  hipLaunchKernelGGL((tile_kernel<KIND, T>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
+  hipLaunchKernelGGL((tile_kernel<KIND, T, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
   if (d.sharers > 1)
-    hipLaunchKernelGGL((join_kernel<KIND, T>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, d,
+    hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, d,
                        (const float *)pieces);
 }
 
-template <int KIND>
-void product(Matrices &a, int step, int tile, float *pieces) {
-  if (tile == 0) small_product<KIND>(a, step);
-  else if (tile == 128) tile_product<KIND, 128>(a, step, pieces);
-  else tile_product<KIND, 256>(a, step, pieces);
+template <int KIND, int N>
+void product(Matrices<N> &a, int step, int tile, float *pieces) {
+  if (tile == 0) small_product<KIND, N>(a, step);
+  else if (tile == 128) tile_product<KIND, 128, N>(a, step, pieces);
+  else tile_product<KIND, 256, N>(a, step, pieces);
 }
 
-void run(Matrices &a, int steps, float mu, int nesterov, char *rest) {
+template <int N>
+void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
   if (by_block(a)) {
-    hipLaunchKernelGGL(block_kernel, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov);
+    hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov);
     return;
   }
   unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
-  hipLaunchKernelGGL(momentum_kernel, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
+  hipLaunchKernelGGL(momentum_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
-  hipLaunchKernelGGL(image_kernel, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
+  hipLaunchKernelGGL(image_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   const int tile = tile_size(a);
   for (int s = 0; s < steps; s++) {
-    product<GRAM>(a, s, tile, (float *)rest);
-    product<SQUARE>(a, s, tile, (float *)rest);
-    if (s + 1 < steps) product<STEP>(a, s, tile, (float *)rest);
-    else product<LAST>(a, s, tile, (float *)rest);
+    product<GRAM, N>(a, s, tile, (float *)rest);
+    product<SQUARE, N>(a, s, tile, (float *)rest);
+    if (s + 1 < steps) product<STEP, N>(a, s, tile, (float *)rest);
+    else product<LAST, N>(a, s, tile, (float *)rest);
   }
 }
 
 // the images (of a group of matrices), and two pieces a workgroup
-size_t ws_of(const Matrices &a, size_t images) {
+template <int N>
+size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
   const int t = tile_size(a);
   return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * (t == 128 ? Shape<128>::GROUPS : Shape<256>::GROUPS));
 }
 
 // `count` matrices of one shape
-void alike(Matrices &a, long count, long rows, long cols, char *ws) {
-  a = {};
+Matrices<1> alike(long count, long rows, long cols, char *ws) {
+  Matrices<1> a = {};
   a.count = (int)(count < ALIKE ? count : ALIKE);
-  a.alike = 1;
   a.images = (long)images_of(rows, cols);
   lay(a.at[0], rows, cols, ws);
+  return a;
 }
 
 }  // namespace
 
 extern "C" size_t tt_k_newton_schulz_ws(long count, long rows, long cols) {
   if (count <= 0 || !good_sides(rows, cols)) return 0;
-  Matrices a;
-  alike(a, count, rows, cols, NULL);
+  const Matrices<1> a = alike(count, rows, cols, NULL);
   return ws_of(a, a.count * (size_t)a.images);
 }
 
@@ -1064,8 +1069,7 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
     ws = own = ttrt_alloc(need);
     if (!ws) return -2;
   }
-  Matrices a;
-  alike(a, count, rows, cols, (char *)ws);
+  Matrices<1> a = alike(count, rows, cols, (char *)ws);
   const int most = by_block(a) ? 1 << 20 : a.count;  // without images any number at once
   for (long base = 0; base < count; base += most) {
     a.count = (int)(count - base < most ? count - base : most);
@@ -1079,7 +1083,7 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
 
 extern "C" size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int count) {
   if (!rows || !cols || count < 1 || count > TT_SGD_MAX) return 0;
-  Matrices a = {};
+  Matrices<MOST> a = {};
   a.count = count;
   size_t bytes = 0;
   char *at = NULL;
@@ -1109,7 +1113,7 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
     ws = own = ttrt_alloc(need);
     if (!ws) return -2;
   }
-  Matrices a = {};
+  Matrices<MOST> a = {};
   a.count = count;
   char *at = (char *)ws;
   for (int i = 0; i < count; i++) {
