@@ -598,19 +598,20 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) 
 // that others have the rest of.  Pieces go to memory, and join_kernel adds them.
 
 #ifndef TT_LARGE
-#define TT_LARGE 3.5e9
+#define TT_LARGE 2.8e9
 #endif
 #ifndef TT_HUGE
-#define TT_HUGE 1.7e10
+#define TT_HUGE 1.5e10
 #endif
 // Tiles of T x T: four waves of 64 x 64 or eight of 128 x 64 values, each FI x 2
 // blocks of 32 x 32.
-template <int T>
+template <int T, int BUFFERS>
 struct Shape {
   static constexpr int WAVES = T == 256 ? 8 : 4, ACROSS = WAVES / 2, FI = T / 64, BLOCKS = 2 * FI;
-  static constexpr int GROUPS = T == 256 ? 256 : 512;  // workgroups at most: one or two a CU
-  static constexpr int PIECE = T * T;                  // floats
-  static constexpr int BUFFER = 2 * T * 128;           // bytes of both operands' block
+  static constexpr int BUFFER = 2 * T * 128;  // bytes of both operands' block
+  static constexpr int GROUPS = 256;          // workgroups at most: one a CU
+  static constexpr int PIECE = T * T;         // floats
+  static constexpr int EACH = T / 8 / WAVES;  // loads of either operand's block a wave
 };
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
@@ -737,11 +738,11 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
 // where the 32 x 32 block f of a wave's lies
 template <int T>
 __device__ __forceinline__ int row_of(int ti, int wave, int f) {
-  return ti * T + (wave / Shape<T>::ACROSS) * (T / 2) + f / 2 * 32;
+  return ti * T + (wave / Shape<T, 2>::ACROSS) * (T / 2) + f / 2 * 32;
 }
 template <int T>
 __device__ __forceinline__ int col_of(int tj, int wave, int f) {
-  return tj * T + (wave % Shape<T>::ACROSS) * 64 + f % 2 * 32;
+  return tj * T + (wave % Shape<T, 2>::ACROSS) * 64 + f % 2 * 32;
 }
 template <int KIND>
 __device__ __forceinline__ bool transposed(const Matrix &M, int ti, int tj) {
@@ -755,14 +756,14 @@ struct Deal {
   unsigned long base, units;
   // the first of workgroup w's share
   __device__ __forceinline__ unsigned long begins(unsigned w) const {
-    return base + (w < sharers ? units * w / sharers : units);
+    return base + (w < sharers ? units * w / sharers : units);  // (no sharers: no units)
   }
 };
 
-template <int KIND, int T, int N>
-__global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<N> a, int step, Deal deal, float *pieces) {
-  typedef Shape<T> S;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * S::BUFFER];
+template <int KIND, int T, int BUFFERS, int N>
+__global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUFFERS>::WAVES / 4)) tile_kernel(Matrices<N> a, int step, Deal deal, float *pieces) {
+  typedef Shape<T, BUFFERS> S;
+  __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * S::BUFFER];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // consecutive workgroups go to the eight XCDs in turn: give each XCD a run of them
   const unsigned groups = gridDim.x, each = groups / 8, b = blockIdx.x;
@@ -775,6 +776,7 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<
         const Operands<KIND> o(a.at[0], step);
         u = ((unsigned long)round * groups + w) * blocks_of(o.k);
         end = u + blocks_of(o.k);
+        if (u >= deal.base) end = u;  // no tile for this workgroup
       } else if (round == deal.rounds) {
         u = deal.begins(w), end = deal.begins(w + 1);
         if (u == end) return;
@@ -782,6 +784,7 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<
         return;
       }
       round++;
+      if (u == end) continue;
     }
     unsigned long in = u;
     const Matrix M = matrix_of(a, in);
@@ -792,7 +795,7 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<
     const int k0 = (int)(in % blocks), k1 = (int)(end - u < (unsigned long)(blocks - k0) ? k0 + (end - u) : blocks);
     // a wave brings every WAVES-th KB of the tiles' T / 32 blocks; a block behind the
     // last is the last once more: its results are not written
-    constexpr int EACH = T / 8 / S::WAVES;
+    constexpr int EACH = S::EACH;
     unsigned off[2][EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
@@ -810,45 +813,81 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<
     };
     f32x16 acc[S::FI][2] = {};
     __syncthreads();  // the last tile's LDS is read
-    bring(0, to);
     const int n = k1 - k0;
+    for (int k = 0; k < BUFFERS - 1 && k < n; k++) bring(k, to + k * S::BUFFER);
     // the wave's blocks of either operand in a buffer
     const char *mine[2] = {lds + (wave / S::ACROSS) * (T / 2) * 128 + lane * 16,
                            lds + (T + (wave % S::ACROSS) * 64) * 128 + lane * 16};
-    for (int k = 0; k < n; k++) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    struct Half {  // 16 of a block's 32: the wave's blocks of either operand
+      half8 ha[S::FI], la[S::FI], hb[2], lb[2];
+    };
+    auto read = [&](int at) {  // (compile-time offsets from one address)
+      Half x;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        x.hb[j] = *(const half8 *)(mine[1] + at + j * 4096);
+        x.lb[j] = *(const half8 *)(mine[1] + at + j * 4096 + 2048);
+      }
+#pragma unroll
+      for (int i = 0; i < S::FI; i++) {
+        x.ha[i] = *(const half8 *)(mine[0] + at + i * 4096);
+        x.la[i] = *(const half8 *)(mine[0] + at + i * 4096 + 2048);
+      }
+      return x;
+    };
+    auto multiply = [&](const Half &x) {
+#pragma unroll
+      for (int i = 0; i < S::FI; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.la[i], x.hb[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < S::FI; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ha[i], x.lb[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < S::FI; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ha[i], x.hb[j], acc[i][j], 0, 0, 0);
+    };
+    auto arrived = [&](int k) {  // block k, in LDS for every wave
+      if (k + BUFFERS - 2 < n)   // with so many behind it still on their way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((BUFFERS - 2) * 2 * S::EACH) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      const int now = (k & 1) * S::BUFFER;
-      if (k + 1 < n) bring(k + 1, to + (S::BUFFER - now));
-#pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const int ph = now + s * 1024, pl = ph + 2048;
-        half8 ha[S::FI], la[S::FI], hb[2], lb[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          hb[j] = *(const half8 *)(mine[1] + ph + j * 4096);
-          lb[j] = *(const half8 *)(mine[1] + pl + j * 4096);
+    };
+    if constexpr (BUFFERS == 2) {
+      for (int k = 0; k < n; k++) {
+        arrived(k);
+        const int now = (k & 1) * S::BUFFER;
+        if (k + 1 < n) bring(k + 1, to + (S::BUFFER - now));
+        multiply(read(now));
+        multiply(read(now + 1024));
+      }
+    } else {
+      // a wave a SIMD: the reads of the next half stand between the products of this one
+      arrived(0);
+      Half x = read(0);
+      int now = 0;
+      for (int k = 0; k < n; k++) {
+        // into the place of the block before, which all have read by the last barrier
+        if (k + BUFFERS - 1 < n) bring(k + BUFFERS - 1, to + (now == 0 ? (BUFFERS - 1) * S::BUFFER : now - S::BUFFER));
+        const Half y = read(now + 1024);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(x);
+        __builtin_amdgcn_sched_barrier(0);
+        const int next = now == (BUFFERS - 1) * S::BUFFER ? 0 : now + S::BUFFER;
+        if (k + 1 < n) {
+          arrived(k + 1);
+          x = read(next);
         }
-#pragma unroll
-        for (int i = 0; i < S::FI; i++) {
-          ha[i] = *(const half8 *)(mine[0] + ph + i * 4096);
-          la[i] = *(const half8 *)(mine[0] + pl + i * 4096);
-        }
-#pragma unroll
-        for (int i = 0; i < S::FI; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(la[i], hb[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < S::FI; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[i], lb[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < S::FI; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha[i], hb[j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(y);
+        __builtin_amdgcn_sched_barrier(0);
+        now = next;
       }
     }
     if (n == blocks) {
@@ -879,7 +918,7 @@ __global__ void __launch_bounds__(Shape<T>::WAVES * 64, 2) tile_kernel(Matrices<
 // wave has 32 x 32 of its values.
 template <int KIND, int T, int N>
 __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal deal, const float *pieces) {
-  typedef Shape<T> S;
+  typedef Shape<T, 2> S;
   __shared__ float buf[4][32][33];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned w = blockIdx.x + 1;
@@ -961,15 +1000,24 @@ bool by_block(const Matrices<N> &a) {
   return !TT_NOBLOCK;
 }
 
-// How the products of such matrices go: by tiles of 32 (0), 128 or 256.
+// How the products of such matrices go: by tiles of 32 (0), 128 or 256 (us):
+//   tiles of       32    128    256
+//   2 x 1024^2    315    364    580
+//   1500^2        657    455    650
+//   2048^2       1170    734    889
+//   2500^2       2950   1469   1349
+//   1024 x 16384 2480   1108   1247
+//   4096^2      10300   4438   3843
 template <int N>
 int tile_size(const Matrices<N> &a) {
   double work = 0;
+  int widest = 0;
   for (int i = 0; i < a.count; i++) {
     const Matrix &M = a.at[N > 1 ? i : 0];
     work += (double)M.m * M.m * M.n;
+    widest = M.m > widest ? M.m : widest;
   }
-  return work < TT_LARGE ? 0 : work < TT_HUGE ? 128 : 256;
+  return work < TT_LARGE ? 0 : work < TT_HUGE || widest < 2048 ? 128 : 256;
 }
 
 template <int KIND, int N>
@@ -980,9 +1028,9 @@ void small_product(Matrices<N> &a, int step) {
   hipLaunchKernelGGL((small_kernel<KIND, N>), dim3((unsigned)grid), dim3(512), 0, stream(), a, step);
 }
 
-template <int KIND, int T, int N>
+template <int KIND, int T, int BUFFERS, int N>
 void tile_product(Matrices<N> &a, int step, float *pieces) {
-  typedef Shape<T> S;
+  typedef Shape<T, BUFFERS> S;
   bool alike = true;  // in their blocks
   long blocks = 0;
   unsigned long tiles = 0;
@@ -994,14 +1042,25 @@ void tile_product(Matrices<N> &a, int step, float *pieces) {
     tiles += (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * (N > 1 ? 1 : a.count);
     return (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * k;
   });
-  const unsigned groups = (unsigned)(d.units < 8 * S::GROUPS ? (d.units + 7) / 8 : S::GROUPS);
-  if (alike) {  // whole tiles side by side read the same blocks at about the same time
-    d.rounds = (unsigned)(tiles / groups);
-    d.base = (unsigned long)d.rounds * groups * blocks;
-    d.units -= d.base;
-  }
+  const unsigned groups = (unsigned)(d.units < S::GROUPS ? d.units : S::GROUPS);
   d.sharers = (unsigned)(d.units < 8ul * groups ? (d.units + 7) / 8 : groups);
-  hipLaunchKernelGGL((tile_kernel<KIND, T, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
+  if (alike) {
+    // In blocks of the busiest workgroup's, a join being worth about 12 (8 where every
+    // workgroup has one piece, and all of them the same parts of the length): whole
+    // tiles as often as they go round, and the rest whole as well, each tile among as
+    // many workgroups as there are for it, or evenly.
+    d.rounds = (unsigned)(tiles / groups);
+    const unsigned long rest = tiles % groups, most = rest ? groups / rest : 1,
+                        ways = most < (unsigned long)blocks ? most : blocks;  // no part is empty
+    const double whole = rest ? (double)blocks : 0, shared = (double)((blocks + ways - 1) / ways) + 8,
+                 even = (double)(rest * blocks) / groups + 12;
+    if (rest && whole <= shared && whole <= even) d.rounds++;
+    d.base = (unsigned long)d.rounds * groups < tiles ? (unsigned long)d.rounds * groups * blocks : d.units;
+    d.units -= d.base;
+    if (!d.units) d.sharers = 0;
+    else if (shared <= even) d.sharers = (unsigned)(rest * ways);
+  }
+  hipLaunchKernelGGL((tile_kernel<KIND, T, BUFFERS, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
   if (d.sharers > 1)
     hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, d,
                        (const float *)pieces);
@@ -1010,8 +1069,8 @@ void tile_product(Matrices<N> &a, int step, float *pieces) {
 template <int KIND, int N>
 void product(Matrices<N> &a, int step, int tile, float *pieces) {
   if (tile == 0) small_product<KIND, N>(a, step);
-  else if (tile == 128) tile_product<KIND, 128, N>(a, step, pieces);
-  else tile_product<KIND, 256, N>(a, step, pieces);
+  else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, pieces);
+  else tile_product<KIND, 256, 2, N>(a, step, pieces);
 }
 
 template <int N>
@@ -1038,7 +1097,7 @@ template <int N>
 size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
   const int t = tile_size(a);
-  return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * (t == 128 ? Shape<128>::GROUPS : Shape<256>::GROUPS));
+  return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * 256);
 }
 
 // `count` matrices of one shape
