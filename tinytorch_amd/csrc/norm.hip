@@ -383,12 +383,15 @@ __global__ void __launch_bounds__(threads_of(NT))
   f32x4 aw[NV], g[NV];
 #pragma unroll
   for (int n = 0; n < NV; n++) aw[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  if (w) gr.load(g, w);
+  // the longest rows leave no registers for the weights from row to row
+  constexpr bool KEEP = NT * NV < 4096;
+  if (w && KEEP) gr.load(g, w);
   for (long row = (long)blockIdx.x * RB + sub; row < rows; row += (long)gridDim.x * RB) {
     f32x4 v[NV], d[NV], u[NV];
     gr.load(v, x + row * cols);
     gr.load(d, dy + row * cols);
     if (ds && dx) gr.load(u, ds + row * cols);
+    if (w && !KEEP) gr.load(g, w);
     const float r = rstd[row];
     gr.mask(v);
     gr.mask(d);
