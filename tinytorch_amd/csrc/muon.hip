@@ -165,16 +165,19 @@ __device__ __forceinline__ half8 along(const char *image, int blocks, int r0, in
 }
 // The transposing read: sixteen lanes read four values each of four rows and sixteen
 // columns (lane l: row l / 4, columns 4 (l % 4) ..) and get the four rows of column l.
-// Eight rows r0 + 8 (lane / 32) .. of column lane % 32 of a block.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ s16x4 read_transposed(const char *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p));
+}
+// eight rows r0 + 8 (lane / 32) .. of column lane % 32 of a block
 __device__ __forceinline__ half8 across(const char *image, int blocks, int r0, int block, int part, int lane) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef short s16x8 __attribute__((ext_vector_type(8)));
   s16x8 v;
   const int l = lane & 15, c = (lane >> 4 & 1) * 16 + 4 * (l & 3);
 #pragma unroll
   for (int x = 0; x < 2; x++) {
     const char *p = chunk_of(image, blocks, r0 + (lane >> 5) * 8 + x * 4 + l / 4, block, part * 4 + c / 8) + (c & 4) * 2;
-    const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p));
+    const s16x4 w = read_transposed(p);
 #pragma unroll
     for (int j = 0; j < 4; j++) v[x * 4 + j] = w[j];
   }
@@ -481,19 +484,20 @@ __device__ __forceinline__ void triangle(unsigned b, int &i, int &j) {
 template <int KIND>
 struct Operands {
   const char *a, *b;    // images whose rows are multiplied
-  const char *add;      // image of the matrix added, times `times` (GRAM: none)
+  const char *add;      // image of the transpose of the matrix added, times `times` (GRAM: none)
+  const char *plain;    // and of that matrix
   char *out, *down;     // images of the result and its transpose
   int rows, cols, k;    // of the result; the products' length
   float by, times;
   __device__ __forceinline__ Operands(const Matrix &M, int step) {
     if (KIND == GRAM) {
-      a = b = M.x, add = nullptr, out = down = M.p;
+      a = b = M.x, add = plain = nullptr, out = down = M.p;
       rows = cols = M.m, k = M.n, by = 1.f, times = 0.f;
     } else if (KIND == SQUARE) {
-      a = b = add = M.p, out = down = M.q;
+      a = b = add = plain = M.p, out = down = M.q;
       rows = cols = k = M.m, by = TT_NS_C, times = TT_NS_B;
     } else {
-      a = M.q, b = step & 1 ? M.t1 : M.t0, add = M.x, out = M.x, down = step & 1 ? M.t0 : M.t1;
+      a = M.q, b = add = step & 1 ? M.t1 : M.t0, plain = M.x, out = M.x, down = step & 1 ? M.t0 : M.t1;
       rows = k = M.m, cols = M.n, by = 1.f, times = TT_NS_A;
     }
   }
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) 
   const int row = ti * 32 + r, col = tj * 32 + c;
   float v[2] = {0.f, 0.f};
   if (KIND != GRAM) {
-    const _Float16 *p = place((char *)o.add, blocks_of(o.cols), row, col);
+    const _Float16 *p = place((char *)o.plain, blocks_of(o.cols), row, col);
     const half2 h = *(const half2 *)p, l = *(const half2 *)(p + 1024);
 #pragma unroll
     for (int e = 0; e < 2; e++) v[e] = o.times * (1.f / UP) * ((float)h[e] + (float)l[e]);
@@ -657,81 +661,97 @@ __device__ __forceinline__ void tile_of(unsigned long tile, int rows, int cols, 
   }
 }
 
-// A wave's 32 x 32 values, `acc` as the matrix instructions leave them, to where
-// they go: through LDS, so that a lane has 16 of a row (and, for the transpose, of a
-// column) and lines are written whole.
+// A wave's 32 x 32 values from (r0, c0) on as the matrix instructions leave them: a
+// lane has of column low = lane % 32 the rows high + 8 i + {0 .. 3}, high = 4 (lane / 32).
+// In the image of the transpose those are 8 bytes that with the other lanes' make
+// 512, so there they are read (what is added: P is symmetric, X^T has an image) and
+// written as they are; the image itself gets its blocks by transposing reads of LDS.
+// Behind the last row and column all of it is 0, as the operands are there.
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+struct Added {
+  half4 h[4], l[4];
+};
+__device__ __forceinline__ int part_of(int i, int lane) {  // in the block of the transpose, bytes
+  return (i >> 1) * 1024 + ((lane & 31) + 32 * (i & 1)) * 16 + (lane >> 5) * 8;
+}
 template <int KIND>
-__device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, int r0, int c0,
-                                        float (*buf)[33], int lane, bool transpose) {
+__device__ __forceinline__ Added added(const Operands<KIND> &o, int r0, int c0, int lane) {
+  Added x = {};
+  if (KIND == GRAM || r0 >= o.rows || c0 >= o.cols) return x;
+  const char *p = o.add + ((c0 >> 5) * blocks_of(o.rows) + (r0 >> 5)) * 4096;
 #pragma unroll
-  for (int i = 0; i < 16; i++) buf[8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
-  __builtin_amdgcn_wave_barrier();
-  const int line = lane >> 1, from = (lane & 1) * 16;
-  float v[16];
-#pragma unroll
-  for (int j = 0; j < 16; j++) v[j] = buf[line][from + j] * (o.by * DOWN2);
-  const int row = r0 + line, col = c0 + from;
-  const long blocks = blocks_of(o.cols);
+  for (int i = 0; i < 4; i++) {
+    x.h[i] = *(const half4 *)(p + part_of(i, lane));
+    x.l[i] = *(const half4 *)(p + part_of(i, lane) + 2048);
+  }
+  return x;
+}
+// buf: 4 KB of LDS, this wave's; both: the image itself too
+template <int KIND>
+__device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, const Added &x,
+                                        int r0, int c0, char *buf, int lane, bool both) {
   if (r0 >= o.rows || c0 >= o.cols) return;
-  if (KIND != GRAM) {
-    const half8 *p = (const half8 *)place((char *)o.add, blocks, row, col);
-    const half8 h[2] = {p[0], p[32]}, l[2] = {p[128], p[160]};
+  f32x4 v[4];
 #pragma unroll
-    for (int j = 0; j < 16; j++) v[j] += o.times * (1.f / UP) * ((float)h[j / 8][j % 8] + (float)l[j / 8][j % 8]);
-  }
+  for (int i = 0; i < 4; i++)
 #pragma unroll
-  for (int j = 0; j < 16; j++)
-    if (row >= o.rows || col + j >= o.cols) v[j] = 0.f;
-  if (transpose) {
-#pragma unroll
-    for (int j = 0; j < 16; j++) buf[line][from + j] = v[j];
-  }
+    for (int j = 0; j < 4; j++) {
+      v[i][j] = acc[i * 4 + j] * (o.by * DOWN2);
+      if (KIND != GRAM) v[i][j] += o.times * (1.f / UP) * ((float)x.h[i][j] + (float)x.l[i][j]);
+    }
   if (KIND == LAST) {
-    if (!transpose && row < o.rows) {
-      float *w = M.w + (long)row * o.cols + col;
-      if (col + 16 <= o.cols) {
+    const int col = c0 + (lane & 31);
+    if (col >= o.cols) return;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          f32x4 u = {v[j], v[j + 1], v[j + 2], v[j + 3]};
-          if (M.v) u = *(const f32x4_any *)(w + j) * M.keep + u * M.rate;
-          *(f32x4_any *)(w + j) = u;
-        }
+    for (int i = 0; i < 4; i++) {
+      const int row = r0 + 8 * i + (lane >> 5) * 4;
+      if (M.turned && row + 4 <= o.rows) {
+        float *w = M.w + (long)col * o.rows + row;
+        *(f32x4_any *)w = M.v ? *(const f32x4_any *)w * M.keep + v[i] * M.rate : v[i];
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-          if (col + j < o.cols) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
+        for (int j = 0; j < 4; j++)
+          if (row + j < o.rows) {
+            float *w = M.w + (M.turned ? (long)col * o.rows + row + j : (long)(row + j) * o.cols + col);
+            *w = M.v ? *w * M.keep + v[i][j] * M.rate : v[i][j];
+          }
       }
     }
-  } else {
-    float up[16];
-#pragma unroll
-    for (int j = 0; j < 16; j++) up[j] = v[j] * UP;
-    put16(o.out, blocks, row, col, up);
+    return;
   }
-  if (!transpose) return;
-  __builtin_amdgcn_wave_barrier();
+  char *down = o.down + ((c0 >> 5) * blocks_of(o.rows) + (r0 >> 5)) * 4096;
 #pragma unroll
-  for (int j = 0; j < 16; j++) v[j] = buf[from + j][line];
-  const int trow = c0 + line, tcol = r0 + from;
-  if (KIND == LAST) {
-    if (trow >= o.cols) return;
-    float *w = M.w + (long)trow * o.rows + tcol;
-    if (tcol + 16 <= o.rows) {
+  for (int i = 0; i < 4; i++) {
+    half4 h, l;
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        f32x4 u = {v[j], v[j + 1], v[j + 2], v[j + 3]};
-        if (M.v) u = *(const f32x4_any *)(w + j) * M.keep + u * M.rate;
-        *(f32x4_any *)(w + j) = u;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (tcol + j < o.rows) w[j] = M.v ? M.keep * w[j] + M.rate * v[j] : v[j];
+    for (int j = 0; j < 4; j++) {
+      _Float16 a, b;
+      split(v[i][j] * UP, a, b);
+      h[j] = a, l[j] = b;
     }
-  } else {
+    *(half4 *)(down + part_of(i, lane)) = h;
+    *(half4 *)(down + part_of(i, lane) + 2048) = l;
+    if (both) {
+      *(half4 *)(buf + part_of(i, lane)) = h;
+      *(half4 *)(buf + part_of(i, lane) + 2048) = l;
+    }
+  }
+  if (!both) return;
+  __builtin_amdgcn_wave_barrier();
+  char *out = o.out + ((r0 >> 5) * blocks_of(o.cols) + (c0 >> 5)) * 4096 + lane * 16;
+  const int l = lane & 15;
 #pragma unroll
-    for (int j = 0; j < 16; j++) v[j] *= UP;
-    put16(o.down, blocks_of(o.rows), trow, tcol, v);
+  for (int f = 0; f < 4; f++) {  // h and l of either 16 columns: eight rows of the transpose's block
+    s16x8 w;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const int r = (f & 1) * 16 + (lane >> 5) * 8 + x * 4 + l / 4;
+      const s16x4 t = read_transposed(buf + (f >> 1) * 2048 + (lane >> 4 & 1) * 1024 + (r + 32 * ((l & 3) / 2)) * 16 +
+                                      (l & 1) * 8);
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[x * 4 + j] = t[j];
+    }
+    *(s16x8 *)(out + (f >> 1) * 2048 + (f & 1) * 1024) = w;
   }
 }
 
@@ -744,11 +764,6 @@ template <int T>
 __device__ __forceinline__ int col_of(int tj, int wave, int f) {
   return tj * T + (wave % Shape<T, 2>::ACROSS) * 64 + f % 2 * 32;
 }
-template <int KIND>
-__device__ __forceinline__ bool transposed(const Matrix &M, int ti, int tj) {
-  return KIND <= SQUARE ? ti != tj : KIND == STEP || M.turned;
-}
-
 // How the units (tiles' blocks, tile by tile) are dealt: `rounds` whole tiles to every
 // workgroup, then the units from `base` on evenly to the first `sharers`.
 struct Deal {
@@ -892,12 +907,14 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
     }
     if (n == blocks) {
       __syncthreads();  // the operands are read
-      const bool transpose = transposed<KIND>(M, ti, tj);
+      Added x = added<KIND>(o, row_of<T>(ti, wave, 0), col_of<T>(tj, wave, 0), lane), next = x;
 #pragma unroll
       for (int f = 0; f < S::BLOCKS; f++) {
-        write32<KIND>(M, o, acc[f / 2][f % 2], row_of<T>(ti, wave, f), col_of<T>(tj, wave, f),
-                      (float(*)[33])(lds + wave * 8192), lane, transpose);
+        if (f + 1 < S::BLOCKS) next = added<KIND>(o, row_of<T>(ti, wave, f + 1), col_of<T>(tj, wave, f + 1), lane);
+        write32<KIND>(M, o, acc[f / 2][f % 2], x, row_of<T>(ti, wave, f), col_of<T>(tj, wave, f), lds + wave * 4096, lane,
+                      KIND == STEP || ti != tj);
         __builtin_amdgcn_wave_barrier();
+        x = next;
       }
     } else {
       f32x4 *p = (f32x4 *)(pieces + (2l * w + (k0 == 0)) * S::PIECE) + wave * S::BLOCKS * 256 + lane;
@@ -919,7 +936,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
 template <int KIND, int T, int N>
 __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal deal, const float *pieces) {
   typedef Shape<T, 2> S;
-  __shared__ float buf[4][32][33];
+  __shared__ __attribute__((aligned(1024))) char buf[4][4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned w = blockIdx.x + 1;
   const unsigned long u = deal.begins(w);
@@ -931,6 +948,8 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal
   int ti, tj;
   tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
   const int block = blockIdx.y * 4 + wave;
+  const int r0 = row_of<T>(ti, block / S::BLOCKS, block % S::BLOCKS), c0 = col_of<T>(tj, block / S::BLOCKS, block % S::BLOCKS);
+  const Added x = added<KIND>(o, r0, c0, lane);
   unsigned stop = w;  // the first workgroup behind the tile
   while (stop < deal.sharers && deal.begins(stop) < last) stop++;
   f32x16 acc = {};
@@ -944,8 +963,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal
       for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
     }
   }
-  write32<KIND>(M, o, acc, row_of<T>(ti, block / S::BLOCKS, block % S::BLOCKS),
-                col_of<T>(tj, block / S::BLOCKS, block % S::BLOCKS), buf[wave], lane, transposed<KIND>(M, ti, tj));
+  write32<KIND>(M, o, acc, x, r0, c0, buf[wave], lane, KIND == STEP || ti != tj);
 }
 
 // ---------------------------------------------------------------- host
