@@ -66,6 +66,48 @@ def test_steps(tlib, rows, cols, kind):
         assert off <= NEAR * np.linalg.norm(want), (steps, off / np.linalg.norm(want))
 
 
+@pytest.mark.parametrize("rows,cols", [(1430, 1400), (1060, 2600)])
+def test_one_step_large(tlib, rows, cols):
+    """By tiles of 128: value by value."""
+    x = _matrix(rows, cols)
+    want, tol = ref.one_step(*ref.normed(x))
+    if rows > cols:
+        want, tol = want.T, tol.T
+    got = _steps(tlib, x, 1)
+    assert (np.abs(got - want) <= tol + ref.U * np.abs(want)).all(), np.max(np.abs(got - want) / tol)
+
+
+def _steps64(x, steps):
+    x = x.astype(np.float64)
+    y = x.T if x.shape[0] > x.shape[1] else x
+    y = y / np.linalg.norm(y)
+    for _ in range(steps):
+        p = y @ y.T
+        y = ref.A * y + (ref.B * p + ref.C * (p @ p)) @ y
+    return y.T if x.shape[0] > x.shape[1] else y
+
+
+@pytest.mark.parametrize("shape,steps", [((1390, 1470), 5), ((1700, 1290), 5), ((2100, 7010), 4), ((7003, 2101), 3),
+                                         ((3, 1020, 1010), 5), ((130, 150, 155), 5)])
+def test_steps_large(tlib, shape, steps):
+    """By tiles of 128 and 256, upright and turned, one matrix and several."""
+    x = np.random.default_rng(7).standard_normal(shape).astype(np.float32)
+    got = _steps(tlib, x, steps)
+    for i in ((0, shape[0] - 1) if len(shape) == 3 else (slice(None),)):
+        want = _steps64(x[i], steps)
+        off = np.linalg.norm(got[i] - want) / np.linalg.norm(want)
+        assert off <= NEAR, off
+        big = np.abs(got[i] - want).max() / np.sqrt((want**2).mean())
+        assert big <= 40 * NEAR, big  # of some millions of values none is off by many times the rest
+    assert np.array_equal(got, _steps(tlib, x, steps, in_place=True))
+    more = 1 << 10
+    need = tlib.tt_k_newton_schulz_ws(x.size // (shape[-1] * shape[-2]), *shape[-2:])
+    ws = DevBuf(need // 4 + more)
+    ws.fill(np.nan)
+    assert np.array_equal(got, _steps(tlib, x, steps, ws.ptr))  # what a workspace holds before does not count
+    assert np.isnan(ws.to_np()[-more:]).all()
+
+
 def test_steps_take_singular_values(tlib):
     """From known singular vectors: a s + b s^3 + c s^5, five times."""
     rng = np.random.default_rng(3)
@@ -148,7 +190,8 @@ def _muon64(w, g, v, lr, mu, nesterov, decay):
 @pytest.mark.parametrize("nesterov", [0, 1])
 @pytest.mark.parametrize("shapes", [[(30, 50)], [(785, 256), (257, 128), (129, 10)],
                                     [(5, 7), (64, 64), (33, 400), (200, 20), (1, 9)],
-                                    [(3 + i, 40 - 2 * i) for i in range(16)]])
+                                    [(3 + i, 40 - 2 * i) for i in range(16)],
+                                    [(1100, 1300), (33, 50), (1200, 1000), (700, 2000)]])
 def test_muon_step(tlib, shapes, nesterov):
     rng = np.random.default_rng(4)
     w, g, v = ([rng.standard_normal(s).astype(np.float32) for s in shapes] for _ in range(3))

@@ -39,9 +39,6 @@ typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
-#ifndef TT_NOBLOCK
-#define TT_NOBLOCK 0
-#endif
 constexpr float UP = 16384.f, DOWN2 = 1.f / (16384.f * 16384.f);
 constexpr int MOST = TT_SGD_MAX;   // matrices of different shapes in one run of launches
 constexpr int ALIKE = 64;          // of one shape
@@ -601,12 +598,6 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) 
 // matrices' shapes: a workgroup has whole tiles and at most two pieces of tiles
 // that others have the rest of.  Pieces go to memory, and join_kernel adds them.
 
-#ifndef TT_LARGE
-#define TT_LARGE 2.8e9
-#endif
-#ifndef TT_HUGE
-#define TT_HUGE 1.5e10
-#endif
 // Tiles of T x T: four waves of 64 x 64 or eight of 128 x 64 values, each FI x 2
 // blocks of 32 x 32.
 template <int T, int BUFFERS>
@@ -883,25 +874,54 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
         multiply(read(now + 1024));
       }
     } else {
-      // a wave a SIMD: the reads of the next half stand between the products of this one
-      arrived(0);
-      Half x = read(0);
-      int now = 0;
-      for (int k = 0; k < n; k++) {
-        // into the place of the block before, which all have read by the last barrier
-        if (k + BUFFERS - 1 < n) bring(k + BUFFERS - 1, to + (now == 0 ? (BUFFERS - 1) * S::BUFFER : now - S::BUFFER));
-        const Half y = read(now + 1024);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(x);
-        __builtin_amdgcn_sched_barrier(0);
-        const int next = now == (BUFFERS - 1) * S::BUFFER ? 0 : now + S::BUFFER;
-        if (k + 1 < n) {
-          arrived(k + 1);
-          x = read(next);
+      // A wave a SIMD: while it waits to hand over a read or a load it starts no
+      // product, so these stand between the products one by one: after each of the
+      // first eight a read of the next half, after the others (load) a KB of one
+      // operand of the block BUFFERS - 1 further (2048 x 2048: 62 us a product with the
+      // reads and loads before the products).
+      static_assert(S::FI == 2 && S::EACH == 4, "one wave a SIMD has 64 x 64");
+      auto half = [&](const Half &x, Half &y, int at, bool load, const char *from, const unsigned *part, unsigned to) {
+#pragma unroll
+        for (int m = 0; m < 12; m++) {
+          const int i = m >> 1 & 1, j = m & 1;
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(m < 4 ? x.la[i] : x.ha[i], m >= 4 && m < 8 ? x.lb[j] : x.hb[j],
+                                                             acc[i][j], 0, 0, 0);
+          if (m < 8) {  // in the order in which the products take them
+            const int q = m & 1, f = m >> 1 & 1;
+            const half8 v = *(const half8 *)(mine[q] + at + f * 4096 + ((m < 4) != (q == 1) ? 2048 : 0));
+            if (m < 4) {
+              if (q) y.hb[f] = v;
+              else y.la[f] = v;
+            } else {
+              if (q) y.lb[f] = v;
+              else y.ha[f] = v;
+            }
+          } else if (load) {
+            dma16(from, part[m - 8], to + (wave * S::EACH + m - 8) * 1024);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(y);
-        __builtin_amdgcn_sched_barrier(0);
+      };
+      arrived(0);
+      Half x = read(0), y;
+      int now = 0, k = 0;
+      for (; k + BUFFERS - 1 < n; k++) {
+        const int next = now == (BUFFERS - 1) * S::BUFFER ? 0 : now + S::BUFFER;
+        // into the place of the block before, which all have read by the last barrier
+        const unsigned free = to + (now == 0 ? (BUFFERS - 1) * S::BUFFER : now - S::BUFFER);
+        half(x, y, now + 1024, true, pa + (long)(k + BUFFERS - 1) * 4096, off[0], free);
+        // block k + 1 is there when what follows it may still be on its way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((BUFFERS - 3) * 2 * S::EACH + S::EACH) : "memory");
+        __syncthreads();
+        half(y, x, next, true, pb + (long)(k + BUFFERS - 1) * 4096, off[1], free + T * 128);
+        now = next;
+      }
+      for (; k < n; k++) {
+        const int next = now == (BUFFERS - 1) * S::BUFFER ? 0 : now + S::BUFFER;
+        half(x, y, now + 1024, false, pa, off[0], 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        half(y, x, next, false, pb, off[1], 0);  // (behind the last block nothing takes what it reads)
         now = next;
       }
     }
@@ -1015,17 +1035,19 @@ template <int N>
 bool by_block(const Matrices<N> &a) {
   for (int i = 0; i < (N > 1 ? a.count : 1); i++)
     if (!fits_block(a.at[i].m, a.at[i].n)) return false;
-  return !TT_NOBLOCK;
+  return true;
 }
 
-// How the products of such matrices go: by tiles of 32 (0), 128 or 256 (us):
-//   tiles of       32    128    256
-//   2 x 1024^2    315    364    580
-//   1500^2        657    455    650
-//   2048^2       1170    734    889
-//   2500^2       2950   1469   1349
-//   1024 x 16384 2480   1108   1247
-//   4096^2      10300   4438   3843
+// How the products of such matrices go: by tiles of 32 (0), 128 or 256, by the work
+// m m n of all of them (us for five steps):
+//   tiles of            32    128    256
+//   2 x 1024^2         321    363      -
+//   1500^2             657    445    650
+//   2048^2            1170    685    876
+//   3 x 2048^2           -   1863   2036
+//   2048 x 8192          -   2019   1892
+//   4096^2           10300   3886   3867
+//   8192^2               -  33066  26650
 template <int N>
 int tile_size(const Matrices<N> &a) {
   double work = 0;
@@ -1035,7 +1057,7 @@ int tile_size(const Matrices<N> &a) {
     work += (double)M.m * M.m * M.n;
     widest = M.m > widest ? M.m : widest;
   }
-  return work < TT_LARGE ? 0 : work < TT_HUGE || widest < 2048 ? 128 : 256;
+  return work < 2.8e9 ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
 }
 
 template <int KIND, int N>
