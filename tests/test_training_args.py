@@ -104,7 +104,10 @@ def test_workspace_sizes(L):
     r, c = (ctypes.c_long * 2)(1024, 512), (ctypes.c_long * 2)(4096, 512)
     both = L.tt_k_muon_multi_ws(r, c, 2)
     assert 12 * 1024 * 4096 + 20 * 512 * 512 <= both <= 14.1 * 1024 * 4096 + 20.2 * 512 * 512 + more
-    assert L.tt_k_embedding_bwd_ws(8192, 32000, 1024) <= 17 * 8192 + 8 * 256 * 1024 + 64
+    # 16 bytes a token, and two parts of 4 bytes a column for every 8 tokens or more
+    for rows in (513, 8192, 100000):
+        assert 16 * rows <= L.tt_k_embedding_bwd_ws(rows, 32000, 1024) <= 16 * (rows + 3) + 8 * 1024 * ((rows + 7) // 8)
+    assert L.tt_k_embedding_bwd_ws(512, 32000, 1024) == 0
 
 
 @pytest.mark.parametrize("args", [(NAN, 0.9, 1, 0.0), (0.1, INF, 1, 0.0), (0.1, 0.9, 1, NAN)])
