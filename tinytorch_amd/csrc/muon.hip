@@ -1038,8 +1038,8 @@ bool by_block(const Matrices<N> &a) {
   return true;
 }
 
-// How the products of such matrices go: by tiles of 32 (0), 128 or 256, by the work
-// m m n of all of them (us for five steps):
+// How a product of such matrices goes: by tiles of 32 (0), 128 or 256, by its work, m m
+// and its length, in all of them (us for five steps, all products alike):
 //   tiles of            32    128    256
 //   2 x 1024^2         321    363      -
 //   1500^2             657    445    650
@@ -1049,12 +1049,12 @@ bool by_block(const Matrices<N> &a) {
 //   4096^2           10300   3886   3867
 //   8192^2               -  33066  26650
 template <int N>
-int tile_size(const Matrices<N> &a) {
+int tile_size(const Matrices<N> &a, int kind) {
   double work = 0;
   int widest = 0;
   for (int i = 0; i < a.count; i++) {
     const Matrix &M = a.at[N > 1 ? i : 0];
-    work += (double)M.m * M.m * M.n;
+    work += (double)M.m * M.m * (kind == SQUARE ? M.m : M.n);
     widest = M.m > widest ? M.m : widest;
   }
   return work < 2.8e9 ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
@@ -1107,7 +1107,8 @@ void tile_product(Matrices<N> &a, int step, float *pieces) {
 }
 
 template <int KIND, int N>
-void product(Matrices<N> &a, int step, int tile, float *pieces) {
+void product(Matrices<N> &a, int step, float *pieces) {
+  const int tile = tile_size(a, KIND);
   if (tile == 0) small_product<KIND, N>(a, step);
   else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, pieces);
   else tile_product<KIND, 256, 2, N>(a, step, pieces);
@@ -1123,12 +1124,11 @@ void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
   hipLaunchKernelGGL(momentum_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
   hipLaunchKernelGGL(image_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
-  const int tile = tile_size(a);
   for (int s = 0; s < steps; s++) {
-    product<GRAM, N>(a, s, tile, (float *)rest);
-    product<SQUARE, N>(a, s, tile, (float *)rest);
-    if (s + 1 < steps) product<STEP, N>(a, s, tile, (float *)rest);
-    else product<LAST, N>(a, s, tile, (float *)rest);
+    product<GRAM, N>(a, s, (float *)rest);
+    product<SQUARE, N>(a, s, (float *)rest);
+    if (s + 1 < steps) product<STEP, N>(a, s, (float *)rest);
+    else product<LAST, N>(a, s, (float *)rest);
   }
 }
 
@@ -1136,7 +1136,7 @@ void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
 template <int N>
 size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
-  const int t = tile_size(a);
+  const int t = tile_size(a, GRAM);  // of the longest product
   return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * 256);
 }
 
