@@ -467,11 +467,11 @@ __global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int
 
 // ---------------------------------------------------------------- products
 
-enum { GRAM, SQUARE, STEP, LAST };  // P = X X^T; Q = b P + c P P; X <- a X + Q X; the same, to w
+enum { GRAM, SQUARE, STEP };  // P = X X^T; Q = b P + c P P; X <- a X + Q X, the last one to w
 
 // Tile `b` of a symmetric matrix: those of the lower triangle row by row.
 __device__ __forceinline__ void triangle(unsigned b, int &i, int &j) {
-  int r = (int)((sqrt(8.0 * b + 1.0) - 1.0) * 0.5);
+  int r = (int)((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
   while ((unsigned)r * (r + 1u) / 2 > b) r--;
   while ((unsigned)(r + 1) * (r + 2u) / 2 <= b) r++;
   i = r;
@@ -500,26 +500,53 @@ struct Operands {
   }
 };
 
+// Consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of them,
+// and the tiles are in bands of eight rows, column by column, so that what an XCD's
+// L2 holds are the rows and columns of a patch.
+__device__ __forceinline__ unsigned dealt(unsigned b, unsigned n) {
+  const unsigned each = n / 8;
+  return b < each * 8 ? (b % 8) * each + b / 8 : b;
+}
+constexpr int BAND = 8;
+template <int KIND, int T, class U>
+__device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int &tj) {
+  const int nr = (rows + T - 1) / T, nc = (cols + T - 1) / T;
+  if (KIND <= SQUARE) {
+    // below band b: 32 b^2 + 4 b tiles of the lower triangle
+    int b = (int)((sqrtf(128.f * (float)tile + 16.f) - 4.f) / 64.f);
+    while (b > 0 && (U)32 * b * b + (U)4 * b > tile) b--;
+    while ((U)32 * (b + 1) * (b + 1) + (U)4 * (b + 1) <= tile) b++;
+    const unsigned in = (unsigned)(tile - ((U)32 * b * b + (U)4 * b));
+    const unsigned h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
+    if (in < (unsigned)b * BAND * h) {
+      ti = b * BAND + (int)(in % h), tj = (int)(in / h);
+    } else {
+      triangle(in - (unsigned)b * BAND * h, ti, tj);
+      ti += b * BAND, tj += b * BAND;
+    }
+  } else {
+    const U band = (U)BAND * nc;
+    const int b = (int)(tile / band);
+    const unsigned in = (unsigned)(tile % band), h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
+    ti = b * BAND + (int)(in % h), tj = (int)(in / h);
+  }
+}
+
 // Tiles of 32 x 32, one a workgroup, the operands read from memory as the matrix
 // instructions take them and each wave with a share of the products' length:
 // eight sums, joined in LDS.  What bounds these is the way from memory (the L2 of
 // another XCD has what the last launch wrote), so the added matrix is on its way
 // first, and a tile on the diagonal reads its rows once.
 template <int KIND, int N>
-__global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) {
+__global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step, int to_w) {
   typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   constexpr int WAVES = 8;
   __shared__ float sums[WAVES][32][33];
-  unsigned t = blockIdx.x;
+  unsigned t = dealt(blockIdx.x, gridDim.x);
   const Matrix M = matrix_of(a, t);
   const Operands<KIND> o(M, step);
   int ti, tj;
-  if (KIND <= SQUARE) {
-    triangle(t, ti, tj);
-  } else {
-    const unsigned across = (unsigned)blocks_of(o.cols);
-    ti = (int)(t / across), tj = (int)(t % across);
-  }
+  tile_of<KIND, 32>(t, o.rows, o.cols, ti, tj);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 2;  // this thread's two results
   const int row = ti * 32 + r, col = tj * 32 + c;
@@ -560,7 +587,7 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) 
     for (int w = 0; w < WAVES; w++) s += sums[w][r][c + e];
     v[e] = in[e] ? v[e] + s * (o.by * DOWN2) : 0.f;
   }
-  if (KIND == LAST) {
+  if (KIND == STEP && to_w) {
 #pragma unroll
     for (int e = 0; e < 2; e++)
       if (in[e] && !M.turned) {
@@ -570,13 +597,13 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step) 
   } else {
     put2(o.out, blocks_of(o.cols), row, col, v[0], v[1]);
   }
-  if ((KIND <= SQUARE && ti == tj) || (KIND == LAST && !M.turned)) return;
+  if ((KIND <= SQUARE && ti == tj) || (KIND == STEP && to_w && !M.turned)) return;
   __syncthreads();
   sums[0][r][c] = v[0];
   sums[0][r][c + 1] = v[1];
   __syncthreads();
   const int trow = tj * 32 + r, tcol = ti * 32 + c;  // the transpose
-  if (KIND == LAST) {
+  if (KIND == STEP && to_w) {
 #pragma unroll
     for (int e = 0; e < 2; e++)
       if (trow < o.cols && tcol + e < o.rows) {
@@ -625,33 +652,6 @@ __device__ __forceinline__ const char *scalar(const char *p) {
                         (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
 }
 
-// Tiles in bands of eight rows, column by column, so that the workgroups of an XCD
-// (consecutive ones) share rows and columns.
-constexpr int BAND = 8;
-template <int KIND, int T>
-__device__ __forceinline__ void tile_of(unsigned long tile, int rows, int cols, int &ti, int &tj) {
-  const int nr = (rows + T - 1) / T, nc = (cols + T - 1) / T;
-  if (KIND <= SQUARE) {
-    // below band b: 32 b^2 + 4 b tiles of the lower triangle
-    int b = (int)((sqrt(128.0 * (double)tile + 16.0) - 4.0) / 64.0);
-    while (b > 0 && 32ul * b * b + 4ul * b > tile) b--;
-    while (32ul * (b + 1) * (b + 1) + 4ul * (b + 1) <= tile) b++;
-    const unsigned in = (unsigned)(tile - (32ul * b * b + 4ul * b));
-    const unsigned h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
-    if (in < (unsigned)b * BAND * h) {
-      ti = b * BAND + (int)(in % h), tj = (int)(in / h);
-    } else {
-      triangle(in - (unsigned)b * BAND * h, ti, tj);
-      ti += b * BAND, tj += b * BAND;
-    }
-  } else {
-    const unsigned long band = (unsigned long)BAND * nc;
-    const int b = (int)(tile / band);
-    const unsigned in = (unsigned)(tile % band), h = nr - b * BAND < BAND ? nr - b * BAND : BAND;
-    ti = b * BAND + (int)(in % h), tj = (int)(in / h);
-  }
-}
-
 // A wave's 32 x 32 values from (r0, c0) on as the matrix instructions leave them: a
 // lane has of column low = lane % 32 the rows high + 8 i + {0 .. 3}, high = 4 (lane / 32).
 // In the image of the transpose those are 8 bytes that with the other lanes' make
@@ -680,7 +680,7 @@ __device__ __forceinline__ Added added(const Operands<KIND> &o, int r0, int c0, 
 // buf: 4 KB of LDS, this wave's; both: the image itself too
 template <int KIND>
 __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, const Added &x,
-                                        int r0, int c0, char *buf, int lane, bool both) {
+                                        int r0, int c0, char *buf, int lane, bool both, bool to_w) {
   if (r0 >= o.rows || c0 >= o.cols) return;
   f32x4 v[4];
 #pragma unroll
@@ -690,23 +690,36 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
       v[i][j] = acc[i * 4 + j] * (o.by * DOWN2);
       if (KIND != GRAM) v[i][j] += o.times * (1.f / UP) * ((float)x.h[i][j] + (float)x.l[i][j]);
     }
-  if (KIND == LAST) {
-    const int col = c0 + (lane & 31);
-    if (col >= o.cols) return;
+  if (KIND == STEP && to_w) {
+    // (as values of their own: the compiler would read `rate` with its neighbours as a
+    // vector, for that put M into LDS, and fetch the launch's packet from the host's
+    // memory to find its place there: 10 us a launch)
+    float rate = M.rate, keep = M.keep;
+    asm("" : "+s"(rate), "+s"(keep));
+    // what is read is on its way at once: behind the last row or column, theirs
+    const int col = c0 + (lane & 31), row = r0 + (lane >> 5) * 4, c = col < o.cols ? col : o.cols - 1;
+    if (M.turned && r0 + 32 <= o.rows) {
+      float *w = M.w + (long)c * o.rows + row;
+      f32x4 old[4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int row = r0 + 8 * i + (lane >> 5) * 4;
-      if (M.turned && row + 4 <= o.rows) {
-        float *w = M.w + (long)col * o.rows + row;
-        *(f32x4_any *)w = M.v ? *(const f32x4_any *)w * M.keep + v[i] * M.rate : v[i];
-      } else {
+      for (int i = 0; i < 4; i++)
+        if (M.v) old[i] = *(const f32x4_any *)(w + 8 * i) * keep;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (row + j < o.rows) {
-            float *w = M.w + (M.turned ? (long)col * o.rows + row + j : (long)(row + j) * o.cols + col);
-            *w = M.v ? *w * M.keep + v[i][j] * M.rate : v[i][j];
-          }
-      }
+      for (int i = 0; i < 4; i++)
+        if (col < o.cols) *(f32x4_any *)(w + 8 * i) = M.v ? old[i] + v[i] * rate : v[i];
+      return;
+    }
+    const long down = M.turned ? 1 : o.cols, start = M.turned ? (long)c * o.rows : c;
+    float old[16] = {};
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int r = row + 8 * (i / 4) + i % 4;
+      if (M.v) old[i] = M.w[start + (r < o.rows ? r : o.rows - 1) * down] * keep;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int r = row + 8 * (i / 4) + i % 4;
+      if (col < o.cols && r < o.rows) M.w[start + r * down] = M.v ? old[i] + v[i / 4][i % 4] * rate : v[i / 4][i % 4];
     }
     return;
   }
@@ -767,13 +780,11 @@ struct Deal {
 };
 
 template <int KIND, int T, int BUFFERS, int N>
-__global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUFFERS>::WAVES / 4)) tile_kernel(Matrices<N> a, int step, Deal deal, float *pieces) {
+__global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUFFERS>::WAVES / 4)) tile_kernel(Matrices<N> a, int step, int to_w, Deal deal, float *pieces) {
   typedef Shape<T, BUFFERS> S;
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * S::BUFFER];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // consecutive workgroups go to the eight XCDs in turn: give each XCD a run of them
-  const unsigned groups = gridDim.x, each = groups / 8, b = blockIdx.x;
-  const unsigned w = b < each * 8 ? (b % 8) * each + b / 8 : b;
+  const unsigned groups = gridDim.x, w = dealt(blockIdx.x, groups);
   const unsigned to = lds_address(lds);
   unsigned round = 0;
   for (unsigned long u = 0, end = 0;;) {
@@ -932,8 +943,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
       for (int f = 0; f < S::BLOCKS; f++) {
         if (f + 1 < S::BLOCKS) next = added<KIND>(o, row_of<T>(ti, wave, f + 1), col_of<T>(tj, wave, f + 1), lane);
         write32<KIND>(M, o, acc[f / 2][f % 2], x, row_of<T>(ti, wave, f), col_of<T>(tj, wave, f), lds + wave * 4096, lane,
-                      KIND == STEP || ti != tj);
-        __builtin_amdgcn_wave_barrier();
+                      KIND == STEP || ti != tj, to_w);
         x = next;
       }
     } else {
@@ -954,7 +964,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
 // tile_kernel's workgroup w begins, where that is the first to begin inside it; a
 // wave has 32 x 32 of its values.
 template <int KIND, int T, int N>
-__global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal deal, const float *pieces) {
+__global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int to_w, Deal deal, const float *pieces) {
   typedef Shape<T, 2> S;
   __shared__ __attribute__((aligned(1024))) char buf[4][4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -983,7 +993,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, Deal
       for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
     }
   }
-  write32<KIND>(M, o, acc, x, r0, c0, buf[wave], lane, KIND == STEP || ti != tj);
+  write32<KIND>(M, o, acc, x, r0, c0, buf[wave], lane, KIND == STEP || ti != tj, to_w);
 }
 
 // ---------------------------------------------------------------- host
@@ -1039,15 +1049,21 @@ bool by_block(const Matrices<N> &a) {
 }
 
 // How a product of such matrices goes: by tiles of 32 (0), 128 or 256, by its work, m m
-// and its length, in all of them (us for five steps, all products alike):
-//   tiles of            32    128    256
-//   2 x 1024^2         321    363      -
-//   1500^2             657    445    650
-//   2048^2            1170    685    876
-//   3 x 2048^2           -   1863   2036
-//   2048 x 8192          -   2019   1892
-//   4096^2           10300   3886   3867
-//   8192^2               -  33066  26650
+// and its length, in all of them.  Of a symmetric result half is computed, and tiles
+// of 32 are used for longer.  us of a product, with what joins its parts:
+//                      P = X X^T            X <- a X + Q X
+//   tiles of         32   128   256        32   128   256
+//   1024^2           11    19     -        15    20     -
+//   700 x 4000       15    21     -        26    24     -
+//   2 x 1024^2       17    20     -        27    26     -
+//   1400^2           18    22     -        33    28     -
+//   1600^2           25    27     -        45    40     -
+//   1024 x 4096      37    26     -        56    30     -
+//   2048^2            -    41    55         -    54    78
+//   2500^2            -    75    75         -   118   115
+//   2048 x 4096       -    78    78         -   109   122
+//   3000 x 5000       -   144   152         -   301   249
+//   2048 x 8192       -   158   117         -   182   189
 template <int N>
 int tile_size(const Matrices<N> &a, int kind) {
   double work = 0;
@@ -1057,19 +1073,19 @@ int tile_size(const Matrices<N> &a, int kind) {
     work += (double)M.m * M.m * (kind == SQUARE ? M.m : M.n);
     widest = M.m > widest ? M.m : widest;
   }
-  return work < 2.8e9 ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
+  return work < (kind == STEP ? 2e9 : 4e9) ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
 }
 
 template <int KIND, int N>
-void small_product(Matrices<N> &a, int step) {
+void small_product(Matrices<N> &a, int step, int to_w) {
   const unsigned long grid = number(a, [](const Matrix &M) {
     return KIND <= SQUARE ? blocks_of(M.m) * (blocks_of(M.m) + 1) / 2 : blocks_of(M.m) * blocks_of(M.n);
   });
-  hipLaunchKernelGGL((small_kernel<KIND, N>), dim3((unsigned)grid), dim3(512), 0, stream(), a, step);
+  hipLaunchKernelGGL((small_kernel<KIND, N>), dim3((unsigned)grid), dim3(512), 0, stream(), a, step, to_w);
 }
 
 template <int KIND, int T, int BUFFERS, int N>
-void tile_product(Matrices<N> &a, int step, float *pieces) {
+void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
   typedef Shape<T, BUFFERS> S;
   bool alike = true;  // in their blocks
   long blocks = 0;
@@ -1100,18 +1116,18 @@ void tile_product(Matrices<N> &a, int step, float *pieces) {
     if (!d.units) d.sharers = 0;
     else if (shared <= even) d.sharers = (unsigned)(rest * ways);
   }
-  hipLaunchKernelGGL((tile_kernel<KIND, T, BUFFERS, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, d, pieces);
+  hipLaunchKernelGGL((tile_kernel<KIND, T, BUFFERS, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, to_w, d, pieces);
   if (d.sharers > 1)
-    hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, d,
+    hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, to_w, d,
                        (const float *)pieces);
 }
 
 template <int KIND, int N>
-void product(Matrices<N> &a, int step, float *pieces) {
+void product(Matrices<N> &a, int step, float *pieces, int to_w = 0) {
   const int tile = tile_size(a, KIND);
-  if (tile == 0) small_product<KIND, N>(a, step);
-  else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, pieces);
-  else tile_product<KIND, 256, 2, N>(a, step, pieces);
+  if (tile == 0) small_product<KIND, N>(a, step, to_w);
+  else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, to_w, pieces);
+  else tile_product<KIND, 256, 2, N>(a, step, to_w, pieces);
 }
 
 template <int N>
@@ -1127,8 +1143,7 @@ void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
   for (int s = 0; s < steps; s++) {
     product<GRAM, N>(a, s, (float *)rest);
     product<SQUARE, N>(a, s, (float *)rest);
-    if (s + 1 < steps) product<STEP, N>(a, s, (float *)rest);
-    else product<LAST, N>(a, s, (float *)rest);
+    product<STEP, N>(a, s, (float *)rest, s + 1 == steps);
   }
 }
 
@@ -1136,7 +1151,7 @@ void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
 template <int N>
 size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
-  const int t = tile_size(a, GRAM);  // of the longest product
+  const int g = tile_size(a, GRAM), s = tile_size(a, STEP), t = g > s ? g : s;  // (SQUARE: no longer than GRAM)
   return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * 256);
 }
 
