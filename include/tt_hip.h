@@ -505,7 +505,7 @@ int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows
  * values s to a s + b s^3 + c s^5.  y may be x.  A matrix with an infinity or a
  * NaN has NaN throughout.  Sides at most 2^20, rows * cols 2^32.  ws: 256-byte
  * aligned; about 14 bytes a value of up to 64 matrices, 20 of square ones, and up
- * to 128 MiB; none (size 0) where a matrix fits a CU's LDS. */
+ * to 128 MiB; none (size 0) where small matrices are kept in LDS. */
 #define TT_NS_A 3.4445f
 #define TT_NS_B (-4.7750f)
 #define TT_NS_C 2.0315f

@@ -165,6 +165,20 @@ def test_steps_of_many(tlib, count, rows, cols):
     assert (ws.to_np()[-16:] == -7).all()
 
 
+@pytest.mark.parametrize("count", [3, 31, 32, 40])
+def test_steps_of_many_with_blocks(tlib, count):
+    """Matrices of many blocks that fit LDS: together they have a workgroup each from 32
+    on, and fewer of them go product by product."""
+    rows, cols = 95, 300
+    assert (tlib.tt_k_newton_schulz_ws(count, rows, cols) == 0) == (count >= 32)
+    x = np.stack([_matrix(rows, cols, seed=i) for i in range(count)])
+    got = _steps(tlib, x, 5)
+    for i in {0, 1, count // 2, count - 1}:
+        want, off = ref.newton_schulz(x[i], 5)
+        assert np.linalg.norm(got[i] - want) <= off
+        assert np.linalg.norm(got[i] - want) <= NEAR * np.linalg.norm(want)
+
+
 def _ptrs(ds):
     return (ctypes.c_void_p * len(ds))(*[d.ptr for d in ds])
 

@@ -21,8 +21,8 @@
 // instructions take them, four times 1 KB: h of the columns 0 to 15, where lane l
 // has eight of row l % 32 from column 8 (l / 32) on, of the columns 16 to 31, and l
 // of both; zeros behind the last row and column.  A wave's load is then 1 KB in one
-// piece (rows of 128 bytes, 32 of them a load, take the address unit 40 cycles: 16 x
-// 4000 20 us a product instead of 6).  Both operands of a product are read along
+// piece (rows of 128 bytes, 32 of them a load, take the address unit 40 cycles: three
+// times as long a product of 16 x 4000).  Both operands of a product are read along
 // rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -136,7 +136,8 @@ __device__ __forceinline__ void put16(char *image, long blocks, int r, int c, co
 // launch.  A wave has blocks of 32 x 32 of each result, kept in registers until all
 // have read what they replace.  X^T is X read by transposing loads.  The products
 // are formed transposed: a lane then holds four neighbours of a row, and P and Q
-// are symmetric.
+// are symmetric.  Latency bounds it, of LDS and between the products of a chain: five
+// steps of 32 x 32 take 23 us, of 64 x 64 26, of 128 x 128 63, of 64 of these 65.
 
 constexpr int BLOCK_WAVES = 16, BLOCK_LDS = 160 * 1024 - 256;
 constexpr int BLOCK_KEEP = 3;  // blocks of X a wave
@@ -145,8 +146,12 @@ __host__ __device__ inline long block_bytes(int m, int n) {
   const long mb = blocks_of(m), nb = blocks_of(n);
   return 4096 * (mb * nb + mb * mb + (mb == 1 ? 7 : mb == 2 ? 4 : 0));
 }
-inline bool fits_block(int m, int n) {
-  return block_bytes(m, n) <= BLOCK_LDS && blocks_of(m) * blocks_of(n) <= BLOCK_WAVES * BLOCK_KEEP;
+// Of a few matrices those whose products have up to 64 blocks (five steps of 128 x 128:
+// 63 us, and 72 by launches of a product each; of 128 x 160 72 and 70, of 96 x 300 84
+// and 71), of many all that fit (32 of 96 x 300: 85 and 82, 500 of 128 x 128: 145 and 683).
+inline bool fits_block(int m, int n, int count) {
+  const long mb = blocks_of(m), nb = blocks_of(n);
+  return block_bytes(m, n) <= BLOCK_LDS && mb * nb <= BLOCK_WAVES * BLOCK_KEEP && (count >= 32 || mb * mb * nb <= 64);
 }
 
 // Chunk (16 bytes) c of a block's eight in row r lies at c ^ (r / 2 % 8), and odd
@@ -385,6 +390,7 @@ __global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices<N> a, 
 
 // v = mu v + g, and the sum of squares of u = g + mu v (nesterov) or v; without
 // momenta of g.  In 64 bits: the squares of any fp32 values are within its range.
+// Bound by memory: 26 us for a block's weights of 12.6 million values (5.8 TB/s).
 template <int N>
 __global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, int nesterov) {
   __shared__ double sums[4];
@@ -418,7 +424,8 @@ __global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, 
 }
 
 // The images of U / |U|_F and its transpose, a tile of 64 x 64 at a time through
-// LDS; both are written along their rows.
+// LDS; both are written along their rows.  Bound by memory: 36 us for 4096 x 4096
+// (5.6 TB/s).
 template <int N>
 __global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int nesterov) {
   __shared__ double sums[4];
@@ -536,7 +543,9 @@ __device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int
 // instructions take them and each wave with a share of the products' length:
 // eight sums, joined in LDS.  What bounds these is the way from memory (the L2 of
 // another XCD has what the last launch wrote), so the added matrix is on its way
-// first, and a tile on the diagonal reads its rows once.
+// first, and a tile on the diagonal reads its rows once.  A launch takes 4 us at least;
+// 517 x 1003: 6 us for P, 5 for Q, 10 for X; 1300 x 1300: 18, 18 and 29 (450 TFLOP/s
+// of fp16 products).
 template <int KIND, int N>
 __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step, int to_w) {
   typedef _Float16 half2 __attribute__((ext_vector_type(2)));
@@ -617,13 +626,19 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step, 
 
 // ---------------------------------------------------------------- large products
 //
-// Tiles of 128 x 128, four waves with a quarter each, the operands through LDS in
-// two buffers of a block (32 of the products' length): while one is multiplied the
-// next is on its way by direct loads.  Per block and wave 24 matrix instructions
-// stand against 16 KB read from LDS, and two workgroups a CU fill each other's
-// waits.  The tiles' blocks are dealt evenly to the workgroups, whatever the
-// matrices' shapes: a workgroup has whole tiles and at most two pieces of tiles
-// that others have the rest of.  Pieces go to memory, and join_kernel adds them.
+// The operands come through LDS by direct loads, a block (32 of the products' length)
+// at a time, in buffers.  In the 32 cycles of a 32 x 32 x 16 product LDS gives a SIMD one
+// of its two operands, so a wave has as large a tile as its registers hold, and what it
+// reads goes into several products:
+//   tiles of 128  four waves of 64 x 64, one a SIMD, three buffers: a block is on its
+//                 way while two are there, and the reads stand between the products
+//   tiles of 256  eight waves of 128 x 64, two a SIMD, two buffers: the other wave of
+//                 the SIMD fills a wave's waits, and memory gives half as much
+// A tile that one workgroup has is finished by it.  The others' parts go to memory,
+// and join_kernel adds them.  The matrix units bound these, at the clock that they
+// leave: X of 4096 x 4096 takes 343 us, 1200 TFLOP/s of fp16 products, with the units
+// 69 % busy at 1.84 GHz; of 2048 x 2048 by tiles of 128 50 us, 1030 TFLOP/s (51 % busy
+// at 2 GHz in a transformer block's six matrices).
 
 // Tiles of T x T: four waves of 64 x 64 or eight of 128 x 64 values, each FI x 2
 // blocks of 32 x 32.
@@ -963,6 +978,8 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
 // Workgroups (w - 1, .) add the pieces of the tile in which the share of
 // tile_kernel's workgroup w begins, where that is the first to begin inside it; a
 // wave has 32 x 32 of its values.
+// Bound by memory (4096 x 4096: 33 us for 100 MB of parts and 36 of results) or by its
+// own latency (7 us at 1024 x 1024).
 template <int KIND, int T, int N>
 __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int to_w, Deal deal, const float *pieces) {
   typedef Shape<T, 2> S;
@@ -1044,7 +1061,7 @@ unsigned long number(Matrices<N> &a, F workgroups) {
 template <int N>
 bool by_block(const Matrices<N> &a) {
   for (int i = 0; i < (N > 1 ? a.count : 1); i++)
-    if (!fits_block(a.at[i].m, a.at[i].n)) return false;
+    if (!fits_block(a.at[i].m, a.at[i].n, a.count)) return false;
   return true;
 }
 
@@ -1131,8 +1148,8 @@ void product(Matrices<N> &a, int step, float *pieces, int to_w = 0) {
 }
 
 template <int N>
-void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest) {
-  if (by_block(a)) {
+void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *rest) {
+  if (blocks) {
     hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov);
     return;
   }
@@ -1184,12 +1201,13 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
     if (!ws) return -2;
   }
   Matrices<1> a = alike(count, rows, cols, (char *)ws);
-  const int most = by_block(a) ? 1 << 20 : a.count;  // without images any number at once
+  const bool blocks = by_block(a);  // (of the last group too, however few are left for it)
+  const int most = blocks ? 1 << 20 : a.count;  // without images any number at once
   for (long base = 0; base < count; base += most) {
     a.count = (int)(count - base < most ? count - base : most);
     a.at[0].g = x + base * rows * cols;
     a.at[0].w = y + base * rows * cols;
-    run(a, steps, 0.f, 0, (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images);
+    run(a, blocks, steps, 0.f, 0, (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images);
   }
   ttrt_free(own);
   return launched();
@@ -1237,7 +1255,7 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
     M.rate = (float)(-(double)lr * TT_MUON_RMS * sqrt((double)(rows[i] > cols[i] ? rows[i] : cols[i])));
     lay(M, rows[i], cols[i], at);
   }
-  run(a, TT_MUON_STEPS, mu, nesterov, at);
+  run(a, by_block(a), TT_MUON_STEPS, mu, nesterov, at);
   ttrt_free(own);
   return launched();
 }
