@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(256)
 
 // s = x + res (res may be NULL), written to sum unless NULL, and its RMS norm.
 // sum may be res or x: a thread reads its own columns before it writes them, and
-// of another's it keeps nothing.
+// of another's it keeps nothing.  Bound by memory: 22 us for 8192 x 1024 with both
+// (6.1 TB/s), 89 for 4096 x 8192 (6.0); one row of 1024 2.7.
 template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(threads_of(NT))
     rms_fwd_kernel(const float *x, const float *res, const float *__restrict__ w, float *__restrict__ y, float *sum,
@@ -369,7 +370,9 @@ __global__ void __launch_bounds__(threads_of(NT))
 }
 
 // dx (which may be ds), and (part) this workgroup's sums over its rows for dw:
-// part[block][cols]
+// part[block][cols].  Bound by memory: 22 us for 8192 x 1024 (6.2 TB/s), 115 for 4096 x
+// 8192 (4.7: one workgroup a CU, for the sums of dw stay in its registers).  TAIL with
+// rows past 8192 columns spills: 346 us for 2000 x 16383, 246 for 2000 x 16384.
 template <int NT, int NV, bool TAIL>
 __global__ void __launch_bounds__(threads_of(NT))
     rms_bwd_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ dy,
