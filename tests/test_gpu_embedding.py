@@ -155,6 +155,31 @@ def test_embedding_node(tlib, bound):
         Node.leaf(w.reshape(13, 3, 2)).embedding(b)
 
 
+@pytest.mark.parametrize("bound", ["ctypes", "pybind"])
+def test_embedding_node_wide_ids(tlib, bound):
+    """Ids past 32 bits are outside the table, whatever their low bits are."""
+    if bound == "ctypes":
+        from tinytorch_amd.torch_py import Node
+    else:
+        import sys
+        import tinytorch_amd
+        if tinytorch_amd.BUILD not in sys.path:
+            sys.path.insert(0, tinytorch_amd.BUILD)
+        from tinytorch_pybind import Node
+    rng = np.random.default_rng(10)
+    w, dy = rng.standard_normal((9, 5)).astype(np.float32), rng.standard_normal((6, 5)).astype(np.float32)
+    ids = np.array([[4, 2**32 + 4, -2**32 + 1], [2**31, -1, 8]])
+    W = Node.leaf(w)
+    y = W.embedding(ids)
+    y.backward(dy)
+    want = np.zeros((6, 5), np.float32)
+    want[0], want[5] = w[4], w[8]
+    grad = np.zeros((9, 5), np.float32)
+    grad[4], grad[8] = dy[0], dy[5]
+    assert np.array_equal(y.value(), want) and np.array_equal(W.grad(), grad)
+    assert np.array_equal(W.embedding([4, 8]).value(), w[[4, 8]])
+
+
 def test_embedding_gradient_by_differences(tlib):
     rng = np.random.default_rng(9)
     ids, dy = _tokens(rng, 60, 17, "padded"), rng.standard_normal((60, 7)).astype(np.float32)

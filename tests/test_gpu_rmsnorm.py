@@ -193,6 +193,36 @@ def test_rmsnorm_node(tlib, bound, needs, has):
         assert first is not None
 
 
+@pytest.mark.parametrize("bound", ["ctypes", "pybind"])
+def test_rmsnorm_node_twice(tlib, bound):
+    """One node as x and as the residual: the sum is twice it, and its gradient has
+    both; and one node as x and as the weight."""
+    if bound == "ctypes":
+        from tinytorch_amd.torch_py import Node
+    else:
+        import sys
+        import tinytorch_amd
+        if tinytorch_amd.BUILD not in sys.path:
+            sys.path.insert(0, tinytorch_amd.BUILD)
+        from tinytorch_pybind import Node
+    x, _, w, dy, _ = _inputs(5, 21)
+    X = Node.leaf(x)
+    y, s = X.rmsnorm(Node.leaf(w, False), X)
+    y.backward(dy)
+    want = ref.rmsnorm(x, x, w, dy)
+    close(y.value(), want[0])
+    assert np.array_equal(s.value(), 2 * x)
+    close(X.grad(), (2 * want[3][0], 2 * want[3][1]))
+    W = Node.leaf(w)
+    y = W.rmsnorm(W)
+    y.backward(dy[0])
+    want = ref.rmsnorm(w[None], None, w, dy[:1])
+    close(y.value(), (want[0][0][0], want[0][1][0]))
+    dx, dw = want[3], want[4]
+    both = dx[0][0] + dw[0]
+    close(W.grad(), (both, dx[1][0] + dw[1] + ref.U * np.abs(both)))
+
+
 def test_rmsnorm_node_refuses(tlib):
     from tinytorch_amd.torch_py import Node
     x, res, w, _, _ = _inputs(4, 8)

@@ -152,8 +152,12 @@ class PyNode {
     if (residual.is_none()) return py::cast(y);
     return py::make_tuple(y, PyNode(sum));
   }
-  PyNode embedding(IntArr ids, float scale) {
-    return PyNode(ag_embedding(get(), ids.data(), (long)ids.size(), scale));
+  // wider ids are outside the table, not what their low 32 bits say
+  PyNode embedding(py::array_t<int64_t, py::array::c_style | py::array::forcecast> ids, float scale) {
+    std::vector<int> tokens((size_t)ids.size());
+    for (size_t i = 0; i < tokens.size(); i++)
+      tokens[i] = ids.data()[i] == (int)ids.data()[i] ? (int)ids.data()[i] : -1;
+    return PyNode(ag_embedding(get(), tokens.data(), (long)tokens.size(), scale));
   }
   PyNode rope(int heads, int head_dim, py::object positions, long seq_len, py::object rot_dim, bool interleaved,
               double base, int scaling, double factor, double trained, double low, double high,

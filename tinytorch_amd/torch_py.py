@@ -159,8 +159,10 @@ class Node:
     def embedding(self, ids, scale=1.0):
         """scale times this table's rows at ids (any shape, flattened); an id outside
         the table: a row of zeros."""
-        ids = np.ascontiguousarray(ids, dtype=np.int32)
-        return Node(_checked(LIB.ag_embedding(self.ptr, ids.ctypes.data, ids.size, scale), "ag_embedding"))
+        ids = np.asarray(ids, dtype=np.int64)
+        tokens = ids.astype(np.int32, order="C")
+        tokens[tokens != ids] = -1  # not what the low 32 bits say
+        return Node(_checked(LIB.ag_embedding(self.ptr, tokens.ctypes.data, tokens.size, scale), "ag_embedding"))
 
     def rope(self, heads, head_dim, positions=None, seq_len=0, rot_dim=None, interleaved=False, base=10000.0,
              scaling=0, factor=1.0, trained=0.0, low=0.0, high=0.0, magnitude=1.0):
