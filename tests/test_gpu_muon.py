@@ -227,6 +227,27 @@ def test_muon_step(tlib, shapes, nesterov):
             assert np.array_equal(G[i].to_np(s), g[i])
 
 
+@pytest.mark.parametrize("shapes", [[(1500, 1600), (1400, 5), (2000, 900), (60, 1900), (900, 900), (40, 3000)],
+                                    [(2200, 6300), (6000, 9), (33, 2100), (500, 400)]])
+def test_muon_step_large_and_small(tlib, shapes):
+    """Tiles of many lengths of product, dealt to workgroups together."""
+    rng = np.random.default_rng(5)
+    w, g, v = ([rng.standard_normal(s).astype(np.float32) for s in shapes] for _ in range(3))
+    W, G, V = ([DevBuf.from_np(t) for t in ts] for ts in (w, g, v))
+    rows, cols = _long([s[0] for s in shapes]), _long([s[1] for s in shapes])
+    need = tlib.tt_k_muon_multi_ws(rows, cols, len(shapes)) // 4
+    ws = DevBuf(need + 16)
+    ws.fill(np.nan)
+    lr, mu, decay = np.float32(0.02), np.float32(0.95), np.float32(0.1)
+    check(tlib.tt_k_muon_multi(_ptrs(W), _ptrs(G), _ptrs(V), rows, cols, len(shapes), lr, mu, 1, decay, ws.ptr), "muon")
+    assert np.isnan(ws.to_np()[need:]).all()
+    for i, s in enumerate(shapes):
+        want, _, tol = _muon64(w[i], g[i], v[i], float(lr), float(mu), 1, float(decay))
+        got = W[i].to_np(s)
+        assert np.linalg.norm(got - want) <= tol
+        assert np.linalg.norm(got - want) <= 2 * NEAR * np.linalg.norm(want - w[i]) + 4 * ref.U * np.linalg.norm(w[i])
+
+
 @pytest.mark.parametrize("rows,cols", [(70, 90), (270, 390)])
 def test_muon_workspace_allocates_nothing(tlib, rows, cols):
     """The smaller needs none."""

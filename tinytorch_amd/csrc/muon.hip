@@ -784,9 +784,12 @@ __device__ __forceinline__ int col_of(int tj, int wave, int f) {
   return tj * T + (wave % Shape<T, 2>::ACROSS) * 64 + f % 2 * 32;
 }
 // How the units (tiles' blocks, tile by tile) are dealt: `rounds` whole tiles to every
-// workgroup, then the units from `base` on evenly to the first `sharers`.
+// workgroup, then the units from `base` on evenly to the first `sharers`.  A tile has
+// `extra` units before those of its blocks, for what it costs besides (with products of
+// one block among long ones a workgroup had dozens of them: X of 2375 x 1041 and 1503 x
+// 570 32 us, and with 3989 x 5 and three more small ones 94).
 struct Deal {
-  unsigned rounds, sharers;
+  unsigned rounds, sharers, extra;
   unsigned long base, units;
   // the first of workgroup w's share
   __device__ __forceinline__ unsigned long begins(unsigned w) const {
@@ -821,10 +824,14 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
     unsigned long in = u;
     const Matrix M = matrix_of(a, in);
     const Operands<KIND> o(M, step);
-    const long blocks = blocks_of(o.k);
+    const int extra = N > 1 ? deal.extra : 0;
+    const long blocks = blocks_of(o.k), units = blocks + extra;
     int ti, tj;
-    tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
-    const int k0 = (int)(in % blocks), k1 = (int)(end - u < (unsigned long)(blocks - k0) ? k0 + (end - u) : blocks);
+    tile_of<KIND, T>(in / units, o.rows, o.cols, ti, tj);
+    const int r0 = (int)(in % units), r1 = (int)(end - u < (unsigned long)(units - r0) ? r0 + (end - u) : units);
+    u += r1 - r0;
+    if (r1 <= extra) continue;  // none of its blocks
+    const int k0 = r0 < extra ? 0 : r0 - extra, k1 = r1 - extra;
     // a wave brings every WAVES-th KB of the tiles' T / 32 blocks; a block behind the
     // last is the last once more: its results are not written
     constexpr int EACH = S::EACH;
@@ -971,7 +978,6 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
         p[i * 64] = v;
       }
     }
-    u += n;
   }
 }
 
@@ -990,10 +996,11 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int 
   unsigned long in = u;
   const Matrix M = matrix_of(a, in);
   const Operands<KIND> o(M, step);
-  const unsigned long blocks = blocks_of(o.k), k0 = in % blocks, first = u - k0, last = first + blocks;
-  if (k0 == 0 || deal.begins(w - 1) > first) return;
+  const unsigned extra = N > 1 ? deal.extra : 0;
+  const unsigned long units = blocks_of(o.k) + extra, first = u - in % units, last = first + units;
+  if (u <= first + extra || deal.begins(w - 1) > first + extra) return;
   int ti, tj;
-  tile_of<KIND, T>(in / blocks, o.rows, o.cols, ti, tj);
+  tile_of<KIND, T>(in / units, o.rows, o.cols, ti, tj);
   const int block = blockIdx.y * 4 + wave;
   const int r0 = row_of<T>(ti, block / S::BLOCKS, block % S::BLOCKS), c0 = col_of<T>(tj, block / S::BLOCKS, block % S::BLOCKS);
   const Added x = added<KIND>(o, r0, c0, lane);
@@ -1104,17 +1111,22 @@ void small_product(Matrices<N> &a, int step, int to_w) {
 template <int KIND, int T, int BUFFERS, int N>
 void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
   typedef Shape<T, BUFFERS> S;
-  bool alike = true;  // in their blocks
-  long blocks = 0;
+  constexpr int EXTRA = T == 128 ? 12 : 6;  // (2375 x 1041 with five: 598 us with 4, 569 with 8, 559 with 12)
+  auto tiles_of = [](const Matrix &M) {
+    const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T;
+    return KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc;
+  };
+  auto length = [](const Matrix &M) { return blocks_of(KIND == GRAM ? M.n : M.m); };
+  const long blocks = length(a.at[0]);
+  bool alike = true;
   unsigned long tiles = 0;
+  for (int i = 0; i < (N > 1 ? a.count : 1); i++) {
+    alike = alike && length(a.at[i]) == blocks;
+    tiles += tiles_of(a.at[i]) * (N > 1 ? 1 : a.count);
+  }
   Deal d = {};
-  d.units = number(a, [&](const Matrix &M) {
-    const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T, k = blocks_of(KIND == GRAM ? M.n : M.m);
-    alike = alike && (!blocks || blocks == k);
-    blocks = k;
-    tiles += (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * (N > 1 ? 1 : a.count);
-    return (KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc) * k;
-  });
+  d.extra = alike ? 0 : EXTRA;
+  d.units = number(a, [&](const Matrix &M) { return tiles_of(M) * (length(M) + d.extra); });
   const unsigned groups = (unsigned)(d.units < S::GROUPS ? d.units : S::GROUPS);
   d.sharers = (unsigned)(d.units < 8ul * groups ? (d.units + 7) / 8 : groups);
   if (alike) {
