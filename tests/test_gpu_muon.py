@@ -66,6 +66,25 @@ def test_steps(tlib, rows, cols, kind):
         assert off <= NEAR * np.linalg.norm(want), (steps, off / np.linalg.norm(want))
 
 
+@pytest.mark.parametrize("rows,cols", [(5, 4000), (3101, 60), (100, 8000), (40, 70001), (220, 3500)])
+def test_one_step_long(tlib, rows, cols):
+    """Few rows of a long product: its length is shared."""
+    x = _matrix(rows, cols)
+    want, tol = ref.one_step(*ref.normed(x))
+    if rows > cols:
+        want, tol = want.T, tol.T
+    got = _steps(tlib, x, 1)
+    assert (np.abs(got - want) <= tol + ref.U * np.abs(want)).all(), np.max(np.abs(got - want) / tol)
+    ws = DevBuf(tlib.tt_k_newton_schulz_ws(1, rows, cols) // 4 + 16)
+    ws.fill(np.nan)
+    assert np.array_equal(got, _steps(tlib, x, 1, ws.ptr))
+    assert np.isnan(ws.to_np()[-16:]).all()
+    want, tol = ref.newton_schulz(x, 5)
+    got = _steps(tlib, np.stack([x, x[::-1], x]), 5)
+    for g, w in zip(got, (want, want[::-1], want)):
+        assert np.linalg.norm(g - w) <= min(tol, NEAR * np.linalg.norm(want))
+
+
 @pytest.mark.parametrize("rows,cols", [(1430, 1400), (1060, 2600)])
 def test_one_step_large(tlib, rows, cols):
     """By tiles of 128: value by value."""
@@ -228,6 +247,7 @@ def test_muon_step(tlib, shapes, nesterov):
 
 
 @pytest.mark.parametrize("shapes", [[(1500, 1600), (1400, 5), (2000, 900), (60, 1900), (900, 900), (40, 3000)],
+                                    [(64, 4000), (30, 50), (129, 3300), (5000, 9)],
                                     [(2200, 6300), (6000, 9), (33, 2100), (500, 400)]])
 def test_muon_step_large_and_small(tlib, shapes):
     """Tiles of many lengths of product, dealt to workgroups together."""

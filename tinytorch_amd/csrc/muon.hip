@@ -32,6 +32,7 @@
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;
@@ -545,13 +546,20 @@ __device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int
 // another XCD has what the last launch wrote), so the added matrix is on its way
 // first, and a tile on the diagonal reads its rows once.  A launch takes 4 us at least;
 // 517 x 1003: 6 us for P, 5 for Q, 10 for X; 1300 x 1300: 18, 18 and 29 (450 TFLOP/s
-// of fp16 products).
-template <int KIND, int N>
-__global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step, int to_w) {
+// of fp16 products).  Of few long tiles of P the length is shared by `ways` workgroups,
+// whose sums a second launch adds (join): a CU alone brings 80 GB/s.
+template <int KIND, bool SHARED, int N>
+__global__ void __launch_bounds__(512, 2)
+    small_kernel(Matrices<N> a, int step, int to_w, int ways, bool join, float *pieces) {
   typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   constexpr int WAVES = 8;
   __shared__ float sums[WAVES][32][33];
-  unsigned t = dealt(blockIdx.x, gridDim.x);
+  unsigned t = dealt(blockIdx.x, gridDim.x), way = 0;
+  f32x2 *piece = nullptr;
+  if (SHARED) {
+    piece = (f32x2 *)pieces + (join ? t * ways : t) * 512l + threadIdx.x;
+    if (!join) way = t % ways, t /= ways;
+  }
   const Matrix M = matrix_of(a, t);
   const Operands<KIND> o(M, step);
   int ti, tj;
@@ -566,35 +574,49 @@ __global__ void __launch_bounds__(512, 2) small_kernel(Matrices<N> a, int step, 
 #pragma unroll
     for (int e = 0; e < 2; e++) v[e] = o.times * (1.f / UP) * ((float)h[e] + (float)l[e]);
   }
-  const int blocks = (int)blocks_of(o.k);
-  const char *pa = o.a + (long)ti * blocks * 4096 + lane * 16, *pb = o.b + (long)tj * blocks * 4096 + lane * 16;
-  f32x16 acc = {};
-  const bool same = KIND <= SQUARE && ti == tj;
-  for (int k = wave; k < blocks; k += WAVES) {
-    half8 x[4], y[4];
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      x[s] = *(const half8 *)(pa + k * 4096l + s * 1024);
-      y[s] = x[s];
+  float sum[2] = {0.f, 0.f};
+  if (SHARED && join) {
+#pragma unroll 8
+    for (int w = 0; w < ways; w++) {
+      const f32x2 p = piece[w * 512l];
+      sum[0] += p[0], sum[1] += p[1];
     }
-    if (!same) {
+  } else {
+    const int blocks = (int)blocks_of(o.k);
+    const char *pa = o.a + (long)ti * blocks * 4096 + lane * 16, *pb = o.b + (long)tj * blocks * 4096 + lane * 16;
+    f32x16 acc = {};
+    const bool same = KIND <= SQUARE && ti == tj;
+    for (int k = way * WAVES + wave; k < blocks; k += (SHARED ? ways : 1) * WAVES) {
+      half8 x[4], y[4];
 #pragma unroll
-      for (int s = 0; s < 4; s++) y[s] = *(const half8 *)(pb + k * 4096l + s * 1024);
+      for (int s = 0; s < 4; s++) {
+        x[s] = *(const half8 *)(pa + k * 4096l + s * 1024);
+        y[s] = x[s];
+      }
+      if (!same) {
+#pragma unroll
+        for (int s = 0; s < 4; s++) y[s] = *(const half8 *)(pb + k * 4096l + s * 1024);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; s++) three(acc, x[s], x[2 + s], y[s], y[2 + s]);
     }
 #pragma unroll
-    for (int s = 0; s < 2; s++) three(acc, x[s], x[2 + s], y[s], y[2 + s]);
+    for (int i = 0; i < 16; i++) sums[wave][8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) sum[e] += sums[w][r][c + e];
+    if (SHARED) {
+      *piece = (f32x2){sum[0], sum[1]};
+      return;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 16; i++) sums[wave][8 * (i / 4) + 4 * (lane >> 5) + i % 4][lane & 31] = acc[i];
-  __syncthreads();
   bool in[2];
 #pragma unroll
   for (int e = 0; e < 2; e++) {
     in[e] = row < o.rows && col + e < o.cols;
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) s += sums[w][r][c + e];
-    v[e] = in[e] ? v[e] + s * (o.by * DOWN2) : 0.f;
+    v[e] = in[e] ? v[e] + sum[e] * (o.by * DOWN2) : 0.f;
   }
   if (KIND == STEP && to_w) {
 #pragma unroll
@@ -1100,12 +1122,28 @@ int tile_size(const Matrices<N> &a, int kind) {
   return work < (kind == STEP ? 2e9 : 4e9) ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
 }
 
+// Workgroups that share tiles of 32, and blocks of the products' length from which on
+// they do (P of 100 x 8000: 21 us by one each, 5.5 twice shared; five steps of 108 x
+// 3940 114 and 102, of 64 x 2000, 63 blocks, 86 and 87).
+constexpr int SHARERS = 512, LONG = 97;
+
 template <int KIND, int N>
-void small_product(Matrices<N> &a, int step, int to_w) {
-  const unsigned long grid = number(a, [](const Matrix &M) {
+void small_product(Matrices<N> &a, int step, int to_w, float *pieces) {
+  const unsigned grid = (unsigned)number(a, [](const Matrix &M) {
     return KIND <= SQUARE ? blocks_of(M.m) * (blocks_of(M.m) + 1) / 2 : blocks_of(M.m) * blocks_of(M.n);
   });
-  hipLaunchKernelGGL((small_kernel<KIND, N>), dim3((unsigned)grid), dim3(512), 0, stream(), a, step, to_w);
+  if constexpr (KIND == GRAM) {
+    long length = 0;
+    for (int i = 0; i < (N > 1 ? a.count : 1); i++) length = length < blocks_of(a.at[i].n) ? blocks_of(a.at[i].n) : length;
+    const long most = length / 16 < 32 ? length / 16 : 32, ways = SHARERS / grid < most ? SHARERS / grid : most;
+    if (length >= LONG && ways > 1) {
+      for (int join = 0; join < 2; join++)
+        hipLaunchKernelGGL((small_kernel<KIND, true, N>), dim3(join ? grid : grid * (unsigned)ways), dim3(512), 0,
+                           stream(), a, step, to_w, (int)ways, join, pieces);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((small_kernel<KIND, false, N>), dim3(grid), dim3(512), 0, stream(), a, step, to_w, 1, false, pieces);
 }
 
 template <int KIND, int T, int BUFFERS, int N>
@@ -1154,7 +1192,7 @@ void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
 template <int KIND, int N>
 void product(Matrices<N> &a, int step, float *pieces, int to_w = 0) {
   const int tile = tile_size(a, KIND);
-  if (tile == 0) small_product<KIND, N>(a, step, to_w);
+  if (tile == 0) small_product<KIND, N>(a, step, to_w, pieces);
   else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, to_w, pieces);
   else tile_product<KIND, 256, 2, N>(a, step, to_w, pieces);
 }
@@ -1176,12 +1214,12 @@ void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *r
   }
 }
 
-// the images (of a group of matrices), and two pieces a workgroup
+// the images (of a group of matrices), and two pieces a workgroup, or one of a small tile
 template <int N>
 size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
   const int g = tile_size(a, GRAM), s = tile_size(a, STEP), t = g > s ? g : s;  // (SQUARE: no longer than GRAM)
-  return images + (t == 0 ? 0 : 2 * sizeof(float) * t * t * 256);
+  return images + sizeof(float) * (t == 0 ? 1024 * SHARERS : 2 * t * t * 256);
 }
 
 // `count` matrices of one shape
