@@ -547,7 +547,7 @@ __device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int
 // first, and a tile on the diagonal reads its rows once.  A launch takes 4 us at least;
 // 517 x 1003: 6 us for P, 5 for Q, 10 for X; 1300 x 1300: 18, 18 and 29 (450 TFLOP/s
 // of fp16 products).  Of few long tiles of P the length is shared by `ways` workgroups,
-// whose sums a second launch adds (join): a CU alone brings 80 GB/s.
+// whose sums a second launch adds (join): one CU alone reads 80 GB/s.
 template <int KIND, bool SHARED, int N>
 __global__ void __launch_bounds__(512, 2)
     small_kernel(Matrices<N> a, int step, int to_w, int ways, bool join, float *pieces) {
@@ -1123,9 +1123,9 @@ int tile_size(const Matrices<N> &a, int kind) {
 }
 
 // Workgroups that share tiles of 32, and blocks of the products' length from which on
-// they do (P of 100 x 8000: 21 us by one each, 5.5 twice shared; five steps of 108 x
-// 3940 114 and 102, of 64 x 2000, 63 blocks, 86 and 87).
-constexpr int SHARERS = 512, LONG = 97;
+// they do (P of 100 x 8000: 21 us by one each, twice 5.5 shared; five steps of 64 x 2000
+// 86 and 79, of 256 x 1500 96 and 99, of 256 x 2000 103 both ways, of 256 x 3000 119 and 116)
+constexpr int SHARERS = 512, LONG = 60;
 
 template <int KIND, int N>
 void small_product(Matrices<N> &a, int step, int to_w, float *pieces) {
