@@ -127,6 +127,17 @@ def test_steps_large(tlib, shape, steps):
     assert np.isnan(ws.to_np()[-more:]).all()
 
 
+@pytest.mark.parametrize("m,n,count", [(3300, 3400, 1), (4430, 4450, 2)])
+def test_one_step_larger(tlib, m, n, count):
+    """The symmetric products by tiles of 128 where the last one is by 256, and by 256."""
+    x = np.random.default_rng(8).standard_normal((m, n)).astype(np.float32)
+    got = _steps(tlib, np.stack([x] * count), 1)
+    want = _steps64(x, 1)
+    for g in got:
+        assert np.linalg.norm(g - want) <= NEAR * np.linalg.norm(want)
+        assert np.abs(g - want).max() <= 40 * NEAR * np.sqrt((want**2).mean())
+
+
 def test_steps_take_singular_values(tlib):
     """From known singular vectors: a s + b s^3 + c s^5, five times."""
     rng = np.random.default_rng(3)
@@ -248,7 +259,7 @@ def test_muon_step(tlib, shapes, nesterov):
 
 @pytest.mark.parametrize("shapes", [[(1500, 1600), (1400, 5), (2000, 900), (60, 1900), (900, 900), (40, 3000)],
                                     [(64, 4000), (30, 50), (129, 3300), (5000, 9)],
-                                    [(2200, 6300), (6000, 9), (33, 2100), (500, 400)]])
+                                    [(2200, 6300), (6000, 9), (33, 2100), (500, 400)], [(3250, 3260), (40, 50)]])
 def test_muon_step_large_and_small(tlib, shapes):
     """Tiles of many lengths of product, dealt to workgroups together."""
     rng = np.random.default_rng(5)

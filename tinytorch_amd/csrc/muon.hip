@@ -1006,8 +1006,8 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
 // Workgroups (w - 1, .) add the pieces of the tile in which the share of
 // tile_kernel's workgroup w begins, where that is the first to begin inside it; a
 // wave has 32 x 32 of its values.
-// Bound by memory (4096 x 4096: 33 us for 100 MB of parts and 36 of results) or by its
-// own latency (7 us at 1024 x 1024).
+// Bound by memory (P of 6000 x 6000, tiles of 256: 20 us) or by its own latency (8 to 12
+// us for tiles of 128).
 template <int KIND, int T, int N>
 __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int to_w, Deal deal, const float *pieces) {
   typedef Shape<T, 2> S;
@@ -1094,9 +1094,16 @@ bool by_block(const Matrices<N> &a) {
   return true;
 }
 
+// blocks of a product's length
+long length_of(int kind, const Matrix &M) { return blocks_of(kind == GRAM ? M.n : M.m); }
+
 // How a product of such matrices goes: by tiles of 32 (0), 128 or 256, by its work, m m
-// and its length, in all of them.  Of a symmetric result half is computed, and tiles
-// of 32 are used for longer.  us of a product, with what joins its parts:
+// and its length, in all of them.  Of a symmetric result half is computed, and smaller
+// tiles are used for longer: they have less to compute twice, and their parts are joined
+// sooner.  But few tiles of 128 (136 of 2048 rows), or tiles of different lengths, are
+// cut into parts that are not in step, so that each XCD reads all of it from afar (two of
+// 4096^2, 1024 x 4096 and its turn: 9137 us with tiles of 256, 9798 with 128).  us of a
+// product, with what joins its parts:
 //                      P = X X^T            X <- a X + Q X
 //   tiles of         32   128   256        32   128   256
 //   1024^2           11    19     -        15    20     -
@@ -1108,18 +1115,29 @@ bool by_block(const Matrices<N> &a) {
 //   2048^2            -    41    55         -    54    78
 //   2500^2            -    75    75         -   118   115
 //   2048 x 4096       -    78    78         -   109   122
-//   3000 x 5000       -   144   152         -   301   249
+//   2200 x 6300       -   108   120         -   194   195
+//   3000 x 5000       -   147   159         -   297   251
 //   2048 x 8192       -   158   117         -   182   189
+//   2100 x 12000      -   205   196         -   370   340
+//   4096^2            -   198   219         -   391   348
+//   4096 x 8192       -   378   385         -   789   682
+//   6000^2            -   610   590         -  1359  1117
+//   8192^2            -  1511  1326         -  3459  2533
 template <int N>
 int tile_size(const Matrices<N> &a, int kind) {
-  double work = 0;
+  double work = 0, tiles = 0;  // (of 128)
   int widest = 0;
+  bool together = kind != STEP;  // of a symmetric result, and in step
   for (int i = 0; i < a.count; i++) {
     const Matrix &M = a.at[N > 1 ? i : 0];
+    const double nr = (M.m + 127) / 128;
     work += (double)M.m * M.m * (kind == SQUARE ? M.m : M.n);
+    tiles += nr * (nr + 1) / 2;
+    together = together && length_of(kind, M) == length_of(kind, a.at[0]);
     widest = M.m > widest ? M.m : widest;
   }
-  return work < (kind == STEP ? 2e9 : 4e9) ? 0 : work < 3e10 || widest < 2048 ? 128 : 256;
+  if (work < (kind == STEP ? 2e9 : 4e9)) return 0;
+  return work < (together && tiles >= 160 ? 1.7e11 : 3e10) || widest < 2048 ? 128 : 256;
 }
 
 // Workgroups that share tiles of 32, and blocks of the products' length from which on
@@ -1154,17 +1172,16 @@ void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
     const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T;
     return KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc;
   };
-  auto length = [](const Matrix &M) { return blocks_of(KIND == GRAM ? M.n : M.m); };
-  const long blocks = length(a.at[0]);
+  const long blocks = length_of(KIND, a.at[0]);
   bool alike = true;
   unsigned long tiles = 0;
   for (int i = 0; i < (N > 1 ? a.count : 1); i++) {
-    alike = alike && length(a.at[i]) == blocks;
+    alike = alike && length_of(KIND, a.at[i]) == blocks;
     tiles += tiles_of(a.at[i]) * (N > 1 ? 1 : a.count);
   }
   Deal d = {};
   d.extra = alike ? 0 : EXTRA;
-  d.units = number(a, [&](const Matrix &M) { return tiles_of(M) * (length(M) + d.extra); });
+  d.units = number(a, [&](const Matrix &M) { return tiles_of(M) * (length_of(KIND, M) + d.extra); });
   const unsigned groups = (unsigned)(d.units < S::GROUPS ? d.units : S::GROUPS);
   d.sharers = (unsigned)(d.units < 8ul * groups ? (d.units + 7) / 8 : groups);
   if (alike) {
@@ -1218,7 +1235,7 @@ void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *r
 template <int N>
 size_t ws_of(const Matrices<N> &a, size_t images) {
   if (by_block(a)) return 0;
-  const int g = tile_size(a, GRAM), s = tile_size(a, STEP), t = g > s ? g : s;  // (SQUARE: no longer than GRAM)
+  const int g = tile_size(a, GRAM), s = tile_size(a, STEP), t = g > s ? g : s;  // (SQUARE's: no larger than these)
   return images + sizeof(float) * (t == 0 ? 1024 * SHARERS : 2 * t * t * 256);
 }
 
