@@ -503,7 +503,10 @@ int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows
  * x (rows x cols, one behind the other): X = x / |x|_F (zeros: zeros), then
  * `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X, which takes singular
  * values s to a s + b s^3 + c s^5.  y may be x.  A matrix with an infinity or a
- * NaN has NaN throughout.  Sides at most 2^20, rows * cols 2^32.  ws: 256-byte
+ * NaN has NaN throughout.  The products take operands of 22 bits (two fp16 parts,
+ * with a scale for each row and column) and sums of 32: every row and every column
+ * is off by about what fp32 products leave of its own size, also where it is much
+ * weaker than the others (but for those under 2^-100 of the whole).  Sides at most 2^20, rows * cols 2^32.  ws: 256-byte
  * aligned; about 14 bytes a value of up to 64 matrices, 20 of square ones, and up
  * to 128 MiB; none (size 0) where small matrices are kept in LDS. */
 #define TT_NS_A 3.4445f

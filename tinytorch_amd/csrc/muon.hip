@@ -9,13 +9,24 @@
 // [0.68, 1.21].  P and P P are symmetric: half of their tiles are computed.
 //
 // The products take fp32 results from the fp16 matrix units, which are 16 times as
-// fast as the fp32 ones: a value times 2^14 is h + l, two fp16 numbers (l what h
-// leaves), 22 bits, and h h' + h l' + l h' has all of the product but l l', 2^-22
-// of it.  That is what fp32 sums of these lengths leave too: against 64 bits both
-// are off by 1e-6 to 9e-6 (what the steps make of the first rounding).  2^14
-// keeps both in the type's range: s stays under 1.21, so the values of X, P and Q
-// are within 1.21, 1.46 and 2.81 (46100 of 65504 times 2^14), and l is exact to
-// 2^-38.
+// fast as the fp32 ones: a value is h + l, two fp16 numbers (l what h leaves), 22
+// bits, and h h' + h l' + l h' has all of the product but l l', 2^-22 of it.  The
+// rounding of the operands so is 4 times fp32's, and what the sums of these lengths
+// leave is of the same size.
+//
+// fp16 has few exponents: under 2^-17 of the largest value the parts lose bits.  So
+// each row of an operand has a scale of its own, a power of two D_i over the norm of
+// X's row i, or F_j over its column j's (without them a row 1e7 times weaker than the
+// others was off by 2e-3 of itself, and is by 1e-6):
+//   G = D^-1 X,  T = F^-1 X^T,  C = G G^T
+//   image of P:  C D               (D^-1 P; what the rows of P P are made of)
+//   image of Q:  (b C + c (C D)(C D)^T) D     (D^-1 Q)
+//   X <- a X + D (image of Q) T^T F
+// The polynomial divided by s lies within [0.64, 3.4445], so a row or column grows by
+// no more than that a step, and to no more than 1.21: the scales are measured once,
+// with `room` for that, 2 at most.  Then the rows of the images have norms under 1,
+// 1.21 and 2.82, and times 2^14 their values (46200) are within the type.  After
+// MOST_STEPS such steps X begins anew from its fp32 values.
 //
 // X, X^T, P and Q are kept as images: blocks of 32 x 32 values as the matrix
 // instructions take them, four times 1 KB: h of the columns 0 to 15, where lane l
@@ -36,6 +47,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+typedef unsigned short Scale;  // the upper half of a power of two
+typedef Scale scale2 __attribute__((ext_vector_type(2)));
+typedef Scale scale4 __attribute__((ext_vector_type(4)));
 
 inline hipStream_t stream() { return (hipStream_t)ttrt_stream(); }
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
@@ -44,17 +58,37 @@ constexpr float UP = 16384.f, DOWN2 = 1.f / (16384.f * 16384.f);
 constexpr int MOST = TT_SGD_MAX;   // matrices of different shapes in one run of launches
 constexpr int ALIKE = 64;          // of one shape
 constexpr int NORM_PARTS = 1024;   // sums of squares of a matrix
+constexpr int MOST_STEPS = 6;      // with the scales measured before the first
+
+__host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
 
 struct Matrix {
   const float *g;   // what is orthogonalised, or the gradient (rows x cols)
-  float *v, *w;     // momenta and weights; v NULL: the result goes to w
-  char *x, *t0, *t1;  // images of X (m rows), X^T (n rows; the steps write one from the other)
-  char *p, *q;      // of P and Q
-  double *norm;     // NORM_PARTS partial sums of squares
-  float keep, rate; // w = keep w + rate X
+  float *v, *w;     // momenta (or NULL) and weights
+  char *base;       // the matrix's workspace
+  long side, square;  // bytes of an image of X, and of P
+  float keep, rate; // w = keep w + rate X where `onto`, else X
   int m, n;         // shorter and longer side
-  int turned;       // more rows than columns: X is U^T
+  short turned;     // more rows than columns: X is U^T
+  short onto;
   int parts;        // of the norm
+  // Images of G (m rows), of T (n rows; the steps write one from the other), of P and Q.
+  __device__ char *x() const { return base; }
+  __device__ char *t(int odd) const { return base + side + (odd ? side : 0); }
+  __device__ char *p() const { return base + side * 3; }
+  __device__ char *q() const { return p() + square; }
+  // D and F, of whole blocks
+  __device__ Scale *d() const { return (Scale *)(q() + square); }
+  __device__ Scale *f() const { return d() + blocks_of(m) * 32; }
+  // partial sums of squares, and behind them what X = U times
+  __device__ double *norm() const { return (double *)(f() + blocks_of(n) * 32); }
+  // and of rows and columns, in 64 of the other: where the second T comes to lie
+  __device__ double *of_rows() const { return (double *)t(1); }
+  __device__ double *of_cols() const { return of_rows() + (long)(turned ? n : m) * (((turned ? m : n) + 63) / 64); }
+  __host__ long bytes() const {
+    const long all = 3 * side + 2 * square + 64 * (blocks_of(m) + blocks_of(n)) + 8 * (NORM_PARTS + 1);
+    return (all + 255) / 256 * 256;
+  }
 };
 // N matrices, or with N = 1 `count` of at[0]'s shape one behind the other.  (A kernel's
 // arguments come from afar: of the longer form each line that it needs costs it 0.5 us.)
@@ -66,17 +100,13 @@ struct Matrices {
   long images;  // N = 1: bytes of a matrix's workspace
 };
 
-__host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
-
 // which matrix a workgroup or unit belongs to; b becomes its number among that one's
 template <int N>
 __device__ __forceinline__ Matrix matrix(const Matrices<N> &a, int i) {
   if (N > 1) return a.at[i];
   Matrix M = a.at[0];
   M.g += (long)i * M.m * M.n, M.w += (long)i * M.m * M.n;
-  const long off = i * a.images;
-  M.x += off, M.t0 += off, M.t1 += off, M.p += off, M.q += off;
-  M.norm += off / (long)sizeof(double);
+  M.base += i * a.images;
   return M;
 }
 template <int N, class U>
@@ -92,37 +122,51 @@ __device__ __forceinline__ Matrix matrix_of(const Matrices<N> &a, U &b) {
   return matrix(a, i);
 }
 
-// x 2^14 in two parts
-__device__ __forceinline__ void split(float y, _Float16 &h, _Float16 &l) {
-  h = (_Float16)y;
-  l = (_Float16)(y - (float)h);
+// The scales: powers of two, at or over the norms.  (A row of zeros has one that
+// sends none to its column's scale, a column of zeros one that sends none to its rows'.)
+constexpr float OF_NO_ROW = 2.f, OF_NO_COLUMN = 0x1p-100f;
+__device__ __forceinline__ Scale scale_over(float norm, unsigned room, float of_none) {
+  const unsigned up = (__float_as_uint(norm) + 0x7fffffu) & 0x7f800000u;
+  const float x = norm > 0.f ? fminf(fmaxf(__uint_as_float(up), 0x1p-100f) * __uint_as_float(0x3f800000u + room), 2.f) : of_none;
+  return (Scale)(__float_as_uint(x) >> 16);
 }
-// where h of row r and column c of an image lies (l 1024 values further)
+// what a row or column may grow by before the last of such steps, in a float's exponent
+inline unsigned room_for(int steps) { return (steps < 6 ? 2u * (steps - 1) : 9u) << 23; }
+__device__ __forceinline__ float value_of(Scale scale) { return __uint_as_float((unsigned)scale << 16); }
+// 1 / x and 2^14 / x of a power of two
+__device__ __forceinline__ float inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+__device__ __forceinline__ float inverse_up(float x) { return __uint_as_float(0x86000000u - __float_as_uint(x)); }
+// y times a power of two in two parts (multiply-adds, whose results are halves)
+__device__ __forceinline__ void split(float y, float scale, _Float16 &h, _Float16 &l) {
+  h = (_Float16)fmaf(y, scale, 0.f);
+  l = (_Float16)fmaf(y, scale, -(float)h);
+}
+// where h of row r and column c of a block lies, in bytes (l 2048 further), and of an image
+__host__ __device__ __forceinline__ unsigned inner(unsigned r, unsigned c) {
+  return (c >> 4) * 1024 + (r + (c >> 3 & 1) * 32) * 16 + (c & 7) * 2;
+}
 __device__ __forceinline__ _Float16 *place(char *image, long blocks, int r, int c) {
-  return (_Float16 *)(image + ((r >> 5) * blocks + (c >> 5)) * 4096 + (c >> 4 & 1) * 1024 +
-                      ((r & 31) + (c >> 3 & 1) * 32) * 16) +
-         (c & 7);
+  return (_Float16 *)(image + ((r >> 5) * blocks + (c >> 5)) * 4096 + inner(r & 31, c & 31));
 }
-// two values of row r from the even column c on
-__device__ __forceinline__ void put2(char *image, long blocks, int r, int c, float x, float y) {
+// two neighbours of a row, times these
+__device__ __forceinline__ void put2(char *p, float x, float y, float sx, float sy) {
   typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   half2 h, l;
   _Float16 a, b;
-  split(x * UP, a, b);
+  split(x, sx, a, b);
   h[0] = a, l[0] = b;
-  split(y * UP, a, b);
+  split(y, sy, a, b);
   h[1] = a, l[1] = b;
-  _Float16 *p = place(image, blocks, r, c);
   *(half2 *)p = h;
-  *(half2 *)(p + 1024) = l;
+  *(half2 *)(p + 2048) = l;
 }
-// 16 values (times 2^14 already) of row r from column c on, a multiple of 16
-__device__ __forceinline__ void put16(char *image, long blocks, int r, int c, const float (&v)[16]) {
+// 16 values, times scale, of row r from column c on, a multiple of 16
+__device__ __forceinline__ void put16(char *image, long blocks, int r, int c, const float (&v)[16], float scale) {
   half8 h[2], l[2];
 #pragma unroll
   for (int j = 0; j < 16; j++) {
     _Float16 a, b;
-    split(v[j], a, b);
+    split(v[j], scale, a, b);
     h[j / 8][j % 8] = a;
     l[j / 8][j % 8] = b;
   }
@@ -132,33 +176,43 @@ __device__ __forceinline__ void put16(char *image, long blocks, int r, int c, co
 
 // ---------------------------------------------------------------- small matrices
 //
-// A matrix whose image of X and of P or Q (which follow each other in one place) fit
-// LDS has a workgroup, which takes it from the gradient to the weights in one
+// A matrix that fits LDS, X and the image of P or Q (which follow each other in one
+// place), has a workgroup, which takes it from the gradient to the weights in one
 // launch.  A wave has blocks of 32 x 32 of each result, kept in registers until all
-// have read what they replace.  X^T is X read by transposing loads.  The products
-// are formed transposed: a lane then holds four neighbours of a row, and P and Q
-// are symmetric.  Latency bounds it, of LDS and between the products of a chain: five
-// steps of 32 x 32 take 23 us, of 64 x 64 26, of 128 x 128 63, of 64 of these 65.
+// have read what they replace.  X^T is X read by transposing loads.  The products are
+// formed transposed: a lane then holds four neighbours of a row, and P and Q are
+// symmetric.
+// X is an image without scales where it is even: the largest values of its weakest row
+// and of its weakest column (zeros aside) have a product of EVEN or more.  The values
+// where these two meet are then off by 2^-17 of themselves at most, whole rows and
+// columns by less than the sums leave.  Else X are fp32 values, whose parts are made as
+// they are read, by rows with their scales for C and by columns with theirs for the
+// step; the scales come from the largest value of a row and its length (five steps of
+// 64 x 64: 26 us and 32, 500 of 128 x 128 157 and 214).
+// Latency bounds it, of LDS and between the products of a chain: five steps of 32 x 32
+// take 22 us, of 64 x 64 26, of 96 x 96 46, of 64 of 64 x 64 27.
 
-constexpr int BLOCK_WAVES = 16, BLOCK_LDS = 160 * 1024 - 256;
+constexpr int BLOCK_WAVES = 16, BLOCK_LDS = 39 * 4096;
 constexpr int BLOCK_KEEP = 3;  // blocks of X a wave
+constexpr float EVEN = 0x1p-22f;
 // X, P and the partial sums of P (one or four blocks of it: eight or two waves each)
 __host__ __device__ inline long block_bytes(int m, int n) {
   const long mb = blocks_of(m), nb = blocks_of(n);
   return 4096 * (mb * nb + mb * mb + (mb == 1 ? 7 : mb == 2 ? 4 : 0));
 }
-// Of a few matrices those whose products have up to 64 blocks (five steps of 128 x 128:
-// 63 us, and 72 by launches of a product each; of 128 x 160 72 and 70, of 96 x 300 84
-// and 71), of many all that fit (32 of 96 x 300: 85 and 82, 500 of 128 x 128: 145 and 683).
+// Of a few matrices those whose products have up to 48 blocks (five steps of 96 x 96:
+// 46 us, and 59 by launches of a product each; of 128 x 128 66 and 60), of many all that
+// fit (32 of 96 x 300: 86 and 79, 500 of 128 x 128: 157 and 739).
 inline bool fits_block(int m, int n, int count) {
   const long mb = blocks_of(m), nb = blocks_of(n);
-  return block_bytes(m, n) <= BLOCK_LDS && mb * nb <= BLOCK_WAVES * BLOCK_KEEP && (count >= 32 || mb * mb * nb <= 64);
+  return block_bytes(m, n) <= BLOCK_LDS && mb * nb <= BLOCK_WAVES * BLOCK_KEEP && (count >= 32 || mb * mb * nb <= 48);
 }
 
 // Chunk (16 bytes) c of a block's eight in row r lies at c ^ (r / 2 % 8), and odd
 // rows begin in the other half of the banks: where a row has an even number of
 // blocks, neighbouring ones change places there.  No two of the lanes that LDS
-// serves at once meet a bank (128 x 128: 71 us with half of them in one).
+// serves at once meet a bank (128 x 128: 71 us with half of them in one).  X has four
+// values a chunk, an image in the first four h and in the others l.
 __device__ __forceinline__ const char *chunk_of(const char *image, int blocks, int r, int block, int c) {
   block ^= r & ~blocks & 1;
   return image + (r * blocks + block) * 128 + ((c ^ (r >> 1 & 7)) << 4);
@@ -173,7 +227,10 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ s16x4 read_transposed(const char *p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p));
 }
-// eight rows r0 + 8 (lane / 32) .. of column lane % 32 of a block
+struct Parts {
+  half8 h, l;
+};
+// eight rows r0 + 8 (lane / 32) .. of column lane % 32 of an image's block
 __device__ __forceinline__ half8 across(const char *image, int blocks, int r0, int block, int part, int lane) {
   s16x8 v;
   const int l = lane & 15, c = (lane >> 4 & 1) * 16 + 4 * (l & 3);
@@ -186,12 +243,45 @@ __device__ __forceinline__ half8 across(const char *image, int blocks, int r0, i
   }
   return __builtin_bit_cast(half8, v);
 }
+__device__ __forceinline__ Parts parts_of(const float (&v)[8], float scale) {
+  Parts x;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    _Float16 a, b;
+    split(v[j], scale, a, b);
+    x.h[j] = a, x.l[j] = b;
+  }
+  return x;
+}
+// of X's values: eight columns of row r0 + lane % 32, times scale
+__device__ __forceinline__ Parts row_parts(const char *X, int blocks, int r0, int block, int half, float scale, int lane) {
+  float v[8];
+#pragma unroll
+  for (int x = 0; x < 2; x++) {
+    const f32x4 w = *(const f32x4 *)chunk_of(X, blocks, r0 + (lane & 31), block, half * 4 + (lane >> 5) * 2 + x);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[x * 4 + j] = w[j];
+  }
+  return parts_of(v, scale);
+}
+// eight rows r0 + 8 (lane / 32) .. of column lane % 32 of a block, times scale
+__device__ __forceinline__ Parts column_parts(const char *X, int blocks, int r0, int block, float scale, int lane) {
+  float v[8];
+#pragma unroll
+  for (int x = 0; x < 8; x++)
+    v[x] = *(const float *)(chunk_of(X, blocks, r0 + (lane >> 5) * 8 + x, block, lane >> 2 & 7) + (lane & 3) * 4);
+  return parts_of(v, scale);
+}
 __device__ __forceinline__ void three(f32x16 &acc, half8 ha, half8 la, half8 hb, half8 lb) {
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(la, hb, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha, lb, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ha, hb, acc, 0, 0, 0);
 }
-// four values of row r from column c on, and back
+// four values of row r from column c on: of X's values, and of an image (times 2^-14) and
+// back, times these
+__device__ __forceinline__ f32x4 *x4(char *X, int blocks, int r, int c) {
+  return (f32x4 *)const_cast<char *>(chunk_of(X, blocks, r, c >> 5, c >> 2 & 7));
+}
 __device__ __forceinline__ f32x4 get4(const char *image, int blocks, int r, int c) {
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   const half4 h = *(const half4 *)(chunk_of(image, blocks, r, c >> 5, c >> 3 & 3) + (c & 4) * 2);
@@ -201,13 +291,13 @@ __device__ __forceinline__ f32x4 get4(const char *image, int blocks, int r, int 
   for (int j = 0; j < 4; j++) v[j] = ((float)h[j] + (float)l[j]) * (1.f / UP);
   return v;
 }
-__device__ __forceinline__ void put4(char *image, int blocks, int r, int c, f32x4 v) {
+__device__ __forceinline__ void put4(char *image, int blocks, int r, int c, f32x4 v, f32x4 scale) {
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   half4 h, l;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     _Float16 a, b;
-    split(v[j] * UP, a, b);
+    split(v[j], scale[j], a, b);
     h[j] = a, l[j] = b;
   }
   *(half4 *)(chunk_of(image, blocks, r, c >> 5, c >> 3 & 3) + (c & 4) * 2) = h;
@@ -227,15 +317,163 @@ __device__ __forceinline__ V momentum(const float *g, float *v, float mu, int ne
   return nesterov ? w * mu + u : w;
 }
 
+// The steps of X in LDS and the result to w; VALUES: X are fp32 values, else an image.
+template <bool VALUES>
+__device__ __forceinline__ void steps_in_lds(const Matrix &M, int steps, char *lds, const Scale *scales, int lane, int wave) {
+  const int mb = (int)blocks_of(M.m), nb = (int)blocks_of(M.n);
+  char *const X = lds, *const P = lds + mb * nb * 4096, *const rest = P + mb * mb * 4096;
+  for (int step = 0;; step++) {
+    __syncthreads();
+    // the lane as the compiler does not know it from step to step: it would keep every
+    // address of the loop in registers, and spill them
+    asm volatile("" : "+v"(lane));
+    auto of_row = [&](int r) { return VALUES ? value_of(scales[r]) : 1.f; };
+    auto of_rows = [&](int r) {  // four of them
+      if (!VALUES) return (f32x4){1.f, 1.f, 1.f, 1.f};
+      const scale4 x = *(const scale4 *)(scales + r);
+      return (f32x4){value_of(x[0]), value_of(x[1]), value_of(x[2]), value_of(x[3])};
+    };
+    const int low = lane & 31, high = (lane >> 5) * 4;  // result i: values high + 8 (i / 4) + i % 4 of row low
+    // C = G G^T: with one block of it (four) eight waves (two) share the sum
+    const int pb = mb * mb, ways = mb == 1 ? 8 : mb == 2 ? 2 : 1;
+    f32x4 c4[4];
+    {
+      const int f = wave % pb, way = wave / pb, ra = f / mb * 32, rb = f % mb * 32;
+      f32x16 acc = {};
+      if (way < ways) {
+        const float da = inverse_up(of_row(ra + low)), db = inverse_up(of_row(rb + low));
+#pragma unroll 1
+        for (int k = way; k < nb; k += ways)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if constexpr (VALUES) {
+              const Parts x = row_parts(X, nb, ra, k, h, da, lane);
+              Parts y = x;
+              if (ra != rb) y = row_parts(X, nb, rb, k, h, db, lane);
+              three(acc, x.h, x.l, y.h, y.l);
+            } else {
+              three(acc, along(X, nb, ra, k, h, 0, lane), along(X, nb, ra, k, h, 1, lane), along(X, nb, rb, k, h, 0, lane),
+                    along(X, nb, rb, k, h, 1, lane));
+            }
+          }
+        if (way > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            *(f32x4 *)(rest + (((way - 1) * pb + f) * 4 + i) * 1024 + lane * 16) =
+                (f32x4){acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
+        }
+      }
+      if (ways > 1) __syncthreads();
+      if (way == 0) {
+#pragma unroll 1
+        for (int w = 1; w < ways; w++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const f32x4 v = *(const f32x4 *)(rest + (((w - 1) * pb + f) * 4 + i) * 1024 + lane * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
+          }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          c4[i] = (f32x4){acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]} * DOWN2;
+          put4(P, mb, rb + low, ra + high + 8 * i, c4[i], of_rows(ra + high + 8 * i) * UP);
+        }
+      }
+    }
+    __syncthreads();
+    {  // the image of Q, in P's place
+      const bool on = wave < pb;
+      const int f = on ? wave : 0, ra = f / mb * 32, rb = f % mb * 32;
+      f32x16 acc = {};
+      if (on) {
+#pragma unroll 1
+        for (int k = 0; k < mb; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            three(acc, along(P, mb, ra, k, h, 0, lane), along(P, mb, ra, k, h, 1, lane), along(P, mb, rb, k, h, 0, lane),
+                  along(P, mb, rb, k, h, 1, lane));
+      }
+      __syncthreads();
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x4 v = {acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
+          const f32x4 q = c4[i] * TT_NS_B + v * (TT_NS_C * DOWN2);
+          put4(P, mb, rb + low, ra + high + 8 * i, q, of_rows(ra + high + 8 * i) * UP);
+        }
+      }
+    }
+    __syncthreads();
+    asm volatile("" : "+v"(lane));
+    // X^T <- a X^T + X^T Q: block f has the columns f % nb of X and its rows f / nb
+    f32x16 acc[BLOCK_KEEP] = {};
+#pragma unroll
+    for (int b = 0; b < BLOCK_KEEP; b++) {
+      const int f = wave + b * BLOCK_WAVES, r0 = f / nb * 32, cb = f % nb;
+      if (f >= mb * nb) continue;
+      const float column = inverse_up(of_row(mb * 32 + cb * 32 + low)), row = of_row(r0 + low) * DOWN2;
+#pragma unroll 1
+      for (int k = 0; k < mb; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          Parts x;
+          if constexpr (VALUES) x = column_parts(X, nb, k * 32 + h * 16, cb, column, lane);
+          else x.h = across(X, nb, k * 32 + h * 16, cb, 0, lane), x.l = across(X, nb, k * 32 + h * 16, cb, 1, lane);
+          three(acc[b], x.h, x.l, along(P, mb, r0, k, h, 0, lane), along(P, mb, r0, k, h, 1, lane));
+        }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int c = cb * 32 + high + 8 * i;
+        const f32x4 v = (VALUES ? *x4(X, nb, r0 + low, c) : get4(X, nb, r0 + low, c)) * TT_NS_A;
+        const f32x4 columns = of_rows(mb * 32 + c);
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[b][i * 4 + j] = v[j] + acc[b][i * 4 + j] * row * columns[j];
+      }
+    }
+    if (step + 1 == steps) {
+#pragma unroll
+      for (int b = 0; b < BLOCK_KEEP; b++) {
+        const int f = wave + b * BLOCK_WAVES, row = f / nb * 32 + low;
+        if (f >= mb * nb || row >= M.m) continue;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int col = f % nb * 32 + high + 8 * (i / 4) + i % 4;
+          if (col >= M.n) continue;
+          float *w = M.w + (M.turned ? col * M.m + row : row * M.n + col);
+          *w = M.onto ? M.keep * *w + M.rate * acc[b][i] : acc[b][i];
+        }
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < BLOCK_KEEP; b++) {
+      const int f = wave + b * BLOCK_WAVES;
+      if (f >= mb * nb) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 v = {acc[b][i * 4], acc[b][i * 4 + 1], acc[b][i * 4 + 2], acc[b][i * 4 + 3]};
+        const int r = f / nb * 32 + low, c = f % nb * 32 + high + 8 * i;
+        if (VALUES) *x4(X, nb, r, c) = v;
+        else put4(X, nb, r, c, v, (f32x4){UP, UP, UP, UP});
+      }
+    }
+  }
+}
+
+// `again`: X is what is given, without its norm.
 template <int N>
-__global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices<N> a, int steps, float mu, int nesterov) {
+__global__ void __launch_bounds__(BLOCK_WAVES * 64)
+    block_kernel(Matrices<N> a, int steps, float mu, int nesterov, int again, unsigned room) {
   __shared__ __attribute__((aligned(1024))) char lds[BLOCK_LDS];
+  __shared__ Scale scales[(4 + 31) * 32];  // of 4 blocks of rows and 31 of columns
   __shared__ double sums[BLOCK_WAVES];
+  __shared__ float least[2][BLOCK_WAVES];
   const Matrix M = matrix(a, blockIdx.x);
-  int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int mb = (int)blocks_of(M.m), nb = (int)blocks_of(M.n), count = M.m * M.n, cols = M.turned ? M.m : M.n;
-  char *const X = lds, *const P = lds + mb * nb * 4096, *const rest = P + mb * mb * 4096;
+  char *const X = lds;
   constexpr int THREADS = BLOCK_WAVES * 64;
   for (int i = threadIdx.x * 16; i < mb * nb * 4096; i += THREADS * 16) *(f32x4 *)(X + i) = (f32x4){0.f, 0.f, 0.f, 0.f};
   double s = 0.0;
@@ -256,13 +494,10 @@ __global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices<N> a, 
   s = 0.0;
 #pragma unroll
   for (int k = 0; k < BLOCK_WAVES; k++) s += sums[k];
-  const double scale = s == 0.0 ? 0.0 : (double)UP / sqrt(s);  // zeros stay zeros
+  const double scale = again ? 1.0 : s == 0.0 ? 0.0 : 1.0 / sqrt(s);  // zeros stay zeros
   auto place1 = [&](int i, float u) {
     const int r = i / cols, c = i % cols, row = M.turned ? c : r, col = M.turned ? r : c;
-    _Float16 h, l;
-    split((float)((double)u * scale), h, l);
-    *(_Float16 *)(chunk_of(X, nb, row, col >> 5, col >> 3 & 3) + (col & 7) * 2) = h;
-    *(_Float16 *)(chunk_of(X, nb, row, col >> 5, 4 + (col >> 3 & 3)) + (col & 7) * 2) = l;
+    ((float *)x4(X, nb, row, col & ~3))[col & 3] = (float)((double)u * scale);
   };
   for (int i = threadIdx.x * 4; i + 4 <= count; i += THREADS * 4) {  // what this thread wrote itself
     const f32x4 u = momentum<f32x4_any>(M.g + i, M.v ? M.v + i : nullptr, mu, nesterov, false);
@@ -270,173 +505,201 @@ __global__ void __launch_bounds__(BLOCK_WAVES * 64) block_kernel(Matrices<N> a, 
     for (int j = 0; j < 4; j++) place1(i + j, u[j]);
   }
   if (tail < count) place1(tail, momentum<float>(M.g + tail, M.v ? M.v + tail : nullptr, mu, nesterov, false));
-
-  for (int step = 0;; step++) {
-    __syncthreads();
-    // the lane as the compiler does not know it from step to step: it would keep every
-    // address of the loop in registers, and spill them
-    asm volatile("" : "+v"(lane));
-    const int low = lane & 31, high = (lane >> 5) * 4;  // result i: values high + 8 (i / 4) + i % 4 of row low
-    // P = X X^T: with one block of it (four) eight waves (two) share the sum
-    const int pb = mb * mb, ways = mb == 1 ? 8 : mb == 2 ? 2 : 1;
-    {
-      const int f = wave % pb, way = wave / pb;
-      f32x16 acc = {};
-      if (way < ways) {
-#pragma unroll 1
-        for (int k = way; k < nb; k += ways)
+  __syncthreads();
+  // the scales, a wave a row, then a thread a column, and the least value of either
+  // (zeros aside)
+  {
+    const float long_row = sqrtf((float)M.n), long_column = sqrtf((float)M.m);
+    float less[2] = {1.f, 1.f};
+    for (int r = wave; r < mb * 32; r += BLOCK_WAVES) {
+      float most = 0.f;
+      for (int c = lane; c < nb * 8; c += 64) {
+        const f32x4 v = *x4(X, nb, r, c * 4);
 #pragma unroll
-          for (int h = 0; h < 2; h++)
-            three(acc, along(X, nb, f / mb * 32, k, h, 0, lane), along(X, nb, f / mb * 32, k, h, 1, lane),
-                  along(X, nb, f % mb * 32, k, h, 0, lane), along(X, nb, f % mb * 32, k, h, 1, lane));
-        if (way > 0) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            *(f32x4 *)(rest + (((way - 1) * pb + f) * 4 + i) * 1024 + lane * 16) =
-                (f32x4){acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
-        }
+        for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(v[j]));
       }
-      if (ways > 1) __syncthreads();
-      if (way == 0) {
-#pragma unroll 1
-        for (int w = 1; w < ways; w++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const f32x4 v = *(const f32x4 *)(rest + (((w - 1) * pb + f) * 4 + i) * 1024 + lane * 16);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
-          }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const f32x4 v = {acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
-          put4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i, v * DOWN2);
-        }
-      }
+      for (int k = 1; k < 64; k <<= 1) most = fmaxf(most, __shfl_xor(most, k));
+      if (lane == 0) scales[r] = scale_over(most * long_row, room, OF_NO_ROW);
+      if (most > 0.f) less[0] = fminf(less[0], most);
     }
-    __syncthreads();
-    {  // Q = b P + c P P, in P's place
-      const bool on = wave < pb;
-      const int f = on ? wave : 0;
-      f32x16 acc = {};
-      f32x4 q[4];
-      if (on) {
-#pragma unroll 1
-        for (int k = 0; k < mb; k++)
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-            three(acc, along(P, mb, f / mb * 32, k, h, 0, lane), along(P, mb, f / mb * 32, k, h, 1, lane),
-                  along(P, mb, f % mb * 32, k, h, 0, lane), along(P, mb, f % mb * 32, k, h, 1, lane));
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const f32x4 v = {acc[i * 4], acc[i * 4 + 1], acc[i * 4 + 2], acc[i * 4 + 3]};
-          q[i] = get4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i) * TT_NS_B + v * (TT_NS_C * DOWN2);
-        }
-      }
-      __syncthreads();
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) put4(P, mb, f % mb * 32 + low, f / mb * 32 + high + 8 * i, q[i]);
-      }
+    if ((int)threadIdx.x < nb * 32) {
+      float most = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < mb * 32; r++) most = fmaxf(most, fabsf(((const float *)x4(X, nb, r, threadIdx.x & ~3))[threadIdx.x & 3]));
+      scales[mb * 32 + threadIdx.x] = scale_over(most * long_column, room, OF_NO_COLUMN);
+      if (most > 0.f) less[1] = fminf(less[1], most);
     }
-    __syncthreads();
-    asm volatile("" : "+v"(lane));
-    // X^T <- a X^T + X^T Q: block f has the columns f % nb of X and its rows f / nb
-    f32x16 acc[BLOCK_KEEP] = {};
 #pragma unroll
-    for (int b = 0; b < BLOCK_KEEP; b++) {
-      const int f = wave + b * BLOCK_WAVES, r0 = f / nb * 32, cb = f % nb;
-      if (f >= mb * nb) continue;
-#pragma unroll 1
-      for (int k = 0; k < mb; k++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-          three(acc[b], across(X, nb, k * 32 + h * 16, cb, 0, lane), across(X, nb, k * 32 + h * 16, cb, 1, lane),
-                along(P, mb, r0, k, h, 0, lane), along(P, mb, r0, k, h, 1, lane));
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const f32x4 v = get4(X, nb, r0 + low, cb * 32 + high + 8 * i) * TT_NS_A;
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[b][i * 4 + j] = v[j] + acc[b][i * 4 + j] * DOWN2;
-      }
-    }
-    if (step + 1 == steps) {
-#pragma unroll
-      for (int b = 0; b < BLOCK_KEEP; b++) {
-        const int f = wave + b * BLOCK_WAVES, row = f / nb * 32 + low;
-        if (f >= mb * nb || row >= M.m) continue;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int col = f % nb * 32 + high + 8 * (i / 4) + i % 4;
-          if (col >= M.n) continue;
-          float *w = M.w + (M.turned ? col * M.m + row : row * M.n + col);
-          *w = M.v ? M.keep * *w + M.rate * acc[b][i] : acc[b][i];
-        }
-      }
-      return;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < BLOCK_KEEP; b++) {
-      const int f = wave + b * BLOCK_WAVES;
-      if (f >= mb * nb) continue;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        put4(X, nb, f / nb * 32 + low, f % nb * 32 + high + 8 * i,
-             (f32x4){acc[b][i * 4], acc[b][i * 4 + 1], acc[b][i * 4 + 2], acc[b][i * 4 + 3]});
-    }
+    for (int k = 1; k < 64; k <<= 1) less[1] = fminf(less[1], __shfl_xor(less[1], k));
+    if (lane == 0) least[0][wave] = less[0], least[1][wave] = less[1];
   }
+  f32x4 x[BLOCK_KEEP][4];  // of this wave's blocks
+  const int low = lane & 31, high = (lane >> 5) * 4;
+#pragma unroll
+  for (int b = 0; b < BLOCK_KEEP; b++) {
+    const int f = wave + b * BLOCK_WAVES;
+    if (f >= mb * nb) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[b][i] = *x4(X, nb, f / nb * 32 + low, f % nb * 32 + high + 8 * i);
+  }
+  __syncthreads();
+  float row = 1.f, column = 1.f;
+#pragma unroll
+  for (int k = 0; k < BLOCK_WAVES; k++) row = fminf(row, least[0][k]), column = fminf(column, least[1][k]);
+  if (row * column < EVEN) {
+    steps_in_lds<true>(M, steps, lds, scales, lane, wave);
+    return;
+  }
+#pragma unroll
+  for (int b = 0; b < BLOCK_KEEP; b++) {
+    const int f = wave + b * BLOCK_WAVES;
+    if (f >= mb * nb) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      put4(X, nb, f / nb * 32 + low, f % nb * 32 + high + 8 * i, x[b][i], (f32x4){UP, UP, UP, UP});
+  }
+  steps_in_lds<false>(M, steps, lds, scales, lane, wave);
 }
 
 // ---------------------------------------------------------------- before the steps
 
-// v = mu v + g, and the sum of squares of u = g + mu v (nesterov) or v; without
-// momenta of g.  In 64 bits: the squares of any fp32 values are within its range.
-// Bound by memory: 26 us for a block's weights of 12.6 million values (5.8 TB/s).
+// x of the lane N further on, round its sixteen
 template <int N>
-__global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, int nesterov) {
-  __shared__ double sums[4];
-  unsigned b = blockIdx.x;
-  const Matrix M = matrix_of(a, b);
-  const long count = (long)M.m * M.n, groups = count / 4;
-  double s = 0.0;
-  for (long i = (long)b * 512 + threadIdx.x; i < groups; i += (long)M.parts * 512) {
-    f32x4 u[2];
+__device__ __forceinline__ double turned_by(double x) {
+  union {
+    double d;
+    int i[2];
+  } v = {x};
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-      u[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      const long at = (i + k * 256) * 4;
-      if (i + k * 256 < groups) u[k] = momentum<f32x4_any>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, true);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) s = fma((double)u[k][j], (double)u[k][j], s);
-  }
-  const long tail = groups * 4 + threadIdx.x;  // up to three more
-  if (b == 0 && tail < count) {
-    const float u = momentum<float>(M.g + tail, M.v ? M.v + tail : nullptr, mu, nesterov, true);
-    s = fma((double)u, (double)u, s);
-  }
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) M.norm[b] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  for (int k = 0; k < 2; k++) v.i[k] = __builtin_amdgcn_update_dpp(0, v.i[k], 0x120 + N, 15, 15, false);
+  return v.d;
 }
 
-// The images of U / |U|_F and its transpose, a tile of 64 x 64 at a time through
-// LDS; both are written along their rows.  Bound by memory: 36 us for 4096 x 4096
-// (5.6 TB/s).
+// v = mu v + g, and the sums of squares of u = g + mu v (nesterov) or v (without
+// momenta of g), in all and of the rows and columns of each tile of 64 x 64.  In 64
+// bits: the squares of any fp32 values are within its range.  Bound by memory: 29 us for
+// a block's weights of 12.6 million values (5.2 TB/s).
 template <int N>
-__global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int nesterov) {
-  __shared__ double sums[4];
+__global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, int nesterov) {
+  __shared__ double down[16][64];
+  unsigned b = blockIdx.x;
+  const Matrix M = matrix_of(a, b);
+  const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned nc = (unsigned)((cols + 63) / 64), tiles = (unsigned)((rows + 63) / 64) * nc;
+  double all = 0.0;
+  for (unsigned tile = b; tile < tiles; tile += M.parts) {
+    // lane l has four columns from 4 (l % 16) on of every fourth row
+    const int ti = (int)(tile / nc), tj = (int)(tile % nc), c = tj * 64 + (lane & 15) * 4;
+    f32x4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int r = ti * 64 + wave * 16 + k * 4 + (lane >> 4);
+      u[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      const long at = (long)r * cols + c;
+      if (r < rows && c + 4 <= cols) {
+        u[k] = momentum<f32x4_any>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, true);
+      } else if (r < rows) {
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+          if (c + j < cols) u[k][j] = momentum<float>(M.g + at + j, M.v ? M.v + at + j : nullptr, mu, nesterov, true);
+      }
+    }
+    double column[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      double row = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const double q = (double)u[k][j] * (double)u[k][j];
+        row += q;
+        column[j] += q;
+      }
+      row += turned_by<8>(row);
+      row += turned_by<4>(row);
+      row += turned_by<2>(row);
+      row += turned_by<1>(row);
+      const int r = ti * 64 + wave * 16 + k * 4 + (lane >> 4);
+      if ((lane & 15) == 0 && r < rows) M.of_rows()[(long)tj * rows + r] = row;
+    }
+    __syncthreads();  // the last tile's are read
+#pragma unroll
+    for (int j = 0; j < 4; j++) down[wave * 4 + (lane >> 4)][(lane & 15) * 4 + j] = column[j];
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      double q = 0.0;
+#pragma unroll
+      for (int k = 0; k < 16; k++) q += down[k][lane];
+      if (tj * 64 + lane < cols) M.of_cols()[(long)ti * cols + tj * 64 + lane] = q;
+      all += q;
+    }
+  }
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) all += __shfl_xor(all, k);
+    if (lane == 0) M.norm()[b] = all;
+  }
+}
+
+// Up to this length the scales are formed with the images (785 x 256 with two smaller
+// ones: a launch of 4 us less; for 16 x 100000 the columns' took 11).
+constexpr int MEASURE = 1024;
+
+// X = U times this; `again`: X is what is given
+__device__ __forceinline__ double scale_of(double norm, int again) {
+  return again ? 1.0 : norm == 0.0 ? 0.0 : 1.0 / sqrt(norm);  // zeros stay zeros
+}
+
+// The scales of X's rows, and of its columns, where they are formed from more than
+// MEASURE / 64 parts: 16 of them a workgroup, 16 or 64 threads each, in a fixed order.
+// 7 us for a block's weights, 5 for 4096 x 4096.
+template <int N>
+__global__ void __launch_bounds__(1024) scale_kernel(Matrices<N> a, int again, unsigned room) {
+  __shared__ double sums[16][16], norms[16];
+  unsigned b = blockIdx.x;
+  const Matrix M = matrix_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned of_x = 2 * (unsigned)blocks_of(M.m);  // workgroups for X's rows; the others have its columns
+  const bool down = b >= of_x;
+  const int i = (int)(down ? b - of_x : b) * 16 + (lane & 15), many = down ? M.n : M.m, other = down ? M.m : M.n;
+  const double *part = down != (bool)M.turned ? M.of_cols() : M.of_rows();
+  double norm = 0.0, s = 0.0;
+  for (int k = threadIdx.x; k < M.parts; k += blockDim.x) norm += M.norm()[k];
+  if (i < many) {
+#pragma unroll 8
+    for (int k = threadIdx.x >> 4; k < (other + 63) / 64; k += blockDim.x >> 4) s += part[(long)k * many + i];
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) norm += __shfl_xor(norm, k);
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (lane == 0) norms[wave] = norm;
+  if (lane < 16) sums[wave][lane] = s;
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  norm = s = 0.0;
+  for (unsigned k = 0; k < blockDim.x >> 6; k++) norm += norms[k], s += sums[k][lane];
+  const double scale = scale_of(norm, again);
+  (down ? M.f() : M.d())[i] = scale_over(i < many ? (float)(sqrt(s) * scale) : 0.f, room, down ? OF_NO_COLUMN : OF_NO_ROW);
+  if (b == 0 && lane == 0) M.norm()[NORM_PARTS] = scale;
+}
+
+// The images of G and T, a tile of 64 x 64 at a time through LDS; both are written
+// along their rows.  `keep`: X goes to w as well.  The other scales are formed here, by
+// every tile of the same rows or columns again, and written by the first.  Bound by
+// memory: 34 us for 4096 x 4096 (5.9 TB/s).
+template <int N>
+__global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int nesterov, int again, int keep, unsigned room) {
   __shared__ float tile[64][65];
+  __shared__ double norms[2];
+  __shared__ Scale scales[2][64];
   unsigned b = blockIdx.x;
   const Matrix M = matrix_of(a, b);
   const int rows = M.turned ? M.n : M.m, cols = M.turned ? M.m : M.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned across = (unsigned)((cols + 63) / 64);
   const int r0 = (int)(b / across) * 64, c0 = (int)(b % across) * 64;
-  float u[16];  // on their way while the norm is added up
+  Scale *of_rows = M.turned ? M.f() : M.d(), *of_cols = M.turned ? M.d() : M.f();
+  float u[16];  // on their way while the scales are formed
 #pragma unroll
   for (int k = 0; k < 16; k++) {
     const int r = r0 + k * 4 + wave, c = c0 + lane;
@@ -446,30 +709,60 @@ __global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int
       u[k] = momentum<float>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, false);
     }
   }
+  // waves 0 and 1: the rows' and the columns' sums of squares; 2 and 3: that of all
+  const int i = (wave ? c0 : r0) + lane, many = wave ? cols : rows, other = wave ? rows : cols;
+  const bool total = M.n <= MEASURE, here = wave < 2 && other <= MEASURE;
   double s = 0.0;
-  for (int i = threadIdx.x; i < M.parts; i += 256) s += M.norm[i];
+  if (here && i < many) {
+    const double *part = (wave ? M.of_cols() : M.of_rows()) + i;
+    double q[MEASURE / 64];  // on their way at once
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  if (lane == 0) sums[wave] = s;
-  __syncthreads();
-  s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  const double scale = s == 0.0 ? 0.0 : (double)UP / sqrt(s);  // zeros stay zeros
+    for (int k = 0; k < MEASURE / 64; k++) q[k] = k < (other + 63) / 64 ? part[(long)k * many] : 0.0;
 #pragma unroll
-  for (int k = 0; k < 16; k++) tile[k * 4 + wave][lane] = (float)((double)u[k] * scale);
+    for (int k = 0; k < MEASURE / 64; k++) s += q[k];
+  } else if (wave >= 2 && total) {
+#pragma unroll 2
+    for (int k = threadIdx.x - 128; k < M.parts; k += 128) s += M.norm()[k];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+    if (lane == 0) norms[wave - 2] = s;
+  }
+  if (total) __syncthreads();
+  const double scale = total ? scale_of(norms[0] + norms[1], again) : M.norm()[NORM_PARTS];
+  if (wave < 2 && i < blocks_of(many) * 32) {
+    Scale *of = wave ? of_cols : of_rows;
+    Scale x = 0;
+    if (here) {
+      x = scale_over((float)(sqrt(s) * scale), room, (bool)wave != (bool)M.turned ? OF_NO_COLUMN : OF_NO_ROW);
+      if ((wave ? r0 : c0) == 0) of[i] = x;
+    } else {
+      x = of[i];
+    }
+    scales[wave][lane] = x;
+  }
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    const int r = r0 + k * 4 + wave, c = c0 + lane;
+    u[k] = (float)((double)u[k] * scale);
+    if (keep && r < rows && c < cols) M.w[(long)r * cols + c] = u[k];
+    tile[k * 4 + wave][lane] = u[k];
+  }
   __syncthreads();
-  char *along = M.turned ? M.t0 : M.x, *down = M.turned ? M.x : M.t0;
+  char *along = M.turned ? M.t(0) : M.x(), *down = M.turned ? M.x() : M.t(0);
   const long row_blocks = blocks_of(cols), col_blocks = blocks_of(rows);
   const int line = threadIdx.x >> 2, from = (threadIdx.x & 3) * 16;  // 16 values of a row, then of a column
   float v[16];
   if ((r0 + line) / 32 < col_blocks && (c0 + from) / 32 < row_blocks) {
+    const float by = inverse_up(value_of(scales[0][line]));
 #pragma unroll
     for (int j = 0; j < 16; j++) v[j] = tile[line][from + j];
-    put16(along, row_blocks, r0 + line, c0 + from, v);
+    put16(along, row_blocks, r0 + line, c0 + from, v, by);
   }
   if ((c0 + line) / 32 < row_blocks && (r0 + from) / 32 < col_blocks) {
+    const float by = inverse_up(value_of(scales[1][line]));
 #pragma unroll
     for (int j = 0; j < 16; j++) v[j] = tile[from + j][line];
-    put16(down, col_blocks, c0 + line, r0 + from, v);
+    put16(down, col_blocks, c0 + line, r0 + from, v, by);
   }
 }
 
@@ -486,26 +779,53 @@ __device__ __forceinline__ void triangle(unsigned b, int &i, int &j) {
   j = (int)(b - (unsigned)r * (r + 1u) / 2);
 }
 
+// A step's parity, and whether what X adds comes from w (`onto`, of the last)
+struct Phase {
+  int odd, from_w;
+};
+
 template <int KIND>
 struct Operands {
   const char *a, *b;    // images whose rows are multiplied
-  const char *add;      // image of the transpose of the matrix added, times `times` (GRAM: none)
-  const char *plain;    // and of that matrix
+  const char *add;      // what is added, in the image of the transpose (GRAM: none)
+  const char *plain;    // and in its own
   char *out, *down;     // images of the result and its transpose
+  const Scale *d, *f;   // scales of the result's rows and columns
   int rows, cols, k;    // of the result; the products' length
   float by, times;
-  __device__ __forceinline__ Operands(const Matrix &M, int step) {
+  __device__ __forceinline__ Operands(const Matrix &M, const Phase &phase) {
+    d = M.d(), f = KIND <= SQUARE ? M.d() : M.f();
     if (KIND == GRAM) {
-      a = b = M.x, add = plain = nullptr, out = down = M.p;
-      rows = cols = M.m, k = M.n, by = 1.f, times = 0.f;
+      a = b = M.x(), add = plain = nullptr, out = down = M.p();
+      rows = cols = M.m, k = M.n, by = DOWN2, times = 0.f;
     } else if (KIND == SQUARE) {
-      a = b = add = plain = M.p, out = down = M.q;
-      rows = cols = k = M.m, by = TT_NS_C, times = TT_NS_B;
+      a = b = add = plain = M.p(), out = down = M.q();
+      rows = cols = k = M.m, by = TT_NS_C * DOWN2, times = TT_NS_B;
     } else {
-      a = M.q, b = add = step & 1 ? M.t1 : M.t0, plain = M.x, out = M.x, down = step & 1 ? M.t0 : M.t1;
-      rows = k = M.m, cols = M.n, by = 1.f, times = TT_NS_A;
+      a = M.q(), b = add = M.t(phase.odd), plain = M.x(), out = M.x(), down = M.t(!phase.odd);
+      rows = k = M.m, cols = M.n, by = DOWN2, times = TT_NS_A;
     }
   }
+  // What is added, of values h + l of its own image or the transpose's: X is in the
+  // image of its rows without d and in that of its columns without f, C in both with the
+  // other's.  Either way a row weaker than the column has it finer in its own image, and
+  // a column weaker than the row in the transpose's.  One of them is read as it comes;
+  // X, whose weak values grow, from the other where that is finer by more than 4 (a
+  // column's of rows longer than 200000 beside 2, the most a scale may be), C by 32.
+  static constexpr float FAR = KIND == STEP ? 4.f : 32.f;
+  __device__ __forceinline__ float plain_scale(float d, float f) const { return times / UP * (KIND == STEP ? d : inverse(f)); }
+  __device__ __forceinline__ float add_scale(float d, float f) const { return times / UP * (KIND == STEP ? f : inverse(d)); }
+  // The products' sum (C, and Q without its scales, are as the sums are), and what is
+  // added.  (Multiply-adds take the halves as they are.)
+  __device__ __forceinline__ float of_sum(float sum, float d, float f) const {
+    return KIND == STEP ? sum * (by * f) * d : sum * by;
+  }
+  __device__ __forceinline__ static float add_to(float sum, _Float16 h, _Float16 l, float scale) {
+    return fmaf((float)h, scale, fmaf((float)l, scale, sum));
+  }
+  // what the images have it times
+  __device__ __forceinline__ static float out_scale(float d, float f) { return KIND == STEP ? inverse_up(d) : UP * f; }
+  __device__ __forceinline__ static float down_scale(float d, float f) { return KIND == STEP ? inverse_up(f) : UP * d; }
 };
 
 // Consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of them,
@@ -545,12 +865,12 @@ __device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int
 // eight sums, joined in LDS.  What bounds these is the way from memory (the L2 of
 // another XCD has what the last launch wrote), so the added matrix is on its way
 // first, and a tile on the diagonal reads its rows once.  A launch takes 4 us at least;
-// 517 x 1003: 6 us for P, 5 for Q, 10 for X; 1300 x 1300: 18, 18 and 29 (450 TFLOP/s
+// 517 x 1003: 6 us for P, 5 for Q, 11 for X; 1400 x 1400: 18, 19 and 34 (490 TFLOP/s
 // of fp16 products).  Of few long tiles of P the length is shared by `ways` workgroups,
 // whose sums a second launch adds (join): one CU alone reads 80 GB/s.
 template <int KIND, bool SHARED, int N>
 __global__ void __launch_bounds__(512, 2)
-    small_kernel(Matrices<N> a, int step, int to_w, int ways, bool join, float *pieces) {
+    small_kernel(Matrices<N> a, Phase phase, int to_w, int ways, bool join, float *pieces) {
   typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   constexpr int WAVES = 8;
   __shared__ float sums[WAVES][32][33];
@@ -561,18 +881,22 @@ __global__ void __launch_bounds__(512, 2)
     if (!join) way = t % ways, t /= ways;
   }
   const Matrix M = matrix_of(a, t);
-  const Operands<KIND> o(M, step);
+  const Operands<KIND> o(M, phase);
   int ti, tj;
   tile_of<KIND, 32>(t, o.rows, o.cols, ti, tj);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 2;  // this thread's two results
-  const int row = ti * 32 + r, col = tj * 32 + c;
-  float v[2] = {0.f, 0.f};
-  if (KIND != GRAM) {
-    const _Float16 *p = place((char *)o.plain, blocks_of(o.cols), row, col);
-    const half2 h = *(const half2 *)p, l = *(const half2 *)(p + 1024);
-#pragma unroll
-    for (int e = 0; e < 2; e++) v[e] = o.times * (1.f / UP) * ((float)h[e] + (float)l[e]);
+  // where these lie in the tile's block of an image, and (their transposes') in the
+  // transpose's; their scales, and the transposes'
+  const unsigned at = inner(r, c);
+  const long block = ((long)ti * blocks_of(o.cols) + tj) * 4096, across = ((long)tj * blocks_of(o.rows) + ti) * 4096;
+  const Scale *rows = o.d + ti * 32, *cols = o.f + tj * 32;
+  const Scale d = rows[(unsigned)r], df = cols[(unsigned)r];
+  const scale2 f = *(const scale2 *)(cols + (unsigned)c), dd = *(const scale2 *)(rows + (unsigned)c);
+  half2 h = {}, l = {};
+  if (KIND != GRAM && !(KIND == STEP && phase.from_w)) {
+    const char *p = o.plain + block;
+    h = *(const half2 *)(p + at), l = *(const half2 *)(p + 2048 + at);
   }
   float sum[2] = {0.f, 0.f};
   if (SHARED && join) {
@@ -613,36 +937,46 @@ __global__ void __launch_bounds__(512, 2)
     }
   }
   bool in[2];
+  float v[2];
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    in[e] = row < o.rows && col + e < o.cols;
-    v[e] = in[e] ? v[e] + sum[e] * (o.by * DOWN2) : 0.f;
+    const float x = value_of(d), y = value_of(f[e]);
+    in[e] = ti * 32 + r < o.rows && tj * 32 + c + e < o.cols;
+    const float product = o.of_sum(sum[e], x, y);
+    v[e] = KIND == GRAM ? product : o.add_to(product, h[e], l[e], o.plain_scale(x, y));
+    if (KIND != GRAM && !phase.from_w && in[e] && x > o.FAR * y) {
+      const _Float16 *p = (const _Float16 *)(o.add + across + inner(c + e, r));
+      v[e] = o.add_to(product, p[0], p[1024], o.add_scale(x, y));
+    }
+    if (!in[e]) v[e] = 0.f;
   }
   if (KIND == STEP && to_w) {
 #pragma unroll
     for (int e = 0; e < 2; e++)
       if (in[e] && !M.turned) {
-        float *w = M.w + (long)row * o.cols + col + e;
-        *w = M.v ? M.keep * *w + M.rate * v[e] : v[e];
+        float *w = M.w + (long)(ti * 32 + r) * o.cols + tj * 32 + c + e;
+        *w = M.onto ? M.keep * *w + M.rate * v[e] : v[e];
       }
   } else {
-    put2(o.out, blocks_of(o.cols), row, col, v[0], v[1]);
+    char *p = o.out + block;
+    put2(p + at, v[0], v[1], o.out_scale(value_of(d), value_of(f[0])), o.out_scale(value_of(d), value_of(f[1])));
   }
   if ((KIND <= SQUARE && ti == tj) || (KIND == STEP && to_w && !M.turned)) return;
   __syncthreads();
   sums[0][r][c] = v[0];
   sums[0][r][c + 1] = v[1];
   __syncthreads();
-  const int trow = tj * 32 + r, tcol = ti * 32 + c;  // the transpose
   if (KIND == STEP && to_w) {
 #pragma unroll
     for (int e = 0; e < 2; e++)
-      if (trow < o.cols && tcol + e < o.rows) {
-        float *w = M.w + (long)trow * o.rows + tcol + e;
-        *w = M.v ? M.keep * *w + M.rate * sums[0][c + e][r] : sums[0][c + e][r];
+      if (tj * 32 + r < o.cols && ti * 32 + c + e < o.rows) {
+        float *w = M.w + (long)(tj * 32 + r) * o.rows + ti * 32 + c + e;
+        *w = M.onto ? M.keep * *w + M.rate * sums[0][c + e][r] : sums[0][c + e][r];
       }
   } else {
-    put2(o.down, blocks_of(o.rows), trow, tcol, sums[0][c][r], sums[0][c + 1][r]);
+    char *p = o.down + across;
+    put2(p + at, sums[0][c][r], sums[0][c + 1][r], o.down_scale(value_of(dd[0]), value_of(df)),
+         o.down_scale(value_of(dd[1]), value_of(df)));
   }
 }
 
@@ -658,7 +992,7 @@ __global__ void __launch_bounds__(512, 2)
 //                 the SIMD fills a wave's waits, and memory gives half as much
 // A tile that one workgroup has is finished by it.  The others' parts go to memory,
 // and join_kernel adds them.  The matrix units bound these, at the clock that they
-// leave: X of 4096 x 4096 takes 343 us, 1200 TFLOP/s of fp16 products, with the units
+// leave: X of 4096 x 4096 takes 345 us, 1200 TFLOP/s of fp16 products, with the units
 // 69 % busy at 1.84 GHz; of 2048 x 2048 by tiles of 128 50 us, 1030 TFLOP/s (51 % busy
 // at 2 GHz in a transformer block's six matrices).
 
@@ -698,14 +1032,26 @@ __device__ __forceinline__ const char *scalar(const char *p) {
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 struct Added {
   half4 h[4], l[4];
+  scale4 d[4];  // scales of the rows and of the column
+  Scale f;
 };
 __device__ __forceinline__ int part_of(int i, int lane) {  // in the block of the transpose, bytes
   return (i >> 1) * 1024 + ((lane & 31) + 32 * (i & 1)) * 16 + (lane >> 5) * 8;
 }
 template <int KIND>
-__device__ __forceinline__ Added added(const Operands<KIND> &o, int r0, int c0, int lane) {
+__device__ __forceinline__ Added added(const Operands<KIND> &o, int r0, int c0, int lane, bool from_w,
+                                       const Added *of_rows = nullptr) {  // (what has the same rows)
   Added x = {};
-  if (KIND == GRAM || r0 >= o.rows || c0 >= o.cols) return x;
+  if (of_rows) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x.d[i] = of_rows->d[i];
+  }
+  if (r0 >= o.rows || c0 >= o.cols || (KIND <= SQUARE && r0 < c0)) return x;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (!of_rows) x.d[i] = *(const scale4 *)(o.d + r0 + (lane >> 5) * 4 + 8 * i);
+  x.f = o.f[c0 + (lane & 31)];
+  if (KIND == GRAM || (KIND == STEP && from_w)) return x;
   const char *p = o.add + ((c0 >> 5) * blocks_of(o.rows) + (r0 >> 5)) * 4096;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -714,19 +1060,42 @@ __device__ __forceinline__ Added added(const Operands<KIND> &o, int r0, int c0, 
   }
   return x;
 }
-// buf: 4 KB of LDS, this wave's; both: the image itself too
+// buf: 4 KB of LDS, this wave's.  Of a symmetric result the blocks behind the diagonal
+// are left to those before it.
 template <int KIND>
 __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o, const f32x16 &acc, const Added &x,
-                                        int r0, int c0, char *buf, int lane, bool both, bool to_w) {
-  if (r0 >= o.rows || c0 >= o.cols) return;
+                                        int r0, int c0, char *buf, int lane, const Phase &phase, bool to_w) {
+  if (r0 >= o.rows || c0 >= o.cols || (KIND <= SQUARE && r0 < c0)) return;
+  const bool both = KIND == STEP || r0 != c0;
+  const int col = c0 + (lane & 31), row = r0 + (lane >> 5) * 4;
   f32x4 v[4];
+  const float f = value_of(x.f);
+  Scale least = x.d[0][0];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      v[i][j] = acc[i * 4 + j] * (o.by * DOWN2);
-      if (KIND != GRAM) v[i][j] += o.times * (1.f / UP) * ((float)x.h[i][j] + (float)x.l[i][j]);
+  for (int i = 0; i < 16; i++) {
+    const float d = value_of(x.d[i / 4][i % 4]);
+    const float product = o.of_sum(acc[i], d, f);
+    v[i / 4][i % 4] = KIND == GRAM ? product : o.add_to(product, x.h[i / 4][i % 4], x.l[i / 4][i % 4], o.add_scale(d, f));
+    least = x.d[i / 4][i % 4] < least ? x.d[i / 4][i % 4] : least;
+  }
+  if (KIND != GRAM && !phase.from_w && __any(col < o.cols && f > o.FAR * value_of(least))) {
+    // by way of LDS, each lane its own: sixteen reads in line were a third of the kernel's code
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+    half2 *mine = (half2 *)buf + lane;
+#pragma unroll 1
+    for (int i = 0; i < 16; i++) {
+      const _Float16 *p = place((char *)o.plain, blocks_of(o.cols), row + 8 * (i >> 2) + (i & 3), col);
+      half2 w = {};
+      if (col < o.cols) w[0] = p[0], w[1] = p[1024];
+      mine[i * 64] = w;
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float d = value_of(x.d[i / 4][i % 4]);
+      const half2 w = mine[i * 64];
+      if (f > o.FAR * d) v[i / 4][i % 4] = o.add_to(o.of_sum(acc[i], d, f), w[0], w[1], o.plain_scale(d, f));
+    }
+  }
   if (KIND == STEP && to_w) {
     // (as values of their own: the compiler would read `rate` with its neighbours as a
     // vector, for that put M into LDS, and fetch the launch's packet from the host's
@@ -734,16 +1103,16 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
     float rate = M.rate, keep = M.keep;
     asm("" : "+s"(rate), "+s"(keep));
     // what is read is on its way at once: behind the last row or column, theirs
-    const int col = c0 + (lane & 31), row = r0 + (lane >> 5) * 4, c = col < o.cols ? col : o.cols - 1;
+    const int c = col < o.cols ? col : o.cols - 1;
     if (M.turned && r0 + 32 <= o.rows) {
       float *w = M.w + (long)c * o.rows + row;
       f32x4 old[4] = {};
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (M.v) old[i] = *(const f32x4_any *)(w + 8 * i) * keep;
+        if (M.onto) old[i] = *(const f32x4_any *)(w + 8 * i) * keep;
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (col < o.cols) *(f32x4_any *)(w + 8 * i) = M.v ? old[i] + v[i] * rate : v[i];
+        if (col < o.cols) *(f32x4_any *)(w + 8 * i) = M.onto ? old[i] + v[i] * rate : v[i];
       return;
     }
     const long down = M.turned ? 1 : o.cols, start = M.turned ? (long)c * o.rows : c;
@@ -751,31 +1120,32 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int r = row + 8 * (i / 4) + i % 4;
-      if (M.v) old[i] = M.w[start + (r < o.rows ? r : o.rows - 1) * down] * keep;
+      if (M.onto) old[i] = M.w[start + (r < o.rows ? r : o.rows - 1) * down] * keep;
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int r = row + 8 * (i / 4) + i % 4;
-      if (col < o.cols && r < o.rows) M.w[start + r * down] = M.v ? old[i] + v[i / 4][i % 4] * rate : v[i / 4][i % 4];
+      if (col < o.cols && r < o.rows) M.w[start + r * down] = M.onto ? old[i] + v[i / 4][i % 4] * rate : v[i / 4][i % 4];
     }
     return;
   }
   char *down = o.down + ((c0 >> 5) * blocks_of(o.rows) + (r0 >> 5)) * 4096;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
+  auto put = [&](char *at, int i, bool out) {
     half4 h, l;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
+      const float d = value_of(x.d[i][j]);
       _Float16 a, b;
-      split(v[i][j] * UP, a, b);
+      split(v[i][j], out ? o.out_scale(d, f) : o.down_scale(d, f), a, b);
       h[j] = a, l[j] = b;
     }
-    *(half4 *)(down + part_of(i, lane)) = h;
-    *(half4 *)(down + part_of(i, lane) + 2048) = l;
-    if (both) {
-      *(half4 *)(buf + part_of(i, lane)) = h;
-      *(half4 *)(buf + part_of(i, lane) + 2048) = l;
-    }
+    *(half4 *)(at + part_of(i, lane)) = h;
+    *(half4 *)(at + part_of(i, lane) + 2048) = l;
+  };
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    put(down, i, false);
+    if (both) put(buf, i, true);
   }
   if (!both) return;
   __builtin_amdgcn_wave_barrier();
@@ -793,6 +1163,20 @@ __device__ __forceinline__ void write32(const Matrix &M, const Operands<KIND> &o
       for (int j = 0; j < 4; j++) w[x * 4 + j] = t[j];
     }
     *(s16x8 *)(out + (f >> 1) * 2048 + (f & 1) * 1024) = w;
+  }
+}
+
+// g of every number from F on (a loop of this length the compiler does not unroll, and
+// registers have no other numbers)
+template <int F>
+struct Number {
+  static constexpr int value = F;
+};
+template <int F, int END, class G>
+__device__ __forceinline__ void each(const G &g) {
+  if constexpr (F < END) {
+    g(Number<F>());
+    each<F + 1, END>(g);
   }
 }
 
@@ -820,7 +1204,7 @@ struct Deal {
 };
 
 template <int KIND, int T, int BUFFERS, int N>
-__global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUFFERS>::WAVES / 4)) tile_kernel(Matrices<N> a, int step, int to_w, Deal deal, float *pieces) {
+__global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUFFERS>::WAVES / 4)) tile_kernel(Matrices<N> a, Phase phase, int to_w, Deal deal, float *pieces) {
   typedef Shape<T, BUFFERS> S;
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * S::BUFFER];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -830,7 +1214,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
   for (unsigned long u = 0, end = 0;;) {
     if (u == end) {
       if (round < deal.rounds) {  // then all tiles have the same number of blocks
-        const Operands<KIND> o(a.at[0], step);
+        const Operands<KIND> o(a.at[0], phase);
         u = ((unsigned long)round * groups + w) * blocks_of(o.k);
         end = u + blocks_of(o.k);
         if (u >= deal.base) end = u;  // no tile for this workgroup
@@ -845,7 +1229,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
     }
     unsigned long in = u;
     const Matrix M = matrix_of(a, in);
-    const Operands<KIND> o(M, step);
+    const Operands<KIND> o(M, phase);
     const int extra = N > 1 ? deal.extra : 0;
     const long blocks = blocks_of(o.k), units = blocks + extra;
     int ti, tj;
@@ -982,14 +1366,16 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
     }
     if (n == blocks) {
       __syncthreads();  // the operands are read
-      Added x = added<KIND>(o, row_of<T>(ti, wave, 0), col_of<T>(tj, wave, 0), lane), next = x;
-#pragma unroll
-      for (int f = 0; f < S::BLOCKS; f++) {
-        if (f + 1 < S::BLOCKS) next = added<KIND>(o, row_of<T>(ti, wave, f + 1), col_of<T>(tj, wave, f + 1), lane);
+      Added x = added<KIND>(o, row_of<T>(ti, wave, 0), col_of<T>(tj, wave, 0), lane, phase.from_w), next = x;
+      each<0, S::BLOCKS>([&](auto number) __attribute__((always_inline)) {
+        constexpr int f = decltype(number)::value;
+        if constexpr (f + 1 < S::BLOCKS)
+          next = added<KIND>(o, row_of<T>(ti, wave, f + 1), col_of<T>(tj, wave, f + 1), lane, phase.from_w,
+                             f % 2 == 0 ? &x : nullptr);
         write32<KIND>(M, o, acc[f / 2][f % 2], x, row_of<T>(ti, wave, f), col_of<T>(tj, wave, f), lds + wave * 4096, lane,
-                      KIND == STEP || ti != tj, to_w);
+                      phase, to_w);
         x = next;
-      }
+      });
     } else {
       f32x4 *p = (f32x4 *)(pieces + (2l * w + (k0 == 0)) * S::PIECE) + wave * S::BLOCKS * 256 + lane;
 #pragma unroll
@@ -1009,7 +1395,7 @@ __global__ void __launch_bounds__((Shape<T, BUFFERS>::WAVES * 64), (Shape<T, BUF
 // Bound by memory (P of 6000 x 6000, tiles of 256: 20 us) or by its own latency (8 to 12
 // us for tiles of 128).
 template <int KIND, int T, int N>
-__global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int to_w, Deal deal, const float *pieces) {
+__global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, Phase phase, int to_w, Deal deal, const float *pieces) {
   typedef Shape<T, 2> S;
   __shared__ __attribute__((aligned(1024))) char buf[4][4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1017,7 +1403,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int 
   const unsigned long u = deal.begins(w);
   unsigned long in = u;
   const Matrix M = matrix_of(a, in);
-  const Operands<KIND> o(M, step);
+  const Operands<KIND> o(M, phase);
   const unsigned extra = N > 1 ? deal.extra : 0;
   const unsigned long units = blocks_of(o.k) + extra, first = u - in % units, last = first + units;
   if (u <= first + extra || deal.begins(w - 1) > first + extra) return;
@@ -1025,7 +1411,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int 
   tile_of<KIND, T>(in / units, o.rows, o.cols, ti, tj);
   const int block = blockIdx.y * 4 + wave;
   const int r0 = row_of<T>(ti, block / S::BLOCKS, block % S::BLOCKS), c0 = col_of<T>(tj, block / S::BLOCKS, block % S::BLOCKS);
-  const Added x = added<KIND>(o, r0, c0, lane);
+  const Added x = added<KIND>(o, r0, c0, lane, phase.from_w);
   unsigned stop = w;  // the first workgroup behind the tile
   while (stop < deal.sharers && deal.begins(stop) < last) stop++;
   f32x16 acc = {};
@@ -1039,7 +1425,7 @@ __global__ void __launch_bounds__(256) join_kernel(Matrices<N> a, int step, int 
       for (int j = 0; j < 4; j++) acc[i * 4 + j] += v[j];
     }
   }
-  write32<KIND>(M, o, acc, x, r0, c0, buf[wave], lane, KIND == STEP || ti != tj, to_w);
+  write32<KIND>(M, o, acc, x, r0, c0, buf[wave], lane, phase, to_w);
 }
 
 // ---------------------------------------------------------------- host
@@ -1048,30 +1434,16 @@ bool good_sides(long rows, long cols) {
   return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= TT_MUON_MAX_VALUES;
 }
 
-size_t images_of(long rows, long cols) {
-  const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-  const size_t mb = blocks_of((int)m), nb = blocks_of((int)n);
-  return 4096 * (3 * mb * nb + 2 * mb * mb) + sizeof(double) * NORM_PARTS;
-}
-
 void lay(Matrix &M, long rows, long cols, char *&ws) {
   M.turned = rows > cols;
   M.m = (int)(M.turned ? cols : rows);
   M.n = (int)(M.turned ? rows : cols);
-  const long parts = ((long)M.m * M.n + 2047) / 2048;
-  M.parts = (int)(parts < NORM_PARTS ? parts : NORM_PARTS);
-  const size_t mb = blocks_of(M.m), nb = blocks_of(M.n);
-  auto take = [&](size_t bytes) {
-    char *p = ws;
-    ws += bytes;
-    return p;
-  };
-  M.x = take(4096 * mb * nb);
-  M.t0 = take(4096 * mb * nb);
-  M.t1 = take(4096 * mb * nb);
-  M.p = take(4096 * mb * mb);
-  M.q = take(4096 * mb * mb);
-  M.norm = (double *)take(sizeof(double) * NORM_PARTS);
+  const long tiles = (long)((M.m + 63) / 64) * ((M.n + 63) / 64);
+  M.parts = (int)(tiles < NORM_PARTS ? tiles : NORM_PARTS);
+  M.base = ws;
+  M.side = 4096 * blocks_of(M.m) * blocks_of(M.n);
+  M.square = 4096 * blocks_of(M.m) * blocks_of(M.m);
+  ws += M.bytes();
 }
 
 template <int N, class F>
@@ -1106,23 +1478,23 @@ long length_of(int kind, const Matrix &M) { return blocks_of(kind == GRAM ? M.n 
 // product, with what joins its parts:
 //                      P = X X^T            X <- a X + Q X
 //   tiles of         32   128   256        32   128   256
-//   1024^2           11    19     -        15    20     -
-//   700 x 4000       15    21     -        26    24     -
-//   2 x 1024^2       17    20     -        27    26     -
-//   1400^2           18    22     -        33    28     -
-//   1600^2           25    27     -        45    40     -
-//   1024 x 4096      37    26     -        56    30     -
-//   2048^2            -    41    55         -    54    78
-//   2500^2            -    75    75         -   118   115
-//   2048 x 4096       -    78    78         -   109   122
-//   2200 x 6300       -   108   120         -   194   195
-//   3000 x 5000       -   147   159         -   297   251
-//   2048 x 8192       -   158   117         -   182   189
-//   2100 x 12000      -   205   196         -   370   340
-//   4096^2            -   198   219         -   391   348
-//   4096 x 8192       -   378   385         -   789   682
-//   6000^2            -   610   590         -  1359  1117
-//   8192^2            -  1511  1326         -  3459  2533
+//   1024^2           11    18     -        16    21     -
+//   700 x 4000       20    22     -        28    26     -
+//   2 x 1024^2       17    21     -        27    27     -
+//   1400^2           18    22     -        34    29     -
+//   1600^2           25    28     -        46    41     -
+//   1024 x 4096      33    25     -        47    31     -
+//   2048^2            -    40    57         -    52    79
+//   2500^2            -    77    79         -   119   119
+//   2048 x 4096       -    75    74         -    96   116
+//   2200 x 6300       -   104   117         -   196   192
+//   3000 x 5000       -   146   152         -   294   245
+//   2048 x 8192       -   157   116         -   188   188
+//   2100 x 12000      -   204   188         -   382   352
+//   4096^2            -   194   209         -   381   332
+//   4096 x 8192       -   376   377         -   792   674
+//   6000^2            -   600   570         -  1368  1074
+//   8192^2            -  1529  1327         -  3501  2529
 template <int N>
 int tile_size(const Matrices<N> &a, int kind) {
   double work = 0, tiles = 0;  // (of 128)
@@ -1146,7 +1518,7 @@ int tile_size(const Matrices<N> &a, int kind) {
 constexpr int SHARERS = 512, LONG = 60;
 
 template <int KIND, int N>
-void small_product(Matrices<N> &a, int step, int to_w, float *pieces) {
+void small_product(Matrices<N> &a, const Phase &phase, int to_w, float *pieces) {
   const unsigned grid = (unsigned)number(a, [](const Matrix &M) {
     return KIND <= SQUARE ? blocks_of(M.m) * (blocks_of(M.m) + 1) / 2 : blocks_of(M.m) * blocks_of(M.n);
   });
@@ -1157,15 +1529,15 @@ void small_product(Matrices<N> &a, int step, int to_w, float *pieces) {
     if (length >= LONG && ways > 1) {
       for (int join = 0; join < 2; join++)
         hipLaunchKernelGGL((small_kernel<KIND, true, N>), dim3(join ? grid : grid * (unsigned)ways), dim3(512), 0,
-                           stream(), a, step, to_w, (int)ways, join, pieces);
+                           stream(), a, phase, to_w, (int)ways, join, pieces);
       return;
     }
   }
-  hipLaunchKernelGGL((small_kernel<KIND, false, N>), dim3(grid), dim3(512), 0, stream(), a, step, to_w, 1, false, pieces);
+  hipLaunchKernelGGL((small_kernel<KIND, false, N>), dim3(grid), dim3(512), 0, stream(), a, phase, to_w, 1, false, pieces);
 }
 
 template <int KIND, int T, int BUFFERS, int N>
-void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
+void tile_product(Matrices<N> &a, const Phase &phase, int to_w, float *pieces) {
   typedef Shape<T, BUFFERS> S;
   constexpr int EXTRA = T == 128 ? 12 : 6;  // (2375 x 1041 with five: 598 us with 4, 569 with 8, 559 with 12)
   auto tiles_of = [](const Matrix &M) {
@@ -1200,34 +1572,51 @@ void tile_product(Matrices<N> &a, int step, int to_w, float *pieces) {
     if (!d.units) d.sharers = 0;
     else if (shared <= even) d.sharers = (unsigned)(rest * ways);
   }
-  hipLaunchKernelGGL((tile_kernel<KIND, T, BUFFERS, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, step, to_w, d, pieces);
+  hipLaunchKernelGGL((tile_kernel<KIND, T, BUFFERS, N>), dim3(groups), dim3(S::WAVES * 64), 0, stream(), a, phase, to_w, d, pieces);
   if (d.sharers > 1)
-    hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, step, to_w, d,
+    hipLaunchKernelGGL((join_kernel<KIND, T, N>), dim3(d.sharers - 1, S::PIECE / 4096), dim3(256), 0, stream(), a, phase, to_w, d,
                        (const float *)pieces);
 }
 
 template <int KIND, int N>
-void product(Matrices<N> &a, int step, float *pieces, int to_w = 0) {
+void product(Matrices<N> &a, const Phase &phase, float *pieces, int to_w = 0) {
   const int tile = tile_size(a, KIND);
-  if (tile == 0) small_product<KIND, N>(a, step, to_w, pieces);
-  else if (tile == 128) tile_product<KIND, 128, 3, N>(a, step, to_w, pieces);
-  else tile_product<KIND, 256, 2, N>(a, step, to_w, pieces);
+  if (tile == 0) small_product<KIND, N>(a, phase, to_w, pieces);
+  else if (tile == 128) tile_product<KIND, 128, 3, N>(a, phase, to_w, pieces);
+  else tile_product<KIND, 256, 2, N>(a, phase, to_w, pieces);
 }
 
+// Steps with the scales measured before the first, MOST_STEPS at most; `again`: of X
+// that is given.  `keep`: X goes to w, and the last step takes a X from there.
 template <int N>
-void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *rest) {
+void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *rest, int again = 0, int keep = 0) {
   if (blocks) {
-    hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov);
+    hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov, again,
+                       room_for(steps));
     return;
   }
   unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
   hipLaunchKernelGGL(momentum_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
+  grid = number(a, [](const Matrix &M) {
+    return (M.n > MEASURE ? 2 * blocks_of(M.m) : 0) + (M.m > MEASURE ? 2 * blocks_of(M.n) : 0);
+  });
+  if (grid) {
+    int longest = 0;
+    for (int i = 0; i < (N > 1 ? a.count : 1); i++) longest = a.at[i].n > longest ? a.at[i].n : longest;
+    // (16 x 100000: 9 us with 16 threads a row, 4 x 4096: 5 and 11 with 64)
+    hipLaunchKernelGGL(scale_kernel<N>, dim3((unsigned)grid), dim3(longest > 16384 ? 1024 : 256), 0, stream(), a, again,
+                       room_for(steps));
+  }
   grid = number(a, [](const Matrix &M) { return (long)((M.m + 63) / 64) * ((M.n + 63) / 64); });
-  hipLaunchKernelGGL(image_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
+  hipLaunchKernelGGL(image_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov, again, keep && !again,
+                     room_for(steps));
   for (int s = 0; s < steps; s++) {
-    product<GRAM, N>(a, s, (float *)rest);
-    product<SQUARE, N>(a, s, (float *)rest);
-    product<STEP, N>(a, s, (float *)rest, s + 1 == steps);
+    const bool last = s + 1 == steps;
+    Phase phase = {s & 1, 0};
+    product<GRAM, N>(a, phase, (float *)rest);
+    product<SQUARE, N>(a, phase, (float *)rest);
+    phase.from_w = last && keep;
+    product<STEP, N>(a, phase, (float *)rest, last);
   }
 }
 
@@ -1243,8 +1632,8 @@ size_t ws_of(const Matrices<N> &a, size_t images) {
 Matrices<1> alike(long count, long rows, long cols, char *ws) {
   Matrices<1> a = {};
   a.count = (int)(count < ALIKE ? count : ALIKE);
-  a.images = (long)images_of(rows, cols);
   lay(a.at[0], rows, cols, ws);
+  a.images = a.at[0].bytes();
   return a;
 }
 
@@ -1274,7 +1663,17 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
     a.count = (int)(count - base < most ? count - base : most);
     a.at[0].g = x + base * rows * cols;
     a.at[0].w = y + base * rows * cols;
-    run(a, blocks, steps, 0.f, 0, (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images);
+    char *rest = (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images;
+    // More steps than the scales hold for go on from y.  By launches then each begins
+    // anew and adds to y: what is weak by its row and its column, and so in every image,
+    // is carried in fp32 (60 x 500 with 1e-7 of half of both: a column's 3e-6 after 16
+    // steps, 2e-4 from images of six).  In LDS X is fp32 throughout.
+    const int each = steps <= MOST_STEPS || blocks ? MOST_STEPS : 1;
+    a.at[0].onto = each == 1, a.at[0].keep = TT_NS_A, a.at[0].rate = 1.f;
+    for (int done = 0; done < steps; done += each) {
+      run(a, blocks, steps - done < each ? steps - done : each, 0.f, 0, rest, done > 0, each == 1);
+      a.at[0].g = a.at[0].w;
+    }
   }
   ttrt_free(own);
   return launched();
@@ -1289,7 +1688,7 @@ extern "C" size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int cou
   for (int i = 0; i < count; i++) {
     if (!good_sides(rows[i], cols[i])) return 0;
     lay(a.at[i], rows[i], cols[i], at);
-    bytes += images_of(rows[i], cols[i]);
+    bytes += (size_t)a.at[i].bytes();
   }
   return ws_of(a, bytes);
 }
@@ -1317,7 +1716,7 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
   char *at = (char *)ws;
   for (int i = 0; i < count; i++) {
     Matrix &M = a.at[i];
-    M.g = g[i], M.v = v[i], M.w = w[i];
+    M.g = g[i], M.v = v[i], M.w = w[i], M.onto = 1;
     M.keep = (float)(1.0 - (double)lr * decay);
     M.rate = (float)(-(double)lr * TT_MUON_RMS * sqrt((double)(rows[i] > cols[i] ? rows[i] : cols[i])));
     lay(M, rows[i], cols[i], at);
