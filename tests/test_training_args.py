@@ -118,3 +118,23 @@ def test_optim_muon_refuses(L, args):
 def test_nodes_refuse_missing_operands(L):
     assert not L.ag_rmsnorm(None, None, None, 1e-5, None)
     assert not L.ag_embedding(None, P, 3, 1.0)
+
+
+def _images(m, n):
+    """What a matrix may take in the workspace, of sides rounded up to 32."""
+    m, n = (32 * ((s + 31) // 32) for s in (min(m, n), max(m, n)))
+    return (12 * m * n + 8 * m * m) * 1.002 + (16 << 10)
+
+
+FLAT = [(1, 1 << 20), (1 << 20, 1), (4, 4096), (9, 5000), (3, 100000), (33, 2000), (257, 300), (1000, 31), (1, 40000)]
+
+
+@pytest.mark.parametrize("m,n", FLAT)
+def test_workspace_of_flat_matrices(L, m, n):
+    more, groups = 128 << 20, 4 << 30
+    for count in (1, 2, 20, 64, 1000):
+        ws = L.tt_k_newton_schulz_ws(count, m, n)
+        assert ws <= max(_images(m, n), min(groups, min(count, 64) * _images(m, n))) + more
+        assert ws == L.tt_k_newton_schulz_ws(count, n, m)
+    r, c = (ctypes.c_long * 2)(m, 300), (ctypes.c_long * 2)(n, 400)
+    assert L.tt_k_muon_multi_ws(r, c, 2) <= _images(m, n) + _images(300, 400) + more

@@ -56,7 +56,8 @@ inline int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 constexpr float UP = 16384.f, DOWN2 = 1.f / (16384.f * 16384.f);
 constexpr int MOST = TT_SGD_MAX;   // matrices of different shapes in one run of launches
-constexpr int ALIKE = 64;          // of one shape
+constexpr int ALIKE = 64;          // of one shape, of up to
+constexpr long ALIKE_BYTES = 1L << 32;  // of images
 constexpr int NORM_PARTS = 1024;   // sums of squares of a matrix
 constexpr int MOST_STEPS = 6;      // with the scales measured before the first
 
@@ -1628,12 +1629,14 @@ size_t ws_of(const Matrices<N> &a, size_t images) {
   return images + sizeof(float) * (t == 0 ? 1024 * SHARERS : 2 * t * t * 256);
 }
 
-// `count` matrices of one shape
+// As many of `count` matrices of one shape as go together (blocks are of 32 x 32, so a
+// flat matrix's images are many times as large as it: 1 x 2^20 has 403 MB)
 Matrices<1> alike(long count, long rows, long cols, char *ws) {
   Matrices<1> a = {};
-  a.count = (int)(count < ALIKE ? count : ALIKE);
   lay(a.at[0], rows, cols, ws);
   a.images = a.at[0].bytes();
+  const long most = ALIKE_BYTES / a.images < 1 ? 1 : ALIKE_BYTES / a.images < ALIKE ? ALIKE_BYTES / a.images : ALIKE;
+  a.count = (int)(count < most ? count : most);
   return a;
 }
 
@@ -1659,15 +1662,15 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
   Matrices<1> a = alike(count, rows, cols, (char *)ws);
   const bool blocks = by_block(a);  // (of the last group too, however few are left for it)
   const int most = blocks ? 1 << 20 : a.count;  // without images any number at once
+  char *const rest = (char *)ws + a.count * a.images;
   for (long base = 0; base < count; base += most) {
     a.count = (int)(count - base < most ? count - base : most);
     a.at[0].g = x + base * rows * cols;
     a.at[0].w = y + base * rows * cols;
-    char *rest = (char *)ws + (size_t)(count < ALIKE ? count : ALIKE) * a.images;
     // More steps than the scales hold for go on from y.  By launches then each begins
     // anew and adds to y: what is weak by its row and its column, and so in every image,
     // is carried in fp32 (60 x 500 with 1e-7 of half of both: a column's 3e-6 after 16
-    // steps, 2e-4 from images of six).  In LDS X is fp32 throughout.
+    // steps, 2e-4 from images of six).  In LDS such an X is fp32 throughout.
     const int each = steps <= MOST_STEPS || blocks ? MOST_STEPS : 1;
     a.at[0].onto = each == 1, a.at[0].keep = TT_NS_A, a.at[0].rate = 1.f;
     for (int done = 0; done < steps; done += each) {
