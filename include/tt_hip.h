@@ -494,7 +494,7 @@ int tt_k_embedding_fwd(const float *w, const int32_t *ids, float *y, long rows, 
 /* The table's gradient: dw[v] = scale * the sum of dy's rows whose token is v, in
  * the order of the rows; accumulate != 0: added to dw, whose other rows are then
  * not touched (0: they are cleared).  ws: 16-byte aligned, 16 bytes a row and at most
- * one a value; none (size 0) for up to 512 rows. */
+ * one a value, rows rounded up to a multiple of 8; none (size 0) for up to 512 rows. */
 size_t tt_k_embedding_bwd_ws(long rows, long vocab, long cols);
 int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows, long vocab,
                        long cols, float scale, int accumulate, void *ws);

@@ -138,3 +138,10 @@ def test_workspace_of_flat_matrices(L, m, n):
         assert ws == L.tt_k_newton_schulz_ws(count, n, m)
     r, c = (ctypes.c_long * 2)(m, 300), (ctypes.c_long * 2)(n, 400)
     assert L.tt_k_muon_multi_ws(r, c, 2) <= _images(m, n) + _images(300, 400) + more
+
+
+@pytest.mark.parametrize("rows,cols", [(513, 1), (514, 3), (520, 1), (8191, 1), (66000, 1), (70001, 5), (100001, 300),
+                                       (8193, 1 << 20)])
+def test_workspace_of_the_tables_gradient(L, rows, cols):
+    full = (rows + 7) // 8 * 8
+    assert 16 * rows <= L.tt_k_embedding_bwd_ws(rows, 1000, cols) <= 16 * full + full * cols
