@@ -132,7 +132,8 @@ int     ag_sgd_step_many(AGNode *const *leaves, int count, float lr);
  *                 (reference tests/gate_cifar_cnn.py:81-98)
  *   muon:         tt_k_muon_multi (tt_hip.h) on shape[0] x the other axes of
  *                 each parameter; a list with a parameter of one axis or of a
- *                 single tensor twice is refused, nothing is updated
+ *                 single tensor twice is refused; then, and where a step's
+ *                 workspace cannot be had, nothing is updated
  * Arithmetic of the first two matches NumPy's on float32 arrays with Python-float
  * hyperparameters.  Returns NULL / -1 on bad arguments or OOM. */
 typedef struct AGOptim AGOptim;

@@ -2097,6 +2097,26 @@ static int muon_takes(AGNode *const *params, int count) {
     return 1;
 }
 
+/* One workspace for all of a step's runs of launches, taken before the first, with
+ * everything on the device: a step that cannot be made leaves nothing half done. */
+static int muon_ready(AGNode *const *params, int count, void **ws) {
+    size_t most = 0;
+    for (int base = 0; base < count; base += TT_SGD_MAX) {
+        long rows[TT_SGD_MAX], cols[TT_SGD_MAX];
+        int k = 0;
+        for (int i = base; i < count && i < base + TT_SGD_MAX; i++) {
+            if (!params[i]->grad) continue;
+            if (!tt_dev(params[i]->val) || !tt_dev(params[i]->grad)) return -1;
+            sides(params[i]->val, &rows[k], &cols[k]);
+            k++;
+        }
+        const size_t need = tt_k_muon_multi_ws(rows, cols, k);
+        if (need > most) most = need;
+    }
+    *ws = most ? ttrt_alloc(most) : NULL;
+    return most && !*ws ? -1 : 0;
+}
+
 void ag_optim_release(AGOptim *o) {
     if (!o) return;
     for (int i = 0; i < o->nslots; i++) {
@@ -2159,6 +2179,8 @@ int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
     for (int i = 0; i < count; i++)
         if (!params[i] || params[i]->val->numel != o->numel[i]) return -1;
 
+    void *ws = NULL;
+    if (o->kind == OPT_MUON && muon_ready(params, count, &ws) != 0) return -1;
     double lr_t = 0.0;
     if (o->kind == OPT_ADAM) {
         /* tests/gate_cifar_cnn.py:93-94 */
@@ -2177,7 +2199,10 @@ int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
             if (!l->grad) continue;   /* no gradient reached it: state untouched */
             w[k] = tt_dev(l->val);
             g[k] = tt_dev(l->grad);
-            if (!w[k] || !g[k]) return -1;
+            if (!w[k] || !g[k]) {
+                ttrt_free(ws);
+                return -1;
+            }
             m[k] = o->m[i];
             v[k] = o->v[i];
             n[k] = o->numel[i];
@@ -2190,12 +2215,16 @@ int ag_optim_step(AGOptim *o, AGNode *const *params, int count) {
             rc = tt_k_momentum_multi(w, g, m, n, k, (float)o->lr, (float)o->mu);
         else if (o->kind == OPT_MUON)
             rc = tt_k_muon_multi(w, g, m, rows, cols, k, (float)o->lr, (float)o->mu, o->nesterov,
-                                 (float)o->decay, NULL);
+                                 (float)o->decay, ws);
         else
             rc = tt_k_adam_multi(w, g, m, v, n, k, (float)o->b1, (float)(1.0 - o->b1),
                                  (float)o->b2, (float)(1.0 - o->b2), (float)o->eps, lr_t);
-        if (rc) return -1;
+        if (rc) {
+            ttrt_free(ws);
+            return -1;
+        }
     }
+    ttrt_free(ws);
     return 0;
 }
 
