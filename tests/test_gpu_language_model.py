@@ -247,3 +247,27 @@ def test_calls_captured_into_a_graph(tlib):
         check(tlib.tth_sync(), "sync")
         assert hip["hipGraphExecDestroy"](ready) == 0
         assert hip["hipGraphDestroy"](graph) == 0
+
+
+def test_updates_of_a_training_step_by_norm(tlib):
+    """What Muon makes of a model's own gradients, some of low rank: as near as of any
+    matrix, two steps on."""
+    from tinytorch_amd.torch_py import Node, Optim
+    p = _params(5)
+    P = {n: Node.leaf(p[n]) for n in NAMES}
+    lr, mu, decay = (float(np.float32(t)) for t in (0.02, 0.9, 0.01))
+    muon, v = Optim.muon(lr=lr, momentum=mu, weight_decay=decay), {n: 0.0 for n in MATRICES}
+    near = ref.A**4 * ref.PART  # a rounding of the products' parts through four steps' slope at 0
+    for step in range(2):
+        P = {n: t.detach() for n, t in P.items()}
+        _loss(Node, P, *_tokens(step)).backward(None)
+        before = {n: P[n].value().astype(np.float64) for n in MATRICES}
+        grads = {n: P[n].grad().astype(np.float64) for n in MATRICES}
+        muon.step([P[n] for n in MATRICES])
+        for n in MATRICES:
+            v[n] = mu * v[n] + grads[n]
+            x, _ = ref.newton_schulz(mu * v[n] + grads[n], 5)
+            new = -lr * 0.2 * np.sqrt(max(x.shape)) * x
+            off = np.linalg.norm(P[n].value() - (1 - lr * decay) * before[n] - new)
+            size = np.linalg.norm(new)
+            assert off <= near * size + 4 * ref.U * (np.linalg.norm(before[n]) + size), (step, n, off / size)
