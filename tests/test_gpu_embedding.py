@@ -191,3 +191,29 @@ def test_embedding_gradient_by_differences(tlib):
 
     g = _grad(tlib, ids, dy, 17, 1.5)
     assert abs((f(1e-3) - f(-1e-3)) / 2e-3 - (g * d).sum()) <= 1e-5 * np.abs(g * d).sum()
+
+
+@pytest.mark.parametrize("bound", ["ctypes", "pybind"])
+def test_embedding_node_ids_of_other_types(tlib, bound):
+    """Ids are whole numbers by type: 1.7 is not taken for 1."""
+    if bound == "ctypes":
+        from tinytorch_amd.torch_py import Node
+    else:
+        import sys
+        import tinytorch_amd
+        if tinytorch_amd.BUILD not in sys.path:
+            sys.path.insert(0, tinytorch_amd.BUILD)
+        from tinytorch_pybind import Node
+    w = np.random.default_rng(11).standard_normal((9, 5)).astype(np.float32)
+    W = Node.leaf(w)
+    for ids in ([1.7, 2.0], np.array([1.0, 2.0]), np.array([1, 2], np.float32), np.array([np.nan]), [1 + 0j], 2.0, ["1"],
+                [], [None]):
+        with pytest.raises(ValueError):
+            W.embedding(ids)
+    for kind in (np.int8, np.uint8, np.int16, np.uint16, np.int32, np.uint32, np.int64, np.uint64):
+        ids = np.array([[3, 0, 8], [1, 1, 2]], kind)
+        assert np.array_equal(W.embedding(ids).value(), w[ids.ravel().astype(int)])
+        assert np.array_equal(W.embedding(ids[:, ::2]).value(), w[ids[:, ::2].ravel().astype(int)])
+    assert np.array_equal(W.embedding(4).value(), w[[4]])
+    top = np.array([2**64 - 1, 2**63 + 4, 5], np.uint64)  # outside, not -1 + 2^64's low bits
+    assert np.array_equal(W.embedding(top).value(), np.stack([0 * w[0], 0 * w[0], w[5]]))

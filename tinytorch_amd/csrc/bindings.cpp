@@ -152,8 +152,15 @@ class PyNode {
     if (residual.is_none()) return py::cast(y);
     return py::make_tuple(y, PyNode(sum));
   }
-  // wider ids are outside the table, not what their low 32 bits say
-  PyNode embedding(py::array_t<int64_t, py::array::c_style | py::array::forcecast> ids, float scale) {
+  // whole numbers by type (a cast would take 1.7 for 1); wider ids are outside the table,
+  // not what their low 32 bits say
+  PyNode embedding(const py::object &given, float scale) {
+    const py::array any = py::array::ensure(given);
+    if (!any || !std::strchr("biu", any.dtype().kind())) {
+      PyErr_Clear();
+      throw py::value_error("tinytorch: ids are not whole numbers");
+    }
+    const auto ids = py::array_t<int64_t, py::array::c_style | py::array::forcecast>::ensure(any);
     std::vector<int> tokens((size_t)ids.size());
     for (size_t i = 0; i < tokens.size(); i++)
       tokens[i] = ids.data()[i] == (int)ids.data()[i] ? (int)ids.data()[i] : -1;

@@ -158,8 +158,11 @@ class Node:
 
     def embedding(self, ids, scale=1.0):
         """scale times this table's rows at ids (any shape, flattened); an id outside
-        the table: a row of zeros."""
-        ids = np.asarray(ids, dtype=np.int64)
+        the table: a row of zeros.  Ids are whole numbers by type."""
+        ids = np.asarray(ids)
+        if ids.dtype.kind not in "biu":
+            raise ValueError("tinytorch: ids are not whole numbers")
+        ids = ids.astype(np.int64)
         tokens = ids.astype(np.int32, order="C")
         tokens[tokens != ids] = -1  # not what the low 32 bits say
         return Node(_checked(LIB.ag_embedding(self.ptr, tokens.ctypes.data, tokens.size, scale), "ag_embedding"))
