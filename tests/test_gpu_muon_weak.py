@@ -140,18 +140,17 @@ def test_bad_values_among_weak(tlib, rows, cols):
         assert (_run(tlib, x, steps) == 0).all()
 
 
-@pytest.mark.parametrize("count,rows,cols", [(12, 1, 1 << 20), (13, 1 << 20, 1)])
+@pytest.mark.parametrize("count,rows,cols", [(6, 33, 1 << 20), (7, 1 << 20, 34)])
 def test_flat_matrices_in_groups(tlib, count, rows, cols):
-    """Their images pass 4 GiB together: a part of them at a time, each as alone."""
+    """Their images pass 4 GiB together: a part of them at a time."""
     alone, all_ws = (tlib.tt_k_newton_schulz_ws(n, rows, cols) for n in (1, count))
     assert all_ws < 5 << 30 and all_ws < count * alone
-    x = np.random.default_rng(5).standard_normal((count, rows, cols)).astype(np.float32)
+    x = np.random.default_rng(5).standard_normal((1, rows, cols), np.float32)
+    x = np.concatenate([x * np.float32(2.0**i) for i in range(count)])
     x[count - 2] = 0
-    got = _run(tlib, x, 5)
-    for i in (0, count // 2, count - 2, count - 1):
-        assert np.array_equal(got[i], _run(tlib, x[i], 5))
-        norm, s = np.linalg.norm(x[i].astype(np.float64)), 1.0
-        for _ in range(5):  # a single row's singular value
-            s = ref.A * s + ref.B * s**3 + ref.C * s**5
-        want = x[i] * (s / norm if norm else 0.0)
-        assert np.linalg.norm(got[i] - want) <= NEAR * abs(s)
+    got, want = _run(tlib, x, 2), _steps(x[0], 2)
+    # (a part's products go by tiles of their own, so the sums' order is not that of one alone)
+    for g in (got[0], got[count // 2], got[count - 1], _run(tlib, x[0], 2)):
+        worst = _worst(g, want)
+        assert max(worst) <= NEAR, worst
+    assert (got[count - 2] == 0).all()

@@ -145,3 +145,12 @@ def test_workspace_of_flat_matrices(L, m, n):
 def test_workspace_of_the_tables_gradient(L, rows, cols):
     full = (rows + 7) // 8 * 8
     assert 16 * rows <= L.tt_k_embedding_bwd_ws(rows, 1000, cols) <= 16 * full + full * cols
+
+
+@pytest.mark.parametrize("m,n", [(1, 1 << 20), (32, 1 << 20), (4, 4096), (3, 1025), (16, 70001)])
+def test_workspace_of_few_rows(L, m, n):
+    for count in (1, 5, 64, 1000):
+        assert 0 < L.tt_k_newton_schulz_ws(count, m, n) <= min(count, 64) * 600000
+        assert L.tt_k_newton_schulz_ws(count, m, min(n, 1024)) == 0
+    many = (ctypes.c_long * 16)(*[m] * 16), (ctypes.c_long * 16)(*[n] * 16)
+    assert L.tt_k_muon_multi_ws(*many, 16) <= 16 * 600000

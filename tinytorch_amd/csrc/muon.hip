@@ -32,9 +32,11 @@
 // instructions take them, four times 1 KB: h of the columns 0 to 15, where lane l
 // has eight of row l % 32 from column 8 (l / 32) on, of the columns 16 to 31, and l
 // of both; zeros behind the last row and column.  A wave's load is then 1 KB in one
-// piece (rows of 128 bytes, 32 of them a load, take the address unit 40 cycles: three
-// times as long a product of 16 x 4000).  Both operands of a product are read along
-// rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
+// piece (rows of 128 bytes, 32 of them a load, take the address unit 40 cycles: a
+// product of few long rows three times as long).  Both operands of a product are read
+// along rows: P = X X^T, P P = P P^T, Q X = Q (X^T)^T.
+//
+// Matrices of up to 32 rows or columns go another way, in 64 bits (FEW).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -60,6 +62,8 @@ constexpr int ALIKE = 64;          // of one shape, of up to
 constexpr long ALIKE_BYTES = 1L << 32;  // of images
 constexpr int NORM_PARTS = 1024;   // sums of squares of a matrix
 constexpr int MOST_STEPS = 6;      // with the scales measured before the first
+constexpr int FEW = 32;            // up to so many rows
+constexpr int FEW_SHORT = 1024, FEW_ALONE = 16384, FEW_PARTS = 64;
 
 __host__ __device__ inline long blocks_of(int k) { return (k + 31) / 32; }
 
@@ -72,7 +76,7 @@ struct Matrix {
   int m, n;         // shorter and longer side
   short turned;     // more rows than columns: X is U^T
   short onto;
-  int parts;        // of the norm
+  int parts;        // of the norm; of few rows' P
   // Images of G (m rows), of T (n rows; the steps write one from the other), of P and Q.
   __device__ char *x() const { return base; }
   __device__ char *t(int odd) const { return base + side + (odd ? side : 0); }
@@ -86,6 +90,8 @@ struct Matrix {
   // and of rows and columns, in 64 of the other: where the second T comes to lie
   __device__ double *of_rows() const { return (double *)t(1); }
   __device__ double *of_cols() const { return of_rows() + (long)(turned ? n : m) * (((turned ? m : n) + 63) / 64); }
+  // Of few long rows: parts of P, and behind them T and what X = U times.
+  __device__ double *few() const { return (double *)base; }
   __host__ long bytes() const {
     const long all = 3 * side + 2 * square + 64 * (blocks_of(m) + blocks_of(n)) + 8 * (NORM_PARTS + 1);
     return (all + 255) / 256 * 256;
@@ -175,6 +181,209 @@ __device__ __forceinline__ void put16(char *image, long blocks, int r, int c, co
   p[0] = h[0], p[32] = h[1], p[128] = l[0], p[160] = l[1];
 }
 
+// v = mu v + g where there are momenta, and u = g + mu v (nesterov) or v; without g
+template <class V>
+__device__ __forceinline__ V momentum(const float *g, float *v, float mu, int nesterov, bool store) {
+  V u = *(const V *)g;
+  if (!v) return u;
+  V w = *(const V *)v;
+  if (store) {
+    w = w * mu + u;
+    *(V *)v = w;
+  }
+  return nesterov ? w * mu + u : w;
+}
+
+// ---------------------------------------------------------------- few rows
+//
+// All steps together are a product from the left, X <- T X, and T is made of P alone:
+//   P = X X^T;  M = a I + b P + c P P,  T <- M T,  P <- M P M
+// (P, M and T have the same eigenvectors, so they are symmetric and their products in
+// any order).  With up to FEW rows these are small, and X is read twice, whatever the
+// steps: for P and for T X.  P has squares of X's values, so it is formed in 64 bits,
+// as are the steps; entries of weak rows are as near as any, since P = D C D keeps its
+// form.  (In images a single row would have blocks of 32 x 32, and where sums are as
+// short as these the parts' 22 bits show: up to 5 times as far off as fp32 products.)
+// A workgroup has a matrix of up to FEW_SHORT columns, bound by latency: five steps of 32 x
+// 32 take 23 us (1.1 us a step of up to 16 rows, 1.8 of more), of 10 x 785 29, of 32 x
+// 1024 49.  Longer ones are cut: parts of P, then one workgroup for the steps, then T X:
+// 16 x 100000 48 us, 32 x 2^20 335 (through images 155 and 1150).
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr double NS_A = 3.4445, NS_B = -4.7750, NS_C = 2.0315;  // not as fp32 rounds them
+static_assert((float)NS_A == TT_NS_A && (float)NS_B == TT_NS_B && (float)NS_C == TT_NS_C, "one polynomial");
+constexpr int FEW_COLS = 256, FEW_THREADS = 1024;
+struct Few {
+  float tile[FEW][FEW_COLS + 1];  // columns of X
+  double a[4][FEW][FEW + 2];      // P, M, T, M P; parts of P before
+};
+// f(k, i, c, at) for this thread's k-th value, row i and column c of X's columns from c0
+// on, at `at` of the matrix as it is given; one behind the last column has at < 0.
+// Along the memory's rows.
+template <class F>
+__device__ __forceinline__ void few_values(const Matrix &M, long c0, const F &f) {
+#pragma unroll
+  for (int k = 0; k < FEW * FEW_COLS / FEW_THREADS; k++) {
+    const unsigned x = threadIdx.x + k * FEW_THREADS, m = (unsigned)M.m;
+    if (x >= m * FEW_COLS) break;
+    const unsigned c = M.turned ? x / m : x % FEW_COLS, i = M.turned ? x - c * m : x / FEW_COLS;
+    f(k, i, c, c0 + c < M.n ? (M.turned ? c0 * m + x : (long)i * M.n + c0 + c) : -1l);
+  }
+}
+// U's columns from `from` to `to` (FEW_COLS, or fewer at the end) in the tile for f(c0),
+// one after the other, the next on their way meanwhile; `store`: with the momenta.
+template <class F>
+__device__ __forceinline__ void few_tiles(const Matrix &M, Few &s, long from, long to, float mu, int nesterov, bool store,
+                                          const F &f) {
+  float u[FEW * FEW_COLS / FEW_THREADS];
+  auto load = [&](long c0) {
+    few_values(M, c0, [&](int k, unsigned, unsigned, long at) {
+      u[k] = at < 0 ? 0.f : momentum<float>(M.g + at, M.v ? M.v + at : nullptr, mu, nesterov, store);
+    });
+  };
+  load(from);
+  for (int i = M.m * FEW_COLS + threadIdx.x; i < FEW * FEW_COLS; i += FEW_THREADS) s.tile[i / FEW_COLS][i % FEW_COLS] = 0.f;
+  for (long c0 = from; c0 < to; c0 += FEW_COLS) {
+    __syncthreads();  // the last columns are read
+    few_values(M, c0, [&](int k, unsigned i, unsigned c, long) { s.tile[i][c] = u[k]; });
+    __syncthreads();
+    if (c0 + FEW_COLS < to) load(c0 + FEW_COLS);
+    f(c0);
+  }
+}
+// a[0] = U U^T of the columns from `from` to `to`.  Of 16 waves four have the same 64 of
+// the columns, a quarter of the result each (but that above the diagonal).  The
+// instruction's lane l holds row l % 16 of either operand and column l / 16 of four, and
+// of the result the rows l / 16 + 4 i of column l % 16.
+__device__ __forceinline__ void few_gram(const Matrix &M, Few &s, long from, long to, float mu, int nesterov) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 15, high = lane >> 4;
+  const int qi = (wave >> 1 & 1) * 16, qj = (wave & 1) * 16, part = wave >> 2;
+  const bool on = qj <= qi && qi < M.m;
+  f64x4 acc = {};
+  few_tiles(M, s, from, to, mu, nesterov, true, [&](long) {
+    if (!on) return;
+#pragma unroll 4
+    for (int k = 0; k < 16; k++) {
+      const int c = part * 64 + k * 4 + high;
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(s.tile[qi + low][c], s.tile[qj + low][c], acc, 0, 0, 0);
+    }
+  });
+#pragma unroll
+  for (int i = 0; i < 4; i++) s.a[part][qi + 4 * i + high][qj + low] = acc[i];
+  __syncthreads();
+  const int r = threadIdx.x >> 5, c = threadIdx.x & 31, i = r < 16 && c >= 16 ? c : r, j = i == r ? c : r;
+  const double v = (s.a[0][i][j] + s.a[1][i][j]) + (s.a[2][i][j] + s.a[3][i][j]);
+  __syncthreads();
+  s.a[0][r][c] = v;
+  __syncthreads();
+}
+// From U U^T in a[0]: T of so many steps to a[2]; what X = U times is returned.  Four
+// waves have a quarter each (one where a quarter is all).
+__device__ __forceinline__ double few_steps(const Matrix &M, Few &s, int steps) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 15, high = lane >> 4;
+  const int qi = (wave >> 1 & 1) * 16, qj = (wave & 1) * 16, k4 = M.m > 16 ? 8 : 4;
+  const bool on = wave < 4 && qi < M.m && qj < M.m;
+  double norm = 0.0;
+#pragma unroll 8
+  for (int i = 0; i < M.m; i++) norm += s.a[0][i][i];
+  // zeros stay zeros; an infinity or a NaN makes all of it NaN
+  const double over = norm == 0.0 ? 0.0 : norm < __builtin_inf() ? 1.0 / norm : __builtin_nan("");
+  __syncthreads();
+  s.a[0][threadIdx.x >> 5][threadIdx.x & 31] *= over;
+  __syncthreads();
+  auto times = [&](int x, int y) {  // (the right one is symmetric)
+    f64x4 acc = {};
+    if (!on) return acc;
+#pragma unroll 4
+    for (int k = 0; k < k4; k++)
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(s.a[x][qi + low][4 * k + high], s.a[y][qj + low][4 * k + high], acc, 0, 0, 0);
+    return acc;
+  };
+  auto put = [&](int x, f64x4 v) {
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) s.a[x][qi + 4 * i + high][qj + low] = v[i];
+  };
+  for (int step = 0; step < steps; step++) {
+    f64x4 m = times(0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = qi + 4 * i + high, c = qj + low;
+      m[i] = (r == c && r < M.m ? NS_A : 0.0) + NS_B * s.a[0][r][c] + NS_C * m[i];
+    }
+    put(1, m);
+    __syncthreads();
+    const bool last = step + 1 == steps;
+    const f64x4 t = step ? times(1, 2) : m;
+    f64x4 r = {};
+    if (!last) r = times(1, 0);
+    __syncthreads();
+    put(2, t);
+    put(3, r);
+    __syncthreads();
+    if (!last) put(0, times(1, 3));
+    __syncthreads();
+  }
+  return sqrt(over);
+}
+// w = T X, or onto w, of the columns from `from` to `to`: a wave has 16 of each 256.
+__device__ __forceinline__ void few_apply(const Matrix &M, Few &s, long from, long to, double scale, float mu, int nesterov) {
+  const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4, col = (threadIdx.x >> 6) * 16 + low;
+  const int k4 = M.m > 16 ? 8 : 4;
+  few_tiles(M, s, from, to, mu, nesterov, false, [&](long c0) {
+    f64x4 x[2] = {};
+#pragma unroll 4
+    for (int k = 0; k < k4; k++) {
+      const double u = s.tile[4 * k + high][col];
+      x[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(s.a[2][low][4 * k + high], u, x[0], 0, 0, 0);
+      if (M.m > 16) x[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(s.a[2][16 + low][4 * k + high], u, x[1], 0, 0, 0);
+    }
+    // (these columns are this wave's)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      s.tile[4 * i + high][col] = (float)(x[0][i] * scale);
+      if (M.m > 16) s.tile[16 + 4 * i + high][col] = (float)(x[1][i] * scale);
+    }
+    __syncthreads();
+    few_values(M, c0, [&](int, unsigned i, unsigned c, long at) {
+      if (at >= 0) M.w[at] = M.onto ? M.keep * M.w[at] + M.rate * s.tile[i][c] : s.tile[i][c];
+    });
+  });
+}
+
+template <int N>
+__global__ void __launch_bounds__(FEW_THREADS) few_gram_kernel(Matrices<N> a, float mu, int nesterov) {
+  __shared__ Few s;
+  unsigned b = blockIdx.x;
+  const Matrix M = matrix_of(a, b);
+  const long tiles = (M.n + FEW_COLS - 1) / FEW_COLS, to = tiles * (b + 1) / M.parts * FEW_COLS;
+  few_gram(M, s, tiles * b / M.parts * FEW_COLS, to < M.n ? to : M.n, mu, nesterov);
+  M.few()[(long)b * FEW * FEW + threadIdx.x] = s.a[0][threadIdx.x >> 5][threadIdx.x & 31];
+}
+template <int N>
+__global__ void __launch_bounds__(FEW_THREADS) few_steps_kernel(Matrices<N> a, int steps) {
+  __shared__ Few s;
+  const Matrix M = matrix(a, blockIdx.x);
+  double v = 0.0, *at = M.few() + threadIdx.x;
+#pragma unroll 16
+  for (int b = 0; b < M.parts; b++, at += FEW * FEW) v += *at;
+  s.a[0][threadIdx.x >> 5][threadIdx.x & 31] = v;
+  __syncthreads();
+  const double scale = few_steps(M, s, steps);
+  *at = s.a[2][threadIdx.x >> 5][threadIdx.x & 31];
+  if (threadIdx.x == 0) at[FEW * FEW] = scale;
+}
+template <int N>
+__global__ void __launch_bounds__(FEW_THREADS) few_apply_kernel(Matrices<N> a, float mu, int nesterov) {
+  __shared__ Few s;
+  unsigned b = blockIdx.x;
+  const Matrix M = matrix_of(a, b);
+  const double *in = M.few() + (long)M.parts * FEW * FEW;
+  s.a[2][threadIdx.x >> 5][threadIdx.x & 31] = in[threadIdx.x];  // (few_tiles waits for it)
+  const long from = (long)b * FEW_COLS, to = from + FEW_COLS;
+  few_apply(M, s, from, to < M.n ? to : M.n, in[FEW * FEW], mu, nesterov);
+}
+
 // ---------------------------------------------------------------- small matrices
 //
 // A matrix that fits LDS, X and the image of P or Q (which follow each other in one
@@ -190,16 +399,16 @@ __device__ __forceinline__ void put16(char *image, long blocks, int r, int c, co
 // they are read, by rows with their scales for C and by columns with theirs for the
 // step; the scales come from the largest value of a row and its length (five steps of
 // 64 x 64: 26 us and 32, 500 of 128 x 128 157 and 214).
-// Latency bounds it, of LDS and between the products of a chain: five steps of 32 x 32
-// take 22 us, of 64 x 64 26, of 96 x 96 46, of 64 of 64 x 64 27.
+// Latency bounds it, of LDS and between the products of a chain: five steps of 64 x 64
+// take 26 us, of 96 x 96 46, of 64 of 64 x 64 27.
 
 constexpr int BLOCK_WAVES = 16, BLOCK_LDS = 39 * 4096;
 constexpr int BLOCK_KEEP = 3;  // blocks of X a wave
 constexpr float EVEN = 0x1p-22f;
-// X, P and the partial sums of P (one or four blocks of it: eight or two waves each)
+// X, P and the partial sums of P (four blocks of it: two waves each)
 __host__ __device__ inline long block_bytes(int m, int n) {
   const long mb = blocks_of(m), nb = blocks_of(n);
-  return 4096 * (mb * nb + mb * mb + (mb == 1 ? 7 : mb == 2 ? 4 : 0));
+  return 4096 * (mb * nb + mb * mb + (mb == 2 ? 4 : 0));
 }
 // Of a few matrices those whose products have up to 48 blocks (five steps of 96 x 96:
 // 46 us, and 59 by launches of a product each; of 128 x 128 66 and 60), of many all that
@@ -305,19 +514,6 @@ __device__ __forceinline__ void put4(char *image, int blocks, int r, int c, f32x
   *(half4 *)(chunk_of(image, blocks, r, c >> 5, 4 + (c >> 3 & 3)) + (c & 4) * 2) = l;
 }
 
-// v = mu v + g where there are momenta, and u = g + mu v (nesterov) or v; without g
-template <class V>
-__device__ __forceinline__ V momentum(const float *g, float *v, float mu, int nesterov, bool store) {
-  V u = *(const V *)g;
-  if (!v) return u;
-  V w = *(const V *)v;
-  if (store) {
-    w = w * mu + u;
-    *(V *)v = w;
-  }
-  return nesterov ? w * mu + u : w;
-}
-
 // The steps of X in LDS and the result to w; VALUES: X are fp32 values, else an image.
 template <bool VALUES>
 __device__ __forceinline__ void steps_in_lds(const Matrix &M, int steps, char *lds, const Scale *scales, int lane, int wave) {
@@ -335,8 +531,8 @@ __device__ __forceinline__ void steps_in_lds(const Matrix &M, int steps, char *l
       return (f32x4){value_of(x[0]), value_of(x[1]), value_of(x[2]), value_of(x[3])};
     };
     const int low = lane & 31, high = (lane >> 5) * 4;  // result i: values high + 8 (i / 4) + i % 4 of row low
-    // C = G G^T: with one block of it (four) eight waves (two) share the sum
-    const int pb = mb * mb, ways = mb == 1 ? 8 : mb == 2 ? 2 : 1;
+    // C = G G^T: with four blocks of it two waves share the sum
+    const int pb = mb * mb, ways = mb == 2 ? 2 : 1;
     f32x4 c4[4];
     {
       const int f = wave % pb, way = wave / pb, ra = f / mb * 32, rb = f % mb * 32;
@@ -467,10 +663,17 @@ template <int N>
 __global__ void __launch_bounds__(BLOCK_WAVES * 64)
     block_kernel(Matrices<N> a, int steps, float mu, int nesterov, int again, unsigned room) {
   __shared__ __attribute__((aligned(1024))) char lds[BLOCK_LDS];
-  __shared__ Scale scales[(4 + 31) * 32];  // of 4 blocks of rows and 31 of columns
+  __shared__ Scale scales[(4 + 15) * 32];  // of 4 blocks of rows and 15 of columns
   __shared__ double sums[BLOCK_WAVES];
   __shared__ float least[2][BLOCK_WAVES];
   const Matrix M = matrix(a, blockIdx.x);
+  if (M.m <= FEW) {
+    Few &few = *(Few *)lds;
+    few_gram(M, few, 0, M.n, mu, nesterov);
+    const double times = few_steps(M, few, steps);
+    few_apply(M, few, 0, M.n, times, mu, nesterov);
+    return;
+  }
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int mb = (int)blocks_of(M.m), nb = (int)blocks_of(M.n), count = M.m * M.n, cols = M.turned ? M.m : M.n;
@@ -1435,16 +1638,20 @@ bool good_sides(long rows, long cols) {
   return rows > 0 && cols > 0 && rows <= TT_MUON_MAX_SIDE && cols <= TT_MUON_MAX_SIDE && rows * cols <= TT_MUON_MAX_VALUES;
 }
 
-void lay(Matrix &M, long rows, long cols, char *&ws) {
+void lay(Matrix &M, long rows, long cols, bool few, char *&ws) {
   M.turned = rows > cols;
   M.m = (int)(M.turned ? cols : rows);
   M.n = (int)(M.turned ? rows : cols);
   const long tiles = (long)((M.m + 63) / 64) * ((M.n + 63) / 64);
   M.parts = (int)(tiles < NORM_PARTS ? tiles : NORM_PARTS);
-  M.base = ws;
+  if (few) {
+    const long few_tiles = (M.n + FEW_COLS - 1) / FEW_COLS;
+    M.parts = (int)(few_tiles < FEW_PARTS ? few_tiles : FEW_PARTS);
+  }
   M.side = 4096 * blocks_of(M.m) * blocks_of(M.n);
   M.square = 4096 * blocks_of(M.m) * blocks_of(M.m);
-  ws += M.bytes();
+  M.base = ws;
+  ws += few ? 8l * FEW * FEW * (M.parts + 1) + 256 : M.bytes();
 }
 
 template <int N, class F>
@@ -1459,12 +1666,31 @@ unsigned long number(Matrices<N> &a, F workgroups) {
   return N > 1 ? at : at * a.count;
 }
 
-// Whether every matrix has a workgroup of its own.
-template <int N>
-bool by_block(const Matrices<N> &a) {
-  for (int i = 0; i < (N > 1 ? a.count : 1); i++)
-    if (!fits_block(a.at[i].m, a.at[i].n, a.count)) return false;
-  return true;
+// How a matrix goes: by itself in a workgroup, as one of few long rows, or by products.
+enum Way { IN_LDS, FEW_LONG, PRODUCTS };
+// those of one way; `ways` of each
+Matrices<MOST> of_way(const Matrices<MOST> &a, const Way *ways, Way way) {
+  Matrices<MOST> some = {};
+  for (int i = 0; i < a.count; i++)
+    if (ways[i] == way) some.at[some.count++] = a.at[i];
+  return some;
+}
+// of many of one shape
+Way way_of(int m, int n, int count) {
+  if (m <= FEW) return n <= FEW_SHORT ? IN_LDS : FEW_LONG;
+  return fits_block(m, n, count) ? IN_LDS : PRODUCTS;
+}
+// Of a list's: matrices of few rows cost next to nothing in the launches that others
+// need anyway (129 x 10 beside 785 x 256 and 257 x 128: 99 us, 115 by itself), but for the
+// longest, whose blocks are mostly empty (1 x 2^20: 196 us, 1020 by products).
+void ways_of(const Matrices<MOST> &a, Way *ways) {
+  bool products = false;
+  for (int i = 0; i < a.count; i++) {
+    ways[i] = way_of(a.at[i].m, a.at[i].n, a.count);
+    products = products || ways[i] == PRODUCTS;
+  }
+  for (int i = 0; i < a.count && products; i++)
+    if (a.at[i].m > FEW || a.at[i].n <= FEW_ALONE) ways[i] = PRODUCTS;
 }
 
 // blocks of a product's length
@@ -1587,15 +1813,30 @@ void product(Matrices<N> &a, const Phase &phase, float *pieces, int to_w = 0) {
   else tile_product<KIND, 256, 2, N>(a, phase, to_w, pieces);
 }
 
+// Steps of matrices that a workgroup has; MOST_STEPS at most (of few rows any number),
+// `again`: of X that is given.
+template <int N>
+void run_in_lds(const Matrices<N> &a, int steps, float mu, int nesterov, int again = 0) {
+  if (a.count)
+    hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov, again,
+                       room_for(steps));
+}
+
+// Any number of steps of matrices of few long rows.
+template <int N>
+void run_few(Matrices<N> &a, int steps, float mu, int nesterov) {
+  if (!a.count) return;
+  unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
+  hipLaunchKernelGGL(few_gram_kernel<N>, dim3((unsigned)grid), dim3(FEW_THREADS), 0, stream(), a, mu, nesterov);
+  hipLaunchKernelGGL(few_steps_kernel<N>, dim3(a.count), dim3(FEW_THREADS), 0, stream(), a, steps);
+  grid = number(a, [](const Matrix &M) { return (long)((M.n + FEW_COLS - 1) / FEW_COLS); });
+  hipLaunchKernelGGL(few_apply_kernel<N>, dim3((unsigned)grid), dim3(FEW_THREADS), 0, stream(), a, mu, nesterov);
+}
+
 // Steps with the scales measured before the first, MOST_STEPS at most; `again`: of X
 // that is given.  `keep`: X goes to w, and the last step takes a X from there.
 template <int N>
-void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *rest, int again = 0, int keep = 0) {
-  if (blocks) {
-    hipLaunchKernelGGL(block_kernel<N>, dim3(a.count), dim3(BLOCK_WAVES * 64), 0, stream(), a, steps, mu, nesterov, again,
-                       room_for(steps));
-    return;
-  }
+void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest, int again = 0, int keep = 0) {
   unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
   hipLaunchKernelGGL(momentum_kernel<N>, dim3((unsigned)grid), dim3(256), 0, stream(), a, mu, nesterov);
   grid = number(a, [](const Matrix &M) {
@@ -1621,21 +1862,42 @@ void run(Matrices<N> &a, bool blocks, int steps, float mu, int nesterov, char *r
   }
 }
 
-// the images (of a group of matrices), and two pieces a workgroup, or one of a small tile
+// two pieces a workgroup, or one of a small tile
 template <int N>
-size_t ws_of(const Matrices<N> &a, size_t images) {
-  if (by_block(a)) return 0;
+size_t pieces_of(const Matrices<N> &a) {
   const int g = tile_size(a, GRAM), s = tile_size(a, STEP), t = g > s ? g : s;  // (SQUARE's: no larger than these)
-  return images + sizeof(float) * (t == 0 ? 1024 * SHARERS : 2 * t * t * 256);
+  return sizeof(float) * (t == 0 ? 1024 * SHARERS : 2 * t * t * 256);
+}
+
+// A list's matrices and their ways, laid into a workspace but for those that need none;
+// what follows them (pieces) is left at ws.  The bytes of all.
+size_t lay_all(Matrices<MOST> &a, Way *ways, const long *rows, const long *cols, int count, char *&ws) {
+  char *const start = ws;
+  a.count = count;
+  for (int i = 0; i < count; i++) {
+    char *none = NULL;
+    lay(a.at[i], rows[i], cols[i], false, none);
+  }
+  ways_of(a, ways);
+  bool products = false;
+  for (int i = 0; i < count; i++) {
+    if (ways[i] != IN_LDS) lay(a.at[i], rows[i], cols[i], ways[i] == FEW_LONG, ws);
+    products = products || ways[i] == PRODUCTS;
+  }
+  return (size_t)(ws - start) + (products ? pieces_of(of_way(a, ways, PRODUCTS)) : 0);
 }
 
 // As many of `count` matrices of one shape as go together (blocks are of 32 x 32, so a
-// flat matrix's images are many times as large as it: 1 x 2^20 has 403 MB)
-Matrices<1> alike(long count, long rows, long cols, char *ws) {
+// flat matrix's images are many times as large as it: 33 x 2^20 has 8 GB)
+Matrices<1> alike(long count, long rows, long cols, char *ws, Way &way) {
   Matrices<1> a = {};
-  lay(a.at[0], rows, cols, ws);
-  a.images = a.at[0].bytes();
-  const long most = ALIKE_BYTES / a.images < 1 ? 1 : ALIKE_BYTES / a.images < ALIKE ? ALIKE_BYTES / a.images : ALIKE;
+  const int m = (int)(rows < cols ? rows : cols), n = (int)(rows < cols ? cols : rows);
+  way = way_of(m, n, (int)(count < ALIKE ? count : ALIKE));
+  char *end = ws;
+  lay(a.at[0], rows, cols, way == FEW_LONG, end);
+  a.images = end - ws;
+  const long fit = ALIKE_BYTES / a.images < 1 ? 1 : ALIKE_BYTES / a.images;
+  const long most = way == IN_LDS ? 1 << 20 : fit < ALIKE ? fit : ALIKE;  // (in LDS any number at once)
   a.count = (int)(count < most ? count : most);
   return a;
 }
@@ -1644,8 +1906,9 @@ Matrices<1> alike(long count, long rows, long cols, char *ws) {
 
 extern "C" size_t tt_k_newton_schulz_ws(long count, long rows, long cols) {
   if (count <= 0 || !good_sides(rows, cols)) return 0;
-  const Matrices<1> a = alike(count, rows, cols, NULL);
-  return ws_of(a, a.count * (size_t)a.images);
+  Way way;
+  const Matrices<1> a = alike(count, rows, cols, NULL, way);
+  return way == IN_LDS ? 0 : a.count * (size_t)a.images + (way == PRODUCTS ? pieces_of(a) : 0);
 }
 
 extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long rows, long cols, int steps, void *ws) {
@@ -1659,22 +1922,27 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
     ws = own = ttrt_alloc(need);
     if (!ws) return -2;
   }
-  Matrices<1> a = alike(count, rows, cols, (char *)ws);
-  const bool blocks = by_block(a);  // (of the last group too, however few are left for it)
-  const int most = blocks ? 1 << 20 : a.count;  // without images any number at once
-  char *const rest = (char *)ws + a.count * a.images;
+  Way way;  // (of the last group too, however few are left for it)
+  Matrices<1> a = alike(count, rows, cols, (char *)ws, way);
+  const int most = a.count;
+  char *const rest = way == PRODUCTS ? (char *)ws + most * a.images : NULL;
+  // More steps than the scales hold for go on from y.  By products then each begins anew
+  // and adds to y: what is weak by its row and its column, and so in every image, is
+  // carried in fp32 (60 x 500 with 1e-7 of half of both: a column's 3e-6 after 16 steps,
+  // 2e-4 from images of six).  In LDS such an X is fp32 throughout.
+  const bool all = a.at[0].m <= FEW || steps <= MOST_STEPS;
+  const int each = all ? steps : way == IN_LDS ? MOST_STEPS : 1;
+  const int keep = way == PRODUCTS && !all;
+  a.at[0].onto = keep, a.at[0].keep = TT_NS_A, a.at[0].rate = 1.f;
   for (long base = 0; base < count; base += most) {
     a.count = (int)(count - base < most ? count - base : most);
     a.at[0].g = x + base * rows * cols;
     a.at[0].w = y + base * rows * cols;
-    // More steps than the scales hold for go on from y.  By launches then each begins
-    // anew and adds to y: what is weak by its row and its column, and so in every image,
-    // is carried in fp32 (60 x 500 with 1e-7 of half of both: a column's 3e-6 after 16
-    // steps, 2e-4 from images of six).  In LDS such an X is fp32 throughout.
-    const int each = steps <= MOST_STEPS || blocks ? MOST_STEPS : 1;
-    a.at[0].onto = each == 1, a.at[0].keep = TT_NS_A, a.at[0].rate = 1.f;
     for (int done = 0; done < steps; done += each) {
-      run(a, blocks, steps - done < each ? steps - done : each, 0.f, 0, rest, done > 0, each == 1);
+      const int n = steps - done < each ? steps - done : each;
+      if (way == IN_LDS) run_in_lds(a, n, 0.f, 0, done > 0);
+      else if (way == FEW_LONG) run_few(a, n, 0.f, 0);
+      else run(a, n, 0.f, 0, rest, done > 0, keep);
       a.at[0].g = a.at[0].w;
     }
   }
@@ -1684,16 +1952,12 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
 
 extern "C" size_t tt_k_muon_multi_ws(const long *rows, const long *cols, int count) {
   if (!rows || !cols || count < 1 || count > TT_SGD_MAX) return 0;
-  Matrices<MOST> a = {};
-  a.count = count;
-  size_t bytes = 0;
-  char *at = NULL;
-  for (int i = 0; i < count; i++) {
+  for (int i = 0; i < count; i++)
     if (!good_sides(rows[i], cols[i])) return 0;
-    lay(a.at[i], rows[i], cols[i], at);
-    bytes += (size_t)a.at[i].bytes();
-  }
-  return ws_of(a, bytes);
+  Matrices<MOST> a = {};
+  Way ways[MOST];
+  char *at = NULL;
+  return lay_all(a, ways, rows, cols, count, at);
 }
 
 extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *const *v, const long *rows,
@@ -1715,16 +1979,19 @@ extern "C" int tt_k_muon_multi(float *const *w, const float *const *g, float *co
     if (!ws) return -2;
   }
   Matrices<MOST> a = {};
-  a.count = count;
+  Way ways[MOST];
   char *at = (char *)ws;
+  lay_all(a, ways, rows, cols, count, at);
   for (int i = 0; i < count; i++) {
     Matrix &M = a.at[i];
     M.g = g[i], M.v = v[i], M.w = w[i], M.onto = 1;
     M.keep = (float)(1.0 - (double)lr * decay);
     M.rate = (float)(-(double)lr * TT_MUON_RMS * sqrt((double)(rows[i] > cols[i] ? rows[i] : cols[i])));
-    lay(M, rows[i], cols[i], at);
   }
-  run(a, by_block(a), TT_MUON_STEPS, mu, nesterov, at);
+  Matrices<MOST> few = of_way(a, ways, FEW_LONG), products = of_way(a, ways, PRODUCTS);
+  run_in_lds(of_way(a, ways, IN_LDS), TT_MUON_STEPS, mu, nesterov);
+  run_few(few, TT_MUON_STEPS, mu, nesterov);
+  if (products.count) run(products, TT_MUON_STEPS, mu, nesterov, at);
   ttrt_free(own);
   return launched();
 }
