@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(256) momentum_kernel(Matrices<N> a, float mu, 
 }
 
 // Up to this length the scales are formed with the images (785 x 256 with two smaller
-// ones: a launch of 4 us less; for 16 x 100000 the columns' took 11).
+// ones: a launch of 4 us less; for 40 x 70001 the launch takes 5).
 constexpr int MEASURE = 1024;
 
 // X = U times this; `again`: X is what is given
@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(1024) scale_kernel(Matrices<N> a, int again, u
 // The images of G and T, a tile of 64 x 64 at a time through LDS; both are written
 // along their rows.  `keep`: X goes to w as well.  The other scales are formed here, by
 // every tile of the same rows or columns again, and written by the first.  Bound by
-// memory: 34 us for 4096 x 4096 (5.9 TB/s).
+// memory: 35 us for 4096 x 4096 (5.7 TB/s).
 template <int N>
 __global__ void __launch_bounds__(256) image_kernel(Matrices<N> a, float mu, int nesterov, int again, int keep, unsigned room) {
   __shared__ float tile[64][65];
@@ -1069,7 +1069,7 @@ __device__ __forceinline__ void tile_of(U tile, int rows, int cols, int &ti, int
 // eight sums, joined in LDS.  What bounds these is the way from memory (the L2 of
 // another XCD has what the last launch wrote), so the added matrix is on its way
 // first, and a tile on the diagonal reads its rows once.  A launch takes 4 us at least;
-// 517 x 1003: 6 us for P, 5 for Q, 11 for X; 1400 x 1400: 18, 19 and 34 (490 TFLOP/s
+// 517 x 1003: 6 us for P, 5 for Q, 11 for X; 1024 x 1024: 11, 12 and 16 (400 TFLOP/s
 // of fp16 products).  Of few long tiles of P the length is shared by `ways` workgroups,
 // whose sums a second launch adds (join): one CU alone reads 80 GB/s.
 template <int KIND, bool SHARED, int N>
@@ -1196,8 +1196,8 @@ __global__ void __launch_bounds__(512, 2)
 //                 the SIMD fills a wave's waits, and memory gives half as much
 // A tile that one workgroup has is finished by it.  The others' parts go to memory,
 // and join_kernel adds them.  The matrix units bound these, at the clock that they
-// leave: X of 4096 x 4096 takes 345 us, 1200 TFLOP/s of fp16 products, with the units
-// 69 % busy at 1.84 GHz; of 2048 x 2048 by tiles of 128 50 us, 1030 TFLOP/s (51 % busy
+// leave: X of 4096 x 4096 takes 351 us, 1170 TFLOP/s of fp16 products, with the units
+// 68 % busy at 1.82 GHz; of 2048 x 2048 by tiles of 128 54 us, 950 TFLOP/s (46 % busy
 // at 2 GHz in a transformer block's six matrices).
 
 // Tiles of T x T: four waves of 64 x 64 or eight of 128 x 64 values, each FI x 2
@@ -1701,27 +1701,27 @@ long length_of(int kind, const Matrix &M) { return blocks_of(kind == GRAM ? M.n 
 // tiles are used for longer: they have less to compute twice, and their parts are joined
 // sooner.  But few tiles of 128 (136 of 2048 rows), or tiles of different lengths, are
 // cut into parts that are not in step, so that each XCD reads all of it from afar (two of
-// 4096^2, 1024 x 4096 and its turn: 9137 us with tiles of 256, 9798 with 128).  us of a
+// 4096^2, 1024 x 4096 and its turn: 9590 us with tiles of 256, 10080 with 128).  us of a
 // product, with what joins its parts:
 //                      P = X X^T            X <- a X + Q X
 //   tiles of         32   128   256        32   128   256
-//   1024^2           11    18     -        16    21     -
-//   700 x 4000       20    22     -        28    26     -
-//   2 x 1024^2       17    21     -        27    27     -
-//   1400^2           18    22     -        34    29     -
-//   1600^2           25    28     -        46    41     -
-//   1024 x 4096      33    25     -        47    31     -
-//   2048^2            -    40    57         -    52    79
-//   2500^2            -    77    79         -   119   119
-//   2048 x 4096       -    75    74         -    96   116
-//   2200 x 6300       -   104   117         -   196   192
-//   3000 x 5000       -   146   152         -   294   245
-//   2048 x 8192       -   157   116         -   188   188
-//   2100 x 12000      -   204   188         -   382   352
-//   4096^2            -   194   209         -   381   332
-//   4096 x 8192       -   376   377         -   792   674
-//   6000^2            -   600   570         -  1368  1074
-//   8192^2            -  1529  1327         -  3501  2529
+//   1024^2           11    18     -        16    24     -
+//   700 x 4000       20    21     -        28    25     -
+//   2 x 1024^2       18    20     -        29    30     -
+//   1400^2           20    23     -        38    30     -
+//   1600^2           27    28     -        50    45     -
+//   1024 x 4096      34    31     -        51    32     -
+//   2048^2            -    41    56         -    54    78
+//   2500^2            -    76    83         -   124   126
+//   2048 x 4096       -    75    75         -   103   120
+//   2200 x 6300       -   110   122         -   209   202
+//   3000 x 5000       -   152   160         -   313   262
+//   2048 x 8192       -   156   120         -   202   197
+//   2100 x 12000      -   204   201         -   387   354
+//   4096^2            -   203   218         -   394   353
+//   4096 x 8192       -   386   392         -   804   693
+//   6000^2            -   615   591         -  1377  1113
+//   8192^2            -  1542  1379         -  3573  2619
 template <int N>
 int tile_size(const Matrices<N> &a, int kind) {
   double work = 0, tiles = 0;  // (of 128)
@@ -1766,7 +1766,7 @@ void small_product(Matrices<N> &a, const Phase &phase, int to_w, float *pieces) 
 template <int KIND, int T, int BUFFERS, int N>
 void tile_product(Matrices<N> &a, const Phase &phase, int to_w, float *pieces) {
   typedef Shape<T, BUFFERS> S;
-  constexpr int EXTRA = T == 128 ? 12 : 6;  // (2375 x 1041 with five: 598 us with 4, 569 with 8, 559 with 12)
+  constexpr int EXTRA = T == 128 ? 12 : 6;  // (2375 x 1041 with five: 651 us with 4, 603 with 8, 590 with 12)
   auto tiles_of = [](const Matrix &M) {
     const long nr = (M.m + T - 1) / T, nc = (M.n + T - 1) / T;
     return KIND <= SQUARE ? nr * (nr + 1) / 2 : nr * nc;
@@ -1845,7 +1845,7 @@ void run(Matrices<N> &a, int steps, float mu, int nesterov, char *rest, int agai
   if (grid) {
     int longest = 0;
     for (int i = 0; i < (N > 1 ? a.count : 1); i++) longest = a.at[i].n > longest ? a.at[i].n : longest;
-    // (16 x 100000: 9 us with 16 threads a row, 4 x 4096: 5 and 11 with 64)
+    // (64 threads a row and 16: 40 x 70001 5 us and 9, four of 4096 x 4096 16 us and 9)
     hipLaunchKernelGGL(scale_kernel<N>, dim3((unsigned)grid), dim3(longest > 16384 ? 1024 : 256), 0, stream(), a, again,
                        room_for(steps));
   }
