@@ -507,8 +507,9 @@ int tt_k_embedding_bwd(const int32_t *ids, const float *dy, float *dw, long rows
  * with a scale for each row and column) and sums of 32: every row and every column
  * is off by about what fp32 products leave of its own size, also where it is much
  * weaker than the others (but for those under 2^-100 of the whole).  Matrices of up
- * to 32 rows or columns have their steps in 64 bits (in a list below, where none goes
- * by such products, or longer than 16384).  Sides at most 2^20, rows * cols 2^32.
+ * to 32 rows or columns have six steps at a time in 64 bits (in a list below, where
+ * none goes by such products, or longer than 16384).  Sides at most 2^20, rows * cols
+ * 2^32.
  * ws: 256-byte aligned; for each of up to 64 matrices (fewer where they pass 4 GiB)
  * 12 bytes a value and 8 a value of a square of the shorter side, sides rounded up to
  * a multiple of 32 (about 14 bytes a value of 1024 x 4096, 20 of a square matrix), and

@@ -1,5 +1,5 @@
 """Newton-Schulz steps and Muon of matrices of up to 32 rows or columns, whose steps are
-taken in 64 bits: values that are off by their own rounding."""
+taken in 64 bits, six at a time: values that are off by their own rounding."""
 import ctypes
 
 import numpy as np
@@ -25,6 +25,17 @@ def _steps64(x, steps):
     for _ in range(steps):
         p = y @ y.T
         y = (ref.A * np.eye(len(y)) + ref.B * p + ref.C * (p @ p)) @ y
+    return y.T if x.shape[0] > x.shape[1] else y
+
+
+def _steps32(x, steps):
+    y = x.astype(np.float64)
+    y = (y.T if x.shape[0] > x.shape[1] else y) / np.linalg.norm(y)
+    y = y.astype(np.float32)
+    a, b, c = (np.float32(t) for t in (ref.A, ref.B, ref.C))
+    for _ in range(steps):
+        p = y @ y.T
+        y = a * y + (b * p + c * (p @ p)) @ y
     return y.T if x.shape[0] > x.shape[1] else y
 
 
@@ -76,14 +87,36 @@ def test_steps_of_few_rows(tlib, rows, cols, kind):
 
 @pytest.mark.parametrize("rows,cols", [(6, 50), (30, 900), (9, 3000), (2500, 20)])
 def test_many_steps_of_few_rows(tlib, rows, cols):
-    """Where values are near 1 the steps enlarge errors, by 4.2 at most and 1.6 at the
-    fixed point 0.87: 2^-53 by 1.6^30 is 2e-10."""
+    """From six steps on X goes on from its fp32 values.  Where these are near 1 the steps
+    enlarge their rounding, by 4.2 at most and 1.6 at the fixed point 0.87 (2^-24 by 1.6^24
+    is 5e-3): fp32 products pass on the same and round more often, and 8 times what they
+    leave is for how it happens to fall."""
     for kind in ("even", "weak"):
         x = _matrix(rows, cols, kind)
         for steps in (12, 30):
-            got, want = _run(tlib, x, steps), _steps64(x, steps)
-            assert np.abs(got - want).max() <= 2.0**-22
+            got, want, single = _run(tlib, x, steps), _steps64(x, steps), _steps32(x, steps)
+            for axis in (0, 1):
+                off, near = (np.linalg.norm(t - want, axis=axis) / np.linalg.norm(want, axis=axis) for t in (got, single))
+                assert off.max() <= max(2.0**-22, 8 * near.max())
     assert np.isfinite(_run(tlib, x, 64)).all()
+
+
+@pytest.mark.parametrize("rows,cols,rank", [(8, 100, 3), (31, 32, 4), (16, 500, 8), (700, 32, 5), (12, 3000, 2),
+                                            (5000, 32, 9)])
+def test_many_steps_of_lower_rank(tlib, rows, cols, rank):
+    """Singular values of 0, of small whole numbers: what the squares' rounding puts in
+    their place, of either sign, grows by A^2 a step.  All stay within 1.21 and what fp32
+    values leave, whose own rounding grows in these directions until it is as large as
+    the rest: the measure is what fp32 products leave, as they fall within 8 times."""
+    rng = np.random.default_rng(rows)
+    x = (rng.integers(-3, 4, (rows, rank)) @ rng.integers(-3, 4, (rank, cols))).astype(np.float32)
+    near = ref.A**4 * ref.PART
+    for steps in (6, 7, 12, 18, 20, 33, 64):
+        got, want = _run(tlib, x, steps).astype(np.float64), _steps64(x, steps)
+        assert np.isfinite(got).all()
+        assert np.linalg.norm(got, 2) <= 1.21
+        off, single = (np.linalg.norm(t - want) for t in (got, _steps32(x, steps)))
+        assert off <= max(near * np.linalg.norm(want), 8 * single), (steps, off, single)
 
 
 @pytest.mark.parametrize("rows,cols", [(5, 40), (40, 31), (3, 2000)])

@@ -154,3 +154,16 @@ def test_flat_matrices_in_groups(tlib, count, rows, cols):
         worst = _worst(g, want)
         assert max(worst) <= NEAR, worst
     assert (got[count - 2] == 0).all()
+
+
+@pytest.mark.parametrize("rows,cols,rank", [(40, 60, 5), (96, 100, 30), (200, 300, 7), (300, 200, 100), (40, 4000, 8)])
+def test_many_steps_of_lower_rank(tlib, rows, cols, rank):
+    """Singular values of 0, of small whole numbers: what rounding puts in their place
+    grows until it is as large as the rest, and no larger."""
+    rng = np.random.default_rng(rows)
+    x = (rng.integers(-3, 4, (rows, rank)) @ rng.integers(-3, 4, (rank, cols))).astype(np.float32)
+    for steps in (6, 7, 18, 33, 64):
+        got, want = _run(tlib, x, steps).astype(np.float64), _steps(x, steps)
+        assert np.linalg.norm(got, 2) <= 1.21
+        off, single = (np.linalg.norm(t - want) for t in (got, _steps(x, steps, np.float32)))
+        assert off <= max(NEAR * np.linalg.norm(want), 8 * single)

@@ -199,10 +199,12 @@ __device__ __forceinline__ V momentum(const float *g, float *v, float mu, int ne
 // All steps together are a product from the left, X <- T X, and T is made of P alone:
 //   P = X X^T;  M = a I + b P + c P P,  T <- M T,  P <- M P M
 // (P, M and T have the same eigenvectors, so they are symmetric and their products in
-// any order).  With up to FEW rows these are small, and X is read twice, whatever the
-// steps: for P and for T X.  P has squares of X's values, so it is formed in 64 bits,
+// any order).  With up to FEW rows these are small, and X is read twice, for P and for
+// T X.  P has squares of X's values, so it is formed in 64 bits,
 // as are the steps; entries of weak rows are as near as any, since P = D C D keeps its
-// form.  (In images a single row would have blocks of 32 x 32, and where sums are as
+// form.  What the rounding leaves in place of an eigenvalue of 0, of either sign, grows
+// by a a = 12 a step, and once negative and large without bounds: after MOST_STEPS (of
+// 2^-36, the most for the longest rows, 2^-18) X begins anew from its fp32 values.  (In images a single row would have blocks of 32 x 32, and where sums are as
 // short as these the parts' 22 bits show: up to 5 times as far off as fp32 products.)
 // A workgroup has a matrix of up to FEW_SHORT columns, bound by latency: five steps of 32 x
 // 32 take 23 us (1.1 us a step of up to 16 rows, 1.8 of more), of 10 x 785 29, of 32 x
@@ -277,9 +279,9 @@ __device__ __forceinline__ void few_gram(const Matrix &M, Few &s, long from, lon
   s.a[0][r][c] = v;
   __syncthreads();
 }
-// From U U^T in a[0]: T of so many steps to a[2]; what X = U times is returned.  Four
-// waves have a quarter each (one where a quarter is all).
-__device__ __forceinline__ double few_steps(const Matrix &M, Few &s, int steps) {
+// From U U^T in a[0]: T of so many steps to a[2]; what X = U times is returned (`again`:
+// 1).  Four waves have a quarter each (one where a quarter is all).
+__device__ __forceinline__ double few_steps(const Matrix &M, Few &s, int steps, int again) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 15, high = lane >> 4;
   const int qi = (wave >> 1 & 1) * 16, qj = (wave & 1) * 16, k4 = M.m > 16 ? 8 : 4;
   const bool on = wave < 4 && qi < M.m && qj < M.m;
@@ -287,7 +289,7 @@ __device__ __forceinline__ double few_steps(const Matrix &M, Few &s, int steps) 
 #pragma unroll 8
   for (int i = 0; i < M.m; i++) norm += s.a[0][i][i];
   // zeros stay zeros; an infinity or a NaN makes all of it NaN
-  const double over = norm == 0.0 ? 0.0 : norm < __builtin_inf() ? 1.0 / norm : __builtin_nan("");
+  const double over = again ? 1.0 : norm == 0.0 ? 0.0 : norm < __builtin_inf() ? 1.0 / norm : __builtin_nan("");
   __syncthreads();
   s.a[0][threadIdx.x >> 5][threadIdx.x & 31] *= over;
   __syncthreads();
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_gram_kernel(Matrices<N> a, fl
   M.few()[(long)b * FEW * FEW + threadIdx.x] = s.a[0][threadIdx.x >> 5][threadIdx.x & 31];
 }
 template <int N>
-__global__ void __launch_bounds__(FEW_THREADS) few_steps_kernel(Matrices<N> a, int steps) {
+__global__ void __launch_bounds__(FEW_THREADS) few_steps_kernel(Matrices<N> a, int steps, int again) {
   __shared__ Few s;
   const Matrix M = matrix(a, blockIdx.x);
   double v = 0.0, *at = M.few() + threadIdx.x;
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_steps_kernel(Matrices<N> a, i
   for (int b = 0; b < M.parts; b++, at += FEW * FEW) v += *at;
   s.a[0][threadIdx.x >> 5][threadIdx.x & 31] = v;
   __syncthreads();
-  const double scale = few_steps(M, s, steps);
+  const double scale = few_steps(M, s, steps, again);
   *at = s.a[2][threadIdx.x >> 5][threadIdx.x & 31];
   if (threadIdx.x == 0) at[FEW * FEW] = scale;
 }
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(BLOCK_WAVES * 64)
   if (M.m <= FEW) {
     Few &few = *(Few *)lds;
     few_gram(M, few, 0, M.n, mu, nesterov);
-    const double times = few_steps(M, few, steps);
+    const double times = few_steps(M, few, steps, again);
     few_apply(M, few, 0, M.n, times, mu, nesterov);
     return;
   }
@@ -1813,8 +1815,7 @@ void product(Matrices<N> &a, const Phase &phase, float *pieces, int to_w = 0) {
   else tile_product<KIND, 256, 2, N>(a, phase, to_w, pieces);
 }
 
-// Steps of matrices that a workgroup has; MOST_STEPS at most (of few rows any number),
-// `again`: of X that is given.
+// Steps of matrices that a workgroup has, MOST_STEPS at most; `again`: of X that is given.
 template <int N>
 void run_in_lds(const Matrices<N> &a, int steps, float mu, int nesterov, int again = 0) {
   if (a.count)
@@ -1822,13 +1823,13 @@ void run_in_lds(const Matrices<N> &a, int steps, float mu, int nesterov, int aga
                        room_for(steps));
 }
 
-// Any number of steps of matrices of few long rows.
+// The same of matrices of few long rows.
 template <int N>
-void run_few(Matrices<N> &a, int steps, float mu, int nesterov) {
+void run_few(Matrices<N> &a, int steps, float mu, int nesterov, int again = 0) {
   if (!a.count) return;
   unsigned long grid = number(a, [](const Matrix &M) { return (long)M.parts; });
   hipLaunchKernelGGL(few_gram_kernel<N>, dim3((unsigned)grid), dim3(FEW_THREADS), 0, stream(), a, mu, nesterov);
-  hipLaunchKernelGGL(few_steps_kernel<N>, dim3(a.count), dim3(FEW_THREADS), 0, stream(), a, steps);
+  hipLaunchKernelGGL(few_steps_kernel<N>, dim3(a.count), dim3(FEW_THREADS), 0, stream(), a, steps, again);
   grid = number(a, [](const Matrix &M) { return (long)((M.n + FEW_COLS - 1) / FEW_COLS); });
   hipLaunchKernelGGL(few_apply_kernel<N>, dim3((unsigned)grid), dim3(FEW_THREADS), 0, stream(), a, mu, nesterov);
 }
@@ -1926,13 +1927,12 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
   Matrices<1> a = alike(count, rows, cols, (char *)ws, way);
   const int most = a.count;
   char *const rest = way == PRODUCTS ? (char *)ws + most * a.images : NULL;
-  // More steps than the scales hold for go on from y.  By products then each begins anew
+  // More steps than the scales or few rows' 64 bits hold for go on from y.  By products then each begins anew
   // and adds to y: what is weak by its row and its column, and so in every image, is
   // carried in fp32 (60 x 500 with 1e-7 of half of both: a column's 3e-6 after 16 steps,
   // 2e-4 from images of six).  In LDS such an X is fp32 throughout.
-  const bool all = a.at[0].m <= FEW || steps <= MOST_STEPS;
-  const int each = all ? steps : way == IN_LDS ? MOST_STEPS : 1;
-  const int keep = way == PRODUCTS && !all;
+  const int keep = way == PRODUCTS && steps > MOST_STEPS;
+  const int each = keep ? 1 : MOST_STEPS;
   a.at[0].onto = keep, a.at[0].keep = TT_NS_A, a.at[0].rate = 1.f;
   for (long base = 0; base < count; base += most) {
     a.count = (int)(count - base < most ? count - base : most);
@@ -1941,7 +1941,7 @@ extern "C" int tt_k_newton_schulz(const float *x, float *y, long count, long row
     for (int done = 0; done < steps; done += each) {
       const int n = steps - done < each ? steps - done : each;
       if (way == IN_LDS) run_in_lds(a, n, 0.f, 0, done > 0);
-      else if (way == FEW_LONG) run_few(a, n, 0.f, 0);
+      else if (way == FEW_LONG) run_few(a, n, 0.f, 0, done > 0);
       else run(a, n, 0.f, 0, rest, done > 0, keep);
       a.at[0].g = a.at[0].w;
     }
