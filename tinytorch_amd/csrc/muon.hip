@@ -200,12 +200,13 @@ __device__ __forceinline__ V momentum(const float *g, float *v, float mu, int ne
 //   P = X X^T;  M = a I + b P + c P P,  T <- M T,  P <- M P M
 // (P, M and T have the same eigenvectors, so they are symmetric and their products in
 // any order).  With up to FEW rows these are small, and X is read twice, for P and for
-// T X.  P has squares of X's values, so it is formed in 64 bits,
-// as are the steps; entries of weak rows are as near as any, since P = D C D keeps its
-// form.  What the rounding leaves in place of an eigenvalue of 0, of either sign, grows
-// by a a = 12 a step, and once negative and large without bounds: after MOST_STEPS (of
-// 2^-36, the most for the longest rows, 2^-18) X begins anew from its fp32 values.  (In images a single row would have blocks of 32 x 32, and where sums are as
-// short as these the parts' 22 bits show: up to 5 times as far off as fp32 products.)
+// T X.  P has squares of X's values, so it is formed in 64 bits, as are the steps; entries
+// of weak rows are as near as any, since P = D C D keeps its form.  What the rounding
+// leaves in place of an eigenvalue of 0, of either sign, grows by a a = 12 a step, and
+// once negative and large without bounds: after MOST_STEPS (of 2^-36, the most for the
+// longest rows, 2^-18) X begins anew from its fp32 values.  (In images a single row
+// would have blocks of 32 x 32, and where sums are as short as these the parts' 22 bits
+// show: up to 5 times as far off as fp32 products.)
 // A workgroup has a matrix of up to FEW_SHORT columns, bound by latency: five steps of 32 x
 // 32 take 23 us (1.1 us a step of up to 16 rows, 1.8 of more), of 10 x 785 29, of 32 x
 // 1024 49.  Longer ones are cut: parts of P, then one workgroup for the steps, then T X:
